@@ -173,7 +173,7 @@ def prepare(case, seed):
     if own:
         from sensenova_u1_b200.ops import paged
         s["cache"] = paged.PagedCache(data, scales)
-        s["plan"] = paged.build_plan(s["cache"], q_lens, kv_lens, table, limits=limits if case["picture"] else None)
+        s["plan"] = paged.build_plan(s["cache"], h, q_lens, kv_lens, table, limits=limits if case["picture"] else None)
         return s
     dev = data.device
     seq = torch.repeat_interleave(torch.arange(len(q_lens)), torch.tensor(q_lens))
