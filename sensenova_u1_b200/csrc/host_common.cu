@@ -64,6 +64,11 @@ static PFN_cuTensorMapEncodeTiled_v12000 get_encode_fn() {
 
 int encode_tmap_bf16(CUtensorMap* out, const void* base, int rank, const uint64_t* dims,
                      const uint64_t* strides, const uint32_t* box) {
+  return encode_tmap(out, TmapType::kBf16, true, base, rank, dims, strides, box);
+}
+
+int encode_tmap(CUtensorMap* out, TmapType type, bool swizzle, const void* base, int rank, const uint64_t* dims,
+                const uint64_t* strides, const uint32_t* box) {
   auto fn = get_encode_fn();
   if (fn == nullptr) {
     set_last_error("cuTensorMapEncodeTiled is not available from this driver");
@@ -90,9 +95,12 @@ int encode_tmap_bf16(CUtensorMap* out, const void* base, int rank, const uint64_
       }
     }
   }
-  CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, static_cast<cuuint32_t>(rank),
-                  const_cast<void*>(base), gdim, gstr, bdim, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+  const CUtensorMapDataType t = type == TmapType::kBf16  ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                : type == TmapType::kF32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                                         : CU_TENSOR_MAP_DATA_TYPE_UINT8;
+  CUresult r = fn(out, t, static_cast<cuuint32_t>(rank), const_cast<void*>(base), gdim, gstr, bdim, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     set_last_error("cuTensorMapEncodeTiled failed with CUresult %d (rank %d dims %llu,%llu box %u,%u)",

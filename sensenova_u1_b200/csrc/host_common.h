@@ -64,4 +64,9 @@ inline cudaError_t launch_pdl(void (*kernel)(P...), dim3 grid, dim3 block, size_
 int encode_tmap_bf16(CUtensorMap* out, const void* base, int rank, const uint64_t* dims,
                      const uint64_t* strides, const uint32_t* box);
 
+// The same for other types, up to rank 5, with 128-byte swizzle or none.
+enum class TmapType { kBf16, kF32, kU8 };
+int encode_tmap(CUtensorMap* out, TmapType type, bool swizzle, const void* base, int rank, const uint64_t* dims,
+                const uint64_t* strides, const uint32_t* box);
+
 }  // namespace snu1

@@ -1,0 +1,77 @@
+// Paged key/value cache: what the kernels that write, read and attend to it share.
+//
+// A cache holds one layer.  Page p keeps ``page`` tokens of all key/value heads, head by head:
+//   data   [pages][2 (key, value)][heads][page][128]   bf16, or e4m3 codes
+//   scales [pages][2][heads][page]                     fp32, e4m3 only: value = code * scale
+// so the rows of one head are contiguous inside a page, which is the unit that an attention CTA asks for (one TMA box for
+// keys and values together).  Sequences own pages through a table in any order; pages of 16 to 128 tokens.
+#pragma once
+#include "attn_common.cuh"
+
+namespace snu1 {
+namespace paged {
+
+constexpr int HEAD = 128;                  // width of a head
+constexpr float E4M3_MAX = 448.f;
+constexpr float TINY = 7.70371977754894342e-34f;   // 2^-110, least row maximum that a scale is made of: 448 / TINY is finite
+
+// One layer's cache, filled by snu1_paged_cache_init.
+struct alignas(64) Cache {
+  CUtensorMap kv;          // box: up to 64 tokens of one head, keys and values (64 values wide; e4m3: all 128)
+  CUtensorMap scale;       // box: the scales of the same
+  CUtensorMap k, v;        // bf16 only: boxes of up to 128 tokens of one head, 64 values wide
+  void* data;
+  float* scales;
+  int pages, heads, page, fp8;
+};
+
+// Device arrays and counts of a plan (ops/paged.py builds it).
+struct Plan {
+  const int* q_start;      // [seqs + 1] first query row of a sequence
+  const int* kv_len;       // [seqs] cached tokens, the new ones among them; may be advanced in place ...
+  const int* cap;          // [seqs] ... up to this
+  const int* table;        // [seqs][width] pages
+  const int* behind;       // [rows] a row reads its sequence's first kv_len - behind keys; null: up to itself
+  const int* row_seq;      // [rows] sequence of a row
+  const int* k_start;      // [seqs + 1] first packed row of a sequence, by the planned lengths
+  const int2* read_pages;  // [read_count] (sequence, page of it) of all planned pages
+  const int2* unpack;      // [unpack_count] (sequence, page) of the e4m3 sequences that the chunk kernel handles, to full tiles of 128
+  const int* unpack_first; // [seqs] first page of such a sequence in the scratch for unpacked rows
+  const int4* few;         // [few_count] work of the kernel for few rows: sequence, first row, part | parts << 16, partial row (-1: none)
+  const int4* chunk;       // [chunk_count] the same for chunks
+  const int4* merge;       // [merge_count] sequence, first row, parts | rows of a part << 16, partial row
+  int seqs, rows, width, page, group;
+  int read_count, few_count, few_rows, chunk_count, merge_count, merge_rows;
+  int partial_rows;        // rows of the scratch for partial results (x heads)
+  int unpack_pages;        // 128-token pages of the scratch for unpacked e4m3 rows
+  int unpack_count;
+};
+
+__device__ __forceinline__ int seq_len(const Plan& p, int b) { return max(0, min(p.kv_len[b], p.cap[b])); }
+
+// Keys that row ``token`` of a sequence may read.
+__device__ __forceinline__ int row_limit(const Plan& p, int q0, int q_len, int kv_len, int token) {
+  const int behind = p.behind != nullptr ? p.behind[q0 + token] : q_len - 1 - token;
+  return max(0, min(kv_len, kv_len - behind));
+}
+
+// Two e4m3 codes in the high bytes of the halves of ``x`` (low bytes zero) as bf16.  The code's exponent and mantissa are put at
+// the bottom of bf16's, which is the value times 2^-120 (also for codes below the smallest normal one: bf16 products keep
+// subnormal inputs), so the product with 2^120 is exact.
+__device__ __forceinline__ uint32_t e4m3x2_to_bf16x2(uint32_t x) {
+  const uint32_t m = (x & 0x80008000u) | ((x >> 4) & 0x07f007f0u);
+  uint32_t r;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(m), "r"(0x7b807b80u));
+  return r;
+}
+
+__device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* m, uint64_t* bar, int x, int y, int z, int w, int u) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(u)
+      : "memory");
+}
+
+}  // namespace paged
+}  // namespace snu1

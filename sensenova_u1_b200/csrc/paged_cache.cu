@@ -1,0 +1,234 @@
+// Paged key/value cache: descriptors, writing (with quantisation) and reading back.
+//
+// Quantising a row x of 128 values (one token, one head, keys or values): a = max(max |x|, 2^-110), scale = a / 448,
+// code = e4m3(x * (448 / a)), all in fp32 with one rounding to e4m3 at the end; e4m3 because a code is a bf16 value
+// exactly, so attention can take codes straight to the tensor cores and apply the scales in fp32.  One scale per row: rows
+// of one head differ in size from token to token, and a row is written once, by itself.  A row that holds a value that is
+// not finite gets NaN as its scale: it reads back as NaN, and attention to it is NaN.
+//
+// Both directions are bound by memory: 16 lanes own a row (16 bytes of bf16, 8 codes each), a warp the key and the value
+// row of one (token, head) when writing, two rows of a page when reading; four of these are in flight per warp.
+#include <cuda_fp8.h>
+#include <string.h>
+
+#include "host_common.h"
+#include "paged.cuh"
+
+namespace snu1 {
+namespace paged {
+
+constexpr int WRITE_THREADS = 256;
+constexpr int WRITE_TOKENS = 4;      // tokens of one head per warp
+
+template <bool FP8>
+__global__ void __launch_bounds__(WRITE_THREADS)
+    paged_write_kernel(const __nv_bfloat16* __restrict__ k, long long ldk, const __nv_bfloat16* __restrict__ v, long long ldv,
+                       uint8_t* __restrict__ data, float* __restrict__ scales, int pages, int heads, int page, Plan p, int* status) {
+  pdl_wait();
+  pdl_trigger();
+  const int lane = threadIdx.x & 31, kv = lane >> 4, c = lane & 15;
+  const long long w = (long long)blockIdx.x * (WRITE_THREADS / 32) + (threadIdx.x >> 5);
+  const int head = (int)(w % heads);
+  const long long row0 = w / heads * WRITE_TOKENS;
+  const __nv_bfloat16* src = kv ? v : k;
+  const long long ld = kv ? ldv : ldk;
+  uint4 x[WRITE_TOKENS];
+  long long at[WRITE_TOKENS];            // row of the cache, -1: none
+#pragma unroll
+  for (int i = 0; i < WRITE_TOKENS; ++i) {
+    const long long row = row0 + i;
+    at[i] = -1;
+    x[i] = make_uint4(0, 0, 0, 0);
+    if (row < p.rows) {
+      x[i] = *reinterpret_cast<const uint4*>(src + row * ld + head * HEAD + c * 8);
+      const int b = p.row_seq[row];
+      const int pos = seq_len(p, b) - (p.q_start[b + 1] - (int)row);
+      if (pos >= 0) {
+        const int pg = p.table[(long long)b * p.width + pos / page];
+        if (pg >= 0 && pg < pages) at[i] = (((long long)pg * 2 + kv) * heads + head) * page + pos % page;
+        else if (lane == 0) report_status(status, kBadPage, 9);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < WRITE_TOKENS; ++i) {
+    if (!FP8) {
+      if (at[i] >= 0) *reinterpret_cast<uint4*>(data + at[i] * (HEAD * 2) + c * 16) = x[i];
+      continue;
+    }
+    const uint32_t u[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+    // as whole numbers: a NaN is larger than infinity, which is larger than every finite value
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) top = max(top, max(u[j] << 16 & 0x7fffffffu, u[j] & 0x7fff0000u));
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const bool finite = top < 0x7f800000u;
+    const float a = fmaxf(__uint_as_float(top), TINY), inv = __fdiv_rn(E4M3_MAX, a);
+    uint2 code;
+    uint32_t q[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      q[j] = __nv_cvt_float2_to_fp8x2(make_float2(__uint_as_float(u[j] << 16) * inv, __uint_as_float(u[j] & 0xffff0000u) * inv),
+                                      __NV_SATFINITE, __NV_E4M3);
+    code.x = q[0] | q[1] << 16;
+    code.y = q[2] | q[3] << 16;
+    if (at[i] >= 0) {
+      *reinterpret_cast<uint2*>(data + at[i] * HEAD + c * 8) = code;
+      if (c == 0) scales[at[i]] = finite ? __fdiv_rn(a, E4M3_MAX) : __int_as_float(0x7fffffff);
+    }
+  }
+}
+
+constexpr int READ_THREADS = 256;
+constexpr int READ_ROWS = 4;                                         // rows of a lane
+constexpr int READ_BLOCK = READ_THREADS / 16 * READ_ROWS;            // rows of a block
+
+// Rows of the planned pages, in order.  PACKED: out = keys, out2 = values [rows][heads][128] at the plan's row numbers;
+// otherwise out = pages of 128 tokens in a cache's own layout, every sequence from a page of its own on, rows behind its
+// last token cleared (the attention kernel multiplies them by probabilities of zero).
+template <bool FP8, bool PACKED>
+__global__ void __launch_bounds__(READ_THREADS)
+    paged_read_kernel(const uint8_t* __restrict__ data, const float* __restrict__ scales, int pages, int heads, int page, Plan p,
+                      __nv_bfloat16* __restrict__ out, __nv_bfloat16* __restrict__ out2, int* status) {
+  pdl_wait();
+  pdl_trigger();
+  const int2 e = (PACKED ? p.read_pages : p.unpack)[blockIdx.x];
+  const int b = e.x, pos0 = e.y * page, c = threadIdx.x & 15;
+  const int k0 = p.k_start[b];
+  const int len = PACKED ? p.k_start[b + 1] - k0 : seq_len(p, b);
+  const int pg = pos0 < len ? p.table[(long long)b * p.width + e.y] : 0;
+  const bool there = pos0 < len && pg >= 0 && pg < pages;
+  if (pos0 < len && !there && threadIdx.x == 0) report_status(status, kBadPage, 9);
+  uint4 x[READ_ROWS];
+  float s[READ_ROWS];
+  const int first = blockIdx.y * READ_BLOCK + (threadIdx.x >> 4), total = 2 * heads * page;
+#pragma unroll
+  for (int i = 0; i < READ_ROWS; ++i) {
+    const int r = first + i * (READ_THREADS / 16);                   // row of the page: (kv, head, token)
+    x[i] = make_uint4(0, 0, 0, 0);
+    s[i] = 0.f;
+    if (there && r < total && pos0 + r % page < len) {
+      const long long at = (long long)pg * total + r;
+      if (FP8) {
+        const uint2 u = *reinterpret_cast<const uint2*>(data + at * HEAD + c * 8);
+        x[i].x = u.x;
+        x[i].y = u.y;
+        s[i] = scales[at];
+      } else {
+        x[i] = *reinterpret_cast<const uint4*>(data + at * (HEAD * 2) + c * 16);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < READ_ROWS; ++i) {
+    const int r = first + i * (READ_THREADS / 16);
+    const int pos = pos0 + r % page, head = r / page % heads, kv = r / page / heads;
+    if (r >= total || (PACKED && pos >= len)) continue;
+    uint4 y = x[i];
+    if (FP8) {
+      const uint32_t u[2] = {x[i].x, x[i].y};
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const __half2 h(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(u[j >> 1] >> (16 * (j & 1))), __NV_E4M3));
+        const float2 f = __half22float2(h);
+        w[j] = pack_bf16x2(f.x * s[i], f.y * s[i]);
+      }
+      y = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    __nv_bfloat16* dst;
+    if (PACKED) {
+      dst = (kv ? out2 : out) + ((long long)(k0 + pos) * heads + head) * HEAD;
+    } else {
+      const long long t = (long long)(p.unpack_first[b]) * 128 + pos;
+      dst = out + ((((t >> 7) * 2 + kv) * heads + head) * 128 + (t & 127)) * HEAD;
+    }
+    *reinterpret_cast<uint4*>(dst + c * 8) = y;
+  }
+}
+
+}  // namespace paged
+}  // namespace snu1
+
+using namespace snu1;
+
+SNU1_API int snu1_paged_cache_bytes() { return (int)sizeof(paged::Cache); }
+SNU1_API int snu1_paged_plan_bytes() { return (int)sizeof(paged::Plan); }
+
+// Fills ``out`` (snu1_paged_cache_bytes) for the cache at data / scales.
+SNU1_API int snu1_paged_cache_init(void* out, void* data, void* scales, int pages, int heads, int page, int fp8) {
+  if (pages <= 0 || heads <= 0 || (page != 16 && page != 32 && page != 64 && page != 128) || (fp8 != 0) != (scales != nullptr) ||
+      ((reinterpret_cast<uintptr_t>(data) | reinterpret_cast<uintptr_t>(scales)) & 15) != 0) {
+    set_last_error("paged_cache: pages of 16, 32, 64 or 128 tokens in 16-byte aligned memory, scales for e4m3 only");
+    return kHostBadArg;
+  }
+  paged::Cache c;
+  memset(&c, 0, sizeof(c));
+  c.data = data;
+  c.scales = (float*)scales;
+  c.pages = pages;
+  c.heads = heads;
+  c.page = page;
+  c.fp8 = fp8;
+  const uint64_t row = fp8 ? 128 : 256, P = page, H = heads;
+  const uint32_t bx = page < 64 ? page : 64;
+  int rc;
+  {
+    const uint64_t dims[5] = {128, P, H, 2, (uint64_t)pages}, str[4] = {row, row * P, row * P * H, row * P * H * 2};
+    const uint32_t box[5] = {fp8 ? 128u : 64u, bx, 1, 2, 1};
+    if ((rc = encode_tmap(&c.kv, fp8 ? TmapType::kU8 : TmapType::kBf16, true, data, 5, dims, str, box)) != kHostOk) return rc;
+  }
+  if (fp8) {
+    const uint64_t dims[4] = {P, H, 2, (uint64_t)pages}, str[3] = {P * 4, P * H * 4, P * H * 8};
+    const uint32_t box[4] = {bx, 1, 2, 1};
+    if ((rc = encode_tmap(&c.scale, TmapType::kF32, false, scales, 4, dims, str, box)) != kHostOk) return rc;
+  } else {
+    const uint64_t dims[4] = {128, P, H, (uint64_t)pages}, str[3] = {row, row * P, row * P * H * 2};
+    const uint32_t box[4] = {64, (uint32_t)page, 1, 1};
+    if ((rc = encode_tmap(&c.k, TmapType::kBf16, true, data, 4, dims, str, box)) != kHostOk) return rc;
+    if ((rc = encode_tmap(&c.v, TmapType::kBf16, true, (uint8_t*)data + row * P * H, 4, dims, str, box)) != kHostOk) return rc;
+  }
+  memcpy(out, &c, sizeof(c));
+  return kHostOk;
+}
+
+// Keys and values of a plan's new rows ([rows][heads][128] bf16, rows ldk / ldv apart) into their sequences' pages.
+SNU1_API int snu1_paged_write(const void* cache, const void* plan, const void* k, long long ldk, const void* v, long long ldv,
+                              void* stream) {
+  paged::Cache c;
+  paged::Plan p;
+  memcpy(&c, cache, sizeof(c));
+  memcpy(&p, plan, sizeof(p));
+  if (p.rows <= 0) return kHostOk;
+  if (p.page != c.page || ldk % 8 || ldv % 8 || ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) != 0) {
+    set_last_error("paged_write: rows must be 16-byte aligned, and the plan made for this page size");
+    return kHostBadArg;
+  }
+  const long long warps = (long long)(p.rows + paged::WRITE_TOKENS - 1) / paged::WRITE_TOKENS * c.heads;
+  const long long blocks = (warps + paged::WRITE_THREADS / 32 - 1) / (paged::WRITE_THREADS / 32);
+  auto kernel = c.fp8 ? paged::paged_write_kernel<true> : paged::paged_write_kernel<false>;
+  SNU1_CUDA_CHECK(launch_pdl(kernel, dim3((unsigned)blocks), dim3(paged::WRITE_THREADS), 0, (cudaStream_t)stream,
+                             (const __nv_bfloat16*)k, ldk, (const __nv_bfloat16*)v, ldv, (uint8_t*)c.data, c.scales, c.pages, c.heads,
+                             c.page, p, device_status_word()));
+  return kHostOk;
+}
+
+// Cached rows of a plan's sequences, packed: k, v [planned keys][heads][128] bf16.
+SNU1_API int snu1_paged_read(const void* cache, const void* plan, void* k, void* v, void* stream) {
+  paged::Cache c;
+  paged::Plan p;
+  memcpy(&c, cache, sizeof(c));
+  memcpy(&p, plan, sizeof(p));
+  if (p.read_count <= 0) return kHostOk;
+  if (p.page != c.page || ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) != 0) {
+    set_last_error("paged_read: outputs must be 16-byte aligned, and the plan made for this page size");
+    return kHostBadArg;
+  }
+  const int total = 2 * c.heads * c.page;
+  auto kernel = c.fp8 ? paged::paged_read_kernel<true, true> : paged::paged_read_kernel<false, true>;
+  SNU1_CUDA_CHECK(launch_pdl(kernel, dim3(p.read_count, (total + paged::READ_BLOCK - 1) / paged::READ_BLOCK),
+                             dim3(paged::READ_THREADS), 0, (cudaStream_t)stream, (const uint8_t*)c.data, c.scales, c.pages, c.heads,
+                             c.page, p, (__nv_bfloat16*)k, (__nv_bfloat16*)v, device_status_word()));
+  return kHostOk;
+}

@@ -23,6 +23,7 @@ enum StatusCode : int {
   kWaitTimeout = 1,     // an mbarrier / flag wait ran out of time
   kBadShape = 2,        // a shape the kernel cannot handle reached the device
   kPeerTimeout = 3,     // a wait on a flag written by another GPU ran out
+  kBadPage = 4,         // a page table names a page that its cache does not have
 };
 
 __device__ __forceinline__ void report_status(int* status, int code, int where) {

@@ -79,7 +79,7 @@ def call(name: str, *args) -> None:
 
 
 _ROLE = {1: "TMA producer", 2: "MMA issuer (accumulator)", 3: "MMA issuer (operands)",
-         4: "epilogue", 5: "softmax", 6: "correction", 7: "peer flag", 8: "expert-parallel plan"}
+         4: "epilogue", 5: "softmax", 6: "correction", 7: "peer flag", 8: "expert-parallel plan", 9: "paged cache", 10: "paged attention"}
 
 
 def check_status() -> None:
@@ -94,5 +94,6 @@ def check_status() -> None:
         code, where = v & 0xff, v >> 8
         what = {1: "a wait on an mbarrier ran out of time",
                 2: "a size limit was exceeded on the device (e.g. expert receive buffer too small)",
-                3: "a wait on a peer flag ran out of time"}.get(code, f"code {code}")
+                3: "a wait on a peer flag ran out of time",
+                4: "a page table names a page that the cache does not have"}.get(code, f"code {code}")
         raise NativeLibraryError(f"kernel status: {what} (role: {_ROLE.get(where, where)})")

@@ -1,0 +1,297 @@
+"""Paged key/value cache and attention over it (csrc/paged_cache.cu, csrc/attn_paged.cu, csrc/attn_paged_sm100.cu).
+
+A :class:`PagedCache` holds the keys and values of one layer in pages of 16, 32, 64 or 128 tokens, as bf16 or as e4m3 codes with
+one fp32 scale per token and head (half the memory: 132 bytes of 256).  A sequence owns pages in any order; several sequences may
+read the same page (a shared prompt), only one may write it.
+
+One :class:`PagedPlan` describes a step: how many new tokens every sequence brings, how many tokens it has then, and its
+pages.  The plan is made once per step on the host and serves every layer::
+
+    plan = build_plan(caches[0], heads, q_lens, kv_lens, tables)
+    for layer, cache in zip(layers, caches):
+        q, k, v = layer.project(x)                     # [rows, heads, 128], rows of all sequences one after another
+        paged_write(cache, k, v, plan)
+        o = paged_attention(q, cache, plan, scale)
+
+A sequence may bring one token (a decode step), a few (drafted tokens) or thousands (a chunk of its prompt), all in one plan.
+For a captured decode loop, ``build_plan(..., grow=n)`` leaves room for ``n`` further tokens and :meth:`PagedPlan.advance` inside
+the graph moves every sequence on by one.
+
+A call runs on the current stream of the tensors' device.  A plan's device arrays belong to the streams that are ordered after
+the one it was built on; calls that only read (write into different caches, attention, reading back) may share it.
+"""
+from __future__ import annotations
+
+import ctypes
+from dataclasses import dataclass, field
+
+import numpy as np
+import torch
+
+from . import _lib
+from ._lib import c_float, c_int, c_ll, c_void_p
+
+PAGE_SIZES = (16, 32, 64, 128)
+HEAD_DIM = 128
+E4M3 = torch.float8_e4m3fn
+KEY_TILE = 64            # keys of a stage of the kernel for few rows
+FEW_SLOTS = 296          # its CTAs that run at once: two on each of 148 SMs
+FEW_LEAST = 4            # a part of a sequence has at least this many key tiles
+FEW_TILE = 64            # rows (new tokens x query heads of a group) of one CTA, at most
+
+
+class PagedCache:
+    """Keys and values of one layer: ``data`` [pages, 2, kv_heads, page, 128] (bf16 or float8_e4m3fn; index 0 of the second
+    dimension are the keys), ``scales`` [pages, 2, kv_heads, page] fp32 for e4m3 (value = code * scale), else None."""
+
+    def __init__(self, data: torch.Tensor, scales: torch.Tensor | None = None):
+        if data.dim() != 5 or data.shape[1] != 2 or data.shape[4] != HEAD_DIM or data.shape[0] < 1 or data.shape[2] < 1:
+            raise ValueError("a paged cache is [pages, 2, kv_heads, page, 128]")
+        if data.dtype not in (torch.bfloat16, E4M3):
+            raise ValueError("a paged cache holds bfloat16 or float8_e4m3fn")
+        if data.shape[3] not in PAGE_SIZES:
+            raise ValueError(f"a page holds 16, 32, 64 or 128 tokens, not {data.shape[3]}")
+        if (data.dtype == E4M3) != (scales is not None):
+            raise ValueError("e4m3 codes, and only they, have scales")
+        if not data.is_contiguous() or (scales is not None and not (
+                scales.dtype == torch.float32 and scales.shape == data.shape[:4] and scales.is_contiguous()
+                and scales.device == data.device)):
+            raise ValueError("data and scales [pages, 2, kv_heads, page] (fp32) must be contiguous, on one device")
+        if not data.is_cuda:
+            raise ValueError("a paged cache is in GPU memory")
+        self._data, self._scales = data, scales
+        self.pages, _, self.kv_heads, self.page, _ = data.shape
+        if self.kv_heads > 65535 or self.pages >= 1 << 31:
+            raise ValueError("too many heads or pages")
+        self._desc = ctypes.create_string_buffer(_lib.load().snu1_paged_cache_bytes())
+        with torch.cuda.device(data.device):
+            _lib.call("paged_cache_init", self._desc, c_void_p(data.data_ptr()), c_void_p(None if scales is None else scales.data_ptr()),
+                      c_int(self.pages), c_int(self.kv_heads), c_int(self.page), c_int(0 if scales is None else 1))
+
+    @classmethod
+    def empty(cls, pages: int, page: int, kv_heads: int, dtype=torch.bfloat16, device="cuda") -> "PagedCache":
+        data = torch.empty(pages, 2, kv_heads, page, HEAD_DIM, dtype=dtype, device=device)
+        return cls(data, torch.empty(data.shape[:4], dtype=torch.float32, device=device) if dtype == E4M3 else None)
+
+    @property
+    def data(self) -> torch.Tensor:
+        return self._data
+
+    @property
+    def scales(self) -> torch.Tensor | None:
+        return self._scales
+
+    @property
+    def device(self) -> torch.device:
+        return self._data.device
+
+
+class _Args(ctypes.Structure):
+    """``Plan`` of csrc/paged.cuh."""
+    _fields_ = ([(n, c_void_p) for n in ("q_start", "kv_len", "cap", "table", "behind", "row_seq", "k_start", "read_pages", "unpack",
+                                         "unpack_first", "few", "chunk", "merge")]
+                + [(n, c_int) for n in ("seqs", "rows", "width", "page", "group", "read_count", "few_count", "few_rows", "chunk_count",
+                                        "merge_count", "merge_rows", "partial_rows", "unpack_pages", "unpack_count")])
+
+
+@dataclass
+class PagedPlan:
+    """One step of a batch; see the module's text.  ``kv_len`` is the device's copy of the lengths."""
+    heads: int
+    kv_heads: int
+    page: int
+    pages: int
+    device: torch.device
+    q_lens: list
+    kv_lens: list
+    rows: int
+    keys: int                     # rows that paged_read gives
+    scratch: int                  # bytes that attention needs beside its output
+    kv_len: torch.Tensor
+    grow: int
+    _store: torch.Tensor = field(repr=False)
+    _args: _Args = field(repr=False)
+
+    def advance(self, tokens: int = 1) -> None:
+        """Every sequence has ``tokens`` more (up to ``grow`` in all): its new rows are the ``q_len`` last ones of the longer
+        sequence.  Runs on the device and may be captured; :func:`paged_read` keeps the lengths that the plan was made with."""
+        self.kv_len.add_(tokens)
+
+
+def _shares(tiles: np.ndarray, heads: int, slots: int, least: int) -> np.ndarray:
+    """Into how many parts the key tiles of every work item are split.  ``heads`` CTAs run per part and ``slots`` at once: parts
+    are as short as they may be (``least`` tiles) while all of them run in one wave; where even whole items are more than
+    that, only items longer than a fair share are split."""
+    tiles = np.maximum(tiles, 1)
+    share = max(least, 1)
+    if len(tiles) * heads <= slots:
+        hi = int(tiles.max())
+        lo = share
+        while lo < hi:                                        # least share whose parts fit
+            mid = (lo + hi) // 2
+            if int((-(-tiles // mid)).sum()) * heads <= slots:
+                hi = mid
+            else:
+                lo = mid + 1
+        share = max(share, lo)
+    else:
+        share = max(share, -(-int(tiles.sum()) * heads // slots))
+    return -(-tiles // share)
+
+
+def _lay_out(q_lens, kv_lens, tables, page: int, pages: int, group: int, kv_heads: int, limits, grow: int):
+    """Host side of :func:`build_plan`: checks, and every array of the plan as int32."""
+    q, kv = np.asarray(q_lens, dtype=np.int64).reshape(-1), np.asarray(kv_lens, dtype=np.int64).reshape(-1)
+    n = len(q)
+    if len(kv) != n or (q < 0).any() or (kv < q).any() or grow < 0:
+        raise ValueError("every sequence has q_len >= 0 new tokens among its kv_len >= q_len tokens, and grow >= 0")
+    if n > 65535 or (n and (kv.max() + grow >= 1 << 30 or q.sum() * group >= 1 << 31 or kv.sum() >= 1 << 31)):
+        raise ValueError("too many sequences or tokens for one plan")
+    cap = np.where(q > 0, kv + grow, kv)
+    need = -(-cap // page)
+    width = max(1, int(need.max()) if n else 1)
+    table = np.zeros((n, width), dtype=np.int32)
+    if isinstance(tables, torch.Tensor):
+        if tables.is_cuda or tables.dim() != 2:
+            raise ValueError("page tables are lists of page numbers, or one host tensor [sequences, pages]")
+        tables = tables.numpy()
+    if len(tables) != n:
+        raise ValueError("one page table per sequence")
+    for i in range(n):
+        if len(tables[i]) < need[i]:
+            raise ValueError(f"sequence {i} needs {need[i]} pages for {cap[i]} tokens, its table has {len(tables[i])}")
+        table[i, :need[i]] = tables[i][:need[i]]
+        if need[i] and (table[i, :need[i]].min() < 0 or table[i, :need[i]].max() >= pages):
+            raise ValueError(f"sequence {i} names a page that the cache does not have")
+    rows = int(q.sum())
+    row_seq = np.repeat(np.arange(n, dtype=np.int32), q)
+    behind = None
+    if limits is not None:
+        lim = np.asarray(limits, dtype=np.int64).reshape(-1)
+        if grow:
+            raise ValueError("limits are fixed: a plan with limits cannot grow")
+        if len(lim) != rows or (lim < 0).any() or (lim > kv[row_seq]).any():
+            raise ValueError("one limit per row, between 0 and the keys of its sequence")
+        behind = (kv[row_seq] - lim).astype(np.int32)
+    start = lambda x: np.concatenate([[0], np.cumsum(x)]).astype(np.int32)
+    read = -(-kv // page)
+    pages_of = lambda c: np.stack([np.repeat(np.arange(n), c), np.arange(int(c.sum())) - np.repeat(np.cumsum(c) - c, c)], 1).astype(np.int32)
+    # attention: tiles of rows, split over keys
+    q_rows = q * group
+    top = int(q_rows.max()) if n else 0
+    few_rows = 16 if top <= 16 else 32 if top <= 32 else FEW_TILE
+    count = -(-q_rows // few_rows)
+    seq = np.repeat(np.arange(n), count)
+    row0 = (np.arange(len(seq)) - np.repeat(np.cumsum(count) - count, count)) * few_rows
+    few, merge, partial = _items(seq, row0, -(-cap[seq] // KEY_TILE), few_rows, kv_heads, FEW_SLOTS, FEW_LEAST, 0)
+    arrays = dict(q_start=start(q), kv_len=kv.astype(np.int32), cap=cap.astype(np.int32), table=table, behind=behind, row_seq=row_seq,
+                  k_start=start(kv), read_pages=pages_of(read), unpack=None, unpack_first=None, few=few, chunk=None, merge=merge)
+    counts = dict(seqs=n, rows=rows, width=width, page=page, group=group, read_count=int(read.sum()), few_count=len(few),
+                  few_rows=few_rows, chunk_count=0, merge_count=len(merge), merge_rows=few_rows, partial_rows=partial, unpack_pages=0,
+                  unpack_count=0)
+    return arrays, counts
+
+
+def _items(seq, row0, tiles, m: int, heads: int, slots: int, least: int, first: int):
+    """Work items [sequence, first row, part | parts << 16, partial row or -1], those with most keys first, the joins of the
+    items that were split, and the rows of partial results up to there."""
+    if not len(seq):
+        return np.zeros((0, 4), np.int32), np.zeros((0, 4), np.int32), first
+    parts = _shares(tiles, heads, slots, least)
+    split = parts > 1
+    at = first + np.cumsum(np.where(split, parts * m, 0)) - np.where(split, parts * m, 0)
+    merge = np.stack([seq, row0, parts | m << 16, at], 1)[split]
+    i = np.repeat(np.arange(len(seq)), parts)
+    part = np.arange(len(i)) - np.repeat(np.cumsum(parts) - parts, parts)
+    items = np.stack([seq[i], row0[i], part | parts[i] << 16, np.where(split[i], at[i] + part * m, -1)], 1)
+    order = np.argsort(-(tiles[i] / parts[i]), kind="stable")
+    return items[order].astype(np.int32), merge.astype(np.int32), int(first + np.where(split, parts * m, 0).sum())
+
+
+def build_plan(cache: PagedCache, heads: int, q_lens, kv_lens, tables, limits=None, grow: int = 0) -> PagedPlan:
+    """Plan of one step, for ``cache`` and every other cache of its geometry on the same device.
+
+    ``heads``: query heads, a multiple of the cache's.  ``q_lens`` / ``kv_lens``: new tokens of every sequence, and all its
+    tokens, the new ones (which are its last) among them.  ``tables``: the pages of every sequence in order, as lists or as one
+    host tensor [sequences, at least the pages needed].  ``limits``: for every new row, how many of its sequence's first keys it
+    may read (0: none, its output is zeros); without it, every row reads up to itself.  A token of a picture, which
+    sees the whole picture, has the picture's end as its limit.  ``grow``: tokens that :meth:`PagedPlan.advance` may add."""
+    if heads < 1 or heads % cache.kv_heads != 0:
+        raise ValueError("the number of query heads must be a multiple of the cache's heads")
+    arrays, counts = _lay_out(q_lens, kv_lens, tables, cache.page, cache.pages, heads // cache.kv_heads, cache.kv_heads, limits, grow)
+    # all arrays in one copy from pinned memory that nothing waits for
+    at, total = {}, 0
+    for name, a in arrays.items():
+        if a is not None:
+            at[name] = total
+            total += -(-a.size // 4) * 4
+    host = torch.empty(max(total, 4), dtype=torch.int32, pin_memory=True)
+    flat = host.numpy()
+    for name, o in at.items():
+        flat[o:o + arrays[name].size] = arrays[name].reshape(-1)
+    store = host.to(cache.device, non_blocking=True)
+    args = _Args(**{name: store.data_ptr() + 4 * o for name, o in at.items()}, **counts)
+    n = counts["seqs"]
+    scratch = counts["partial_rows"] * cache.kv_heads * (HEAD_DIM + 2) * 4
+    return PagedPlan(heads, cache.kv_heads, cache.page, cache.pages, cache.device, [int(x) for x in q_lens], [int(x) for x in kv_lens],
+                     counts["rows"], int(arrays["k_start"][-1]), scratch, store[at["kv_len"]:at["kv_len"] + n], grow, store, args)
+
+
+def _check(cache: PagedCache, plan: PagedPlan) -> None:
+    if cache.page != plan.page or cache.kv_heads != plan.kv_heads or cache.pages < plan.pages or cache.device != plan.device:
+        raise ValueError("the plan was made for caches of another geometry or device")
+
+
+def _rows_ok(t, rows, heads, device) -> bool:
+    return (t.dtype is torch.bfloat16 and t.dim() == 3 and t.shape[0] >= rows and t.shape[1] == heads and t.shape[2] == HEAD_DIM
+            and t.stride(2) == 1 and t.stride(1) == HEAD_DIM and t.device == device)
+
+
+def _call(device, name, *args) -> None:
+    """On the tensors' device, whichever is current."""
+    if device.index == torch._C._cuda_getDevice():
+        _lib.call(name, *args, c_void_p(_lib.stream()))
+    else:
+        with torch.cuda.device(device):
+            _lib.call(name, *args, c_void_p(_lib.stream()))
+
+
+def paged_write(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, plan: PagedPlan) -> None:
+    """Keys and values of the plan's new rows into their sequences' pages, quantised where the cache holds e4m3.  ``k`` / ``v``:
+    [at least plan.rows, kv_heads, 128] bf16, rows may be slices of wider ones; rows behind the last sequence are ignored.  A
+    row is scaled so that its largest value is 448, the largest e4m3 value; one that holds a value that is not finite
+    reads back as NaN."""
+    _check(cache, plan)
+    if not (_rows_ok(k, plan.rows, cache.kv_heads, plan.device) and _rows_ok(v, plan.rows, cache.kv_heads, plan.device)):
+        raise ValueError(f"k and v must be bf16 [{plan.rows} or more, {cache.kv_heads}, 128] with contiguous heads on the plan's device")
+    if plan.rows:
+        _call(plan.device, "paged_write", cache._desc, ctypes.byref(plan._args), c_void_p(k.data_ptr()), c_ll(k.stride(0)),
+              c_void_p(v.data_ptr()), c_ll(v.stride(0)))
+
+
+def paged_read(cache: PagedCache, plan: PagedPlan) -> tuple[torch.Tensor, torch.Tensor]:
+    """The cached keys and values of the plan's sequences, one sequence after another: two tensors [plan.keys, kv_heads, 128] bf16
+    (e4m3: code times scale, rounded once)."""
+    _check(cache, plan)
+    k, v = (torch.empty(plan.keys, cache.kv_heads, HEAD_DIM, dtype=torch.bfloat16, device=plan.device) for _ in range(2))
+    if plan.keys:
+        _call(plan.device, "paged_read", cache._desc, ctypes.byref(plan._args), c_void_p(k.data_ptr()), c_void_p(v.data_ptr()))
+    return k, v
+
+
+def paged_attention(q: torch.Tensor, cache: PagedCache, plan: PagedPlan, scale: float, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of the plan's new rows over their sequences' cached keys, softmax in fp32.  ``q``: [at least plan.rows, heads,
+    128] bf16, rows may be slices of wider ones; returns ``out`` (default: new, [plan.rows, heads, 128]), whose rows behind
+    the last sequence are left as they are."""
+    _check(cache, plan)
+    if not _rows_ok(q, plan.rows, plan.heads, plan.device):
+        raise ValueError(f"q must be bf16 [{plan.rows} or more, {plan.heads}, 128] with contiguous heads on the plan's device")
+    if out is None:
+        out = torch.empty(plan.rows, plan.heads, HEAD_DIM, dtype=torch.bfloat16, device=plan.device)
+    elif not _rows_ok(out, plan.rows, plan.heads, plan.device):
+        raise ValueError(f"out must be bf16 [{plan.rows} or more, {plan.heads}, 128] with contiguous heads on the plan's device")
+    if plan.rows:
+        scratch = torch.empty(plan.scratch, dtype=torch.uint8, device=plan.device) if plan.scratch else None
+        _call(plan.device, "paged_attention", cache._desc, ctypes.byref(plan._args), c_void_p(q.data_ptr()), c_ll(q.stride(0)),
+              c_void_p(out.data_ptr()), c_ll(out.stride(0)), c_float(scale), c_void_p(None if scratch is None else scratch.data_ptr()))
+    return out

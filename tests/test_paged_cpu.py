@@ -1,0 +1,115 @@
+"""Host side of the paged cache (ops/paged.py): refusals, page tables, and how the work is split."""
+import numpy as np
+import pytest
+import torch
+
+from sensenova_u1_b200.ops import paged
+
+
+def lay(q=(1, 3), kv=(5, 40), tables=((0,), (1, 2, 3)), page=16, pages=4, group=4, heads=2, limits=None, grow=0):
+    return paged._lay_out(list(q), list(kv), [list(t) for t in tables], page, pages, group, heads, limits, grow)
+
+
+def test_arrays():
+    a, c = lay()
+    assert a["q_start"].tolist() == [0, 1, 4] and a["k_start"].tolist() == [0, 5, 45] and a["row_seq"].tolist() == [0, 1, 1, 1]
+    assert a["table"].tolist() == [[0, 0, 0], [1, 2, 3]] and a["behind"] is None
+    assert a["read_pages"].tolist() == [[0, 0], [1, 0], [1, 1], [1, 2]]
+    assert c["rows"] == 4 and c["read_count"] == 4 and c["width"] == 3
+
+
+def test_limits_are_kept_from_the_end():
+    a, _ = lay(limits=[5, 0, 40, 39])
+    assert a["behind"].tolist() == [0, 40, 0, 1]
+
+
+@pytest.mark.parametrize("change", [
+    dict(q=(1, 41)),                                     # more new tokens than tokens
+    dict(q=(-1, 3)),
+    dict(kv=(5,)),
+    dict(grow=-1),
+    dict(tables=((0,),)),                                # a table missing
+    dict(tables=((0,), (1, 2))),                         # a page missing
+    dict(grow=9, tables=((0,), (1, 2, 3))),              # no page for what may be added
+    dict(tables=((0,), (1, 2, 4))),                      # a page that does not exist
+    dict(tables=((0,), (1, -1, 3))),
+    dict(limits=[5, 0, 40]),                             # a limit missing
+    dict(limits=[5, 0, 40, 41]),                         # beyond the sequence
+    dict(limits=[5, -1, 40, 39]),
+    dict(limits=[5, 0, 40, 39], grow=1, tables=((0,), (1, 2, 3))),
+    dict(kv=(1 << 30, 40)),
+])
+def test_refusals(change):
+    with pytest.raises(ValueError):
+        lay(**change)
+
+
+def test_page_tables_as_a_tensor():
+    a, _ = lay(tables=torch.tensor([[0, 77, 99], [1, 2, 3]]))          # what a table holds beyond its pages is ignored
+    assert a["table"].tolist() == [[0, 0, 0], [1, 2, 3]]
+    with pytest.raises(ValueError):
+        paged._lay_out([1], [1], torch.zeros(1, dtype=torch.int32), 16, 4, 1, 1, None, 0)
+
+
+def test_sequences_without_rows_or_keys():
+    a, c = lay(q=(0, 0, 0), kv=(0, 7, 0), tables=((), (2,), ()))
+    assert c["rows"] == 0 and c["few_count"] == 0 and c["merge_count"] == 0 and c["read_count"] == 1
+    a, c = paged._lay_out([], [], [], 16, 4, 1, 1, None, 0)
+    assert c["seqs"] == 0 and c["rows"] == 0
+
+
+@pytest.mark.parametrize("group,heads", [(1, 1), (4, 8), (3, 5), (8, 4), (100, 1)])
+@pytest.mark.parametrize("q,kv", [([1], [840]), ([1] * 24, [62 + 60 * i for i in range(24)]), ([1] * 700, [17] * 700),
+                                  ([5, 0, 17, 1], [12000, 3, 17, 1]), ([300], [30000]), ([1] * 3, [0 + 1, 64, 65])])
+def test_every_row_meets_every_key_once(q, kv, group, heads):
+    page, n = 16, len(q)
+    need = [-(-k // page) for k in kv]
+    tables = [list(range(sum(need[:i]), sum(need[:i + 1]))) for i in range(n)]
+    a, c = paged._lay_out(q, kv, tables, page, sum(need), group, heads, None, 0)
+    parts, written = {}, set()
+    for name, m in (("few", c["few_rows"]),):
+        for b, row0, z, at in a[name].tolist():
+            part, count = z & 0xffff, z >> 16
+            parts.setdefault((b, row0, m, count), []).append(part)
+            assert (at < 0) == (count == 1)
+            if at >= 0:                                               # nobody else's scratch
+                rows = set(range(at, at + m))
+                assert not rows & written and at + m <= c["partial_rows"]
+                written |= rows
+    seen = {}
+    for (b, row0, m, count), got in parts.items():
+        assert sorted(got) == list(range(count))
+        for r in range(row0, min(row0 + m, q[b] * group)):
+            assert (b, r) not in seen
+            seen[(b, r)] = count
+    assert len(seen) == sum(q) * group
+    joined = {(b, row0): (z & 0xffff, z >> 16, at) for b, row0, z, at in a["merge"].tolist()}
+    assert set(joined) == {(b, r0) for (b, r0, m, count) in parts if count > 1}
+    for b, row0, z, at in a["few"].tolist():
+        if at >= 0:
+            count, m, first = joined[(b, row0)]
+            assert count == z >> 16 and at == first + (z & 0xffff) * m
+
+
+def test_parts_fill_one_wave():
+    """Parts are as short as they can be while their CTAs run at once."""
+    for tiles, heads in ((np.array([500]), 8), (np.array([64, 3, 200]), 8), (np.array([10] * 48), 4)):
+        parts = paged._shares(tiles, heads, 296, 4)
+        assert parts.sum() * heads <= 296
+        share = -(-tiles // parts).max()
+        assert share <= 4 or (-(-tiles // (share - 1))).sum() * heads > 296
+
+
+def test_a_cache_is_refused_in_host_memory():
+    data = torch.zeros(2, 2, 1, 16, 128, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="GPU"):
+        paged.PagedCache(data)
+    for bad in (data[..., :64], data[:, :1], data.float(), data.view(2, 2, 2, 8, 128), data.transpose(2, 3)):
+        with pytest.raises(ValueError):
+            paged.PagedCache(bad)
+    with pytest.raises(ValueError):
+        paged.PagedCache(data, torch.zeros(2, 2, 1, 16))                # bf16 has no scales
+    with pytest.raises(ValueError):
+        paged.PagedCache(data.to(torch.float8_e4m3fn))                  # e4m3 has
+    with pytest.raises(ValueError):
+        paged.PagedCache(data.to(torch.float8_e4m3fn), torch.zeros(2, 2, 16))

@@ -1,0 +1,504 @@
+"""Paged key/value cache (csrc/paged_cache.cu, attn_paged.cu, attn_paged_sm100.cu) against plain arithmetic in 64 bits."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+D = 128
+SCALE = D ** -0.5
+BF16, E4M3 = torch.bfloat16, torch.float8_e4m3fn
+
+
+def tables_for(kv_lens, page, spare=3, seed=0):
+    """Pages of every sequence in an order that no address computation gets right by chance, and how many there are."""
+    need = [-(-k // page) for k in kv_lens]
+    order = torch.randperm(sum(need) + spare, generator=torch.Generator().manual_seed(seed)).tolist()
+    out = []
+    for n in need:
+        out.append(order[:n])
+        order = order[n:]
+    return out, sum(need) + spare
+
+
+def quantised(x):
+    """The definition in fp32: codes and scales of rows of 128.  (A number divided by a tensor would be the product with its reciprocal.)"""
+    a = x.float().abs().amax(-1).clamp_min(2.0 ** -110)
+    return (x.float() * (torch.full_like(a, 448.0) / a)[..., None]).to(E4M3), a / torch.full_like(a, 448.0)
+
+
+def make(kv_lens, page, hk, dtype, seed=0, spare=3):
+    """A cache full of random values, and per sequence what it holds, in 64 bits: [2, heads, keys, 128]."""
+    from sensenova_u1_b200.ops import paged
+    tables, pages = tables_for(kv_lens, page, spare, seed)
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x = torch.randn(pages, 2, hk, page, D, device="cuda", generator=g).to(BF16)
+    if dtype == E4M3:
+        x = x * torch.exp2(torch.randint(-3, 4, x.shape[:4] + (1,), device="cuda", generator=g)).to(BF16)
+        codes, scales = quantised(x)
+        cache, held = paged.PagedCache(codes, scales), codes.double() * scales.double()[..., None]
+    else:
+        cache, held = paged.PagedCache(x), x.double()
+    rows = [torch.cat([held[p] for p in t], 2)[:, :, :k] if k else held[0, :, :, :0] for t, k in zip(tables, kv_lens)]
+    return cache, tables, rows
+
+
+def exact(q, q_lens, rows, limits):
+    """Attention in 64 bits, and per output element the mean of |v| under the same probabilities."""
+    out, size, r = torch.zeros(q.shape, dtype=torch.float64, device=q.device), torch.zeros(q.shape, dtype=torch.float64, device=q.device), 0
+    for n, kv in zip(q_lens, rows):
+        if n and kv.shape[2]:
+            g = q.shape[1] // kv.shape[1]
+            k, v = kv[0].repeat_interleave(g, 0), kv[1].repeat_interleave(g, 0)
+            s = torch.einsum("rhd,hkd->hrk", q[r:r + n].double(), k) * SCALE
+            hidden = torch.arange(kv.shape[2], device=q.device)[None] >= limits[r:r + n, None]
+            p = torch.nan_to_num(torch.softmax(s.masked_fill(hidden, float("-inf")), -1), nan=0.0)
+            out[r:r + n] = torch.einsum("hrk,hkd->rhd", p, v)
+            size[r:r + n] = torch.einsum("hrk,hkd->rhd", p, v.abs())
+        r += n
+    return out, size
+
+
+def causal(q_lens, kv_lens):
+    return torch.tensor([k - n + i + 1 for n, k in zip(q_lens, kv_lens) for i in range(n)], device="cuda")
+
+
+def near(got, ref, size):
+    """One rounding of every probability (2^-8 of it, so 2^-8 of the mean of |v|) and one of the result (2^-8 of it).  Sums, the
+    approximate exponentials (2^-22) and the fp32 scores add less than 2^-11 of the mean of |v|: scores below 2^6 have an
+    error below 2^6 * 128 * 2^-24."""
+    return ((got.double() - ref).abs() <= (2.0 ** -8 + 2.0 ** -11) * size + 2.0 ** -8 * ref.abs()).all()
+
+
+def attend(q_lens, kv_lens, hq, hk, page, dtype, limits=None, seed=0):
+    from sensenova_u1_b200.ops import paged
+    cache, tables, rows = make(kv_lens, page, hk, dtype, seed)
+    n = sum(q_lens)
+    g = torch.Generator(device="cuda").manual_seed(seed + 1)
+    q = torch.randn(n + 2, hq + 3, D, device="cuda", generator=g).to(BF16)[:, 1:hq + 1]         # rows of a wider buffer
+    out = torch.full((n + 2, hq, D), 7.0, device="cuda", dtype=BF16)
+    plan = paged.build_plan(cache, hq, q_lens, kv_lens, tables, limits=limits)
+    paged.paged_attention(q, cache, plan, SCALE, out=out)
+    lim = causal(q_lens, kv_lens) if limits is None else torch.as_tensor(limits, device="cuda")
+    ref, size = exact(q[:n], q_lens, rows, lim)
+    assert near(out[:n], ref, size)
+    assert (out[n:] == 7).all()                           # rows behind the last sequence
+    assert (out[:n][lim == 0] == 0).all()                 # rows without keys
+    again = paged.paged_attention(q, cache, plan, SCALE)
+    assert torch.equal(again, out[:n])                    # the same bits, whatever order the CTAs ran in
+
+
+# ------------------------------------------------------------------ writing and reading
+@pytest.mark.parametrize("dtype", [BF16, E4M3])
+@pytest.mark.parametrize("page", [16, 32, 64, 128])
+@pytest.mark.parametrize("hk", [1, 4, 7])
+def test_write_then_read(page, hk, dtype):
+    from sensenova_u1_b200.ops import paged
+    q_lens, kv_lens = [1, 0, 130, 17, 5], [1, 3, 130, 200, 16]
+    tables, pages = tables_for(kv_lens, page)
+    cache = paged.PagedCache.empty(pages, page, hk, dtype)
+    cache.data.view(torch.uint8).fill_(0x3c)
+    if dtype == E4M3:
+        cache.scales.fill_(0.25)
+    before = cache.data.clone()
+    n = sum(q_lens)
+    g = torch.Generator(device="cuda").manual_seed(page + hk)
+    x = (torch.randn(n + 3, 2 * hk + 2, D, device="cuda", generator=g) * torch.exp2(torch.randint(
+        -40, 40, (n + 3, 2 * hk + 2, 1), device="cuda", generator=g))).to(BF16)
+    k, v = x[:, 1:1 + hk], x[:, 2 + hk:]
+    plan = paged.build_plan(cache, hk, q_lens, kv_lens, tables)
+    paged.paged_write(cache, k, v, plan)
+    want, touched = before.clone(), torch.zeros(pages, page, dtype=torch.bool, device="cuda")
+    scales = None if dtype == BF16 else torch.full((pages, 2, hk, page), 0.25, device="cuda")
+    r = 0
+    for n_, kv, t in zip(q_lens, kv_lens, tables):
+        for i in range(n_):
+            pos = kv - n_ + i
+            pg, off = t[pos // page], pos % page
+            row = torch.stack([k[r], v[r]])
+            if dtype == BF16:
+                want[pg, :, :, off] = row
+            else:
+                c, s = quantised(row)
+                want.view(torch.uint8)[pg, :, :, off] = c.view(torch.uint8)
+                scales[pg, :, :, off] = s
+            touched[pg, off] = True
+            r += 1
+    assert torch.equal(cache.data.view(torch.uint8), want.view(torch.uint8))         # and nothing else was written
+    if dtype == E4M3:
+        assert torch.equal(cache.scales, scales)
+    kr, vr = paged.paged_read(cache, plan)
+    assert kr.shape == (sum(kv_lens), hk, D)
+    at = 0
+    for i, (kv, t) in enumerate(zip(kv_lens, tables)):
+        for which, got in ((0, kr), (1, vr)):
+            held = torch.cat([cache.data.view(torch.uint8)[p, which].view(dtype).float() for p in t], 1)[:, :kv] if kv else None
+            if dtype == E4M3 and kv:
+                held = held * torch.cat([cache.scales[p, which] for p in t], 1)[:, :kv, None]
+            if kv:
+                assert torch.equal(got[at:at + kv].transpose(0, 1), held.to(BF16))
+        at += kv
+
+
+def test_quantised_rows_are_within_half_a_step():
+    """e4m3 has four significant bits: half a step is 2^-4 of the value, or 2^-10 of the row's scale below its smallest normal value
+    (2^-6, steps of 2^-9); the product with the scale is rounded once more to bf16 (2^-8); fp32 steps before add 2^-22."""
+    from sensenova_u1_b200.ops import paged
+    cache = paged.PagedCache.empty(4, 128, 2, E4M3)
+    plan = paged.build_plan(cache, 2, [512], [512], [[2, 0, 3, 1]])
+    x = torch.randn(2, 512, 2, D, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)).to(BF16)
+    paged.paged_write(cache, x[0], x[1], plan)
+    got = torch.stack(paged.paged_read(cache, plan)).double()
+    scale = x.double().abs().amax(-1, keepdim=True) / 448
+    step = torch.maximum(x.double().abs() * 2.0 ** -4, scale * 2.0 ** -10)
+    assert ((got - x.double()).abs() <= step * (1 + 2.0 ** -8) + (2.0 ** -8 + 2.0 ** -20) * x.double().abs()).all()
+
+
+def test_rows_at_the_ends_of_the_range():
+    from sensenova_u1_b200.ops import paged
+    cache = paged.PagedCache.empty(1, 16, 1, E4M3)
+    big = torch.finfo(BF16).max
+    x = torch.zeros(8, 1, D, device="cuda", dtype=BF16)
+    x[1, 0, 5] = 2.0 ** -130                             # subnormal: below what a scale is made of
+    x[2, 0, :2] = torch.tensor([big, -big])
+    x[3, 0, 7], x[4, 0, 9], x[5, 0, 1] = float("inf"), float("nan"), float("-inf")
+    x[6, 0] = 2.0 ** -100
+    x[7, 0] = -1.0
+    plan = paged.build_plan(cache, 1, [8], [8], [[0]])
+    paged.paged_write(cache, x, x, plan)
+    k, v = paged.paged_read(cache, plan)
+    assert torch.equal(k.view(torch.int16), v.view(torch.int16))
+    assert (k[0] == 0).all() and (k[1].abs() <= 2.0 ** -113).all() and torch.isnan(k[3:6]).all()
+    assert torch.equal(k[2], x[2]) and torch.equal(k[6:], x[6:])
+
+
+def test_every_code_is_widened_exactly():
+    """Scores of one-hot queries with a key row of all 256 codes (in two rows) show how attention widens them; read does the same."""
+    from sensenova_u1_b200.ops import paged
+    cache = paged.PagedCache.empty(1, 16, 1, E4M3)
+    codes = torch.arange(256, dtype=torch.uint8, device="cuda")
+    codes[127], codes[255] = 0, 0                         # the NaN codes never stand in a cache
+    cache.data.view(torch.uint8).zero_()
+    cache.data.view(torch.uint8)[0, :, 0, :2] = codes.view(2, D)
+    cache.scales.fill_(1.0)
+    plan = paged.build_plan(cache, 1, [2], [2], [[0]], limits=[1, 2])
+    q = torch.zeros(2, 1, D, device="cuda", dtype=BF16)
+    value = codes.view(torch.uint8).view(E4M3).double().view(2, D)
+    out = paged.paged_attention(q, cache, plan, 1.0)      # one key: its value; two keys of equal scores: their mean
+    assert torch.equal(out[0, 0].double(), value[0])
+    assert ((out[1, 0].double() - value.mean(0)).abs() <= 2.0 ** -8 * value.mean(0).abs()).all()
+    k, _ = paged.paged_read(cache, plan)
+    assert torch.equal(k[:, 0].double(), value)
+    # keys: query e_d gives the score k_d of row 0 and k'_d of row 1; v = (1, 0, ...), (0, 1, ...) shows both probabilities
+    cache.data.view(torch.uint8)[0, 1].zero_()
+    cache.data[0, 1, 0, 0, 0] = 1.0
+    cache.data[0, 1, 0, 1, 1] = 1.0
+    eye = torch.eye(D, device="cuda").to(BF16).view(D, 1, D)
+    for a in range(0, D, 16):
+        plan = paged.build_plan(cache, 1, [16], [16], [[0]], limits=[2] * 16)
+        out = paged.paged_attention(eye[a:a + 16], cache, plan, 2.0 ** -6)[:, 0, :2].double()
+        p = torch.softmax(value[:, a:a + 16].T * 2.0 ** -6, -1)
+        assert ((out - p).abs() <= (2 * 2.0 ** -8 + 2.0 ** -12) * p).all()
+
+
+# ------------------------------------------------------------------ attention
+@pytest.mark.parametrize("dtype", [BF16, E4M3])
+@pytest.mark.parametrize("page", [16, 64, 128])
+@pytest.mark.parametrize("hq,hk", [(4, 4), (4, 2), (12, 4), (8, 1), (20, 1)])
+def test_one_token(hq, hk, page, dtype):
+    attend([1] * 6, [1, 63, 64, 65, 700, 129], hq, hk, page, dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF16, E4M3])
+@pytest.mark.parametrize("page", [16, 32, 128])
+@pytest.mark.parametrize("q_lens,kv_lens", [([5, 0, 3, 1], [5, 9, 300, 1000]), ([8, 7], [8, 71]), ([16], [2000]), ([33, 2], [33, 200])])
+def test_a_few_tokens(q_lens, kv_lens, page, dtype):
+    attend(q_lens, kv_lens, 8, 2, page, dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF16, E4M3])
+@pytest.mark.parametrize("q_lens,kv_lens,hq,hk,page", [
+    ([130, 1, 257], [130, 500, 1000], 8, 2, 16), ([64], [64], 4, 1, 64), ([300], [301], 3, 3, 32), ([97, 1, 1], [5000, 3, 129], 12, 4, 128),
+    ([1, 200, 31, 0, 90], [64, 200, 95, 7, 128], 20, 2, 16), ([70], [70], 100, 1, 16)])
+def test_chunks(q_lens, kv_lens, hq, hk, page, dtype):
+    attend(q_lens, kv_lens, hq, hk, page, dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF16, E4M3])
+@pytest.mark.parametrize("hq,hk", [(4, 1), (6, 2), (32, 8)])
+def test_limits(hq, hk, dtype):
+    """Pictures, rows without any key, rows that read a prefix only."""
+    q_lens, kv_lens = [40, 3, 150], [90, 3, 700]
+    lim = causal(q_lens, kv_lens).tolist()
+    for i in range(10, 30):
+        lim[i] = 50 + 30                                  # rows 10 .. 29 of the first sequence are a picture
+    lim[0] = lim[41] = 0
+    lim[40] = 3
+    for i in range(60, 90):
+        lim[i] = 700
+    for i in range(90, 120):
+        lim[i] = (i * 37) % 650                           # in any order
+    lim[130:193] = [0] * 63
+    attend(q_lens, kv_lens, hq, hk, 32, dtype, limits=lim)
+
+
+@pytest.mark.parametrize("dtype", [BF16, E4M3])
+def test_all_rows_without_keys(dtype):
+    attend([3, 40], [64, 40], 8, 2, 16, dtype, limits=[0] * 43)
+
+
+@pytest.mark.parametrize("q_len", [1, 6, 60])
+def test_one_long_sequence_in_many_parts(q_len):
+    attend([q_len], [20000 + q_len], 8, 2, 16, E4M3)
+    attend([q_len], [9001], 4, 4, 64, BF16)
+
+
+@pytest.mark.parametrize("dtype", [BF16, E4M3])
+@pytest.mark.parametrize("q_lens,kv_lens", [([1, 1], [50, 64]), ([5], [70]), ([100, 1], [300, 10])])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_what_no_row_may_read_does_not_matter(q_lens, kv_lens, bad, dtype):
+    """Places behind a sequence's last token, pages of nobody, and keys beyond every limit hold NaN or infinities."""
+    from sensenova_u1_b200.ops import paged
+    page = 16
+    cache, tables, _ = make(kv_lens, page, 2, dtype)
+    lim = [max(0, x - 3) for x in causal(q_lens, kv_lens).tolist()]
+    plan = paged.build_plan(cache, 8, q_lens, kv_lens, tables, limits=lim)
+    q = torch.randn(sum(q_lens), 8, D, device="cuda", generator=torch.Generator(device="cuda").manual_seed(2)).to(BF16)
+    clean = paged.paged_attention(q, cache, plan, SCALE).clone()
+    own = torch.zeros(cache.pages, page, dtype=torch.bool, device="cuda")
+    r = 0
+    for n, t in zip(q_lens, tables):
+        for pos in range(max(lim[r:r + n])):
+            own[t[pos // page], pos % page] = True
+        r += n
+    hide = ~own[:, None, None, :].expand(cache.pages, 2, 2, page)
+    if dtype == E4M3:
+        cache.scales[hide] = bad
+        cache.data.view(torch.uint8)[hide] = 0x7e
+    else:
+        cache.data[hide] = bad
+    assert torch.equal(paged.paged_attention(q, cache, plan, SCALE), clean)
+
+
+@pytest.mark.parametrize("dtype", [BF16, E4M3])
+@pytest.mark.parametrize("which", [0, 1])
+@pytest.mark.parametrize("q_len,kv_len,at", [(5, 70, 67), (5, 70, 65), (100, 300, 250), (100, 300, 201), (300, 600, 511), (40, 2000, 1990)])
+def test_a_value_that_is_not_finite_reaches_the_rows_that_read_it(q_len, kv_len, at, which, dtype):
+    from sensenova_u1_b200.ops import paged
+    cache, tables, _ = make([kv_len], 32, 2, dtype)
+    plan = paged.build_plan(cache, 8, [q_len], [kv_len], tables)
+    q = torch.randn(q_len, 8, D, device="cuda", generator=torch.Generator(device="cuda").manual_seed(2)).to(BF16)
+    clean = paged.paged_attention(q, cache, plan, SCALE).clone()
+    pg, off = tables[0][at // 32], at % 32
+    if dtype == E4M3:
+        cache.scales[pg, which, 1, off] = float("nan")
+    else:
+        cache.data[pg, which, 1, off, 77] = float("nan")
+    out = paged.paged_attention(q, cache, plan, SCALE)
+    reads = torch.arange(kv_len - q_len, kv_len, device="cuda") >= at
+    assert torch.equal(out[~reads], clean[~reads]) and torch.equal(out[:, :4], clean[:, :4])
+    assert torch.isnan(out[reads][:, 4:]).any(-1).all()
+
+
+def test_large_scores():
+    """The running maximum moves by hundreds, and some keys' probabilities are 0 in fp32."""
+    from sensenova_u1_b200.ops import paged
+    kv, q_lens = [900, 400], [70, 1]
+    cache, tables, rows = make(kv, 16, 2, BF16)
+    q = (40 * torch.randn(71, 4, D, device="cuda", generator=torch.Generator(device="cuda").manual_seed(3))).to(BF16)
+    plan = paged.build_plan(cache, 4, q_lens, kv, tables)
+    out = paged.paged_attention(q, cache, plan, SCALE)
+    ref, size = exact(q, q_lens, rows, causal(q_lens, kv))
+    # scores up to 2^9: products of 2^9 sqrt(128) summed in fp32 are off by at most 2^12.5 * 128 / 2 * 2^-24 = 2^-5.5 in the worst
+    # case of all terms of one sign; terms of random sign stay below 2^12.5 * 2^-24 * sqrt(128) = 2^-8
+    assert ((out.double() - ref).abs() <= 2 * (2.0 ** -8 + 2.0 ** -8) * size + 2.0 ** -8 * ref.abs()).all()
+
+
+# ------------------------------------------------------------------ together
+@pytest.mark.parametrize("dtype", [BF16, E4M3])
+def test_a_prompt_in_chunks_then_tokens(dtype):
+    """Two sequences: one prompt in three chunks while the other decodes, then both decode in a captured step."""
+    from sensenova_u1_b200.ops import paged
+    hq, hk, page = 8, 2, 16
+    steps = [[200, 40], [90, 1], [31, 1]] + [[1, 1]] * 9
+    total = [sum(s[i] for s in steps) for i in range(2)]
+    g = torch.Generator(device="cuda").manual_seed(5)
+    q, k, v = (torch.randn(2, max(total), h, D, device="cuda", generator=g).to(BF16) for h in (hq, hk, hk))
+    tables, pages = tables_for(total, page)
+    cache = paged.PagedCache.empty(pages, page, hk, dtype)
+    cache.data.view(torch.uint8).fill_(0x7f)
+    out, at = torch.zeros(2, max(total), hq, D, device="cuda", dtype=BF16), [0, 0]
+    pick = lambda t, n: torch.cat([t[i, at[i]:at[i] + n[i]] for i in range(2)])
+    for s in steps[:4]:
+        plan = paged.build_plan(cache, hq, s, [a + n for a, n in zip(at, s)], tables)
+        paged.paged_write(cache, pick(k, s), pick(v, s), plan)
+        o = paged.paged_attention(pick(q, s), cache, plan, SCALE)
+        for i in range(2):
+            out[i, at[i]:at[i] + s[i]] = o[sum(s[:i]):sum(s[:i + 1])]
+            at[i] += s[i]
+    # a captured step that moves itself on
+    left = len(steps) - 4
+    plan = paged.build_plan(cache, hq, [1, 1], at, tables, grow=left)
+    bufs = [torch.empty(2, h, D, device="cuda", dtype=BF16) for h in (hq, hk, hk)]
+    o = torch.empty(2, hq, D, device="cuda", dtype=BF16)
+
+    def step():
+        plan.advance()
+        paged.paged_write(cache, bufs[1], bufs[2], plan)
+        paged.paged_attention(bufs[0], cache, plan, SCALE, out=o)
+
+    def feed():
+        for b, t in zip(bufs, (q, k, v)):
+            b.copy_(pick(t, [1, 1]))
+
+    feed()
+    step()
+    graph = torch.cuda.CUDAGraph()
+    plan.advance(-1)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        step()
+    for _ in range(left):
+        feed()
+        graph.replay()
+        for i in range(2):
+            out[i, at[i]] = o[i]
+            at[i] += 1
+    assert at == total
+    held = torch.stack([k, v], 1).transpose(2, 3)                       # [2, k v, heads, tokens, 128]
+    if dtype == E4M3:
+        codes, scales = quantised(held)
+        held = codes.double() * scales.double()[..., None]
+    for i in range(2):
+        lim = torch.arange(1, total[i] + 1, device="cuda")
+        ref, size = exact(q[i, :total[i]], [total[i]], [held[i, :, :, :total[i]].double()], lim)
+        assert near(out[i, :total[i]], ref, size)
+
+
+def test_the_whole_prompt_as_the_packed_kernel_sees_it():
+    """Chunks over pages against the contiguous kernel on the same prompt with a picture in it."""
+    from sensenova_u1_b200.ops import attention as A, paged
+    n, hq, hk, a, b = 333, 8, 2, 100, 260
+    g = torch.Generator(device="cuda").manual_seed(9)
+    q, k, v = (torch.randn(n, h, D, device="cuda", generator=g).to(BF16) for h in (hq, hk, hk))
+    pos = torch.arange(n, device="cuda", dtype=torch.int32)
+    pos[a:b], pos[b:] = a, torch.arange(a + 1, a + 1 + n - b, device="cuda")
+    img = torch.zeros_like(pos)
+    img[a:b] = 1
+    meta = A.make_meta(torch.zeros_like(pos), pos, img)
+    ref, _ = A.attention_fwd(q, k, v, A.build_plan(meta), SCALE, want_lse=False)
+    lim = [b if a <= i < b else i + 1 for i in range(n)]
+    cache = paged.PagedCache.empty(6, 64, hk)
+    tables, out = [[3, 0, 5, 1, 4, 2]], []
+    for lo, hi in ((0, 90), (90, 261), (261, n)):
+        plan = paged.build_plan(cache, hq, [hi - lo], [hi], tables, limits=lim[lo:hi])
+        paged.paged_write(cache, k[lo:hi], v[lo:hi], plan)
+        out.append(paged.paged_attention(q[lo:hi], cache, plan, SCALE))
+    dense, size = exact(q, [n], [torch.stack([k, v]).transpose(1, 2).double()], torch.tensor(lim, device="cuda"))
+    assert near(torch.cat(out), dense, size) and near(ref, dense, size)
+
+
+def test_two_streams_and_a_shared_prompt():
+    """Two batches at once on two streams; their sequences read the same first pages."""
+    from sensenova_u1_b200.ops import paged
+    kv, page = [700, 650], 16
+    cache, tables, _ = make(kv, page, 2, E4M3)
+    tables[1] = tables[0][:20] + tables[1][20:]
+    g = torch.Generator(device="cuda").manual_seed(4)
+    jobs = []
+    for s, q_lens in ((torch.cuda.Stream(), [1, 1]), (torch.cuda.Stream(), [60, 3])):
+        q = torch.randn(sum(q_lens), 8, D, device="cuda", generator=g).to(BF16)
+        plan = paged.build_plan(cache, 8, q_lens, kv, tables)
+        jobs.append((s, q, plan, paged.paged_attention(q, cache, plan, SCALE)))
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for _ in range(20):
+        for i, (s, q, plan, _) in enumerate(jobs):
+            with torch.cuda.stream(s):
+                outs[i].append(paged.paged_attention(q, cache, plan, SCALE))
+    torch.cuda.synchronize()
+    for (_, _, _, ref), got in zip(jobs, outs):
+        assert all(torch.equal(o, ref) for o in got)
+
+
+def test_offsets_beyond_32_bits():
+    """Pages behind the first four gigabytes of a cache."""
+    from sensenova_u1_b200.ops import paged
+    page, hk = 128, 8
+    pages = (5 << 30) // (2 * hk * page * D)
+    cache = paged.PagedCache.empty(pages, page, hk, E4M3)
+    last = list(range(pages - 3, pages))
+    q_lens, kv = [300], [300]
+    k, v, q = (torch.randn(300, h, D, device="cuda", generator=torch.Generator(device="cuda").manual_seed(h)).to(BF16) for h in (hk, hk, 16))
+    plan = paged.build_plan(cache, 16, q_lens, kv, [last])
+    paged.paged_write(cache, k, v, plan)
+    held = []
+    for x in (k, v):
+        c, s = quantised(x)
+        held.append((c.double() * s.double()[..., None]).transpose(0, 1))
+    got = paged.paged_read(cache, plan)
+    for x, h in zip(got, held):
+        assert torch.equal(x.transpose(0, 1), h.float().to(BF16))
+    ref, size = exact(q, q_lens, [torch.stack(held)], causal(q_lens, kv))
+    assert near(paged.paged_attention(q, cache, plan, SCALE), ref, size)
+
+
+# ------------------------------------------------------------------ refusals
+def test_refusals():
+    from sensenova_u1_b200.ops import paged
+    cache, tables, _ = make([40], 16, 2, BF16)
+    plan = paged.build_plan(cache, 8, [3], [40], tables)
+    q, k = torch.zeros(3, 8, D, device="cuda", dtype=BF16), torch.zeros(3, 2, D, device="cuda", dtype=BF16)
+    with pytest.raises(ValueError):
+        paged.build_plan(cache, 7, [3], [40], tables)                    # heads
+    for bad in (q[:2], q[:, :4], q.float(), q.cpu(), q[..., :64], q.transpose(0, 1)):
+        with pytest.raises(ValueError):
+            paged.paged_attention(bad, cache, plan, SCALE)
+        with pytest.raises(ValueError):
+            paged.paged_attention(q, cache, plan, SCALE, out=bad)
+    for bad in (k[:2], k[:, :1], k.float(), k.cpu()):
+        with pytest.raises(ValueError):
+            paged.paged_write(cache, bad, k, plan)
+        with pytest.raises(ValueError):
+            paged.paged_write(cache, k, bad, plan)
+    other = paged.PagedCache.empty(cache.pages, 32, 2)
+    for call in (lambda: paged.paged_attention(q, other, plan, SCALE), lambda: paged.paged_write(other, k, k, plan),
+                 lambda: paged.paged_read(other, plan)):
+        with pytest.raises(ValueError):
+            call()
+    shifted = torch.zeros(3 * 8 * D + 1, device="cuda", dtype=BF16)[1:].view(3, 8, D)      # rows of 16 bytes, off by two
+    with pytest.raises(RuntimeError, match="aligned"):
+        paged.paged_attention(shifted, cache, plan, SCALE)
+
+
+def test_empty_calls():
+    from sensenova_u1_b200.ops import paged
+    cache, tables, _ = make([40], 16, 2, BF16)
+    plan = paged.build_plan(cache, 8, [0], [40], tables)
+    e = lambda h: torch.empty(0, h, D, device="cuda", dtype=BF16)
+    assert paged.paged_attention(e(8), cache, plan, SCALE).shape == (0, 8, D)
+    paged.paged_write(cache, e(2), e(2), plan)
+    plan = paged.build_plan(cache, 8, [], [], [])
+    assert paged.paged_read(cache, plan)[0].shape == (0, 2, D)
+
+
+def test_a_page_that_does_not_exist_is_reported():
+    """The table was changed on the device behind the plan's back: the launch ends, touches nothing outside, and says so."""
+    from sensenova_u1_b200.ops import _lib, paged
+    cache, tables, _ = make([40, 20], 16, 2, BF16)
+    plan = paged.build_plan(cache, 8, [1, 1], [40, 20], tables)
+    q, k = torch.zeros(2, 8, D, device="cuda", dtype=BF16), torch.zeros(2, 2, D, device="cuda", dtype=BF16)
+    at = (plan._args.table - plan._store.data_ptr()) // 4
+    for page in (cache.pages, -1):
+        plan._store[at + 2] = page                       # third page of the first sequence, its new token's
+        before = cache.data.clone()
+        for call in (lambda: paged.paged_write(cache, k, k, plan), lambda: paged.paged_read(cache, plan),
+                     lambda: paged.paged_attention(q, cache, plan, SCALE)):
+            _lib.check_status()
+            call()
+            with pytest.raises(_lib.NativeLibraryError, match="page"):
+                _lib.check_status()
+        same = cache.data == before
+        same[tables[1][1], :, :, 3] = True               # the second sequence's new token
+        assert same.all()
