@@ -493,7 +493,7 @@ static int launch_few(const Cache& c, const Plan& p, const FewArgs& a, cudaStrea
 using namespace snu1;
 
 // o_r = attention of row r over its sequence's first keys, rows [rows][heads of queries][128] bf16, ldq / ldo apart.
-// scratch: snu1_paged_attention_scratch bytes.
+// scratch: partial results (partial_rows x heads x (128 values, maximum, sum) in fp32), then unpack_pages bf16 pages of 128 tokens.
 SNU1_API int snu1_paged_attention(const void* cache, const void* plan, const void* q, long long ldq, void* o, long long ldo,
                                   float scale, void* scratch, void* stream) {
   using namespace paged;
@@ -520,6 +520,11 @@ SNU1_API int snu1_paged_attention(const void* cache, const void* plan, const voi
   a.status = device_status_word();
   cudaStream_t st = (cudaStream_t)stream;
   int rc = kHostOk;
+  if (p.chunk_count > 0) {
+    void* wide = a.part_ml + (((long long)p.partial_rows * c.heads + 15) & ~15ll);      // 128-byte aligned
+    if (c.fp8 && (rc = launch_widen(c, p, wide, st)) != kHostOk) return rc;
+    if ((rc = launch_chunks(c, p, q, ldq, p.rows, o, ldo, a.part, a.part_ml, a.scale_log2, wide, st)) != kHostOk) return rc;
+  }
   if (p.few_count > 0) {
     if (c.fp8)
       rc = p.few_rows <= 16 ? launch_few<true, 1>(c, p, a, st) : p.few_rows <= 32 ? launch_few<true, 2>(c, p, a, st) : launch_few<true, 4>(c, p, a, st);

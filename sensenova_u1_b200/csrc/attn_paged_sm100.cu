@@ -1,0 +1,696 @@
+// Attention of chunks of new tokens over a paged cache: many rows per key/value head, so the products belong on the
+// tensor cores (tcgen05.mma, scores and output of two row tiles in tensor memory).  The pipeline is that of attn_infer_sm100.cu:
+// warp 0 asks for pages through TMA, warp 1 issues the products in the order S_A(j+1) PV_A(j) S_B(j+1) PV_B(j), eight softmax
+// warps per tile of 16 rows each, probabilities over the other tile's scores as the A operand of the second product.
+//
+// What is different:
+// * A row tile holds all query heads of one key/value head: 128 / group tokens, head after head (one TMA box from q).  A
+//   chunk of a few dozen tokens fills the tensor cores' 128 rows, and the heads of a group read keys and values once.
+// * Keys and values come page by page (a lane of the loading warp per page).  e4m3 codes are widened into bf16 pages of scratch
+//   first (paged_read_kernel), which is exact; the scales are applied in fp32, a key's to its scores, a value's to its
+//   probabilities (rounding code times scale to bf16 instead would shift every score by up to 2^-8 of the sum of |q k|).
+// * The mask is one number per row, the keys that it may read; tiles that all rows read whole need no test.
+// * A work item is a part of the key tiles of two row tiles; unnormalised results of parts are joined by
+//   paged_merge_kernel.  ops/paged.py chooses the parts so that the waves of CTAs are full.
+// * Two warps that have nothing else to do bring the scales of an e4m3 cache, and otherwise clear values that are not finite (and rows behind the last token) in the tiles that
+//   some row may not read whole: a probability of zero does not hide them from the product.  Rows that may read such a
+//   value give NaN, the others are as if it were not there.
+#include <string.h>
+
+#include <mutex>
+
+#include "host_common.h"
+#include "paged.cuh"
+
+namespace snu1 {
+namespace paged {
+
+constexpr int BK = 128;                         // keys of a tile
+constexpr int CHALF = 128 * 64 * 2;             // 64 columns of a 128-row tile
+constexpr int CTILE = 2 * CHALF;
+constexpr int CK_STAGES = 3, CV_STAGES = 2;
+constexpr int CHUNK_THREADS = 640;
+constexpr int CS_STAGES = 2;                    // scales of a tile: 128 keys', then 128 values'
+constexpr int CHUNK_SMEM = (2 + CK_STAGES + CV_STAGES) * CTILE + CS_STAGES * 1024 + 512;
+
+struct ChunkArgs {
+  __nv_bfloat16* o;
+  long long ldo;
+  float* part;
+  float2* part_ml;
+  const int* first_page;   // scratch of widened rows: a sequence's first page there; null: the cache's own pages
+  const float* scales;     // of an e4m3 cache, whose pages (scale_page tokens) the table names
+  int page, pages, heads, scale_page, scale_pages;
+  float scale_log2;
+  int* status;
+};
+
+// see attn_infer_sm100.cu
+__device__ __forceinline__ void tally_add(int* c) {
+  asm volatile("red.release.cta.shared::cta.add.s32 [%0], 1;" ::"r"(smem_u32(c)) : "memory");
+}
+__device__ __forceinline__ bool tally_wait(const int* c, int target, volatile int* abort_flag, int* status, int where) {
+  const uint32_t a = smem_u32(c);
+  uint64_t t0 = 0;
+  for (uint32_t spins = 0;; ++spins) {
+    int v;
+    asm volatile("ld.acquire.cta.shared::cta.s32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+    if (v >= target) return true;
+    if ((spins & 0x3ff) == 32) {
+      if (*abort_flag) return false;
+      const uint64_t now = globaltimer_ns();
+      if (t0 == 0) t0 = now;
+      if (now - t0 > kLocalWaitNs) {
+        *abort_flag = 1;
+        report_status(status, kWaitTimeout, where);
+        return false;
+      }
+    }
+  }
+}
+
+template <bool FP8>
+__global__ void __launch_bounds__(CHUNK_THREADS, 1)
+    paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                       const __grid_constant__ CUtensorMap tm_v, const Plan p, const ChunkArgs args) {
+  // no room to align it by hand: there is no other shared memory, so it starts on a boundary of 1024 bytes
+  extern __shared__ __align__(1024) uint8_t smem_chunk[];
+  if ((smem_u32(smem_chunk) & 1023) != 0) {
+    if (threadIdx.x == 0) report_status(args.status, kBadShape, 10);
+    return;
+  }
+  uint8_t* sQ = smem_chunk;
+  uint8_t* sK = sQ + 2 * CTILE;
+  uint8_t* sV = sK + CK_STAGES * CTILE;
+  float* s_scale = reinterpret_cast<float*>(sV + CV_STAGES * CTILE);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(s_scale + CS_STAGES * 256);
+  uint64_t* q_full = bars;
+  uint64_t* k_full = bars + 1;
+  uint64_t* k_empty = k_full + CK_STAGES;
+  uint64_t* v_full = k_empty + CK_STAGES;
+  uint64_t* v_empty = v_full + CV_STAGES;
+  uint64_t* v_dirty = v_empty + CV_STAGES;      // [stages] the stage has to be cleaned
+  uint64_t* v_clean = v_dirty + CV_STAGES;      // [stages] the cleaning warps are done with it
+  uint64_t* s_full = v_clean + CV_STAGES;       // [2] per row tile
+  uint64_t* s_empty = s_full + 2;
+  uint64_t* p_full = s_empty + 2;
+  uint64_t* pv_done = p_full + 2;
+  uint64_t* sc_full = pv_done + 2;              // [CS_STAGES]
+  uint64_t* sc_empty = sc_full + CS_STAGES;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sc_empty + CS_STAGES);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* drained = reinterpret_cast<int*>(tmem_slot + 2);   // [2] softmax warps that have read a score tile, all tiles so far
+  int* lim_max = drained + 2;                              // [2] the largest and the smallest limit of a row tile
+  int* lim_min = lim_max + 2;
+  int* poison = lim_min + 2;                               // first key of a tile not read whole whose value was not finite
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    for (int i = 0; i < CK_STAGES; ++i) {
+      mbar_init(&k_full[i], 1);
+      mbar_init(&k_empty[i], 1);
+    }
+    for (int i = 0; i < CV_STAGES; ++i) {
+      mbar_init(&v_full[i], 1);
+      mbar_init(&v_empty[i], 1);
+      mbar_init(&v_dirty[i], 1);
+      mbar_init(&v_clean[i], 2);
+    }
+    for (int i = 0; i < CS_STAGES; ++i) {
+      mbar_init(&sc_full[i], 2);
+      mbar_init(&sc_empty[i], 16);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&s_empty[i], 8);
+      mbar_init(&p_full[i], 8);
+      mbar_init(&pv_done[i], 1);
+      drained[i] = lim_max[i] = 0;
+      lim_min[i] = *poison = 0x7fffffff;
+    }
+    *abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&tm_q);
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  pdl_wait();
+  pdl_trigger();
+
+  const int4 item = p.chunk[blockIdx.x / args.heads];
+  const int b = item.x, part = item.z & 0xffff, parts = item.z >> 16;
+  const int kvh = blockIdx.x % args.heads, G = p.group, T = 128 / G;       // tokens of a row tile
+  const int q0 = p.q_start[b], q_len = p.q_start[b + 1] - q0;
+  const int kv_len = seq_len(p, b);
+  const int token0 = item.y / G;
+  if (threadIdx.x < 2 * T) {
+    const int t = threadIdx.x / T, token = token0 + threadIdx.x;
+    if (token < q_len) {
+      const int l = row_limit(p, q0, q_len, kv_len, token);
+      atomicMax(&lim_max[t], l);
+      atomicMin(&lim_min[t], l);
+    }
+  }
+  __syncthreads();
+  const int most = max(lim_max[0], lim_max[1]);
+  const int all = (most + BK - 1) / BK;
+  const int j0 = (int)((long long)all * part / parts), n = (int)((long long)all * (part + 1) / parts) - j0;
+  // how a row tile reads key tile j of this part: not at all, in part, whole
+  auto cls = [&](int j, int t) -> int {
+    const int k0 = (j0 + j) * BK;
+    return k0 >= lim_max[t] ? kTileSkip : k0 + BK <= lim_min[t] ? kTileFull : kTilePartial;
+  };
+  auto dirty = [&](int j) -> bool { return !FP8 && (cls(j, 0) == kTilePartial || cls(j, 1) == kTilePartial); };
+  // columns: S_A and P_B [0,128), S_B and P_A [128,256), O_A [256,384), O_B [384,512)
+
+  // 640 threads start with 96 registers: 128 x 64 + 512 x 104 = 640 x 96
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    if (warp == 0) {
+      if (n > 0) {
+        if (lane == 0) {
+          mbar_expect_tx(q_full, 4 * T * G * 128);
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            tma_load_3d(sQ + t * CTILE, &tm_q, q_full, 0, kvh * G, q0 + token0 + t * T);
+            tma_load_3d(sQ + t * CTILE + CHALF, &tm_q, q_full, 64, kvh * G, q0 + token0 + t * T);
+          }
+        }
+        __syncwarp();
+        const int page = args.page, per = BK / page, used = (most + page - 1) / page;   // pages of a tile, of the sequence
+        const int* table = args.first_page == nullptr ? p.table + (long long)b * p.width : nullptr;
+        const int base = args.first_page == nullptr ? 0 : args.first_page[b];
+        // a lane's page of tile j, read a tile ahead
+        auto page_of = [&](int j) -> int {
+          const int i = (j0 + j) * per + lane;
+          return j < n && lane < per && i < used ? (table != nullptr ? table[i] : base + i) : 0;
+        };
+        int pk = page_of(0), pv = pk, ahead = page_of(1);
+        bool ok = true;
+        auto load = [&](uint8_t* dst, const CUtensorMap* tm, uint64_t* full, int j, int pg) {
+          const int live = min(per, used - (j0 + j) * per);
+          if (lane == 0) mbar_expect_tx(full, live * page * 256);
+          __syncwarp();
+          if (lane < live) {
+            if (pg < 0 || pg >= args.pages) report_status(args.status, kBadPage, 10);     // reads as zeros
+            tma_load_4d(dst + lane * page * 128, tm, full, 0, 0, kvh, pg);
+            tma_load_4d(dst + CHALF + lane * page * 128, tm, full, 64, 0, kvh, pg);
+          }
+          __syncwarp();
+        };
+        auto load_k = [&](int j, int pg) {
+          const int s = j % CK_STAGES;
+          ok = mbar_wait_warp(&k_empty[s], ((j / CK_STAGES) & 1) ^ 1, abort_flag, args.status, 1);
+          if (ok) load(sK + s * CTILE, &tm_k, &k_full[s], j, pg);
+        };
+        load_k(0, pk);
+        for (int j = 0; j < n && ok; ++j) {
+          if (j + 1 < n) {
+            pk = ahead;
+            ahead = page_of(j + 2);
+            load_k(j + 1, pk);
+          }
+          if (!ok) break;
+          const int s = j % CV_STAGES;
+          ok = mbar_wait_warp(&v_empty[s], ((j / CV_STAGES) & 1) ^ 1, abort_flag, args.status, 1);
+          if (!ok) break;
+          load(sV + s * CTILE, &tm_v, &v_full[s], j, pv);
+          pv = pk;
+        }
+      }
+    } else if (warp == 1) {
+      // The whole warp walks the tiles and one elected lane issues (see mbar_ready in attn_common.cuh).
+      if (n > 0) {
+        constexpr uint32_t idesc_s = make_idesc_bf16(128, 128, false, false);
+        constexpr uint32_t idesc_pv = make_idesc_bf16(128, 128, false, true);
+        const uint64_t q_desc = make_smem_desc(smem_u32(sQ), 0, 1024);
+        const uint64_t k_desc = make_smem_desc(smem_u32(sK), 0, 1024);
+        const uint64_t v_desc = make_smem_desc(smem_u32(sV), CHALF, 1024);
+        bool ok = mbar_wait(q_full, 0, abort_flag, args.status, 3);   // this lane's; see mbar_wait_warp
+        int s_cnt[2] = {0, 0}, pv_cnt[2] = {0, 0};
+        uint32_t cleaned = 0;                   // phase of every stage's v_clean
+        auto issue_s = [&](int j, int t) {
+          if (cls(j, t) != kTileSkip) {
+            ok &= mbar_wait(&s_empty[t], (s_cnt[t] & 1) ^ 1, abort_flag, args.status, 2);
+            tc_fence_after();
+            const uint64_t qd = q_desc + t * (CTILE >> 4), kd = k_desc + (j % CK_STAGES) * (CTILE >> 4);
+            __syncwarp();
+            if (elect_one()) {
+#pragma unroll
+              for (int k = 0; k < 8; ++k) {
+                constexpr uint32_t half = CHALF >> 4;
+                const uint32_t off = (k >> 2) * half + (k & 3) * 2;
+                umma_bf16_ss(tmem_base + t * 128, qd + off, kd + off, idesc_s, k > 0 ? 1u : 0u);
+              }
+              umma_commit(&s_full[t]);
+            }
+            __syncwarp();
+            ++s_cnt[t];
+          }
+        };
+        auto issue_pv = [&](int j, int t) {
+          if (cls(j, t) != kTileSkip) {
+            ok &= mbar_wait(&p_full[t], pv_cnt[t] & 1, abort_flag, args.status, 2);
+            tc_fence_after();
+            const uint64_t vd = v_desc + (j % CV_STAGES) * (CTILE >> 4);
+            const uint32_t p_tmem = tmem_base + (t ^ 1) * 128;
+            const uint32_t acc0 = pv_cnt[t] > 0 ? 1u : 0u;
+            __syncwarp();
+            if (elect_one()) {
+#pragma unroll
+              for (int k = 0; k < 8; ++k)
+                umma_bf16_ts(tmem_base + 256 + t * 128, p_tmem + k * 8, vd + k * (2048 >> 4), idesc_pv, k > 0 ? 1u : acc0);
+              umma_commit(&pv_done[t]);
+            }
+            __syncwarp();
+            ++pv_cnt[t];
+          }
+        };
+        auto release = [&](uint64_t* bar) {
+          if (elect_one()) umma_commit(bar);
+          __syncwarp();
+        };
+        ok &= mbar_wait(&k_full[0], 0, abort_flag, args.status, 3);
+        issue_s(0, 0);
+        issue_s(0, 1);
+        release(&k_empty[0]);
+        if (n > 1) ok &= mbar_wait(&k_full[1], 0, abort_flag, args.status, 3);
+        ok &= mbar_wait(&v_full[0], 0, abort_flag, args.status, 3);
+        for (int j = 0; j < n; ++j) {      // all tiles also after a time-out
+          const bool more = j + 1 < n, clean = dirty(j);
+          if (clean && lane == 0) mbar_arrive(&v_dirty[j % CV_STAGES]);
+          if (more) issue_s(j + 1, 0);
+          if (clean) {
+            const int s = j % CV_STAGES;
+            ok &= mbar_wait(&v_clean[s], (cleaned >> s) & 1, abort_flag, args.status, 3);
+            cleaned ^= 1u << s;
+          }
+          issue_pv(j, 0);
+          if (more) {
+            issue_s(j + 1, 1);
+            release(&k_empty[(j + 1) % CK_STAGES]);
+          }
+          issue_pv(j, 1);
+          if (more) {
+            release(&v_empty[j % CV_STAGES]);
+            if (j + 2 < n) ok &= mbar_wait(&k_full[(j + 2) % CK_STAGES], ((j + 2) / CK_STAGES) & 1, abort_flag, args.status, 3);
+            ok &= mbar_wait(&v_full[(j + 1) % CV_STAGES], ((j + 1) / CV_STAGES) & 1, abort_flag, args.status, 3);
+          }
+        }
+      }
+    } else if (FP8) {
+      // ------------------------------ scales --------------------------------
+      // A thread brings those of two keys, in registers a tile ahead.  Those of values that are not finite are cleared in tiles
+      // that some row may not read whole, as the values of a bf16 cache are.
+      const int tid = threadIdx.x - 64;
+      const int* table = p.table + (long long)b * p.width;
+      const long long to_values = (long long)args.heads * args.scale_page;
+      float2 ks, vs;
+      auto fetch = [&](int j) {
+        ks = vs = make_float2(0.f, 0.f);
+        const int key = (j0 + j) * BK + 2 * tid;
+        if (j < n && key < kv_len) {
+          const int pg = table[key / args.scale_page];
+          if (pg >= 0 && pg < args.scale_pages) {
+            const float* at = args.scales + ((long long)pg * 2 * args.heads + kvh) * args.scale_page + key % args.scale_page;
+            ks = *reinterpret_cast<const float2*>(at);
+            vs = *reinterpret_cast<const float2*>(at + to_values);
+          }
+        }
+      };
+      fetch(0);
+      bool ok = true;
+      for (int j = 0; j < n && ok; ++j) {
+        const int s = j % CS_STAGES, key = (j0 + j) * BK + 2 * tid;
+        ok = mbar_wait_warp(&sc_empty[s], ((j / CS_STAGES) & 1) ^ 1, abort_flag, args.status, 3);
+        if (!ok) break;
+        if (key + 1 >= kv_len) ks.y = vs.y = 0.f;
+        if (cls(j, 0) == kTilePartial || cls(j, 1) == kTilePartial) {
+          if (!(fabsf(vs.y) < INFINITY)) {
+            atomicMin(poison, key + 1);
+            vs.y = 0.f;
+          }
+          if (!(fabsf(vs.x) < INFINITY)) {
+            atomicMin(poison, key);
+            vs.x = 0.f;
+          }
+        }
+        *reinterpret_cast<float2*>(s_scale + s * 256 + 2 * tid) = ks;
+        *reinterpret_cast<float2*>(s_scale + s * 256 + 128 + 2 * tid) = vs;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sc_full[s]);
+        fetch(j + 1);
+      }
+    } else {
+      // ------------------------------ cleaning --------------------------------
+      bool ok = true;
+      const int tid = threadIdx.x - 64;
+      uint32_t told = 0;                        // phase of every stage's v_dirty
+      for (int j = 0; j < n && ok; ++j) {
+        if (!dirty(j)) continue;
+        const int s = j % CV_STAGES, k0 = (j0 + j) * BK;
+        // v_full alone would not do: its phases go on while these warps pass over tiles that are read whole
+        ok = mbar_wait_warp(&v_dirty[s], (told >> s) & 1, abort_flag, args.status, 3);
+        told ^= 1u << s;
+        if (ok) ok = mbar_wait_warp(&v_full[s], (j / CV_STAGES) & 1, abort_flag, args.status, 3);
+#pragma unroll 4
+        for (int i = 0; i < 32; ++i) {
+          const int key = i * 4 + (tid >> 4), ch = tid & 15;
+          uint4* at = reinterpret_cast<uint4*>(sV + s * CTILE + (ch >> 3) * CHALF + swz128_offset(key, ch & 7));
+          uint4 x = *at;
+          uint32_t* w = reinterpret_cast<uint32_t*>(&x);
+          bool bad = false;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const bool lo = (w[e] & 0x7f80u) == 0x7f80u, hi = (w[e] & 0x7f800000u) == 0x7f800000u;
+            bad |= lo || hi;
+            w[e] &= (lo ? 0xffff0000u : 0xffffffffu) & (hi ? 0xffffu : 0xffffffffu);
+          }
+          if (bad) {
+            *at = x;
+            if (k0 + key < kv_len) atomicMin(poison, k0 + key);
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&v_clean[s]);
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+    // ------------------------------ softmax --------------------------------
+    // A warp owns 16 rows; its threads hold columns 2 (lane % 4) + 8 i + {0, 1} of rows lane / 4 and lane / 4 + 8.
+    const int t = (warp - 4) >> 3;
+    const int base = (warp & 3) * 32 + ((warp - 4) >> 2 & 1) * 16;
+    const int q2 = (lane & 3) * 2;
+    const uint32_t lane_sel = (uint32_t)base << 16;
+    const uint32_t tmem_S = tmem_base + t * 128 + lane_sel;
+    const uint32_t tmem_O = tmem_base + 256 + t * 128 + lane_sel;
+    const uint32_t tmem_P = tmem_base + (t ^ 1) * 128 + lane_sel;   // over the other tile's scores
+    uint8_t* sOt = sQ + t * CTILE;
+    const uint32_t st_row = smem_u32(sOt) + (base + ((lane >> 3) & 1) * 8 + (lane & 7)) * 128;
+    const uint32_t st_chunk = (uint32_t)((lane >> 4) ^ (lane & 7)) << 4;
+    int lim[2];          // -1: no row of this sequence
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int row = base + (lane >> 2) + 8 * r, token = token0 + t * T + row / G;
+      lim[r] = row < T * G && token < q_len ? row_limit(p, q0, q_len, kv_len, token) : -1;
+    }
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    const float sc = args.scale_log2;
+    bool ok = true;
+    int cnt = 0;
+    // score tiles of the other row tile that are issued before PV_t(j): key tiles 0 .. j of B for A, 0 .. j + 1 of A for B
+    int other = t == 1 && n > 0 && cls(0, 0) != kTileSkip;
+    for (int j = 0; j < n; ++j) {        // all tiles also after a time-out, see mbar_wait_warp
+      other += t == 0 ? cls(j, 1) != kTileSkip : j + 1 < n && cls(j + 1, 0) != kTileSkip;
+      const int cls_t = cls(j, t);
+      const int cs = j % CS_STAGES;
+      const float* scale_k = s_scale + cs * 256 + q2;
+      if (cls_t == kTileSkip) {
+        if (FP8) {                           // not before the scales are there: an arrival counts for one tile
+          ok &= mbar_wait(&sc_full[cs], (j / CS_STAGES) & 1, abort_flag, args.status, 5);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sc_empty[cs]);
+        }
+        continue;
+      }
+      ok &= mbar_wait(&s_full[t], cnt & 1, abort_flag, args.status, 5);
+      tc_fence_after();
+      float sv[2][32];   // [columns 0-63, 64-127][4 i + 2 row + e]
+      {
+        uint32_t r0[32], r1[32];
+        tmem_ld_16x256b_x8(tmem_S, r0);
+        tmem_ld_16x256b_x8(tmem_S + 64, r1);
+        tmem_ld_wait();
+#pragma unroll
+        for (int c = 0; c < 32; ++c) {
+          sv[0][c] = __uint_as_float(r0[c]);
+          sv[1][c] = __uint_as_float(r1[c]);
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&s_empty[t]);
+        tally_add(&drained[t]);
+      }
+      if (FP8) {
+        ok &= mbar_wait(&sc_full[cs], (j / CS_STAGES) & 1, abort_flag, args.status, 5);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const uint64_t f = *reinterpret_cast<const uint64_t*>(scale_k + h * 64 + i * 8);
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              float& x = sv[h][4 * i + 2 * r];
+              float& y = sv[h][4 * i + 2 * r + 1];
+              unpack_f32x2(mul_f32x2(pack_f32x2(x, y), f), x, y);
+            }
+          }
+      }
+      if (cls_t != kTileFull) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const int end = lim[r] - (j0 + j) * BK - q2;       // columns 8 i + e from here on are hidden
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+                if (h * 64 + i * 8 + e >= end) sv[h][4 * i + 2 * r + e] = -INFINITY;
+        }
+      }
+      float mx[2];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        float m0 = fmaxf(sv[0][2 * r], sv[0][2 * r + 1]), m1 = fmaxf(sv[1][2 * r], sv[1][2 * r + 1]);
+#pragma unroll
+        for (int i = 1; i < 8; ++i) {
+          m0 = max3(m0, sv[0][4 * i + 2 * r], sv[0][4 * i + 2 * r + 1]);
+          m1 = max3(m1, sv[1][4 * i + 2 * r], sv[1][4 * i + 2 * r + 1]);
+        }
+        mx[r] = lim[r] < 0 ? -INFINITY : fmaxf(m0, m1);      // what other rows hold decides nothing here
+      }
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
+        mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
+      }
+      // the running maximum moves only when it is outgrown by more than 2^8, see attn_infer_sm100.cu
+      const bool rescale = __any_sync(0xffffffffu, mx[0] * sc > m[0] * sc + 8.f || mx[1] * sc > m[1] * sc + 8.f);
+      float alpha[2];
+      uint64_t nb2[2], acc[2][2];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const float m_new = rescale ? fmaxf(m[r], mx[r]) : m[r];
+        const float m_use = m_new == -INFINITY ? 0.f : m_new;
+        alpha[r] = rescale ? fast_exp2((m[r] - m_use) * sc) : 1.f;
+        m[r] = m_new;
+        nb2[r] = pack_f32x2(-m_use * sc, -m_use * sc);
+        acc[r][0] = acc[r][1] = 0ull;
+      }
+      const uint64_t sc2 = pack_f32x2(sc, sc);
+      uint32_t pk[32];      // probabilities, bf16 pairs: [2 (8-column group) + row]
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          uint64_t f = 0;
+          if (FP8) f = *reinterpret_cast<const uint64_t*>(scale_k + 128 + h * 64 + i * 8);
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            float x, y;
+            unpack_f32x2(fma_f32x2(pack_f32x2(sv[h][4 * i + 2 * r], sv[h][4 * i + 2 * r + 1]), sc2, nb2[r]), x, y);
+            x = fast_exp2(x);
+            y = fast_exp2(y);
+            const uint64_t xy = pack_f32x2(x, y);
+            acc[r][i & 1] = add_f32x2(acc[r][i & 1], xy);
+            if (FP8) unpack_f32x2(mul_f32x2(xy, f), x, y);
+            pk[16 * h + 2 * i + r] = pack_bf16x2(x, y);
+          }
+        }
+      if (FP8) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sc_empty[cs]);
+      }
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        float s0, s1;
+        unpack_f32x2(add_f32x2(acc[r][0], acc[r][1]), s0, s1);
+        l[r] = l[r] * alpha[r] + (s0 + s1);      // of this thread's columns; summed over the four threads at the end
+      }
+      if (cnt > 0) ok &= mbar_wait(&pv_done[t], (cnt - 1) & 1, abort_flag, args.status, 5);
+      // the other tile's warps have read the scores that P goes over
+      ok &= tally_wait(&drained[t ^ 1], 8 * other, abort_flag, args.status, 5);
+      tc_fence_after();
+      tmem_st_16x128b_x16(tmem_P, pk);
+      if (cnt > 0 && rescale) {
+        const uint64_t al0 = pack_f32x2(alpha[0], alpha[0]), al1 = pack_f32x2(alpha[1], alpha[1]);
+#pragma unroll 1
+        for (int c = 0; c < 2; ++c) {
+          uint32_t r[32];
+          tmem_ld_16x256b_x8(tmem_O + c * 64, r);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            float y0, y1;
+            unpack_f32x2(mul_f32x2(pack_f32x2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), (i & 2) ? al1 : al0),
+                         y0, y1);
+            r[i] = __float_as_uint(y0);
+            r[i + 1] = __float_as_uint(y1);
+          }
+          tmem_st_16x256b_x8(tmem_O + c * 64, r);
+        }
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full[t]);
+      ++cnt;
+    }
+    if (cnt > 0) ok &= mbar_wait(&pv_done[t], (cnt - 1) & 1, abort_flag, args.status, 5);
+    ok = __all_sync(0xffffffffu, ok);
+    if (ok) {
+      tc_fence_after();
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+        if (lim[r] > *poison) l[r] = __int_as_float(0x7fffffff);
+      }
+      if (item.w < 0) {
+        // Output rows leave through this warp's rows of the row tile's buffer (no product reads it any more), so that 16
+        // lanes store one row's 256 bytes.
+        const float inv[2] = {l[0] == 0.f ? 0.f : 1.f / l[0], l[1] == 0.f ? 0.f : 1.f / l[1]};
+        if (cnt > 0) {
+#pragma unroll 1
+          for (int h = 0; h < 2; ++h) {
+            uint32_t r[32];
+            tmem_ld_16x256b_x8(tmem_O + h * 64, r);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+              uint32_t w[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                w[e] = pack_bf16x2(__uint_as_float(r[4 * i + 2 * e]) * inv[e & 1], __uint_as_float(r[4 * i + 2 * e + 1]) * inv[e & 1]);
+              stmatrix_x4(st_row + h * CHALF + (st_chunk ^ (i << 4)), w[0], w[1], w[2], w[3]);
+            }
+          }
+          __syncwarp();
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int r = base + 2 * i + (lane >> 4), c = lane & 15, token = token0 + t * T + r / G;
+          if (r < T * G && token < q_len)
+            *reinterpret_cast<uint4*>(args.o + (long long)(q0 + token) * args.ldo + (long long)(kvh * G + r % G) * HEAD + c * 8) =
+                cnt > 0 ? *reinterpret_cast<const uint4*>(sOt + (c >> 3) * CHALF + swz128_offset(r, c & 7)) : make_uint4(0, 0, 0, 0);
+        }
+      } else {
+        const long long at0 = ((long long)item.w + t * T * G + base + (lane >> 2)) * args.heads + kvh;
+#pragma unroll 1
+        for (int h = 0; h < 2; ++h) {
+          uint32_t r[32];
+          if (cnt > 0) {
+            tmem_ld_16x256b_x8(tmem_O + h * 64, r);
+            tmem_ld_wait();
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) r[i] = 0;
+          }
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if (lim[e] >= 0) {
+              float* dst = args.part + (at0 + 8ll * e * args.heads) * HEAD + h * 64 + q2;
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                *reinterpret_cast<float2*>(dst + i * 8) = make_float2(__uint_as_float(r[4 * i + 2 * e]), __uint_as_float(r[4 * i + 2 * e + 1]));
+            }
+          __syncwarp();
+        }
+        if ((lane & 3) == 0) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if (lim[e] >= 0)        // scores that were all NaN are not to be taken for no keys at all
+              args.part_ml[at0 + 8ll * e * args.heads] = make_float2(m[e] == -INFINITY && l[e] != l[e] ? 0.f : m[e] * sc, l[e]);
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    if (*abort_flag) {
+      uint64_t t0 = globaltimer_ns();
+      while (globaltimer_ns() - t0 < 2000000ull) {
+      }
+    }
+    tc_fence_after();
+    tmem_dealloc(tmem_base, 512);
+  }
+}
+
+int launch_chunks(const Cache& c, const Plan& p, const void* q, long long ldq, int q_rows, void* o, long long ldo, float* part,
+                  float2* part_ml, float scale_log2, void* wide, cudaStream_t st) {
+  const int G = p.group, T = 128 / G;
+  CUtensorMap tm_q, tm_k = c.k, tm_v = c.v;
+  int rc;
+  {
+    const uint64_t dims[3] = {128, (uint64_t)c.heads * G, (uint64_t)q_rows}, str[2] = {256, (uint64_t)ldq * 2};
+    const uint32_t box[3] = {64, (uint32_t)G, (uint32_t)T};
+    if ((rc = encode_tmap(&tm_q, TmapType::kBf16, true, q, 3, dims, str, box)) != kHostOk) return rc;
+  }
+  ChunkArgs a;
+  a.first_page = nullptr;
+  a.scales = c.scales;
+  a.page = a.scale_page = c.page;
+  a.pages = a.scale_pages = c.pages;
+  if (c.fp8) {
+    const uint64_t dims[4] = {128, 128, (uint64_t)c.heads, (uint64_t)p.unpack_pages};
+    const uint64_t str[3] = {256, 256 * 128, 256ull * 128 * c.heads * 2};
+    const uint32_t box[4] = {64, 128, 1, 1};
+    if ((rc = encode_tmap(&tm_k, TmapType::kBf16, true, wide, 4, dims, str, box)) != kHostOk) return rc;
+    if ((rc = encode_tmap(&tm_v, TmapType::kBf16, true, (uint8_t*)wide + 256ull * 128 * c.heads, 4, dims, str, box)) != kHostOk) return rc;
+    a.first_page = p.unpack_first;
+    a.page = 128;
+    a.pages = p.unpack_pages;
+  }
+  a.o = (__nv_bfloat16*)o;
+  a.ldo = ldo;
+  a.part = part;
+  a.part_ml = part_ml;
+  a.heads = c.heads;
+  a.scale_log2 = scale_log2;
+  a.status = device_status_word();
+  int dev = 0;
+  SNU1_CUDA_CHECK(cudaGetDevice(&dev));
+  static std::once_flag once[64];
+  cudaError_t err = cudaSuccess;
+  std::call_once(once[dev & 63], [&]() {
+    err = cudaFuncSetAttribute(paged_chunk_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, CHUNK_SMEM);
+    if (err == cudaSuccess)
+      err = cudaFuncSetAttribute(paged_chunk_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, CHUNK_SMEM);
+  });
+  SNU1_CUDA_CHECK(err);
+  auto kernel = c.fp8 ? paged_chunk_kernel<true> : paged_chunk_kernel<false>;
+  SNU1_CUDA_CHECK(launch_pdl(kernel, dim3(c.heads * p.chunk_count), dim3(CHUNK_THREADS), CHUNK_SMEM, st, tm_q, tm_k, tm_v, p, a));
+  return kHostOk;
+}
+
+}  // namespace paged
+}  // namespace snu1

@@ -7,6 +7,7 @@
 // keys and values together).  Sequences own pages through a table in any order; pages of 16 to 128 tokens.
 #pragma once
 #include "attn_common.cuh"
+#include "host_common.h"
 
 namespace snu1 {
 namespace paged {
@@ -72,6 +73,12 @@ __device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* m, 
       "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(u)
       : "memory");
 }
+
+// paged_cache.cu: a plan's ``unpack`` pages of an e4m3 cache as bf16 pages of 128 tokens at ``wide``
+int launch_widen(const Cache& c, const Plan& p, void* wide, cudaStream_t st);
+// attn_paged_sm100.cu: a plan's ``chunk`` items
+int launch_chunks(const Cache& c, const Plan& p, const void* q, long long ldq, int q_rows, void* o, long long ldo, float* part,
+                  float2* part_ml, float scale_log2, void* wide, cudaStream_t st);
 
 }  // namespace paged
 }  // namespace snu1

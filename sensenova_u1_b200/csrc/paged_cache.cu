@@ -85,8 +85,8 @@ constexpr int READ_ROWS = 4;                                         // rows of 
 constexpr int READ_BLOCK = READ_THREADS / 16 * READ_ROWS;            // rows of a block
 
 // Rows of the planned pages, in order.  PACKED: out = keys, out2 = values [rows][heads][128] at the plan's row numbers;
-// otherwise out = pages of 128 tokens in a cache's own layout, every sequence from a page of its own on, rows behind its
-// last token cleared (the attention kernel multiplies them by probabilities of zero).
+// otherwise out = codes as bf16 (without their scales) in pages of 128 tokens in a cache's own layout, every sequence from a
+// page of its own on, rows behind its last token cleared (the attention kernel multiplies them by probabilities of zero).
 template <bool FP8, bool PACKED>
 __global__ void __launch_bounds__(READ_THREADS)
     paged_read_kernel(const uint8_t* __restrict__ data, const float* __restrict__ scales, int pages, int heads, int page, Plan p,
@@ -114,7 +114,7 @@ __global__ void __launch_bounds__(READ_THREADS)
         const uint2 u = *reinterpret_cast<const uint2*>(data + at * HEAD + c * 8);
         x[i].x = u.x;
         x[i].y = u.y;
-        s[i] = scales[at];
+        s[i] = PACKED ? scales[at] : 1.f;
       } else {
         x[i] = *reinterpret_cast<const uint4*>(data + at * (HEAD * 2) + c * 16);
       }
@@ -146,6 +146,14 @@ __global__ void __launch_bounds__(READ_THREADS)
     }
     *reinterpret_cast<uint4*>(dst + c * 8) = y;
   }
+}
+
+int launch_widen(const Cache& c, const Plan& p, void* wide, cudaStream_t st) {
+  const int total = 2 * c.heads * c.page;
+  SNU1_CUDA_CHECK(launch_pdl(paged_read_kernel<true, false>, dim3(p.unpack_count, (total + READ_BLOCK - 1) / READ_BLOCK),
+                             dim3(READ_THREADS), 0, st, (const uint8_t*)c.data, (const float*)c.scales, c.pages, c.heads, c.page, p,
+                             (__nv_bfloat16*)wide, (__nv_bfloat16*)nullptr, device_status_word()));
+  return kHostOk;
 }
 
 }  // namespace paged

@@ -38,6 +38,9 @@ KEY_TILE = 64            # keys of a stage of the kernel for few rows
 FEW_SLOTS = 296          # its CTAs that run at once: two on each of 148 SMs
 FEW_LEAST = 4            # a part of a sequence has at least this many key tiles
 FEW_TILE = 64            # rows (new tokens x query heads of a group) of one CTA, at most
+CHUNK_TILE = 128         # keys of a tile of the kernel for chunks, and rows of a row tile
+CHUNK_SLOTS = 148        # its CTAs that run at once
+CHUNK_START = 3          # what starting and ending a CTA costs, in key tiles
 
 
 class PagedCache:
@@ -61,7 +64,7 @@ class PagedCache:
             raise ValueError("a paged cache is in GPU memory")
         self._data, self._scales = data, scales
         self.pages, _, self.kv_heads, self.page, _ = data.shape
-        if self.kv_heads > 65535 or self.pages >= 1 << 31:
+        if self.kv_heads > 1023 or self.pages >= 1 << 31:
             raise ValueError("too many heads or pages")
         self._desc = ctypes.create_string_buffer(_lib.load().snu1_paged_cache_bytes())
         with torch.cuda.device(data.device):
@@ -101,6 +104,7 @@ class PagedPlan:
     kv_heads: int
     page: int
     pages: int
+    dtype: torch.dtype            # of the caches
     device: torch.device
     q_lens: list
     kv_lens: list
@@ -122,6 +126,8 @@ def _shares(tiles: np.ndarray, heads: int, slots: int, least: int) -> np.ndarray
     """Into how many parts the key tiles of every work item are split.  ``heads`` CTAs run per part and ``slots`` at once: parts
     are as short as they may be (``least`` tiles) while all of them run in one wave; where even whole items are more than
     that, only items longer than a fair share are split."""
+    if not len(tiles):
+        return tiles
     tiles = np.maximum(tiles, 1)
     share = max(least, 1)
     if len(tiles) * heads <= slots:
@@ -139,13 +145,13 @@ def _shares(tiles: np.ndarray, heads: int, slots: int, least: int) -> np.ndarray
     return -(-tiles // share)
 
 
-def _lay_out(q_lens, kv_lens, tables, page: int, pages: int, group: int, kv_heads: int, limits, grow: int):
+def _lay_out(q_lens, kv_lens, tables, page: int, pages: int, group: int, kv_heads: int, fp8: bool, limits, grow: int):
     """Host side of :func:`build_plan`: checks, and every array of the plan as int32."""
     q, kv = np.asarray(q_lens, dtype=np.int64).reshape(-1), np.asarray(kv_lens, dtype=np.int64).reshape(-1)
     n = len(q)
     if len(kv) != n or (q < 0).any() or (kv < q).any() or grow < 0:
         raise ValueError("every sequence has q_len >= 0 new tokens among its kv_len >= q_len tokens, and grow >= 0")
-    if n > 65535 or (n and (kv.max() + grow >= 1 << 30 or q.sum() * group >= 1 << 31 or kv.sum() >= 1 << 31)):
+    if n > 65535 or group > 65535 or (n and (kv.max() + grow >= 1 << 30 or q.sum() * group >= 1 << 31 or kv.sum() >= 1 << 31)):
         raise ValueError("too many sequences or tokens for one plan")
     cap = np.where(q > 0, kv + grow, kv)
     need = -(-cap // page)
@@ -178,26 +184,66 @@ def _lay_out(q_lens, kv_lens, tables, page: int, pages: int, group: int, kv_head
     pages_of = lambda c: np.stack([np.repeat(np.arange(n), c), np.arange(int(c.sum())) - np.repeat(np.cumsum(c) - c, c)], 1).astype(np.int32)
     # attention: tiles of rows, split over keys
     q_rows = q * group
-    top = int(q_rows.max()) if n else 0
+    chunked = (q_rows > FEW_TILE) & (group <= CHUNK_TILE)
+    few_q = np.where(chunked, 0, q_rows)
+    top = int(few_q.max()) if n else 0
     few_rows = 16 if top <= 16 else 32 if top <= 32 else FEW_TILE
-    count = -(-q_rows // few_rows)
-    seq = np.repeat(np.arange(n), count)
-    row0 = (np.arange(len(seq)) - np.repeat(np.cumsum(count) - count, count)) * few_rows
-    few, merge, partial = _items(seq, row0, -(-cap[seq] // KEY_TILE), few_rows, kv_heads, FEW_SLOTS, FEW_LEAST, 0)
+    chunk_rows = 2 * (CHUNK_TILE // group) * group if group <= CHUNK_TILE else 1        # two row tiles of whole tokens
+
+    def tiles_of(q_rows, m):
+        count = -(-q_rows // m)
+        seq = np.repeat(np.arange(n), count)
+        return seq, (np.arange(len(seq)) - np.repeat(np.cumsum(count) - count, count)) * m
+
+    seq, row0 = tiles_of(few_q, few_rows)
+    tiles = -(-cap[seq] // KEY_TILE)
+    few, merge, partial = _items(seq, row0, tiles, _shares(tiles, kv_heads, FEW_SLOTS, FEW_LEAST), few_rows, 0)
+    seq, row0 = tiles_of(np.where(chunked, q_rows, 0), chunk_rows)
+    if limits is None:                                        # a row tile reads up to its last token
+        last = np.minimum((row0 + chunk_rows - 1) // group, q[seq] - 1)
+        tiles = -(-(cap[seq] - q[seq] + 1 + last) // CHUNK_TILE)
+    else:
+        tiles = -(-kv[seq] // CHUNK_TILE)
+    chunk, more, partial = _items(seq, row0, tiles, _waves(tiles, kv_heads, CHUNK_SLOTS), chunk_rows, partial)
+    unpack = unpack_first = None
+    unpack_pages = 0
+    if fp8 and len(chunk):
+        wide = np.where(chunked, -(-cap // CHUNK_TILE), 0)    # 128-token pages
+        unpack, unpack_first, unpack_pages = pages_of(wide * (CHUNK_TILE // page)), start(wide)[:n], int(wide.sum())
+    merge = np.concatenate([merge, more])
     arrays = dict(q_start=start(q), kv_len=kv.astype(np.int32), cap=cap.astype(np.int32), table=table, behind=behind, row_seq=row_seq,
-                  k_start=start(kv), read_pages=pages_of(read), unpack=None, unpack_first=None, few=few, chunk=None, merge=merge)
+                  k_start=start(kv), read_pages=pages_of(read), unpack=unpack, unpack_first=unpack_first, few=few, chunk=chunk,
+                  merge=merge)
     counts = dict(seqs=n, rows=rows, width=width, page=page, group=group, read_count=int(read.sum()), few_count=len(few),
-                  few_rows=few_rows, chunk_count=0, merge_count=len(merge), merge_rows=few_rows, partial_rows=partial, unpack_pages=0,
-                  unpack_count=0)
+                  few_rows=few_rows, chunk_count=len(chunk), merge_count=len(merge), merge_rows=chunk_rows if len(more) else few_rows,
+                  partial_rows=partial, unpack_pages=unpack_pages, unpack_count=0 if unpack is None else len(unpack))
     return arrays, counts
 
 
-def _items(seq, row0, tiles, m: int, heads: int, slots: int, least: int, first: int):
+def _waves(tiles: np.ndarray, heads: int, slots: int) -> np.ndarray:
+    """Parts of the chunk kernel's items: of the shares that cut the longest item into up to 16 parts, the one whose waves of
+    CTAs (longest first, a wave as long as its longest CTA) are shortest together.  Every CTA pays ``CHUNK_START``."""
+    if not len(tiles):
+        return tiles
+    tiles = np.maximum(tiles, 1)
+    best = None
+    for cut in range(1, 17):
+        share = -(-int(tiles.max()) // cut)
+        parts = -(-tiles // share)
+        sizes = np.repeat(-(-tiles // parts), parts * heads)
+        cost = float((np.sort(sizes)[::-1][::slots] + CHUNK_START).sum()) + (CHUNK_START if cut > 1 else 0)
+        if best is None or cost < 0.98 * best[0]:
+            best = (cost, parts)
+        if share <= 2:
+            break
+    return best[1]
+
+
+def _items(seq, row0, tiles, parts, m: int, first: int):
     """Work items [sequence, first row, part | parts << 16, partial row or -1], those with most keys first, the joins of the
     items that were split, and the rows of partial results up to there."""
     if not len(seq):
         return np.zeros((0, 4), np.int32), np.zeros((0, 4), np.int32), first
-    parts = _shares(tiles, heads, slots, least)
     split = parts > 1
     at = first + np.cumsum(np.where(split, parts * m, 0)) - np.where(split, parts * m, 0)
     merge = np.stack([seq, row0, parts | m << 16, at], 1)[split]
@@ -218,7 +264,8 @@ def build_plan(cache: PagedCache, heads: int, q_lens, kv_lens, tables, limits=No
     sees the whole picture, has the picture's end as its limit.  ``grow``: tokens that :meth:`PagedPlan.advance` may add."""
     if heads < 1 or heads % cache.kv_heads != 0:
         raise ValueError("the number of query heads must be a multiple of the cache's heads")
-    arrays, counts = _lay_out(q_lens, kv_lens, tables, cache.page, cache.pages, heads // cache.kv_heads, cache.kv_heads, limits, grow)
+    arrays, counts = _lay_out(q_lens, kv_lens, tables, cache.page, cache.pages, heads // cache.kv_heads, cache.kv_heads,
+                              cache.scales is not None, limits, grow)
     # all arrays in one copy from pinned memory that nothing waits for
     at, total = {}, 0
     for name, a in arrays.items():
@@ -232,13 +279,15 @@ def build_plan(cache: PagedCache, heads: int, q_lens, kv_lens, tables, limits=No
     store = host.to(cache.device, non_blocking=True)
     args = _Args(**{name: store.data_ptr() + 4 * o for name, o in at.items()}, **counts)
     n = counts["seqs"]
-    scratch = counts["partial_rows"] * cache.kv_heads * (HEAD_DIM + 2) * 4
-    return PagedPlan(heads, cache.kv_heads, cache.page, cache.pages, cache.device, [int(x) for x in q_lens], [int(x) for x in kv_lens],
+    joined = counts["partial_rows"] * cache.kv_heads
+    scratch = joined * HEAD_DIM * 4 + (joined + 15) // 16 * 128 + counts["unpack_pages"] * 2 * cache.kv_heads * CHUNK_TILE * HEAD_DIM * 2
+    return PagedPlan(heads, cache.kv_heads, cache.page, cache.pages, cache.data.dtype, cache.device,
+                     [int(x) for x in q_lens], [int(x) for x in kv_lens],
                      counts["rows"], int(arrays["k_start"][-1]), scratch, store[at["kv_len"]:at["kv_len"] + n], grow, store, args)
 
 
 def _check(cache: PagedCache, plan: PagedPlan) -> None:
-    if cache.page != plan.page or cache.kv_heads != plan.kv_heads or cache.pages < plan.pages or cache.device != plan.device:
+    if cache.data.dtype != plan.dtype or cache.page != plan.page or cache.kv_heads != plan.kv_heads or cache.pages < plan.pages or cache.device != plan.device:
         raise ValueError("the plan was made for caches of another geometry or device")
 
 

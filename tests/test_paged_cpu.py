@@ -7,7 +7,7 @@ from sensenova_u1_b200.ops import paged
 
 
 def lay(q=(1, 3), kv=(5, 40), tables=((0,), (1, 2, 3)), page=16, pages=4, group=4, heads=2, limits=None, grow=0):
-    return paged._lay_out(list(q), list(kv), [list(t) for t in tables], page, pages, group, heads, limits, grow)
+    return paged._lay_out(list(q), list(kv), [list(t) for t in tables], page, pages, group, heads, False, limits, grow)
 
 
 def test_arrays():
@@ -48,13 +48,13 @@ def test_page_tables_as_a_tensor():
     a, _ = lay(tables=torch.tensor([[0, 77, 99], [1, 2, 3]]))          # what a table holds beyond its pages is ignored
     assert a["table"].tolist() == [[0, 0, 0], [1, 2, 3]]
     with pytest.raises(ValueError):
-        paged._lay_out([1], [1], torch.zeros(1, dtype=torch.int32), 16, 4, 1, 1, None, 0)
+        paged._lay_out([1], [1], torch.zeros(1, dtype=torch.int32), 16, 4, 1, 1, False, None, 0)
 
 
 def test_sequences_without_rows_or_keys():
     a, c = lay(q=(0, 0, 0), kv=(0, 7, 0), tables=((), (2,), ()))
     assert c["rows"] == 0 and c["few_count"] == 0 and c["merge_count"] == 0 and c["read_count"] == 1
-    a, c = paged._lay_out([], [], [], 16, 4, 1, 1, None, 0)
+    a, c = paged._lay_out([], [], [], 16, 4, 1, 1, False, None, 0)
     assert c["seqs"] == 0 and c["rows"] == 0
 
 
@@ -65,9 +65,11 @@ def test_every_row_meets_every_key_once(q, kv, group, heads):
     page, n = 16, len(q)
     need = [-(-k // page) for k in kv]
     tables = [list(range(sum(need[:i]), sum(need[:i + 1]))) for i in range(n)]
-    a, c = paged._lay_out(q, kv, tables, page, sum(need), group, heads, None, 0)
+    a, c = paged._lay_out(q, kv, tables, page, sum(need), group, heads, True, None, 0)
     parts, written = {}, set()
-    for name, m in (("few", c["few_rows"]),):
+    for name, m in (("few", c["few_rows"]), ("chunk", 2 * (128 // group) * group)):
+        if a[name] is None:
+            continue
         for b, row0, z, at in a[name].tolist():
             part, count = z & 0xffff, z >> 16
             parts.setdefault((b, row0, m, count), []).append(part)
@@ -85,10 +87,15 @@ def test_every_row_meets_every_key_once(q, kv, group, heads):
     assert len(seen) == sum(q) * group
     joined = {(b, row0): (z & 0xffff, z >> 16, at) for b, row0, z, at in a["merge"].tolist()}
     assert set(joined) == {(b, r0) for (b, r0, m, count) in parts if count > 1}
-    for b, row0, z, at in a["few"].tolist():
+    for b, row0, z, at in a["few"].tolist() + a["chunk"].tolist():
         if at >= 0:
             count, m, first = joined[(b, row0)]
             assert count == z >> 16 and at == first + (z & 0xffff) * m
+            assert m <= c["merge_rows"]
+    if c["unpack_count"]:                                             # every key of a chunk's sequence has its place
+        wide = [-(-k // 128) if any(b == i for b, *_ in a["chunk"].tolist()) else 0 for i, k in enumerate(kv)]
+        assert c["unpack_pages"] == sum(wide) and a["unpack_first"].tolist() == [sum(wide[:i]) for i in range(n)]
+        assert a["unpack"].tolist() == [[i, y] for i in range(n) for y in range(wide[i] * (128 // page))]
 
 
 def test_parts_fill_one_wave():
