@@ -9,16 +9,22 @@
 // weighted values, fp32) are joined by a second kernel in a fixed order, without atomics.
 //
 // One warp asks for whole pages through TMA (keys and values of one head in one box), several stages ahead; four warps
-// compute with mma.sync m16n8k16: at 16 rows and up to 8 bytes of cache per clock and warp the legacy tensor path is far from
-// its limit, and its fragments let e4m3 codes be widened to bf16 in registers (exactly, see e4m3x2_to_bf16x2): the scale
-// of a key goes into its score, that of a value into its probability, both in fp32.  Up to 16 rows every warp takes other
-// keys, up to 32 rows two warps share them, up to 64 rows all four do.
+// compute with mma.sync m16n8k16, keys (then the width of a head) on the 16-side and rows on the 8-side: S^T = K q^T,
+// o^T = V^T p^T.  So a step of a group of 4 or 8 heads fills the product, and what a warp has read and widened of the cache
+// serves all rows.  At 1 - 2 products per KB of cache the legacy tensor path is far from its limit.
 //
-// Masked places: scores of keys at or beyond a row's limit are -inf whatever the cache holds.  A probability of zero does
-// not hide an infinite or NaN value from the matrix product, so in a tile that some row may not read whole, bf16 values
-// that are not finite are cleared in shared memory and the first key that held one is kept: rows that may read it give
-// NaN, the others are as if it were not there.  (e4m3 codes are finite; what is not finite there is the row's scale, and that
-// is only used where the mask allows.)
+// e4m3 codes are widened to fp16, which is exact, two per instruction.  For that the queries go to fp16 as well, each row
+// times the power of two that brings its largest value to [2^13, 2^14): values down to 2^-27 of the largest keep all their
+// bits, and what smaller ones lose is below the rounding of the fp32 sum.  The scale of a key goes into its score.  The
+// scale of a value goes into its probability, in the exponent: p' = exp2(s + log2(scale) - m') with a maximum of its own,
+// so that the fp16 probabilities of the product are relative to the largest p' whatever sizes the values have (2^-11 each;
+// bf16 caches: bf16 probabilities, 2^-8).  The sum of the probabilities is taken in fp32 from p itself.
+//
+// Masked places: scores of keys at or beyond a row's limit are -inf whatever the cache holds, and places that no row of the
+// tile may read are cleared in shared memory.  A probability of zero does not hide an infinite or NaN value from the
+// matrix product, so in a tile that some row may not read whole, bf16 values that are not finite are cleared too and the
+// first key that held one is kept: rows that may read it give NaN, the others are as if it were not there.  (e4m3 codes are
+// finite; what is not finite there is the row's scale, and that is only used where the mask allows.)
 #include <string.h>
 
 #include <mutex>
@@ -29,18 +35,18 @@
 namespace snu1 {
 namespace paged {
 
-constexpr int KT = 64;                       // keys of a stage
-constexpr int FEW_THREADS = 160;             // four warps that compute, one that asks for pages
+constexpr int FEW_WARPS = 4;                              // warps that compute; one more asks for pages
+constexpr int FEW_THREADS = FEW_WARPS * 32 + 32;
 
 template <bool FP8>
 struct Few {
-  static constexpr int HALVES = FP8 ? 1 : 2;                    // boxes of 128 bytes per row
-  static constexpr int DATA = KT * 2 * 128 * HALVES;            // keys and values of a stage
-  static constexpr int STAGE = DATA + (FP8 ? KT * 2 * 4 : 0);
-  static constexpr int STAGES = FP8 ? 5 : 3;
-  static constexpr int DATA_ALL = STAGES * DATA;
-  static constexpr int SCALES_ALL = STAGES * (STAGE - DATA);
-  static constexpr int SMEM = DATA_ALL + SCALES_ALL + 1024;
+  static constexpr int KT = FP8 ? 128 : 64;               // keys of a stage
+  static constexpr int HALVES = FP8 ? 1 : 2;              // boxes of 128 bytes per row
+  static constexpr int DATA = KT * 2 * 128 * HALVES;      // keys and values of a stage
+  static constexpr int SCALES = FP8 ? KT * 2 * 4 : 0;
+  static constexpr int STAGES = 3;
+  static constexpr int RING = STAGES * (DATA + SCALES);
+  static constexpr int SMEM = RING + 1024;
 };
 
 __device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
@@ -55,10 +61,43 @@ __device__ __forceinline__ void ldsm_x4_t(uint32_t addr, uint32_t (&r)[4]) {
                : "r"(addr)
                : "memory");
 }
-__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+// transposes an 8x8 matrix of 16-bit elements held as a fragment
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+template <bool HALF>
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (HALF)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// the two codes in the low or the high half of ``w`` as fp16
+__device__ __forceinline__ uint32_t widen_lo(uint32_t w) {
+  uint32_t r;
+  asm("{\n.reg .b16 l, h;\nmov.b32 {l, h}, %1;\ncvt.rn.f16x2.e4m3x2 %0, l;\n}" : "=r"(r) : "r"(w));
+  return r;
+}
+__device__ __forceinline__ uint32_t widen_hi(uint32_t w) {
+  uint32_t r;
+  asm("{\n.reg .b16 l, h;\nmov.b32 {l, h}, %1;\ncvt.rn.f16x2.e4m3x2 %0, h;\n}" : "=r"(r) : "r"(w));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ float fast_log2(float x) {
+  float y;
+  asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
 struct FewArgs {
@@ -72,25 +111,26 @@ struct FewArgs {
   int* status;
 };
 
-// WR: warps along the rows (16 each); the others take other keys.
-template <bool FP8, int WR>
-__global__ void __launch_bounds__(FEW_THREADS)
+// NR: groups of eight rows that a warp computes.  WR: sets of warps with other rows; the warps of a set take other keys.
+template <bool FP8, int NR, int WR>
+__global__ void __launch_bounds__(FEW_THREADS, NR == 1 ? 3 : 2)
     paged_few_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_constant__ CUtensorMap tm_scale, const Plan p,
                      const FewArgs a) {
   using F = Few<FP8>;
-  constexpr int WK = 4 / WR, M = 16 * WR, NB = KT / 16 / WK;     // warps along the keys, rows, blocks of 16 keys per warp
+  constexpr int KT = F::KT, WK = FEW_WARPS / WR, M = 8 * NR * WR, NB = KT / 16 / WK;     // NB: blocks of 16 keys of a warp
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  float* s_scales = reinterpret_cast<float*>(smem + F::DATA_ALL);   // [stage][page box][keys, values][box rows]
+  float* s_scales = reinterpret_cast<float*>(smem + F::STAGES * F::DATA);   // [stage][page box][keys, values][box rows]
   __shared__ uint64_t full[F::STAGES], empty[F::STAGES];
   __shared__ int abort_word, s_poison;
-  __shared__ float s_m[4][16], s_l[4][16];
+  __shared__ float s_m[FEW_WARPS][8 * NR], s_l[FEW_WARPS][8 * NR];
+  __shared__ float s_rs[M];                                      // a row's score scale, log2 units
   volatile int* abort_flag = &abort_word;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < F::STAGES; ++i) {
       mbar_init(&full[i], 1);
-      mbar_init(&empty[i], 4);
+      mbar_init(&empty[i], FEW_WARPS);
     }
     abort_word = 0;
     s_poison = 0x7fffffff;
@@ -120,96 +160,135 @@ __global__ void __launch_bounds__(FEW_THREADS)
   }
   const int tiles = (max_lim + KT - 1) / KT;
   const int j0 = (int)((long long)tiles * part / parts), j1 = (int)((long long)tiles * (part + 1) / parts);
-  const int bx = min(p.page, KT), boxes = KT / bx;               // rows of a box, boxes of a stage
-  const int box_bytes = 2 * bx * 128;
+  const int page_log = __ffs(p.page) - 1;
+  const int bx_log = min(page_log, KT == 128 ? 7 : 6), bx = 1 << bx_log;      // rows of a box
+  const int box_bytes = 2 * 128 << bx_log;
 
-  if (warp == 4) {
-    if (lane == 0) {
-      bool gave_up = false;
-      const int* table = p.table + (long long)b * p.width;
-      const int pages_used = (max_lim + p.page - 1) / p.page;
-      for (int j = j0; j < j1; ++j) {
-        const int n = j - j0, s = n % F::STAGES;
-        if (!mbar_wait(&empty[s], ((n / F::STAGES) & 1) ^ 1, abort_flag, a.status, 10)) {
-          gave_up = true;
-          break;
-        }
-        const int k0 = j * KT;
-        int live = 0;
-        for (int i = 0; i < boxes; ++i) live += (k0 + i * bx) / p.page < pages_used;
-        mbar_expect_tx(&full[s], live * (box_bytes * F::HALVES + (FP8 ? bx * 8 : 0)));
-        for (int i = 0; i < live; ++i) {
-          const int k = k0 + i * bx;
-          const int pg = table[k / p.page];
-          if (pg < 0 || pg >= a.pages) report_status(a.status, kBadPage, 10);     // reads as zeros
+  if (warp == FEW_WARPS) {
+    // a lane per box of the stage; its page is read a stage ahead
+    const int boxes = KT >> bx_log;
+    const int* table = p.table + (long long)b * p.width;
+    auto page_of = [&](int j) -> int {
+      const int k = j * KT + (lane << bx_log);
+      return j < j1 && lane < boxes && k < max_lim ? table[k >> page_log] : 0;
+    };
+    int next = page_of(j0);
+    bool ok = true;
+    for (int j = j0; j < j1; ++j) {
+      const int n = j - j0, s = n % F::STAGES;
+      const int pg = next;
+      next = page_of(j + 1);
+      ok = mbar_wait_warp(&empty[s], ((n / F::STAGES) & 1) ^ 1, abort_flag, a.status, 10);
+      if (!ok) break;
+      const int live = min(boxes, (max_lim - j * KT + bx - 1) >> bx_log);
+      if (lane == 0) mbar_expect_tx(&full[s], live * (box_bytes * F::HALVES + (FP8 ? bx * 8 : 0)));
+      __syncwarp();
+      if (lane < live) {
+        if (pg < 0 || pg >= a.pages) report_status(a.status, kBadPage, 10);     // reads as zeros
+        const int y = (j * KT + (lane << bx_log)) & (p.page - 1);
 #pragma unroll
-          for (int h = 0; h < F::HALVES; ++h)
-            tma_load_5d(smem_u32(smem + s * F::DATA + (i * F::HALVES + h) * box_bytes), &tm_kv, &full[s], h * 64, k % p.page, head,
-                        0, pg);
-          if (FP8)
-            tma_load_4d(s_scales + (s * KT + i * bx) * 2, &tm_scale, &full[s], k % p.page, head, 0, pg);
-        }
+        for (int h = 0; h < F::HALVES; ++h)
+          tma_load_5d(smem_u32(smem + s * F::DATA + (lane * F::HALVES + h) * box_bytes), &tm_kv, &full[s], h * 64, y, head, 0, pg);
+        if (FP8) tma_load_4d(s_scales + (s * KT + (lane << bx_log)) * 2, &tm_scale, &full[s], y, head, 0, pg);
       }
-      if (gave_up) {                       // copies may be on their way into this CTA's memory
-        const uint64_t t0 = globaltimer_ns();
-        while (globaltimer_ns() - t0 < 2000000ull) {
-        }
+      __syncwarp();
+    }
+    if (!ok) {                             // copies may be on their way into this CTA's memory
+      const uint64_t t0 = globaltimer_ns();
+      while (globaltimer_ns() - t0 < 2000000ull) {
       }
     }
   } else {
     const int wr = warp / WK, wk = warp % WK;
     const int g = lane >> 2, c = lane & 3;
-    // query fragments of rows g and g + 8 of this warp
-    uint32_t qf[8][4];
-    int lim[2];
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int row = wr * 16 + g + r * 8;
+    // Query fragments of eight rows: values 2 c + {0, 1} and 2 c + 8 + {0, 1} of every 16, or for e4m3 4 c + {0 .. 3}: there a
+    // thread's four codes of 16 stand side by side.  Rows behind the last are zeros.
+    auto load_q = [&](int rg, uint32_t (&f)[8][2]) {
+      const int row = rg * 8 + g;
       const bool on = row < rows;
-      const int t = (row0 + row) / G;
-      lim[r] = on ? row_limit(p, q0, q_len, kv_len, t) : 0;
-      const __nv_bfloat16* qp = a.q + (long long)(q0 + t) * a.ldq + (long long)(head * G + (row0 + row) % G) * HEAD;
+      const __nv_bfloat16* qp = a.q + (long long)(q0 + (row0 + row) / G) * a.ldq + (long long)(head * G + (row0 + row) % G) * HEAD;
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        // e4m3: a thread's four codes of a 16-value piece stand side by side, and so do its query values
-        uint32_t lo = 0, hi = 0;
+        f[k][0] = f[k][1] = 0u;
         if (on) {
           if (FP8) {
             const uint2 u = *reinterpret_cast<const uint2*>(qp + k * 16 + c * 4);
-            lo = u.x;
-            hi = u.y;
+            f[k][0] = u.x;
+            f[k][1] = u.y;
           } else {
-            lo = *reinterpret_cast<const uint32_t*>(qp + k * 16 + c * 2);
-            hi = *reinterpret_cast<const uint32_t*>(qp + k * 16 + c * 2 + 8);
+            f[k][0] = *reinterpret_cast<const uint32_t*>(qp + k * 16 + c * 2);
+            f[k][1] = *reinterpret_cast<const uint32_t*>(qp + k * 16 + c * 2 + 8);
           }
         }
-        qf[k][r] = lo;
-        qf[k][2 + r] = hi;
       }
-    }
-    float acc[16][4];
+      float rs = a.scale_log2;
+      if (FP8) {
+        uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
+        for (int k = 0; k < 8; ++k)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[i][e] = 0.f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+          for (int i = 0; i < 2; ++i) top = max(top, max((f[k][i] << 16) & 0x7fffffffu, f[k][i] & 0x7fff0000u));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int e = (int)(top >> 23) - 127;                    // of the largest value; zero and what is not finite: as it is
+        const int up = top == 0 || e == 128 ? 0 : min(13 - e, 120);
+        const float f2 = __int_as_float((127 + up) << 23);
+        rs *= __int_as_float((127 - up) << 23);
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            f[k][i] = pack_f16x2(__uint_as_float(f[k][i] << 16) * f2, __uint_as_float(f[k][i] & 0xffff0000u) * f2);
+      }
+      if (c == 0) s_rs[row] = rs;
+    };
+    uint32_t qf[NR][8][2];
+#pragma unroll
+    for (int i = 0; i < NR; ++i) load_q(wr * NR + i, qf[i]);
+    named_bar_sync(1, FEW_WARPS * 32);
+    // this thread's rows of a group of eight: 2 c and 2 c + 1
+    float rs[NR][2];
+    int lim[NR][2];
+#pragma unroll
+    for (int i = 0; i < NR; ++i)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int row = (wr * NR + i) * 8 + 2 * c + e;
+        rs[i][e] = s_rs[row];
+        lim[i][e] = row < rows ? row_limit(p, q0, q_len, kv_len, (row0 + row) / G) : 0;
+      }
+    float acc[NR][8][4];                   // o^T: 16 values x 8 rows
+#pragma unroll
+    for (int i = 0; i < NR; ++i)
+#pragma unroll
+      for (int d = 0; d < 8; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][d][e] = 0.f;
+    // running maxima of the scores (for the sums l) and of scores + log2 of the values' scales (for acc); bf16: the same
+    float m[NR][2], mv[NR][2], l[NR][2];
+#pragma unroll
+    for (int i = 0; i < NR; ++i)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        m[i][e] = mv[i][e] = -INFINITY;
+        l[i][e] = 0.f;
+      }
     bool ok = true;
+    const int krow = (lane & 7) + ((lane >> 3) & 1) * 8, vrow = (lane & 7) + (lane >> 4) * 8;
     for (int j = j0; j < j1; ++j) {
       const int n = j - j0, s = n % F::STAGES, k0 = j * KT;
       ok &= mbar_wait(&full[s], (n / F::STAGES) & 1, abort_flag, a.status, 10);
       const uint32_t data = smem_u32(smem + s * F::DATA);
-      const float* sc = s_scales + s * KT * 2;
       const bool partial = k0 + KT > min_lim;
-      if (!FP8 && partial) {
-        // values that are not finite, and rows that no box has filled
-        for (int i = threadIdx.x; i < KT * 16; i += 128) {
-          const int key = i >> 4, ch = i & 15;
-          const int box = key / bx, row = key % bx;
-          uint4* at = reinterpret_cast<uint4*>(smem + s * F::DATA + (box * 2 + (ch >> 3)) * box_bytes + bx * 128 +
-                                               swz128_offset(row, ch & 7));
-          if (k0 + key >= kv_len) {
+      if (partial && (!FP8 || k0 + KT > max_lim)) {
+        // values that no row may read, and bf16 values that are not finite
+        for (int i = threadIdx.x; i < KT * 8 * F::HALVES; i += FEW_WARPS * 32) {
+          const int key = FP8 ? i >> 3 : i >> 4, ch = FP8 ? i & 7 : i & 15;
+          uint4* at = reinterpret_cast<uint4*>(smem + s * F::DATA + ((key >> bx_log) * F::HALVES + (ch >> 3)) * box_bytes + (bx << 7) +
+                                               swz128_offset(key & (bx - 1), ch & 7));
+          if (k0 + key >= max_lim) {
             *at = make_uint4(0, 0, 0, 0);
-          } else {
+          } else if (!FP8) {
             uint4 x = *at;
             uint32_t* w = reinterpret_cast<uint32_t*>(&x);
             bool bad = false;
@@ -226,130 +305,158 @@ __global__ void __launch_bounds__(FEW_THREADS)
           }
         }
         fence_proxy_async_smem();          // TMA writes here again
-        named_bar_sync(1, 128);
+        named_bar_sync(1, FEW_WARPS * 32);
       }
-      float sv[NB][2][4];
+      float sv[NR][NB][4];                 // S^T: keys g, g + 8 x rows 2 c, 2 c + 1
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        const int key0 = (wk * NB + nb) * 16, box = key0 / bx, brow = key0 % bx;
-        const uint32_t kb = data + box * F::HALVES * box_bytes + brow * 128;
+      for (int i = 0; i < NR; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sv[nb][0][e] = sv[nb][1][e] = 0.f;
-        if (FP8) {
-          // matrices: keys 0-7 and 8-15 of a 16-byte piece, then of the next piece
-          const int row = (lane & 7) + ((lane >> 3) & 1) * 8, pc = lane >> 4;
+        for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-          for (int k = 0; k < 8; k += 2) {
+          for (int e = 0; e < 4; ++e) sv[i][nb][e] = 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; k += 2) {     // 32 values at a time
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          const int key0 = (wk * NB + nb) * 16;
+          const uint32_t kb = data + (key0 >> bx_log) * F::HALVES * box_bytes + ((key0 & (bx - 1)) << 7);
+          if (FP8) {
+            // matrices: keys 0-7 and 8-15 of a 16-value piece, then of the next piece
             uint32_t r[4];
-            ldsm_x4(kb + swz128_offset(row, k + pc), r);
+            ldsm_x4(kb + swz128_offset(krow, k + (lane >> 4)), r);
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t w0 = r[2 * h], w1 = r[2 * h + 1];
+              const uint32_t f[4] = {widen_lo(w0), widen_lo(w1), widen_hi(w0), widen_hi(w1)};
 #pragma unroll
-              for (int t = 0; t < 2; ++t) {
-                const uint32_t w = r[i * 2 + t];
-                mma_bf16(sv[nb][t], qf[k + i], e4m3x2_to_bf16x2(__byte_perm(w, 0, 0x1404)), e4m3x2_to_bf16x2(__byte_perm(w, 0, 0x3424)));
-              }
-          }
-        } else {
-          // matrices: two pieces of keys 0-7, two of keys 8-15
-          const int row = (lane & 7) + (lane >> 4) * 8, pc = (lane >> 3) & 1;
+              for (int i = 0; i < NR; ++i) mma_16816<true>(sv[i][nb], f, qf[i][k + h][0], qf[i][k + h][1]);
+            }
+          } else {
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            uint32_t r[4];
-            ldsm_x4(kb + (k >> 2) * box_bytes + swz128_offset(row, (k & 3) * 2 + pc), r);
-            mma_bf16(sv[nb][0], qf[k], r[0], r[1]);
-            mma_bf16(sv[nb][1], qf[k], r[2], r[3]);
+            for (int h = 0; h < 2; ++h) {
+              uint32_t r[4];
+              ldsm_x4(kb + (k >> 2) * box_bytes + swz128_offset(krow, ((k + h) & 3) * 2 + (lane >> 4)), r);
+#pragma unroll
+              for (int i = 0; i < NR; ++i) mma_16816<false>(sv[i][nb], r, qf[i][k + h][0], qf[i][k + h][1]);
+            }
           }
         }
       }
-      // scores in log2 units, masked; the largest of a row
-      float mx[2] = {-INFINITY, -INFINITY};
+      // scores in log2 units, masked; largest of this thread's keys
+      float lv[NB][2];                     // log2 of the values' scales
+      float mx[NR][2], mxv[NR][2];
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb)
+      for (int i = 0; i < NR; ++i)
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const int key = (wk * NB + nb) * 16 + t * 8 + c * 2;
-          float f[2] = {a.scale_log2, a.scale_log2};
-          if (FP8) {
-            const float2 u = *reinterpret_cast<const float2*>(sc + (key / bx) * 2 * bx + key % bx);
-            f[0] *= u.x;
-            f[1] *= u.y;
-          }
+        for (int e = 0; e < 2; ++e) mx[i][e] = mxv[i][e] = -INFINITY;
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        const int key = (wk * NB + nb) * 16 + g;
+        float ks[2] = {1.f, 1.f};
+        lv[nb][0] = lv[nb][1] = 0.f;
+        if (FP8) {
+          const int key0 = (wk * NB + nb) * 16;
+          const float* sc = s_scales + s * KT * 2 + ((key0 >> bx_log) << (bx_log + 1)) + (key0 & (bx - 1)) + g;
+          ks[0] = sc[0];
+          ks[1] = sc[8];
+          lv[nb][0] = fast_log2(sc[bx]);
+          lv[nb][1] = fast_log2(sc[bx + 8]);
+        }
+#pragma unroll
+        for (int i = 0; i < NR; ++i)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            float x = sv[nb][t][e] * f[e & 1];
-            if (partial && k0 + key + (e & 1) >= lim[e >> 1]) x = -INFINITY;
-            sv[nb][t][e] = x;
-            mx[e >> 1] = fmaxf(mx[e >> 1], x);
+            float x = sv[i][nb][e] * (FP8 ? rs[i][e & 1] * ks[e >> 1] : rs[i][e & 1]);
+            if (partial && k0 + key + (e >> 1) * 8 >= lim[i][e & 1]) x = -INFINITY;
+            sv[i][nb][e] = x;
+            mx[i][e & 1] = fmaxf(mx[i][e & 1], x);
+            if (FP8) mxv[i][e & 1] = fmaxf(mxv[i][e & 1], x + lv[nb][e >> 1]);
           }
+      }
+      // A running maximum moves only when it is outgrown by more than 2^8 (see attn_infer_sm100.cu), so most tiles need no
+      // reduction over the lanes.
+      bool move = false;
+#pragma unroll
+      for (int i = 0; i < NR; ++i)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) move |= mx[i][e] > m[i][e] + 8.f || (FP8 && mxv[i][e] > mv[i][e] + 8.f);
+      if (__any_sync(0xffffffffu, move)) {
+#pragma unroll
+        for (int i = 0; i < NR; ++i)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) {
+              mx[i][e] = fmaxf(mx[i][e], __shfl_xor_sync(0xffffffffu, mx[i][e], o));
+              if (FP8) mxv[i][e] = fmaxf(mxv[i][e], __shfl_xor_sync(0xffffffffu, mxv[i][e], o));
+            }
+            const float mn = fmaxf(m[i][e], mx[i][e]);
+            const float f = m[i][e] == -INFINITY ? 0.f : fast_exp2(m[i][e] - mn);
+            m[i][e] = mn;
+            l[i][e] *= f;
+            float fv = f;
+            if (FP8) {
+              const float nv = fmaxf(mv[i][e], mxv[i][e]);
+              fv = mv[i][e] == -INFINITY ? 0.f : fast_exp2(mv[i][e] - nv);
+              mv[i][e] = nv;
+            }
+#pragma unroll
+            for (int d = 0; d < 8; ++d) {
+              acc[i][d][e] *= fv;
+              acc[i][d][2 + e] *= fv;
+            }
+          }
+      }
+      uint32_t pf[NR][NB][2];              // p^T: rows g x keys 2 c + {0, 1}, then + 8
+#pragma unroll
+      for (int i = 0; i < NR; ++i) {
+        float mu[2], muv[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          mu[e] = m[i][e] == -INFINITY ? 0.f : m[i][e];
+          muv[e] = FP8 && mv[i][e] != -INFINITY ? mv[i][e] : 0.f;
         }
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
-        mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
-      }
-      // the running maximum moves only when it is outgrown by more than 2^8, see attn_infer_sm100.cu
-      if (__any_sync(0xffffffffu, mx[0] > m[0] + 8.f || mx[1] > m[1] + 8.f)) {
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const float mn = fmaxf(m[r], mx[r]);
-          const float f = m[r] == -INFINITY ? 0.f : fast_exp2(m[r] - mn);
-          m[r] = mn;
-          l[r] *= f;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            acc[i][2 * r] *= f;
-            acc[i][2 * r + 1] *= f;
-          }
-        }
-      }
-      const float mu[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        uint32_t pf[4];
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
+        for (int nb = 0; nb < NB; ++nb) {
           float x[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            x[e] = fast_exp2(sv[nb][t][e] - mu[e >> 1]);
-            l[e >> 1] += x[e];
+            x[e] = fast_exp2(sv[i][nb][e] - mu[e & 1]);
+            l[i][e & 1] += x[e];
+            // (the logarithm of a masked key's scale may be anything)
+            if (FP8) x[e] = partial && sv[i][nb][e] == -INFINITY ? 0.f : fast_exp2(sv[i][nb][e] + lv[nb][e >> 1] - muv[e & 1]);
           }
-          if (FP8) {
-            const int key = (wk * NB + nb) * 16 + t * 8 + c * 2;
-            const float2 u = *reinterpret_cast<const float2*>(sc + (key / bx) * 2 * bx + bx + key % bx);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              x[e] *= (e & 1) ? u.y : u.x;
-              if (partial && k0 + key + (e & 1) >= lim[e >> 1]) x[e] = 0.f;
-            }
-          }
-          pf[t * 2] = pack_bf16x2(x[0], x[1]);
-          pf[t * 2 + 1] = pack_bf16x2(x[2], x[3]);
+          for (int h = 0; h < 2; ++h)
+            pf[i][nb][h] = transpose_8x8(FP8 ? pack_f16x2(x[2 * h], x[2 * h + 1]) : pack_bf16x2(x[2 * h], x[2 * h + 1]));
         }
-        const int key0 = (wk * NB + nb) * 16, box = key0 / bx, brow = key0 % bx;
-        const uint32_t vb = data + box * F::HALVES * box_bytes + bx * 128 + brow * 128;
-        const int row = (lane & 7) + ((lane >> 3) & 1) * 8, pc = lane >> 4;   // keys 0-7, 8-15 of a piece, then of the next
+      }
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        const int key0 = (wk * NB + nb) * 16;
+        const uint32_t vb = data + (key0 >> bx_log) * F::HALVES * box_bytes + ((bx + (key0 & (bx - 1))) << 7);
         if (FP8) {
 #pragma unroll
-          for (int k = 0; k < 8; k += 2) {
+          for (int d = 0; d < 8; d += 2) {
+            // matrices: keys 0-7 and 8-15 of a piece, then of the next.  A thread has two values of two keys: the even values of a
+            // piece are the upper eight lines of the product, the odd ones the lower.
             uint32_t r[4];
-            ldsm_x4_t(vb + swz128_offset(row, k + pc), r);
-            // a thread has two values side by side of two keys: the even and the odd columns of a piece are two tiles
+            ldsm_x4_t(vb + swz128_offset(krow, d + (lane >> 4)), r);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const uint32_t w0 = r[2 * i], w1 = r[2 * i + 1];
-              mma_bf16(acc[2 * (k + i)], pf, e4m3x2_to_bf16x2((w0 << 8) & 0xff00ff00u), e4m3x2_to_bf16x2((w1 << 8) & 0xff00ff00u));
-              mma_bf16(acc[2 * (k + i) + 1], pf, e4m3x2_to_bf16x2(w0 & 0xff00ff00u), e4m3x2_to_bf16x2(w1 & 0xff00ff00u));
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t w0 = __byte_perm(r[2 * h], 0, 0x3120), w1 = __byte_perm(r[2 * h + 1], 0, 0x3120);
+              const uint32_t f[4] = {widen_lo(w0), widen_hi(w0), widen_lo(w1), widen_hi(w1)};
+#pragma unroll
+              for (int i = 0; i < NR; ++i) mma_16816<true>(acc[i][d + h], f, pf[i][nb][0], pf[i][nb][1]);
             }
           }
         } else {
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            uint32_t r[4];
-            ldsm_x4_t(vb + (k >> 2) * box_bytes + swz128_offset(row, (k & 3) * 2 + pc), r);
-            mma_bf16(acc[2 * k], pf, r[0], r[1]);
-            mma_bf16(acc[2 * k + 1], pf, r[2], r[3]);
+          for (int d = 0; d < 8; ++d) {
+            uint32_t r[4];                 // matrices: two pieces of keys 0-7, two of keys 8-15
+            ldsm_x4_t(vb + (d >> 2) * box_bytes + swz128_offset(vrow, (d & 3) * 2 + ((lane >> 3) & 1)), r);
+#pragma unroll
+            for (int i = 0; i < NR; ++i) mma_16816<false>(acc[i][d], r, pf[i][nb][0], pf[i][nb][1]);
           }
         }
       }
@@ -357,48 +464,41 @@ __global__ void __launch_bounds__(FEW_THREADS)
       if (lane == 0) mbar_arrive(&empty[s]);
     }
     ok = __all_sync(0xffffffffu, ok);
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-      if (l[r] != l[r] && m[r] == -INFINITY) m[r] = 0.f;         // scores that were all NaN: not to be taken for no keys at all
-    }
-    // Warps of the same rows meet in the ring: every stage has been read (a barrier below), and TMA asks for nothing more.
-    named_bar_sync(1, 128);
-    if (!FP8) {
-#pragma unroll
-      for (int r = 0; r < 2; ++r)
-        if (lim[r] > s_poison) {
-          l[r] = __int_as_float(0x7fffffff);
-          m[r] = fmaxf(m[r], 0.f);
-        }
-    }
-    float* ring = reinterpret_cast<float*>(smem);                // [warp][16][132]
+    // Warps of the same rows meet in the ring: every stage has been read (the barrier), and TMA asks for nothing more.
+    named_bar_sync(1, FEW_WARPS * 32);
+    float* ring = reinterpret_cast<float*>(smem);                // [warp][8 NR][132]
     constexpr int LD = 132;
-    if (c == 0) {
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        s_m[warp][g + 8 * r] = m[r];
-        s_l[warp][g + 8 * r] = l[r];
-      }
-    }
+    for (int i = 0; i < NR; ++i)
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
+      for (int e = 0; e < 2; ++e) {
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        float* at = ring + (warp * 16 + g + 8 * r) * LD;
-        if (FP8) {                         // columns 2 c, 2 c + 1 of an even / odd tile: values 4 c + {0, 2} / {1, 3} of a piece
-          at[(i >> 1) * 16 + c * 4 + (i & 1)] = acc[i][2 * r];
-          at[(i >> 1) * 16 + c * 4 + 2 + (i & 1)] = acc[i][2 * r + 1];
-        } else {
-          *reinterpret_cast<float2*>(at + i * 8 + c * 2) = make_float2(acc[i][2 * r], acc[i][2 * r + 1]);
+        for (int o = 4; o < 32; o <<= 1) l[i][e] += __shfl_xor_sync(0xffffffffu, l[i][e], o);
+        if (!FP8 && lim[i][e] > s_poison) l[i][e] = __int_as_float(0x7fffffff);
+        if (l[i][e] != l[i][e] && m[i][e] == -INFINITY) m[i][e] = 0.f;       // all NaN: not to be taken for no keys at all
+        // acc relative to the scores' maximum
+        const float f = !FP8 || mv[i][e] == -INFINITY ? 1.f : exp2f(mv[i][e] - m[i][e]);
+        const int row = i * 8 + 2 * c + e;
+        if (g == 0) {
+          s_m[warp][row] = m[i][e];
+          s_l[warp][row] = l[i][e];
+        }
+        float* at = ring + (warp * 8 * NR + row) * LD;
+#pragma unroll
+        for (int d = 0; d < 8; ++d) {
+          if (FP8) {
+            *reinterpret_cast<float2*>(at + d * 16 + 2 * g) = make_float2(acc[i][d][e] * f, acc[i][d][2 + e] * f);
+          } else {
+            at[d * 16 + g] = acc[i][d][e];
+            at[d * 16 + g + 8] = acc[i][d][2 + e];
+          }
         }
       }
-    named_bar_sync(1, 128);
+    named_bar_sync(1, FEW_WARPS * 32);
     const bool direct = item.w < 0;
     // a warp finishes one row at a time, four values per lane
-    for (int row = warp; row < rows; row += 4) {
-      const int w0 = row / 16 * WK, rr = row % 16;
+    for (int row = warp; row < rows; row += FEW_WARPS) {
+      const int w0 = row / (8 * NR) * WK, rr = row % (8 * NR);
       float mt = s_m[w0][rr];
 #pragma unroll
       for (int w = 1; w < WK; ++w) mt = fmaxf(mt, s_m[w0 + w][rr]);
@@ -408,7 +508,7 @@ __global__ void __launch_bounds__(FEW_THREADS)
       for (int w = 0; w < WK; ++w) {
         const float mw = s_m[w0 + w][rr];
         const float f = mw == -INFINITY ? 0.f : fast_exp2(mw - mt);
-        const float4 y = *reinterpret_cast<const float4*>(ring + ((w0 + w) * 16 + rr) * LD + lane * 4);
+        const float4 y = *reinterpret_cast<const float4*>(ring + ((w0 + w) * 8 * NR + rr) * LD + lane * 4);
         x.x += f * y.x;
         x.y += f * y.y;
         x.z += f * y.z;
@@ -472,9 +572,9 @@ __global__ void __launch_bounds__(MERGE_THREADS) paged_merge_kernel(const Plan p
   *reinterpret_cast<uint2*>(a.o + (long long)(q0 + t) * a.ldo + (long long)(head * G + (row0 + row) % G) * HEAD + lane * 4) = u;
 }
 
-template <bool FP8, int WR>
+template <bool FP8, int NR, int WR>
 static int launch_few(const Cache& c, const Plan& p, const FewArgs& a, cudaStream_t st) {
-  auto kernel = paged_few_kernel<FP8, WR>;
+  auto kernel = paged_few_kernel<FP8, NR, WR>;
   int dev = 0;
   SNU1_CUDA_CHECK(cudaGetDevice(&dev));
   static std::once_flag once[64];
@@ -485,6 +585,16 @@ static int launch_few(const Cache& c, const Plan& p, const FewArgs& a, cudaStrea
   SNU1_CUDA_CHECK(err);
   SNU1_CUDA_CHECK(launch_pdl(kernel, dim3(p.few_count, c.heads), dim3(FEW_THREADS), Few<FP8>::SMEM, st, c.kv, c.scale, p, a));
   return kHostOk;
+}
+
+template <bool FP8>
+static int launch_few(const Cache& c, const Plan& p, const FewArgs& a, cudaStream_t st) {
+  switch (p.few_rows) {
+    case 8: return launch_few<FP8, 1, 1>(c, p, a, st);
+    case 16: return launch_few<FP8, 2, 1>(c, p, a, st);
+    case 32: return launch_few<FP8, 2, 2>(c, p, a, st);
+    default: return launch_few<FP8, 2, 4>(c, p, a, st);
+  }
 }
 
 }  // namespace paged
@@ -526,10 +636,8 @@ SNU1_API int snu1_paged_attention(const void* cache, const void* plan, const voi
     if ((rc = launch_chunks(c, p, q, ldq, p.rows, o, ldo, a.part, a.part_ml, a.scale_log2, wide, st)) != kHostOk) return rc;
   }
   if (p.few_count > 0) {
-    if (c.fp8)
-      rc = p.few_rows <= 16 ? launch_few<true, 1>(c, p, a, st) : p.few_rows <= 32 ? launch_few<true, 2>(c, p, a, st) : launch_few<true, 4>(c, p, a, st);
-    else
-      rc = p.few_rows <= 16 ? launch_few<false, 1>(c, p, a, st) : p.few_rows <= 32 ? launch_few<false, 2>(c, p, a, st) : launch_few<false, 4>(c, p, a, st);
+    if (c.fp8) rc = launch_few<true>(c, p, a, st);
+    else rc = launch_few<false>(c, p, a, st);
     if (rc != kHostOk) return rc;
   }
   if (p.merge_count > 0)

@@ -18,7 +18,7 @@ constexpr float TINY = 7.70371977754894342e-34f;   // 2^-110, least row maximum 
 
 // One layer's cache, filled by snu1_paged_cache_init.
 struct alignas(64) Cache {
-  CUtensorMap kv;          // box: up to 64 tokens of one head, keys and values (64 values wide; e4m3: all 128)
+  CUtensorMap kv;          // box: up to 128 tokens of one head, keys and values, of bf16 up to 64 and 64 values wide
   CUtensorMap scale;       // box: the scales of the same
   CUtensorMap k, v;        // bf16 only: boxes of up to 128 tokens of one head, 64 values wide
   void* data;
@@ -54,16 +54,6 @@ __device__ __forceinline__ int seq_len(const Plan& p, int b) { return max(0, min
 __device__ __forceinline__ int row_limit(const Plan& p, int q0, int q_len, int kv_len, int token) {
   const int behind = p.behind != nullptr ? p.behind[q0 + token] : q_len - 1 - token;
   return max(0, min(kv_len, kv_len - behind));
-}
-
-// Two e4m3 codes in the high bytes of the halves of ``x`` (low bytes zero) as bf16.  The code's exponent and mantissa are put at
-// the bottom of bf16's, which is the value times 2^-120 (also for codes below the smallest normal one: bf16 products keep
-// subnormal inputs), so the product with 2^120 is exact.
-__device__ __forceinline__ uint32_t e4m3x2_to_bf16x2(uint32_t x) {
-  const uint32_t m = (x & 0x80008000u) | ((x >> 4) & 0x07f007f0u);
-  uint32_t r;
-  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(m), "r"(0x7b807b80u));
-  return r;
 }
 
 __device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* m, uint64_t* bar, int x, int y, int z, int w, int u) {

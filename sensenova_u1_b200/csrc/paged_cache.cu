@@ -63,7 +63,7 @@ __global__ void __launch_bounds__(WRITE_THREADS)
     for (int j = 0; j < 4; ++j) top = max(top, max(u[j] << 16 & 0x7fffffffu, u[j] & 0x7fff0000u));
 #pragma unroll
     for (int o = 1; o < 16; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const bool finite = top < 0x7f800000u;
+    const bool finite = top < 0x7f800000u;           // otherwise NaN is the scale, and the codes are zeros
     const float a = fmaxf(__uint_as_float(top), TINY), inv = __fdiv_rn(E4M3_MAX, a);
     uint2 code;
     uint32_t q[4];
@@ -71,8 +71,8 @@ __global__ void __launch_bounds__(WRITE_THREADS)
     for (int j = 0; j < 4; ++j)
       q[j] = __nv_cvt_float2_to_fp8x2(make_float2(__uint_as_float(u[j] << 16) * inv, __uint_as_float(u[j] & 0xffff0000u) * inv),
                                       __NV_SATFINITE, __NV_E4M3);
-    code.x = q[0] | q[1] << 16;
-    code.y = q[2] | q[3] << 16;
+    code.x = finite ? q[0] | q[1] << 16 : 0u;
+    code.y = finite ? q[2] | q[3] << 16 : 0u;
     if (at[i] >= 0) {
       *reinterpret_cast<uint2*>(data + at[i] * HEAD + c * 8) = code;
       if (c == 0) scales[at[i]] = finite ? __fdiv_rn(a, E4M3_MAX) : __int_as_float(0x7fffffff);
@@ -180,7 +180,7 @@ SNU1_API int snu1_paged_cache_init(void* out, void* data, void* scales, int page
   c.page = page;
   c.fp8 = fp8;
   const uint64_t row = fp8 ? 128 : 256, P = page, H = heads;
-  const uint32_t bx = page < 64 ? page : 64;
+  const uint32_t bx = fp8 || page < 64 ? page : 64;      // a stage of attn_paged.cu: 128 tokens of e4m3, 64 of bf16
   int rc;
   {
     const uint64_t dims[5] = {128, P, H, 2, (uint64_t)pages}, str[4] = {row, row * P, row * P * H, row * P * H * 2};

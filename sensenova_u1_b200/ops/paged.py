@@ -187,7 +187,7 @@ def _lay_out(q_lens, kv_lens, tables, page: int, pages: int, group: int, kv_head
     chunked = (q_rows > FEW_TILE) & (group <= CHUNK_TILE)
     few_q = np.where(chunked, 0, q_rows)
     top = int(few_q.max()) if n else 0
-    few_rows = 16 if top <= 16 else 32 if top <= 32 else FEW_TILE
+    few_rows = 8 if top <= 8 else 16 if top <= 16 else 32 if top <= 32 else FEW_TILE
     chunk_rows = 2 * (CHUNK_TILE // group) * group if group <= CHUNK_TILE else 1        # two row tiles of whole tokens
 
     def tiles_of(q_rows, m):
