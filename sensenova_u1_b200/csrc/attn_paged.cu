@@ -117,7 +117,8 @@ __global__ void __launch_bounds__(FEW_THREADS, NR == 1 ? 3 : 2)
     paged_few_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_constant__ CUtensorMap tm_scale, const Plan p,
                      const FewArgs a) {
   using F = Few<FP8>;
-  constexpr int KT = F::KT, WK = FEW_WARPS / WR, M = 8 * NR * WR, NB = KT / 16 / WK;     // NB: blocks of 16 keys of a warp
+  constexpr int KT = F::KT, WK = FEW_WARPS / WR, M = 8 * NR * WR;
+  constexpr int BLOCKS = KT / 16 / WK, NB = BLOCKS < 2 ? BLOCKS : 2;     // blocks of 16 keys of a warp, and how many at a time
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   float* s_scales = reinterpret_cast<float*>(smem + F::STAGES * F::DATA);   // [stage][page box][keys, values][box rows]
@@ -307,156 +308,159 @@ __global__ void __launch_bounds__(FEW_THREADS, NR == 1 ? 3 : 2)
         fence_proxy_async_smem();          // TMA writes here again
         named_bar_sync(1, FEW_WARPS * 32);
       }
-      float sv[NR][NB][4];                 // S^T: keys g, g + 8 x rows 2 c, 2 c + 1
+#pragma unroll 1
+      for (int u0 = wk * BLOCKS; u0 < (wk + 1) * BLOCKS; u0 += NB) {
+        float sv[NR][NB][4];                 // S^T: keys g, g + 8 x rows 2 c, 2 c + 1
 #pragma unroll
-      for (int i = 0; i < NR; ++i)
+        for (int i = 0; i < NR; ++i)
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
+          for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) sv[i][nb][e] = 0.f;
+            for (int e = 0; e < 4; ++e) sv[i][nb][e] = 0.f;
 #pragma unroll
-      for (int k = 0; k < 8; k += 2) {     // 32 values at a time
+        for (int k = 0; k < 8; k += 2) {     // 32 values at a time
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) {
+            const int key0 = (u0 + nb) * 16;
+            const uint32_t kb = data + (key0 >> bx_log) * F::HALVES * box_bytes + ((key0 & (bx - 1)) << 7);
+            if (FP8) {
+              // matrices: keys 0-7 and 8-15 of a 16-value piece, then of the next piece
+              uint32_t r[4];
+              ldsm_x4(kb + swz128_offset(krow, k + (lane >> 4)), r);
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const uint32_t w0 = r[2 * h], w1 = r[2 * h + 1];
+                const uint32_t f[4] = {widen_lo(w0), widen_lo(w1), widen_hi(w0), widen_hi(w1)};
+#pragma unroll
+                for (int i = 0; i < NR; ++i) mma_16816<true>(sv[i][nb], f, qf[i][k + h][0], qf[i][k + h][1]);
+              }
+            } else {
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                uint32_t r[4];
+                ldsm_x4(kb + (k >> 2) * box_bytes + swz128_offset(krow, ((k + h) & 3) * 2 + (lane >> 4)), r);
+#pragma unroll
+                for (int i = 0; i < NR; ++i) mma_16816<false>(sv[i][nb], r, qf[i][k + h][0], qf[i][k + h][1]);
+              }
+            }
+          }
+        }
+        // scores in log2 units, masked; largest of this thread's keys
+        float lv[NB][2];                     // log2 of the values' scales
+        float mx[NR][2], mxv[NR][2];
+#pragma unroll
+        for (int i = 0; i < NR; ++i)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) mx[i][e] = mxv[i][e] = -INFINITY;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
-          const int key0 = (wk * NB + nb) * 16;
-          const uint32_t kb = data + (key0 >> bx_log) * F::HALVES * box_bytes + ((key0 & (bx - 1)) << 7);
+          const int key = (u0 + nb) * 16 + g;
+          float ks[2] = {1.f, 1.f};
+          lv[nb][0] = lv[nb][1] = 0.f;
           if (FP8) {
-            // matrices: keys 0-7 and 8-15 of a 16-value piece, then of the next piece
-            uint32_t r[4];
-            ldsm_x4(kb + swz128_offset(krow, k + (lane >> 4)), r);
+            const int key0 = (u0 + nb) * 16;
+            const float* sc = s_scales + s * KT * 2 + ((key0 >> bx_log) << (bx_log + 1)) + (key0 & (bx - 1)) + g;
+            ks[0] = sc[0];
+            ks[1] = sc[8];
+            lv[nb][0] = fast_log2(sc[bx]);
+            lv[nb][1] = fast_log2(sc[bx + 8]);
+          }
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const uint32_t w0 = r[2 * h], w1 = r[2 * h + 1];
-              const uint32_t f[4] = {widen_lo(w0), widen_lo(w1), widen_hi(w0), widen_hi(w1)};
+          for (int i = 0; i < NR; ++i)
 #pragma unroll
-              for (int i = 0; i < NR; ++i) mma_16816<true>(sv[i][nb], f, qf[i][k + h][0], qf[i][k + h][1]);
+            for (int e = 0; e < 4; ++e) {
+              float x = sv[i][nb][e] * (FP8 ? rs[i][e & 1] * ks[e >> 1] : rs[i][e & 1]);
+              if (partial && k0 + key + (e >> 1) * 8 >= lim[i][e & 1]) x = -INFINITY;
+              sv[i][nb][e] = x;
+              mx[i][e & 1] = fmaxf(mx[i][e & 1], x);
+              if (FP8) mxv[i][e & 1] = fmaxf(mxv[i][e & 1], x + lv[nb][e >> 1]);
+            }
+        }
+        // A running maximum moves only when it is outgrown by more than 2^8 (see attn_infer_sm100.cu), so most tiles need no
+        // reduction over the lanes.
+        bool move = false;
+#pragma unroll
+        for (int i = 0; i < NR; ++i)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) move |= mx[i][e] > m[i][e] + 8.f || (FP8 && mxv[i][e] > mv[i][e] + 8.f);
+        if (__any_sync(0xffffffffu, move)) {
+#pragma unroll
+          for (int i = 0; i < NR; ++i)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+#pragma unroll
+              for (int o = 4; o < 32; o <<= 1) {
+                mx[i][e] = fmaxf(mx[i][e], __shfl_xor_sync(0xffffffffu, mx[i][e], o));
+                if (FP8) mxv[i][e] = fmaxf(mxv[i][e], __shfl_xor_sync(0xffffffffu, mxv[i][e], o));
+              }
+              const float mn = fmaxf(m[i][e], mx[i][e]);
+              const float f = m[i][e] == -INFINITY ? 0.f : fast_exp2(m[i][e] - mn);
+              m[i][e] = mn;
+              l[i][e] *= f;
+              float fv = f;
+              if (FP8) {
+                const float nv = fmaxf(mv[i][e], mxv[i][e]);
+                fv = mv[i][e] == -INFINITY ? 0.f : fast_exp2(mv[i][e] - nv);
+                mv[i][e] = nv;
+              }
+#pragma unroll
+              for (int d = 0; d < 8; ++d) {
+                acc[i][d][e] *= fv;
+                acc[i][d][2 + e] *= fv;
+              }
+            }
+        }
+        uint32_t pf[NR][NB][2];              // p^T: rows g x keys 2 c + {0, 1}, then + 8
+#pragma unroll
+        for (int i = 0; i < NR; ++i) {
+          float mu[2], muv[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            mu[e] = m[i][e] == -INFINITY ? 0.f : m[i][e];
+            muv[e] = FP8 && mv[i][e] != -INFINITY ? mv[i][e] : 0.f;
+          }
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) {
+            float x[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              x[e] = fast_exp2(sv[i][nb][e] - mu[e & 1]);
+              l[i][e & 1] += x[e];
+              // (the logarithm of a masked key's scale may be anything)
+              if (FP8) x[e] = partial && sv[i][nb][e] == -INFINITY ? 0.f : fast_exp2(sv[i][nb][e] + lv[nb][e >> 1] - muv[e & 1]);
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              pf[i][nb][h] = transpose_8x8(FP8 ? pack_f16x2(x[2 * h], x[2 * h + 1]) : pack_bf16x2(x[2 * h], x[2 * h + 1]));
+          }
+        }
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          const int key0 = (u0 + nb) * 16;
+          const uint32_t vb = data + (key0 >> bx_log) * F::HALVES * box_bytes + ((bx + (key0 & (bx - 1))) << 7);
+          if (FP8) {
+#pragma unroll
+            for (int d = 0; d < 8; d += 2) {
+              // matrices: keys 0-7 and 8-15 of a piece, then of the next.  A thread has two values of two keys: the even values of a
+              // piece are the upper eight lines of the product, the odd ones the lower.
+              uint32_t r[4];
+              ldsm_x4_t(vb + swz128_offset(krow, d + (lane >> 4)), r);
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const uint32_t w0 = __byte_perm(r[2 * h], 0, 0x3120), w1 = __byte_perm(r[2 * h + 1], 0, 0x3120);
+                const uint32_t f[4] = {widen_lo(w0), widen_hi(w0), widen_lo(w1), widen_hi(w1)};
+#pragma unroll
+                for (int i = 0; i < NR; ++i) mma_16816<true>(acc[i][d + h], f, pf[i][nb][0], pf[i][nb][1]);
+              }
             }
           } else {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              uint32_t r[4];
-              ldsm_x4(kb + (k >> 2) * box_bytes + swz128_offset(krow, ((k + h) & 3) * 2 + (lane >> 4)), r);
-#pragma unroll
-              for (int i = 0; i < NR; ++i) mma_16816<false>(sv[i][nb], r, qf[i][k + h][0], qf[i][k + h][1]);
-            }
-          }
-        }
-      }
-      // scores in log2 units, masked; largest of this thread's keys
-      float lv[NB][2];                     // log2 of the values' scales
-      float mx[NR][2], mxv[NR][2];
-#pragma unroll
-      for (int i = 0; i < NR; ++i)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) mx[i][e] = mxv[i][e] = -INFINITY;
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        const int key = (wk * NB + nb) * 16 + g;
-        float ks[2] = {1.f, 1.f};
-        lv[nb][0] = lv[nb][1] = 0.f;
-        if (FP8) {
-          const int key0 = (wk * NB + nb) * 16;
-          const float* sc = s_scales + s * KT * 2 + ((key0 >> bx_log) << (bx_log + 1)) + (key0 & (bx - 1)) + g;
-          ks[0] = sc[0];
-          ks[1] = sc[8];
-          lv[nb][0] = fast_log2(sc[bx]);
-          lv[nb][1] = fast_log2(sc[bx + 8]);
-        }
-#pragma unroll
-        for (int i = 0; i < NR; ++i)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float x = sv[i][nb][e] * (FP8 ? rs[i][e & 1] * ks[e >> 1] : rs[i][e & 1]);
-            if (partial && k0 + key + (e >> 1) * 8 >= lim[i][e & 1]) x = -INFINITY;
-            sv[i][nb][e] = x;
-            mx[i][e & 1] = fmaxf(mx[i][e & 1], x);
-            if (FP8) mxv[i][e & 1] = fmaxf(mxv[i][e & 1], x + lv[nb][e >> 1]);
-          }
-      }
-      // A running maximum moves only when it is outgrown by more than 2^8 (see attn_infer_sm100.cu), so most tiles need no
-      // reduction over the lanes.
-      bool move = false;
-#pragma unroll
-      for (int i = 0; i < NR; ++i)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) move |= mx[i][e] > m[i][e] + 8.f || (FP8 && mxv[i][e] > mv[i][e] + 8.f);
-      if (__any_sync(0xffffffffu, move)) {
-#pragma unroll
-        for (int i = 0; i < NR; ++i)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-#pragma unroll
-            for (int o = 4; o < 32; o <<= 1) {
-              mx[i][e] = fmaxf(mx[i][e], __shfl_xor_sync(0xffffffffu, mx[i][e], o));
-              if (FP8) mxv[i][e] = fmaxf(mxv[i][e], __shfl_xor_sync(0xffffffffu, mxv[i][e], o));
-            }
-            const float mn = fmaxf(m[i][e], mx[i][e]);
-            const float f = m[i][e] == -INFINITY ? 0.f : fast_exp2(m[i][e] - mn);
-            m[i][e] = mn;
-            l[i][e] *= f;
-            float fv = f;
-            if (FP8) {
-              const float nv = fmaxf(mv[i][e], mxv[i][e]);
-              fv = mv[i][e] == -INFINITY ? 0.f : fast_exp2(mv[i][e] - nv);
-              mv[i][e] = nv;
-            }
-#pragma unroll
             for (int d = 0; d < 8; ++d) {
-              acc[i][d][e] *= fv;
-              acc[i][d][2 + e] *= fv;
+              uint32_t r[4];                 // matrices: two pieces of keys 0-7, two of keys 8-15
+              ldsm_x4_t(vb + (d >> 2) * box_bytes + swz128_offset(vrow, (d & 3) * 2 + ((lane >> 3) & 1)), r);
+#pragma unroll
+              for (int i = 0; i < NR; ++i) mma_16816<false>(acc[i][d], r, pf[i][nb][0], pf[i][nb][1]);
             }
-          }
-      }
-      uint32_t pf[NR][NB][2];              // p^T: rows g x keys 2 c + {0, 1}, then + 8
-#pragma unroll
-      for (int i = 0; i < NR; ++i) {
-        float mu[2], muv[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          mu[e] = m[i][e] == -INFINITY ? 0.f : m[i][e];
-          muv[e] = FP8 && mv[i][e] != -INFINITY ? mv[i][e] : 0.f;
-        }
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-          float x[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            x[e] = fast_exp2(sv[i][nb][e] - mu[e & 1]);
-            l[i][e & 1] += x[e];
-            // (the logarithm of a masked key's scale may be anything)
-            if (FP8) x[e] = partial && sv[i][nb][e] == -INFINITY ? 0.f : fast_exp2(sv[i][nb][e] + lv[nb][e >> 1] - muv[e & 1]);
-          }
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-            pf[i][nb][h] = transpose_8x8(FP8 ? pack_f16x2(x[2 * h], x[2 * h + 1]) : pack_bf16x2(x[2 * h], x[2 * h + 1]));
-        }
-      }
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        const int key0 = (wk * NB + nb) * 16;
-        const uint32_t vb = data + (key0 >> bx_log) * F::HALVES * box_bytes + ((bx + (key0 & (bx - 1))) << 7);
-        if (FP8) {
-#pragma unroll
-          for (int d = 0; d < 8; d += 2) {
-            // matrices: keys 0-7 and 8-15 of a piece, then of the next.  A thread has two values of two keys: the even values of a
-            // piece are the upper eight lines of the product, the odd ones the lower.
-            uint32_t r[4];
-            ldsm_x4_t(vb + swz128_offset(krow, d + (lane >> 4)), r);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const uint32_t w0 = __byte_perm(r[2 * h], 0, 0x3120), w1 = __byte_perm(r[2 * h + 1], 0, 0x3120);
-              const uint32_t f[4] = {widen_lo(w0), widen_hi(w0), widen_lo(w1), widen_hi(w1)};
-#pragma unroll
-              for (int i = 0; i < NR; ++i) mma_16816<true>(acc[i][d + h], f, pf[i][nb][0], pf[i][nb][1]);
-            }
-          }
-        } else {
-#pragma unroll
-          for (int d = 0; d < 8; ++d) {
-            uint32_t r[4];                 // matrices: two pieces of keys 0-7, two of keys 8-15
-            ldsm_x4_t(vb + (d >> 2) * box_bytes + swz128_offset(vrow, (d & 3) * 2 + ((lane >> 3) & 1)), r);
-#pragma unroll
-            for (int i = 0; i < NR; ++i) mma_16816<false>(acc[i][d], r, pf[i][nb][0], pf[i][nb][1]);
           }
         }
       }

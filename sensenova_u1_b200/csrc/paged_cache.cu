@@ -6,8 +6,9 @@
 // of one head differ in size from token to token, and a row is written once, by itself.  A row that holds a value that is
 // not finite gets NaN as its scale: it reads back as NaN, and attention to it is NaN.
 //
-// Both directions are bound by memory: 16 lanes own a row (16 bytes of bf16, 8 codes each), a warp the key and the value
-// row of one (token, head) when writing, two rows of a page when reading; four of these are in flight per warp.
+// Both directions are bound by memory: 16 lanes own a row (16 bytes of bf16, 8 codes each), four rows are in flight per
+// lane.  Where a token or a page lives takes three dependent loads, so a block looks that up once for many rows: up to 16
+// tokens of all heads when writing, 256 rows of a page when reading.
 #include <cuda_fp8.h>
 #include <string.h>
 
@@ -18,71 +19,83 @@ namespace snu1 {
 namespace paged {
 
 constexpr int WRITE_THREADS = 256;
-constexpr int WRITE_TOKENS = 4;      // tokens of one head per warp
+constexpr int WRITE_TOKENS = 16;     // most tokens of a block
+constexpr int WRITE_DEEP = 4;        // (token, head) pairs that a warp has in flight
 
+// A block writes ``tokens`` rows of all heads; a warp a (token, head) at a time, 16 lanes the key, 16 the value.
 template <bool FP8>
 __global__ void __launch_bounds__(WRITE_THREADS)
     paged_write_kernel(const __nv_bfloat16* __restrict__ k, long long ldk, const __nv_bfloat16* __restrict__ v, long long ldv,
-                       uint8_t* __restrict__ data, float* __restrict__ scales, int pages, int heads, int page, Plan p, int* status) {
+                       uint8_t* __restrict__ data, float* __restrict__ scales, int pages, int heads, int tokens, Plan p, int* status) {
+  __shared__ long long place[WRITE_TOKENS];          // the token's row for head 0's keys, -1: none
   pdl_wait();
   pdl_trigger();
-  const int lane = threadIdx.x & 31, kv = lane >> 4, c = lane & 15;
-  const long long w = (long long)blockIdx.x * (WRITE_THREADS / 32) + (threadIdx.x >> 5);
-  const int head = (int)(w % heads);
-  const long long row0 = w / heads * WRITE_TOKENS;
-  const __nv_bfloat16* src = kv ? v : k;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, kv = lane >> 4, c = lane & 15;
+  const int row0 = blockIdx.x * tokens, count = min(tokens, p.rows - row0);
+  if (threadIdx.x < count) {
+    const int row = row0 + threadIdx.x, b = p.row_seq[row];
+    const int pos = seq_len(p, b) - (p.q_start[b + 1] - row);
+    long long at = -1;
+    if (pos >= 0) {
+      const int pg = p.table[(long long)b * p.width + pos / p.page];
+      if (pg >= 0 && pg < pages) at = (long long)pg * 2 * heads * p.page + pos % p.page;
+      else report_status(status, kBadPage, 9);
+    }
+    place[threadIdx.x] = at;
+  }
+  const __nv_bfloat16* src = (kv ? v : k) + (long long)row0 * (kv ? ldv : ldk) + c * 8;
   const long long ld = kv ? ldv : ldk;
-  uint4 x[WRITE_TOKENS];
-  long long at[WRITE_TOKENS];            // row of the cache, -1: none
+  const int pairs = count * heads;
+  bool known = false;
+  for (int first = warp; first < pairs; first += WRITE_THREADS / 32 * WRITE_DEEP) {
+    uint4 x[WRITE_DEEP];
+    int token[WRITE_DEEP], head[WRITE_DEEP];
 #pragma unroll
-  for (int i = 0; i < WRITE_TOKENS; ++i) {
-    const long long row = row0 + i;
-    at[i] = -1;
-    x[i] = make_uint4(0, 0, 0, 0);
-    if (row < p.rows) {
-      x[i] = *reinterpret_cast<const uint4*>(src + row * ld + head * HEAD + c * 8);
-      const int b = p.row_seq[row];
-      const int pos = seq_len(p, b) - (p.q_start[b + 1] - (int)row);
-      if (pos >= 0) {
-        const int pg = p.table[(long long)b * p.width + pos / page];
-        if (pg >= 0 && pg < pages) at[i] = (((long long)pg * 2 + kv) * heads + head) * page + pos % page;
-        else if (lane == 0) report_status(status, kBadPage, 9);
+    for (int i = 0; i < WRITE_DEEP; ++i) {
+      const int pair = first + i * (WRITE_THREADS / 32);
+      token[i] = pair / heads;
+      head[i] = pair - token[i] * heads;
+      x[i] = pair < pairs ? *reinterpret_cast<const uint4*>(src + token[i] * ld + head[i] * HEAD) : make_uint4(0, 0, 0, 0);
+    }
+    if (!known) {
+      __syncthreads();
+      known = true;
+    }
+#pragma unroll
+    for (int i = 0; i < WRITE_DEEP; ++i) {
+      const bool on = first + i * (WRITE_THREADS / 32) < pairs;
+      const long long base = on ? place[token[i]] : -1;
+      const long long at = base + (long long)(kv * heads + head[i]) * p.page;
+      if (!FP8) {
+        if (base >= 0) *reinterpret_cast<uint4*>(data + at * (HEAD * 2) + c * 16) = x[i];
+        continue;
+      }
+      const uint32_t u[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+      // as whole numbers: a NaN is larger than infinity, which is larger than every finite value
+      uint32_t top = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) top = max(top, max(u[j] << 16 & 0x7fffffffu, u[j] & 0x7fff0000u));
+#pragma unroll
+      for (int o = 1; o < 16; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const bool finite = top < 0x7f800000u;           // otherwise NaN is the scale, and the codes are zeros
+      const float a = fmaxf(__uint_as_float(top), TINY), inv = __fdiv_rn(E4M3_MAX, a);
+      uint32_t q[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        q[j] = __nv_cvt_float2_to_fp8x2(make_float2(__uint_as_float(u[j] << 16) * inv, __uint_as_float(u[j] & 0xffff0000u) * inv),
+                                        __NV_SATFINITE, __NV_E4M3);
+      if (base >= 0) {
+        *reinterpret_cast<uint2*>(data + at * HEAD + c * 8) = finite ? make_uint2(q[0] | q[1] << 16, q[2] | q[3] << 16) : make_uint2(0, 0);
+        if (c == 0) scales[at] = finite ? __fdiv_rn(a, E4M3_MAX) : __int_as_float(0x7fffffff);
       }
     }
   }
-#pragma unroll
-  for (int i = 0; i < WRITE_TOKENS; ++i) {
-    if (!FP8) {
-      if (at[i] >= 0) *reinterpret_cast<uint4*>(data + at[i] * (HEAD * 2) + c * 16) = x[i];
-      continue;
-    }
-    const uint32_t u[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-    // as whole numbers: a NaN is larger than infinity, which is larger than every finite value
-    uint32_t top = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) top = max(top, max(u[j] << 16 & 0x7fffffffu, u[j] & 0x7fff0000u));
-#pragma unroll
-    for (int o = 1; o < 16; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const bool finite = top < 0x7f800000u;           // otherwise NaN is the scale, and the codes are zeros
-    const float a = fmaxf(__uint_as_float(top), TINY), inv = __fdiv_rn(E4M3_MAX, a);
-    uint2 code;
-    uint32_t q[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      q[j] = __nv_cvt_float2_to_fp8x2(make_float2(__uint_as_float(u[j] << 16) * inv, __uint_as_float(u[j] & 0xffff0000u) * inv),
-                                      __NV_SATFINITE, __NV_E4M3);
-    code.x = finite ? q[0] | q[1] << 16 : 0u;
-    code.y = finite ? q[2] | q[3] << 16 : 0u;
-    if (at[i] >= 0) {
-      *reinterpret_cast<uint2*>(data + at[i] * HEAD + c * 8) = code;
-      if (c == 0) scales[at[i]] = finite ? __fdiv_rn(a, E4M3_MAX) : __int_as_float(0x7fffffff);
-    }
-  }
+  if (!known) __syncthreads();
 }
 
 constexpr int READ_THREADS = 256;
-constexpr int READ_ROWS = 4;                                         // rows of a lane
-constexpr int READ_BLOCK = READ_THREADS / 16 * READ_ROWS;            // rows of a block
+constexpr int READ_DEEP = 4;                                         // rows that a lane has in flight
+constexpr int READ_BLOCK = 256;                                      // rows of a block
 
 // Rows of the planned pages, in order.  PACKED: out = keys, out2 = values [rows][heads][128] at the plan's row numbers;
 // otherwise out = codes as bf16 (without their scales) in pages of 128 tokens in a cache's own layout, every sequence from a
@@ -94,57 +107,60 @@ __global__ void __launch_bounds__(READ_THREADS)
   pdl_wait();
   pdl_trigger();
   const int2 e = (PACKED ? p.read_pages : p.unpack)[blockIdx.x];
+  const int page_log = __ffs(page) - 1;
   const int b = e.x, pos0 = e.y * page, c = threadIdx.x & 15;
   const int k0 = p.k_start[b];
   const int len = PACKED ? p.k_start[b + 1] - k0 : seq_len(p, b);
   const int pg = pos0 < len ? p.table[(long long)b * p.width + e.y] : 0;
   const bool there = pos0 < len && pg >= 0 && pg < pages;
   if (pos0 < len && !there && threadIdx.x == 0) report_status(status, kBadPage, 9);
-  uint4 x[READ_ROWS];
-  float s[READ_ROWS];
-  const int first = blockIdx.y * READ_BLOCK + (threadIdx.x >> 4), total = 2 * heads * page;
+  const int total = 2 * heads * page, end = min(total, (int)(blockIdx.y + 1) * READ_BLOCK);
+  for (int first = blockIdx.y * READ_BLOCK + (threadIdx.x >> 4); first < end; first += READ_THREADS / 16 * READ_DEEP) {
+    uint4 x[READ_DEEP];
+    float s[READ_DEEP];
 #pragma unroll
-  for (int i = 0; i < READ_ROWS; ++i) {
-    const int r = first + i * (READ_THREADS / 16);                   // row of the page: (kv, head, token)
-    x[i] = make_uint4(0, 0, 0, 0);
-    s[i] = 0.f;
-    if (there && r < total && pos0 + r % page < len) {
-      const long long at = (long long)pg * total + r;
+    for (int i = 0; i < READ_DEEP; ++i) {
+      const int r = first + i * (READ_THREADS / 16);                 // row of the page: (kv, head, token)
+      x[i] = make_uint4(0, 0, 0, 0);
+      s[i] = 0.f;
+      if (there && r < end && pos0 + (r & (page - 1)) < len) {
+        const long long at = (long long)pg * total + r;
+        if (FP8) {
+          const uint2 u = *reinterpret_cast<const uint2*>(data + at * HEAD + c * 8);
+          x[i].x = u.x;
+          x[i].y = u.y;
+          s[i] = PACKED ? scales[at] : 1.f;
+        } else {
+          x[i] = *reinterpret_cast<const uint4*>(data + at * (HEAD * 2) + c * 16);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < READ_DEEP; ++i) {
+      const int r = first + i * (READ_THREADS / 16);
+      const int pos = pos0 + (r & (page - 1)), kvh = r >> page_log, kv = kvh >= heads, head = kvh - kv * heads;
+      if (r >= end || (PACKED && pos >= len)) continue;
+      uint4 y = x[i];
       if (FP8) {
-        const uint2 u = *reinterpret_cast<const uint2*>(data + at * HEAD + c * 8);
-        x[i].x = u.x;
-        x[i].y = u.y;
-        s[i] = PACKED ? scales[at] : 1.f;
+        const uint32_t u[2] = {x[i].x, x[i].y};
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const __half2 h(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(u[j >> 1] >> (16 * (j & 1))), __NV_E4M3));
+          const float2 f = __half22float2(h);
+          w[j] = pack_bf16x2(f.x * s[i], f.y * s[i]);
+        }
+        y = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+      __nv_bfloat16* dst;
+      if (PACKED) {
+        dst = (kv ? out2 : out) + ((long long)(k0 + pos) * heads + head) * HEAD;
       } else {
-        x[i] = *reinterpret_cast<const uint4*>(data + at * (HEAD * 2) + c * 16);
+        const long long t = (long long)p.unpack_first[b] * 128 + pos;
+        dst = out + (((t >> 7) * 2 * heads + kvh) * 128 + (t & 127)) * HEAD;
       }
+      *reinterpret_cast<uint4*>(dst + c * 8) = y;
     }
-  }
-#pragma unroll
-  for (int i = 0; i < READ_ROWS; ++i) {
-    const int r = first + i * (READ_THREADS / 16);
-    const int pos = pos0 + r % page, head = r / page % heads, kv = r / page / heads;
-    if (r >= total || (PACKED && pos >= len)) continue;
-    uint4 y = x[i];
-    if (FP8) {
-      const uint32_t u[2] = {x[i].x, x[i].y};
-      uint32_t w[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const __half2 h(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(u[j >> 1] >> (16 * (j & 1))), __NV_E4M3));
-        const float2 f = __half22float2(h);
-        w[j] = pack_bf16x2(f.x * s[i], f.y * s[i]);
-      }
-      y = make_uint4(w[0], w[1], w[2], w[3]);
-    }
-    __nv_bfloat16* dst;
-    if (PACKED) {
-      dst = (kv ? out2 : out) + ((long long)(k0 + pos) * heads + head) * HEAD;
-    } else {
-      const long long t = (long long)(p.unpack_first[b]) * 128 + pos;
-      dst = out + ((((t >> 7) * 2 + kv) * heads + head) * 128 + (t & 127)) * HEAD;
-    }
-    *reinterpret_cast<uint4*>(dst + c * 8) = y;
   }
 }
 
@@ -213,12 +229,12 @@ SNU1_API int snu1_paged_write(const void* cache, const void* plan, const void* k
     set_last_error("paged_write: rows must be 16-byte aligned, and the plan made for this page size");
     return kHostBadArg;
   }
-  const long long warps = (long long)(p.rows + paged::WRITE_TOKENS - 1) / paged::WRITE_TOKENS * c.heads;
-  const long long blocks = (warps + paged::WRITE_THREADS / 32 - 1) / (paged::WRITE_THREADS / 32);
+  // many tokens share a block's look-up, as long as there are blocks for every SM
+  const int tokens = max(1, min(paged::WRITE_TOKENS, p.rows / (4 * num_sms())));
   auto kernel = c.fp8 ? paged::paged_write_kernel<true> : paged::paged_write_kernel<false>;
-  SNU1_CUDA_CHECK(launch_pdl(kernel, dim3((unsigned)blocks), dim3(paged::WRITE_THREADS), 0, (cudaStream_t)stream,
+  SNU1_CUDA_CHECK(launch_pdl(kernel, dim3((p.rows + tokens - 1) / tokens), dim3(paged::WRITE_THREADS), 0, (cudaStream_t)stream,
                              (const __nv_bfloat16*)k, ldk, (const __nv_bfloat16*)v, ldv, (uint8_t*)c.data, c.scales, c.pages, c.heads,
-                             c.page, p, device_status_word()));
+                             tokens, p, device_status_word()));
   return kHostOk;
 }
 

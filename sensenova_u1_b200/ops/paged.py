@@ -43,6 +43,18 @@ CHUNK_SLOTS = 148        # its CTAs that run at once
 CHUNK_START = 3          # what starting and ending a CTA costs, in key tiles
 
 
+def _library():
+    """The library, its entry points told the types of their arguments (cheaper than an object per argument and call)."""
+    lib = _lib.load()
+    if lib.snu1_paged_write.argtypes is None:
+        P, L, I = c_void_p, c_ll, c_int
+        lib.snu1_paged_cache_init.argtypes = (P, P, P, I, I, I, I)
+        lib.snu1_paged_read.argtypes = (P, P, P, P, P)
+        lib.snu1_paged_attention.argtypes = (P, P, P, L, P, L, c_float, P, P)
+        lib.snu1_paged_write.argtypes = (P, P, P, L, P, L, P)
+    return lib
+
+
 class PagedCache:
     """Keys and values of one layer: ``data`` [pages, 2, kv_heads, page, 128] (bf16 or float8_e4m3fn; index 0 of the second
     dimension are the keys), ``scales`` [pages, 2, kv_heads, page] fp32 for e4m3 (value = code * scale), else None."""
@@ -66,10 +78,12 @@ class PagedCache:
         self.pages, _, self.kv_heads, self.page, _ = data.shape
         if self.kv_heads > 1023 or self.pages >= 1 << 31:
             raise ValueError("too many heads or pages")
-        self._desc = ctypes.create_string_buffer(_lib.load().snu1_paged_cache_bytes())
+        self._key = (data.dtype, self.page, self.kv_heads, data.get_device())
+        self._desc = ctypes.create_string_buffer(_library().snu1_paged_cache_bytes())
+        self._addr = ctypes.addressof(self._desc)
         with torch.cuda.device(data.device):
-            _lib.call("paged_cache_init", self._desc, c_void_p(data.data_ptr()), c_void_p(None if scales is None else scales.data_ptr()),
-                      c_int(self.pages), c_int(self.kv_heads), c_int(self.page), c_int(0 if scales is None else 1))
+            _lib.call("paged_cache_init", self._addr, data.data_ptr(), None if scales is None else scales.data_ptr(), self.pages,
+                      self.kv_heads, self.page, 0 if scales is None else 1)
 
     @classmethod
     def empty(cls, pages: int, page: int, kv_heads: int, dtype=torch.bfloat16, device="cuda") -> "PagedCache":
@@ -115,6 +129,11 @@ class PagedPlan:
     grow: int
     _store: torch.Tensor = field(repr=False)
     _args: _Args = field(repr=False)
+
+    def __post_init__(self):
+        self._index = self.device.index
+        self._key = (self.dtype, self.page, self.kv_heads, self._index)
+        self._addr = ctypes.addressof(self._args)
 
     def advance(self, tokens: int = 1) -> None:
         """Every sequence has ``tokens`` more (up to ``grow`` in all): its new rows are the ``q_len`` last ones of the longer
@@ -286,23 +305,30 @@ def build_plan(cache: PagedCache, heads: int, q_lens, kv_lens, tables, limits=No
                      counts["rows"], int(arrays["k_start"][-1]), scratch, store[at["kv_len"]:at["kv_len"] + n], grow, store, args)
 
 
+_BF16 = torch.bfloat16
+
+
 def _check(cache: PagedCache, plan: PagedPlan) -> None:
-    if cache.data.dtype != plan.dtype or cache.page != plan.page or cache.kv_heads != plan.kv_heads or cache.pages < plan.pages or cache.device != plan.device:
-        raise ValueError("the plan was made for caches of another geometry or device")
+    if cache._key != plan._key or cache.pages < plan.pages:
+        raise ValueError("the plan was made for caches of another geometry, type or device")
 
 
-def _rows_ok(t, rows, heads, device) -> bool:
-    return (t.dtype is torch.bfloat16 and t.dim() == 3 and t.shape[0] >= rows and t.shape[1] == heads and t.shape[2] == HEAD_DIM
-            and t.stride(2) == 1 and t.stride(1) == HEAD_DIM and t.device == device)
+def _row_stride(name: str, t: torch.Tensor, plan: PagedPlan, heads: int) -> int:
+    """Elements from one row to the next of a [plan.rows or more, heads, 128] tensor."""
+    shape, stride = t.shape, t.stride()
+    if (len(shape) != 3 or shape[0] < plan.rows or shape[1] != heads or shape[2] != HEAD_DIM or stride[2] != 1 or stride[1] != HEAD_DIM
+            or t.dtype is not _BF16 or t.get_device() != plan._index):
+        raise ValueError(f"{name} must be bf16 [{plan.rows} or more, {heads}, {HEAD_DIM}] with contiguous heads on the plan's device")
+    return stride[0]
 
 
-def _call(device, name, *args) -> None:
+def _call(index: int, name: str, *args) -> None:
     """On the tensors' device, whichever is current."""
-    if device.index == torch._C._cuda_getDevice():
-        _lib.call(name, *args, c_void_p(_lib.stream()))
+    if index == torch._C._cuda_getDevice():
+        _lib.call(name, *args, _lib.stream())
     else:
-        with torch.cuda.device(device):
-            _lib.call(name, *args, c_void_p(_lib.stream()))
+        with torch.cuda.device(index):
+            _lib.call(name, *args, _lib.stream())
 
 
 def paged_write(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, plan: PagedPlan) -> None:
@@ -311,20 +337,18 @@ def paged_write(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, plan: Paged
     row is scaled so that its largest value is 448, the largest e4m3 value; one that holds a value that is not finite
     reads back as NaN."""
     _check(cache, plan)
-    if not (_rows_ok(k, plan.rows, cache.kv_heads, plan.device) and _rows_ok(v, plan.rows, cache.kv_heads, plan.device)):
-        raise ValueError(f"k and v must be bf16 [{plan.rows} or more, {cache.kv_heads}, 128] with contiguous heads on the plan's device")
+    ldk, ldv = _row_stride("k", k, plan, cache.kv_heads), _row_stride("v", v, plan, cache.kv_heads)
     if plan.rows:
-        _call(plan.device, "paged_write", cache._desc, ctypes.byref(plan._args), c_void_p(k.data_ptr()), c_ll(k.stride(0)),
-              c_void_p(v.data_ptr()), c_ll(v.stride(0)))
+        _call(plan._index, "paged_write", cache._addr, plan._addr, k.data_ptr(), ldk, v.data_ptr(), ldv)
 
 
 def paged_read(cache: PagedCache, plan: PagedPlan) -> tuple[torch.Tensor, torch.Tensor]:
     """The cached keys and values of the plan's sequences, one sequence after another: two tensors [plan.keys, kv_heads, 128] bf16
     (e4m3: code times scale, rounded once)."""
     _check(cache, plan)
-    k, v = (torch.empty(plan.keys, cache.kv_heads, HEAD_DIM, dtype=torch.bfloat16, device=plan.device) for _ in range(2))
+    k, v = (torch.empty(plan.keys, cache.kv_heads, HEAD_DIM, dtype=_BF16, device=plan.device) for _ in range(2))
     if plan.keys:
-        _call(plan.device, "paged_read", cache._desc, ctypes.byref(plan._args), c_void_p(k.data_ptr()), c_void_p(v.data_ptr()))
+        _call(plan._index, "paged_read", cache._addr, plan._addr, k.data_ptr(), v.data_ptr())
     return k, v
 
 
@@ -333,14 +357,14 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, plan: PagedPlan, scale: 
     128] bf16, rows may be slices of wider ones; returns ``out`` (default: new, [plan.rows, heads, 128]), whose rows behind
     the last sequence are left as they are."""
     _check(cache, plan)
-    if not _rows_ok(q, plan.rows, plan.heads, plan.device):
-        raise ValueError(f"q must be bf16 [{plan.rows} or more, {plan.heads}, 128] with contiguous heads on the plan's device")
+    ldq = _row_stride("q", q, plan, plan.heads)
     if out is None:
-        out = torch.empty(plan.rows, plan.heads, HEAD_DIM, dtype=torch.bfloat16, device=plan.device)
-    elif not _rows_ok(out, plan.rows, plan.heads, plan.device):
-        raise ValueError(f"out must be bf16 [{plan.rows} or more, {plan.heads}, 128] with contiguous heads on the plan's device")
+        out = torch.empty(plan.rows, plan.heads, HEAD_DIM, dtype=_BF16, device=plan.device)
+        ldo = plan.heads * HEAD_DIM
+    else:
+        ldo = _row_stride("out", out, plan, plan.heads)
     if plan.rows:
         scratch = torch.empty(plan.scratch, dtype=torch.uint8, device=plan.device) if plan.scratch else None
-        _call(plan.device, "paged_attention", cache._desc, ctypes.byref(plan._args), c_void_p(q.data_ptr()), c_ll(q.stride(0)),
-              c_void_p(out.data_ptr()), c_ll(out.stride(0)), c_float(scale), c_void_p(None if scratch is None else scratch.data_ptr()))
+        _call(plan._index, "paged_attention", cache._addr, plan._addr, q.data_ptr(), ldq, out.data_ptr(), ldo, scale,
+              scratch.data_ptr() if plan.scratch else None)
     return out
