@@ -163,13 +163,14 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     }
   }
   __syncthreads();
-  const int most = max(lim_max[0], lim_max[1]);
+  const int max_a = lim_max[0], max_b = lim_max[1], min_a = lim_min[0], min_b = lim_min[1];
+  const int most = max(max_a, max_b);
   const int all = (most + BK - 1) / BK;
   const int j0 = (int)((long long)all * part / parts), n = (int)((long long)all * (part + 1) / parts) - j0;
   // how a row tile reads key tile j of this part: not at all, in part, whole
   auto cls = [&](int j, int t) -> int {
     const int k0 = (j0 + j) * BK;
-    return k0 >= lim_max[t] ? kTileSkip : k0 + BK <= lim_min[t] ? kTileFull : kTilePartial;
+    return k0 >= (t ? max_b : max_a) ? kTileSkip : k0 + BK <= (t ? min_b : min_a) ? kTileFull : kTilePartial;
   };
   auto dirty = [&](int j) -> bool { return !FP8 && (cls(j, 0) == kTilePartial || cls(j, 1) == kTilePartial); };
   // columns: S_A and P_B [0,128), S_B and P_A [128,256), O_A [256,384), O_B [384,512)
