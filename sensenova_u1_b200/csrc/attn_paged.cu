@@ -17,14 +17,15 @@
 // times the power of two that brings its largest value to [2^13, 2^14): values down to 2^-27 of the largest keep all their
 // bits, and what smaller ones lose is below the rounding of the fp32 sum.  The scale of a key goes into its score.  The
 // scale of a value goes into its probability, in the exponent: p' = exp2(s + log2(scale) - m') with a maximum of its own,
-// so that the fp16 probabilities of the product are relative to the largest p' whatever sizes the values have (2^-11 each;
-// bf16 caches: bf16 probabilities, 2^-8).  The sum of the probabilities is taken in fp32 from p itself.
+// so that the fp16 probabilities of the product are relative to the largest p' whatever sizes the values have (the largest
+// is brought to 2^7, so that one is only lost below 2^-32 of it; rounding 2^-11 each; bf16 caches: bf16 probabilities, 2^-8).  The sum of the probabilities is taken in fp32 from p itself.
 //
 // Masked places: scores of keys at or beyond a row's limit are -inf whatever the cache holds, and places that no row of the
 // tile may read are cleared in shared memory.  A probability of zero does not hide an infinite or NaN value from the
 // matrix product, so in a tile that some row may not read whole, bf16 values that are not finite are cleared too and the
 // first key that held one is kept: rows that may read it give NaN, the others are as if it were not there.  (e4m3 codes are
 // finite; what is not finite there is the row's scale, and that is only used where the mask allows.)
+#include <math.h>
 #include <string.h>
 
 #include <mutex>
@@ -87,11 +88,6 @@ __device__ __forceinline__ uint32_t widen_lo(uint32_t w) {
 __device__ __forceinline__ uint32_t widen_hi(uint32_t w) {
   uint32_t r;
   asm("{\n.reg .b16 l, h;\nmov.b32 {l, h}, %1;\ncvt.rn.f16x2.e4m3x2 %0, h;\n}" : "=r"(r) : "r"(w));
-  return r;
-}
-__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
 __device__ __forceinline__ float fast_log2(float x) {
@@ -417,7 +413,7 @@ __global__ void __launch_bounds__(FEW_THREADS, NR == 1 ? 3 : 2)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             mu[e] = m[i][e] == -INFINITY ? 0.f : m[i][e];
-            muv[e] = FP8 && mv[i][e] != -INFINITY ? mv[i][e] : 0.f;
+            muv[e] = FP8 && mv[i][e] != -INFINITY ? mv[i][e] - P_TOP : 0.f;
           }
 #pragma unroll
           for (int nb = 0; nb < NB; ++nb) {
@@ -481,7 +477,7 @@ __global__ void __launch_bounds__(FEW_THREADS, NR == 1 ? 3 : 2)
         if (!FP8 && lim[i][e] > s_poison) l[i][e] = __int_as_float(0x7fffffff);
         if (l[i][e] != l[i][e] && m[i][e] == -INFINITY) m[i][e] = 0.f;       // all NaN: not to be taken for no keys at all
         // acc relative to the scores' maximum
-        const float f = !FP8 || mv[i][e] == -INFINITY ? 1.f : exp2f(mv[i][e] - m[i][e]);
+        const float f = !FP8 || mv[i][e] == -INFINITY ? 1.f : exp2f(mv[i][e] - P_TOP - m[i][e]);
         const int row = i * 8 + 2 * c + e;
         if (g == 0) {
           s_m[warp][row] = m[i][e];
@@ -607,7 +603,8 @@ static int launch_few(const Cache& c, const Plan& p, const FewArgs& a, cudaStrea
 using namespace snu1;
 
 // o_r = attention of row r over its sequence's first keys, rows [rows][heads of queries][128] bf16, ldq / ldo apart.
-// scratch: partial results (partial_rows x heads x (128 values, maximum, sum) in fp32), then unpack_pages bf16 pages of 128 tokens.
+// scratch: partial results (partial_rows x heads x (128 values, maximum, sum) in fp32), then unpack_count
+// fp16 pages of 128 tokens and their factors (a float2 per page and head).
 SNU1_API int snu1_paged_attention(const void* cache, const void* plan, const void* q, long long ldq, void* o, long long ldo,
                                   float scale, void* scratch, void* stream) {
   using namespace paged;
@@ -622,6 +619,10 @@ SNU1_API int snu1_paged_attention(const void* cache, const void* plan, const voi
     return kHostBadArg;
   }
   FewArgs a;
+  if (!(scale > 0.f) || isinf(scale)) {
+    set_last_error("paged_attention: the scale must be a positive number");
+    return kHostBadArg;
+  }
   a.q = (const __nv_bfloat16*)q;
   a.o = (__nv_bfloat16*)o;
   a.ldq = ldq;
@@ -636,8 +637,9 @@ SNU1_API int snu1_paged_attention(const void* cache, const void* plan, const voi
   int rc = kHostOk;
   if (p.chunk_count > 0) {
     void* wide = a.part_ml + (((long long)p.partial_rows * c.heads + 15) & ~15ll);      // 128-byte aligned
-    if (c.fp8 && (rc = launch_widen(c, p, wide, st)) != kHostOk) return rc;
-    if ((rc = launch_chunks(c, p, q, ldq, p.rows, o, ldo, a.part, a.part_ml, a.scale_log2, wide, st)) != kHostOk) return rc;
+    float2* factors = (float2*)((uint8_t*)wide + 2ll * 128 * HEAD * 2 * p.unpack_count * c.heads);
+    if (c.fp8 && (rc = launch_widen(c, p, wide, factors, st)) != kHostOk) return rc;
+    if ((rc = launch_chunks(c, p, q, ldq, p.rows, o, ldo, a.part, a.part_ml, a.scale_log2, wide, factors, st)) != kHostOk) return rc;
   }
   if (p.few_count > 0) {
     if (c.fp8) rc = launch_few<true>(c, p, a, st);

@@ -6,13 +6,17 @@
 // What is different:
 // * A row tile holds all query heads of one key/value head: 128 / group tokens, head after head (one TMA box from q).  A
 //   chunk of a few dozen tokens fills the tensor cores' 128 rows, and the heads of a group read keys and values once.
-// * Keys and values come page by page (a lane of the loading warp per page).  e4m3 codes are widened into bf16 pages of scratch
-//   first (paged_read_kernel), which is exact; the scales are applied in fp32, a key's to its scores, a value's to its
-//   probabilities (rounding code times scale to bf16 instead would shift every score by up to 2^-8 of the sum of |q k|).
+// * Keys and values come page by page (a lane of the loading warp per page).  An e4m3 cache is widened to fp16 pages of scratch
+//   first (paged_widen_kernel: code times scale, divided by one power of two per tile and head), and queries and probabilities
+//   are fp16 as well.  So the softmax pays for the scales once per tile and row, not per score: the keys' power of two goes
+//   into the factor of the scores, the values' into the exponent of the probabilities (and out of their sum).  Scales
+//   applied per score and probability in fp32 took 2.33 us per pair of tiles instead of 1.78 (2 x 512 new tokens, 8192 keys);
+//   keys rounded to bf16 would move every score by up to 2^-8 of the sum of |q k|.  The queries are scaled row by row as in
+//   attn_paged.cu, by the softmax warps.
 // * The mask is one number per row, the keys that it may read; tiles that all rows read whole need no test.
 // * A work item is a part of the key tiles of two row tiles; unnormalised results of parts are joined by
 //   paged_merge_kernel.  ops/paged.py chooses the parts so that the waves of CTAs are full.
-// * Two warps that have nothing else to do bring the scales of an e4m3 cache, and otherwise clear values that are not finite (and rows behind the last token) in the tiles that
+// * Two warps that have nothing else to do clear values that are not finite (and rows behind the last token) in the tiles that
 //   some row may not read whole: a probability of zero does not hide them from the product.  Rows that may read such a
 //   value give NaN, the others are as if it were not there.
 #include <string.h>
@@ -30,8 +34,7 @@ constexpr int CHALF = 128 * 64 * 2;             // 64 columns of a 128-row tile
 constexpr int CTILE = 2 * CHALF;
 constexpr int CK_STAGES = 3, CV_STAGES = 2;
 constexpr int CHUNK_THREADS = 640;
-constexpr int CS_STAGES = 2;                    // scales of a tile: 128 keys', then 128 values'
-constexpr int CHUNK_SMEM = (2 + CK_STAGES + CV_STAGES) * CTILE + CS_STAGES * 1024 + 512;
+constexpr int CHUNK_SMEM = (2 + CK_STAGES + CV_STAGES) * CTILE + 512 + 1024;
 
 struct ChunkArgs {
   __nv_bfloat16* o;
@@ -39,8 +42,8 @@ struct ChunkArgs {
   float* part;
   float2* part_ml;
   const int* first_page;   // scratch of widened rows: a sequence's first page there; null: the cache's own pages
-  const float* scales;     // of an e4m3 cache, whose pages (scale_page tokens) the table names
-  int page, pages, heads, scale_page, scale_pages;
+  const float2* factors;   // of the widened pages: the keys' power of two, the exponent of the values'
+  int page, pages, heads;
   float scale_log2;
   int* status;
 };
@@ -73,17 +76,12 @@ template <bool FP8>
 __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                        const __grid_constant__ CUtensorMap tm_v, const Plan p, const ChunkArgs args) {
-  // no room to align it by hand: there is no other shared memory, so it starts on a boundary of 1024 bytes
-  extern __shared__ __align__(1024) uint8_t smem_chunk[];
-  if ((smem_u32(smem_chunk) & 1023) != 0) {
-    if (threadIdx.x == 0) report_status(args.status, kBadShape, 10);
-    return;
-  }
-  uint8_t* sQ = smem_chunk;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* sQ = smem;
   uint8_t* sK = sQ + 2 * CTILE;
   uint8_t* sV = sK + CK_STAGES * CTILE;
-  float* s_scale = reinterpret_cast<float*>(sV + CV_STAGES * CTILE);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(s_scale + CS_STAGES * 256);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sV + CV_STAGES * CTILE);
   uint64_t* q_full = bars;
   uint64_t* k_full = bars + 1;
   uint64_t* k_empty = k_full + CK_STAGES;
@@ -95,9 +93,8 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
   uint64_t* s_empty = s_full + 2;
   uint64_t* p_full = s_empty + 2;
   uint64_t* pv_done = p_full + 2;
-  uint64_t* sc_full = pv_done + 2;              // [CS_STAGES]
-  uint64_t* sc_empty = sc_full + CS_STAGES;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sc_empty + CS_STAGES);
+  uint64_t* q_ready = pv_done + 2;              // e4m3: the queries are fp16
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_ready + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* drained = reinterpret_cast<int*>(tmem_slot + 2);   // [2] softmax warps that have read a score tile, all tiles so far
   int* lim_max = drained + 2;                              // [2] the largest and the smallest limit of a row tile
@@ -117,10 +114,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
       mbar_init(&v_dirty[i], 1);
       mbar_init(&v_clean[i], 2);
     }
-    for (int i = 0; i < CS_STAGES; ++i) {
-      mbar_init(&sc_full[i], 2);
-      mbar_init(&sc_empty[i], 16);
-    }
+    mbar_init(q_ready, 16);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&s_empty[i], 8);
@@ -167,12 +161,10 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
   const int most = max(max_a, max_b);
   const int all = (most + BK - 1) / BK;
   const int j0 = (int)((long long)all * part / parts), n = (int)((long long)all * (part + 1) / parts) - j0;
-  // how a row tile reads key tile j of this part: not at all, in part, whole
-  auto cls = [&](int j, int t) -> int {
-    const int k0 = (j0 + j) * BK;
-    return k0 >= (t ? max_b : max_a) ? kTileSkip : k0 + BK <= (t ? min_b : min_a) ? kTileFull : kTilePartial;
-  };
-  auto dirty = [&](int j) -> bool { return !FP8 && (cls(j, 0) == kTilePartial || cls(j, 1) == kTilePartial); };
+  // Row tile A (B) reads the part's first n_a (n_b) key tiles, all but the first full_a (full_b) of them with the mask.
+  const int n_a = max(0, min(n, (max_a + BK - 1) / BK - j0)), n_b = max(0, min(n, (max_b + BK - 1) / BK - j0));
+  const int full_a = min_a / BK - j0, full_b = min_b / BK - j0;
+  auto dirty = [&](int j) -> bool { return (j < n_a && j >= full_a) || (j < n_b && j >= full_b); };
   // columns: S_A and P_B [0,128), S_B and P_A [128,256), O_A [256,384), O_B [384,512)
 
   // 640 threads start with 96 registers: 128 x 64 + 512 x 104 = 640 x 96
@@ -233,17 +225,18 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     } else if (warp == 1) {
       // The whole warp walks the tiles and one elected lane issues (see mbar_ready in attn_common.cuh).
       if (n > 0) {
-        constexpr uint32_t idesc_s = make_idesc_bf16(128, 128, false, false);
-        constexpr uint32_t idesc_pv = make_idesc_bf16(128, 128, false, true);
+        // bits [7,10) and [10,13) of the descriptor: bf16 (1) or fp16 (0) operands
+        constexpr uint32_t type = FP8 ? ~(1u << 7 | 1u << 10) : ~0u;
+        constexpr uint32_t idesc_s = make_idesc_bf16(128, 128, false, false) & type;
+        constexpr uint32_t idesc_pv = make_idesc_bf16(128, 128, false, true) & type;
         const uint64_t q_desc = make_smem_desc(smem_u32(sQ), 0, 1024);
         const uint64_t k_desc = make_smem_desc(smem_u32(sK), 0, 1024);
         const uint64_t v_desc = make_smem_desc(smem_u32(sV), CHALF, 1024);
-        bool ok = mbar_wait(q_full, 0, abort_flag, args.status, 3);   // this lane's; see mbar_wait_warp
-        int s_cnt[2] = {0, 0}, pv_cnt[2] = {0, 0};
+        bool ok = mbar_wait(FP8 ? q_ready : q_full, 0, abort_flag, args.status, 3);   // this lane's; see mbar_wait_warp
         uint32_t cleaned = 0;                   // phase of every stage's v_clean
         auto issue_s = [&](int j, int t) {
-          if (cls(j, t) != kTileSkip) {
-            ok &= mbar_wait(&s_empty[t], (s_cnt[t] & 1) ^ 1, abort_flag, args.status, 2);
+          if (j < (t ? n_b : n_a)) {
+            ok &= mbar_wait(&s_empty[t], (j & 1) ^ 1, abort_flag, args.status, 2);
             tc_fence_after();
             const uint64_t qd = q_desc + t * (CTILE >> 4), kd = k_desc + (j % CK_STAGES) * (CTILE >> 4);
             __syncwarp();
@@ -257,16 +250,15 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
               umma_commit(&s_full[t]);
             }
             __syncwarp();
-            ++s_cnt[t];
           }
         };
         auto issue_pv = [&](int j, int t) {
-          if (cls(j, t) != kTileSkip) {
-            ok &= mbar_wait(&p_full[t], pv_cnt[t] & 1, abort_flag, args.status, 2);
+          if (j < (t ? n_b : n_a)) {
+            ok &= mbar_wait(&p_full[t], j & 1, abort_flag, args.status, 2);
             tc_fence_after();
             const uint64_t vd = v_desc + (j % CV_STAGES) * (CTILE >> 4);
             const uint32_t p_tmem = tmem_base + (t ^ 1) * 128;
-            const uint32_t acc0 = pv_cnt[t] > 0 ? 1u : 0u;
+            const uint32_t acc0 = j > 0 ? 1u : 0u;
             __syncwarp();
             if (elect_one()) {
 #pragma unroll
@@ -275,7 +267,6 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
               umma_commit(&pv_done[t]);
             }
             __syncwarp();
-            ++pv_cnt[t];
           }
         };
         auto release = [&](uint64_t* bar) {
@@ -310,49 +301,6 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
           }
         }
       }
-    } else if (FP8) {
-      // ------------------------------ scales --------------------------------
-      // A thread brings those of two keys, in registers a tile ahead.  Those of values that are not finite are cleared in tiles
-      // that some row may not read whole, as the values of a bf16 cache are.
-      const int tid = threadIdx.x - 64;
-      const int* table = p.table + (long long)b * p.width;
-      const long long to_values = (long long)args.heads * args.scale_page;
-      float2 ks, vs;
-      auto fetch = [&](int j) {
-        ks = vs = make_float2(0.f, 0.f);
-        const int key = (j0 + j) * BK + 2 * tid;
-        if (j < n && key < kv_len) {
-          const int pg = table[key / args.scale_page];
-          if (pg >= 0 && pg < args.scale_pages) {
-            const float* at = args.scales + ((long long)pg * 2 * args.heads + kvh) * args.scale_page + key % args.scale_page;
-            ks = *reinterpret_cast<const float2*>(at);
-            vs = *reinterpret_cast<const float2*>(at + to_values);
-          }
-        }
-      };
-      fetch(0);
-      bool ok = true;
-      for (int j = 0; j < n && ok; ++j) {
-        const int s = j % CS_STAGES, key = (j0 + j) * BK + 2 * tid;
-        ok = mbar_wait_warp(&sc_empty[s], ((j / CS_STAGES) & 1) ^ 1, abort_flag, args.status, 3);
-        if (!ok) break;
-        if (key + 1 >= kv_len) ks.y = vs.y = 0.f;
-        if (cls(j, 0) == kTilePartial || cls(j, 1) == kTilePartial) {
-          if (!(fabsf(vs.y) < INFINITY)) {
-            atomicMin(poison, key + 1);
-            vs.y = 0.f;
-          }
-          if (!(fabsf(vs.x) < INFINITY)) {
-            atomicMin(poison, key);
-            vs.x = 0.f;
-          }
-        }
-        *reinterpret_cast<float2*>(s_scale + s * 256 + 2 * tid) = ks;
-        *reinterpret_cast<float2*>(s_scale + s * 256 + 128 + 2 * tid) = vs;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sc_full[s]);
-        fetch(j + 1);
-      }
     } else {
       // ------------------------------ cleaning --------------------------------
       bool ok = true;
@@ -374,7 +322,8 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
           bool bad = false;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const bool lo = (w[e] & 0x7f80u) == 0x7f80u, hi = (w[e] & 0x7f800000u) == 0x7f800000u;
+            constexpr uint32_t ex = FP8 ? 0x7c00u : 0x7f80u;         // an exponent of all ones
+            const bool lo = (w[e] & ex) == ex, hi = (w[e] & ex << 16) == ex << 16;
             bad |= lo || hi;
             w[e] &= (lo ? 0xffff0000u : 0xffffffffu) & (hi ? 0xffffu : 0xffffffffu);
           }
@@ -408,26 +357,45 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
       const int row = base + (lane >> 2) + 8 * r, token = token0 + t * T + row / G;
       lim[r] = row < T * G && token < q_len ? row_limit(p, q0, q_len, kv_len, token) : -1;
     }
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-    const float sc = args.scale_log2;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};      // running maximum, log2 units
+    float sc[2] = {args.scale_log2, args.scale_log2};
     bool ok = true;
-    int cnt = 0;
-    // score tiles of the other row tile that are issued before PV_t(j): key tiles 0 .. j of B for A, 0 .. j + 1 of A for B
-    int other = t == 1 && n > 0 && cls(0, 0) != kTileSkip;
-    for (int j = 0; j < n; ++j) {        // all tiles also after a time-out, see mbar_wait_warp
-      other += t == 0 ? cls(j, 1) != kTileSkip : j + 1 < n && cls(j + 1, 0) != kTileSkip;
-      const int cls_t = cls(j, t);
-      const int cs = j % CS_STAGES;
-      const float* scale_k = s_scale + cs * 256 + q2;
-      if (cls_t == kTileSkip) {
-        if (FP8) {                           // not before the scales are there: an arrival counts for one tile
-          ok &= mbar_wait(&sc_full[cs], (j / CS_STAGES) & 1, abort_flag, args.status, 5);
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&sc_empty[cs]);
-        }
-        continue;
+    if (FP8 && n > 0) {
+      // this warp's 16 query rows to fp16, each times a power of two (see attn_paged.cu)
+      ok &= mbar_wait(q_full, 0, abort_flag, args.status, 5);
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int c = lane & 15;
+        uint4* at = reinterpret_cast<uint4*>(sOt + (c >> 3) * CHALF + swz128_offset(base + 2 * i + (lane >> 4), c & 7));
+        uint4 u = *at;
+        uint32_t* w = reinterpret_cast<uint32_t*>(&u);
+        uint32_t top = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top = max(top, max((w[e] << 16) & 0x7fffffffu, w[e] & 0x7fff0000u));
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const int ex = (int)(top >> 23) - 127, up = top == 0 || ex == 128 ? 0 : min(13 - ex, 120);
+        const float f = __int_as_float((127 + up) << 23);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          w[e] = pack_f16x2(__uint_as_float(w[e] << 16) * f, __uint_as_float(w[e] & 0xffff0000u) * f);
+        *at = u;
+        const int own = __shfl_sync(0xffffffffu, up, (lane >> 2 & 1) * 16);     // of row 2 i or 2 i + 1
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+          if (i == (lane >> 3) + 4 * r) sc[r] *= __int_as_float((127 - own) << 23);
       }
-      ok &= mbar_wait(&s_full[t], cnt & 1, abort_flag, args.status, 5);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_ready);
+    }
+    const float2* factors = FP8 ? args.factors + (long long)(args.first_page[b] + j0) * args.heads + kvh : nullptr;
+    const int mine = t ? n_b : n_a, full = t ? full_b : full_a;
+    for (int j = 0; j < mine; ++j) {        // all tiles also after a time-out, see mbar_wait_warp
+      float2 factor = make_float2(1.f, 0.f);      // of this tile's keys and values
+      if (FP8) factor = __ldg(factors + (long long)j * args.heads);
+      ok &= mbar_wait(&s_full[t], j & 1, abort_flag, args.status, 5);
       tc_fence_after();
       float sv[2][32];   // [columns 0-63, 64-127][4 i + 2 row + e]
       {
@@ -447,22 +415,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         mbar_arrive(&s_empty[t]);
         tally_add(&drained[t]);
       }
-      if (FP8) {
-        ok &= mbar_wait(&sc_full[cs], (j / CS_STAGES) & 1, abort_flag, args.status, 5);
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const uint64_t f = *reinterpret_cast<const uint64_t*>(scale_k + h * 64 + i * 8);
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-              float& x = sv[h][4 * i + 2 * r];
-              float& y = sv[h][4 * i + 2 * r + 1];
-              unpack_f32x2(mul_f32x2(pack_f32x2(x, y), f), x, y);
-            }
-          }
-      }
-      if (cls_t != kTileFull) {
+      if (j >= full) {
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           const int end = lim[r] - (j0 + j) * BK - q2;       // columns 8 i + e from here on are hidden
@@ -492,54 +445,54 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
       }
       // the running maximum moves only when it is outgrown by more than 2^8, see attn_infer_sm100.cu
-      const bool rescale = __any_sync(0xffffffffu, mx[0] * sc > m[0] * sc + 8.f || mx[1] * sc > m[1] * sc + 8.f);
+      float f[2];                            // scores in log2 units: s f
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        f[r] = FP8 ? sc[r] * factor.x : sc[r];
+        mx[r] = FP8 ? fmaf(mx[r], f[r], factor.y) : mx[r] * f[r];
+      }
+      const bool rescale = __any_sync(0xffffffffu, mx[0] > m[0] + 8.f || mx[1] > m[1] + 8.f);
       float alpha[2];
-      uint64_t nb2[2], acc[2][2];
+      uint64_t nb2[2], sc2[2], acc[2][2];
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         const float m_new = rescale ? fmaxf(m[r], mx[r]) : m[r];
         const float m_use = m_new == -INFINITY ? 0.f : m_new;
-        alpha[r] = rescale ? fast_exp2((m[r] - m_use) * sc) : 1.f;
+        alpha[r] = rescale ? fast_exp2(m[r] - m_use) : 1.f;
         m[r] = m_new;
-        nb2[r] = pack_f32x2(-m_use * sc, -m_use * sc);
+        const float nb = FP8 ? factor.y + P_TOP - m_use : -m_use;
+        nb2[r] = pack_f32x2(nb, nb);
+        sc2[r] = pack_f32x2(f[r], f[r]);
         acc[r][0] = acc[r][1] = 0ull;
       }
-      const uint64_t sc2 = pack_f32x2(sc, sc);
       uint32_t pk[32];      // probabilities, bf16 pairs: [2 (8-column group) + row]
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          uint64_t f = 0;
-          if (FP8) f = *reinterpret_cast<const uint64_t*>(scale_k + 128 + h * 64 + i * 8);
+        for (int i = 0; i < 8; ++i)
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
             float x, y;
-            unpack_f32x2(fma_f32x2(pack_f32x2(sv[h][4 * i + 2 * r], sv[h][4 * i + 2 * r + 1]), sc2, nb2[r]), x, y);
+            unpack_f32x2(fma_f32x2(pack_f32x2(sv[h][4 * i + 2 * r], sv[h][4 * i + 2 * r + 1]), sc2[r], nb2[r]), x, y);
             x = fast_exp2(x);
             y = fast_exp2(y);
-            const uint64_t xy = pack_f32x2(x, y);
-            acc[r][i & 1] = add_f32x2(acc[r][i & 1], xy);
-            if (FP8) unpack_f32x2(mul_f32x2(xy, f), x, y);
-            pk[16 * h + 2 * i + r] = pack_bf16x2(x, y);
+            acc[r][i & 1] = add_f32x2(acc[r][i & 1], pack_f32x2(x, y));
+            pk[16 * h + 2 * i + r] = FP8 ? pack_f16x2(x, y) : pack_bf16x2(x, y);
           }
-        }
-      if (FP8) {
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sc_empty[cs]);
-      }
+      const float out_of = FP8 ? fast_exp2(-factor.y) : 1.f;       // the sum is of probabilities, without the values' power of two
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         float s0, s1;
         unpack_f32x2(add_f32x2(acc[r][0], acc[r][1]), s0, s1);
-        l[r] = l[r] * alpha[r] + (s0 + s1);      // of this thread's columns; summed over the four threads at the end
+        l[r] = l[r] * alpha[r] + (s0 + s1) * out_of;      // of this thread's columns; summed over the four threads at the end
       }
-      if (cnt > 0) ok &= mbar_wait(&pv_done[t], (cnt - 1) & 1, abort_flag, args.status, 5);
-      // the other tile's warps have read the scores that P goes over
-      ok &= tally_wait(&drained[t ^ 1], 8 * other, abort_flag, args.status, 5);
+      if (j > 0) ok &= mbar_wait(&pv_done[t], (j - 1) & 1, abort_flag, args.status, 5);
+      // The other tile's warps have read the scores that P goes over: of the score tiles issued before PV_t(j), which are key tiles
+      // 0 .. j of B for A, 0 .. j + 1 of A for B.
+      ok &= tally_wait(&drained[t ^ 1], 8 * (t == 0 ? min(j + 1, n_b) : min(j + 2, n_a)), abort_flag, args.status, 5);
       tc_fence_after();
       tmem_st_16x128b_x16(tmem_P, pk);
-      if (cnt > 0 && rescale) {
+      if (j > 0 && rescale) {
         const uint64_t al0 = pack_f32x2(alpha[0], alpha[0]), al1 = pack_f32x2(alpha[1], alpha[1]);
 #pragma unroll 1
         for (int c = 0; c < 2; ++c) {
@@ -561,9 +514,8 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_full[t]);
-      ++cnt;
     }
-    if (cnt > 0) ok &= mbar_wait(&pv_done[t], (cnt - 1) & 1, abort_flag, args.status, 5);
+    if (mine > 0) ok &= mbar_wait(&pv_done[t], (mine - 1) & 1, abort_flag, args.status, 5);
     ok = __all_sync(0xffffffffu, ok);
     if (ok) {
       tc_fence_after();
@@ -577,7 +529,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         // Output rows leave through this warp's rows of the row tile's buffer (no product reads it any more), so that 16
         // lanes store one row's 256 bytes.
         const float inv[2] = {l[0] == 0.f ? 0.f : 1.f / l[0], l[1] == 0.f ? 0.f : 1.f / l[1]};
-        if (cnt > 0) {
+        if (mine > 0) {
 #pragma unroll 1
           for (int h = 0; h < 2; ++h) {
             uint32_t r[32];
@@ -599,14 +551,14 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
           const int r = base + 2 * i + (lane >> 4), c = lane & 15, token = token0 + t * T + r / G;
           if (r < T * G && token < q_len)
             *reinterpret_cast<uint4*>(args.o + (long long)(q0 + token) * args.ldo + (long long)(kvh * G + r % G) * HEAD + c * 8) =
-                cnt > 0 ? *reinterpret_cast<const uint4*>(sOt + (c >> 3) * CHALF + swz128_offset(r, c & 7)) : make_uint4(0, 0, 0, 0);
+                mine > 0 ? *reinterpret_cast<const uint4*>(sOt + (c >> 3) * CHALF + swz128_offset(r, c & 7)) : make_uint4(0, 0, 0, 0);
         }
       } else {
         const long long at0 = ((long long)item.w + t * T * G + base + (lane >> 2)) * args.heads + kvh;
 #pragma unroll 1
         for (int h = 0; h < 2; ++h) {
           uint32_t r[32];
-          if (cnt > 0) {
+          if (mine > 0) {
             tmem_ld_16x256b_x8(tmem_O + h * 64, r);
             tmem_ld_wait();
           } else {
@@ -627,7 +579,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
 #pragma unroll
           for (int e = 0; e < 2; ++e)
             if (lim[e] >= 0)        // scores that were all NaN are not to be taken for no keys at all
-              args.part_ml[at0 + 8ll * e * args.heads] = make_float2(m[e] == -INFINITY && l[e] != l[e] ? 0.f : m[e] * sc, l[e]);
+              args.part_ml[at0 + 8ll * e * args.heads] = make_float2(m[e] == -INFINITY && l[e] != l[e] ? 0.f : FP8 ? m[e] - P_TOP : m[e], l[e]);
         }
       }
     }
@@ -647,7 +599,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
 }
 
 int launch_chunks(const Cache& c, const Plan& p, const void* q, long long ldq, int q_rows, void* o, long long ldo, float* part,
-                  float2* part_ml, float scale_log2, void* wide, cudaStream_t st) {
+                  float2* part_ml, float scale_log2, void* wide, const float2* factors, cudaStream_t st) {
   const int G = p.group, T = 128 / G;
   CUtensorMap tm_q, tm_k = c.k, tm_v = c.v;
   int rc;
@@ -658,18 +610,18 @@ int launch_chunks(const Cache& c, const Plan& p, const void* q, long long ldq, i
   }
   ChunkArgs a;
   a.first_page = nullptr;
-  a.scales = c.scales;
-  a.page = a.scale_page = c.page;
-  a.pages = a.scale_pages = c.pages;
+  a.factors = factors;
+  a.page = c.page;
+  a.pages = c.pages;
   if (c.fp8) {
-    const uint64_t dims[4] = {128, 128, (uint64_t)c.heads, (uint64_t)p.unpack_pages};
+    const uint64_t dims[4] = {128, 128, (uint64_t)c.heads, (uint64_t)p.unpack_count};
     const uint64_t str[3] = {256, 256 * 128, 256ull * 128 * c.heads * 2};
     const uint32_t box[4] = {64, 128, 1, 1};
     if ((rc = encode_tmap(&tm_k, TmapType::kBf16, true, wide, 4, dims, str, box)) != kHostOk) return rc;
     if ((rc = encode_tmap(&tm_v, TmapType::kBf16, true, (uint8_t*)wide + 256ull * 128 * c.heads, 4, dims, str, box)) != kHostOk) return rc;
     a.first_page = p.unpack_first;
     a.page = 128;
-    a.pages = p.unpack_pages;
+    a.pages = p.unpack_count;
   }
   a.o = (__nv_bfloat16*)o;
   a.ldo = ldo;

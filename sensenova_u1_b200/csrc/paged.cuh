@@ -16,6 +16,8 @@ constexpr int HEAD = 128;                  // width of a head
 constexpr float E4M3_MAX = 448.f;
 constexpr float TINY = 7.70371977754894342e-34f;   // 2^-110, least row maximum that a scale is made of: 448 / TINY is finite
 
+constexpr float P_TOP = 7.f;               // fp16 probabilities: the largest is 2^7, or up to 2^15 while the running maximum is old
+
 // One layer's cache, filled by snu1_paged_cache_init.
 struct alignas(64) Cache {
   CUtensorMap kv;          // box: up to 128 tokens of one head, keys and values, of bf16 up to 64 and 64 values wide
@@ -36,7 +38,7 @@ struct Plan {
   const int* row_seq;      // [rows] sequence of a row
   const int* k_start;      // [seqs + 1] first packed row of a sequence, by the planned lengths
   const int2* read_pages;  // [read_count] (sequence, page of it) of all planned pages
-  const int2* unpack;      // [unpack_count] (sequence, page) of the e4m3 sequences that the chunk kernel handles, to full tiles of 128
+  const int2* unpack;      // [unpack_count] (sequence, tile of 128 tokens) of the e4m3 sequences that the chunk kernel handles
   const int* unpack_first; // [seqs] first page of such a sequence in the scratch for unpacked rows
   const int4* few;         // [few_count] work of the kernel for few rows: sequence, first row, part | parts << 16, partial row (-1: none)
   const int4* chunk;       // [chunk_count] the same for chunks
@@ -44,8 +46,7 @@ struct Plan {
   int seqs, rows, width, page, group;
   int read_count, few_count, few_rows, chunk_count, merge_count, merge_rows;
   int partial_rows;        // rows of the scratch for partial results (x heads)
-  int unpack_pages;        // 128-token pages of the scratch for unpacked e4m3 rows
-  int unpack_count;
+  int unpack_count;        // also the 128-token pages of the scratch for unpacked rows
 };
 
 __device__ __forceinline__ int seq_len(const Plan& p, int b) { return max(0, min(p.kv_len[b], p.cap[b])); }
@@ -56,6 +57,12 @@ __device__ __forceinline__ int row_limit(const Plan& p, int q0, int q_len, int k
   return max(0, min(kv_len, kv_len - behind));
 }
 
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
 __device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* m, uint64_t* bar, int x, int y, int z, int w, int u) {
   asm volatile(
       "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes "
@@ -64,11 +71,11 @@ __device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* m, 
       : "memory");
 }
 
-// paged_cache.cu: a plan's ``unpack`` pages of an e4m3 cache as bf16 pages of 128 tokens at ``wide``
-int launch_widen(const Cache& c, const Plan& p, void* wide, cudaStream_t st);
+// paged_cache.cu: a plan's ``unpack`` tiles of an e4m3 cache as fp16 pages at ``wide``
+int launch_widen(const Cache& c, const Plan& p, void* wide, float2* factors, cudaStream_t st);
 // attn_paged_sm100.cu: a plan's ``chunk`` items
 int launch_chunks(const Cache& c, const Plan& p, const void* q, long long ldq, int q_rows, void* o, long long ldo, float* part,
-                  float2* part_ml, float scale_log2, void* wide, cudaStream_t st);
+                  float2* part_ml, float scale_log2, void* wide, const float2* factors, cudaStream_t st);
 
 }  // namespace paged
 }  // namespace snu1

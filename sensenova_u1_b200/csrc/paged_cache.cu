@@ -18,6 +18,17 @@
 namespace snu1 {
 namespace paged {
 
+// eight codes as numbers
+__device__ __forceinline__ void decode8(uint2 u, float (&f)[8]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const __half2 h(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)((j < 2 ? u.x : u.y) >> (16 * (j & 1))), __NV_E4M3));
+    const float2 g = __half22float2(h);
+    f[2 * j] = g.x;
+    f[2 * j + 1] = g.y;
+  }
+}
+
 constexpr int WRITE_THREADS = 256;
 constexpr int WRITE_TOKENS = 16;     // most tokens of a block
 constexpr int WRITE_DEEP = 4;        // (token, head) pairs that a warp has in flight
@@ -97,23 +108,20 @@ constexpr int READ_THREADS = 256;
 constexpr int READ_DEEP = 4;                                         // rows that a lane has in flight
 constexpr int READ_BLOCK = 256;                                      // rows of a block
 
-// Rows of the planned pages, in order.  PACKED: out = keys, out2 = values [rows][heads][128] at the plan's row numbers;
-// otherwise out = codes as bf16 (without their scales) in pages of 128 tokens in a cache's own layout, every sequence from a
-// page of its own on, rows behind its last token cleared (the attention kernel multiplies them by probabilities of zero).
-template <bool FP8, bool PACKED>
+// Rows of the planned pages, in order: keys to ``out``, values to ``out2``, [rows][heads][128].
+template <bool FP8>
 __global__ void __launch_bounds__(READ_THREADS)
     paged_read_kernel(const uint8_t* __restrict__ data, const float* __restrict__ scales, int pages, int heads, int page, Plan p,
                       __nv_bfloat16* __restrict__ out, __nv_bfloat16* __restrict__ out2, int* status) {
   pdl_wait();
   pdl_trigger();
-  const int2 e = (PACKED ? p.read_pages : p.unpack)[blockIdx.x];
+  const int2 e = p.read_pages[blockIdx.x];
   const int page_log = __ffs(page) - 1;
   const int b = e.x, pos0 = e.y * page, c = threadIdx.x & 15;
-  const int k0 = p.k_start[b];
-  const int len = PACKED ? p.k_start[b + 1] - k0 : seq_len(p, b);
-  const int pg = pos0 < len ? p.table[(long long)b * p.width + e.y] : 0;
-  const bool there = pos0 < len && pg >= 0 && pg < pages;
-  if (pos0 < len && !there && threadIdx.x == 0) report_status(status, kBadPage, 9);
+  const int k0 = p.k_start[b], len = p.k_start[b + 1] - k0;
+  const int pg = p.table[(long long)b * p.width + e.y];
+  const bool there = pg >= 0 && pg < pages;
+  if (!there && threadIdx.x == 0) report_status(status, kBadPage, 9);
   const int total = 2 * heads * page, end = min(total, (int)(blockIdx.y + 1) * READ_BLOCK);
   for (int first = blockIdx.y * READ_BLOCK + (threadIdx.x >> 4); first < end; first += READ_THREADS / 16 * READ_DEEP) {
     uint4 x[READ_DEEP];
@@ -129,7 +137,7 @@ __global__ void __launch_bounds__(READ_THREADS)
           const uint2 u = *reinterpret_cast<const uint2*>(data + at * HEAD + c * 8);
           x[i].x = u.x;
           x[i].y = u.y;
-          s[i] = PACKED ? scales[at] : 1.f;
+          s[i] = scales[at];
         } else {
           x[i] = *reinterpret_cast<const uint4*>(data + at * (HEAD * 2) + c * 16);
         }
@@ -139,36 +147,90 @@ __global__ void __launch_bounds__(READ_THREADS)
     for (int i = 0; i < READ_DEEP; ++i) {
       const int r = first + i * (READ_THREADS / 16);
       const int pos = pos0 + (r & (page - 1)), kvh = r >> page_log, kv = kvh >= heads, head = kvh - kv * heads;
-      if (r >= end || (PACKED && pos >= len)) continue;
+      if (r >= end || pos >= len) continue;
       uint4 y = x[i];
       if (FP8) {
-        const uint32_t u[2] = {x[i].x, x[i].y};
-        uint32_t w[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const __half2 h(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(u[j >> 1] >> (16 * (j & 1))), __NV_E4M3));
-          const float2 f = __half22float2(h);
-          w[j] = pack_bf16x2(f.x * s[i], f.y * s[i]);
-        }
-        y = make_uint4(w[0], w[1], w[2], w[3]);
+        float f[8];
+        decode8(make_uint2(x[i].x, x[i].y), f);
+        y = make_uint4(pack_bf16x2(f[0] * s[i], f[1] * s[i]), pack_bf16x2(f[2] * s[i], f[3] * s[i]),
+                       pack_bf16x2(f[4] * s[i], f[5] * s[i]), pack_bf16x2(f[6] * s[i], f[7] * s[i]));
       }
-      __nv_bfloat16* dst;
-      if (PACKED) {
-        dst = (kv ? out2 : out) + ((long long)(k0 + pos) * heads + head) * HEAD;
-      } else {
-        const long long t = (long long)p.unpack_first[b] * 128 + pos;
-        dst = out + (((t >> 7) * 2 * heads + kvh) * 128 + (t & 127)) * HEAD;
-      }
-      *reinterpret_cast<uint4*>(dst + c * 8) = y;
+      *reinterpret_cast<uint4*>((kv ? out2 : out) + ((long long)(k0 + pos) * heads + head) * HEAD + c * 8) = y;
     }
   }
 }
 
-int launch_widen(const Cache& c, const Plan& p, void* wide, cudaStream_t st) {
-  const int total = 2 * c.heads * c.page;
-  SNU1_CUDA_CHECK(launch_pdl(paged_read_kernel<true, false>, dim3(p.unpack_count, (total + READ_BLOCK - 1) / READ_BLOCK),
-                             dim3(READ_THREADS), 0, st, (const uint8_t*)c.data, (const float*)c.scales, c.pages, c.heads, c.page, p,
-                             (__nv_bfloat16*)wide, (__nv_bfloat16*)nullptr, device_status_word()));
+// Tiles of 128 tokens of an e4m3 cache for attn_paged_sm100.cu: fp16 pages of 128 tokens in a cache's own layout, every
+// sequence from a page of its own on, rows behind its last token cleared.  A tile of one head is divided by a power of two,
+// so that its largest value is at most 1 (2^-126 to 2^90; that factor goes into the scores, or into the probabilities): code times
+// scale is rounded to 11 bits, and what falls below fp16's normal range is 2^14 times smaller than the tile's largest value.
+// factors [page][heads]: the keys' power of two, and the exponent of the values'.
+constexpr int WIDEN_THREADS = 256;
+
+__global__ void __launch_bounds__(WIDEN_THREADS)
+    paged_widen_kernel(const uint8_t* __restrict__ data, const float* __restrict__ scales, int pages, int heads, Plan p,
+                       uint8_t* __restrict__ wide, float2* __restrict__ factors, int* status) {
+  __shared__ long long s_at[128];          // the token's row of the cache, -1: none
+  __shared__ float s_scale[128];
+  __shared__ float s_top[4];
+  pdl_wait();
+  pdl_trigger();
+  const int2 e = p.unpack[blockIdx.x];
+  const int kv = blockIdx.y >= heads, head = blockIdx.y - kv * heads, b = e.x, t = threadIdx.x;
+  const int len = seq_len(p, b);
+  if (t < 128) {
+    const int pos = e.y * 128 + t;
+    long long at = -1;
+    float s = 0.f;
+    if (pos < len) {
+      const int pg = p.table[(long long)b * p.width + pos / p.page];
+      if (pg >= 0 && pg < pages) {
+        at = (((long long)pg * 2 + kv) * heads + head) * p.page + pos % p.page;
+        s = scales[at];
+      } else {
+        report_status(status, kBadPage, 9);
+      }
+    }
+    s_at[t] = at;
+    s_scale[t] = s;
+    const uint32_t top = __reduce_max_sync(0xffffffffu, fabsf(s) < INFINITY ? __float_as_uint(fabsf(s)) : 0u);
+    if ((t & 31) == 0) s_top[t >> 5] = __uint_as_float(top);
+  }
+  __syncthreads();
+  const float top = E4M3_MAX * fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
+  const int ex = max(-90, min(126, (int)(__float_as_uint(top) >> 23) - 126));
+  const float down = __int_as_float((127 - ex) << 23);
+  const long long page = p.unpack_first[b] + e.y;
+  if (t == 0) {
+    float* f = reinterpret_cast<float*>(factors + page * heads + head);
+    f[kv] = kv ? (float)ex : __int_as_float((127 + ex) << 23);
+  }
+  const int c = t & 15;
+  uint2 x[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const long long at = s_at[(t >> 4) + 16 * i];
+    x[i] = at >= 0 ? *reinterpret_cast<const uint2*>(data + at * HEAD + c * 8) : make_uint2(0, 0);
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int row = (t >> 4) + 16 * i;
+    const float s = s_scale[row] * down;
+    float f[8];
+    decode8(x[i], f);
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const __half2 h = __floats2half2_rn(f[2 * j] * s, f[2 * j + 1] * s);
+      w[j] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    *reinterpret_cast<uint4*>(wide + (((page * 2 + kv) * heads + head) * 128 + row) * 256 + c * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+int launch_widen(const Cache& c, const Plan& p, void* wide, float2* factors, cudaStream_t st) {
+  SNU1_CUDA_CHECK(launch_pdl(paged_widen_kernel, dim3(p.unpack_count, 2 * c.heads), dim3(WIDEN_THREADS), 0, st, (const uint8_t*)c.data,
+                             (const float*)c.scales, c.pages, c.heads, p, (uint8_t*)wide, factors, device_status_word()));
   return kHostOk;
 }
 
@@ -250,7 +312,7 @@ SNU1_API int snu1_paged_read(const void* cache, const void* plan, void* k, void*
     return kHostBadArg;
   }
   const int total = 2 * c.heads * c.page;
-  auto kernel = c.fp8 ? paged::paged_read_kernel<true, true> : paged::paged_read_kernel<false, true>;
+  auto kernel = c.fp8 ? paged::paged_read_kernel<true> : paged::paged_read_kernel<false>;
   SNU1_CUDA_CHECK(launch_pdl(kernel, dim3(p.read_count, (total + paged::READ_BLOCK - 1) / paged::READ_BLOCK),
                              dim3(paged::READ_THREADS), 0, (cudaStream_t)stream, (const uint8_t*)c.data, c.scales, c.pages, c.heads,
                              c.page, p, (__nv_bfloat16*)k, (__nv_bfloat16*)v, device_status_word()));

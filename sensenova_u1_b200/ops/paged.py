@@ -108,7 +108,7 @@ class _Args(ctypes.Structure):
     _fields_ = ([(n, c_void_p) for n in ("q_start", "kv_len", "cap", "table", "behind", "row_seq", "k_start", "read_pages", "unpack",
                                          "unpack_first", "few", "chunk", "merge")]
                 + [(n, c_int) for n in ("seqs", "rows", "width", "page", "group", "read_count", "few_count", "few_rows", "chunk_count",
-                                        "merge_count", "merge_rows", "partial_rows", "unpack_pages", "unpack_count")])
+                                        "merge_count", "merge_rows", "partial_rows", "unpack_count")])
 
 
 @dataclass
@@ -225,17 +225,16 @@ def _lay_out(q_lens, kv_lens, tables, page: int, pages: int, group: int, kv_head
         tiles = -(-kv[seq] // CHUNK_TILE)
     chunk, more, partial = _items(seq, row0, tiles, _waves(tiles, kv_heads, CHUNK_SLOTS), chunk_rows, partial)
     unpack = unpack_first = None
-    unpack_pages = 0
     if fp8 and len(chunk):
         wide = np.where(chunked, -(-cap // CHUNK_TILE), 0)    # 128-token pages
-        unpack, unpack_first, unpack_pages = pages_of(wide * (CHUNK_TILE // page)), start(wide)[:n], int(wide.sum())
+        unpack, unpack_first = pages_of(wide), start(wide)[:n]
     merge = np.concatenate([merge, more])
     arrays = dict(q_start=start(q), kv_len=kv.astype(np.int32), cap=cap.astype(np.int32), table=table, behind=behind, row_seq=row_seq,
                   k_start=start(kv), read_pages=pages_of(read), unpack=unpack, unpack_first=unpack_first, few=few, chunk=chunk,
                   merge=merge)
     counts = dict(seqs=n, rows=rows, width=width, page=page, group=group, read_count=int(read.sum()), few_count=len(few),
                   few_rows=few_rows, chunk_count=len(chunk), merge_count=len(merge), merge_rows=chunk_rows if len(more) else few_rows,
-                  partial_rows=partial, unpack_pages=unpack_pages, unpack_count=0 if unpack is None else len(unpack))
+                  partial_rows=partial, unpack_count=0 if unpack is None else len(unpack))
     return arrays, counts
 
 
@@ -299,7 +298,7 @@ def build_plan(cache: PagedCache, heads: int, q_lens, kv_lens, tables, limits=No
     args = _Args(**{name: store.data_ptr() + 4 * o for name, o in at.items()}, **counts)
     n = counts["seqs"]
     joined = counts["partial_rows"] * cache.kv_heads
-    scratch = joined * HEAD_DIM * 4 + (joined + 15) // 16 * 128 + counts["unpack_pages"] * 2 * cache.kv_heads * CHUNK_TILE * HEAD_DIM * 2
+    scratch = joined * HEAD_DIM * 4 + (joined + 15) // 16 * 128 + counts["unpack_count"] * cache.kv_heads * (2 * CHUNK_TILE * HEAD_DIM * 2 + 8)
     return PagedPlan(heads, cache.kv_heads, cache.page, cache.pages, cache.data.dtype, cache.device,
                      [int(x) for x in q_lens], [int(x) for x in kv_lens],
                      counts["rows"], int(arrays["k_start"][-1]), scratch, store[at["kv_len"]:at["kv_len"] + n], grow, store, args)
@@ -355,7 +354,7 @@ def paged_read(cache: PagedCache, plan: PagedPlan) -> tuple[torch.Tensor, torch.
 def paged_attention(q: torch.Tensor, cache: PagedCache, plan: PagedPlan, scale: float, out: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of the plan's new rows over their sequences' cached keys, softmax in fp32.  ``q``: [at least plan.rows, heads,
     128] bf16, rows may be slices of wider ones; returns ``out`` (default: new, [plan.rows, heads, 128]), whose rows behind
-    the last sequence are left as they are."""
+    the last sequence are left as they are.  ``scale`` is positive."""
     _check(cache, plan)
     ldq = _row_stride("q", q, plan, plan.heads)
     if out is None:

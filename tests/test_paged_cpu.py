@@ -94,8 +94,8 @@ def test_every_row_meets_every_key_once(q, kv, group, heads):
             assert m <= c["merge_rows"]
     if c["unpack_count"]:                                             # every key of a chunk's sequence has its place
         wide = [-(-k // 128) if any(b == i for b, *_ in a["chunk"].tolist()) else 0 for i, k in enumerate(kv)]
-        assert c["unpack_pages"] == sum(wide) and a["unpack_first"].tolist() == [sum(wide[:i]) for i in range(n)]
-        assert a["unpack"].tolist() == [[i, y] for i in range(n) for y in range(wide[i] * (128 // page))]
+        assert c["unpack_count"] == sum(wide) and a["unpack_first"].tolist() == [sum(wide[:i]) for i in range(n)]
+        assert a["unpack"].tolist() == [[i, y] for i in range(n) for y in range(wide[i])]
 
 
 def test_parts_fill_one_wave():
