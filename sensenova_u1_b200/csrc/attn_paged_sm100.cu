@@ -72,6 +72,35 @@ __device__ __forceinline__ bool tally_wait(const int* c, int target, volatile in
   }
 }
 
+// The products with descriptors given by their lower words (the upper word is the same for all tiles here): the issuing
+// warp has 64 registers, and pairs of them per product do not fit.
+constexpr uint32_t DESC_HI = (1024u >> 4) | 1u << 14 | 2u << 29;     // see make_smem_desc
+__device__ __forceinline__ void umma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      ".reg .b64 da, db;\n"
+      "setp.ne.b32 p, %4, 0;\n"
+      "mov.b64 da, {%1, %5};\n"
+      "mov.b64 db, {%2, %5};\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n"
+      "}\n" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "r"(DESC_HI)
+      : "memory");
+}
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      ".reg .b64 db;\n"
+      "setp.ne.b32 p, %4, 0;\n"
+      "mov.b64 db, {%2, %5};\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n"
+      "}\n" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "r"(DESC_HI)
+      : "memory");
+}
+
 template <bool FP8>
 __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
@@ -229,23 +258,23 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         constexpr uint32_t type = FP8 ? ~(1u << 7 | 1u << 10) : ~0u;
         constexpr uint32_t idesc_s = make_idesc_bf16(128, 128, false, false) & type;
         constexpr uint32_t idesc_pv = make_idesc_bf16(128, 128, false, true) & type;
-        const uint64_t q_desc = make_smem_desc(smem_u32(sQ), 0, 1024);
-        const uint64_t k_desc = make_smem_desc(smem_u32(sK), 0, 1024);
-        const uint64_t v_desc = make_smem_desc(smem_u32(sV), CHALF, 1024);
+        const uint32_t q_desc = (uint32_t)make_smem_desc(smem_u32(sQ), 0, 1024);
+        const uint32_t k_desc = (uint32_t)make_smem_desc(smem_u32(sK), 0, 1024);
+        const uint32_t v_desc = (uint32_t)make_smem_desc(smem_u32(sV), CHALF, 1024);
         bool ok = mbar_wait(FP8 ? q_ready : q_full, 0, abort_flag, args.status, 3);   // this lane's; see mbar_wait_warp
         uint32_t cleaned = 0;                   // phase of every stage's v_clean
         auto issue_s = [&](int j, int t) {
           if (j < (t ? n_b : n_a)) {
             ok &= mbar_wait(&s_empty[t], (j & 1) ^ 1, abort_flag, args.status, 2);
             tc_fence_after();
-            const uint64_t qd = q_desc + t * (CTILE >> 4), kd = k_desc + (j % CK_STAGES) * (CTILE >> 4);
+            const uint32_t qd = q_desc + t * (CTILE >> 4), kd = k_desc + (j % CK_STAGES) * (CTILE >> 4);
             __syncwarp();
             if (elect_one()) {
 #pragma unroll
               for (int k = 0; k < 8; ++k) {
                 constexpr uint32_t half = CHALF >> 4;
                 const uint32_t off = (k >> 2) * half + (k & 3) * 2;
-                umma_bf16_ss(tmem_base + t * 128, qd + off, kd + off, idesc_s, k > 0 ? 1u : 0u);
+                umma_ss(tmem_base + t * 128, qd + off, kd + off, idesc_s, k > 0 ? 1u : 0u);
               }
               umma_commit(&s_full[t]);
             }
@@ -256,14 +285,14 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
           if (j < (t ? n_b : n_a)) {
             ok &= mbar_wait(&p_full[t], j & 1, abort_flag, args.status, 2);
             tc_fence_after();
-            const uint64_t vd = v_desc + (j % CV_STAGES) * (CTILE >> 4);
+            const uint32_t vd = v_desc + (j % CV_STAGES) * (CTILE >> 4);
             const uint32_t p_tmem = tmem_base + (t ^ 1) * 128;
             const uint32_t acc0 = j > 0 ? 1u : 0u;
             __syncwarp();
             if (elect_one()) {
 #pragma unroll
               for (int k = 0; k < 8; ++k)
-                umma_bf16_ts(tmem_base + 256 + t * 128, p_tmem + k * 8, vd + k * (2048 >> 4), idesc_pv, k > 0 ? 1u : acc0);
+                umma_ts(tmem_base + 256 + t * 128, p_tmem + k * 8, vd + k * (2048 >> 4), idesc_pv, k > 0 ? 1u : acc0);
               umma_commit(&pv_done[t]);
             }
             __syncwarp();
@@ -349,8 +378,6 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     const uint32_t tmem_O = tmem_base + 256 + t * 128 + lane_sel;
     const uint32_t tmem_P = tmem_base + (t ^ 1) * 128 + lane_sel;   // over the other tile's scores
     uint8_t* sOt = sQ + t * CTILE;
-    const uint32_t st_row = smem_u32(sOt) + (base + ((lane >> 3) & 1) * 8 + (lane & 7)) * 128;
-    const uint32_t st_chunk = (uint32_t)((lane >> 4) ^ (lane & 7)) << 4;
     int lim[2];          // -1: no row of this sequence
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
@@ -528,6 +555,8 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
       if (item.w < 0) {
         // Output rows leave through this warp's rows of the row tile's buffer (no product reads it any more), so that 16
         // lanes store one row's 256 bytes.
+        const uint32_t st_row = smem_u32(sOt) + (base + ((lane >> 3) & 1) * 8 + (lane & 7)) * 128;
+        const uint32_t st_chunk = (uint32_t)((lane >> 4) ^ (lane & 7)) << 4;
         const float inv[2] = {l[0] == 0.f ? 0.f : 1.f / l[0], l[1] == 0.f ? 0.f : 1.f / l[1]};
         if (mine > 0) {
 #pragma unroll 1
