@@ -105,6 +105,7 @@ struct FewArgs {
   int pages, heads;   // of the cache
   float scale_log2;
   int* status;
+  int beside;         // the launch in front is that of the chunks: run beside it
 };
 
 // NR: groups of eight rows that a warp computes.  WR: sets of warps with other rows; the warps of a set take other keys.
@@ -134,7 +135,9 @@ __global__ void __launch_bounds__(FEW_THREADS, NR == 1 ? 3 : 2)
     mbar_fence_init();
   }
   __syncthreads();
-  pdl_wait();
+  // Chunks in front (attn_paged_sm100.cu) have waited for all work before them when this kernel may start, and nothing that
+  // they write is read here: it only has to end after them.
+  if (!a.beside) pdl_wait();
   pdl_trigger();
 
   const int4 item = p.few[blockIdx.x];
@@ -530,23 +533,22 @@ __global__ void __launch_bounds__(FEW_THREADS, NR == 1 ? 3 : 2)
       }
     }
   }
+  if (a.beside) pdl_wait();
 }
 
-// Joins the parts of a row: one warp per (row, key/value head), four values per lane.
+// Joins the parts of a row: a block per four rows of a key/value head, a warp per row, four values per lane.
 constexpr int MERGE_THREADS = 128;
 
 __global__ void __launch_bounds__(MERGE_THREADS) paged_merge_kernel(const Plan p, const FewArgs a) {
   pdl_wait();
   pdl_trigger();
   const int4 e = p.merge[blockIdx.x];
-  const int b = e.x, row0 = e.y, parts = e.z & 0xffff, rows = e.z >> 16;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = p.group;
-  const int q0 = p.q_start[b], q_len = p.q_start[b + 1] - q0;
-  const int w = blockIdx.y * (MERGE_THREADS / 32) + warp;
-  const int row = w / a.heads, head = w % a.heads;
-  if (row >= rows || row0 + row >= q_len * G) return;
+  const int b = e.x, parts = e.z & 0xffff, rows = e.z >> 16;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = p.group, head = blockIdx.y;
+  const int q0 = p.q_start[b], row = e.y + warp;
+  if (row >= (p.q_start[b + 1] - q0) * G) return;
   const long long step = (long long)rows * a.heads;
-  const long long at = (long long)(e.w + row) * a.heads + head;
+  const long long at = (long long)(e.w + warp) * a.heads + head;
   float mt = -INFINITY;
   for (int s = lane; s < parts; s += 32) mt = fmaxf(mt, a.part_ml[at + s * step].x);
 #pragma unroll
@@ -565,11 +567,11 @@ __global__ void __launch_bounds__(MERGE_THREADS) paged_merge_kernel(const Plan p
     lt += ml.x == -INFINITY ? 0.f : f * ml.y;
   }
   const float inv = lt == 0.f ? 0.f : 1.f / lt;
-  const int t = (row0 + row) / G;
+  const int t = row / G;
   uint2 u;
   u.x = pack_bf16x2(x.x * inv, x.y * inv);
   u.y = pack_bf16x2(x.z * inv, x.w * inv);
-  *reinterpret_cast<uint2*>(a.o + (long long)(q0 + t) * a.ldo + (long long)(head * G + (row0 + row) % G) * HEAD + lane * 4) = u;
+  *reinterpret_cast<uint2*>(a.o + (long long)(q0 + t) * a.ldo + (long long)(head * G + row % G) * HEAD + lane * 4) = u;
 }
 
 template <bool FP8, int NR, int WR>
@@ -604,7 +606,7 @@ using namespace snu1;
 
 // o_r = attention of row r over its sequence's first keys, rows [rows][heads of queries][128] bf16, ldq / ldo apart.
 // scratch: partial results (partial_rows x heads x (128 values, maximum, sum) in fp32), then unpack_count
-// fp16 pages of 128 tokens and their factors (a float2 per page and head).
+// fp16 pages of 128 tokens and their factors (a float4 per page and head).
 SNU1_API int snu1_paged_attention(const void* cache, const void* plan, const void* q, long long ldq, void* o, long long ldo,
                                   float scale, void* scratch, void* stream) {
   using namespace paged;
@@ -633,11 +635,12 @@ SNU1_API int snu1_paged_attention(const void* cache, const void* plan, const voi
   a.heads = c.heads;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.status = device_status_word();
+  a.beside = p.chunk_count > 0;
   cudaStream_t st = (cudaStream_t)stream;
   int rc = kHostOk;
   if (p.chunk_count > 0) {
     void* wide = a.part_ml + (((long long)p.partial_rows * c.heads + 15) & ~15ll);      // 128-byte aligned
-    float2* factors = (float2*)((uint8_t*)wide + 2ll * 128 * HEAD * 2 * p.unpack_count * c.heads);
+    float4* factors = (float4*)((uint8_t*)wide + 2ll * 128 * HEAD * 2 * p.unpack_count * c.heads);
     if (c.fp8 && (rc = launch_widen(c, p, wide, factors, st)) != kHostOk) return rc;
     if ((rc = launch_chunks(c, p, q, ldq, p.rows, o, ldo, a.part, a.part_ml, a.scale_log2, wide, factors, st)) != kHostOk) return rc;
   }
@@ -647,6 +650,6 @@ SNU1_API int snu1_paged_attention(const void* cache, const void* plan, const voi
     if (rc != kHostOk) return rc;
   }
   if (p.merge_count > 0)
-    SNU1_CUDA_CHECK(launch_pdl(paged_merge_kernel, dim3(p.merge_count, (p.merge_rows * c.heads + 3) / 4), dim3(MERGE_THREADS), 0, st, p, a));
+    SNU1_CUDA_CHECK(launch_pdl(paged_merge_kernel, dim3(p.merge_count, c.heads), dim3(MERGE_THREADS), 0, st, p, a));
   return kHostOk;
 }

@@ -16,8 +16,8 @@
 // * The mask is one number per row, the keys that it may read; tiles that all rows read whole need no test.
 // * A work item is a part of the key tiles of two row tiles; unnormalised results of parts are joined by
 //   paged_merge_kernel.  ops/paged.py chooses the parts so that the waves of CTAs are full.
-// * Two warps that have nothing else to do clear values that are not finite (and rows behind the last token) in the tiles that
-//   some row may not read whole: a probability of zero does not hide them from the product.  Rows that may read such a
+// * Two warps that have nothing else to do clear values that are not finite (and rows behind the last token) in the bf16 tiles
+//   that some row may not read whole (widening does so for e4m3): a probability of zero does not hide them from the product.  Rows that may read such a
 //   value give NaN, the others are as if it were not there.
 #include <string.h>
 
@@ -42,7 +42,7 @@ struct ChunkArgs {
   float* part;
   float2* part_ml;
   const int* first_page;   // scratch of widened rows: a sequence's first page there; null: the cache's own pages
-  const float2* factors;   // of the widened pages: the keys' power of two, the exponent of the values'
+  const float4* factors;   // of the widened pages, see paged_widen_kernel
   int page, pages, heads;
   float scale_log2;
   int* status;
@@ -177,23 +177,32 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
   const int q0 = p.q_start[b], q_len = p.q_start[b + 1] - q0;
   const int kv_len = seq_len(p, b);
   const int token0 = item.y / G;
-  if (threadIdx.x < 2 * T) {
-    const int t = threadIdx.x / T, token = token0 + threadIdx.x;
-    if (token < q_len) {
-      const int l = row_limit(p, q0, q_len, kv_len, token);
-      atomicMax(&lim_max[t], l);
-      atomicMin(&lim_min[t], l);
+  int max_a, max_b, min_a, min_b;               // the largest and the smallest limit of row tiles A and B
+  if (p.behind == nullptr) {                    // limits grow from token to token
+    const int ends = min(token0 + 2 * T, q_len) - 1;
+    min_a = row_limit(p, q0, q_len, kv_len, token0);
+    max_a = row_limit(p, q0, q_len, kv_len, min(token0 + T - 1, ends));
+    min_b = token0 + T <= ends ? row_limit(p, q0, q_len, kv_len, token0 + T) : 0x7fffffff;
+    max_b = token0 + T <= ends ? row_limit(p, q0, q_len, kv_len, ends) : 0;
+  } else {
+    if (threadIdx.x < 2 * T) {
+      const int t = threadIdx.x / T, token = token0 + threadIdx.x;
+      if (token < q_len) {
+        const int l = row_limit(p, q0, q_len, kv_len, token);
+        atomicMax(&lim_max[t], l);
+        atomicMin(&lim_min[t], l);
+      }
     }
+    __syncthreads();
+    max_a = lim_max[0], max_b = lim_max[1], min_a = lim_min[0], min_b = lim_min[1];
   }
-  __syncthreads();
-  const int max_a = lim_max[0], max_b = lim_max[1], min_a = lim_min[0], min_b = lim_min[1];
   const int most = max(max_a, max_b);
   const int all = (most + BK - 1) / BK;
   const int j0 = (int)((long long)all * part / parts), n = (int)((long long)all * (part + 1) / parts) - j0;
   // Row tile A (B) reads the part's first n_a (n_b) key tiles, all but the first full_a (full_b) of them with the mask.
   const int n_a = max(0, min(n, (max_a + BK - 1) / BK - j0)), n_b = max(0, min(n, (max_b + BK - 1) / BK - j0));
   const int full_a = min_a / BK - j0, full_b = min_b / BK - j0;
-  auto dirty = [&](int j) -> bool { return (j < n_a && j >= full_a) || (j < n_b && j >= full_b); };
+  auto dirty = [&](int j) -> bool { return !FP8 && ((j < n_a && j >= full_a) || (j < n_b && j >= full_b)); };
   // columns: S_A and P_B [0,128), S_B and P_A [128,256), O_A [256,384), O_B [384,512)
 
   // 640 threads start with 96 registers: 128 x 64 + 512 x 104 = 640 x 96
@@ -330,7 +339,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
           }
         }
       }
-    } else {
+    } else if (!FP8) {
       // ------------------------------ cleaning --------------------------------
       bool ok = true;
       const int tid = threadIdx.x - 64;
@@ -342,23 +351,29 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         ok = mbar_wait_warp(&v_dirty[s], (told >> s) & 1, abort_flag, args.status, 3);
         told ^= 1u << s;
         if (ok) ok = mbar_wait_warp(&v_full[s], (j / CV_STAGES) & 1, abort_flag, args.status, 3);
-#pragma unroll 4
-        for (int i = 0; i < 32; ++i) {
-          const int key = i * 4 + (tid >> 4), ch = tid & 15;
-          uint4* at = reinterpret_cast<uint4*>(sV + s * CTILE + (ch >> 3) * CHALF + swz128_offset(key, ch & 7));
-          uint4 x = *at;
-          uint32_t* w = reinterpret_cast<uint32_t*>(&x);
-          bool bad = false;
+        // eight loads at a time, or a store in between holds the next load up: 5 -> 2 us for a last tile
+        uint8_t* at = sV + s * CTILE + ((tid & 15) >> 3) * CHALF;
+#pragma unroll 1
+        for (int i = 0; i < 32; i += 8) {
+          uint4 x[8];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            constexpr uint32_t ex = FP8 ? 0x7c00u : 0x7f80u;         // an exponent of all ones
-            const bool lo = (w[e] & ex) == ex, hi = (w[e] & ex << 16) == ex << 16;
-            bad |= lo || hi;
-            w[e] &= (lo ? 0xffff0000u : 0xffffffffu) & (hi ? 0xffffu : 0xffffffffu);
-          }
-          if (bad) {
-            *at = x;
-            if (k0 + key < kv_len) atomicMin(poison, k0 + key);
+          for (int u = 0; u < 8; ++u) x[u] = *reinterpret_cast<const uint4*>(at + swz128_offset((i + u) * 4 + (tid >> 4), tid & 7));
+#pragma unroll
+          for (int u = 0; u < 8; ++u) {
+            uint32_t* w = reinterpret_cast<uint32_t*>(&x[u]);
+            constexpr uint32_t ex = 0x7f80u;         // an exponent of all ones
+            // the upper bit of a half is set where its exponent is all ones
+            uint32_t bad = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) bad |= ((w[e] & (ex | ex << 16)) + 0x00800080u) & 0x80008000u;
+            if (bad) {
+              const int key = (i + u) * 4 + (tid >> 4);
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                w[e] &= ((w[e] & ex) == ex ? 0xffff0000u : 0xffffffffu) & ((w[e] & ex << 16) == ex << 16 ? 0xffffu : 0xffffffffu);
+              *reinterpret_cast<uint4*>(at + swz128_offset(key, tid & 7)) = x[u];
+              if (k0 + key < kv_len) atomicMin(poison, k0 + key);
+            }
           }
         }
         fence_proxy_async_smem();
@@ -391,12 +406,13 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
       // this warp's 16 query rows to fp16, each times a power of two (see attn_paged.cu)
       ok &= mbar_wait(q_full, 0, abort_flag, args.status, 5);
       __syncwarp();
+      uint8_t* at = sOt + ((lane & 15) >> 3) * CHALF;
+      uint4 u[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) u[i] = *reinterpret_cast<const uint4*>(at + swz128_offset(base + 2 * i + (lane >> 4), lane & 7));
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const int c = lane & 15;
-        uint4* at = reinterpret_cast<uint4*>(sOt + (c >> 3) * CHALF + swz128_offset(base + 2 * i + (lane >> 4), c & 7));
-        uint4 u = *at;
-        uint32_t* w = reinterpret_cast<uint32_t*>(&u);
+        uint32_t* w = reinterpret_cast<uint32_t*>(&u[i]);
         uint32_t top = 0;
 #pragma unroll
         for (int e = 0; e < 4; ++e) top = max(top, max((w[e] << 16) & 0x7fffffffu, w[e] & 0x7fff0000u));
@@ -407,7 +423,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           w[e] = pack_f16x2(__uint_as_float(w[e] << 16) * f, __uint_as_float(w[e] & 0xffff0000u) * f);
-        *at = u;
+        *reinterpret_cast<uint4*>(at + swz128_offset(base + 2 * i + (lane >> 4), lane & 7)) = u[i];
         const int own = __shfl_sync(0xffffffffu, up, (lane >> 2 & 1) * 16);     // of row 2 i or 2 i + 1
 #pragma unroll
         for (int r = 0; r < 2; ++r)
@@ -417,11 +433,15 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(q_ready);
     }
-    const float2* factors = FP8 ? args.factors + (long long)(args.first_page[b] + j0) * args.heads + kvh : nullptr;
+    const float4* factors = FP8 ? args.factors + (long long)(args.first_page[b] + j0) * args.heads + kvh : nullptr;
+    int bad = 0x7fffffff;                   // first key whose value is not finite
     const int mine = t ? n_b : n_a, full = t ? full_b : full_a;
     for (int j = 0; j < mine; ++j) {        // all tiles also after a time-out, see mbar_wait_warp
-      float2 factor = make_float2(1.f, 0.f);      // of this tile's keys and values
-      if (FP8) factor = __ldg(factors + (long long)j * args.heads);
+      float4 factor = make_float4(1.f, 0.f, 0.f, 0.f);      // of this tile's keys and values
+      if (FP8) {
+        factor = __ldg(factors + (long long)j * args.heads);
+        bad = min(bad, __float_as_int(factor.z));
+      }
       ok &= mbar_wait(&s_full[t], j & 1, abort_flag, args.status, 5);
       tc_fence_after();
       float sv[2][32];   // [columns 0-63, 64-127][4 i + 2 row + e]
@@ -550,7 +570,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
       for (int r = 0; r < 2; ++r) {
         l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
         l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-        if (lim[r] > *poison) l[r] = __int_as_float(0x7fffffff);
+        if (lim[r] > (FP8 ? bad : *poison)) l[r] = __int_as_float(0x7fffffff);
       }
       if (item.w < 0) {
         // Output rows leave through this warp's rows of the row tile's buffer (no product reads it any more), so that 16
@@ -575,11 +595,12 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
           }
           __syncwarp();
         }
+        const uint32_t per = 65536u / G + 1;               // r / G = r per >> 16 for r < 128
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const int r = base + 2 * i + (lane >> 4), c = lane & 15, token = token0 + t * T + r / G;
+          const int r = base + 2 * i + (lane >> 4), c = lane & 15, of = r * per >> 16, token = token0 + t * T + of;
           if (r < T * G && token < q_len)
-            *reinterpret_cast<uint4*>(args.o + (long long)(q0 + token) * args.ldo + (long long)(kvh * G + r % G) * HEAD + c * 8) =
+            *reinterpret_cast<uint4*>(args.o + (long long)(q0 + token) * args.ldo + (long long)(kvh * G + r - of * G) * HEAD + c * 8) =
                 mine > 0 ? *reinterpret_cast<const uint4*>(sOt + (c >> 3) * CHALF + swz128_offset(r, c & 7)) : make_uint4(0, 0, 0, 0);
         }
       } else {
@@ -628,7 +649,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
 }
 
 int launch_chunks(const Cache& c, const Plan& p, const void* q, long long ldq, int q_rows, void* o, long long ldo, float* part,
-                  float2* part_ml, float scale_log2, void* wide, const float2* factors, cudaStream_t st) {
+                  float2* part_ml, float scale_log2, void* wide, const float4* factors, cudaStream_t st) {
   const int G = p.group, T = 128 / G;
   CUtensorMap tm_q, tm_k = c.k, tm_v = c.v;
   int rc;

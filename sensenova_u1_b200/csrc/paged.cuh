@@ -42,9 +42,9 @@ struct Plan {
   const int* unpack_first; // [seqs] first page of such a sequence in the scratch for unpacked rows
   const int4* few;         // [few_count] work of the kernel for few rows: sequence, first row, part | parts << 16, partial row (-1: none)
   const int4* chunk;       // [chunk_count] the same for chunks
-  const int4* merge;       // [merge_count] sequence, first row, parts | rows of a part << 16, partial row
+  const int4* merge;       // [merge_count] four rows to join: sequence, first row, parts | rows of a part << 16, first partial row
   int seqs, rows, width, page, group;
-  int read_count, few_count, few_rows, chunk_count, merge_count, merge_rows;
+  int read_count, few_count, few_rows, chunk_count, merge_count;
   int partial_rows;        // rows of the scratch for partial results (x heads)
   int unpack_count;        // also the 128-token pages of the scratch for unpacked rows
 };
@@ -72,10 +72,10 @@ __device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* m, 
 }
 
 // paged_cache.cu: a plan's ``unpack`` tiles of an e4m3 cache as fp16 pages at ``wide``
-int launch_widen(const Cache& c, const Plan& p, void* wide, float2* factors, cudaStream_t st);
+int launch_widen(const Cache& c, const Plan& p, void* wide, float4* factors, cudaStream_t st);
 // attn_paged_sm100.cu: a plan's ``chunk`` items
 int launch_chunks(const Cache& c, const Plan& p, const void* q, long long ldq, int q_rows, void* o, long long ldo, float* part,
-                  float2* part_ml, float scale_log2, void* wide, const float2* factors, cudaStream_t st);
+                  float2* part_ml, float scale_log2, void* wide, const float4* factors, cudaStream_t st);
 
 }  // namespace paged
 }  // namespace snu1

@@ -164,15 +164,17 @@ __global__ void __launch_bounds__(READ_THREADS)
 // sequence from a page of its own on, rows behind its last token cleared.  A tile of one head is divided by a power of two,
 // so that its largest value is at most 1 (2^-126 to 2^90; that factor goes into the scores, or into the probabilities): code times
 // scale is rounded to 11 bits, and what falls below fp16's normal range is 2^14 times smaller than the tile's largest value.
-// factors [page][heads]: the keys' power of two, and the exponent of the values'.
+// factors [page][heads]: the keys' power of two, the exponent of the values' (log2), and, as a whole number, the first
+// key of the sequence in this tile whose value is not finite (its scale is not); that value is cleared.
 constexpr int WIDEN_THREADS = 256;
 
 __global__ void __launch_bounds__(WIDEN_THREADS)
     paged_widen_kernel(const uint8_t* __restrict__ data, const float* __restrict__ scales, int pages, int heads, Plan p,
-                       uint8_t* __restrict__ wide, float2* __restrict__ factors, int* status) {
+                       uint8_t* __restrict__ wide, float4* __restrict__ factors, int* status) {
   __shared__ long long s_at[128];          // the token's row of the cache, -1: none
   __shared__ float s_scale[128];
   __shared__ float s_top[4];
+  __shared__ int s_bad[4];
   pdl_wait();
   pdl_trigger();
   const int2 e = p.unpack[blockIdx.x];
@@ -191,10 +193,15 @@ __global__ void __launch_bounds__(WIDEN_THREADS)
         report_status(status, kBadPage, 9);
       }
     }
-    s_at[t] = at;
-    s_scale[t] = s;
-    const uint32_t top = __reduce_max_sync(0xffffffffu, fabsf(s) < INFINITY ? __float_as_uint(fabsf(s)) : 0u);
-    if ((t & 31) == 0) s_top[t >> 5] = __uint_as_float(top);
+    const bool finite = fabsf(s) < INFINITY;
+    const uint32_t top = __reduce_max_sync(0xffffffffu, finite ? __float_as_uint(fabsf(s)) : 0u);
+    const int bad = __reduce_min_sync(0xffffffffu, finite ? 0x7fffffff : pos);
+    s_at[t] = kv && !finite ? -1 : at;
+    s_scale[t] = kv && !finite ? 0.f : s;
+    if ((t & 31) == 0) {
+      s_top[t >> 5] = __uint_as_float(top);
+      s_bad[t >> 5] = bad;
+    }
   }
   __syncthreads();
   const float top = E4M3_MAX * fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
@@ -204,6 +211,7 @@ __global__ void __launch_bounds__(WIDEN_THREADS)
   if (t == 0) {
     float* f = reinterpret_cast<float*>(factors + page * heads + head);
     f[kv] = kv ? (float)ex : __int_as_float((127 + ex) << 23);
+    if (kv) f[2] = __int_as_float(min(min(s_bad[0], s_bad[1]), min(s_bad[2], s_bad[3])));
   }
   const int c = t & 15;
   uint2 x[8];
@@ -228,7 +236,7 @@ __global__ void __launch_bounds__(WIDEN_THREADS)
   }
 }
 
-int launch_widen(const Cache& c, const Plan& p, void* wide, float2* factors, cudaStream_t st) {
+int launch_widen(const Cache& c, const Plan& p, void* wide, float4* factors, cudaStream_t st) {
   SNU1_CUDA_CHECK(launch_pdl(paged_widen_kernel, dim3(p.unpack_count, 2 * c.heads), dim3(WIDEN_THREADS), 0, st, (const uint8_t*)c.data,
                              (const float*)c.scales, c.pages, c.heads, p, (uint8_t*)wide, factors, device_status_word()));
   return kHostOk;

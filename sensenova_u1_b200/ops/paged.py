@@ -40,7 +40,8 @@ FEW_LEAST = 4            # a part of a sequence has at least this many key tiles
 FEW_TILE = 64            # rows (new tokens x query heads of a group) of one CTA, at most
 CHUNK_TILE = 128         # keys of a tile of the kernel for chunks, and rows of a row tile
 CHUNK_SLOTS = 148        # its CTAs that run at once
-CHUNK_START = 3          # what starting and ending a CTA costs, in key tiles
+CHUNK_START = 5          # what starting and ending a CTA costs, in key tiles (1.8 us): 8 to 10 us from its start to its end
+CHUNK_JOIN = 3           # what a part costs besides: 128 KB written and read again
 
 
 def _library():
@@ -108,7 +109,7 @@ class _Args(ctypes.Structure):
     _fields_ = ([(n, c_void_p) for n in ("q_start", "kv_len", "cap", "table", "behind", "row_seq", "k_start", "read_pages", "unpack",
                                          "unpack_first", "few", "chunk", "merge")]
                 + [(n, c_int) for n in ("seqs", "rows", "width", "page", "group", "read_count", "few_count", "few_rows", "chunk_count",
-                                        "merge_count", "merge_rows", "partial_rows", "unpack_count")])
+                                        "merge_count", "partial_rows", "unpack_count")])
 
 
 @dataclass
@@ -216,14 +217,14 @@ def _lay_out(q_lens, kv_lens, tables, page: int, pages: int, group: int, kv_head
 
     seq, row0 = tiles_of(few_q, few_rows)
     tiles = -(-cap[seq] // KEY_TILE)
-    few, merge, partial = _items(seq, row0, tiles, _shares(tiles, kv_heads, FEW_SLOTS, FEW_LEAST), few_rows, 0)
+    few, merge, partial = _items(seq, row0, tiles, _shares(tiles, kv_heads, FEW_SLOTS, FEW_LEAST), few_q, few_rows, 0)
     seq, row0 = tiles_of(np.where(chunked, q_rows, 0), chunk_rows)
     if limits is None:                                        # a row tile reads up to its last token
         last = np.minimum((row0 + chunk_rows - 1) // group, q[seq] - 1)
         tiles = -(-(cap[seq] - q[seq] + 1 + last) // CHUNK_TILE)
     else:
         tiles = -(-kv[seq] // CHUNK_TILE)
-    chunk, more, partial = _items(seq, row0, tiles, _waves(tiles, kv_heads, CHUNK_SLOTS), chunk_rows, partial)
+    chunk, more, partial = _items(seq, row0, tiles, _waves(tiles, kv_heads, CHUNK_SLOTS), q_rows, chunk_rows, partial)
     unpack = unpack_first = None
     if fp8 and len(chunk):
         wide = np.where(chunked, -(-cap // CHUNK_TILE), 0)    # 128-token pages
@@ -233,14 +234,14 @@ def _lay_out(q_lens, kv_lens, tables, page: int, pages: int, group: int, kv_head
                   k_start=start(kv), read_pages=pages_of(read), unpack=unpack, unpack_first=unpack_first, few=few, chunk=chunk,
                   merge=merge)
     counts = dict(seqs=n, rows=rows, width=width, page=page, group=group, read_count=int(read.sum()), few_count=len(few),
-                  few_rows=few_rows, chunk_count=len(chunk), merge_count=len(merge), merge_rows=chunk_rows if len(more) else few_rows,
-                  partial_rows=partial, unpack_count=0 if unpack is None else len(unpack))
+                  few_rows=few_rows, chunk_count=len(chunk), merge_count=len(merge), partial_rows=partial, unpack_count=0 if unpack is None else len(unpack))
     return arrays, counts
 
 
 def _waves(tiles: np.ndarray, heads: int, slots: int) -> np.ndarray:
-    """Parts of the chunk kernel's items: of the shares that cut the longest item into up to 16 parts, the one whose waves of
-    CTAs (longest first, a wave as long as its longest CTA) are shortest together.  Every CTA pays ``CHUNK_START``."""
+    """Parts of the chunk kernel's items: of the shares that cut the longest item into up to 16 parts, the one that is done
+    first when the CTAs are taken up longest first.  Starting and ending a CTA costs ``CHUNK_START`` key tiles, what a part
+    writes and its join reads ``CHUNK_JOIN``."""
     if not len(tiles):
         return tiles
     tiles = np.maximum(tiles, 1)
@@ -248,23 +249,33 @@ def _waves(tiles: np.ndarray, heads: int, slots: int) -> np.ndarray:
     for cut in range(1, 17):
         share = -(-int(tiles.max()) // cut)
         parts = -(-tiles // share)
-        sizes = np.repeat(-(-tiles // parts), parts * heads)
-        cost = float((np.sort(sizes)[::-1][::slots] + CHUNK_START).sum()) + (CHUNK_START if cut > 1 else 0)
-        if best is None or cost < 0.98 * best[0]:
-            best = (cost, parts)
+        cost = -(-tiles // parts) + CHUNK_START + np.where(parts > 1, CHUNK_JOIN, 0)
+        cost = np.sort(np.repeat(cost, parts * heads))[::-1]
+        busy = np.zeros(slots)
+        for i in range(0, len(cost), slots):                  # the longest that are left go to those that are free first
+            wave = cost[i:i + slots]
+            busy.sort()
+            busy[:len(wave)] += wave
+        done = busy.max() + (CHUNK_START / 2 if cut > 1 else 0)
+        if best is None or done < 0.98 * best[0]:
+            best = (done, parts)
         if share <= 2:
             break
     return best[1]
 
 
-def _items(seq, row0, tiles, parts, m: int, first: int):
+def _items(seq, row0, tiles, parts, q_rows, m: int, first: int):
     """Work items [sequence, first row, part | parts << 16, partial row or -1], those with most keys first, the joins of the
-    items that were split, and the rows of partial results up to there."""
+    items that were split (four rows each), and the rows of partial results up to there."""
     if not len(seq):
         return np.zeros((0, 4), np.int32), np.zeros((0, 4), np.int32), first
     split = parts > 1
     at = first + np.cumsum(np.where(split, parts * m, 0)) - np.where(split, parts * m, 0)
-    merge = np.stack([seq, row0, parts | m << 16, at], 1)[split]
+    join = np.where(split, -(-np.minimum(m, q_rows[seq] - row0) // 4), 0)
+    four = 4 * (np.arange(int(join.sum())) - np.repeat(np.cumsum(join) - join, join))
+    merge = np.stack([np.repeat(x, join) for x in (seq, row0, parts | m << 16, at)], 1)
+    merge[:, 1] += four
+    merge[:, 3] += four
     i = np.repeat(np.arange(len(seq)), parts)
     part = np.arange(len(i)) - np.repeat(np.cumsum(parts) - parts, parts)
     items = np.stack([seq[i], row0[i], part | parts[i] << 16, np.where(split[i], at[i] + part * m, -1)], 1)
@@ -298,7 +309,7 @@ def build_plan(cache: PagedCache, heads: int, q_lens, kv_lens, tables, limits=No
     args = _Args(**{name: store.data_ptr() + 4 * o for name, o in at.items()}, **counts)
     n = counts["seqs"]
     joined = counts["partial_rows"] * cache.kv_heads
-    scratch = joined * HEAD_DIM * 4 + (joined + 15) // 16 * 128 + counts["unpack_count"] * cache.kv_heads * (2 * CHUNK_TILE * HEAD_DIM * 2 + 8)
+    scratch = joined * HEAD_DIM * 4 + (joined + 15) // 16 * 128 + counts["unpack_count"] * cache.kv_heads * (2 * CHUNK_TILE * HEAD_DIM * 2 + 16)
     return PagedPlan(heads, cache.kv_heads, cache.page, cache.pages, cache.data.dtype, cache.device,
                      [int(x) for x in q_lens], [int(x) for x in kv_lens],
                      counts["rows"], int(arrays["k_start"][-1]), scratch, store[at["kv_len"]:at["kv_len"] + n], grow, store, args)

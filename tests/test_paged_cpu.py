@@ -85,13 +85,19 @@ def test_every_row_meets_every_key_once(q, kv, group, heads):
             assert (b, r) not in seen
             seen[(b, r)] = count
     assert len(seen) == sum(q) * group
-    joined = {(b, row0): (z & 0xffff, z >> 16, at) for b, row0, z, at in a["merge"].tolist()}
-    assert set(joined) == {(b, r0) for (b, r0, m, count) in parts if count > 1}
+    joined = {}
+    for b, row0, z, at in a["merge"].tolist():                        # four rows each
+        for r in range(row0, min(row0 + 4, q[b] * group)):
+            assert (b, r) not in joined
+            joined[(b, r)] = (z & 0xffff, z >> 16, at + r - row0)
+    assert set(joined) == {(b, r) for (b, r), count in seen.items() if count > 1}
     for b, row0, z, at in a["few"].tolist() + a["chunk"].tolist():
         if at >= 0:
-            count, m, first = joined[(b, row0)]
-            assert count == z >> 16 and at == first + (z & 0xffff) * m
-            assert m <= c["merge_rows"]
+            for r in range(row0, q[b] * group):
+                count, m, first = joined[(b, r)]
+                assert count == z >> 16 and (r - row0 >= m or at + r - row0 == first + (z & 0xffff) * m)
+                if r - row0 + 1 >= m:
+                    break
     if c["unpack_count"]:                                             # every key of a chunk's sequence has its place
         wide = [-(-k // 128) if any(b == i for b, *_ in a["chunk"].tolist()) else 0 for i, k in enumerate(kv)]
         assert c["unpack_count"] == sum(wide) and a["unpack_first"].tolist() == [sum(wide[:i]) for i in range(n)]
