@@ -6,7 +6,7 @@
 // The rows of a (sequence, key/value head) are its new tokens times the query heads of the group, up to 64 per CTA.  What
 // bounds it is the stream of keys and values, so the work is split over keys: a work item is one part of a sequence, the
 // parts are made as equal as they can be over the whole batch (ops/paged.py), and their unnormalised results (maximum, sum,
-// weighted values, fp32) are joined by a second kernel in a fixed order, without atomics.
+// weighted values, fp32) are joined in a fixed order by whichever CTA finds all parts there: see join_parts.
 //
 // One warp asks for whole pages through TMA (keys and values of one head in one box), several stages ahead; four warps
 // compute with mma.sync m16n8k16, keys (then the width of a head) on the 16-side and rows on the 8-side: S^T = K q^T,
@@ -39,13 +39,15 @@ namespace paged {
 constexpr int FEW_WARPS = 4;                              // warps that compute; one more asks for pages
 constexpr int FEW_THREADS = FEW_WARPS * 32 + 32;
 
-template <bool FP8>
+// SMALL: up to eight rows.  Their registers let three CTAs run on an SM, with two stages each instead of three.
+template <bool FP8, bool SMALL>
 struct Few {
   static constexpr int KT = FP8 ? 128 : 64;               // keys of a stage
   static constexpr int HALVES = FP8 ? 1 : 2;              // boxes of 128 bytes per row
   static constexpr int DATA = KT * 2 * 128 * HALVES;      // keys and values of a stage
   static constexpr int SCALES = FP8 ? KT * 2 * 4 : 0;
-  static constexpr int STAGES = 3;
+  static constexpr int CTAS = SMALL ? 3 : 2;
+  static constexpr int STAGES = SMALL ? 2 : 3;
   static constexpr int RING = STAGES * (DATA + SCALES);
   static constexpr int SMEM = RING + 1024;
 };
@@ -102,29 +104,140 @@ struct FewArgs {
   long long ldq, ldo;
   float* part;        // [partial rows][heads][128]
   float2* part_ml;    // [partial rows][heads] maximum (log2 units), sum
+  unsigned long long* flags;   // [parts of few rows][heads], see last_part
+  unsigned long long word;
   int pages, heads;   // of the cache
   float scale_log2;
   int* status;
   int beside;         // the launch in front is that of the chunks: run beside it
 };
 
+// Up to so many rows the parts join themselves, more are joined by a launch of their own (paged_join_kernel, which has as many
+// warps as rows and not four): 24 x 1 token, 4 rows each, 27.7 -> 26.6 us, one conversation 12.2 -> 10.4; 8 x 5 tokens, 20 rows
+// each, 44.5 -> 47.9.
+constexpr int JOIN_ROWS = 8;
+
+// Joins ``parts`` results of a row, ``step`` apart from ``at`` on; a whole warp, four values per lane.
+__device__ __forceinline__ void join_row(const FewArgs& a, long long at, long long step, int parts, __nv_bfloat16* out) {
+  const int lane = threadIdx.x & 31;
+  float mt = -INFINITY;
+  for (int s = lane; s < parts; s += 32) mt = fmaxf(mt, __ldcg(&a.part_ml[at + s * step].x));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, o));
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+  float lt = 0.f;
+#pragma unroll 4
+  for (int s = 0; s < parts; ++s) {
+    const float2 ml = __ldcg(&a.part_ml[at + s * step]);
+    const float4 y = __ldcg(reinterpret_cast<const float4*>(a.part + (at + s * step) * HEAD) + lane);
+    const float f = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - mt);
+    x.x += f * y.x;
+    x.y += f * y.y;
+    x.z += f * y.z;
+    x.w += f * y.w;
+    lt += ml.x == -INFINITY ? 0.f : f * ml.y;
+  }
+  const float inv = lt == 0.f ? 0.f : 1.f / lt;                  // a row without keys gives zeros
+  uint2 u;
+  u.x = pack_bf16x2(x.x * inv, x.y * inv);
+  u.y = pack_bf16x2(x.z * inv, x.w * inv);
+  *reinterpret_cast<uint2*>(out + lane * 4) = u;
+}
+
+// The same with 16 lanes per row, eight values each, and four parts on their way at a time.
+__device__ __forceinline__ void join_eight(const FewArgs& a, long long at, long long step, int parts, __nv_bfloat16* out) {
+  constexpr int U = 4;
+  const int c = threadIdx.x & 15;
+  float x[8], lt = 0.f, mt = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = 0.f;
+  for (int s0 = 0; s0 < parts; s0 += U) {
+    float2 ml[U];
+    float4 y[U][2];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const long long r = at + min(s0 + u, parts - 1) * step;
+      ml[u] = __ldcg(&a.part_ml[r]);
+      y[u][0] = __ldcg(reinterpret_cast<const float4*>(a.part + r * HEAD) + 2 * c);
+      y[u][1] = __ldcg(reinterpret_cast<const float4*>(a.part + r * HEAD) + 2 * c + 1);
+    }
+    float mn = mt;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (s0 + u < parts) mn = fmaxf(mn, ml[u].x);
+    const float old = mt == -INFINITY ? 0.f : fast_exp2(mt - mn);
+    mt = mn;
+    lt *= old;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] *= old;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (s0 + u >= parts || ml[u].x == -INFINITY) continue;
+      const float f = fast_exp2(ml[u].x - mt);
+      lt += f * ml[u].y;
+      x[0] += f * y[u][0].x;
+      x[1] += f * y[u][0].y;
+      x[2] += f * y[u][0].z;
+      x[3] += f * y[u][0].w;
+      x[4] += f * y[u][1].x;
+      x[5] += f * y[u][1].y;
+      x[6] += f * y[u][1].z;
+      x[7] += f * y[u][1].w;
+    }
+  }
+  const float inv = lt == 0.f ? 0.f : 1.f / lt;                  // a row without keys gives zeros
+  *reinterpret_cast<uint4*>(out + c * 8) = make_uint4(pack_bf16x2(x[0] * inv, x[1] * inv), pack_bf16x2(x[2] * inv, x[3] * inv),
+                                                      pack_bf16x2(x[4] * inv, x[5] * inv), pack_bf16x2(x[6] * inv, x[7] * inv));
+}
+
+// Whether this CTA has to join the parts that it is one of; all its threads call it, after their last store of a result.
+// A part that is done sets its flag and then looks at all flags: the one that sets its flag last sees the others (stores and
+// loads on both sides of a fence.sc), others may see them too and join as well, to the same bits.  Scratch starts with
+// whatever was there, so a flag is set to a word of this call (64 random bits), and is cleared again by those who joined:
+// the same launch replayed from a graph finds no flag of its last run.
+__device__ __forceinline__ bool last_part(unsigned long long* flags, int part, int parts, int step, unsigned long long word, int* s_vote,
+                                          int threads) {
+  named_bar_sync(1, threads);
+  if (threadIdx.x < 32) {
+    __threadfence();                                             // of all stores before the barrier
+    if (threadIdx.x == 0) *reinterpret_cast<volatile unsigned long long*>(flags + (long long)part * step) = word;
+    __threadfence();
+    __syncwarp();
+    bool all = true;
+    for (int s = threadIdx.x; s < parts; s += 32) {
+      unsigned long long f;
+      asm volatile("ld.acquire.gpu.global.u64 %0, [%1];" : "=l"(f) : "l"(flags + (long long)s * step) : "memory");
+      all &= s == part || f == word;
+    }
+    all = __all_sync(0xffffffffu, all);
+    if (threadIdx.x == 0) *s_vote = all;
+  }
+  named_bar_sync(1, threads);
+  return *s_vote != 0;
+}
+
 // NR: groups of eight rows that a warp computes.  WR: sets of warps with other rows; the warps of a set take other keys.
 template <bool FP8, int NR, int WR>
-__global__ void __launch_bounds__(FEW_THREADS, NR == 1 ? 3 : 2)
+__global__ void __launch_bounds__(FEW_THREADS, Few<FP8, NR * WR == 1>::CTAS)
     paged_few_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_constant__ CUtensorMap tm_scale, const Plan p,
                      const FewArgs a) {
-  using F = Few<FP8>;
+  using F = Few<FP8, NR * WR == 1>;
   constexpr int KT = F::KT, WK = FEW_WARPS / WR, M = 8 * NR * WR;
+  constexpr bool JOIN = M <= JOIN_ROWS;
   constexpr int BLOCKS = KT / 16 / WK, NB = BLOCKS < 2 ? BLOCKS : 2;     // blocks of 16 keys of a warp, and how many at a time
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   float* s_scales = reinterpret_cast<float*>(smem + F::STAGES * F::DATA);   // [stage][page box][keys, values][box rows]
   __shared__ uint64_t full[F::STAGES], empty[F::STAGES];
-  __shared__ int abort_word, s_poison;
+  __shared__ int abort_word, s_poison, s_vote;
   __shared__ float s_m[FEW_WARPS][8 * NR], s_l[FEW_WARPS][8 * NR];
   __shared__ float s_rs[M];                                      // a row's score scale, log2 units
   volatile int* abort_flag = &abort_word;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 128) {
+    tma_prefetch_desc(&tm_kv);
+    if (FP8) tma_prefetch_desc(&tm_scale);
+  }
   if (threadIdx.x == 0) {
     for (int i = 0; i < F::STAGES; ++i) {
       mbar_init(&full[i], 1);
@@ -532,60 +645,48 @@ __global__ void __launch_bounds__(FEW_THREADS, NR == 1 ? 3 : 2)
         if (lane == 0) a.part_ml[at] = make_float2(mt, lt);
       }
     }
+    if (JOIN && !direct) {
+      const int first = item.w - part * M;                       // partial rows of part 0
+      unsigned long long* flags = a.flags + (long long)(first / M) * a.heads + head;
+      if (last_part(flags, part, parts, a.heads, a.word, &s_vote, FEW_WARPS * 32)) {
+        const int row = threadIdx.x >> 4;
+        if (row < rows && ok)
+          join_eight(a, (long long)(first + row) * a.heads + head, (long long)M * a.heads, parts,
+                     a.o + (long long)(q0 + (row0 + row) / G) * a.ldo + (long long)(head * G + (row0 + row) % G) * HEAD);
+        for (int s = threadIdx.x; s < parts; s += FEW_WARPS * 32) flags[(long long)s * a.heads] = 0;
+      }
+    }
   }
   if (a.beside) pdl_wait();
 }
 
-// Joins the parts of a row: a block per four rows of a key/value head, a warp per row, four values per lane.
-constexpr int MERGE_THREADS = 128;
+// Parts of the chunk kernel: a block per four rows of a key/value head, a warp per row.
+constexpr int JOIN_THREADS = 128;
 
-__global__ void __launch_bounds__(MERGE_THREADS) paged_merge_kernel(const Plan p, const FewArgs a) {
+__global__ void __launch_bounds__(JOIN_THREADS) paged_join_kernel(const Plan p, const FewArgs a) {
   pdl_wait();
   pdl_trigger();
   const int4 e = p.merge[blockIdx.x];
-  const int b = e.x, parts = e.z & 0xffff, rows = e.z >> 16;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = p.group, head = blockIdx.y;
-  const int q0 = p.q_start[b], row = e.y + warp;
+  const int b = e.x, parts = e.z & 0xffff, rows = e.z >> 16, warp = threadIdx.x >> 5, head = blockIdx.y;
+  const int q0 = p.q_start[b], row = e.y + warp, G = p.group;
   if (row >= (p.q_start[b + 1] - q0) * G) return;
-  const long long step = (long long)rows * a.heads;
-  const long long at = (long long)(e.w + warp) * a.heads + head;
-  float mt = -INFINITY;
-  for (int s = lane; s < parts; s += 32) mt = fmaxf(mt, a.part_ml[at + s * step].x);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, o));
-  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-  float lt = 0.f;
-#pragma unroll 4
-  for (int s = 0; s < parts; ++s) {
-    const float2 ml = a.part_ml[at + s * step];
-    const float4 y = *reinterpret_cast<const float4*>(a.part + (at + s * step) * HEAD + lane * 4);
-    const float f = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - mt);
-    x.x += f * y.x;
-    x.y += f * y.y;
-    x.z += f * y.z;
-    x.w += f * y.w;
-    lt += ml.x == -INFINITY ? 0.f : f * ml.y;
-  }
-  const float inv = lt == 0.f ? 0.f : 1.f / lt;
-  const int t = row / G;
-  uint2 u;
-  u.x = pack_bf16x2(x.x * inv, x.y * inv);
-  u.y = pack_bf16x2(x.z * inv, x.w * inv);
-  *reinterpret_cast<uint2*>(a.o + (long long)(q0 + t) * a.ldo + (long long)(head * G + row % G) * HEAD + lane * 4) = u;
+  join_row(a, (long long)(e.w + warp) * a.heads + head, (long long)rows * a.heads, parts,
+           a.o + (long long)(q0 + row / G) * a.ldo + (long long)(head * G + row % G) * HEAD);
 }
 
 template <bool FP8, int NR, int WR>
 static int launch_few(const Cache& c, const Plan& p, const FewArgs& a, cudaStream_t st) {
   auto kernel = paged_few_kernel<FP8, NR, WR>;
+  constexpr int SMEM = Few<FP8, NR * WR == 1>::SMEM;
   int dev = 0;
   SNU1_CUDA_CHECK(cudaGetDevice(&dev));
   static std::once_flag once[64];
   cudaError_t err = cudaSuccess;
   std::call_once(once[dev & 63], [&]() {
-    err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Few<FP8>::SMEM);
+    err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
   });
   SNU1_CUDA_CHECK(err);
-  SNU1_CUDA_CHECK(launch_pdl(kernel, dim3(p.few_count, c.heads), dim3(FEW_THREADS), Few<FP8>::SMEM, st, c.kv, c.scale, p, a));
+  SNU1_CUDA_CHECK(launch_pdl(kernel, dim3(p.few_count, c.heads), dim3(FEW_THREADS), SMEM, st, c.kv, c.scale, p, a));
   return kHostOk;
 }
 
@@ -605,10 +706,11 @@ static int launch_few(const Cache& c, const Plan& p, const FewArgs& a, cudaStrea
 using namespace snu1;
 
 // o_r = attention of row r over its sequence's first keys, rows [rows][heads of queries][128] bf16, ldq / ldo apart.
-// scratch: partial results (partial_rows x heads x (128 values, maximum, sum) in fp32), then unpack_count
-// fp16 pages of 128 tokens and their factors (a float4 per page and head).
+// scratch: partial results (partial_rows x heads x (128 values, maximum, sum) in fp32) and a 64-bit flag per part of the few
+// rows (few_parts x heads), to a multiple of 128 bytes; then unpack_count fp16 pages of 128 tokens and their factors (a float4
+// per page and head).  word: see last_part; another one for every call.
 SNU1_API int snu1_paged_attention(const void* cache, const void* plan, const void* q, long long ldq, void* o, long long ldo,
-                                  float scale, void* scratch, void* stream) {
+                                  float scale, void* scratch, unsigned long long word, void* stream) {
   using namespace paged;
   Cache c;
   Plan p;
@@ -631,6 +733,8 @@ SNU1_API int snu1_paged_attention(const void* cache, const void* plan, const voi
   a.ldo = ldo;
   a.part = (float*)scratch;
   a.part_ml = (float2*)(a.part + (long long)p.partial_rows * c.heads * HEAD);
+  a.flags = (unsigned long long*)(a.part_ml + (long long)p.partial_rows * c.heads);
+  a.word = word;
   a.pages = c.pages;
   a.heads = c.heads;
   a.scale_log2 = scale * 1.4426950408889634f;
@@ -639,7 +743,7 @@ SNU1_API int snu1_paged_attention(const void* cache, const void* plan, const voi
   cudaStream_t st = (cudaStream_t)stream;
   int rc = kHostOk;
   if (p.chunk_count > 0) {
-    void* wide = a.part_ml + (((long long)p.partial_rows * c.heads + 15) & ~15ll);      // 128-byte aligned
+    void* wide = a.flags + (((long long)(p.partial_rows + p.few_parts) * c.heads + 15) / 16 * 16 - (long long)p.partial_rows * c.heads);
     float4* factors = (float4*)((uint8_t*)wide + 2ll * 128 * HEAD * 2 * p.unpack_count * c.heads);
     if (c.fp8 && (rc = launch_widen(c, p, wide, factors, st)) != kHostOk) return rc;
     if ((rc = launch_chunks(c, p, q, ldq, p.rows, o, ldo, a.part, a.part_ml, a.scale_log2, wide, factors, st)) != kHostOk) return rc;
@@ -650,6 +754,6 @@ SNU1_API int snu1_paged_attention(const void* cache, const void* plan, const voi
     if (rc != kHostOk) return rc;
   }
   if (p.merge_count > 0)
-    SNU1_CUDA_CHECK(launch_pdl(paged_merge_kernel, dim3(p.merge_count, c.heads), dim3(MERGE_THREADS), 0, st, p, a));
+    SNU1_CUDA_CHECK(launch_pdl(paged_join_kernel, dim3(p.merge_count, c.heads), dim3(JOIN_THREADS), 0, st, p, a));
   return kHostOk;
 }

@@ -42,9 +42,9 @@ struct Plan {
   const int* unpack_first; // [seqs] first page of such a sequence in the scratch for unpacked rows
   const int4* few;         // [few_count] work of the kernel for few rows: sequence, first row, part | parts << 16, partial row (-1: none)
   const int4* chunk;       // [chunk_count] the same for chunks
-  const int4* merge;       // [merge_count] four rows to join: sequence, first row, parts | rows of a part << 16, first partial row
+  const int4* merge;       // [merge_count] four rows of a chunk to join: sequence, first row, parts | rows of a part << 16, first partial row
   int seqs, rows, width, page, group;
-  int read_count, few_count, few_rows, chunk_count, merge_count;
+  int read_count, few_count, few_rows, few_parts, chunk_count, merge_count;
   int partial_rows;        // rows of the scratch for partial results (x heads)
   int unpack_count;        // also the 128-token pages of the scratch for unpacked rows
 };

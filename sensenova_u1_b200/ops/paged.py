@@ -23,6 +23,7 @@ the one it was built on; calls that only read (write into different caches, atte
 from __future__ import annotations
 
 import ctypes
+import random
 from dataclasses import dataclass, field
 
 import numpy as np
@@ -35,8 +36,9 @@ PAGE_SIZES = (16, 32, 64, 128)
 HEAD_DIM = 128
 E4M3 = torch.float8_e4m3fn
 KEY_TILE = 64            # keys of a stage of the kernel for few rows
-FEW_SLOTS = 296          # its CTAs that run at once: two on each of 148 SMs
+FEW_SLOTS = (296, 444)   # its CTAs that run at once: two on each of 148 SMs, three of those for up to eight rows
 FEW_LEAST = 4            # a part of a sequence has at least this many key tiles
+FEW_JOIN = 8             # up to so many rows the parts of few rows join themselves (JOIN_ROWS in attn_paged.cu)
 FEW_TILE = 64            # rows (new tokens x query heads of a group) of one CTA, at most
 CHUNK_TILE = 128         # keys of a tile of the kernel for chunks, and rows of a row tile
 CHUNK_SLOTS = 148        # its CTAs that run at once
@@ -51,7 +53,7 @@ def _library():
         P, L, I = c_void_p, c_ll, c_int
         lib.snu1_paged_cache_init.argtypes = (P, P, P, I, I, I, I)
         lib.snu1_paged_read.argtypes = (P, P, P, P, P)
-        lib.snu1_paged_attention.argtypes = (P, P, P, L, P, L, c_float, P, P)
+        lib.snu1_paged_attention.argtypes = (P, P, P, L, P, L, c_float, P, ctypes.c_ulonglong, P)
         lib.snu1_paged_write.argtypes = (P, P, P, L, P, L, P)
     return lib
 
@@ -108,7 +110,7 @@ class _Args(ctypes.Structure):
     """``Plan`` of csrc/paged.cuh."""
     _fields_ = ([(n, c_void_p) for n in ("q_start", "kv_len", "cap", "table", "behind", "row_seq", "k_start", "read_pages", "unpack",
                                          "unpack_first", "few", "chunk", "merge")]
-                + [(n, c_int) for n in ("seqs", "rows", "width", "page", "group", "read_count", "few_count", "few_rows", "chunk_count",
+                + [(n, c_int) for n in ("seqs", "rows", "width", "page", "group", "read_count", "few_count", "few_rows", "few_parts", "chunk_count",
                                         "merge_count", "partial_rows", "unpack_count")])
 
 
@@ -217,24 +219,25 @@ def _lay_out(q_lens, kv_lens, tables, page: int, pages: int, group: int, kv_head
 
     seq, row0 = tiles_of(few_q, few_rows)
     tiles = -(-cap[seq] // KEY_TILE)
-    few, merge, partial = _items(seq, row0, tiles, _shares(tiles, kv_heads, FEW_SLOTS, FEW_LEAST), few_q, few_rows, 0)
+    few, merge, partial = _items(seq, row0, tiles, _shares(tiles, kv_heads, FEW_SLOTS[few_rows <= FEW_JOIN], FEW_LEAST), few_q, few_rows, 0)
     seq, row0 = tiles_of(np.where(chunked, q_rows, 0), chunk_rows)
     if limits is None:                                        # a row tile reads up to its last token
         last = np.minimum((row0 + chunk_rows - 1) // group, q[seq] - 1)
         tiles = -(-(cap[seq] - q[seq] + 1 + last) // CHUNK_TILE)
     else:
         tiles = -(-kv[seq] // CHUNK_TILE)
+    few_parts = partial // few_rows if few_rows <= FEW_JOIN else 0       # parts that join themselves
     chunk, more, partial = _items(seq, row0, tiles, _waves(tiles, kv_heads, CHUNK_SLOTS), q_rows, chunk_rows, partial)
+    merge = more if few_rows <= FEW_JOIN else np.concatenate([merge, more])
     unpack = unpack_first = None
     if fp8 and len(chunk):
         wide = np.where(chunked, -(-cap // CHUNK_TILE), 0)    # 128-token pages
         unpack, unpack_first = pages_of(wide), start(wide)[:n]
-    merge = np.concatenate([merge, more])
     arrays = dict(q_start=start(q), kv_len=kv.astype(np.int32), cap=cap.astype(np.int32), table=table, behind=behind, row_seq=row_seq,
                   k_start=start(kv), read_pages=pages_of(read), unpack=unpack, unpack_first=unpack_first, few=few, chunk=chunk,
                   merge=merge)
     counts = dict(seqs=n, rows=rows, width=width, page=page, group=group, read_count=int(read.sum()), few_count=len(few),
-                  few_rows=few_rows, chunk_count=len(chunk), merge_count=len(merge), partial_rows=partial, unpack_count=0 if unpack is None else len(unpack))
+                  few_rows=few_rows, few_parts=few_parts, chunk_count=len(chunk), merge_count=len(merge), partial_rows=partial, unpack_count=0 if unpack is None else len(unpack))
     return arrays, counts
 
 
@@ -309,13 +312,14 @@ def build_plan(cache: PagedCache, heads: int, q_lens, kv_lens, tables, limits=No
     args = _Args(**{name: store.data_ptr() + 4 * o for name, o in at.items()}, **counts)
     n = counts["seqs"]
     joined = counts["partial_rows"] * cache.kv_heads
-    scratch = joined * HEAD_DIM * 4 + (joined + 15) // 16 * 128 + counts["unpack_count"] * cache.kv_heads * (2 * CHUNK_TILE * HEAD_DIM * 2 + 16)
+    scratch = joined * HEAD_DIM * 4 + (joined + counts["few_parts"] * cache.kv_heads + 15) // 16 * 128 + counts["unpack_count"] * cache.kv_heads * (2 * CHUNK_TILE * HEAD_DIM * 2 + 16)
     return PagedPlan(heads, cache.kv_heads, cache.page, cache.pages, cache.data.dtype, cache.device,
                      [int(x) for x in q_lens], [int(x) for x in kv_lens],
                      counts["rows"], int(arrays["k_start"][-1]), scratch, store[at["kv_len"]:at["kv_len"] + n], grow, store, args)
 
 
 _BF16 = torch.bfloat16
+_words = random.Random()          # never 0, the word of a flag that is not set; of its own: a program that seeds the global one does not repeat them
 
 
 def _check(cache: PagedCache, plan: PagedPlan) -> None:
@@ -376,5 +380,5 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, plan: PagedPlan, scale: 
     if plan.rows:
         scratch = torch.empty(plan.scratch, dtype=torch.uint8, device=plan.device) if plan.scratch else None
         _call(plan._index, "paged_attention", cache._addr, plan._addr, q.data_ptr(), ldq, out.data_ptr(), ldo, scale,
-              scratch.data_ptr() if plan.scratch else None)
+              scratch.data_ptr() if plan.scratch else None, _words.getrandbits(64) | 1)
     return out

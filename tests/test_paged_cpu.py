@@ -90,11 +90,16 @@ def test_every_row_meets_every_key_once(q, kv, group, heads):
         for r in range(row0, min(row0 + 4, q[b] * group)):
             assert (b, r) not in joined
             joined[(b, r)] = (z & 0xffff, z >> 16, at + r - row0)
-    assert set(joined) == {(b, r) for (b, r), count in seen.items() if count > 1}
-    for b, row0, z, at in a["few"].tolist() + a["chunk"].tolist():
+    assert set(joined) == {(b, r) for (b, r), count in seen.items() if count > 1 and (
+        c["few_rows"] > paged.FEW_JOIN or q[b] * group > paged.FEW_TILE and group <= 128)}
+    first = {(b, row0): at for b, row0, z, at in a["few"].tolist() if at >= 0 and z & 0xffff == 0}
+    for b, row0, z, at in a["few"].tolist():                          # joined by the parts themselves: side by side, in whole parts
+        assert at < 0 or at == first[(b, row0)] + (z & 0xffff) * c["few_rows"] and at % c["few_rows"] == 0
+        assert at < 0 or c["few_rows"] > paged.FEW_JOIN or at < c["few_parts"] * c["few_rows"]
+    for b, row0, z, at in a["chunk"].tolist():
         if at >= 0:
             for r in range(row0, q[b] * group):
-                count, m, first = joined[(b, r)]
+                count, _, first = joined[(b, r)]
                 assert count == z >> 16 and (r - row0 >= m or at + r - row0 == first + (z & 0xffff) * m)
                 if r - row0 + 1 >= m:
                     break
