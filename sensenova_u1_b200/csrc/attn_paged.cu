@@ -248,15 +248,16 @@ __global__ void __launch_bounds__(FEW_THREADS, Few<FP8, NR * WR == 1>::CTAS)
     mbar_fence_init();
   }
   __syncthreads();
+  // what the plan's host side has set, before the wait: no launch in front writes it
+  const int4 item = p.few[blockIdx.x];
+  const int b = item.x, row0 = item.y, part = item.z & 0xffff, parts = item.z >> 16;
+  const int head = blockIdx.y, G = p.group;
+  const int q0 = p.q_start[b], q_len = p.q_start[b + 1] - q0;
   // Chunks in front (attn_paged_sm100.cu) have waited for all work before them when this kernel may start, and nothing that
   // they write is read here: it only has to end after them.
   if (!a.beside) pdl_wait();
   pdl_trigger();
 
-  const int4 item = p.few[blockIdx.x];
-  const int b = item.x, row0 = item.y, part = item.z & 0xffff, parts = item.z >> 16;
-  const int head = blockIdx.y, G = p.group;
-  const int q0 = p.q_start[b], q_len = p.q_start[b + 1] - q0;
   const int kv_len = seq_len(p, b);
   const int rows = min(M, q_len * G - row0);
   // the furthest key that a row of this tile may read, and the nearest limit

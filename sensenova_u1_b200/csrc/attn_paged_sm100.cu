@@ -168,13 +168,13 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  pdl_wait();
-  pdl_trigger();
-
+  // what the plan's host side has set, before the wait: no launch in front writes it
   const int4 item = p.chunk[blockIdx.x / args.heads];
   const int b = item.x, part = item.z & 0xffff, parts = item.z >> 16;
   const int kvh = blockIdx.x % args.heads, G = p.group, T = 128 / G;       // tokens of a row tile
   const int q0 = p.q_start[b], q_len = p.q_start[b + 1] - q0;
+  pdl_wait();
+  pdl_trigger();
   const int kv_len = seq_len(p, b);
   const int token0 = item.y / G;
   int max_a, max_b, min_a, min_b;               // the largest and the smallest limit of row tiles A and B

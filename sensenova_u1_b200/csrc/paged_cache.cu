@@ -29,11 +29,25 @@ __device__ __forceinline__ void decode8(uint2 u, float (&f)[8]) {
   }
 }
 
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+// two numbers as codes, the first in the low byte
+__device__ __forceinline__ uint32_t e4m3x2(uint64_t x) {
+  float lo, hi;
+  unpack_f32x2(x, lo, hi);
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
 constexpr int WRITE_THREADS = 256;
 constexpr int WRITE_TOKENS = 16;     // most tokens of a block
-constexpr int WRITE_DEEP = 4;        // (token, head) pairs that a warp has in flight
+constexpr int WRITE_DEEP = 4;        // heads of a token that a warp has in flight
 
-// A block writes ``tokens`` rows of all heads; a warp a (token, head) at a time, 16 lanes the key, 16 the value.
+// A block writes ``tokens`` rows of all heads; a warp four heads of a token at a time, 16 lanes the keys, 16 the values.
 template <bool FP8>
 __global__ void __launch_bounds__(WRITE_THREADS)
     paged_write_kernel(const __nv_bfloat16* __restrict__ k, long long ldk, const __nv_bfloat16* __restrict__ v, long long ldv,
@@ -56,49 +70,58 @@ __global__ void __launch_bounds__(WRITE_THREADS)
   }
   const __nv_bfloat16* src = (kv ? v : k) + (long long)row0 * (kv ? ldv : ldk) + c * 8;
   const long long ld = kv ? ldv : ldk;
-  const int pairs = count * heads;
+  const int fours = (heads + WRITE_DEEP - 1) / WRITE_DEEP, tasks = count * fours;
   bool known = false;
-  for (int first = warp; first < pairs; first += WRITE_THREADS / 32 * WRITE_DEEP) {
+  for (int task = warp; task < tasks; task += WRITE_THREADS / 32) {
+    const int token = task / fours, head = (task - token * fours) * WRITE_DEEP;
+    const __nv_bfloat16* from = src + token * ld + head * HEAD;
     uint4 x[WRITE_DEEP];
-    int token[WRITE_DEEP], head[WRITE_DEEP];
 #pragma unroll
-    for (int i = 0; i < WRITE_DEEP; ++i) {
-      const int pair = first + i * (WRITE_THREADS / 32);
-      token[i] = pair / heads;
-      head[i] = pair - token[i] * heads;
-      x[i] = pair < pairs ? *reinterpret_cast<const uint4*>(src + token[i] * ld + head[i] * HEAD) : make_uint4(0, 0, 0, 0);
-    }
+    for (int i = 0; i < WRITE_DEEP; ++i)
+      x[i] = head + i < heads ? *reinterpret_cast<const uint4*>(from + i * HEAD) : make_uint4(0, 0, 0, 0);
     if (!known) {
       __syncthreads();
       known = true;
     }
+    const long long base = place[token];
+    if (base < 0) continue;                          // (the whole warp)
+    const long long at = base + (long long)(kv * heads + head) * p.page;      // of the first head; the next is a page's rows on
+    uint8_t* to = data + at * (FP8 ? HEAD : 2 * HEAD) + c * (FP8 ? 8 : 16);
+    const int step = p.page * (FP8 ? HEAD : 2 * HEAD);
+    if (!FP8) {
+#pragma unroll
+      for (int i = 0; i < WRITE_DEEP; ++i)
+        if (head + i < heads) *reinterpret_cast<uint4*>(to + i * step) = x[i];
+      continue;
+    }
+    // The instructions bound this (144 per warp and head took 44 us for 32001 tokens of 8 heads, the bytes take 31), so a warp has
+    // four heads of one token, the largest value is found two 16-bit words at a time, and a lane divides for one of the
+    // four rows.  As whole numbers a NaN is larger than infinity, which is larger than every finite value.
+    uint32_t tops[WRITE_DEEP];
 #pragma unroll
     for (int i = 0; i < WRITE_DEEP; ++i) {
-      const bool on = first + i * (WRITE_THREADS / 32) < pairs;
-      const long long base = on ? place[token[i]] : -1;
-      const long long at = base + (long long)(kv * heads + head[i]) * p.page;
-      if (!FP8) {
-        if (base >= 0) *reinterpret_cast<uint4*>(data + at * (HEAD * 2) + c * 16) = x[i];
-        continue;
-      }
+      uint32_t t = max_u16x2(max_u16x2(x[i].x & 0x7fff7fffu, x[i].y & 0x7fff7fffu), max_u16x2(x[i].z & 0x7fff7fffu, x[i].w & 0x7fff7fffu));
+#pragma unroll
+      for (int o = 1; o < 16; o <<= 1) t = max_u16x2(t, __shfl_xor_sync(0xffffffffu, t, o));
+      tops[i] = t;
+    }
+    // (picked by hand: an index would put the array in local memory)
+    const uint32_t t = c & 2 ? (c & 1 ? tops[3] : tops[2]) : (c & 1 ? tops[1] : tops[0]);
+    const uint32_t top = max(t << 16, t & 0xffff0000u);
+    const bool finite = top < 0x7f800000u;           // otherwise NaN is the scale, and the codes are zeros
+    const float a = fmaxf(__uint_as_float(top), TINY), inv = finite ? __fdiv_rn(E4M3_MAX, a) : 0.f;
+    if (c < WRITE_DEEP && head + c < heads) scales[at + c * p.page] = finite ? __fdiv_rn(a, E4M3_MAX) : __int_as_float(0x7fffffff);
+#pragma unroll
+    for (int i = 0; i < WRITE_DEEP; ++i) {
+      const float f = __shfl_sync(0xffffffffu, inv, (lane & 16) + i);
+      const uint64_t f2 = pack_f32x2(f, f);
       const uint32_t u[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-      // as whole numbers: a NaN is larger than infinity, which is larger than every finite value
-      uint32_t top = 0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) top = max(top, max(u[j] << 16 & 0x7fffffffu, u[j] & 0x7fff0000u));
-#pragma unroll
-      for (int o = 1; o < 16; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-      const bool finite = top < 0x7f800000u;           // otherwise NaN is the scale, and the codes are zeros
-      const float a = fmaxf(__uint_as_float(top), TINY), inv = __fdiv_rn(E4M3_MAX, a);
       uint32_t q[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        q[j] = __nv_cvt_float2_to_fp8x2(make_float2(__uint_as_float(u[j] << 16) * inv, __uint_as_float(u[j] & 0xffff0000u) * inv),
-                                        __NV_SATFINITE, __NV_E4M3);
-      if (base >= 0) {
-        *reinterpret_cast<uint2*>(data + at * HEAD + c * 8) = finite ? make_uint2(q[0] | q[1] << 16, q[2] | q[3] << 16) : make_uint2(0, 0);
-        if (c == 0) scales[at] = finite ? __fdiv_rn(a, E4M3_MAX) : __int_as_float(0x7fffffff);
-      }
+      for (int j = 0; j < 4; ++j) q[j] = e4m3x2(mul_f32x2(bf16x2_to_f32x2(u[j]), f2));
+      if (head + i < heads)
+        *reinterpret_cast<uint2*>(to + i * step) =
+            f != 0.f ? make_uint2(__byte_perm(q[0], q[1], 0x5410), __byte_perm(q[2], q[3], 0x5410)) : make_uint2(0, 0);
     }
   }
   if (!known) __syncthreads();
@@ -113,12 +136,12 @@ template <bool FP8>
 __global__ void __launch_bounds__(READ_THREADS)
     paged_read_kernel(const uint8_t* __restrict__ data, const float* __restrict__ scales, int pages, int heads, int page, Plan p,
                       __nv_bfloat16* __restrict__ out, __nv_bfloat16* __restrict__ out2, int* status) {
-  pdl_wait();
-  pdl_trigger();
-  const int2 e = p.read_pages[blockIdx.x];
+  const int2 e = p.read_pages[blockIdx.x];                           // set by the host, as is k_start
   const int page_log = __ffs(page) - 1;
   const int b = e.x, pos0 = e.y * page, c = threadIdx.x & 15;
   const int k0 = p.k_start[b], len = p.k_start[b + 1] - k0;
+  pdl_wait();
+  pdl_trigger();
   const int pg = p.table[(long long)b * p.width + e.y];
   const bool there = pg >= 0 && pg < pages;
   if (!there && threadIdx.x == 0) report_status(status, kBadPage, 9);

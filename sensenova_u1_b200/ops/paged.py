@@ -135,6 +135,7 @@ class PagedPlan:
 
     def __post_init__(self):
         self._index = self.device.index
+        self._out = (self.rows, self.heads, HEAD_DIM)
         self._key = (self.dtype, self.page, self.kv_heads, self._index)
         self._addr = ctypes.addressof(self._args)
 
@@ -360,7 +361,8 @@ def paged_read(cache: PagedCache, plan: PagedPlan) -> tuple[torch.Tensor, torch.
     """The cached keys and values of the plan's sequences, one sequence after another: two tensors [plan.keys, kv_heads, 128] bf16
     (e4m3: code times scale, rounded once)."""
     _check(cache, plan)
-    k, v = (torch.empty(plan.keys, cache.kv_heads, HEAD_DIM, dtype=_BF16, device=plan.device) for _ in range(2))
+    k = torch.empty(plan.keys, cache.kv_heads, HEAD_DIM, dtype=_BF16, device=plan.device)
+    v = torch.empty_like(k)
     if plan.keys:
         _call(plan._index, "paged_read", cache._addr, plan._addr, k.data_ptr(), v.data_ptr())
     return k, v
@@ -373,12 +375,12 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, plan: PagedPlan, scale: 
     _check(cache, plan)
     ldq = _row_stride("q", q, plan, plan.heads)
     if out is None:
-        out = torch.empty(plan.rows, plan.heads, HEAD_DIM, dtype=_BF16, device=plan.device)
+        out = q.new_empty(plan._out)
         ldo = plan.heads * HEAD_DIM
     else:
         ldo = _row_stride("out", out, plan, plan.heads)
     if plan.rows:
-        scratch = torch.empty(plan.scratch, dtype=torch.uint8, device=plan.device) if plan.scratch else None
+        scratch = q.new_empty(plan.scratch // 2) if plan.scratch else None
         _call(plan._index, "paged_attention", cache._addr, plan._addr, q.data_ptr(), ldq, out.data_ptr(), ldo, scale,
               scratch.data_ptr() if plan.scratch else None, _words.getrandbits(64) | 1)
     return out
