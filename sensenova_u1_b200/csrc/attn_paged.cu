@@ -6,7 +6,9 @@
 // The rows of a (sequence, key/value head) are its new tokens times the query heads of the group, up to 64 per CTA.  What
 // bounds it is the stream of keys and values, so the work is split over keys: a work item is one part of a sequence, the
 // parts are made as equal as they can be over the whole batch (ops/paged.py), and their unnormalised results (maximum, sum,
-// weighted values, fp32) are joined in a fixed order by whichever CTA finds all parts there: see join_parts.
+// weighted values, fp32) are joined in a fixed order.  Where every sequence can have as many parts as the longest, up to
+// eight, and all CTAs still run at once, the parts of a sequence are a cluster and meet in distributed shared memory: a
+// small batch, where latency counts.  Otherwise they meet in scratch, see last_part and paged_join_kernel.
 //
 // One warp asks for whole pages through TMA (keys and values of one head in one box), several stages ahead; four warps
 // compute with mma.sync m16n8k16, keys (then the width of a head) on the 16-side and rows on the 8-side: S^T = K q^T,
@@ -38,6 +40,7 @@ namespace paged {
 
 constexpr int FEW_WARPS = 4;                              // warps that compute; one more asks for pages
 constexpr int FEW_THREADS = FEW_WARPS * 32 + 32;
+constexpr int FEW_LD = 132;                               // a row of 128 values where warps meet, padded
 
 // SMALL: up to eight rows.  Their registers let three CTAs run on an SM, with two stages each instead of three.
 template <bool FP8, bool SMALL>
@@ -110,6 +113,7 @@ struct FewArgs {
   float scale_log2;
   int* status;
   int beside;         // the launch in front is that of the chunks: run beside it
+  int cluster;        // parts of every sequence, which are a cluster; 1: parts meet in scratch
 };
 
 // Up to so many rows the parts join themselves, more are joined by a launch of their own (paged_join_kernel, which has as many
@@ -232,6 +236,10 @@ __global__ void __launch_bounds__(FEW_THREADS, Few<FP8, NR * WR == 1>::CTAS)
   __shared__ int abort_word, s_poison, s_vote;
   __shared__ float s_m[FEW_WARPS][8 * NR], s_l[FEW_WARPS][8 * NR];
   __shared__ float s_rs[M];                                      // a row's score scale, log2 units
+  // in the ring, behind where warps meet at the end: this CTA's results, read by its cluster
+  float* s_part = reinterpret_cast<float*>(smem) + FEW_WARPS * 8 * NR * FEW_LD;      // [rows][128]
+  float2* s_part_ml = reinterpret_cast<float2*>(s_part + M * HEAD);
+  static_assert(FEW_WARPS * 8 * NR * FEW_LD * 4 + M * (HEAD * 4 + 8) <= F::SMEM - 1024, "results fit the ring");
   volatile int* abort_flag = &abort_word;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 128) {
@@ -583,8 +591,8 @@ __global__ void __launch_bounds__(FEW_THREADS, Few<FP8, NR * WR == 1>::CTAS)
     ok = __all_sync(0xffffffffu, ok);
     // Warps of the same rows meet in the ring: every stage has been read (the barrier), and TMA asks for nothing more.
     named_bar_sync(1, FEW_WARPS * 32);
-    float* ring = reinterpret_cast<float*>(smem);                // [warp][8 NR][132]
-    constexpr int LD = 132;
+    float* ring = reinterpret_cast<float*>(smem);                // [warp][8 NR][FEW_LD]
+    constexpr int LD = FEW_LD;
 #pragma unroll
     for (int i = 0; i < NR; ++i)
 #pragma unroll
@@ -613,6 +621,7 @@ __global__ void __launch_bounds__(FEW_THREADS, Few<FP8, NR * WR == 1>::CTAS)
       }
     named_bar_sync(1, FEW_WARPS * 32);
     const bool direct = item.w < 0;
+    const bool near = a.cluster > 1;
     // a warp finishes one row at a time, four values per lane
     for (int row = warp; row < rows; row += FEW_WARPS) {
       const int w0 = row / (8 * NR) * WK, rr = row % (8 * NR);
@@ -633,7 +642,10 @@ __global__ void __launch_bounds__(FEW_THREADS, Few<FP8, NR * WR == 1>::CTAS)
         lt += mw == -INFINITY ? 0.f : f * s_l[w0 + w][rr];
       }
       if (!ok) continue;
-      if (direct) {
+      if (near) {
+        *reinterpret_cast<float4*>(s_part + row * HEAD + lane * 4) = x;
+        if (lane == 0) s_part_ml[row] = make_float2(mt, lt);
+      } else if (direct) {
         const float inv = lt == 0.f ? 0.f : 1.f / lt;            // a row without keys gives zeros
         const int t = (row0 + row) / G;
         uint2 u;
@@ -657,6 +669,38 @@ __global__ void __launch_bounds__(FEW_THREADS, Few<FP8, NR * WR == 1>::CTAS)
         for (int s = threadIdx.x; s < parts; s += FEW_WARPS * 32) flags[(long long)s * a.heads] = 0;
       }
     }
+  }
+  if (a.cluster > 1) {
+    __syncwarp();
+    cluster_sync_all();
+    if (warp < FEW_WARPS) {
+      for (int row = part * FEW_WARPS + warp; row < rows; row += parts * FEW_WARPS) {
+        const float* ml = reinterpret_cast<const float*>(s_part_ml + row);
+        float mt = -INFINITY;
+        for (int s = 0; s < parts; ++s) mt = fmaxf(mt, ld_cluster(ml[0], s));
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+        float lt = 0.f;
+#pragma unroll 4
+        for (int s = 0; s < parts; ++s) {
+          const float ms = ld_cluster(ml[0], s), ls = ld_cluster(ml[1], s);
+          const float4 y = ld_cluster_f4(smem_u32(s_part + row * HEAD + lane * 4), s);
+          const float f = ms == -INFINITY ? 0.f : fast_exp2(ms - mt);
+          x.x += f * y.x;
+          x.y += f * y.y;
+          x.z += f * y.z;
+          x.w += f * y.w;
+          lt += ms == -INFINITY ? 0.f : f * ls;
+        }
+        const float inv = lt == 0.f ? 0.f : 1.f / lt;            // a row without keys gives zeros
+        const int t = (row0 + row) / G;
+        uint2 u;
+        u.x = pack_bf16x2(x.x * inv, x.y * inv);
+        u.y = pack_bf16x2(x.z * inv, x.w * inv);
+        *reinterpret_cast<uint2*>(a.o + (long long)(q0 + t) * a.ldo + (long long)(head * G + (row0 + row) % G) * HEAD + lane * 4) = u;
+      }
+    }
+    __syncwarp();
+    cluster_sync_all();                    // nobody leaves while its results are read
   }
   if (a.beside) pdl_wait();
 }
@@ -687,7 +731,22 @@ static int launch_few(const Cache& c, const Plan& p, const FewArgs& a, cudaStrea
     err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
   });
   SNU1_CUDA_CHECK(err);
-  SNU1_CUDA_CHECK(launch_pdl(kernel, dim3(p.few_count, c.heads), dim3(FEW_THREADS), SMEM, st, c.kv, c.scale, p, a));
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = a.cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.gridDim = dim3(p.few_count, c.heads);
+  cfg.blockDim = dim3(FEW_THREADS);
+  cfg.dynamicSmemBytes = SMEM;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = a.cluster > 1 ? 2 : 1;
+  SNU1_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, c.kv, c.scale, p, a));
   return kHostOk;
 }
 
@@ -717,6 +776,10 @@ SNU1_API int snu1_paged_attention(const void* cache, const void* plan, const voi
   Plan p;
   memcpy(&c, cache, sizeof(c));
   memcpy(&p, plan, sizeof(p));
+  if (p.layout != paged::PLAN_LAYOUT) {
+    set_last_error("paged: this plan was made for another version of the library");
+    return kHostBadArg;
+  }
   if (p.rows <= 0) return kHostOk;
   if (p.page != c.page || ldq % 8 || ldo % 8 ||
       ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(o) | reinterpret_cast<uintptr_t>(scratch)) & 15) != 0) {
@@ -741,6 +804,7 @@ SNU1_API int snu1_paged_attention(const void* cache, const void* plan, const voi
   a.scale_log2 = scale * 1.4426950408889634f;
   a.status = device_status_word();
   a.beside = p.chunk_count > 0;
+  a.cluster = p.few_cluster;
   cudaStream_t st = (cudaStream_t)stream;
   int rc = kHostOk;
   if (p.chunk_count > 0) {

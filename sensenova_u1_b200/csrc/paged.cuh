@@ -28,6 +28,8 @@ struct alignas(64) Cache {
   int pages, heads, page, fp8;
 };
 
+constexpr int PLAN_LAYOUT = 0x70670001;
+
 // Device arrays and counts of a plan (ops/paged.py builds it).
 struct Plan {
   const int* q_start;      // [seqs + 1] first query row of a sequence
@@ -44,9 +46,10 @@ struct Plan {
   const int4* chunk;       // [chunk_count] the same for chunks
   const int4* merge;       // [merge_count] four rows of a chunk to join: sequence, first row, parts | rows of a part << 16, first partial row
   int seqs, rows, width, page, group;
-  int read_count, few_count, few_rows, few_parts, chunk_count, merge_count;
+  int read_count, few_count, few_rows, few_parts, few_cluster, chunk_count, merge_count;
   int partial_rows;        // rows of the scratch for partial results (x heads)
   int unpack_count;        // also the 128-token pages of the scratch for unpacked rows
+  int layout;              // PLAN_LAYOUT; changes with the fields
 };
 
 __device__ __forceinline__ int seq_len(const Plan& p, int b) { return max(0, min(p.kv_len[b], p.cap[b])); }

@@ -317,6 +317,10 @@ SNU1_API int snu1_paged_write(const void* cache, const void* plan, const void* k
   paged::Plan p;
   memcpy(&c, cache, sizeof(c));
   memcpy(&p, plan, sizeof(p));
+  if (p.layout != paged::PLAN_LAYOUT) {
+    set_last_error("paged: this plan was made for another version of the library");
+    return kHostBadArg;
+  }
   if (p.rows <= 0) return kHostOk;
   if (p.page != c.page || ldk % 8 || ldv % 8 || ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) != 0) {
     set_last_error("paged_write: rows must be 16-byte aligned, and the plan made for this page size");
@@ -337,6 +341,10 @@ SNU1_API int snu1_paged_read(const void* cache, const void* plan, void* k, void*
   paged::Plan p;
   memcpy(&c, cache, sizeof(c));
   memcpy(&p, plan, sizeof(p));
+  if (p.layout != paged::PLAN_LAYOUT) {
+    set_last_error("paged: this plan was made for another version of the library");
+    return kHostBadArg;
+  }
   if (p.read_count <= 0) return kHostOk;
   if (p.page != c.page || ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) != 0) {
     set_last_error("paged_read: outputs must be 16-byte aligned, and the plan made for this page size");

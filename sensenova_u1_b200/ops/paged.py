@@ -39,6 +39,7 @@ KEY_TILE = 64            # keys of a stage of the kernel for few rows
 FEW_SLOTS = (296, 444)   # its CTAs that run at once: two on each of 148 SMs, three of those for up to eight rows
 FEW_LEAST = 4            # a part of a sequence has at least this many key tiles
 FEW_JOIN = 8             # up to so many rows the parts of few rows join themselves (JOIN_ROWS in attn_paged.cu)
+FEW_CLUSTER = 8          # up to so many parts are a cluster, if all sequences can have as many
 FEW_TILE = 64            # rows (new tokens x query heads of a group) of one CTA, at most
 CHUNK_TILE = 128         # keys of a tile of the kernel for chunks, and rows of a row tile
 CHUNK_SLOTS = 148        # its CTAs that run at once
@@ -106,12 +107,15 @@ class PagedCache:
         return self._data.device
 
 
+PLAN_LAYOUT = 0x70670001     # last word of a plan: the library refuses one whose fields lie elsewhere
+
+
 class _Args(ctypes.Structure):
     """``Plan`` of csrc/paged.cuh."""
     _fields_ = ([(n, c_void_p) for n in ("q_start", "kv_len", "cap", "table", "behind", "row_seq", "k_start", "read_pages", "unpack",
                                          "unpack_first", "few", "chunk", "merge")]
-                + [(n, c_int) for n in ("seqs", "rows", "width", "page", "group", "read_count", "few_count", "few_rows", "few_parts", "chunk_count",
-                                        "merge_count", "partial_rows", "unpack_count")])
+                + [(n, c_int) for n in ("seqs", "rows", "width", "page", "group", "read_count", "few_count", "few_rows", "few_parts", "few_cluster",
+                                        "chunk_count", "merge_count", "partial_rows", "unpack_count", "layout")])
 
 
 @dataclass
@@ -220,7 +224,16 @@ def _lay_out(q_lens, kv_lens, tables, page: int, pages: int, group: int, kv_head
 
     seq, row0 = tiles_of(few_q, few_rows)
     tiles = -(-cap[seq] // KEY_TILE)
-    few, merge, partial = _items(seq, row0, tiles, _shares(tiles, kv_heads, FEW_SLOTS[few_rows <= FEW_JOIN], FEW_LEAST), few_q, few_rows, 0)
+    slots = FEW_SLOTS[few_rows <= FEW_JOIN]
+    parts = _shares(tiles, kv_heads, slots, FEW_LEAST)
+    cluster = int(parts.max()) if len(parts) else 1
+    if 1 < cluster <= FEW_CLUSTER and len(seq) * cluster * kv_heads <= slots:      # as many parts for everybody, side by side
+        part = np.tile(np.arange(cluster), len(seq))
+        few = np.stack([np.repeat(seq, cluster), np.repeat(row0, cluster), part | cluster << 16, np.full(len(part), -1)], 1).astype(np.int32)
+        merge, partial = np.zeros((0, 4), np.int32), 0
+    else:
+        few, merge, partial = _items(seq, row0, tiles, parts, few_q, few_rows, 0)
+        cluster = 1
     seq, row0 = tiles_of(np.where(chunked, q_rows, 0), chunk_rows)
     if limits is None:                                        # a row tile reads up to its last token
         last = np.minimum((row0 + chunk_rows - 1) // group, q[seq] - 1)
@@ -238,7 +251,8 @@ def _lay_out(q_lens, kv_lens, tables, page: int, pages: int, group: int, kv_head
                   k_start=start(kv), read_pages=pages_of(read), unpack=unpack, unpack_first=unpack_first, few=few, chunk=chunk,
                   merge=merge)
     counts = dict(seqs=n, rows=rows, width=width, page=page, group=group, read_count=int(read.sum()), few_count=len(few),
-                  few_rows=few_rows, few_parts=few_parts, chunk_count=len(chunk), merge_count=len(merge), partial_rows=partial, unpack_count=0 if unpack is None else len(unpack))
+                  few_rows=few_rows, few_parts=few_parts, few_cluster=cluster, chunk_count=len(chunk), merge_count=len(merge),
+                  partial_rows=partial, unpack_count=0 if unpack is None else len(unpack), layout=PLAN_LAYOUT)
     return arrays, counts
 
 

@@ -73,7 +73,7 @@ def test_every_row_meets_every_key_once(q, kv, group, heads):
         for b, row0, z, at in a[name].tolist():
             part, count = z & 0xffff, z >> 16
             parts.setdefault((b, row0, m, count), []).append(part)
-            assert (at < 0) == (count == 1)
+            assert (at < 0) == (count == 1 or name == "few" and c["few_cluster"] > 1)
             if at >= 0:                                               # nobody else's scratch
                 rows = set(range(at, at + m))
                 assert not rows & written and at + m <= c["partial_rows"]
@@ -90,8 +90,13 @@ def test_every_row_meets_every_key_once(q, kv, group, heads):
         for r in range(row0, min(row0 + 4, q[b] * group)):
             assert (b, r) not in joined
             joined[(b, r)] = (z & 0xffff, z >> 16, at + r - row0)
+    if c["few_cluster"] > 1:                                          # the parts of every tile of rows side by side
+        k = c["few_cluster"]
+        assert len(a["few"]) % k == 0 and len(a["few"]) * heads <= 444
+        assert [z for _, _, z, _ in a["few"].tolist()] == [i % k | k << 16 for i in range(len(a["few"]))]
+        assert all(len({tuple(x) for x in a["few"][i:i + k, :2].tolist()}) == 1 for i in range(0, len(a["few"]), k))
     assert set(joined) == {(b, r) for (b, r), count in seen.items() if count > 1 and (
-        c["few_rows"] > paged.FEW_JOIN or q[b] * group > paged.FEW_TILE and group <= 128)}
+        c["few_rows"] > paged.FEW_JOIN and c["few_cluster"] == 1 or q[b] * group > paged.FEW_TILE and group <= 128)}
     first = {(b, row0): at for b, row0, z, at in a["few"].tolist() if at >= 0 and z & 0xffff == 0}
     for b, row0, z, at in a["few"].tolist():                          # joined by the parts themselves: side by side, in whole parts
         assert at < 0 or at == first[(b, row0)] + (z & 0xffff) * c["few_rows"] and at % c["few_rows"] == 0
@@ -131,3 +136,19 @@ def test_a_cache_is_refused_in_host_memory():
         paged.PagedCache(data.to(torch.float8_e4m3fn))                  # e4m3 has
     with pytest.raises(ValueError):
         paged.PagedCache(data.to(torch.float8_e4m3fn), torch.zeros(2, 2, 16))
+
+
+def test_the_plan_has_the_fields_of_the_kernels():
+    """ops/paged.py hands ``Plan`` of csrc/paged.cuh over by address: the same fields in the same order, or nothing is where it should be."""
+    import re
+    from pathlib import Path
+    src = (Path(paged.__file__).parent.parent / "csrc" / "paged.cuh").read_text()
+    body = src[src.index("struct Plan {"):]
+    names = []
+    for line in body[:body.index("};")].splitlines()[1:]:
+        m = re.match(r"\s*(const int\d?\*|int)\s+([^;]*);", line)
+        if m:
+            kind = paged.c_void_p if "*" in m.group(1) else paged.c_int
+            names += [(x.strip(), kind) for x in m.group(2).split(",")]
+    assert names == paged._Args._fields_
+    assert f"PLAN_LAYOUT = {paged.PLAN_LAYOUT:#x}" in src
