@@ -139,7 +139,9 @@ class PagedPlan:
 
     def __post_init__(self):
         self._index = self.device.index
-        self._out = (self.rows, self.heads, HEAD_DIM)
+        # what an output and the scratch are like (half the host time of naming shape, type and device)
+        like = self._store.view(torch.bfloat16)[:1]
+        self._out, self._scratch = like.expand(self.rows, self.heads, HEAD_DIM), like.expand(self.scratch // 2)
         self._key = (self.dtype, self.page, self.kv_heads, self._index)
         self._addr = ctypes.addressof(self._args)
 
@@ -389,12 +391,12 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, plan: PagedPlan, scale: 
     _check(cache, plan)
     ldq = _row_stride("q", q, plan, plan.heads)
     if out is None:
-        out = q.new_empty(plan._out)
+        out = torch.empty_like(plan._out)
         ldo = plan.heads * HEAD_DIM
     else:
         ldo = _row_stride("out", out, plan, plan.heads)
     if plan.rows:
-        scratch = q.new_empty(plan.scratch // 2) if plan.scratch else None
+        scratch = torch.empty_like(plan._scratch) if plan.scratch else None
         _call(plan._index, "paged_attention", cache._addr, plan._addr, q.data_ptr(), ldq, out.data_ptr(), ldo, scale,
               scratch.data_ptr() if plan.scratch else None, _words.getrandbits(64) | 1)
     return out
