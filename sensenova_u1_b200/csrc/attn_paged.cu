@@ -712,9 +712,9 @@ __global__ void __launch_bounds__(JOIN_THREADS) paged_join_kernel(const Plan p, 
   pdl_wait();
   pdl_trigger();
   const int4 e = p.merge[blockIdx.x];
-  const int b = e.x, parts = e.z & 0xffff, rows = e.z >> 16, warp = threadIdx.x >> 5, head = blockIdx.y;
+  const int b = e.x, parts = e.z & 0xfff, rows = e.z >> 16, warp = threadIdx.x >> 5, head = blockIdx.y;
   const int q0 = p.q_start[b], row = e.y + warp, G = p.group;
-  if (row >= (p.q_start[b + 1] - q0) * G) return;
+  if (warp >= (e.z >> 12 & 15)) return;
   join_row(a, (long long)(e.w + warp) * a.heads + head, (long long)rows * a.heads, parts,
            a.o + (long long)(q0 + row / G) * a.ldo + (long long)(head * G + row % G) * HEAD);
 }
@@ -803,15 +803,15 @@ SNU1_API int snu1_paged_attention(const void* cache, const void* plan, const voi
   a.heads = c.heads;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.status = device_status_word();
-  a.beside = p.chunk_count > 0;
+  a.beside = p.chunk_count + p.one_count > 0;
   a.cluster = p.few_cluster;
   cudaStream_t st = (cudaStream_t)stream;
   int rc = kHostOk;
-  if (p.chunk_count > 0) {
+  if (a.beside) {
     void* wide = a.flags + (((long long)(p.partial_rows + p.few_parts) * c.heads + 15) / 16 * 16 - (long long)p.partial_rows * c.heads);
     float4* factors = (float4*)((uint8_t*)wide + 2ll * 128 * HEAD * 2 * p.unpack_count * c.heads);
-    if (c.fp8 && (rc = launch_widen(c, p, wide, factors, st)) != kHostOk) return rc;
-    if ((rc = launch_chunks(c, p, q, ldq, p.rows, o, ldo, a.part, a.part_ml, a.scale_log2, wide, factors, st)) != kHostOk) return rc;
+    if (c.fp8 && p.chunk_count > 0 && (rc = launch_widen(c, p, wide, factors, st)) != kHostOk) return rc;
+    if ((rc = launch_chunks(c, p, q, ldq, o, ldo, a.part, a.part_ml, a.scale_log2, wide, factors, st)) != kHostOk) return rc;
   }
   if (p.few_count > 0) {
     if (c.fp8) rc = launch_few<true>(c, p, a, st);

@@ -19,6 +19,7 @@
 // * Two warps that have nothing else to do clear values that are not finite (and rows behind the last token) in the bf16 tiles
 //   that some row may not read whole (widening does so for e4m3): a probability of zero does not hide them from the product.  Rows that may read such a
 //   value give NaN, the others are as if it were not there.
+#include <cuda_fp16.h>
 #include <string.h>
 
 #include <mutex>
@@ -32,9 +33,20 @@ namespace paged {
 constexpr int BK = 128;                         // keys of a tile
 constexpr int CHALF = 128 * 64 * 2;             // 64 columns of a 128-row tile
 constexpr int CTILE = 2 * CHALF;
-constexpr int CK_STAGES = 3, CV_STAGES = 2;
 constexpr int CHUNK_THREADS = 640;
-constexpr int CHUNK_SMEM = (2 + CK_STAGES + CV_STAGES) * CTILE + 512 + 1024;
+constexpr int RAW_UNIT = 128 * 128;             // codes of a tile's keys, or of its values
+constexpr int RAW_STAGES = 3, SCALE_STAGES = 4;
+
+// What a CTA reads: bf16 pages, e4m3 pages that have been widened to fp16, or e4m3 pages as they are.
+enum ChunkMode { kPages, kWide, kRaw };
+template <int MODE>
+struct Chunk {
+  static constexpr bool FP16 = MODE != kPages, RAW = MODE == kRaw;
+  static constexpr int TILES = RAW ? 1 : 2;     // row tiles
+  static constexpr int K_STAGES = RAW ? 2 : 3, V_STAGES = 2;
+  static constexpr int RING = RAW ? RAW_STAGES * RAW_UNIT + SCALE_STAGES * 1024 : 0;
+  static constexpr int SMEM = (TILES + K_STAGES + V_STAGES) * CTILE + RING + 512 + 1024;
+};
 
 struct ChunkArgs {
   __nv_bfloat16* o;
@@ -42,6 +54,7 @@ struct ChunkArgs {
   float* part;
   float2* part_ml;
   const int* first_page;   // scratch of widened rows: a sequence's first page there; null: the cache's own pages
+  const int4* items;
   const float4* factors;   // of the widened pages, see paged_widen_kernel
   int page, pages, heads;
   float scale_log2;
@@ -101,16 +114,31 @@ __device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint32_t b, uint
       : "memory");
 }
 
-template <bool FP8>
+// the two codes in the low half of ``w`` times a number, as fp16
+__device__ __forceinline__ uint32_t widen_scaled(uint32_t w, uint64_t f2) {
+  uint32_t h;
+  asm("{\n.reg .b16 l, u;\nmov.b32 {l, u}, %1;\ncvt.rn.f16x2.e4m3x2 %0, l;\n}" : "=r"(h) : "r"(w));
+  const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&h));
+  float x, y;
+  unpack_f32x2(mul_f32x2(pack_f32x2(g.x, g.y), f2), x, y);
+  return pack_f16x2(x, y);
+}
+
+template <int MODE>
 __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                        const __grid_constant__ CUtensorMap tm_v, const Plan p, const ChunkArgs args) {
+  using C = Chunk<MODE>;
+  constexpr bool FP16 = C::FP16, RAW = C::RAW;
+  constexpr int TILES = C::TILES, CK_STAGES = C::K_STAGES, CV_STAGES = C::V_STAGES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* sQ = smem;
-  uint8_t* sK = sQ + 2 * CTILE;
+  uint8_t* sK = sQ + TILES * CTILE;
   uint8_t* sV = sK + CK_STAGES * CTILE;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sV + CV_STAGES * CTILE);
+  uint8_t* s_raw = sV + CV_STAGES * CTILE;                 // [RAW_STAGES] codes of keys and of values in turn
+  float* s_scale = reinterpret_cast<float*>(s_raw + RAW_STAGES * RAW_UNIT);     // [SCALE_STAGES][page][keys, values][token]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(s_raw + C::RING);
   uint64_t* q_full = bars;
   uint64_t* k_full = bars + 1;
   uint64_t* k_empty = k_full + CK_STAGES;
@@ -123,7 +151,10 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
   uint64_t* p_full = s_empty + 2;
   uint64_t* pv_done = p_full + 2;
   uint64_t* q_ready = pv_done + 2;              // e4m3: the queries are fp16
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_ready + 1);
+  uint64_t* raw_full = q_ready + 1;             // [RAW_STAGES]
+  uint64_t* raw_empty = raw_full + RAW_STAGES;
+  float2* s_factor = reinterpret_cast<float2*>(raw_empty + RAW_STAGES);         // [4] of tiles: see ChunkArgs::factors
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_factor + 4);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* drained = reinterpret_cast<int*>(tmem_slot + 2);   // [2] softmax warps that have read a score tile, all tiles so far
   int* lim_max = drained + 2;                              // [2] the largest and the smallest limit of a row tile
@@ -134,16 +165,20 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
     for (int i = 0; i < CK_STAGES; ++i) {
-      mbar_init(&k_full[i], 1);
+      mbar_init(&k_full[i], RAW ? 8 : 1);
       mbar_init(&k_empty[i], 1);
     }
+    for (int i = 0; i < RAW_STAGES; ++i) {
+      mbar_init(&raw_full[i], 1);
+      mbar_init(&raw_empty[i], 8);
+    }
     for (int i = 0; i < CV_STAGES; ++i) {
-      mbar_init(&v_full[i], 1);
+      mbar_init(&v_full[i], RAW ? 8 : 1);
       mbar_init(&v_empty[i], 1);
       mbar_init(&v_dirty[i], 1);
       mbar_init(&v_clean[i], 2);
     }
-    mbar_init(q_ready, 16);
+    mbar_init(q_ready, 8 * TILES);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&s_empty[i], 8);
@@ -169,7 +204,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   // what the plan's host side has set, before the wait: no launch in front writes it
-  const int4 item = p.chunk[blockIdx.x / args.heads];
+  const int4 item = args.items[blockIdx.x / args.heads];
   const int b = item.x, part = item.z & 0xffff, parts = item.z >> 16;
   const int kvh = blockIdx.x % args.heads, G = p.group, T = 128 / G;       // tokens of a row tile
   const int q0 = p.q_start[b], q_len = p.q_start[b + 1] - q0;
@@ -179,13 +214,13 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
   const int token0 = item.y / G;
   int max_a, max_b, min_a, min_b;               // the largest and the smallest limit of row tiles A and B
   if (p.behind == nullptr) {                    // limits grow from token to token
-    const int ends = min(token0 + 2 * T, q_len) - 1;
+    const int ends = min(token0 + TILES * T, q_len) - 1;
     min_a = row_limit(p, q0, q_len, kv_len, token0);
     max_a = row_limit(p, q0, q_len, kv_len, min(token0 + T - 1, ends));
     min_b = token0 + T <= ends ? row_limit(p, q0, q_len, kv_len, token0 + T) : 0x7fffffff;
     max_b = token0 + T <= ends ? row_limit(p, q0, q_len, kv_len, ends) : 0;
   } else {
-    if (threadIdx.x < 2 * T) {
+    if (threadIdx.x < TILES * T) {
       const int t = threadIdx.x / T, token = token0 + threadIdx.x;
       if (token < q_len) {
         const int l = row_limit(p, q0, q_len, kv_len, token);
@@ -202,7 +237,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
   // Row tile A (B) reads the part's first n_a (n_b) key tiles, all but the first full_a (full_b) of them with the mask.
   const int n_a = max(0, min(n, (max_a + BK - 1) / BK - j0)), n_b = max(0, min(n, (max_b + BK - 1) / BK - j0));
   const int full_a = min_a / BK - j0, full_b = min_b / BK - j0;
-  auto dirty = [&](int j) -> bool { return !FP8 && ((j < n_a && j >= full_a) || (j < n_b && j >= full_b)); };
+  auto dirty = [&](int j) -> bool { return !FP16 && ((j < n_a && j >= full_a) || (j < n_b && j >= full_b)); };
   // columns: S_A and P_B [0,128), S_B and P_A [128,256), O_A [256,384), O_B [384,512)
 
   // 640 threads start with 96 registers: 128 x 64 + 512 x 104 = 640 x 96
@@ -211,9 +246,9 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     if (warp == 0) {
       if (n > 0) {
         if (lane == 0) {
-          mbar_expect_tx(q_full, 4 * T * G * 128);
+          mbar_expect_tx(q_full, 2 * TILES * T * G * 128);
 #pragma unroll
-          for (int t = 0; t < 2; ++t) {
+          for (int t = 0; t < TILES; ++t) {
             tma_load_3d(sQ + t * CTILE, &tm_q, q_full, 0, kvh * G, q0 + token0 + t * T);
             tma_load_3d(sQ + t * CTILE + CHALF, &tm_q, q_full, 64, kvh * G, q0 + token0 + t * T);
           }
@@ -245,8 +280,31 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
           ok = mbar_wait_warp(&k_empty[s], ((j / CK_STAGES) & 1) ^ 1, abort_flag, args.status, 1);
           if (ok) load(sK + s * CTILE, &tm_k, &k_full[s], j, pg);
         };
-        load_k(0, pk);
-        for (int j = 0; j < n && ok; ++j) {
+        if (RAW) {
+          // codes of keys, with the scales of keys and values, then codes of values, into one ring
+          for (int j = 0; j < n && ok; ++j) {
+            const int pg = pk, live = min(per, used - (j0 + j) * per);
+            pk = ahead;
+            ahead = page_of(j + 2);
+#pragma unroll
+            for (int kv = 0; kv < 2; ++kv) {
+              const int u = 2 * j + kv, s = u % RAW_STAGES;
+              ok = ok && mbar_wait_warp(&raw_empty[s], ((u / RAW_STAGES) & 1) ^ 1, abort_flag, args.status, 1);
+              if (!ok) break;
+              if (lane == 0) mbar_expect_tx(&raw_full[s], live * page * (kv ? 128 : 128 + 8));
+              __syncwarp();
+              if (lane < live) {
+                if (pg < 0 || pg >= args.pages) report_status(args.status, kBadPage, 10);     // reads as zeros
+                tma_load_5d(smem_u32(s_raw + s * RAW_UNIT + lane * page * 128), &tm_k, &raw_full[s], 0, 0, kvh, kv, pg);
+                if (kv == 0) tma_load_4d(s_scale + (j % SCALE_STAGES) * 256 + lane * page * 2, &tm_v, &raw_full[s], 0, kvh, 0, pg);
+              }
+              __syncwarp();
+            }
+          }
+        } else {
+          load_k(0, pk);
+        }
+        for (int j = 0; j < n && ok && !RAW; ++j) {
           if (j + 1 < n) {
             pk = ahead;
             ahead = page_of(j + 2);
@@ -264,13 +322,13 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
       // The whole warp walks the tiles and one elected lane issues (see mbar_ready in attn_common.cuh).
       if (n > 0) {
         // bits [7,10) and [10,13) of the descriptor: bf16 (1) or fp16 (0) operands
-        constexpr uint32_t type = FP8 ? ~(1u << 7 | 1u << 10) : ~0u;
+        constexpr uint32_t type = FP16 ? ~(1u << 7 | 1u << 10) : ~0u;
         constexpr uint32_t idesc_s = make_idesc_bf16(128, 128, false, false) & type;
         constexpr uint32_t idesc_pv = make_idesc_bf16(128, 128, false, true) & type;
         const uint32_t q_desc = (uint32_t)make_smem_desc(smem_u32(sQ), 0, 1024);
         const uint32_t k_desc = (uint32_t)make_smem_desc(smem_u32(sK), 0, 1024);
         const uint32_t v_desc = (uint32_t)make_smem_desc(smem_u32(sV), CHALF, 1024);
-        bool ok = mbar_wait(FP8 ? q_ready : q_full, 0, abort_flag, args.status, 3);   // this lane's; see mbar_wait_warp
+        bool ok = mbar_wait(FP16 ? q_ready : q_full, 0, abort_flag, args.status, 3);   // this lane's; see mbar_wait_warp
         uint32_t cleaned = 0;                   // phase of every stage's v_clean
         auto issue_s = [&](int j, int t) {
           if (j < (t ? n_b : n_a)) {
@@ -339,7 +397,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
           }
         }
       }
-    } else if (!FP8) {
+    } else if (!FP16) {
       // ------------------------------ cleaning --------------------------------
       bool ok = true;
       const int tid = threadIdx.x - 64;
@@ -383,6 +441,75 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+    if (RAW && warp >= 12) {
+      // ------------------------------ widening --------------------------------
+      // A thread has half a row: code times scale, divided by the tile's power of two, as paged_widen_kernel does it.  Rows that
+      // nobody reads and values that are not finite are cleared.
+      const int tid = threadIdx.x - 384, row = tid & 127, half = tid >> 7;
+      const int page = args.page, page_log = __ffs(page) - 1;
+      auto scale_at = [&](const float* sc, int r, int kv) -> float { return sc[(((r >> page_log) * 2 + kv) << page_log) + (r & (page - 1))]; };
+      bool ok = true;
+      for (int j = 0; j < n && ok; ++j) {
+        const float* sc = s_scale + (j % SCALE_STAGES) * 256;
+        const int k0 = (j0 + j) * BK;
+        float factor[2];
+        float2 told;
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+          const int u = 2 * j + kv, s = u % RAW_STAGES;
+          ok = ok && mbar_wait_warp(&raw_full[s], (u / RAW_STAGES) & 1, abort_flag, args.status, 3);
+          if (!ok) break;
+          if (kv == 0) {                   // both scales have come with the keys
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+              uint32_t top = 0;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float x = fabsf(scale_at(sc, lane + 32 * i, w));
+                if (k0 + lane + 32 * i < most && x < INFINITY) top = max(top, __float_as_uint(x));
+              }
+              top = __reduce_max_sync(0xffffffffu, top);
+              const int ex = tile_exponent(__uint_as_float(top));
+              const float x = k0 + row < most ? scale_at(sc, row, w) : 0.f;
+              factor[w] = x * __int_as_float((127 - ex) << 23);
+              if (w == 0) told.x = __int_as_float((127 + ex) << 23);
+              else told.y = (float)ex;
+            }
+            if (!(fabsf(factor[1]) < INFINITY)) {
+              if (half == 0) atomicMin(poison, k0 + row);
+              factor[1] = 0.f;
+            }
+            if (tid == 0) s_factor[j & 3] = told;
+          }
+          const uint8_t* from = s_raw + s * RAW_UNIT;
+          uint4 x[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const uint4*>(from + swz128_offset(row, half * 4 + i));
+          const int to = j % (kv ? CV_STAGES : CK_STAGES);
+          ok = mbar_wait_warp(kv ? &v_empty[to] : &k_empty[to], ((j / (kv ? CV_STAGES : CK_STAGES)) & 1) ^ 1, abort_flag, args.status, 3);
+          if (!ok) break;
+          uint8_t* dst = (kv ? sV : sK) + to * CTILE + half * CHALF;
+          const bool clear = k0 + row >= most || (kv && factor[1] == 0.f);
+          const uint64_t f2 = pack_f32x2(factor[kv], factor[kv]);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const uint32_t w0 = i & 1 ? x[i >> 1].z : x[i >> 1].x, w1 = i & 1 ? x[i >> 1].w : x[i >> 1].y;
+            uint4 y;
+            y.x = widen_scaled(w0, f2);
+            y.y = widen_scaled(w0 >> 16, f2);
+            y.z = widen_scaled(w1, f2);
+            y.w = widen_scaled(w1 >> 16, f2);
+            *reinterpret_cast<uint4*>(dst + swz128_offset(row, i)) = clear ? make_uint4(0, 0, 0, 0) : y;
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(kv ? &v_full[to] : &k_full[to]);
+            mbar_arrive(&raw_empty[s]);
+          }
+        }
+      }
+    } else {
     // ------------------------------ softmax --------------------------------
     // A warp owns 16 rows; its threads hold columns 2 (lane % 4) + 8 i + {0, 1} of rows lane / 4 and lane / 4 + 8.
     const int t = (warp - 4) >> 3;
@@ -402,7 +529,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};      // running maximum, log2 units
     float sc[2] = {args.scale_log2, args.scale_log2};
     bool ok = true;
-    if (FP8 && n > 0) {
+    if (FP16 && n > 0) {
       // this warp's 16 query rows to fp16, each times a power of two (see attn_paged.cu)
       ok &= mbar_wait(q_full, 0, abort_flag, args.status, 5);
       __syncwarp();
@@ -433,17 +560,22 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(q_ready);
     }
-    const float4* factors = FP8 ? args.factors + (long long)(args.first_page[b] + j0) * args.heads + kvh : nullptr;
+    const float4* factors = MODE == kWide ? args.factors + (long long)(args.first_page[b] + j0) * args.heads + kvh : nullptr;
     int bad = 0x7fffffff;                   // first key whose value is not finite
     const int mine = t ? n_b : n_a, full = t ? full_b : full_a;
     for (int j = 0; j < mine; ++j) {        // all tiles also after a time-out, see mbar_wait_warp
       float4 factor = make_float4(1.f, 0.f, 0.f, 0.f);      // of this tile's keys and values
-      if (FP8) {
+      if (MODE == kWide) {
         factor = __ldg(factors + (long long)j * args.heads);
         bad = min(bad, __float_as_int(factor.z));
       }
       ok &= mbar_wait(&s_full[t], j & 1, abort_flag, args.status, 5);
       tc_fence_after();
+      if (RAW) {                             // told before the keys were; the place is used again four tiles on
+        const float2 told = s_factor[j & 3];
+        factor.x = told.x;
+        factor.y = told.y;
+      }
       float sv[2][32];   // [columns 0-63, 64-127][4 i + 2 row + e]
       {
         uint32_t r0[32], r1[32];
@@ -495,8 +627,8 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
       float f[2];                            // scores in log2 units: s f
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        f[r] = FP8 ? sc[r] * factor.x : sc[r];
-        mx[r] = FP8 ? fmaf(mx[r], f[r], factor.y) : mx[r] * f[r];
+        f[r] = FP16 ? sc[r] * factor.x : sc[r];
+        mx[r] = FP16 ? fmaf(mx[r], f[r], factor.y) : mx[r] * f[r];
       }
       const bool rescale = __any_sync(0xffffffffu, mx[0] > m[0] + 8.f || mx[1] > m[1] + 8.f);
       float alpha[2];
@@ -507,7 +639,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         const float m_use = m_new == -INFINITY ? 0.f : m_new;
         alpha[r] = rescale ? fast_exp2(m[r] - m_use) : 1.f;
         m[r] = m_new;
-        const float nb = FP8 ? factor.y + P_TOP - m_use : -m_use;
+        const float nb = FP16 ? factor.y + P_TOP - m_use : -m_use;
         nb2[r] = pack_f32x2(nb, nb);
         sc2[r] = pack_f32x2(f[r], f[r]);
         acc[r][0] = acc[r][1] = 0ull;
@@ -524,9 +656,9 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
             x = fast_exp2(x);
             y = fast_exp2(y);
             acc[r][i & 1] = add_f32x2(acc[r][i & 1], pack_f32x2(x, y));
-            pk[16 * h + 2 * i + r] = FP8 ? pack_f16x2(x, y) : pack_bf16x2(x, y);
+            pk[16 * h + 2 * i + r] = FP16 ? pack_f16x2(x, y) : pack_bf16x2(x, y);
           }
-      const float out_of = FP8 ? fast_exp2(-factor.y) : 1.f;       // the sum is of probabilities, without the values' power of two
+      const float out_of = FP16 ? fast_exp2(-factor.y) : 1.f;       // the sum is of probabilities, without the values' power of two
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         float s0, s1;
@@ -570,7 +702,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
       for (int r = 0; r < 2; ++r) {
         l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
         l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-        if (lim[r] > (FP8 ? bad : *poison)) l[r] = __int_as_float(0x7fffffff);
+        if (lim[r] > (MODE == kWide ? bad : *poison)) l[r] = __int_as_float(0x7fffffff);
       }
       if (item.w < 0) {
         // Output rows leave through this warp's rows of the row tile's buffer (no product reads it any more), so that 16
@@ -629,9 +761,10 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
 #pragma unroll
           for (int e = 0; e < 2; ++e)
             if (lim[e] >= 0)        // scores that were all NaN are not to be taken for no keys at all
-              args.part_ml[at0 + 8ll * e * args.heads] = make_float2(m[e] == -INFINITY && l[e] != l[e] ? 0.f : FP8 ? m[e] - P_TOP : m[e], l[e]);
+              args.part_ml[at0 + 8ll * e * args.heads] = make_float2(m[e] == -INFINITY && l[e] != l[e] ? 0.f : FP16 ? m[e] - P_TOP : m[e], l[e]);
         }
       }
+    }
     }
   }
 
@@ -648,31 +781,36 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
   }
 }
 
-int launch_chunks(const Cache& c, const Plan& p, const void* q, long long ldq, int q_rows, void* o, long long ldo, float* part,
-                  float2* part_ml, float scale_log2, void* wide, const float4* factors, cudaStream_t st) {
+template <int MODE>
+static int launch_chunks(const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUtensorMap& tm_v, const Plan& p, const ChunkArgs& a,
+                         int items, cudaStream_t st) {
+  int dev = 0;
+  SNU1_CUDA_CHECK(cudaGetDevice(&dev));
+  static std::once_flag once[64];
+  cudaError_t err = cudaSuccess;
+  std::call_once(once[dev & 63], [&]() {
+    err = cudaFuncSetAttribute(paged_chunk_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, Chunk<MODE>::SMEM);
+  });
+  SNU1_CUDA_CHECK(err);
+  SNU1_CUDA_CHECK(launch_pdl(paged_chunk_kernel<MODE>, dim3(a.heads * items), dim3(CHUNK_THREADS), Chunk<MODE>::SMEM, st, tm_q, tm_k, tm_v, p, a));
+  return kHostOk;
+}
+
+int launch_chunks(const Cache& c, const Plan& p, const void* q, long long ldq, void* o, long long ldo, float* part, float2* part_ml,
+                  float scale_log2, void* wide, const float4* factors, cudaStream_t st) {
   const int G = p.group, T = 128 / G;
-  CUtensorMap tm_q, tm_k = c.k, tm_v = c.v;
+  CUtensorMap tm_q, tm_k, tm_v;
   int rc;
   {
-    const uint64_t dims[3] = {128, (uint64_t)c.heads * G, (uint64_t)q_rows}, str[2] = {256, (uint64_t)ldq * 2};
+    const uint64_t dims[3] = {128, (uint64_t)c.heads * G, (uint64_t)p.rows}, str[2] = {256, (uint64_t)ldq * 2};
     const uint32_t box[3] = {64, (uint32_t)G, (uint32_t)T};
     if ((rc = encode_tmap(&tm_q, TmapType::kBf16, true, q, 3, dims, str, box)) != kHostOk) return rc;
   }
   ChunkArgs a;
   a.first_page = nullptr;
-  a.factors = factors;
+  a.factors = nullptr;
   a.page = c.page;
   a.pages = c.pages;
-  if (c.fp8) {
-    const uint64_t dims[4] = {128, 128, (uint64_t)c.heads, (uint64_t)p.unpack_count};
-    const uint64_t str[3] = {256, 256 * 128, 256ull * 128 * c.heads * 2};
-    const uint32_t box[4] = {64, 128, 1, 1};
-    if ((rc = encode_tmap(&tm_k, TmapType::kBf16, true, wide, 4, dims, str, box)) != kHostOk) return rc;
-    if ((rc = encode_tmap(&tm_v, TmapType::kBf16, true, (uint8_t*)wide + 256ull * 128 * c.heads, 4, dims, str, box)) != kHostOk) return rc;
-    a.first_page = p.unpack_first;
-    a.page = 128;
-    a.pages = p.unpack_count;
-  }
   a.o = (__nv_bfloat16*)o;
   a.ldo = ldo;
   a.part = part;
@@ -680,19 +818,23 @@ int launch_chunks(const Cache& c, const Plan& p, const void* q, long long ldq, i
   a.heads = c.heads;
   a.scale_log2 = scale_log2;
   a.status = device_status_word();
-  int dev = 0;
-  SNU1_CUDA_CHECK(cudaGetDevice(&dev));
-  static std::once_flag once[64];
-  cudaError_t err = cudaSuccess;
-  std::call_once(once[dev & 63], [&]() {
-    err = cudaFuncSetAttribute(paged_chunk_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, CHUNK_SMEM);
-    if (err == cudaSuccess)
-      err = cudaFuncSetAttribute(paged_chunk_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, CHUNK_SMEM);
-  });
-  SNU1_CUDA_CHECK(err);
-  auto kernel = c.fp8 ? paged_chunk_kernel<true> : paged_chunk_kernel<false>;
-  SNU1_CUDA_CHECK(launch_pdl(kernel, dim3(c.heads * p.chunk_count), dim3(CHUNK_THREADS), CHUNK_SMEM, st, tm_q, tm_k, tm_v, p, a));
-  return kHostOk;
+  if (p.one_count > 0) {
+    a.items = p.one;
+    if ((rc = launch_chunks<kRaw>(tm_q, c.k, c.scale, p, a, p.one_count, st)) != kHostOk) return rc;
+  }
+  if (p.chunk_count == 0) return kHostOk;
+  a.items = p.chunk;
+  if (!c.fp8) return launch_chunks<kPages>(tm_q, c.k, c.v, p, a, p.chunk_count, st);
+  const uint64_t dims[4] = {128, 128, (uint64_t)c.heads, (uint64_t)p.unpack_count};
+  const uint64_t str[3] = {256, 256 * 128, 256ull * 128 * c.heads * 2};
+  const uint32_t box[4] = {64, 128, 1, 1};
+  if ((rc = encode_tmap(&tm_k, TmapType::kBf16, true, wide, 4, dims, str, box)) != kHostOk) return rc;
+  if ((rc = encode_tmap(&tm_v, TmapType::kBf16, true, (uint8_t*)wide + 256ull * 128 * c.heads, 4, dims, str, box)) != kHostOk) return rc;
+  a.factors = factors;
+  a.first_page = p.unpack_first;
+  a.page = 128;
+  a.pages = p.unpack_count;
+  return launch_chunks<kWide>(tm_q, tm_k, tm_v, p, a, p.chunk_count, st);
 }
 
 }  // namespace paged

@@ -22,13 +22,13 @@ constexpr float P_TOP = 7.f;               // fp16 probabilities: the largest is
 struct alignas(64) Cache {
   CUtensorMap kv;          // box: up to 128 tokens of one head, keys and values, of bf16 up to 64 and 64 values wide
   CUtensorMap scale;       // box: the scales of the same
-  CUtensorMap k, v;        // bf16 only: boxes of up to 128 tokens of one head, 64 values wide
+  CUtensorMap k, v;        // boxes of up to 128 tokens of one head, 64 values wide; e4m3: k takes keys or values, 128 wide
   void* data;
   float* scales;
   int pages, heads, page, fp8;
 };
 
-constexpr int PLAN_LAYOUT = 0x70670001;
+constexpr int PLAN_LAYOUT = 0x70670002;
 
 // Device arrays and counts of a plan (ops/paged.py builds it).
 struct Plan {
@@ -44,13 +44,19 @@ struct Plan {
   const int* unpack_first; // [seqs] first page of such a sequence in the scratch for unpacked rows
   const int4* few;         // [few_count] work of the kernel for few rows: sequence, first row, part | parts << 16, partial row (-1: none)
   const int4* chunk;       // [chunk_count] the same for chunks
-  const int4* merge;       // [merge_count] four rows of a chunk to join: sequence, first row, parts | rows of a part << 16, first partial row
+  const int4* one;         // [one_count] the same for e4m3 chunks of one row tile per CTA
+  const int4* merge;       // [merge_count] up to four rows to join: sequence, first row, parts | rows << 12 | rows of a part << 16, first partial row
   int seqs, rows, width, page, group;
-  int read_count, few_count, few_rows, few_parts, few_cluster, chunk_count, merge_count;
+  int read_count, few_count, few_rows, few_parts, few_cluster, chunk_count, one_count, merge_count;
   int partial_rows;        // rows of the scratch for partial results (x heads)
   int unpack_count;        // also the 128-token pages of the scratch for unpacked rows
   int layout;              // PLAN_LAYOUT; changes with the fields
 };
+
+// The power of two that a tile whose largest scale is ``top`` is divided by: its values are at most 1 then (codes are up to 448).
+__device__ __forceinline__ int tile_exponent(float top) {
+  return max(-90, min(126, (int)(__float_as_uint(E4M3_MAX * top) >> 23) - 126));
+}
 
 __device__ __forceinline__ int seq_len(const Plan& p, int b) { return max(0, min(p.kv_len[b], p.cap[b])); }
 
@@ -76,8 +82,8 @@ __device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* m, 
 
 // paged_cache.cu: a plan's ``unpack`` tiles of an e4m3 cache as fp16 pages at ``wide``
 int launch_widen(const Cache& c, const Plan& p, void* wide, float4* factors, cudaStream_t st);
-// attn_paged_sm100.cu: a plan's ``chunk`` items
-int launch_chunks(const Cache& c, const Plan& p, const void* q, long long ldq, int q_rows, void* o, long long ldo, float* part,
+// attn_paged_sm100.cu: a plan's ``one`` and ``chunk`` items
+int launch_chunks(const Cache& c, const Plan& p, const void* q, long long ldq, void* o, long long ldo, float* part,
                   float2* part_ml, float scale_log2, void* wide, const float4* factors, cudaStream_t st);
 
 }  // namespace paged

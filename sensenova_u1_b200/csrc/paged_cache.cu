@@ -227,8 +227,7 @@ __global__ void __launch_bounds__(WIDEN_THREADS)
     }
   }
   __syncthreads();
-  const float top = E4M3_MAX * fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
-  const int ex = max(-90, min(126, (int)(__float_as_uint(top) >> 23) - 126));
+  const int ex = tile_exponent(fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3])));
   const float down = __int_as_float((127 - ex) << 23);
   const long long page = p.unpack_first[b] + e.y;
   if (t == 0) {
@@ -299,6 +298,9 @@ SNU1_API int snu1_paged_cache_init(void* out, void* data, void* scales, int page
   if (fp8) {
     const uint64_t dims[4] = {P, H, 2, (uint64_t)pages}, str[3] = {P * 4, P * H * 4, P * H * 8};
     const uint32_t box[4] = {bx, 1, 2, 1};
+    const uint64_t kdims[5] = {128, P, H, 2, (uint64_t)pages}, kstr[4] = {row, row * P, row * P * H, row * P * H * 2};
+    const uint32_t kbox[5] = {128, (uint32_t)page, 1, 1, 1};
+    if ((rc = encode_tmap(&c.k, TmapType::kU8, true, data, 5, kdims, kstr, kbox)) != kHostOk) return rc;
     if ((rc = encode_tmap(&c.scale, TmapType::kF32, false, scales, 4, dims, str, box)) != kHostOk) return rc;
   } else {
     const uint64_t dims[4] = {128, P, H, (uint64_t)pages}, str[3] = {row, row * P, row * P * H * 2};

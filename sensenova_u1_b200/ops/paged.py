@@ -36,12 +36,16 @@ PAGE_SIZES = (16, 32, 64, 128)
 HEAD_DIM = 128
 E4M3 = torch.float8_e4m3fn
 KEY_TILE = 64            # keys of a stage of the kernel for few rows
-FEW_SLOTS = (296, 444)   # its CTAs that run at once: two on each of 148 SMs, three of those for up to eight rows
+FEW_SLOTS = (444, 296)   # its CTAs that run at once: of up to eight rows three on each of 148 SMs, otherwise two
 FEW_LEAST = 4            # a part of a sequence has at least this many key tiles
 FEW_JOIN = 8             # up to so many rows the parts of few rows join themselves (JOIN_ROWS in attn_paged.cu)
 FEW_CLUSTER = 8          # up to so many parts are a cluster, if all sequences can have as many
-FEW_TILE = 64            # rows (new tokens x query heads of a group) of one CTA, at most
+FEW_TILE = (32, 64)      # rows (new tokens x query heads of a group) of one CTA, at most: bf16, e4m3
+# More rows of a sequence are a chunk.  Chunk kernel / few rows, us, 32 / 8 heads, sequences of 12000 keys: bf16 1 x 32 rows
+# 22 / 23, 8 x 32 76 / 66, 1 x 48 22 / 29, 8 x 48 82 / 107.
+CHUNK_FROM = FEW_TILE
 CHUNK_TILE = 128         # keys of a tile of the kernel for chunks, and rows of a row tile
+ONE_MOST = 256           # e4m3 chunks of up to so many rows are widened by the CTAs that read them, one row tile each
 CHUNK_SLOTS = 148        # its CTAs that run at once
 CHUNK_START = 5          # what starting and ending a CTA costs, in key tiles (1.8 us): 8 to 10 us from its start to its end
 CHUNK_JOIN = 3           # what a part costs besides: 128 KB written and read again
@@ -107,15 +111,15 @@ class PagedCache:
         return self._data.device
 
 
-PLAN_LAYOUT = 0x70670001     # last word of a plan: the library refuses one whose fields lie elsewhere
+PLAN_LAYOUT = 0x70670002     # last word of a plan: the library refuses one whose fields lie elsewhere
 
 
 class _Args(ctypes.Structure):
     """``Plan`` of csrc/paged.cuh."""
     _fields_ = ([(n, c_void_p) for n in ("q_start", "kv_len", "cap", "table", "behind", "row_seq", "k_start", "read_pages", "unpack",
-                                         "unpack_first", "few", "chunk", "merge")]
+                                         "unpack_first", "few", "chunk", "one", "merge")]
                 + [(n, c_int) for n in ("seqs", "rows", "width", "page", "group", "read_count", "few_count", "few_rows", "few_parts", "few_cluster",
-                                        "chunk_count", "merge_count", "partial_rows", "unpack_count", "layout")])
+                                        "chunk_count", "one_count", "merge_count", "partial_rows", "unpack_count", "layout")])
 
 
 @dataclass
@@ -213,11 +217,12 @@ def _lay_out(q_lens, kv_lens, tables, page: int, pages: int, group: int, kv_head
     pages_of = lambda c: np.stack([np.repeat(np.arange(n), c), np.arange(int(c.sum())) - np.repeat(np.cumsum(c) - c, c)], 1).astype(np.int32)
     # attention: tiles of rows, split over keys
     q_rows = q * group
-    chunked = (q_rows > FEW_TILE) & (group <= CHUNK_TILE)
+    chunked = (q_rows > CHUNK_FROM[fp8]) & (group <= CHUNK_TILE)
     few_q = np.where(chunked, 0, q_rows)
     top = int(few_q.max()) if n else 0
-    few_rows = 8 if top <= 8 else 16 if top <= 16 else 32 if top <= 32 else FEW_TILE
-    chunk_rows = 2 * (CHUNK_TILE // group) * group if group <= CHUNK_TILE else 1        # two row tiles of whole tokens
+    few_rows = 8 if top <= 8 else 16 if top <= 16 else 32 if top <= 32 else FEW_TILE[fp8]
+    tile_rows = (CHUNK_TILE // group) * group if group <= CHUNK_TILE else 1      # a row tile is made of whole tokens
+    single = chunked & fp8 & (q_rows <= ONE_MOST)              # widened by the CTAs that read it
 
     def tiles_of(q_rows, m):
         count = -(-q_rows // m)
@@ -226,7 +231,7 @@ def _lay_out(q_lens, kv_lens, tables, page: int, pages: int, group: int, kv_head
 
     seq, row0 = tiles_of(few_q, few_rows)
     tiles = -(-cap[seq] // KEY_TILE)
-    slots = FEW_SLOTS[few_rows <= FEW_JOIN]
+    slots = FEW_SLOTS[few_rows > 8]
     parts = _shares(tiles, kv_heads, slots, FEW_LEAST)
     cluster = int(parts.max()) if len(parts) else 1
     if 1 < cluster <= FEW_CLUSTER and len(seq) * cluster * kv_heads <= slots:      # as many parts for everybody, side by side
@@ -236,24 +241,32 @@ def _lay_out(q_lens, kv_lens, tables, page: int, pages: int, group: int, kv_head
     else:
         few, merge, partial = _items(seq, row0, tiles, parts, few_q, few_rows, 0)
         cluster = 1
-    seq, row0 = tiles_of(np.where(chunked, q_rows, 0), chunk_rows)
-    if limits is None:                                        # a row tile reads up to its last token
-        last = np.minimum((row0 + chunk_rows - 1) // group, q[seq] - 1)
-        tiles = -(-(cap[seq] - q[seq] + 1 + last) // CHUNK_TILE)
-    else:
-        tiles = -(-kv[seq] // CHUNK_TILE)
     few_parts = partial // few_rows if few_rows <= FEW_JOIN else 0       # parts that join themselves
-    chunk, more, partial = _items(seq, row0, tiles, _waves(tiles, kv_heads, CHUNK_SLOTS), q_rows, chunk_rows, partial)
-    merge = more if few_rows <= FEW_JOIN else np.concatenate([merge, more])
+    merge = [] if few_rows <= FEW_JOIN else [merge]
+
+    def chunks_of(which, m, partial):
+        seq, row0 = tiles_of(np.where(which, q_rows, 0), m)
+        if limits is None:                                    # a row tile reads up to its last token
+            last = np.minimum((row0 + m - 1) // group, q[seq] - 1)
+            tiles = -(-(cap[seq] - q[seq] + 1 + last) // CHUNK_TILE)
+        else:
+            tiles = -(-kv[seq] // CHUNK_TILE)
+        items, join, partial = _items(seq, row0, tiles, _waves(tiles, kv_heads, CHUNK_SLOTS), q_rows, m, partial)
+        merge.append(join)
+        return items, partial
+
+    one, partial = chunks_of(single, tile_rows, partial)
+    chunk, partial = chunks_of(chunked & ~single, 2 * tile_rows, partial)
+    merge = np.concatenate(merge)
     unpack = unpack_first = None
     if fp8 and len(chunk):
-        wide = np.where(chunked, -(-cap // CHUNK_TILE), 0)    # 128-token pages
+        wide = np.where(chunked & ~single, -(-cap // CHUNK_TILE), 0)    # 128-token pages
         unpack, unpack_first = pages_of(wide), start(wide)[:n]
     arrays = dict(q_start=start(q), kv_len=kv.astype(np.int32), cap=cap.astype(np.int32), table=table, behind=behind, row_seq=row_seq,
                   k_start=start(kv), read_pages=pages_of(read), unpack=unpack, unpack_first=unpack_first, few=few, chunk=chunk,
-                  merge=merge)
+                  one=one, merge=merge)
     counts = dict(seqs=n, rows=rows, width=width, page=page, group=group, read_count=int(read.sum()), few_count=len(few),
-                  few_rows=few_rows, few_parts=few_parts, few_cluster=cluster, chunk_count=len(chunk), merge_count=len(merge),
+                  few_rows=few_rows, few_parts=few_parts, few_cluster=cluster, chunk_count=len(chunk), one_count=len(one), merge_count=len(merge),
                   partial_rows=partial, unpack_count=0 if unpack is None else len(unpack), layout=PLAN_LAYOUT)
     return arrays, counts
 
@@ -291,9 +304,11 @@ def _items(seq, row0, tiles, parts, q_rows, m: int, first: int):
         return np.zeros((0, 4), np.int32), np.zeros((0, 4), np.int32), first
     split = parts > 1
     at = first + np.cumsum(np.where(split, parts * m, 0)) - np.where(split, parts * m, 0)
-    join = np.where(split, -(-np.minimum(m, q_rows[seq] - row0) // 4), 0)
+    have = np.minimum(m, q_rows[seq] - row0)                  # rows of an item
+    join = np.where(split, -(-have // 4), 0)
     four = 4 * (np.arange(int(join.sum())) - np.repeat(np.cumsum(join) - join, join))
     merge = np.stack([np.repeat(x, join) for x in (seq, row0, parts | m << 16, at)], 1)
+    merge[:, 2] |= np.minimum(4, np.repeat(have, join) - four) << 12
     merge[:, 1] += four
     merge[:, 3] += four
     i = np.repeat(np.arange(len(seq)), parts)

@@ -67,7 +67,7 @@ def test_every_row_meets_every_key_once(q, kv, group, heads):
     tables = [list(range(sum(need[:i]), sum(need[:i + 1]))) for i in range(n)]
     a, c = paged._lay_out(q, kv, tables, page, sum(need), group, heads, True, None, 0)
     parts, written = {}, set()
-    for name, m in (("few", c["few_rows"]), ("chunk", 2 * (128 // group) * group)):
+    for name, m in (("few", c["few_rows"]), ("chunk", 2 * (128 // group) * group), ("one", 128 // group * group)):
         if a[name] is None:
             continue
         for b, row0, z, at in a[name].tolist():
@@ -86,22 +86,23 @@ def test_every_row_meets_every_key_once(q, kv, group, heads):
             seen[(b, r)] = count
     assert len(seen) == sum(q) * group
     joined = {}
-    for b, row0, z, at in a["merge"].tolist():                        # four rows each
-        for r in range(row0, min(row0 + 4, q[b] * group)):
+    for b, row0, z, at in a["merge"].tolist():                        # up to four rows each
+        assert 1 <= (z >> 12 & 15) <= 4
+        for r in range(row0, row0 + (z >> 12 & 15)):
             assert (b, r) not in joined
-            joined[(b, r)] = (z & 0xffff, z >> 16, at + r - row0)
+            joined[(b, r)] = (z & 0xfff, z >> 16, at + r - row0)
     if c["few_cluster"] > 1:                                          # the parts of every tile of rows side by side
         k = c["few_cluster"]
         assert len(a["few"]) % k == 0 and len(a["few"]) * heads <= 444
         assert [z for _, _, z, _ in a["few"].tolist()] == [i % k | k << 16 for i in range(len(a["few"]))]
         assert all(len({tuple(x) for x in a["few"][i:i + k, :2].tolist()}) == 1 for i in range(0, len(a["few"]), k))
     assert set(joined) == {(b, r) for (b, r), count in seen.items() if count > 1 and (
-        c["few_rows"] > paged.FEW_JOIN and c["few_cluster"] == 1 or q[b] * group > paged.FEW_TILE and group <= 128)}
+        c["few_rows"] > paged.FEW_JOIN and c["few_cluster"] == 1 or q[b] * group > paged.CHUNK_FROM[1] and group <= 128)}
     first = {(b, row0): at for b, row0, z, at in a["few"].tolist() if at >= 0 and z & 0xffff == 0}
     for b, row0, z, at in a["few"].tolist():                          # joined by the parts themselves: side by side, in whole parts
         assert at < 0 or at == first[(b, row0)] + (z & 0xffff) * c["few_rows"] and at % c["few_rows"] == 0
         assert at < 0 or c["few_rows"] > paged.FEW_JOIN or at < c["few_parts"] * c["few_rows"]
-    for b, row0, z, at in a["chunk"].tolist():
+    for b, row0, z, at in a["chunk"].tolist() + a["one"].tolist():
         if at >= 0:
             for r in range(row0, q[b] * group):
                 count, _, first = joined[(b, r)]
