@@ -3,7 +3,7 @@
 //
 //   o_r = sum_j p_rj v_j / sum_j p_rj,   p_rj = exp(scale q_r k_j - m_r),   j < limit_r
 //
-// The rows of a (sequence, key/value head) are its new tokens times the query heads of the group, up to 64 per CTA.  What
+// The rows of a (sequence, key/value head) are its new tokens times the query heads of the group, up to 32 per CTA.  What
 // bounds it is the stream of keys and values, so the work is split over keys: a work item is one part of a sequence, the
 // parts are made as equal as they can be over the whole batch (ops/paged.py), and their unnormalised results (maximum, sum,
 // weighted values, fp32) are joined in a fixed order.  Where every sequence can have as many parts as the longest, up to
@@ -20,7 +20,9 @@
 // bits, and what smaller ones lose is below the rounding of the fp32 sum.  The scale of a key goes into its score.  The
 // scale of a value goes into its probability, in the exponent: p' = exp2(s + log2(scale) - m') with a maximum of its own,
 // so that the fp16 probabilities of the product are relative to the largest p' whatever sizes the values have (the largest
-// is brought to 2^7, so that one is only lost below 2^-32 of it; rounding 2^-11 each; bf16 caches: bf16 probabilities, 2^-8).  The sum of the probabilities is taken in fp32 from p itself.
+// is brought to 2^7, so that one is only lost below 2^-32 of it; rounding 2^-11 each).  The sum of the probabilities is taken in
+// fp32 from p itself.  bf16 caches take a probability as two bf16 numbers (2^-16): one alone, 2^-8, would make the error of
+// the result 1.4 times that of its rounding, and the second product costs nothing beside the stream of the cache.
 //
 // Masked places: scores of keys at or beyond a row's limit are -inf whatever the cache holds, and places that no row of the
 // tile may read are cleared in shared memory.  A probability of zero does not hide an infinite or NaN value from the
@@ -532,6 +534,7 @@ __global__ void __launch_bounds__(FEW_THREADS, Few<FP8, NR * WR == 1>::CTAS)
             }
         }
         uint32_t pf[NR][NB][2];              // p^T: rows g x keys 2 c + {0, 1}, then + 8
+        uint32_t pr[NR][NB][2];              // bf16: what rounding has left
 #pragma unroll
         for (int i = 0; i < NR; ++i) {
           float mu[2], muv[2];
@@ -551,8 +554,12 @@ __global__ void __launch_bounds__(FEW_THREADS, Few<FP8, NR * WR == 1>::CTAS)
               if (FP8) x[e] = partial && sv[i][nb][e] == -INFINITY ? 0.f : fast_exp2(sv[i][nb][e] + lv[nb][e >> 1] - muv[e & 1]);
             }
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-              pf[i][nb][h] = transpose_8x8(FP8 ? pack_f16x2(x[2 * h], x[2 * h + 1]) : pack_bf16x2(x[2 * h], x[2 * h + 1]));
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t w = FP8 ? pack_f16x2(x[2 * h], x[2 * h + 1]) : pack_bf16x2(x[2 * h], x[2 * h + 1]);
+              pf[i][nb][h] = transpose_8x8(w);
+              if (!FP8)
+                pr[i][nb][h] = transpose_8x8(pack_bf16x2(x[2 * h] - __uint_as_float(w << 16), x[2 * h + 1] - __uint_as_float(w & 0xffff0000u)));
+            }
           }
         }
 #pragma unroll
@@ -580,7 +587,10 @@ __global__ void __launch_bounds__(FEW_THREADS, Few<FP8, NR * WR == 1>::CTAS)
               uint32_t r[4];                 // matrices: two pieces of keys 0-7, two of keys 8-15
               ldsm_x4_t(vb + (d >> 2) * box_bytes + swz128_offset(vrow, (d & 3) * 2 + ((lane >> 3) & 1)), r);
 #pragma unroll
-              for (int i = 0; i < NR; ++i) mma_16816<false>(acc[i][d], r, pf[i][nb][0], pf[i][nb][1]);
+              for (int i = 0; i < NR; ++i) {
+                mma_16816<false>(acc[i][d], r, pf[i][nb][0], pf[i][nb][1]);
+                mma_16816<false>(acc[i][d], r, pr[i][nb][0], pr[i][nb][1]);
+              }
             }
           }
         }
@@ -756,7 +766,7 @@ static int launch_few(const Cache& c, const Plan& p, const FewArgs& a, cudaStrea
     case 8: return launch_few<FP8, 1, 1>(c, p, a, st);
     case 16: return launch_few<FP8, 2, 1>(c, p, a, st);
     case 32: return launch_few<FP8, 2, 2>(c, p, a, st);
-    default: return launch_few<FP8, 2, 4>(c, p, a, st);
+    default: set_last_error("paged_attention: no kernel for %d rows", p.few_rows); return kHostBadArg;
   }
 }
 

@@ -114,14 +114,15 @@ __device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint32_t b, uint
       : "memory");
 }
 
-// the two codes in the low half of ``w`` times a number, as fp16
-__device__ __forceinline__ uint32_t widen_scaled(uint32_t w, uint64_t f2) {
-  uint32_t h;
-  asm("{\n.reg .b16 l, u;\nmov.b32 {l, u}, %1;\ncvt.rn.f16x2.e4m3x2 %0, l;\n}" : "=r"(h) : "r"(w));
-  const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&h));
-  float x, y;
-  unpack_f32x2(mul_f32x2(pack_f32x2(g.x, g.y), f2), x, y);
-  return pack_f16x2(x, y);
+// The two codes in the low half of ``w`` times hi + lo, as fp16: the product with hi has 15 bits and is rounded once, together with
+// the product with lo.
+__device__ __forceinline__ uint32_t widen_scaled(uint32_t w, uint32_t hi, uint32_t lo) {
+  uint32_t r;
+  asm("{\n.reg .b16 l, u;\n.reg .b32 h, t;\nmov.b32 {l, u}, %1;\ncvt.rn.f16x2.e4m3x2 h, l;\n"
+      "mul.rn.f16x2 t, h, %3;\nfma.rn.f16x2 %0, h, %2, t;\n}"
+      : "=r"(r)
+      : "r"(w), "r"(hi), "r"(lo));
+  return r;
 }
 
 template <int MODE>
@@ -443,8 +444,9 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
     if (RAW && warp >= 12) {
       // ------------------------------ widening --------------------------------
-      // A thread has half a row: code times scale, divided by the tile's power of two, as paged_widen_kernel does it.  Rows that
-      // nobody reads and values that are not finite are cleared.
+      // A thread has half a row: code times scale as fp16, the tile times a power of two that brings its largest value to 2^12
+      // to 2^13.  A scale is two fp16 numbers then, and a pair of codes three instructions instead of five.  Rows that nobody
+      // reads and values that are not finite are cleared.
       const int tid = threadIdx.x - 384, row = tid & 127, half = tid >> 7;
       const int page = args.page, page_log = __ffs(page) - 1;
       auto scale_at = [&](const float* sc, int r, int kv) -> float { return sc[(((r >> page_log) * 2 + kv) << page_log) + (r & (page - 1))]; };
@@ -454,6 +456,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         const int k0 = (j0 + j) * BK;
         float factor[2];
         float2 told;
+        constexpr int UP = 13;
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv) {
           const int u = 2 * j + kv, s = u % RAW_STAGES;
@@ -471,9 +474,9 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
               top = __reduce_max_sync(0xffffffffu, top);
               const int ex = tile_exponent(__uint_as_float(top));
               const float x = k0 + row < most ? scale_at(sc, row, w) : 0.f;
-              factor[w] = x * __int_as_float((127 - ex) << 23);
-              if (w == 0) told.x = __int_as_float((127 + ex) << 23);
-              else told.y = (float)ex;
+              factor[w] = x * __int_as_float((127 - ex + UP) << 23);
+              if (w == 0) told.x = __int_as_float((127 + ex - UP) << 23);
+              else told.y = (float)(ex - UP);
             }
             if (!(fabsf(factor[1]) < INFINITY)) {
               if (half == 0) atomicMin(poison, k0 + row);
@@ -490,16 +493,19 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
           if (!ok) break;
           uint8_t* dst = (kv ? sV : sK) + to * CTILE + half * CHALF;
           const bool clear = k0 + row >= most || (kv && factor[1] == 0.f);
-          const uint64_t f2 = pack_f32x2(factor[kv], factor[kv]);
+          if (__any_sync(0xffffffffu, clear)) {      // (their codes may be NaN)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (clear) x[i] = make_uint4(0, 0, 0, 0);
+          }
+          const uint32_t hi = pack_f16x2(factor[kv], factor[kv]);
+          const float rest = clear ? 0.f : factor[kv] - __low2float(*reinterpret_cast<const __half2*>(&hi));
+          const uint32_t lo = pack_f16x2(rest, rest);
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const uint32_t w0 = i & 1 ? x[i >> 1].z : x[i >> 1].x, w1 = i & 1 ? x[i >> 1].w : x[i >> 1].y;
-            uint4 y;
-            y.x = widen_scaled(w0, f2);
-            y.y = widen_scaled(w0 >> 16, f2);
-            y.z = widen_scaled(w1, f2);
-            y.w = widen_scaled(w1 >> 16, f2);
-            *reinterpret_cast<uint4*>(dst + swz128_offset(row, i)) = clear ? make_uint4(0, 0, 0, 0) : y;
+            *reinterpret_cast<uint4*>(dst + swz128_offset(row, i)) = make_uint4(
+                widen_scaled(w0, hi, lo), widen_scaled(w0 >> 16, hi, lo), widen_scaled(w1, hi, lo), widen_scaled(w1 >> 16, hi, lo));
           }
           fence_proxy_async_smem();
           __syncwarp();

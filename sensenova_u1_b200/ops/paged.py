@@ -40,12 +40,15 @@ FEW_SLOTS = (444, 296)   # its CTAs that run at once: of up to eight rows three 
 FEW_LEAST = 4            # a part of a sequence has at least this many key tiles
 FEW_JOIN = 8             # up to so many rows the parts of few rows join themselves (JOIN_ROWS in attn_paged.cu)
 FEW_CLUSTER = 8          # up to so many parts are a cluster, if all sequences can have as many
-FEW_TILE = (32, 64)      # rows (new tokens x query heads of a group) of one CTA, at most: bf16, e4m3
+FEW_TILE = 32            # rows (new tokens x query heads of a group) of one CTA, at most
 # More rows of a sequence are a chunk.  Chunk kernel / few rows, us, 32 / 8 heads, sequences of 12000 keys: bf16 1 x 32 rows
-# 22 / 23, 8 x 32 76 / 66, 1 x 48 22 / 29, 8 x 48 82 / 107.
+# 22 / 23, 8 x 32 76 / 66, 1 x 48 22 / 29, 8 x 48 82 / 107; e4m3 1 x 32 22 / 25, 8 x 32 93 / 86, 1 x 48 24 / 32, 8 x 48 95 / 139.
 CHUNK_FROM = FEW_TILE
 CHUNK_TILE = 128         # keys of a tile of the kernel for chunks, and rows of a row tile
-ONE_MOST = 256           # e4m3 chunks of up to so many rows are widened by the CTAs that read them, one row tile each
+# e4m3 chunks of up to so many rows are widened by the CTAs that read them, one row tile each; longer ones are widened once.
+# Us, the former / the latter: 8 sequences of 12000 keys, 128 rows 98 / 191, 256 178 / 210, 512 363 / 291; of 1000 keys 22 / 29, 23 / 33,
+# 44 / 35.
+ONE_MOST = 256
 CHUNK_SLOTS = 148        # its CTAs that run at once
 CHUNK_START = 5          # what starting and ending a CTA costs, in key tiles (1.8 us): 8 to 10 us from its start to its end
 CHUNK_JOIN = 3           # what a part costs besides: 128 KB written and read again
@@ -217,10 +220,10 @@ def _lay_out(q_lens, kv_lens, tables, page: int, pages: int, group: int, kv_head
     pages_of = lambda c: np.stack([np.repeat(np.arange(n), c), np.arange(int(c.sum())) - np.repeat(np.cumsum(c) - c, c)], 1).astype(np.int32)
     # attention: tiles of rows, split over keys
     q_rows = q * group
-    chunked = (q_rows > CHUNK_FROM[fp8]) & (group <= CHUNK_TILE)
+    chunked = (q_rows > CHUNK_FROM) & (group <= CHUNK_TILE)
     few_q = np.where(chunked, 0, q_rows)
     top = int(few_q.max()) if n else 0
-    few_rows = 8 if top <= 8 else 16 if top <= 16 else 32 if top <= 32 else FEW_TILE[fp8]
+    few_rows = 8 if top <= 8 else 16 if top <= 16 else FEW_TILE
     tile_rows = (CHUNK_TILE // group) * group if group <= CHUNK_TILE else 1      # a row tile is made of whole tokens
     single = chunked & fp8 & (q_rows <= ONE_MOST)              # widened by the CTAs that read it
 
@@ -284,6 +287,8 @@ def _waves(tiles: np.ndarray, heads: int, slots: int) -> np.ndarray:
         parts = -(-tiles // share)
         cost = -(-tiles // parts) + CHUNK_START + np.where(parts > 1, CHUNK_JOIN, 0)
         cost = np.sort(np.repeat(cost, parts * heads))[::-1]
+        if best is not None and len(cost) > 8 * slots:        # so many waves are full enough
+            break
         busy = np.zeros(slots)
         for i in range(0, len(cost), slots):                  # the longest that are left go to those that are free first
             wave = cost[i:i + slots]

@@ -97,7 +97,7 @@ def test_every_row_meets_every_key_once(q, kv, group, heads):
         assert [z for _, _, z, _ in a["few"].tolist()] == [i % k | k << 16 for i in range(len(a["few"]))]
         assert all(len({tuple(x) for x in a["few"][i:i + k, :2].tolist()}) == 1 for i in range(0, len(a["few"]), k))
     assert set(joined) == {(b, r) for (b, r), count in seen.items() if count > 1 and (
-        c["few_rows"] > paged.FEW_JOIN and c["few_cluster"] == 1 or q[b] * group > paged.CHUNK_FROM[1] and group <= 128)}
+        c["few_rows"] > paged.FEW_JOIN and c["few_cluster"] == 1 or q[b] * group > paged.CHUNK_FROM and group <= 128)}
     first = {(b, row0): at for b, row0, z, at in a["few"].tolist() if at >= 0 and z & 0xffff == 0}
     for b, row0, z, at in a["few"].tolist():                          # joined by the parts themselves: side by side, in whole parts
         assert at < 0 or at == first[(b, row0)] + (z & 0xffff) * c["few_rows"] and at % c["few_rows"] == 0
@@ -105,7 +105,7 @@ def test_every_row_meets_every_key_once(q, kv, group, heads):
     for b, row0, z, at in a["chunk"].tolist() + a["one"].tolist():
         if at >= 0:
             for r in range(row0, q[b] * group):
-                count, _, first = joined[(b, r)]
+                count, m, first = joined[(b, r)]
                 assert count == z >> 16 and (r - row0 >= m or at + r - row0 == first + (z & 0xffff) * m)
                 if r - row0 + 1 >= m:
                     break

@@ -59,7 +59,7 @@ def exact(q, q_lens, rows, limits, dtype=BF16):
             p = torch.nan_to_num(torch.softmax(s.masked_fill(hidden, float("-inf")), -1), nan=0.0)
             out[r:r + n] = torch.einsum("hrk,hkd->rhd", p, v)
             room[r:r + n] = torch.einsum("hrk,hkd->rhd", p, v.abs()) * (2.0 ** -8 + 2.0 ** -11)
-            if dtype == E4M3 and n * g > paged.CHUNK_FROM[1]:
+            if dtype == E4M3 and n * g > paged.CHUNK_FROM:
                 most = (torch.einsum("rhd,hkd->hrk", x.abs(), k.abs()) * SCALE).masked_fill(hidden, 0.0).amax(-1)       # [heads, rows]
                 room[r:r + n] *= 1 + 2 * 2.0 ** -11 * most.T[..., None] / (2.0 ** -8 + 2.0 ** -11)
         r += n
