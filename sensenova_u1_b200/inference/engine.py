@@ -23,7 +23,7 @@ from ..data.batch import apply_time_schedule
 from ..models import oracle
 from ..models.engine import Workspace
 from ..models.params import GEN, UND, ParamStore
-from ..ops import _lib, attention as attn_ops, decode_stack, fused, gemm, moe
+from ..ops import _lib, attention as attn_ops, decode_stack, fused, gemm, moe, paged
 from ..ops._lib import c_float, c_int, c_void_p
 
 CFG_NORMS = {"none": 0, "global": 1, "channel": 2, "cfg_zero_star": 3}
@@ -143,10 +143,13 @@ class InferenceEngine:
         self.vc = [torch.zeros(kv_rows, cfg.num_kv_heads, 128, dtype=torch.bfloat16, device=self.dev)
                    for _ in range(cfg.num_layers)]
 
-    def layers(self, x, branch: int, pos3, plan, kv_rows, kv_len: int, publish=None):
+    def layers(self, x, branch: int, pos3, plan, kv_rows, kv_len: int, publish=None, caches=None):
         """Runs the decoder stack on rows ``x`` [R,H] with one branch's weights.  The rows'
         K/V are written to cache rows ``kv_rows`` (int64 [R]); attention reads cache rows
         [0, kv_len).  Returns the final hidden state (before the final norm).
+
+        With a ``paged.PagedPlan`` the rows' K/V go to their sequences' pages in ``caches`` (one per layer) and attention
+        reads those; ``kv_rows`` and ``kv_len`` are not used.
 
         ``publish`` (sequence-parallel sampling): runs of rows [(first row of x, count, first cache row)]
         whose K/V go to every rank of the sequence-parallel group instead of the local cache only."""
@@ -165,7 +168,7 @@ class InferenceEngine:
         q = qf.unflatten(1, (cfg.num_heads, 128))
         o = ws.get("i.o", (R, cfg.num_heads, 128))
         of = o.view(R, qd)
-        decode = isinstance(plan, DecodeRows)
+        decode, pages = isinstance(plan, DecodeRows), isinstance(plan, paged.PagedPlan)
         act = None
         if not cfg.is_moe:
             act = ws.get("i.act", (R, cfg.ffn_size))
@@ -182,7 +185,12 @@ class InferenceEngine:
                 fused.rmsnorm_fwd(x, W("attn_norm"), None, h1, None, cfg.rms_eps)
             normed = False
             gemm.gemm_nt(h1, W("wqkv"), out=qkv, w_static=static, in_parts=True)
-            if publish is None:
+            if pages:
+                fused.qknorm_rope_fwd(qkv, qk, W("qk_norm"), None, pos3, self.inv_t, self.inv_hw, cfg.num_heads, cfg.num_kv_heads,
+                                      cfg.rms_eps)
+                heads = (cfg.num_kv_heads, 128)
+                paged.paged_write(caches[l], qk[:, qd:].unflatten(1, heads), qkv[:, qd + kd:].unflatten(1, heads), plan)
+            elif publish is None:
                 fused.qknorm_rope_cache(qkv, qf, self.kc[l], self.vc[l], kv_rows, W("qk_norm"), pos3, self.inv_t,
                                         self.inv_hw, cfg.num_heads, cfg.num_kv_heads, cfg.rms_eps)
             else:
@@ -199,8 +207,10 @@ class InferenceEngine:
                 # every peer's slice of this layer is in my cache after the barrier; a peer can only come
                 # back to this layer (next step) after the barriers of all later layers, i.e. after I read
                 self.sp["bar"].barrier()
-            k, v = self.kc[l][:kv_len], self.vc[l][:kv_len]
-            if decode:
+            k, v = (None, None) if pages else (self.kc[l][:kv_len], self.vc[l][:kv_len])
+            if pages:
+                paged.paged_attention(q, caches[l], plan, self.scale, out=o)
+            elif decode:
                 attn_ops.attention_decode(q, k, v, plan.meta_q, plan.meta_k, plan.first, kv_rows, plan.max_keys,
                                           self.scale, o)
             else:
@@ -320,6 +330,29 @@ class InferenceEngine:
         self._meta_k = mk
         self._doc_starts = [lay.kv_start for lay in layouts]
         return layouts, x.index_select(0, last)
+
+    # ------------------------------------------------------------ paged cache
+    def paged_caches(self, pages: int, page: int = 64, dtype=torch.bfloat16) -> List[paged.PagedCache]:
+        """A paged K/V cache per layer, ``dtype`` bfloat16 or float8_e4m3fn (half the memory)."""
+        return [paged.PagedCache.empty(pages, page, self.cfg.num_kv_heads, dtype, self.dev) for _ in range(self.cfg.num_layers)]
+
+    def paged_step(self, plan: paged.PagedPlan, caches: Sequence[paged.PagedCache], ids: Optional[torch.Tensor] = None,
+                   embeds: Optional[torch.Tensor] = None, pos3: Optional[torch.Tensor] = None):
+        """Understanding-branch forward of a plan's new tokens: chunks of prompts, decode steps, or both.  ``ids`` [plan.rows] or
+        ``embeds`` [plan.rows, H] are those of all sequences one after another, ``pos3`` their (t, h, w) indexes (default: text,
+        at the tokens' places in their sequences).  Returns the hidden rows after the last layer, as :meth:`prefill` does for
+        the last ones.  May be captured in a CUDA graph that begins with ``plan.advance()``, with ``ids`` on the device."""
+        if len(caches) != self.cfg.num_layers:
+            raise ValueError(f"paged_step needs one cache per layer ({self.cfg.num_layers})")
+        if (ids is None) == (embeds is None):
+            raise ValueError("paged_step takes ids or embeds")
+        x = self.p["embed_tokens"].index_select(0, ids.to(self.dev).long()) if embeds is None else embeds.contiguous()
+        if x.shape[0] != plan.rows:
+            raise ValueError(f"the plan has {plan.rows} new tokens, not {x.shape[0]}")
+        if pos3 is None:
+            pos = plan.positions()
+            pos3 = torch.stack([pos, torch.zeros_like(pos), torch.zeros_like(pos)])
+        return self.layers(x, UND, pos3.to(self.dev).int().contiguous(), plan, None, 0, caches=caches).clone()
 
     # ------------------------------------------------------------ text decoding
     def decode_greedy(self, layouts: List[DocLayout], last_hidden, max_new_tokens: int,

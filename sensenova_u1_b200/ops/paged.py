@@ -143,6 +143,8 @@ class PagedPlan:
     grow: int
     _store: torch.Tensor = field(repr=False)
     _args: _Args = field(repr=False)
+    _rows: torch.Tensor = field(repr=False)       # sequence of every row
+    _ends: torch.Tensor = field(repr=False)       # row behind the last of every sequence
 
     def __post_init__(self):
         self._index = self.device.index
@@ -156,6 +158,11 @@ class PagedPlan:
         """Every sequence has ``tokens`` more (up to ``grow`` in all): its new rows are the ``q_len`` last ones of the longer
         sequence.  Runs on the device and may be captured; :func:`paged_read` keeps the lengths that the plan was made with."""
         self.kv_len.add_(tokens)
+
+    def positions(self) -> torch.Tensor:
+        """Place of every new row in its sequence, int32 on the device (by the lengths that the device has, also in a captured step)."""
+        seq = self._rows.long()
+        return self.kv_len[seq] - self._ends[seq] + torch.arange(self.rows, dtype=torch.int32, device=self.device)
 
 
 def _shares(tiles: np.ndarray, heads: int, slots: int, least: int) -> np.ndarray:
@@ -352,7 +359,8 @@ def build_plan(cache: PagedCache, heads: int, q_lens, kv_lens, tables, limits=No
     scratch = joined * HEAD_DIM * 4 + (joined + counts["few_parts"] * cache.kv_heads + 15) // 16 * 128 + counts["unpack_count"] * cache.kv_heads * (2 * CHUNK_TILE * HEAD_DIM * 2 + 16)
     return PagedPlan(heads, cache.kv_heads, cache.page, cache.pages, cache.data.dtype, cache.device,
                      [int(x) for x in q_lens], [int(x) for x in kv_lens],
-                     counts["rows"], int(arrays["k_start"][-1]), scratch, store[at["kv_len"]:at["kv_len"] + n], grow, store, args)
+                     counts["rows"], int(arrays["k_start"][-1]), scratch, store[at["kv_len"]:at["kv_len"] + n], grow, store, args,
+                     store[at["row_seq"]:at["row_seq"] + counts["rows"]], store[at["q_start"] + 1:at["q_start"] + 1 + n])
 
 
 _BF16 = torch.bfloat16

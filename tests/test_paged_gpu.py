@@ -515,3 +515,90 @@ def test_a_page_that_does_not_exist_is_reported():
         same = cache.data == before
         same[tables[1][1], :, :, 3] = True               # the second sequence's new token
         assert same.all()
+
+
+# ------------------------------------------------------------------ the engine over pages
+@pytest.mark.parametrize("dtype", [BF16, E4M3])
+def test_engine_in_chunks_and_captured_tokens(dtype):
+    """Two documents through ``InferenceEngine.paged_step``: prompts in chunks while the other decodes, then fixed tokens in a captured
+    step, against the layers of the oracle in fp32."""
+    from sensenova_u1_b200.config import tiny_mot
+    from sensenova_u1_b200.inference.engine import InferenceEngine
+    from sensenova_u1_b200.models import oracle
+    from sensenova_u1_b200.models.params import ParamStore
+    from sensenova_u1_b200.ops import paged
+    from sensenova_u1_b200.ops.attention import make_meta
+    cfg = tiny_mot(head_dim=128, patch_size=16, num_layers=2)
+    store = ParamStore(cfg, device="cuda", with_grads=False)
+    store.init_weights(3, std=0.05)
+    eng = InferenceEngine(cfg, store)
+    steps = [[150, 30], [61, 1], [1, 1], [1, 1], [1, 1], [1, 1]]
+    total = [sum(s[i] for s in steps) for i in range(2)]
+    g = torch.Generator().manual_seed(2)
+    ids = [torch.randint(8, cfg.vocab_size, (n,), generator=g) for n in total]
+    tables, pages = tables_for(total, 32)
+    caches = eng.paged_caches(pages, 32, dtype)
+    got, at = [[], []], [0, 0]
+
+    def take(h, s):
+        for i in range(2):
+            got[i].append(h[sum(s[:i]):sum(s[:i + 1])].clone())
+            at[i] += s[i]
+
+    for s in steps[:3]:
+        plan = paged.build_plan(caches[0], cfg.num_heads, s, [a + n for a, n in zip(at, s)], tables)
+        take(eng.paged_step(plan, caches, ids=torch.cat([ids[i][at[i]:at[i] + s[i]] for i in range(2)])), s)
+    left = len(steps) - 3
+    plan = paged.build_plan(caches[0], cfg.num_heads, [1, 1], at, tables, grow=left)
+    tok = torch.zeros(2, dtype=torch.long, device="cuda")
+    out = torch.zeros(2, cfg.hidden_size, device="cuda", dtype=BF16)
+
+    def step():
+        plan.advance()
+        out.copy_(eng.paged_step(plan, caches, ids=tok))
+
+    tok.copy_(torch.tensor([ids[i][at[i]] for i in range(2)]))
+    step()                                                # warm
+    plan.advance(-1)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        step()
+    for _ in range(left):
+        tok.copy_(torch.tensor([ids[i][at[i]] for i in range(2)]))
+        graph.replay()
+        take(out, [1, 1])
+    assert at == total
+    p32 = {k: v.float() for k, v in store.p.items()}
+    for i, n in enumerate(total):
+        x = p32["embed_tokens"][ids[i].cuda()]
+        pos = torch.arange(n, device="cuda")
+        meta = make_meta(torch.zeros(n, device="cuda"), pos)
+        mask, isg = oracle.dense_mask(meta, meta), torch.zeros(n, dtype=torch.bool, device="cuda")
+        pos3 = torch.stack([pos, torch.zeros_like(pos), torch.zeros_like(pos)])
+        for l in range(cfg.num_layers):
+            x = oracle.decoder_layer(p32, l, x, isg, pos3, mask, cfg)
+        h = torch.cat(got[i]).float()
+        # bf16 activations: the bound of the engine's other tests.  e4m3: half a step of every cached value, 2^-4, besides.
+        assert ((h - x).norm() / x.norm()).item() < 3e-2 + (0 if dtype == BF16 else 2.0 ** -4)
+
+
+def test_engine_refusals():
+    from sensenova_u1_b200.config import tiny_mot
+    from sensenova_u1_b200.inference.engine import InferenceEngine
+    from sensenova_u1_b200.models.params import ParamStore
+    from sensenova_u1_b200.ops import paged
+    cfg = tiny_mot(head_dim=128, patch_size=16, num_layers=2)
+    store = ParamStore(cfg, device="cuda", with_grads=False)
+    store.init_weights(0)
+    eng = InferenceEngine(cfg, store)
+    caches = eng.paged_caches(4, 16)
+    plan = paged.build_plan(caches[0], cfg.num_heads, [3], [3], [[1]])
+    ids = torch.tensor([5, 6, 7])
+    with pytest.raises(ValueError):
+        eng.paged_step(plan, caches[:1], ids=ids)
+    with pytest.raises(ValueError):
+        eng.paged_step(plan, caches, ids=ids[:2])
+    with pytest.raises(ValueError):
+        eng.paged_step(plan, caches)
+    assert eng.paged_step(plan, caches, ids=ids).shape == (3, cfg.hidden_size)
