@@ -61,7 +61,9 @@ __global__ void __launch_bounds__(WRITE_THREADS)
     const int row = row0 + threadIdx.x, b = p.row_seq[row];
     const int pos = seq_len(p, b) - (p.q_start[b + 1] - row);
     long long at = -1;
-    if (pos >= 0) {
+    if (p.kv_len[b] > p.cap[b]) {                    // grown past what the plan has pages for
+      report_status(status, kBadShape, 9);
+    } else if (pos >= 0) {
       const int pg = p.table[(long long)b * p.width + pos / p.page];
       if (pg >= 0 && pg < pages) at = (long long)pg * 2 * heads * p.page + pos % p.page;
       else report_status(status, kBadPage, 9);
@@ -307,6 +309,10 @@ SNU1_API int snu1_paged_cache_init(void* out, void* data, void* scales, int page
     const uint32_t box[4] = {64, (uint32_t)page, 1, 1};
     if ((rc = encode_tmap(&c.k, TmapType::kBf16, true, data, 4, dims, str, box)) != kHostOk) return rc;
     if ((rc = encode_tmap(&c.v, TmapType::kBf16, true, (uint8_t*)data + row * P * H, 4, dims, str, box)) != kHostOk) return rc;
+  }
+  if (device_status_word() == nullptr) {          // here and not in a first call that may be captured
+    set_last_error("paged_cache: no status word (cudaMalloc failed?)");
+    return kHostCuda;
   }
   memcpy(out, &c, sizeof(c));
   return kHostOk;

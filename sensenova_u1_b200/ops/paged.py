@@ -155,8 +155,8 @@ class PagedPlan:
         self._addr = ctypes.addressof(self._args)
 
     def advance(self, tokens: int = 1) -> None:
-        """Every sequence has ``tokens`` more (up to ``grow`` in all): its new rows are the ``q_len`` last ones of the longer
-        sequence.  Runs on the device and may be captured; :func:`paged_read` keeps the lengths that the plan was made with."""
+        """Every sequence has ``tokens`` more (up to ``grow`` in all; beyond that nothing is written, and ``check_status`` raises):
+        its new rows are the ``q_len`` last ones of the longer sequence.  Runs on the device and may be captured; :func:`paged_read` keeps the lengths that the plan was made with."""
         self.kv_len.add_(tokens)
 
     def positions(self) -> torch.Tensor:
@@ -415,7 +415,12 @@ def paged_read(cache: PagedCache, plan: PagedPlan) -> tuple[torch.Tensor, torch.
 def paged_attention(q: torch.Tensor, cache: PagedCache, plan: PagedPlan, scale: float, out: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of the plan's new rows over their sequences' cached keys, softmax in fp32.  ``q``: [at least plan.rows, heads,
     128] bf16, rows may be slices of wider ones; returns ``out`` (default: new, [plan.rows, heads, 128]), whose rows behind
-    the last sequence are left as they are.  ``scale`` is positive."""
+    the last sequence are left as they are.  ``scale`` is positive.
+
+    A row that may read a key or value that is not finite is NaN, in part or whole; other rows are as if it were not there.
+    What lies behind a sequence's last token or in pages of nobody does not matter.  Chunks (more than 32 rows per key/value
+    head) over e4m3 hold 128 cached values of a head relative to the largest of them: values 2^14 times smaller than that lose
+    bits."""
     _check(cache, plan)
     ldq = _row_stride("q", q, plan, plan.heads)
     if out is None:

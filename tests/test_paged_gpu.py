@@ -454,6 +454,94 @@ def test_offsets_beyond_32_bits():
     assert near(paged.paged_attention(q, cache, plan, SCALE), ref, room)
 
 
+def test_two_graphs_of_one_plan_at_once():
+    """Scratch belongs to a call: two captured graphs of the same plan run on two streams at the same time."""
+    from sensenova_u1_b200.ops import paged
+    kv = [3000, 900, 5000, 17]
+    cache, tables, _ = make(kv, 16, 8, E4M3)
+    q = torch.randn(2, 4, 32, D, device="cuda", generator=torch.Generator(device="cuda").manual_seed(8)).to(BF16)
+    plan = paged.build_plan(cache, 32, [1] * 4, kv, tables)
+    assert plan.scratch > 0                               # parts meet in scratch
+    want = [paged.paged_attention(x, cache, plan, SCALE).clone() for x in q]
+    graphs, outs = [], [torch.empty(4, 32, D, device="cuda", dtype=BF16) for _ in q]
+    torch.cuda.synchronize()
+    for x, o in zip(q, outs):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            for _ in range(8):
+                paged.paged_attention(x, cache, plan, SCALE, out=o)
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in q]
+    for _ in range(10):
+        for s, g, o in zip(streams, graphs, outs):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                o.fill_(7.0)
+                g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, w) for o, w in zip(outs, want))
+
+
+@pytest.mark.parametrize("dtype", [BF16, E4M3])
+@pytest.mark.parametrize("q_lens,kv_lens", [([3, 1], [200, 90]), ([40, 100], [500, 100]), ([200], [200])])
+def test_a_query_that_is_not_finite_is_its_own_matter(q_lens, kv_lens, dtype):
+    from sensenova_u1_b200.ops import paged
+    cache, tables, _ = make(kv_lens, 16, 2, dtype)
+    plan = paged.build_plan(cache, 8, q_lens, kv_lens, tables)
+    q = torch.randn(sum(q_lens), 8, D, device="cuda", generator=torch.Generator(device="cuda").manual_seed(2)).to(BF16)
+    clean = paged.paged_attention(q, cache, plan, SCALE)
+    bad = q.clone()
+    bad[1, 3, 5], bad[2, 6, 100], bad[0, 0, 0] = float("nan"), float("inf"), -float("inf")
+    out = paged.paged_attention(bad, cache, plan, SCALE)
+    hit = torch.zeros(q.shape[:2], dtype=torch.bool, device="cuda")
+    hit[1, 3] = hit[2, 6] = hit[0, 0] = True
+    assert torch.equal(out[~hit], clean[~hit]) and not torch.isfinite(out[hit]).all(-1).any()
+
+
+def test_many_short_sequences():
+    attend([1] * 300, [1 + (7 * i) % 40 for i in range(300)], 8, 2, 16, E4M3)
+    attend([2] * 300, [2 + (7 * i) % 40 for i in range(300)], 8, 2, 16, BF16)
+    attend([9 + i % 8 for i in range(100)], [60 + (7 * i) % 90 for i in range(100)], 8, 2, 16, E4M3)
+
+
+@pytest.mark.parametrize("dtype", [BF16, E4M3])
+def test_more_heads_in_a_group_than_rows_in_a_tile(dtype):
+    attend([1, 3], [40, 200], 130, 1, 16, dtype)
+
+
+def test_values_of_very_different_sizes():
+    """Scales from 2^-40 to 2^40 in one sequence: a token's probabilities are kept relative to the largest product, not the largest value."""
+    from sensenova_u1_b200.ops import paged
+    kv, page = [300, 700], 32
+    tables, pages = tables_for(kv, page)
+    g = torch.Generator(device="cuda").manual_seed(6)
+    x = torch.randn(pages, 2, 2, page, D, device="cuda", generator=g).to(BF16)
+    x[:, 1] *= torch.exp2(torch.randint(-40, 41, (pages, 2, page, 1), device="cuda", generator=g)).to(BF16)
+    codes, scales = quantised(x)
+    cache, held = paged.PagedCache(codes, scales), codes.double() * scales.double()[..., None]
+    rows = [torch.cat([held[p] for p in t], 2)[:, :, :k] for t, k in zip(tables, kv)]
+    q = (3 * torch.randn(3, 8, D, device="cuda", generator=g)).to(BF16)
+    plan = paged.build_plan(cache, 8, [1, 2], kv, tables)
+    ref, room = exact(q, [1, 2], rows, causal([1, 2], kv), E4M3)
+    assert near(paged.paged_attention(q, cache, plan, SCALE), ref, room)
+
+
+def test_growing_past_the_plan_is_reported():
+    from sensenova_u1_b200.ops import _lib, paged
+    cache = paged.PagedCache.empty(2, 16, 1)
+    cache.data.zero_()
+    plan = paged.build_plan(cache, 1, [1], [3], [[1, 0]], grow=2)
+    one = torch.ones(1, 1, D, device="cuda", dtype=BF16)
+    for n in range(3):
+        paged.paged_write(cache, one, one, plan)
+        _lib.check_status()
+        plan.advance()
+    paged.paged_write(cache, one, one, plan)             # a sixth token
+    with pytest.raises(_lib.NativeLibraryError, match="limit"):
+        _lib.check_status()
+    assert cache.data[1, 0, 0, :, 0].tolist() == [0, 0, 1, 1, 1] + [0] * 11 and (cache.data[0] == 0).all()
+
+
 # ------------------------------------------------------------------ refusals
 def test_refusals():
     from sensenova_u1_b200.ops import paged
