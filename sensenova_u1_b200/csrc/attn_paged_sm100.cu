@@ -11,8 +11,8 @@
 //   are fp16 as well.  So the softmax pays for the scales once per tile and row, not per score: the keys' power of two goes
 //   into the factor of the scores, the values' into the exponent of the probabilities (and out of their sum).  Scales
 //   applied per score and probability in fp32 took 2.33 us per pair of tiles instead of 1.78 (2 x 512 new tokens, 8192 keys);
-//   keys rounded to bf16 would move every score by up to 2^-8 of the sum of |q k|.  The queries are scaled row by row as in
-//   attn_paged.cu, by the softmax warps.
+//   keys rounded to bf16 would move every score by up to 2^-8 of the sum of |q k|.  The queries are scaled 16 rows at a time, by
+//   the softmax warps.
 // * The mask is one number per row, the keys that it may read; tiles that all rows read whole need no test.
 // * A work item is a part of the key tiles of two row tiles; unnormalised results of parts are joined by
 //   paged_merge_kernel.  ops/paged.py chooses the parts so that the waves of CTAs are full.
@@ -209,10 +209,18 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
   const int b = item.x, part = item.z & 0xffff, parts = item.z >> 16;
   const int kvh = blockIdx.x % args.heads, G = p.group, T = 128 / G;       // tokens of a row tile
   const int q0 = p.q_start[b], q_len = p.q_start[b + 1] - q0;
+  const int token0 = item.y / G;
   pdl_wait();
   pdl_trigger();
+  if (threadIdx.x == 0) {                       // the queries do not depend on what is looked up below
+    mbar_expect_tx(q_full, 2 * TILES * T * G * 128);
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) {
+      tma_load_3d(sQ + t * CTILE, &tm_q, q_full, 0, kvh * G, q0 + token0 + t * T);
+      tma_load_3d(sQ + t * CTILE + CHALF, &tm_q, q_full, 64, kvh * G, q0 + token0 + t * T);
+    }
+  }
   const int kv_len = seq_len(p, b);
-  const int token0 = item.y / G;
   int max_a, max_b, min_a, min_b;               // the largest and the smallest limit of row tiles A and B
   if (p.behind == nullptr) {                    // limits grow from token to token
     const int ends = min(token0 + TILES * T, q_len) - 1;
@@ -245,16 +253,9 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     if (warp == 0) {
-      if (n > 0) {
-        if (lane == 0) {
-          mbar_expect_tx(q_full, 2 * TILES * T * G * 128);
-#pragma unroll
-          for (int t = 0; t < TILES; ++t) {
-            tma_load_3d(sQ + t * CTILE, &tm_q, q_full, 0, kvh * G, q0 + token0 + t * T);
-            tma_load_3d(sQ + t * CTILE + CHALF, &tm_q, q_full, 64, kvh * G, q0 + token0 + t * T);
-          }
-        }
-        __syncwarp();
+      if (n == 0) {
+        mbar_wait_warp(q_full, 0, abort_flag, args.status, 1);      // nobody else does, and the CTA has to outlive the copy
+      } else {
         const int page = args.page, per = BK / page, used = (most + page - 1) / page;   // pages of a tile, of the sequence
         const int* table = args.first_page == nullptr ? p.table + (long long)b * p.width : nullptr;
         const int base = args.first_page == nullptr ? 0 : args.first_page[b];
@@ -536,31 +537,50 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     float sc[2] = {args.scale_log2, args.scale_log2};
     bool ok = true;
     if (FP16 && n > 0) {
-      // this warp's 16 query rows to fp16, each times a power of two (see attn_paged.cu)
+      // This warp's 16 query rows to fp16, all times the power of two that brings the largest value to [2^13, 2^14).  Smaller rows
+      // lose 2^-38 of that value at most, so a score is off by less than 2^-34 of the largest one's sum of |q k|.
       ok &= mbar_wait(q_full, 0, abort_flag, args.status, 5);
       __syncwarp();
       uint8_t* at = sOt + ((lane & 15) >> 3) * CHALF;
       uint4 u[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) u[i] = *reinterpret_cast<const uint4*>(at + swz128_offset(base + 2 * i + (lane >> 4), lane & 7));
+      // rows of nobody decide nothing
+      const int mine = (min(token0 + (t + 1) * T, q_len) - (token0 + t * T)) * G - base;     // rows of this warp that are somebody's
+      uint32_t top = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (2 * i + (lane >> 4) >= mine) u[i] = make_uint4(0, 0, 0, 0);
+        top = max_u16x2(top, max_u16x2(max_u16x2(u[i].x & 0x7fff7fffu, u[i].y & 0x7fff7fffu), max_u16x2(u[i].z & 0x7fff7fffu, u[i].w & 0x7fff7fffu)));
+      }
+      top = __reduce_max_sync(0xffffffffu, max(top << 16, top & 0xffff0000u));
+      if (top >= 0x7f800000u) {              // some value is not finite: the largest of the others
+        top = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const uint32_t* w = reinterpret_cast<const uint32_t*>(&u[i]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t lo = (w[e] << 16) & 0x7fffffffu, hi = w[e] & 0x7fff0000u;
+            top = max(top, max(lo < 0x7f800000u ? lo : 0u, hi < 0x7f800000u ? hi : 0u));
+          }
+        }
+        top = __reduce_max_sync(0xffffffffu, top);
+      }
+      const int up = top == 0 ? 0 : min(13 - ((int)(top >> 23) - 127), 120);
+      const float f = __int_as_float((127 + up) << 23);
+      const uint64_t f2 = pack_f32x2(f, f);
+      sc[0] = sc[1] = args.scale_log2 * __int_as_float((127 - up) << 23);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         uint32_t* w = reinterpret_cast<uint32_t*>(&u[i]);
-        uint32_t top = 0;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) top = max(top, max((w[e] << 16) & 0x7fffffffu, w[e] & 0x7fff0000u));
-#pragma unroll
-        for (int o = 1; o < 16; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const int ex = (int)(top >> 23) - 127, up = top == 0 || ex == 128 ? 0 : min(13 - ex, 120);
-        const float f = __int_as_float((127 + up) << 23);
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          w[e] = pack_f16x2(__uint_as_float(w[e] << 16) * f, __uint_as_float(w[e] & 0xffff0000u) * f);
+        for (int e = 0; e < 4; ++e) {
+          float x, y;
+          unpack_f32x2(mul_f32x2(bf16x2_to_f32x2(w[e]), f2), x, y);
+          w[e] = pack_f16x2(x, y);
+        }
         *reinterpret_cast<uint4*>(at + swz128_offset(base + 2 * i + (lane >> 4), lane & 7)) = u[i];
-        const int own = __shfl_sync(0xffffffffu, up, (lane >> 2 & 1) * 16);     // of row 2 i or 2 i + 1
-#pragma unroll
-        for (int r = 0; r < 2; ++r)
-          if (i == (lane >> 3) + 4 * r) sc[r] *= __int_as_float((127 - own) << 23);
       }
       fence_proxy_async_smem();
       __syncwarp();

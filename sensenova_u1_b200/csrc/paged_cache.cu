@@ -29,11 +29,6 @@ __device__ __forceinline__ void decode8(uint2 u, float (&f)[8]) {
   }
 }
 
-__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
-  uint32_t r;
-  asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
-}
 // two numbers as codes, the first in the low byte
 __device__ __forceinline__ uint32_t e4m3x2(uint64_t x) {
   float lo, hi;
