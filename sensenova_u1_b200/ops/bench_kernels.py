@@ -6,7 +6,9 @@ small cases that profiler captures are taken on:
 
 Kernels: gemm_w13 / gemm_w2 / gemm_qkv (8B-MoT projection shapes at 16384 rows, grouped by MoT
 branch), gemm_wgrad (dy^T x), attn_fwd / attn_bwd (causal packed documents, 32 query / 8 kv heads,
-head 128), rmsnorm, qknorm_rope, swiglu, adamw.  Prints one JSON line per kernel with the time,
+head 128), rmsnorm, qknorm_rope, swiglu, adamw, paged_write / paged_read (32 K tokens into and out of an e4m3 cache, 8 heads),
+paged_step (24 sequences of up to 4 K keys, one new token each, 32 / 8 heads), paged_drafts (8 new tokens each), paged_chunk
+(2 x 512 new tokens over 8 K keys), each over bf16 and e4m3 pages.  Prints one JSON line per kernel with the time,
 achieved TFLOP/s or GB/s and the fraction of the measured peaks when MEASURED_PEAKS.json is present.
 """
 from __future__ import annotations
@@ -209,6 +211,39 @@ def main():
                    args.iters, flush)
         sb = 4 if args.adamw_state == "fp32" else 2
         report(f"adamw_{args.adamw_state}_moments_{n >> 20}Mi", ms, nbytes=n * (6.0 + 2 * sb) + n * (4.0 + 2 * sb))
+    for fmt in (torch.bfloat16, torch.float8_e4m3fn):
+        from . import paged
+        tag = "bf16" if fmt == torch.bfloat16 else "e4m3"
+        Hq, Hk, D, page = 32, 8, 128, 64
+        row = Hk * 2 * (2 * D if tag == "bf16" else D + 4)                # bytes of a cached token
+
+        def paged_case(q_lens, kv_lens):
+            need = [-(-n // page) for n in kv_lens]
+            order = torch.randperm(sum(need)).tolist()
+            tables = [order[sum(need[:i]):sum(need[:i + 1])] for i in range(len(need))]
+            cache = paged.PagedCache.empty(sum(need), page, Hk, fmt)
+            fill = paged.build_plan(cache, Hq, kv_lens, kv_lens, tables)
+            kv = rnd(2, sum(kv_lens), Hk, D) * 20
+            paged.paged_write(cache, kv[0], kv[1], fill)
+            return cache, paged.build_plan(cache, Hq, q_lens, kv_lens, tables), rnd(max(1, sum(q_lens)), Hq, D) * 20, fill, kv
+
+        if want("paged_write") or want("paged_read"):
+            cache, _, _, fill, kv = paged_case([0], [32000])
+            if want("paged_write"):
+                ms = _time(lambda: paged.paged_write(cache, kv[0], kv[1], fill), args.iters, flush)
+                report("paged_write_" + tag, ms, nbytes=32000.0 * (row + Hk * D * 4))
+            if want("paged_read"):
+                ms = _time(lambda: paged.paged_read(cache, fill), args.iters, flush)
+                report("paged_read_" + tag, ms, nbytes=32000.0 * (row + Hk * D * 4))
+        steps = [62 + 175 * i for i in range(24)]
+        for name, q_lens, kv_lens in (("paged_step", [1] * 24, steps), ("paged_drafts", [8] * 24, steps), ("paged_chunk", [512] * 2, [8192] * 2)):
+            if not want(name):
+                continue
+            cache, plan, q, _, _ = paged_case(q_lens, kv_lens)
+            o = torch.empty_like(q)
+            ms = _time(lambda: paged.paged_attention(q, cache, plan, D ** -0.5, out=o), args.iters, flush)
+            pairs = sum(n * (k - n) + n * (n + 1) / 2 for n, k in zip(q_lens, kv_lens))
+            report(f"{name}_{tag}", ms, flops=4.0 * D * Hq * pairs, nbytes=float(sum(kv_lens) * row + 4 * sum(q_lens) * Hq * D))
     check_status()
 
 
