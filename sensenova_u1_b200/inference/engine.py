@@ -349,6 +349,8 @@ class InferenceEngine:
         x = self.p["embed_tokens"].index_select(0, ids.to(self.dev).long()) if embeds is None else embeds.contiguous()
         if x.shape[0] != plan.rows:
             raise ValueError(f"the plan has {plan.rows} new tokens, not {x.shape[0]}")
+        if plan.rows == 0:
+            return x
         if pos3 is None:
             pos = plan.positions()
             pos3 = torch.stack([pos, torch.zeros_like(pos), torch.zeros_like(pos)])

@@ -1,7 +1,8 @@
 """Paged key/value cache and attention over it (csrc/paged_cache.cu, csrc/attn_paged.cu, csrc/attn_paged_sm100.cu).
 
 A :class:`PagedCache` holds the keys and values of one layer in pages of 16, 32, 64 or 128 tokens, as bf16 or as e4m3 codes with
-one fp32 scale per token and head (half the memory: 132 bytes of 256).  A sequence owns pages in any order; several sequences may
+one fp32 scale per token and head (half the memory: 132 bytes of 256).  Codes are finite and scales not negative, as
+:func:`paged_write` leaves them; a row that holds a value that is not finite has NaN as its scale.  A sequence owns pages in any order; several sequences may
 read the same page (a shared prompt), only one may write it.
 
 One :class:`PagedPlan` describes a step: how many new tokens every sequence brings, how many tokens it has then, and its
@@ -199,9 +200,9 @@ def _lay_out(q_lens, kv_lens, tables, page: int, pages: int, group: int, kv_head
     cap = np.where(q > 0, kv + grow, kv)
     need = -(-cap // page)
     width = max(1, int(need.max()) if n else 1)
-    table = np.zeros((n, width), dtype=np.int32)
+    table = np.zeros((n, width), dtype=np.int64)
     if isinstance(tables, torch.Tensor):
-        if tables.is_cuda or tables.dim() != 2:
+        if tables.is_cuda or tables.dim() != 2 or tables.is_floating_point():
             raise ValueError("page tables are lists of page numbers, or one host tensor [sequences, pages]")
         tables = tables.numpy()
     if len(tables) != n:
@@ -210,8 +211,10 @@ def _lay_out(q_lens, kv_lens, tables, page: int, pages: int, group: int, kv_head
         if len(tables[i]) < need[i]:
             raise ValueError(f"sequence {i} needs {need[i]} pages for {cap[i]} tokens, its table has {len(tables[i])}")
         table[i, :need[i]] = tables[i][:need[i]]
-        if need[i] and (table[i, :need[i]].min() < 0 or table[i, :need[i]].max() >= pages):
-            raise ValueError(f"sequence {i} names a page that the cache does not have")
+    if n and (table.min() < 0 or table.max() >= pages):          # (places that are not needed hold 0)
+        i = int(((table < 0) | (table >= pages)).any(1).argmax())
+        raise ValueError(f"sequence {i} names a page that the cache does not have")
+    table = table.astype(np.int32)
     rows = int(q.sum())
     row_seq = np.repeat(np.arange(n, dtype=np.int32), q)
     behind = None
@@ -255,6 +258,8 @@ def _lay_out(q_lens, kv_lens, tables, page: int, pages: int, group: int, kv_head
     merge = [] if few_rows <= FEW_JOIN else [merge]
 
     def chunks_of(which, m, partial):
+        if not which.any():
+            return np.zeros((0, 4), np.int32), partial
         seq, row0 = tiles_of(np.where(which, q_rows, 0), m)
         if limits is None:                                    # a row tile reads up to its last token
             last = np.minimum((row0 + m - 1) // group, q[seq] - 1)
@@ -267,7 +272,7 @@ def _lay_out(q_lens, kv_lens, tables, page: int, pages: int, group: int, kv_head
 
     one, partial = chunks_of(single, tile_rows, partial)
     chunk, partial = chunks_of(chunked & ~single, 2 * tile_rows, partial)
-    merge = np.concatenate(merge)
+    merge = np.concatenate(merge) if merge else np.zeros((0, 4), np.int32)
     unpack = unpack_first = None
     if fp8 and len(chunk):
         wide = np.where(chunked & ~single, -(-cap // CHUNK_TILE), 0)    # 128-token pages
@@ -293,6 +298,8 @@ def _waves(tiles: np.ndarray, heads: int, slots: int) -> np.ndarray:
         share = -(-int(tiles.max()) // cut)
         parts = -(-tiles // share)
         cost = -(-tiles // parts) + CHUNK_START + np.where(parts > 1, CHUNK_JOIN, 0)
+        if best is not None and max(int((cost * parts).sum()) * heads / slots, int(cost.max())) + CHUNK_START / 2 >= 0.98 * best[0]:
+            continue                                          # could not be done sooner even if every CTA were as long
         cost = np.sort(np.repeat(cost, parts * heads))[::-1]
         if best is not None and len(cost) > 8 * slots:        # so many waves are full enough
             break
@@ -340,6 +347,8 @@ def build_plan(cache: PagedCache, heads: int, q_lens, kv_lens, tables, limits=No
     sees the whole picture, has the picture's end as its limit.  ``grow``: tokens that :meth:`PagedPlan.advance` may add."""
     if heads < 1 or heads % cache.kv_heads != 0:
         raise ValueError("the number of query heads must be a multiple of the cache's heads")
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("a plan is made before a CUDA graph is captured: the graph would copy from host memory that is gone")
     arrays, counts = _lay_out(q_lens, kv_lens, tables, cache.page, cache.pages, heads // cache.kv_heads, cache.kv_heads,
                               cache.scales is not None, limits, grow)
     # all arrays in one copy from pinned memory that nothing waits for
@@ -375,9 +384,13 @@ def _check(cache: PagedCache, plan: PagedPlan) -> None:
 def _row_stride(name: str, t: torch.Tensor, plan: PagedPlan, heads: int) -> int:
     """Elements from one row to the next of a [plan.rows or more, heads, 128] tensor."""
     shape, stride = t.shape, t.stride()
-    if (len(shape) != 3 or shape[0] < plan.rows or shape[1] != heads or shape[2] != HEAD_DIM or stride[2] != 1 or stride[1] != HEAD_DIM
-            or t.dtype is not _BF16 or t.get_device() != plan._index):
+    if (len(shape) != 3 or shape[0] < plan.rows or shape[1] != heads or shape[2] != HEAD_DIM or stride[2] != 1
+            or (stride[1] != HEAD_DIM and heads > 1) or t.dtype is not _BF16 or t.get_device() != plan._index):
         raise ValueError(f"{name} must be bf16 [{plan.rows} or more, {heads}, {HEAD_DIM}] with contiguous heads on the plan's device")
+    if stride[0] < heads * HEAD_DIM:
+        if shape[0] > 1:
+            raise ValueError(f"the rows of {name} overlap")
+        return heads * HEAD_DIM                                   # (one row's stride says nothing)
     return stride[0]
 
 
@@ -415,12 +428,13 @@ def paged_read(cache: PagedCache, plan: PagedPlan) -> tuple[torch.Tensor, torch.
 def paged_attention(q: torch.Tensor, cache: PagedCache, plan: PagedPlan, scale: float, out: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of the plan's new rows over their sequences' cached keys, softmax in fp32.  ``q``: [at least plan.rows, heads,
     128] bf16, rows may be slices of wider ones; returns ``out`` (default: new, [plan.rows, heads, 128]), whose rows behind
-    the last sequence are left as they are.  ``scale`` is positive.
+    the last sequence are left as they are; ``out`` may be ``q``.  ``scale`` is positive.
 
     A row that may read a key or value that is not finite is NaN, in part or whole; other rows are as if it were not there.
     What lies behind a sequence's last token or in pages of nobody does not matter.  Chunks (more than 32 rows per key/value
-    head) over e4m3 hold 128 cached values of a head relative to the largest of them: values 2^14 times smaller than that lose
-    bits."""
+    head) over e4m3 hold 128 cached tokens' values of a head relative to the largest of them: values 2^14 times smaller than that
+    lose bits.  Where the largest value of another 128 tokens is 2^d times larger (zeros count as 2^-90), probabilities below
+    2^(d - 133) of the largest one are lost."""
     _check(cache, plan)
     ldq = _row_stride("q", q, plan, plan.heads)
     if out is None:

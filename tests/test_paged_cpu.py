@@ -153,3 +153,10 @@ def test_the_plan_has_the_fields_of_the_kernels():
             names += [(x.strip(), kind) for x in m.group(2).split(",")]
     assert names == paged._Args._fields_
     assert f"PLAN_LAYOUT = {paged.PLAN_LAYOUT:#x}" in src
+
+
+@pytest.mark.parametrize("tables", [torch.tensor([[0, 0, 0], [1, 2, (1 << 32) + 3]]),           # would be page 3 in 32 bits
+                                    torch.tensor([[0, 0, 0], [1, 2, -(1 << 32)]]), torch.zeros(2, 3)])
+def test_page_numbers_that_are_none(tables):
+    with pytest.raises(ValueError):
+        paged._lay_out([1, 3], [5, 40], tables, 16, 4, 4, 2, False, None, 0)

@@ -605,6 +605,59 @@ def test_a_page_that_does_not_exist_is_reported():
         assert same.all()
 
 
+def test_rows_that_overlap_are_refused():
+    from sensenova_u1_b200.ops import paged
+    cache, tables, _ = make([40], 16, 2, BF16)
+    plan = paged.build_plan(cache, 8, [3], [40], tables)
+    q, k = torch.zeros(3, 8, D, device="cuda", dtype=BF16), torch.zeros(3, 2, D, device="cuda", dtype=BF16)
+    for call in (lambda: paged.paged_attention(q, cache, plan, SCALE, out=q[:1].expand(3, 8, D)),
+                 lambda: paged.paged_attention(q[:1].expand(3, 8, D), cache, plan, SCALE),
+                 lambda: paged.paged_write(cache, k[:1].expand(3, 2, D), k, plan)):
+        with pytest.raises(ValueError, match="overlap"):
+            call()
+
+
+@pytest.mark.parametrize("dtype", [BF16, E4M3])
+def test_the_stride_of_one_row_or_one_head_says_nothing(dtype):
+    from sensenova_u1_b200.ops import paged
+    cache, tables, _ = make([40], 16, 1, dtype)
+    one = lambda x: torch.as_strided(x, x.shape, (1, 8 if x.shape[1] == 1 else D, 1), x.storage_offset())
+    plan = paged.build_plan(cache, 4, [1], [40], tables)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    q, k, v = (torch.randn(1, h, D, device="cuda", generator=g).to(BF16) for h in (4, 1, 1))
+    paged.paged_write(cache, k, v, plan)
+    want, held = paged.paged_attention(q, cache, plan, SCALE), cache.data.view(torch.uint8).clone()
+    paged.paged_write(cache, one(k), one(v), plan)
+    assert torch.equal(cache.data.view(torch.uint8), held)
+    out = torch.empty(1, 4, D, device="cuda", dtype=BF16)
+    paged.paged_attention(one(q), cache, plan, SCALE, out=one(out))
+    assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("dtype", [BF16, E4M3])
+@pytest.mark.parametrize("q_lens,kv_lens", [([1], [3000]), ([1] * 9, [70 * i + 1 for i in range(9)]), ([6, 300, 1, 40], [800, 5000, 9, 40])])
+def test_the_output_may_be_the_queries(q_lens, kv_lens, dtype):
+    from sensenova_u1_b200.ops import paged
+    cache, tables, _ = make(kv_lens, 32, 2, dtype)
+    plan = paged.build_plan(cache, 8, q_lens, kv_lens, tables)
+    g = torch.Generator(device="cuda").manual_seed(6)
+    q = torch.randn(sum(q_lens), 8, D, device="cuda", generator=g).to(BF16)
+    want = paged.paged_attention(q, cache, plan, SCALE)
+    assert paged.paged_attention(q, cache, plan, SCALE, out=q) is q
+    assert torch.equal(q, want)
+
+
+def test_a_plan_is_not_made_in_a_capture():
+    from sensenova_u1_b200.ops import paged
+    cache, tables, _ = make([40], 16, 2, BF16)
+    graph, x = torch.cuda.CUDAGraph(), torch.zeros(4, device="cuda")
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        x.add_(1)
+        with pytest.raises(RuntimeError, match="captured"):
+            paged.build_plan(cache, 8, [3], [40], tables)
+
+
 # ------------------------------------------------------------------ the engine over pages
 @pytest.mark.parametrize("dtype", [BF16, E4M3])
 def test_engine_in_chunks_and_captured_tokens(dtype):
@@ -690,3 +743,5 @@ def test_engine_refusals():
     with pytest.raises(ValueError):
         eng.paged_step(plan, caches)
     assert eng.paged_step(plan, caches, ids=ids).shape == (3, cfg.hidden_size)
+    empty = paged.build_plan(caches[0], cfg.num_heads, [0], [3], [[1]])
+    assert eng.paged_step(empty, caches, ids=ids[:0]).shape == (0, cfg.hidden_size)
