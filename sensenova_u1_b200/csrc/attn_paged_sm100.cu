@@ -618,7 +618,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
       __syncwarp();
       if (lane == 0) {
         mbar_arrive(&s_empty[t]);
-        tally_add(&drained[t]);
+        if (TILES > 1) tally_add(&drained[t]);
       }
       if (j >= full) {
 #pragma unroll
@@ -694,7 +694,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
       if (j > 0) ok &= mbar_wait(&pv_done[t], (j - 1) & 1, abort_flag, args.status, 5);
       // The other tile's warps have read the scores that P goes over: of the score tiles issued before PV_t(j), which are key tiles
       // 0 .. j of B for A, 0 .. j + 1 of A for B.
-      ok &= tally_wait(&drained[t ^ 1], 8 * (t == 0 ? min(j + 1, n_b) : min(j + 2, n_a)), abort_flag, args.status, 5);
+      if (TILES > 1) ok &= tally_wait(&drained[t ^ 1], 8 * (t == 0 ? min(j + 1, n_b) : min(j + 2, n_a)), abort_flag, args.status, 5);
       tc_fence_after();
       tmem_st_16x128b_x16(tmem_P, pk);
       if (j > 0 && rescale) {
