@@ -10,8 +10,7 @@
 // eight, and all CTAs still run at once, the parts of a sequence are a cluster and meet in distributed shared memory: a
 // small batch, where latency counts.  Otherwise they meet in scratch, see last_part and paged_join_kernel.
 //
-// One warp asks for whole pages through TMA (keys and values of one head in one box), several stages ahead; four warps
-// compute with mma.sync m16n8k16, keys (then the width of a head) on the 16-side and rows on the 8-side: S^T = K q^T,
+// Pages come whole through TMA (keys and values of one head in one box), several stages ahead.  Four warps compute with mma.sync m16n8k16, keys (then the width of a head) on the 16-side and rows on the 8-side: S^T = K q^T,
 // o^T = V^T p^T.  So a step of a group of 4 or 8 heads fills the product, and what a warp has read and widened of the cache
 // serves all rows.  At 1 - 2 products per KB of cache the legacy tensor path is far from its limit.
 //
@@ -40,13 +39,18 @@
 namespace snu1 {
 namespace paged {
 
-constexpr int FEW_WARPS = 4;                              // warps that compute; one more asks for pages
-constexpr int FEW_THREADS = FEW_WARPS * 32 + 32;
+constexpr int FEW_WARPS = 4;                              // warps that compute
 constexpr int FEW_LD = 132;                               // a row of 128 values where warps meet, padded
 
-// SMALL: up to eight rows.  Their registers let three CTAs run on an SM, with two stages each instead of three.
-template <bool FP8, bool SMALL>
+// Up to eight rows: their registers let three CTAs run on an SM, with two stages each instead of three.
+// SELF: a fifth warp asks for pages, except with 24 rows per warp.  Five warps of two CTAs are three in a quarter of the SM,
+// 168 registers each; four have 255, which 24 rows need, so there the warp that is the last to be done with a stage asks
+// for what goes there next.  (17 to 24 rows, 8 x 12000 keys: e4m3 61 us, as 2 x 2 groups of eight rows 85, each code then
+// widened by two warps; bf16 67 and 71.  32 rows as four groups per warp: 152 and 89.  Up to 16 rows without the fifth warp: 1 to 4 % slower.)
+template <bool FP8, int NR, int WR>
 struct Few {
+  static constexpr bool SMALL = NR * WR == 1, SELF = NR == 3;
+  static constexpr int THREADS = (FEW_WARPS + !SELF) * 32;
   static constexpr int KT = FP8 ? 128 : 64;               // keys of a stage
   static constexpr int HALVES = FP8 ? 1 : 2;              // boxes of 128 bytes per row
   static constexpr int DATA = KT * 2 * 128 * HALVES;      // keys and values of a stage
@@ -224,10 +228,10 @@ __device__ __forceinline__ bool last_part(unsigned long long* flags, int part, i
 
 // NR: groups of eight rows that a warp computes.  WR: sets of warps with other rows; the warps of a set take other keys.
 template <bool FP8, int NR, int WR>
-__global__ void __launch_bounds__(FEW_THREADS, Few<FP8, NR * WR == 1>::CTAS)
+__global__ void __launch_bounds__(Few<FP8, NR, WR>::THREADS, Few<FP8, NR, WR>::CTAS)
     paged_few_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_constant__ CUtensorMap tm_scale, const Plan p,
                      const FewArgs a) {
-  using F = Few<FP8, NR * WR == 1>;
+  using F = Few<FP8, NR, WR>;
   constexpr int KT = F::KT, WK = FEW_WARPS / WR, M = 8 * NR * WR;
   constexpr bool JOIN = M <= JOIN_ROWS;
   constexpr int BLOCKS = KT / 16 / WK, NB = BLOCKS < 2 ? BLOCKS : 2;     // blocks of 16 keys of a warp, and how many at a time
@@ -235,6 +239,7 @@ __global__ void __launch_bounds__(FEW_THREADS, Few<FP8, NR * WR == 1>::CTAS)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   float* s_scales = reinterpret_cast<float*>(smem + F::STAGES * F::DATA);   // [stage][page box][keys, values][box rows]
   __shared__ uint64_t full[F::STAGES], empty[F::STAGES];
+  __shared__ int s_done[F::STAGES];                              // SELF: warps that are done with a stage, all its tiles so far
   __shared__ int abort_word, s_poison, s_vote;
   __shared__ float s_m[FEW_WARPS][8 * NR], s_l[FEW_WARPS][8 * NR];
   __shared__ float s_rs[M];                                      // a row's score scale, log2 units
@@ -244,14 +249,13 @@ __global__ void __launch_bounds__(FEW_THREADS, Few<FP8, NR * WR == 1>::CTAS)
   static_assert(FEW_WARPS * 8 * NR * FEW_LD * 4 + M * (HEAD * 4 + 8) <= F::SMEM - 1024, "results fit the ring");
   volatile int* abort_flag = &abort_word;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (threadIdx.x == 128) {
+  if (threadIdx.x == 0) {
     tma_prefetch_desc(&tm_kv);
     if (FP8) tma_prefetch_desc(&tm_scale);
-  }
-  if (threadIdx.x == 0) {
     for (int i = 0; i < F::STAGES; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], FEW_WARPS);
+      s_done[i] = 0;
     }
     abort_word = 0;
     s_poison = 0x7fffffff;
@@ -288,46 +292,48 @@ __global__ void __launch_bounds__(FEW_THREADS, Few<FP8, NR * WR == 1>::CTAS)
   const int bx_log = min(page_log, KT == 128 ? 7 : 6), bx = 1 << bx_log;      // rows of a box
   const int box_bytes = 2 * 128 << bx_log;
 
-  if (warp == FEW_WARPS) {
-    // a lane per box of the stage; its page is read a stage ahead
-    const int boxes = KT >> bx_log;
-    const int* table = p.table + (long long)b * p.width;
-    auto page_of = [&](int j) -> int {
-      const int k = j * KT + (lane << bx_log);
-      return j < j1 && lane < boxes && k < max_lim ? table[k >> page_log] : 0;
-    };
-    int next = page_of(j0);
-    bool ok = true;
+  // a lane per box of the stage
+  const int boxes = KT >> bx_log;
+  const int* table = p.table + (long long)b * p.width;
+  auto page_of = [&](int j) -> int {
+    const int k = j * KT + (lane << bx_log);
+    return j < j1 && lane < boxes && k < max_lim ? table[k >> page_log] : 0;
+  };
+  auto ask = [&](int j, int s, int pg) {               // (a whole warp)
+    const int live = min(boxes, (max_lim - j * KT + bx - 1) >> bx_log);
+    if (lane == 0) mbar_expect_tx(&full[s], live * (box_bytes * F::HALVES + (FP8 ? bx * 8 : 0)));
+    __syncwarp();
+    if (lane < live) {
+      if (pg < 0 || pg >= a.pages) report_status(a.status, kBadPage, 10);     // reads as zeros
+      const int y = (j * KT + (lane << bx_log)) & (p.page - 1);
+#pragma unroll
+      for (int h = 0; h < F::HALVES; ++h)
+        tma_load_5d(smem_u32(smem + s * F::DATA + (lane * F::HALVES + h) * box_bytes), &tm_kv, &full[s], h * 64, y, head, 0, pg);
+      if (FP8) tma_load_4d(s_scales + (s * KT + (lane << bx_log)) * 2, &tm_scale, &full[s], y, head, 0, pg);
+    }
+    __syncwarp();
+  };
+  if (!F::SELF && warp == FEW_WARPS) {
+    int next = page_of(j0);                              // read a stage ahead
     for (int j = j0; j < j1; ++j) {
       const int n = j - j0, s = n % F::STAGES;
       const int pg = next;
       next = page_of(j + 1);
-      ok = mbar_wait_warp(&empty[s], ((n / F::STAGES) & 1) ^ 1, abort_flag, a.status, 10);
-      if (!ok) break;
-      const int live = min(boxes, (max_lim - j * KT + bx - 1) >> bx_log);
-      if (lane == 0) mbar_expect_tx(&full[s], live * (box_bytes * F::HALVES + (FP8 ? bx * 8 : 0)));
-      __syncwarp();
-      if (lane < live) {
-        if (pg < 0 || pg >= a.pages) report_status(a.status, kBadPage, 10);     // reads as zeros
-        const int y = (j * KT + (lane << bx_log)) & (p.page - 1);
-#pragma unroll
-        for (int h = 0; h < F::HALVES; ++h)
-          tma_load_5d(smem_u32(smem + s * F::DATA + (lane * F::HALVES + h) * box_bytes), &tm_kv, &full[s], h * 64, y, head, 0, pg);
-        if (FP8) tma_load_4d(s_scales + (s * KT + (lane << bx_log)) * 2, &tm_scale, &full[s], y, head, 0, pg);
-      }
-      __syncwarp();
-    }
-    if (!ok) {                             // copies may be on their way into this CTA's memory
-      const uint64_t t0 = globaltimer_ns();
-      while (globaltimer_ns() - t0 < 2000000ull) {
-      }
+      if (!mbar_wait_warp(&empty[s], ((n / F::STAGES) & 1) ^ 1, abort_flag, a.status, 10)) break;
+      ask(j, s, pg);
     }
   } else {
+    int first[F::STAGES], next = 0;
+    if (F::SELF) {
+#pragma unroll
+      for (int s = 0; s < F::STAGES; ++s) first[s] = warp == 0 ? page_of(j0 + s) : 0;
+      next = page_of(j0 + F::STAGES);                    // of the tile that goes where this one is
+    }
     const int wr = warp / WK, wk = warp % WK;
     const int g = lane >> 2, c = lane & 3;
     // Query fragments of eight rows: values 2 c + {0, 1} and 2 c + 8 + {0, 1} of every 16, or for e4m3 4 c + {0 .. 3}: there a
     // thread's four codes of 16 stand side by side.  Rows behind the last are zeros.
-    auto load_q = [&](int rg, uint32_t (&f)[8][2]) {
+    auto fetch_q = [&](int rg, uint32_t (&f)[8][2]) {
       const int row = rg * 8 + g;
       const bool on = row < rows;
       const __nv_bfloat16* qp = a.q + (long long)(q0 + (row0 + row) / G) * a.ldq + (long long)(head * G + (row0 + row) % G) * HEAD;
@@ -345,6 +351,8 @@ __global__ void __launch_bounds__(FEW_THREADS, Few<FP8, NR * WR == 1>::CTAS)
           }
         }
       }
+    };
+    auto widen_q = [&](int rg, uint32_t (&f)[8][2]) {
       float rs = a.scale_log2;
       if (FP8) {
         uint32_t top = 0;
@@ -364,11 +372,18 @@ __global__ void __launch_bounds__(FEW_THREADS, Few<FP8, NR * WR == 1>::CTAS)
           for (int i = 0; i < 2; ++i)
             f[k][i] = pack_f16x2(__uint_as_float(f[k][i] << 16) * f2, __uint_as_float(f[k][i] & 0xffff0000u) * f2);
       }
-      if (c == 0) s_rs[row] = rs;
+      if (c == 0) s_rs[rg * 8 + g] = rs;
     };
     uint32_t qf[NR][8][2];
 #pragma unroll
-    for (int i = 0; i < NR; ++i) load_q(wr * NR + i, qf[i]);
+    for (int i = 0; i < NR; ++i) fetch_q(wr * NR + i, qf[i]);
+    if (F::SELF && warp == 0) {
+#pragma unroll
+      for (int s = 0; s < F::STAGES; ++s)
+        if (j0 + s < j1) ask(j0 + s, s, first[s]);
+    }
+#pragma unroll
+    for (int i = 0; i < NR; ++i) widen_q(wr * NR + i, qf[i]);
     named_bar_sync(1, FEW_WARPS * 32);
     // this thread's rows of a group of eight: 2 c and 2 c + 1
     float rs[NR][2];
@@ -401,6 +416,8 @@ __global__ void __launch_bounds__(FEW_THREADS, Few<FP8, NR * WR == 1>::CTAS)
     const int krow = (lane & 7) + ((lane >> 3) & 1) * 8, vrow = (lane & 7) + (lane >> 4) * 8;
     for (int j = j0; j < j1; ++j) {
       const int n = j - j0, s = n % F::STAGES, k0 = j * KT;
+      const int pg = next;
+      if (F::SELF) next = page_of(j + 1 + F::STAGES);
       ok &= mbar_wait(&full[s], (n / F::STAGES) & 1, abort_flag, a.status, 10);
       const uint32_t data = smem_u32(smem + s * F::DATA);
       const bool partial = k0 + KT > min_lim;
@@ -596,7 +613,15 @@ __global__ void __launch_bounds__(FEW_THREADS, Few<FP8, NR * WR == 1>::CTAS)
         }
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&empty[s]);
+      if (!F::SELF) {
+        if (lane == 0) mbar_arrive(&empty[s]);
+      } else if (j + F::STAGES < j1) {
+        int before = 0;
+        if (lane == 0)
+          asm volatile("atom.acq_rel.cta.shared::cta.add.s32 %0, [%1], 1;" : "=r"(before) : "r"(smem_u32(&s_done[s])) : "memory");
+        before = __shfl_sync(0xffffffffu, before, 0);
+        if (before % FEW_WARPS == FEW_WARPS - 1) ask(j + F::STAGES, s, pg);
+      }
     }
     ok = __all_sync(0xffffffffu, ok);
     // Warps of the same rows meet in the ring: every stage has been read (the barrier), and TMA asks for nothing more.
@@ -680,6 +705,11 @@ __global__ void __launch_bounds__(FEW_THREADS, Few<FP8, NR * WR == 1>::CTAS)
       }
     }
   }
+  if (*abort_flag) {                       // copies may be on their way into this CTA's memory
+    const uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 2000000ull) {
+    }
+  }
   if (a.cluster > 1) {
     __syncwarp();
     cluster_sync_all();
@@ -732,7 +762,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) paged_join_kernel(const Plan p, 
 template <bool FP8, int NR, int WR>
 static int launch_few(const Cache& c, const Plan& p, const FewArgs& a, cudaStream_t st) {
   auto kernel = paged_few_kernel<FP8, NR, WR>;
-  constexpr int SMEM = Few<FP8, NR * WR == 1>::SMEM;
+  constexpr int SMEM = Few<FP8, NR, WR>::SMEM;
   int dev = 0;
   SNU1_CUDA_CHECK(cudaGetDevice(&dev));
   static std::once_flag once[64];
@@ -751,7 +781,7 @@ static int launch_few(const Cache& c, const Plan& p, const FewArgs& a, cudaStrea
   attr[1].val.clusterDim.y = 1;
   attr[1].val.clusterDim.z = 1;
   cfg.gridDim = dim3(p.few_count, c.heads);
-  cfg.blockDim = dim3(FEW_THREADS);
+  cfg.blockDim = dim3(Few<FP8, NR, WR>::THREADS);
   cfg.dynamicSmemBytes = SMEM;
   cfg.stream = st;
   cfg.attrs = attr;
@@ -765,6 +795,7 @@ static int launch_few(const Cache& c, const Plan& p, const FewArgs& a, cudaStrea
   switch (p.few_rows) {
     case 8: return launch_few<FP8, 1, 1>(c, p, a, st);
     case 16: return launch_few<FP8, 2, 1>(c, p, a, st);
+    case 24: return launch_few<FP8, 3, 1>(c, p, a, st);
     case 32: return launch_few<FP8, 2, 2>(c, p, a, st);
     default: set_last_error("paged_attention: no kernel for %d rows", p.few_rows); return kHostBadArg;
   }

@@ -39,6 +39,10 @@ E4M3 = torch.float8_e4m3fn
 KEY_TILE = 64            # keys of a stage of the kernel for few rows
 FEW_SLOTS = (444, 296)   # its CTAs that run at once: of up to eight rows three on each of 148 SMs, otherwise two
 FEW_LEAST = 4            # a part of a sequence has at least this many key tiles
+# 17 to 24 rows have a kernel of their own (else that for 32): e4m3 always, bf16 from so many key tiles per CTA on.  Us, 20 rows,
+# 32 / 8 heads, the former / the latter: e4m3 1 x 1000 keys 12.0 / 12.6, 8 x 12000 61 / 85; bf16 1 x 1000 12.7 / 11.3, 8 x 1000 16.0 / 15.0,
+# 8 x 12000 67.6 / 71.1, 24 x 4000 80 / 89.
+FEW_24 = 16
 FEW_JOIN = 8             # up to so many rows the parts of few rows join themselves (JOIN_ROWS in attn_paged.cu)
 FEW_CLUSTER = 8          # up to so many parts are a cluster, if all sequences can have as many
 FEW_TILE = 32            # rows (new tokens x query heads of a group) of one CTA, at most
@@ -234,6 +238,8 @@ def _lay_out(q_lens, kv_lens, tables, page: int, pages: int, group: int, kv_head
     few_q = np.where(chunked, 0, q_rows)
     top = int(few_q.max()) if n else 0
     few_rows = 8 if top <= 8 else 16 if top <= 16 else FEW_TILE
+    if 16 < top <= 24 and (fp8 or int((-(-cap[few_q > 0] // KEY_TILE)).sum()) * kv_heads >= FEW_24 * FEW_SLOTS[1]):
+        few_rows = 24
     tile_rows = (CHUNK_TILE // group) * group if group <= CHUNK_TILE else 1      # a row tile is made of whole tokens
     single = chunked & fp8 & (q_rows <= ONE_MOST)              # widened by the CTAs that read it
 

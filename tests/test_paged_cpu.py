@@ -160,3 +160,11 @@ def test_the_plan_has_the_fields_of_the_kernels():
 def test_page_numbers_that_are_none(tables):
     with pytest.raises(ValueError):
         paged._lay_out([1, 3], [5, 40], tables, 16, 4, 4, 2, False, None, 0)
+
+
+def test_rows_of_a_tile():
+    rows = lambda n, fp8, keys=100: paged._lay_out([n], [keys], [range(-(-keys // 64))], 64, 2000, 1, 8, fp8, None, 0)[1]["few_rows"]
+    for fp8 in (False, True):
+        assert [rows(n, fp8) for n in (1, 8, 9, 16, 25, 32)] == [8, 8, 16, 16, 32, 32]
+    assert [rows(n, True) for n in (17, 24)] == [24, 24]
+    assert [rows(n, False) for n in (17, 24)] == [32, 32] and [rows(n, False, 40000) for n in (16, 17, 24, 25)] == [16, 24, 24, 32]

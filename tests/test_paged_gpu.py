@@ -265,6 +265,12 @@ def test_one_long_sequence_in_many_parts(q_len):
 
 
 @pytest.mark.parametrize("dtype", [BF16, E4M3])
+@pytest.mark.parametrize("q_lens", [[5], [6], [5, 1, 0, 6]])
+def test_seventeen_to_twenty_four_rows(q_lens, dtype):
+    attend(q_lens, [38100 - 9300 * i for i in range(len(q_lens))], 32, 8, 64, dtype, seed=4)
+
+
+@pytest.mark.parametrize("dtype", [BF16, E4M3])
 @pytest.mark.parametrize("q_lens,kv_lens", [([1, 1], [50, 64]), ([5], [70]), ([100, 1], [300, 10])])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
 def test_what_no_row_may_read_does_not_matter(q_lens, kv_lens, bad, dtype):
