@@ -398,6 +398,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
             ok &= mbar_wait(&v_full[(j + 1) % CV_STAGES], ((j + 1) / CV_STAGES) & 1, abort_flag, args.status, 3);
           }
         }
+        ok = __all_sync(0xffffffffu, ok);       // (nothing here depends on it; the warp goes on as one)
       }
     } else if (!FP16) {
       // ------------------------------ cleaning --------------------------------

@@ -156,6 +156,7 @@ class PagedPlan:
         # what an output and the scratch are like (half the host time of naming shape, type and device)
         like = self._store.view(torch.bfloat16)[:1]
         self._out, self._scratch = like.expand(self.rows, self.heads, HEAD_DIM), like.expand(self.scratch // 2)
+        self._read = like.expand(self.keys, self.kv_heads, HEAD_DIM)
         self._key = (self.dtype, self.page, self.kv_heads, self._index)
         self._addr = ctypes.addressof(self._args)
 
@@ -424,8 +425,7 @@ def paged_read(cache: PagedCache, plan: PagedPlan) -> tuple[torch.Tensor, torch.
     """The cached keys and values of the plan's sequences, one sequence after another: two tensors [plan.keys, kv_heads, 128] bf16
     (e4m3: code times scale, rounded once)."""
     _check(cache, plan)
-    k = torch.empty(plan.keys, cache.kv_heads, HEAD_DIM, dtype=_BF16, device=plan.device)
-    v = torch.empty_like(k)
+    k, v = torch.empty_like(plan._read), torch.empty_like(plan._read)
     if plan.keys:
         _call(plan._index, "paged_read", cache._addr, plan._addr, k.data_ptr(), v.data_ptr())
     return k, v
