@@ -10,7 +10,8 @@
 // eight, and all CTAs still run at once, the parts of a sequence are a cluster and meet in distributed shared memory: a
 // small batch, where latency counts.  Otherwise they meet in scratch, see last_part and paged_join_kernel.
 //
-// Pages come whole through TMA (keys and values of one head in one box), several stages ahead.  Four warps compute with mma.sync m16n8k16, keys (then the width of a head) on the 16-side and rows on the 8-side: S^T = K q^T,
+// Pages come whole through TMA (keys and values of one head in one box), several stages ahead.  Four warps compute with
+// mma.sync m16n8k16, keys (then the width of a head) on the 16-side and rows on the 8-side: S^T = K q^T,
 // o^T = V^T p^T.  So a step of a group of 4 or 8 heads fills the product, and what a warp has read and widened of the cache
 // serves all rows.  At 1 - 2 products per KB of cache the legacy tensor path is far from its limit.
 //
@@ -28,6 +29,11 @@
 // matrix product, so in a tile that some row may not read whole, bf16 values that are not finite are cleared too and the
 // first key that held one is kept: rows that may read it give NaN, the others are as if it were not there.  (e4m3 codes are
 // finite; what is not finite there is the row's scale, and that is only used where the mask allows.)
+//
+// Measured (32 / 8 heads unless said, of a measured copy bandwidth of 6456 GB/s): e4m3, 48 x 1 token over 32700 keys, 4 heads, 152 us,
+// 5.9 TB/s or 0.91; 24 x 1 over up to 4096 keys 23 us, 0.65, of which 6 are a launch's start and end and the join; one
+// conversation of 840 bf16 keys 7 us in a graph, 8.5 called one by one, latency alone.  8 x 5 tokens over up to 12000 bf16 keys 44 us,
+// 0.73.  From 16 rows on instructions count: e4m3 8 x 12000 keys 4 / 16 / 24 / 32 rows 37 / 47 / 61 / 86 us.
 #include <math.h>
 #include <string.h>
 

@@ -17,8 +17,15 @@
 // * A work item is a part of the key tiles of two row tiles; unnormalised results of parts are joined by
 //   paged_merge_kernel.  ops/paged.py chooses the parts so that the waves of CTAs are full.
 // * Two warps that have nothing else to do clear values that are not finite (and rows behind the last token) in the bf16 tiles
-//   that some row may not read whole (widening does so for e4m3): a probability of zero does not hide them from the product.  Rows that may read such a
-//   value give NaN, the others are as if it were not there.
+//   that some row may not read whole (widening does so for e4m3): a probability of zero does not hide them from the product.
+//   Rows that may read such a value give NaN, the others are as if it were not there.
+//
+// Measured (32 / 8 heads): bf16, 2 x 512 new tokens over 8300 keys 127 us in a graph, 1.06 PFLOP/s, 148 when called for a second on end
+// (the power limit takes the clocks down); a pair of tiles takes 1.78 us, 0.82 of the tensor cores' measured rate if all SMs were at
+// it (128 CTAs on 148 SMs), and a CTA 8 to 10 us to start and end.  e4m3, 4096 tokens at the end of 32001: 1.72 ms, 1.17 PFLOP/s, or 2.03 in
+// a loop.  Chunks of up to 256 rows over e4m3: 3500 clocks per tile of 128 rows, in which the softmax warps and those that widen
+// are busy nearly all the time (clock stamps; 2400 and 2500).  Taking the scales' part from the widening warps, or all of it apart
+// for keys and values, or letting softmax warps without rows rest, changed nothing or made it 3 to 10 % slower.
 #include <cuda_fp16.h>
 #include <string.h>
 

@@ -8,7 +8,9 @@
 //
 // Both directions are bound by memory: 16 lanes own a row (16 bytes of bf16, 8 codes each), four rows are in flight per
 // lane.  Where a token or a page lives takes three dependent loads, so a block looks that up once for many rows: up to 16
-// tokens of all heads when writing, 256 rows of a page when reading.
+// tokens of all heads when writing, 256 rows of a page when reading.  Measured, e4m3: 32001 tokens of 8 heads written in 38 us, 5.2 TB/s
+// or 0.80 of what a long copy reaches; 32001 of 4 heads read back in 20 us, 4.9 TB/s.  A plain copy of as many bytes takes as long:
+// 100 MB read and written 38 us, 53 MB 22 to 25.
 #include <cuda_fp8.h>
 #include <string.h>
 

@@ -16,7 +16,7 @@ pages.  The plan is made once per step on the host and serves every layer::
 
 A sequence may bring one token (a decode step), a few (drafted tokens) or thousands (a chunk of its prompt), all in one plan.
 For a captured decode loop, ``build_plan(..., grow=n)`` leaves room for ``n`` further tokens and :meth:`PagedPlan.advance` inside
-the graph moves every sequence on by one.
+the graph moves every sequence on by one.  A graph reads the plan's arrays whenever it is replayed: keep the plan as long as the graph.
 
 A call runs on the current stream of the tensors' device.  A plan's device arrays belong to the streams that are ordered after
 the one it was built on; calls that only read (write into different caches, attention, reading back) may share it.
