@@ -347,8 +347,11 @@ class InferenceEngine:
         if (ids is None) == (embeds is None):
             raise ValueError("paged_step takes ids or embeds")
         x = self.p["embed_tokens"].index_select(0, ids.to(self.dev).long()) if embeds is None else embeds.contiguous()
-        if x.shape[0] != plan.rows:
-            raise ValueError(f"the plan has {plan.rows} new tokens, not {x.shape[0]}")
+        if x.shape != (plan.rows, self.cfg.hidden_size) or x.dtype != torch.bfloat16 or x.device != self.p["embed_tokens"].device:
+            raise ValueError(f"the plan has {plan.rows} new tokens: ids [{plan.rows}], or bf16 embeds [{plan.rows}, {self.cfg.hidden_size}] "
+                             f"on the engine's device, not {tuple(x.shape)} {x.dtype}")
+        if pos3 is not None and pos3.shape != (3, plan.rows):
+            raise ValueError(f"pos3 is [3, {plan.rows}], not {tuple(pos3.shape)}")
         if plan.rows == 0:
             return x
         if pos3 is None:

@@ -751,3 +751,11 @@ def test_engine_refusals():
     assert eng.paged_step(plan, caches, ids=ids).shape == (3, cfg.hidden_size)
     empty = paged.build_plan(caches[0], cfg.num_heads, [0], [3], [[1]])
     assert eng.paged_step(empty, caches, ids=ids[:0]).shape == (0, cfg.hidden_size)
+    x = torch.zeros(3, cfg.hidden_size, device="cuda", dtype=BF16)
+    assert eng.paged_step(plan, caches, embeds=x).shape == x.shape
+    for bad in (x.float(), x[:, :-8], x[:2], x.cpu()):
+        with pytest.raises(ValueError):
+            eng.paged_step(plan, caches, embeds=bad)
+    for bad in (torch.zeros(3, 2), torch.zeros(2, 3), torch.zeros(3)):
+        with pytest.raises(ValueError):
+            eng.paged_step(plan, caches, ids=ids, pos3=bad.int())
