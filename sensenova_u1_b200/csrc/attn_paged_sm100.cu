@@ -453,8 +453,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
     if (RAW && warp >= 12) {
       // ------------------------------ widening --------------------------------
-      // A thread has half a row: code times scale as fp16, the tile times a power of two that brings its largest value to 2^12
-      // to 2^13.  A scale is two fp16 numbers then, and a pair of codes three instructions instead of five.  Rows that nobody
+      // A thread has half a row: code times scale as fp16, scaled like the tiles of paged_widen_kernel.  A scale is two fp16 numbers then, and a pair of codes three instructions instead of five.  Rows that nobody
       // reads and values that are not finite are cleared.
       const int tid = threadIdx.x - 384, row = tid & 127, half = tid >> 7;
       const int page = args.page, page_log = __ffs(page) - 1;
@@ -465,7 +464,6 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         const int k0 = (j0 + j) * BK;
         float factor[2];
         float2 told;
-        constexpr int UP = 13;
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv) {
           const int u = 2 * j + kv, s = u % RAW_STAGES;
@@ -481,11 +479,11 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
                 if (k0 + lane + 32 * i < most && x < INFINITY) top = max(top, __float_as_uint(x));
               }
               top = __reduce_max_sync(0xffffffffu, top);
-              const int ex = tile_exponent(__uint_as_float(top));
+              const int ex = tile_exponent(__uint_as_float(top)) - WIDEN_UP;
               const float x = k0 + row < most ? scale_at(sc, row, w) : 0.f;
-              factor[w] = x * __int_as_float((127 - ex + UP) << 23);
-              if (w == 0) told.x = __int_as_float((127 + ex - UP) << 23);
-              else told.y = (float)(ex - UP);
+              factor[w] = x * __int_as_float((127 - ex) << 23);
+              if (w == 0) told.x = __int_as_float((127 + ex) << 23);
+              else told.y = (float)ex;
             }
             if (!(fabsf(factor[1]) < INFINITY)) {
               if (half == 0) atomicMin(poison, k0 + row);

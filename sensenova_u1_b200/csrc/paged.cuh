@@ -53,7 +53,9 @@ struct Plan {
   int layout;              // PLAN_LAYOUT; changes with the fields
 };
 
-// The power of two that a tile whose largest scale is ``top`` is divided by: its values are at most 1 then (codes are up to 448).
+// A tile whose largest scale is ``top`` is divided by a power of two for fp16: 2^tile_exponent would make its values at most 1 (codes are
+// up to 448), and they are taken 2^WIDEN_UP times larger, up to 2^15 if the exponent is at its upper limit.
+constexpr int WIDEN_UP = 13;
 __device__ __forceinline__ int tile_exponent(float top) {
   return max(-90, min(126, (int)(__float_as_uint(E4M3_MAX * top) >> 23) - 126));
 }
