@@ -23,9 +23,11 @@
 // Measured (32 / 8 heads): bf16, 2 x 512 new tokens over 8300 keys 127 us in a graph, 1.06 PFLOP/s, 148 when called for a second on end
 // (the power limit takes the clocks down); a pair of tiles takes 1.78 us, 0.82 of the tensor cores' measured rate if all SMs were at
 // it (128 CTAs on 148 SMs), and a CTA 8 to 10 us to start and end.  e4m3, 4096 tokens at the end of 32001: 1.72 ms, 1.17 PFLOP/s, or 2.03 in
-// a loop.  Chunks of up to 256 rows over e4m3: 3500 clocks per tile of 128 rows, in which the softmax warps and those that widen
-// are busy nearly all the time (clock stamps; 2400 and 2500).  Taking the scales' part from the widening warps, or all of it apart
-// for keys and values, or letting softmax warps without rows rest, changed nothing or made it 3 to 10 % slower.
+// a loop.  Chunks of up to 256 rows over e4m3, 8 x 64 rows over 12000 keys: 86 us, 2.4 TB/s, 3100 clocks per tile of 128 rows.  Four warps
+// widen keys, four values, and two turn scales into factors two tiles ahead; with eight warps doing all three one after the
+// other it was 97.  Without the multiplications 80, without the exponentials 76, without both 71: what bounds it is each warp's own
+// chain.  Softmax warps without rows that only keep step made it 87, two places for P (so that its store need not wait for the
+// product before) 95.
 #include <cuda_fp16.h>
 #include <string.h>
 
@@ -42,7 +44,7 @@ constexpr int CHALF = 128 * 64 * 2;             // 64 columns of a 128-row tile
 constexpr int CTILE = 2 * CHALF;
 constexpr int CHUNK_THREADS = 640;
 constexpr int RAW_UNIT = 128 * 128;             // codes of a tile's keys, or of its values
-constexpr int RAW_STAGES = 3, SCALE_STAGES = 4;
+constexpr int RAW_STAGES = 3, SCALE_STAGES = 4;    // of units; of tiles
 
 // What a CTA reads: bf16 pages, e4m3 pages that have been widened to fp16, or e4m3 pages as they are.
 enum ChunkMode { kPages, kWide, kRaw };
@@ -51,7 +53,7 @@ struct Chunk {
   static constexpr bool FP16 = MODE != kPages, RAW = MODE == kRaw;
   static constexpr int TILES = RAW ? 1 : 2;     // row tiles
   static constexpr int K_STAGES = RAW ? 2 : 3, V_STAGES = 2;
-  static constexpr int RING = RAW ? RAW_STAGES * RAW_UNIT + SCALE_STAGES * 1024 : 0;
+  static constexpr int RING = RAW ? RAW_STAGES * RAW_UNIT + SCALE_STAGES * 2048 : 0;
   static constexpr int SMEM = (TILES + K_STAGES + V_STAGES) * CTILE + RING + 512 + 1024;
 };
 
@@ -121,16 +123,18 @@ __device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint32_t b, uint
       : "memory");
 }
 
-// The two codes in the low half of ``w`` times hi + lo, as fp16: the product with hi has 15 bits and is rounded once, together with
-// the product with lo.
-__device__ __forceinline__ uint32_t widen_scaled(uint32_t w, uint32_t hi, uint32_t lo) {
-  uint32_t r;
-  asm("{\n.reg .b16 l, u;\n.reg .b32 h, t;\nmov.b32 {l, u}, %1;\ncvt.rn.f16x2.e4m3x2 h, l;\n"
-      "mul.rn.f16x2 t, h, %3;\nfma.rn.f16x2 %0, h, %2, t;\n}"
-      : "=r"(r)
+// Two of the four codes in ``w`` (the lower, then the upper half) times hi + lo, as fp16: the product with hi has 15 bits and is
+// rounded once, together with the product with lo.
+__device__ __forceinline__ uint2 widen_scaled(uint32_t w, uint32_t hi, uint32_t lo) {
+  uint2 r;
+  asm("{\n.reg .b16 l, u;\n.reg .b32 h, t;\nmov.b32 {l, u}, %2;\n"
+      "cvt.rn.f16x2.e4m3x2 h, l;\nmul.rn.f16x2 t, h, %4;\nfma.rn.f16x2 %0, h, %3, t;\n"
+      "cvt.rn.f16x2.e4m3x2 h, u;\nmul.rn.f16x2 t, h, %4;\nfma.rn.f16x2 %1, h, %3, t;\n}"
+      : "=r"(r.x), "=r"(r.y)
       : "r"(w), "r"(hi), "r"(lo));
   return r;
 }
+constexpr uint32_t CLEAR_ROW = 0x80000000u;     // a row's factor: + 0 and - 0, which no scale gives
 
 template <int MODE>
 __global__ void __launch_bounds__(CHUNK_THREADS, 1)
@@ -146,6 +150,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
   uint8_t* sV = sK + CK_STAGES * CTILE;
   uint8_t* s_raw = sV + CV_STAGES * CTILE;                 // [RAW_STAGES] codes of keys and of values in turn
   float* s_scale = reinterpret_cast<float*>(s_raw + RAW_STAGES * RAW_UNIT);     // [SCALE_STAGES][page][keys, values][token]
+  uint32_t* s_mult = reinterpret_cast<uint32_t*>(s_scale + SCALE_STAGES * 256);  // [SCALE_STAGES][keys, values][token]: two fp16 numbers
   uint64_t* bars = reinterpret_cast<uint64_t*>(s_raw + C::RING);
   uint64_t* q_full = bars;
   uint64_t* k_full = bars + 1;
@@ -159,10 +164,14 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
   uint64_t* p_full = s_empty + 2;
   uint64_t* pv_done = p_full + 2;
   uint64_t* q_ready = pv_done + 2;              // e4m3: the queries are fp16
-  uint64_t* raw_full = q_ready + 1;             // [RAW_STAGES]
-  uint64_t* raw_empty = raw_full + RAW_STAGES;
-  float2* s_factor = reinterpret_cast<float2*>(raw_empty + RAW_STAGES);         // [4] of tiles: see ChunkArgs::factors
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_factor + 4);
+  // (units of keys and of values go through one ring, but each has barriers of its own: who waits for every other phase of a
+  // barrier cannot tell it from the one before)
+  uint64_t* raw_full = q_ready + 1;             // [2 RAW_STAGES] by unit
+  uint64_t* raw_empty = raw_full + 2 * RAW_STAGES;
+  uint64_t* scale_full = raw_empty + 2 * RAW_STAGES;      // [SCALE_STAGES] by tile: s_scale
+  uint64_t* mult_full = scale_full + SCALE_STAGES;        // [SCALE_STAGES] by tile: s_mult and s_factor
+  float2* s_factor = reinterpret_cast<float2*>(mult_full + SCALE_STAGES);        // [2 SCALE_STAGES] of tiles: see ChunkArgs::factors
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_factor + 2 * SCALE_STAGES);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* drained = reinterpret_cast<int*>(tmem_slot + 2);   // [2] softmax warps that have read a score tile, all tiles so far
   int* lim_max = drained + 2;                              // [2] the largest and the smallest limit of a row tile
@@ -173,15 +182,19 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
     for (int i = 0; i < CK_STAGES; ++i) {
-      mbar_init(&k_full[i], RAW ? 8 : 1);
+      mbar_init(&k_full[i], RAW ? 4 : 1);
       mbar_init(&k_empty[i], 1);
     }
-    for (int i = 0; i < RAW_STAGES; ++i) {
+    for (int i = 0; i < 2 * RAW_STAGES; ++i) {
       mbar_init(&raw_full[i], 1);
-      mbar_init(&raw_empty[i], 8);
+      mbar_init(&raw_empty[i], 4);
+    }
+    for (int i = 0; i < SCALE_STAGES; ++i) {
+      mbar_init(&scale_full[i], 1);
+      mbar_init(&mult_full[i], 2);
     }
     for (int i = 0; i < CV_STAGES; ++i) {
-      mbar_init(&v_full[i], RAW ? 8 : 1);
+      mbar_init(&v_full[i], RAW ? 4 : 1);
       mbar_init(&v_empty[i], 1);
       mbar_init(&v_dirty[i], 1);
       mbar_init(&v_clean[i], 2);
@@ -290,24 +303,38 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
           if (ok) load(sK + s * CTILE, &tm_k, &k_full[s], j, pg);
         };
         if (RAW) {
-          // codes of keys, with the scales of keys and values, then codes of values, into one ring
+          // Codes of keys and codes of values in turn into one ring, and two tiles ahead the scales of both.
+          int far = page_of(2);
+          auto load_scales = [&](int j, int pg) {
+            if (j >= n) return;
+            const int live = min(per, used - (j0 + j) * per), s = j % SCALE_STAGES;
+            if (lane == 0) mbar_expect_tx(&scale_full[s], live * page * 8);
+            __syncwarp();
+            if (lane < live) tma_load_4d(s_scale + s * 256 + lane * page * 2, &tm_v, &scale_full[s], 0, kvh, 0, pg);
+            __syncwarp();
+          };
+          load_scales(0, pk);
+          load_scales(1, ahead);
           for (int j = 0; j < n && ok; ++j) {
-            const int pg = pk, live = min(per, used - (j0 + j) * per);
+            const int pg = pk, two = far, live = min(per, used - (j0 + j) * per);
             pk = ahead;
-            ahead = page_of(j + 2);
+            ahead = far;
+            far = page_of(j + 3);
 #pragma unroll
             for (int kv = 0; kv < 2; ++kv) {
-              const int u = 2 * j + kv, s = u % RAW_STAGES;
-              ok = ok && mbar_wait_warp(&raw_empty[s], ((u / RAW_STAGES) & 1) ^ 1, abort_flag, args.status, 1);
+              const int u = 2 * j + kv, s = u % RAW_STAGES, w = u - RAW_STAGES;
+              if (w >= 0) ok = ok && mbar_wait_warp(&raw_empty[w % (2 * RAW_STAGES)], (w / (2 * RAW_STAGES)) & 1, abort_flag, args.status, 1);
               if (!ok) break;
-              if (lane == 0) mbar_expect_tx(&raw_full[s], live * page * (kv ? 128 : 128 + 8));
+              uint64_t* full = &raw_full[u % (2 * RAW_STAGES)];
+              if (lane == 0) mbar_expect_tx(full, live * page * 128);
               __syncwarp();
               if (lane < live) {
                 if (pg < 0 || pg >= args.pages) report_status(args.status, kBadPage, 10);     // reads as zeros
-                tma_load_5d(smem_u32(s_raw + s * RAW_UNIT + lane * page * 128), &tm_k, &raw_full[s], 0, 0, kvh, kv, pg);
-                if (kv == 0) tma_load_4d(s_scale + (j % SCALE_STAGES) * 256 + lane * page * 2, &tm_v, &raw_full[s], 0, kvh, 0, pg);
+                tma_load_5d(smem_u32(s_raw + s * RAW_UNIT + lane * page * 128), &tm_k, full, 0, 0, kvh, kv, pg);
               }
               __syncwarp();
+              // what was made of the scales four tiles before has been read: keys and values of that tile have left the ring
+              if (kv == 0) load_scales(j + 2, two);
             }
           }
         } else {
@@ -407,6 +434,48 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         }
         ok = __all_sync(0xffffffffu, ok);       // (nothing here depends on it; the warp goes on as one)
       }
+    } else if (RAW) {
+      // ------------------------------ scales --------------------------------
+      // A tile is scaled like those of paged_widen_kernel; a scale is two fp16 numbers then.  The exponents go to the softmax.  Rows that nobody reads and values that are not finite are to be cleared.
+      const int tid = threadIdx.x - 64, page = args.page, page_log = __ffs(page) - 1;
+      auto place = [&](int r, int kv) -> int { return (((r >> page_log) * 2 + kv) << page_log) + (r & (page - 1)); };
+      bool ok = true;
+      for (int j = 0; j < n && ok; ++j) {
+        const int k0 = (j0 + j) * BK, s = j % SCALE_STAGES;
+        ok = mbar_wait_warp(&scale_full[s], (j / SCALE_STAGES) & 1, abort_flag, args.status, 3);
+        const float* sc = s_scale + s * 256;
+        uint32_t* out = s_mult + s * 256;
+        int ex[2];
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+          const float4 x = *reinterpret_cast<const float4*>(sc + place(4 * lane, kv));       // four rows, which lie in one page
+          const float y[4] = {x.x, x.y, x.z, x.w};
+          uint32_t top = 0;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (k0 + 4 * lane + i < most && fabsf(y[i]) < INFINITY) top = max(top, __float_as_uint(fabsf(y[i])));
+          ex[kv] = tile_exponent(__uint_as_float(__reduce_max_sync(0xffffffffu, top))) - WIDEN_UP;
+          const float2 mine = *reinterpret_cast<const float2*>(sc + place(2 * tid, kv));
+          uint32_t w[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int key = k0 + 2 * tid + i;
+            const float f = (i ? mine.y : mine.x) * __int_as_float((127 - ex[kv]) << 23);
+            const __half hi = __float2half_rn(f), lo = __float2half_rn(f - __half2float(hi));
+            w[i] = (uint32_t)__half_as_ushort(hi) | (uint32_t)__half_as_ushort(lo) << 16;
+            if (key >= most) {
+              w[i] = CLEAR_ROW;
+            } else if (kv && !(fabsf(f) < INFINITY)) {
+              w[i] = CLEAR_ROW;
+              atomicMin(poison, key);
+            }
+          }
+          *reinterpret_cast<uint2*>(out + kv * 128 + 2 * tid) = make_uint2(w[0], w[1]);
+        }
+        if (tid == 0) s_factor[j % (2 * SCALE_STAGES)] = make_float2(__int_as_float((127 + ex[0]) << 23), (float)ex[1]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&mult_full[s]);
+      }
     } else if (!FP16) {
       // ------------------------------ cleaning --------------------------------
       bool ok = true;
@@ -453,74 +522,41 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
     if (RAW && warp >= 12) {
       // ------------------------------ widening --------------------------------
-      // A thread has half a row: code times scale as fp16, scaled like the tiles of paged_widen_kernel.  A scale is two fp16 numbers then, and a pair of codes three instructions instead of five.  Rows that nobody
-      // reads and values that are not finite are cleared.
-      const int tid = threadIdx.x - 384, row = tid & 127, half = tid >> 7;
-      const int page = args.page, page_log = __ffs(page) - 1;
-      auto scale_at = [&](const float* sc, int r, int kv) -> float { return sc[(((r >> page_log) * 2 + kv) << page_log) + (r & (page - 1))]; };
+      // Four warps widen keys, four values; a thread has a row: code times scale, three instructions per pair.
+      const int row = threadIdx.x & 127, kv = (warp - 12) >> 2, sw = (row & 7) << 4;
+      const int stages = kv ? CV_STAGES : CK_STAGES;
+      uint64_t *const free = kv ? v_empty : k_empty, *const done = kv ? v_full : k_full;
+      uint8_t* const tiles = (kv ? sV : sK) + row * 128;
       bool ok = true;
       for (int j = 0; j < n && ok; ++j) {
-        const float* sc = s_scale + (j % SCALE_STAGES) * 256;
-        const int k0 = (j0 + j) * BK;
-        float factor[2];
-        float2 told;
+        const int u = 2 * j + kv, w = u % (2 * RAW_STAGES), to = j % stages;
+        ok = mbar_wait_warp(&mult_full[j % SCALE_STAGES], (j / SCALE_STAGES) & 1, abort_flag, args.status, 3) &&
+             mbar_wait_warp(&raw_full[w], (u / (2 * RAW_STAGES)) & 1, abort_flag, args.status, 3);
+        if (!ok) break;
+        const uint32_t f = s_mult[(j % SCALE_STAGES) * 256 + kv * 128 + row];
+        const uint8_t* from = s_raw + u % RAW_STAGES * RAW_UNIT + row * 128;
+        uint4 x[8];
 #pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
-          const int u = 2 * j + kv, s = u % RAW_STAGES;
-          ok = ok && mbar_wait_warp(&raw_full[s], (u / RAW_STAGES) & 1, abort_flag, args.status, 3);
-          if (!ok) break;
-          if (kv == 0) {                   // both scales have come with the keys
+        for (int i = 0; i < 8; ++i) x[i] = *reinterpret_cast<const uint4*>(from + ((i << 4) ^ sw));
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&raw_empty[w]);
+        if (__any_sync(0xffffffffu, f == CLEAR_ROW)) {      // (their codes may be NaN)
 #pragma unroll
-            for (int w = 0; w < 2; ++w) {
-              uint32_t top = 0;
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const float x = fabsf(scale_at(sc, lane + 32 * i, w));
-                if (k0 + lane + 32 * i < most && x < INFINITY) top = max(top, __float_as_uint(x));
-              }
-              top = __reduce_max_sync(0xffffffffu, top);
-              const int ex = tile_exponent(__uint_as_float(top)) - WIDEN_UP;
-              const float x = k0 + row < most ? scale_at(sc, row, w) : 0.f;
-              factor[w] = x * __int_as_float((127 - ex) << 23);
-              if (w == 0) told.x = __int_as_float((127 + ex) << 23);
-              else told.y = (float)ex;
-            }
-            if (!(fabsf(factor[1]) < INFINITY)) {
-              if (half == 0) atomicMin(poison, k0 + row);
-              factor[1] = 0.f;
-            }
-            if (tid == 0) s_factor[j & 3] = told;
-          }
-          const uint8_t* from = s_raw + s * RAW_UNIT;
-          uint4 x[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const uint4*>(from + swz128_offset(row, half * 4 + i));
-          const int to = j % (kv ? CV_STAGES : CK_STAGES);
-          ok = mbar_wait_warp(kv ? &v_empty[to] : &k_empty[to], ((j / (kv ? CV_STAGES : CK_STAGES)) & 1) ^ 1, abort_flag, args.status, 3);
-          if (!ok) break;
-          uint8_t* dst = (kv ? sV : sK) + to * CTILE + half * CHALF;
-          const bool clear = k0 + row >= most || (kv && factor[1] == 0.f);
-          if (__any_sync(0xffffffffu, clear)) {      // (their codes may be NaN)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (clear) x[i] = make_uint4(0, 0, 0, 0);
-          }
-          const uint32_t hi = pack_f16x2(factor[kv], factor[kv]);
-          const float rest = clear ? 0.f : factor[kv] - __low2float(*reinterpret_cast<const __half2*>(&hi));
-          const uint32_t lo = pack_f16x2(rest, rest);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const uint32_t w0 = i & 1 ? x[i >> 1].z : x[i >> 1].x, w1 = i & 1 ? x[i >> 1].w : x[i >> 1].y;
-            *reinterpret_cast<uint4*>(dst + swz128_offset(row, i)) = make_uint4(
-                widen_scaled(w0, hi, lo), widen_scaled(w0 >> 16, hi, lo), widen_scaled(w1, hi, lo), widen_scaled(w1 >> 16, hi, lo));
-          }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            mbar_arrive(kv ? &v_full[to] : &k_full[to]);
-            mbar_arrive(&raw_empty[s]);
-          }
+          for (int i = 0; i < 8; ++i)
+            if (f == CLEAR_ROW) x[i] = make_uint4(0, 0, 0, 0);
         }
+        const uint32_t hi = __byte_perm(f, f, 0x1010), lo = __byte_perm(f, f, 0x3232);
+        ok = mbar_wait_warp(&free[to], ((j / stages) & 1) ^ 1, abort_flag, args.status, 3);
+        if (!ok) break;
+        uint8_t* dst = tiles + to * CTILE;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const uint2 y0 = widen_scaled(i & 1 ? x[i >> 1].z : x[i >> 1].x, hi, lo), y1 = widen_scaled(i & 1 ? x[i >> 1].w : x[i >> 1].y, hi, lo);
+          *reinterpret_cast<uint4*>(dst + (i >> 3) * CHALF + (((i & 7) << 4) ^ sw)) = make_uint4(y0.x, y0.y, y1.x, y1.y);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&done[to]);
       }
     } else {
     // ------------------------------ softmax --------------------------------
@@ -603,8 +639,8 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
       }
       ok &= mbar_wait(&s_full[t], j & 1, abort_flag, args.status, 5);
       tc_fence_after();
-      if (RAW) {                             // told before the keys were; the place is used again four tiles on
-        const float2 told = s_factor[j & 3];
+      if (RAW) {                             // told before the keys were; the place is used again eight tiles on
+        const float2 told = s_factor[j % (2 * SCALE_STAGES)];
         factor.x = told.x;
         factor.y = told.y;
       }

@@ -47,12 +47,13 @@ FEW_JOIN = 8             # up to so many rows the parts of few rows join themsel
 FEW_CLUSTER = 8          # up to so many parts are a cluster, if all sequences can have as many
 FEW_TILE = 32            # rows (new tokens x query heads of a group) of one CTA, at most
 # More rows of a sequence are a chunk.  Chunk kernel / few rows, us, 32 / 8 heads, sequences of 12000 keys: bf16 1 x 32 rows
-# 22 / 23, 8 x 32 76 / 66, 1 x 48 22 / 29, 8 x 48 82 / 107; e4m3 1 x 32 22 / 25, 8 x 32 93 / 86, 1 x 48 24 / 32, 8 x 48 95 / 139.
+# 22 / 25, 8 x 32 75 / 72, 1 x 48 22 / 29, 8 x 48 77 / 134; e4m3 1 x 32 22 / 25, 8 x 32 85 / 86, 24 x 32 of 4000 keys 114 / 109, 8 x 32 of
+# 1000 20 / 16, 1 x 48 22 / 33, 8 x 48 86 / 155.
 CHUNK_FROM = FEW_TILE
 CHUNK_TILE = 128         # keys of a tile of the kernel for chunks, and rows of a row tile
 # e4m3 chunks of up to so many rows are widened by the CTAs that read them, one row tile each; longer ones are widened once.
-# Us, the former / the latter: 8 sequences of 12000 keys, 128 rows 98 / 191, 256 178 / 210, 512 363 / 291; of 1000 keys 22 / 29, 23 / 33,
-# 44 / 35.
+# Us, the former / the latter: 8 sequences of 12000 keys, 128 rows 89 / 190, 256 154 / 209, 512 314 / 294; of 1000 keys 20 / 29, 22 / 32,
+# 41 / 34.
 ONE_MOST = 256
 CHUNK_SLOTS = 148        # its CTAs that run at once
 CHUNK_START = 5          # what starting and ending a CTA costs, in key tiles (1.8 us): 8 to 10 us from its start to its end
