@@ -123,17 +123,6 @@ __device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint32_t b, uint
       : "memory");
 }
 
-// Two of the four codes in ``w`` (the lower, then the upper half) times hi + lo, as fp16: the product with hi has 15 bits and is
-// rounded once, together with the product with lo.
-__device__ __forceinline__ uint2 widen_scaled(uint32_t w, uint32_t hi, uint32_t lo) {
-  uint2 r;
-  asm("{\n.reg .b16 l, u;\n.reg .b32 h, t;\nmov.b32 {l, u}, %2;\n"
-      "cvt.rn.f16x2.e4m3x2 h, l;\nmul.rn.f16x2 t, h, %4;\nfma.rn.f16x2 %0, h, %3, t;\n"
-      "cvt.rn.f16x2.e4m3x2 h, u;\nmul.rn.f16x2 t, h, %4;\nfma.rn.f16x2 %1, h, %3, t;\n}"
-      : "=r"(r.x), "=r"(r.y)
-      : "r"(w), "r"(hi), "r"(lo));
-  return r;
-}
 constexpr uint32_t CLEAR_ROW = 0x80000000u;     // a row's factor: + 0 and - 0, which no scale gives
 
 template <int MODE>
@@ -461,8 +450,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
           for (int i = 0; i < 2; ++i) {
             const int key = k0 + 2 * tid + i;
             const float f = (i ? mine.y : mine.x) * __int_as_float((127 - ex[kv]) << 23);
-            const __half hi = __float2half_rn(f), lo = __float2half_rn(f - __half2float(hi));
-            w[i] = (uint32_t)__half_as_ushort(hi) | (uint32_t)__half_as_ushort(lo) << 16;
+            w[i] = split_f16(f);
             if (key >= most) {
               w[i] = CLEAR_ROW;
             } else if (kv && !(fabsf(f) < INFINITY)) {

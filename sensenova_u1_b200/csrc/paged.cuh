@@ -6,6 +6,8 @@
 // so the rows of one head are contiguous inside a page, which is the unit that an attention CTA asks for (one TMA box for
 // keys and values together).  Sequences own pages through a table in any order; pages of 16 to 128 tokens.
 #pragma once
+#include <cuda_fp16.h>
+
 #include "attn_common.cuh"
 #include "host_common.h"
 
@@ -74,6 +76,23 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   return r;
 }
 
+// A factor as two fp16 numbers, hi + lo.
+__device__ __forceinline__ uint32_t split_f16(float f) {
+  const __half hi = __float2half_rn(f), lo = __float2half_rn(f - __half2float(hi));
+  return (uint32_t)__half_as_ushort(hi) | (uint32_t)__half_as_ushort(lo) << 16;
+}
+
+// The four codes in ``w`` times a factor as fp16, ``hi`` and ``lo`` twice each: the product with hi has 15 bits and is rounded once,
+// together with the product with lo.
+__device__ __forceinline__ uint2 widen_scaled(uint32_t w, uint32_t hi, uint32_t lo) {
+  uint2 r;
+  asm("{\n.reg .b16 l, u;\n.reg .b32 h, t;\nmov.b32 {l, u}, %2;\n"
+      "cvt.rn.f16x2.e4m3x2 h, l;\nmul.rn.f16x2 t, h, %4;\nfma.rn.f16x2 %0, h, %3, t;\n"
+      "cvt.rn.f16x2.e4m3x2 h, u;\nmul.rn.f16x2 t, h, %4;\nfma.rn.f16x2 %1, h, %3, t;\n}"
+      : "=r"(r.x), "=r"(r.y)
+      : "r"(w), "r"(hi), "r"(lo));
+  return r;
+}
 __device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
   uint32_t r;
   asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));

@@ -194,18 +194,18 @@ __global__ void __launch_bounds__(WIDEN_THREADS)
     paged_widen_kernel(const uint8_t* __restrict__ data, const float* __restrict__ scales, int pages, int heads, Plan p,
                        uint8_t* __restrict__ wide, float4* __restrict__ factors, int* status) {
   __shared__ long long s_at[128];          // the token's row of the cache, -1: none
-  __shared__ float s_scale[128];
+  __shared__ uint32_t s_mult[128];         // the row's factor, see split_f16
   __shared__ float s_top[4];
   __shared__ int s_bad[4];
+  const int2 e = p.unpack[blockIdx.x];     // set by the host
   pdl_wait();
   pdl_trigger();
-  const int2 e = p.unpack[blockIdx.x];
   const int kv = blockIdx.y >= heads, head = blockIdx.y - kv * heads, b = e.x, t = threadIdx.x;
   const int len = seq_len(p, b);
+  float s = 0.f;
   if (t < 128) {
     const int pos = e.y * 128 + t;
     long long at = -1;
-    float s = 0.f;
     if (pos < len) {
       const int pg = p.table[(long long)b * p.width + pos / p.page];
       if (pg >= 0 && pg < pages) {
@@ -218,8 +218,11 @@ __global__ void __launch_bounds__(WIDEN_THREADS)
     const bool finite = fabsf(s) < INFINITY;
     const uint32_t top = __reduce_max_sync(0xffffffffu, finite ? __float_as_uint(fabsf(s)) : 0u);
     const int bad = __reduce_min_sync(0xffffffffu, finite ? 0x7fffffff : pos);
-    s_at[t] = kv && !finite ? -1 : at;
-    s_scale[t] = kv && !finite ? 0.f : s;
+    if (kv && !finite) {
+      at = -1;
+      s = 0.f;
+    }
+    s_at[t] = at;
     if ((t & 31) == 0) {
       s_top[t >> 5] = __uint_as_float(top);
       s_bad[t >> 5] = bad;
@@ -234,6 +237,7 @@ __global__ void __launch_bounds__(WIDEN_THREADS)
     f[kv] = kv ? (float)ex : __int_as_float((127 + ex) << 23);
     if (kv) f[2] = __int_as_float(min(min(s_bad[0], s_bad[1]), min(s_bad[2], s_bad[3])));
   }
+  if (t < 128) s_mult[t] = split_f16(s * down);
   const int c = t & 15;
   uint2 x[8];
 #pragma unroll
@@ -241,19 +245,14 @@ __global__ void __launch_bounds__(WIDEN_THREADS)
     const long long at = s_at[(t >> 4) + 16 * i];
     x[i] = at >= 0 ? *reinterpret_cast<const uint2*>(data + at * HEAD + c * 8) : make_uint2(0, 0);
   }
+  __syncthreads();
+  uint8_t* to = wide + ((page * 2 + kv) * heads + head) * 128 * 256 + c * 16;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int row = (t >> 4) + 16 * i;
-    const float s = s_scale[row] * down;
-    float f[8];
-    decode8(x[i], f);
-    uint32_t w[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const __half2 h = __floats2half2_rn(f[2 * j] * s, f[2 * j + 1] * s);
-      w[j] = *reinterpret_cast<const uint32_t*>(&h);
-    }
-    *reinterpret_cast<uint4*>(wide + (((page * 2 + kv) * heads + head) * 128 + row) * 256 + c * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+    const uint32_t f = s_mult[row], hi = __byte_perm(f, f, 0x1010), lo = __byte_perm(f, f, 0x3232);
+    const uint2 y = widen_scaled(x[i].x, hi, lo), z = widen_scaled(x[i].y, hi, lo);
+    *reinterpret_cast<uint4*>(to + row * 256) = make_uint4(y.x, y.y, z.x, z.y);
   }
 }
 
