@@ -611,6 +611,26 @@ def test_a_page_that_does_not_exist_is_reported():
         assert same.all()
 
 
+@pytest.mark.parametrize("q_len,dtype", [(5, E4M3), (40, BF16), (40, E4M3), (300, E4M3)])      # every kernel that looks up pages
+def test_a_bad_page_under_a_chunk_is_reported(q_len, dtype):
+    from sensenova_u1_b200.ops import _lib, paged
+    cache, tables, rows = make([600], 32, 2, dtype)
+    plan = paged.build_plan(cache, 8, [q_len], [600], tables)
+    q = torch.randn(q_len, 8, D, device="cuda", generator=torch.Generator(device="cuda").manual_seed(3)).to(BF16)
+    want = paged.paged_attention(q, cache, plan, SCALE)
+    at = (plan._args.table - plan._store.data_ptr()) // 4 + 7
+    good = plan._store[at].clone()
+    for page in (cache.pages, -1):
+        plan._store[at] = page
+        _lib.check_status()
+        paged.paged_attention(q, cache, plan, SCALE)
+        with pytest.raises(_lib.NativeLibraryError, match="page"):
+            _lib.check_status()
+    plan._store[at] = good
+    assert torch.equal(paged.paged_attention(q, cache, plan, SCALE), want)
+    _lib.check_status()
+
+
 def test_rows_that_overlap_are_refused():
     from sensenova_u1_b200.ops import paged
     cache, tables, _ = make([40], 16, 2, BF16)
