@@ -74,8 +74,13 @@ def call(name: str, *args) -> None:
     fn = getattr(lib, "snu1_" + name)
     rc = fn(*args)
     if rc != 0:
-        msg = lib.snu1_last_error()
-        raise NativeLibraryError(f"snu1_{name} failed ({rc}): {msg.decode() if msg else ''}")
+        raise error(name, rc)
+
+
+def error(name: str, rc: int) -> NativeLibraryError:
+    """What to raise for the return code ``rc`` of ``snu1_<name>``."""
+    msg = load().snu1_last_error()
+    return NativeLibraryError(f"snu1_{name} failed ({rc}): {msg.decode() if msg else ''}")
 
 
 _ROLE = {1: "TMA producer", 2: "MMA issuer (accumulator)", 3: "MMA issuer (operands)",

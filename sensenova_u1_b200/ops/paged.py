@@ -60,6 +60,9 @@ CHUNK_START = 5          # what starting and ending a CTA costs, in key tiles (1
 CHUNK_JOIN = 3           # what a part costs besides: 128 KB written and read again
 
 
+_ENTRY: dict = {}         # the entry points that calls go to
+
+
 def _library():
     """The library, its entry points told the types of their arguments (cheaper than an object per argument and call)."""
     lib = _lib.load()
@@ -69,6 +72,8 @@ def _library():
         lib.snu1_paged_read.argtypes = (P, P, P, P, P)
         lib.snu1_paged_attention.argtypes = (P, P, P, L, P, L, c_float, P, ctypes.c_ulonglong, P)
         lib.snu1_paged_write.argtypes = (P, P, P, L, P, L, P)
+        for name in ("paged_write", "paged_read", "paged_attention"):
+            _ENTRY[name] = getattr(lib, "snu1_" + name)
     return lib
 
 
@@ -391,24 +396,30 @@ def _check(cache: PagedCache, plan: PagedPlan) -> None:
 
 def _row_stride(name: str, t: torch.Tensor, plan: PagedPlan, heads: int) -> int:
     """Elements from one row to the next of a [plan.rows or more, heads, 128] tensor."""
-    shape, stride = t.shape, t.stride()
-    if (len(shape) != 3 or shape[0] < plan.rows or shape[1] != heads or shape[2] != HEAD_DIM or stride[2] != 1
-            or (stride[1] != HEAD_DIM and heads > 1) or t.dtype is not _BF16 or t.get_device() != plan._index):
+    try:
+        rows, n, dim = t.shape
+        row, head, one = t.stride()
+    except ValueError:                                            # of other dimensions
+        rows = -1
+    if (rows < plan.rows or n != heads or dim != HEAD_DIM or one != 1 or (head != HEAD_DIM and heads > 1) or t.dtype is not _BF16
+            or t.get_device() != plan._index):
         raise ValueError(f"{name} must be bf16 [{plan.rows} or more, {heads}, {HEAD_DIM}] with contiguous heads on the plan's device")
-    if stride[0] < heads * HEAD_DIM:
-        if shape[0] > 1:
+    if row < heads * HEAD_DIM:
+        if rows > 1:
             raise ValueError(f"the rows of {name} overlap")
         return heads * HEAD_DIM                                   # (one row's stride says nothing)
-    return stride[0]
+    return row
 
 
 def _call(index: int, name: str, *args) -> None:
-    """On the tensors' device, whichever is current."""
-    if index == torch._C._cuda_getDevice():
-        _lib.call(name, *args, _lib.stream())
-    else:
+    """On the tensors' device, whichever is current.  (What ``_lib.call`` does, without looking the entry point up: 0.5 us of 6.)"""
+    if index != torch._C._cuda_getDevice():
         with torch.cuda.device(index):
-            _lib.call(name, *args, _lib.stream())
+            return _call(index, name, *args)
+    _lib.LAUNCHES += 1
+    rc = _ENTRY[name](*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc != 0:
+        raise _lib.error(name, rc)
 
 
 def paged_write(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, plan: PagedPlan) -> None:
