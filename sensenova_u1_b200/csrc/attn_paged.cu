@@ -32,7 +32,7 @@
 //
 // Measured (32 / 8 heads unless said, of a measured copy bandwidth of 6456 GB/s): e4m3, 48 x 1 token over 32700 keys, 4 heads, 152 us,
 // 5.9 TB/s or 0.91; 24 x 1 over up to 4096 keys 23 us, 0.65, of which 6 are a launch's start and end and the join; one
-// conversation of 840 bf16 keys 7 us in a graph, 8.5 called one by one, latency alone.  8 x 5 tokens over up to 12000 bf16 keys 44 us,
+// conversation of 840 bf16 keys 6.3 us in a graph, 7.8 called one by one, latency alone.  8 x 5 tokens over up to 12000 bf16 keys 44 us,
 // 0.73.  From 16 rows on instructions count: e4m3 8 x 12000 keys 4 / 16 / 24 / 32 rows 37 / 47 / 61 / 86 us.
 #include <math.h>
 #include <string.h>
