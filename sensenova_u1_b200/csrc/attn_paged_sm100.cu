@@ -29,6 +29,7 @@
 // chain.  Softmax warps without rows that only keep step made it 87, two places for P (so that its store need not wait for the
 // product before) 95.
 #include <cuda_fp16.h>
+#include <float.h>
 #include <string.h>
 
 #include <mutex>
@@ -683,7 +684,8 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
       float f[2];                            // scores in log2 units: s f
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        f[r] = FP16 ? sc[r] * factor.x : sc[r];
+        // (not 0, or a hidden score, -inf, would be NaN.  Sums are up to 2^34: where the factor is raised, all scores are below 2^-92.)
+        f[r] = FP16 ? fmaxf(sc[r] * factor.x, FLT_MIN) : sc[r];
         mx[r] = FP16 ? fmaf(mx[r], f[r], factor.y) : mx[r] * f[r];
       }
       const bool rescale = __any_sync(0xffffffffu, mx[0] > m[0] + 8.f || mx[1] > m[1] + 8.f);

@@ -779,3 +779,39 @@ def test_engine_refusals():
     for bad in (torch.zeros(3, 2), torch.zeros(2, 3), torch.zeros(3)):
         with pytest.raises(ValueError):
             eng.paged_step(plan, caches, ids=ids, pos3=bad.int())
+
+
+# ------------------------------------------------------------------ keys, values and queries of very different sizes
+def filled(kv, page, seed=0):
+    """An e4m3 cache that holds, per sequence, the given keys and values ([2, heads, keys, 128]), and what it then holds in 64 bits."""
+    from sensenova_u1_b200.ops import paged
+    lens, hk = [x.shape[2] for x in kv], kv[0].shape[1]
+    tables, pages = tables_for(lens, page, seed=seed)
+    data, scales = torch.zeros(pages, 2, hk, page, D, device="cuda", dtype=E4M3), torch.ones(pages, 2, hk, page, device="cuda")
+    rows = []
+    for x, t in zip(kv, tables):
+        codes, s = quantised(x.to(BF16))
+        rows.append(codes.double() * s.double()[..., None])
+        pos = torch.arange(x.shape[2])
+        pg, off = torch.tensor(t)[pos // page].cuda(), (pos % page).cuda()
+        data.view(torch.uint8)[pg, :, :, off] = codes.view(torch.uint8).permute(2, 0, 1, 3)
+        scales[pg, :, :, off] = s.permute(2, 0, 1)
+    return paged.PagedCache(data, scales), tables, rows
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+@pytest.mark.parametrize("q_len", [3, 40, 300])
+@pytest.mark.parametrize("q_size,k_size", [(2.0 ** -34, 0.0), (2.0 ** -64, 2.0 ** -64), (2.0 ** -100, 1.0), (2.0 ** -64, 2.0 ** 64)])
+def test_tiny_queries_and_keys(q_len, q_size, k_size):
+    """The factors of queries and keys together may be smaller than fp32 holds: hidden keys stay hidden."""
+    from sensenova_u1_b200.ops import paged
+    x = torch.randn(2, 2, q_len + 150, D, device="cuda", generator=gen(q_len))
+    x[0] *= k_size
+    cache, tables, rows = filled([x], 32)
+    q = (torch.randn(q_len, 8, D, device="cuda", generator=gen(1)) * q_size).to(BF16)
+    plan = paged.build_plan(cache, 8, [q_len], [q_len + 150], tables)
+    ref, room = exact(q, [q_len], rows, causal([q_len], [q_len + 150]), E4M3)
+    assert near(paged.paged_attention(q, cache, plan, SCALE), ref, room)
