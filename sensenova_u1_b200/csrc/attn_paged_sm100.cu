@@ -29,6 +29,7 @@
 // chain.  Softmax warps without rows that only keep step made it 87, two places for P (so that its store need not wait for the
 // product before) 95.
 #include <cuda_fp16.h>
+#include <cuda_fp8.h>
 #include <float.h>
 #include <string.h>
 
@@ -59,6 +60,8 @@ struct Chunk {
 };
 
 struct ChunkArgs {
+  const __nv_bfloat16* q;
+  long long ldq;
   __nv_bfloat16* o;
   long long ldo;
   float* part;
@@ -68,6 +71,9 @@ struct ChunkArgs {
   const float4* factors;   // of the widened pages, see paged_widen_kernel
   int page, pages, heads;
   float scale_log2;
+  const uint8_t* data;     // the cache itself
+  const float* scales;
+  int cache_pages;
   int* status;
 };
 
@@ -126,10 +132,76 @@ __device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint32_t b, uint
 
 constexpr uint32_t CLEAR_ROW = 0x80000000u;     // a row's factor: + 0 and - 0, which no scale gives
 
+// One row's attention to keys [k0, k1) of its sequence by one warp, in fp32 on the cache as it is; four values per lane.  The softmax of the
+// chunk kernel takes a score's product and the running maximum's difference in one step.  The maximum is rounded, the product is not, so
+// 2^-24 of the score is left over: beyond 2^20 that would show, and from 2^26 on probabilities overflow.  A warp that meets such a
+// row computes it again here.  (As a branch of the softmax's loop, rounding such scores first made all calls 5 to 18 % slower.)
+constexpr float FAR = 1048576.f;                // 2^20, log2 units
+template <bool FP8>
+__noinline__ __device__ void far_row(const Plan& p, const ChunkArgs& a, int b, int row, int head, int kvh, int k0, int k1, float4* x, float2* ml) {
+  const int lane = threadIdx.x & 31, group = 4;
+  const uint2 u = *reinterpret_cast<const uint2*>(a.q + row * a.ldq + head * HEAD + lane * 4);
+  const float q[4] = {__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16), __uint_as_float(u.y & 0xffff0000u)};
+  float m = -INFINITY, l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int k = k0; k < k1; k += group) {
+    float v[group][4], s[group];
+#pragma unroll
+    for (int i = 0; i < group; ++i) {
+      const int key = min(k + i, k1 - 1), pg = p.table[(long long)b * p.width + key / p.page];
+      float c[2][4];
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv) {
+        const long long at = (((long long)pg * 2 + kv) * a.heads + kvh) * p.page + key % p.page;
+        const bool there = pg >= 0 && pg < a.cache_pages;        // (reported by who asked for the page)
+        if (FP8) {
+          const uint32_t w = there ? *reinterpret_cast<const uint32_t*>(a.data + at * HEAD + lane * 4) : 0u;
+          const float scale = there ? a.scales[at] : 0.f;
+          const float2 lo = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)w, __NV_E4M3)));
+          const float2 hi = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> 16), __NV_E4M3)));
+          c[kv][0] = lo.x * scale, c[kv][1] = lo.y * scale, c[kv][2] = hi.x * scale, c[kv][3] = hi.y * scale;
+        } else {
+          const uint2 w = there ? *reinterpret_cast<const uint2*>(a.data + at * (2 * HEAD) + lane * 8) : make_uint2(0, 0);
+          c[kv][0] = __uint_as_float(w.x << 16), c[kv][1] = __uint_as_float(w.x & 0xffff0000u);
+          c[kv][2] = __uint_as_float(w.y << 16), c[kv][3] = __uint_as_float(w.y & 0xffff0000u);
+        }
+      }
+      s[i] = 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s[i] = fmaf(q[e], c[0][e], s[i]);
+        v[i][e] = c[1][e];
+      }
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < group; ++i) {
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) s[i] += __shfl_xor_sync(0xffffffffu, s[i], o);
+      s[i] = k + i < k1 ? __fmul_rn(s[i], a.scale_log2) : -INFINITY;
+      top = fmaxf(top, s[i]);
+    }
+    const float now = fmaxf(m, top), f = m == -INFINITY ? 0.f : fast_exp2(m - now);
+    m = now;
+    l *= f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] *= f;
+#pragma unroll
+    for (int i = 0; i < group; ++i) {
+      if (k + i >= k1) break;
+      const float pr = fast_exp2(s[i] - m);
+      l += pr;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] = fmaf(pr, v[i][e], acc[e]);
+    }
+  }
+  *x = make_float4(acc[0], acc[1], acc[2], acc[3]);
+  *ml = make_float2(m, l);
+}
+
 template <int MODE>
 __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
-                       const __grid_constant__ CUtensorMap tm_v, const Plan p, const ChunkArgs args) {
+                       const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ Plan p, const __grid_constant__ ChunkArgs args) {
   using C = Chunk<MODE>;
   constexpr bool FP16 = C::FP16, RAW = C::RAW;
   constexpr int TILES = C::TILES, CK_STAGES = C::K_STAGES, CV_STAGES = C::V_STAGES;
@@ -762,6 +834,33 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
         if (lim[r] > (MODE == kWide ? bad : *poison)) l[r] = __int_as_float(0x7fffffff);
       }
+      // rows with scores whose rounding counts; infinite ones stay what they are
+      uint32_t done = 0;                     // this warp's rows that are computed again
+      {
+        const bool far[2] = {lim[0] >= 0 && fabsf(m[0]) > FAR && fabsf(m[0]) < INFINITY, lim[1] >= 0 && fabsf(m[1]) > FAR && fabsf(m[1]) < INFINITY};
+        const uint32_t f0 = __ballot_sync(0xffffffffu, far[0]), f1 = __ballot_sync(0xffffffffu, far[1]);
+        if (f0 | f1) {
+#pragma unroll 1
+          for (int i = 0; i < 16; ++i) {
+            if (((i < 8 ? f0 : f1) >> (i & 7) * 4 & 1) == 0) continue;
+            const int r = base + i, row = q0 + token0 + t * T + r / G, head = kvh * G + r % G;
+            const int end = __shfl_sync(0xffffffffu, i < 8 ? lim[0] : lim[1], (i & 7) * 4);
+            float4 x;
+            float2 ml;
+            far_row<FP16>(p, args, b, row, head, kvh, j0 * BK, min(end, (j0 + mine) * BK), &x, &ml);
+            if (item.w < 0) {
+              const float inv = ml.y == 0.f ? 0.f : 1.f / ml.y;
+              *reinterpret_cast<uint2*>(args.o + row * args.ldo + head * HEAD + lane * 4) =
+                  make_uint2(pack_bf16x2(x.x * inv, x.y * inv), pack_bf16x2(x.z * inv, x.w * inv));
+            } else {
+              const long long at = ((long long)item.w + t * T * G + r) * args.heads + kvh;
+              *reinterpret_cast<float4*>(args.part + at * HEAD + lane * 4) = x;
+              if (lane == 0) args.part_ml[at] = ml;
+            }
+            done |= 1u << i;
+          }
+        }
+      }
       if (item.w < 0) {
         // Output rows leave through this warp's rows of the row tile's buffer (no product reads it any more), so that 16
         // lanes store one row's 256 bytes.
@@ -789,7 +888,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const int r = base + 2 * i + (lane >> 4), c = lane & 15, of = r * per >> 16, token = token0 + t * T + of;
-          if (r < T * G && token < q_len)
+          if (r < T * G && token < q_len && (done >> (r - base) & 1) == 0)
             *reinterpret_cast<uint4*>(args.o + (long long)(q0 + token) * args.ldo + (long long)(kvh * G + r - of * G) * HEAD + c * 8) =
                 mine > 0 ? *reinterpret_cast<const uint4*>(sOt + (c >> 3) * CHALF + swz128_offset(r, c & 7)) : make_uint4(0, 0, 0, 0);
         }
@@ -807,7 +906,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
           }
 #pragma unroll
           for (int e = 0; e < 2; ++e)
-            if (lim[e] >= 0) {
+            if (lim[e] >= 0 && (done >> (lane >> 2) + 8 * e & 1) == 0) {
               float* dst = args.part + (at0 + 8ll * e * args.heads) * HEAD + h * 64 + q2;
 #pragma unroll
               for (int i = 0; i < 8; ++i)
@@ -818,7 +917,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         if ((lane & 3) == 0) {
 #pragma unroll
           for (int e = 0; e < 2; ++e)
-            if (lim[e] >= 0)        // scores that were all NaN are not to be taken for no keys at all
+            if (lim[e] >= 0 && (done >> (lane >> 2) + 8 * e & 1) == 0)        // scores that were all NaN are not to be taken for no keys at all
               args.part_ml[at0 + 8ll * e * args.heads] = make_float2(m[e] == -INFINITY && l[e] != l[e] ? 0.f : FP16 ? m[e] - P_TOP : m[e], l[e]);
         }
       }
@@ -869,6 +968,11 @@ int launch_chunks(const Cache& c, const Plan& p, const void* q, long long ldq, v
   a.factors = nullptr;
   a.page = c.page;
   a.pages = c.pages;
+  a.q = (const __nv_bfloat16*)q;
+  a.ldq = ldq;
+  a.data = (const uint8_t*)c.data;
+  a.scales = c.scales;
+  a.cache_pages = c.pages;
   a.o = (__nv_bfloat16*)o;
   a.ldo = ldo;
   a.part = part;

@@ -815,3 +815,38 @@ def test_tiny_queries_and_keys(q_len, q_size, k_size):
     plan = paged.build_plan(cache, 8, [q_len], [q_len + 150], tables)
     ref, room = exact(q, [q_len], rows, causal([q_len], [q_len + 150]), E4M3)
     assert near(paged.paged_attention(q, cache, plan, SCALE), ref, room)
+
+
+def scores_of_any_size(q_len, size, dtype):
+    """One channel of every query is ``size``, and one key that all rows read has 8 there, the others 3 at most: the result is that key's
+    value, rounded once as a product (2^-8, fp16 2^-11) and once as a result."""
+    from sensenova_u1_b200.ops import paged
+    n = q_len + 170
+    x = torch.randn(2, 2, n, D, device="cuda", generator=gen(q_len))
+    x[0].clamp_(-3, 3)
+    at = torch.randint(170, (2, D), device="cuda", generator=gen(2))
+    x[0].scatter_(1, at[:, None], 8.0)
+    if dtype == E4M3:
+        x[1] *= torch.exp2(torch.randint(-3, 4, (2, n, 1), device="cuda", generator=gen(3)).float())
+        cache, tables, rows = filled([x], 32)
+    else:
+        tables, pages = tables_for([n], 32)
+        cache = paged.PagedCache.empty(pages, 32, 2)
+        fill = paged.build_plan(cache, 8, [n], [n], tables)
+        kv = x.to(BF16).transpose(1, 2).contiguous()
+        paged.paged_write(cache, kv[0], kv[1], fill)
+        rows = [x.to(BF16).double()]
+    d = torch.arange(q_len * 8, device="cuda").view(q_len, 8) * 5 % D
+    q = torch.zeros(q_len, 8, D, device="cuda", dtype=BF16).scatter_(2, d[..., None], size)
+    plan = paged.build_plan(cache, 8, [q_len], [n], tables)
+    head = torch.arange(8, device="cuda") // 4
+    want = rows[0][1][head, at[head, d]]
+    out = paged.paged_attention(q, cache, plan, SCALE).double()
+    assert ((out - want).abs() <= (2 * 2.0 ** -8 + 2.0 ** -11) * want.abs()).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, E4M3])
+@pytest.mark.parametrize("q_len", [40, 300])
+@pytest.mark.parametrize("size", [2.0 ** e for e in (12, 17, 20, 22, 24, 26, 28, 30, 33, 60, 100)])
+def test_scores_of_any_size_in_chunks(q_len, size, dtype):
+    scores_of_any_size(q_len, size, dtype)
