@@ -11,8 +11,8 @@
 //   are fp16 as well.  So the softmax pays for the scales once per tile and row, not per score: the keys' power of two goes
 //   into the factor of the scores, the values' into the exponent of the probabilities (and out of their sum).  Scales
 //   applied per score and probability in fp32 took 2.33 us per pair of tiles instead of 1.78 (2 x 512 new tokens, 8192 keys);
-//   keys rounded to bf16 would move every score by up to 2^-8 of the sum of |q k|.  The queries are scaled 16 rows at a time, by
-//   the softmax warps.
+//   keys rounded to bf16 would move every score by up to 2^-8 of the sum of |q k|.  The queries are scaled row by row, by the
+//   softmax warps.
 // * The mask is one number per row, the keys that it may read; tiles that all rows read whole need no test.
 // * A work item is a part of the key tiles of two row tiles; unnormalised results of parts are joined by
 //   paged_merge_kernel.  ops/paged.py chooses the parts so that the waves of CTAs are full.
@@ -640,50 +640,37 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     float sc[2] = {args.scale_log2, args.scale_log2};
     bool ok = true;
     if (FP16 && n > 0) {
-      // This warp's 16 query rows to fp16, all times the power of two that brings the largest value to [2^13, 2^14).  Smaller rows
-      // lose 2^-38 of that value at most, so a score is off by less than 2^-34 of the largest one's sum of |q k|.
+      // This warp's 16 query rows to fp16, each times the power of two that brings its largest value to [2^13, 2^14): a value
+      // loses 2^-38 of its row's largest at most.  (One power of two for all of them would let a large row take its neighbours' bits.)
       ok &= mbar_wait(q_full, 0, abort_flag, args.status, 5);
       __syncwarp();
       uint8_t* at = sOt + ((lane & 15) >> 3) * CHALF;
-      uint4 u[8];
+      uint4 u[8];                            // 16 lanes have a row: 2 i + lane / 16
 #pragma unroll
       for (int i = 0; i < 8; ++i) u[i] = *reinterpret_cast<const uint4*>(at + swz128_offset(base + 2 * i + (lane >> 4), lane & 7));
-      // rows of nobody decide nothing
       const int mine = (min(token0 + (t + 1) * T, q_len) - (token0 + t * T)) * G - base;     // rows of this warp that are somebody's
-      uint32_t top = 0;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         if (2 * i + (lane >> 4) >= mine) u[i] = make_uint4(0, 0, 0, 0);
-        top = max_u16x2(top, max_u16x2(max_u16x2(u[i].x & 0x7fff7fffu, u[i].y & 0x7fff7fffu), max_u16x2(u[i].z & 0x7fff7fffu, u[i].w & 0x7fff7fffu)));
-      }
-      top = __reduce_max_sync(0xffffffffu, max(top << 16, top & 0xffff0000u));
-      if (top >= 0x7f800000u) {              // some value is not finite: the largest of the others
-        top = 0;
+        uint32_t top = max_u16x2(max_u16x2(u[i].x & 0x7fff7fffu, u[i].y & 0x7fff7fffu), max_u16x2(u[i].z & 0x7fff7fffu, u[i].w & 0x7fff7fffu));
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const uint32_t* w = reinterpret_cast<const uint32_t*>(&u[i]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t lo = (w[e] << 16) & 0x7fffffffu, hi = w[e] & 0x7fff0000u;
-            top = max(top, max(lo < 0x7f800000u ? lo : 0u, hi < 0x7f800000u ? hi : 0u));
-          }
-        }
-        top = __reduce_max_sync(0xffffffffu, top);
-      }
-      const int up = top == 0 ? 0 : min(13 - ((int)(top >> 23) - 127), 120);
-      const float f = __int_as_float((127 + up) << 23);
-      const uint64_t f2 = pack_f32x2(f, f);
-      sc[0] = sc[1] = args.scale_log2 * __int_as_float((127 - up) << 23);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
+        for (int o = 1; o < 16; o <<= 1) top = max_u16x2(top, __shfl_xor_sync(0xffffffffu, top, o));
+        top = max(top << 16, top & 0xffff0000u);
+        const int e = (int)(top >> 23) - 127;                    // of the largest value; zero and what is not finite: as it is
+        const int up = top == 0 || e == 128 ? 0 : min(13 - e, 120);
+        const float f = __int_as_float((127 + up) << 23);
+        const uint64_t f2 = pack_f32x2(f, f);
         uint32_t* w = reinterpret_cast<uint32_t*>(&u[i]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+        for (int h = 0; h < 4; ++h) {
           float x, y;
-          unpack_f32x2(mul_f32x2(bf16x2_to_f32x2(w[e]), f2), x, y);
-          w[e] = pack_f16x2(x, y);
+          unpack_f32x2(mul_f32x2(bf16x2_to_f32x2(w[h]), f2), x, y);
+          w[h] = pack_f16x2(x, y);
         }
         *reinterpret_cast<uint4*>(at + swz128_offset(base + 2 * i + (lane >> 4), lane & 7)) = u[i];
+        // to the threads that hold this row's scores: rows lane / 4 and lane / 4 + 8
+        const float back = __shfl_sync(0xffffffffu, __int_as_float((127 - up) << 23), (lane & 4) << 2);
+        if ((i & 3) == lane >> 3) sc[i >> 2] = args.scale_log2 * back;
       }
       fence_proxy_async_smem();
       __syncwarp();

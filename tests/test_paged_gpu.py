@@ -850,3 +850,20 @@ def scores_of_any_size(q_len, size, dtype):
 @pytest.mark.parametrize("size", [2.0 ** e for e in (12, 17, 20, 22, 24, 26, 28, 30, 33, 60, 100)])
 def test_scores_of_any_size_in_chunks(q_len, size, dtype):
     scores_of_any_size(q_len, size, dtype)
+
+
+@pytest.mark.parametrize("q_len,kv_len", [(2, 150), (40, 300), (70, 1000), (300, 700)])
+def test_a_large_query_is_its_own_matter(q_len, kv_len):
+    """Rows side by side whose sizes are 2^60 and 2^-60: every other row is as near as without them."""
+    from sensenova_u1_b200.ops import paged
+    cache, tables, rows = make([kv_len], 32, 2, E4M3)
+    q = torch.randn(q_len, 8, D, device="cuda", generator=gen(q_len)).to(BF16)
+    large = torch.zeros(q_len, 8, dtype=torch.bool, device="cuda")
+    large[1::7, 3] = large[0::9, 6] = True
+    q[large] *= 2.0 ** 60
+    q[1::5, 1] *= 2.0 ** -60
+    plan = paged.build_plan(cache, 8, [q_len], [kv_len], tables)
+    ref, room = exact(q, [q_len], rows, causal([q_len], [kv_len]), E4M3)
+    out = paged.paged_attention(q, cache, plan, SCALE)
+    assert near(out[~large], ref[~large], room[~large])
+    assert torch.isfinite(out).all()
