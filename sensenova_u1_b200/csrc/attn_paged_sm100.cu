@@ -130,6 +130,9 @@ __device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint32_t b, uint
       : "memory");
 }
 
+// Sums of probabilities over e4m3 are kept 2^12 times smaller.  A tile of zeros (or values below 2^-80) has 2^-93 as its power of two: a
+// probability, up to 2^15, counts 2^96 then, and 2^30 keys of them stay below 2^128.  At the other end, 2^113, a factor is 2^-125.
+constexpr float SUM_DOWN = 12.f;
 constexpr uint32_t CLEAR_ROW = 0x80000000u;     // a row's factor: + 0 and - 0, which no scale gives
 
 // One row's attention to keys [k0, k1) of its sequence by one warp, in fp32 on the cache as it is; four values per lane.  The softmax of the
@@ -775,7 +778,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
             acc[r][i & 1] = add_f32x2(acc[r][i & 1], pack_f32x2(x, y));
             pk[16 * h + 2 * i + r] = FP16 ? pack_f16x2(x, y) : pack_bf16x2(x, y);
           }
-      const float out_of = FP16 ? fast_exp2(-factor.y) : 1.f;       // the sum is of probabilities, without the values' power of two
+      const float out_of = FP16 ? fast_exp2(-SUM_DOWN - factor.y) : 1.f;       // the sum is of probabilities, without the values' power of two
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         float s0, s1;
@@ -848,6 +851,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
           }
         }
       }
+      const float down = FP16 ? 1.f / 4096.f : 1.f;      // as the sums: SUM_DOWN
       if (item.w < 0) {
         // Output rows leave through this warp's rows of the row tile's buffer (no product reads it any more), so that 16
         // lanes store one row's 256 bytes.
@@ -865,7 +869,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
               uint32_t w[4];
 #pragma unroll
               for (int e = 0; e < 4; ++e)
-                w[e] = pack_bf16x2(__uint_as_float(r[4 * i + 2 * e]) * inv[e & 1], __uint_as_float(r[4 * i + 2 * e + 1]) * inv[e & 1]);
+                w[e] = pack_bf16x2(down * __uint_as_float(r[4 * i + 2 * e]) * inv[e & 1], down * __uint_as_float(r[4 * i + 2 * e + 1]) * inv[e & 1]);
               stmatrix_x4(st_row + h * CHALF + (st_chunk ^ (i << 4)), w[0], w[1], w[2], w[3]);
             }
           }
@@ -897,7 +901,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
               float* dst = args.part + (at0 + 8ll * e * args.heads) * HEAD + h * 64 + q2;
 #pragma unroll
               for (int i = 0; i < 8; ++i)
-                *reinterpret_cast<float2*>(dst + i * 8) = make_float2(__uint_as_float(r[4 * i + 2 * e]), __uint_as_float(r[4 * i + 2 * e + 1]));
+                *reinterpret_cast<float2*>(dst + i * 8) = make_float2(down * __uint_as_float(r[4 * i + 2 * e]), down * __uint_as_float(r[4 * i + 2 * e + 1]));
             }
           __syncwarp();
         }
@@ -905,7 +909,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
 #pragma unroll
           for (int e = 0; e < 2; ++e)
             if (lim[e] >= 0 && (done >> (lane >> 2) + 8 * e & 1) == 0)        // scores that were all NaN are not to be taken for no keys at all
-              args.part_ml[at0 + 8ll * e * args.heads] = make_float2(m[e] == -INFINITY && l[e] != l[e] ? 0.f : FP16 ? m[e] - P_TOP : m[e], l[e]);
+              args.part_ml[at0 + 8ll * e * args.heads] = make_float2(m[e] == -INFINITY && l[e] != l[e] ? 0.f : FP16 ? m[e] - P_TOP + SUM_DOWN : m[e], l[e]);
         }
       }
     }

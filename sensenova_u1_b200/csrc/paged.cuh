@@ -59,7 +59,7 @@ struct Plan {
 // up to 448), and they are taken 2^WIDEN_UP times larger, up to 2^15 if the exponent is at its upper limit.
 constexpr int WIDEN_UP = 13;
 __device__ __forceinline__ int tile_exponent(float top) {
-  return max(-90, min(126, (int)(__float_as_uint(E4M3_MAX * top) >> 23) - 126));
+  return max(-80, min(126, (int)(__float_as_uint(E4M3_MAX * top) >> 23) - 126));
 }
 
 __device__ __forceinline__ int seq_len(const Plan& p, int b) { return max(0, min(p.kv_len[b], p.cap[b])); }

@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(READ_THREADS)
 
 // Tiles of 128 tokens of an e4m3 cache for attn_paged_sm100.cu: fp16 pages of 128 tokens in a cache's own layout, every
 // sequence from a page of its own on, rows behind its last token cleared.  A tile of one head is divided by a power of two,
-// so that its largest value is at most 2^13 (2^-103 to 2^113; that factor goes into the scores, or into the probabilities): code times
+// so that its largest value is at most 2^13 (2^-93 to 2^113; that factor goes into the scores, or into the probabilities): code times
 // scale is rounded to 11 bits, and what falls below fp16's normal range is 2^27 times smaller than the tile's largest value.
 // factors [page][heads]: the keys' power of two, the exponent of the values' (log2), and, as a whole number, the first
 // key of the sequence in this tile whose value is not finite (its scale is not); that value is cleared.

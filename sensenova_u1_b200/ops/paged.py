@@ -452,7 +452,7 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, plan: PagedPlan, scale: 
     What lies behind a sequence's last token or in pages of nobody does not matter.  Over e4m3
     a key adds nothing to the output where its probability times the size of its value is below 2^-32 of the largest such
     product.  Chunks (more than 32 rows per key/value head) over e4m3 hold 128 cached tokens' values of a head relative to the largest of them: values 2^27 times smaller than that
-    lose bits.  Where the largest value of another 128 tokens is 2^d times larger (zeros count as 2^-90), probabilities below
+    lose bits.  Where the largest value of another 128 tokens is 2^d times larger (less than 2^-80 counts as that), probabilities below
     2^(d - 133) of the largest one are lost."""
     _check(cache, plan)
     ldq = _row_stride("q", q, plan, plan.heads)

@@ -867,3 +867,22 @@ def test_a_large_query_is_its_own_matter(q_len, kv_len):
     out = paged.paged_attention(q, cache, plan, SCALE)
     assert near(out[~large], ref[~large], room[~large])
     assert torch.isfinite(out).all()
+
+
+@pytest.mark.parametrize("q_len,split", [(3, False), (40, False), (40, True), (300, False), (300, True)])
+def test_many_keys_without_values(q_len, split, monkeypatch):
+    """Thousands of keys whose values are zero count in the sums that the others are divided by: values in the last 100 keys only, and
+    all scores but those of the first tile nearly 2^8 times the first tile's (the running maximum is left behind)."""
+    from sensenova_u1_b200.ops import paged
+    if not split:
+        monkeypatch.setattr(paged, "_waves", lambda tiles, heads, slots: tiles * 0 + 1)
+    n = 9000 + q_len
+    x = torch.zeros(2, 2, n, D, device="cuda")
+    x[0, :, 128:, 0] = 5.4
+    x[1, :, 8900:] = torch.randn(2, n - 8900, D, device="cuda", generator=gen(3)) + 0.5
+    cache, tables, rows = filled([x], 64)
+    q = torch.zeros(q_len, 8, D, device="cuda", dtype=BF16)
+    q[..., 0] = 11.25                                     # scores of 5.37 = 7.74 in log2 units
+    plan = paged.build_plan(cache, 8, [q_len], [n], tables)
+    ref, room = exact(q, [q_len], rows, causal([q_len], [n]), E4M3)
+    assert near(paged.paged_attention(q, cache, plan, SCALE), ref, room)
