@@ -409,7 +409,8 @@ __global__ void __launch_bounds__(Few<FP8, NR, WR>::THREADS, Few<FP8, NR, WR>::C
       for (int d = 0; d < 8; ++d)
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[i][d][e] = 0.f;
-    // running maxima of the scores (for the sums l) and of scores + log2 of the values' scales (for acc); bf16: the same
+    // running maxima of the scores (for the sums l) and of scores + log2 of the values' scales (for acc; relative to m: beside a large
+    // score a small logarithm would be rounded away, and the value's scale with it); bf16: the same
     float m[NR][2], mv[NR][2], l[NR][2];
 #pragma unroll
     for (int i = 0; i < NR; ++i)
@@ -491,7 +492,7 @@ __global__ void __launch_bounds__(Few<FP8, NR, WR>::THREADS, Few<FP8, NR, WR>::C
             }
           }
         }
-        // scores in log2 units, masked; largest of this thread's keys
+        // scores in log2 units, masked, relative to m; largest of this thread's keys
         float lv[NB][2];                     // log2 of the values' scales
         float mx[NR][2], mxv[NR][2];
 #pragma unroll
@@ -515,8 +516,9 @@ __global__ void __launch_bounds__(Few<FP8, NR, WR>::THREADS, Few<FP8, NR, WR>::C
           for (int i = 0; i < NR; ++i)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              float x = sv[i][nb][e] * (FP8 ? rs[i][e & 1] * ks[e >> 1] : rs[i][e & 1]);
+              float x = __fmul_rn(sv[i][nb][e], FP8 ? rs[i][e & 1] * ks[e >> 1] : rs[i][e & 1]);      // (never fused with the difference)
               if (partial && k0 + key + (e >> 1) * 8 >= lim[i][e & 1]) x = -INFINITY;
+              x -= m[i][e & 1] == -INFINITY ? 0.f : m[i][e & 1];
               sv[i][nb][e] = x;
               mx[i][e & 1] = fmaxf(mx[i][e & 1], x);
               if (FP8) mxv[i][e & 1] = fmaxf(mxv[i][e & 1], x + lv[nb][e >> 1]);
@@ -528,25 +530,34 @@ __global__ void __launch_bounds__(Few<FP8, NR, WR>::THREADS, Few<FP8, NR, WR>::C
 #pragma unroll
         for (int i = 0; i < NR; ++i)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) move |= mx[i][e] > m[i][e] + 8.f || (FP8 && mxv[i][e] > mv[i][e] + 8.f);
+          for (int e = 0; e < 2; ++e) move |= mx[i][e] > (m[i][e] == -INFINITY ? -INFINITY : 8.f) || (FP8 && mxv[i][e] > mv[i][e] + 8.f);
         if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
           for (int i = 0; i < NR; ++i)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
 #pragma unroll
-              for (int o = 4; o < 32; o <<= 1) {
-                mx[i][e] = fmaxf(mx[i][e], __shfl_xor_sync(0xffffffffu, mx[i][e], o));
-                if (FP8) mxv[i][e] = fmaxf(mxv[i][e], __shfl_xor_sync(0xffffffffu, mxv[i][e], o));
-              }
-              const float mn = fmaxf(m[i][e], mx[i][e]);
-              const float f = m[i][e] == -INFINITY ? 0.f : fast_exp2(m[i][e] - mn);
-              m[i][e] = mn;
+              for (int o = 4; o < 32; o <<= 1) mx[i][e] = fmaxf(mx[i][e], __shfl_xor_sync(0xffffffffu, mx[i][e], o));
+              const bool fresh = m[i][e] == -INFINITY;
+              // (by the difference itself, not by that of two rounded maxima: the largest score here is 0 then)
+              const float by = fresh ? (mx[i][e] == -INFINITY ? 0.f : mx[i][e]) : fmaxf(mx[i][e], 0.f);
+              const float f = fresh ? 0.f : fast_exp2(-by);
+              m[i][e] = fresh ? mx[i][e] : m[i][e] + by;
               l[i][e] *= f;
               float fv = f;
+              mxv[i][e] = -INFINITY;
+#pragma unroll
+              for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                  sv[i][nb][2 * h + e] -= by;
+                  if (FP8) mxv[i][e] = fmaxf(mxv[i][e], sv[i][nb][2 * h + e] + lv[nb][h]);
+                }
               if (FP8) {
-                const float nv = fmaxf(mv[i][e], mxv[i][e]);
-                fv = mv[i][e] == -INFINITY ? 0.f : fast_exp2(mv[i][e] - nv);
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) mxv[i][e] = fmaxf(mxv[i][e], __shfl_xor_sync(0xffffffffu, mxv[i][e], o));
+                const float nv = fmaxf(mv[i][e] - by, mxv[i][e]);
+                fv = mv[i][e] == -INFINITY ? 0.f : fast_exp2(mv[i][e] - by - nv);
                 mv[i][e] = nv;
               }
 #pragma unroll
@@ -560,18 +571,15 @@ __global__ void __launch_bounds__(Few<FP8, NR, WR>::THREADS, Few<FP8, NR, WR>::C
         uint32_t pr[NR][NB][2];              // bf16: what rounding has left
 #pragma unroll
         for (int i = 0; i < NR; ++i) {
-          float mu[2], muv[2];
+          float muv[2];
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            mu[e] = m[i][e] == -INFINITY ? 0.f : m[i][e];
-            muv[e] = FP8 && mv[i][e] != -INFINITY ? mv[i][e] - P_TOP : 0.f;
-          }
+          for (int e = 0; e < 2; ++e) muv[e] = FP8 && mv[i][e] != -INFINITY ? mv[i][e] - P_TOP : 0.f;
 #pragma unroll
           for (int nb = 0; nb < NB; ++nb) {
             float x[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              x[e] = fast_exp2(sv[i][nb][e] - mu[e & 1]);
+              x[e] = fast_exp2(sv[i][nb][e]);
               l[i][e & 1] += x[e];
               // (the logarithm of a masked key's scale may be anything)
               if (FP8) x[e] = partial && sv[i][nb][e] == -INFINITY ? 0.f : fast_exp2(sv[i][nb][e] + lv[nb][e >> 1] - muv[e & 1]);
@@ -643,7 +651,7 @@ __global__ void __launch_bounds__(Few<FP8, NR, WR>::THREADS, Few<FP8, NR, WR>::C
         if (!FP8 && lim[i][e] > s_poison) l[i][e] = __int_as_float(0x7fffffff);
         if (l[i][e] != l[i][e] && m[i][e] == -INFINITY) m[i][e] = 0.f;       // all NaN: not to be taken for no keys at all
         // acc relative to the scores' maximum
-        const float f = !FP8 || mv[i][e] == -INFINITY ? 1.f : exp2f(mv[i][e] - P_TOP - m[i][e]);
+        const float f = !FP8 || mv[i][e] == -INFINITY ? 1.f : exp2f(mv[i][e] - P_TOP);
         const int row = i * 8 + 2 * c + e;
         if (g == 0) {
           s_m[warp][row] = m[i][e];

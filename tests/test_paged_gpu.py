@@ -886,3 +886,39 @@ def test_many_keys_without_values(q_len, split, monkeypatch):
     plan = paged.build_plan(cache, 8, [q_len], [n], tables)
     ref, room = exact(q, [q_len], rows, causal([q_len], [n]), E4M3)
     assert near(paged.paged_attention(q, cache, plan, SCALE), ref, room)
+
+
+@pytest.mark.parametrize("dtype", [BF16, E4M3])
+@pytest.mark.parametrize("q_len", [1, 4, 6, 8])
+@pytest.mark.parametrize("size", [2.0 ** e for e in (12, 17, 20, 22, 24, 26, 28, 30, 33, 60, 100)])
+def test_scores_of_any_size_in_few_rows(q_len, size, dtype):
+    scores_of_any_size(q_len, size, dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF16, E4M3])
+@pytest.mark.parametrize("q_len", [1, 4, 6, 8, 40, 300])
+@pytest.mark.parametrize("size", [2.0 ** e for e in (12, 20, 24, 27, 30, 33, 60, 100)])
+def test_equal_scores_of_any_size(q_len, size, dtype):
+    """The largest score occurs in several tiles (the mean of equal values is that value), behind tiles of ordinary and negative ones."""
+    from sensenova_u1_b200.ops import paged
+    n = q_len + 900
+    x = torch.zeros(2, 2, n, D, device="cuda")
+    x[0] = -2.0 * torch.rand(2, n, D, device="cuda", generator=gen(q_len))
+    x[0, :, :140, :64] = 2.0 ** -14                       # channels whose first scores are ordinary
+    x[0, :, 300:900:75] = 7.0
+    x[1] = torch.randn(2, 1, D, device="cuda", generator=gen(3))
+    x[1, :, :300] *= -1
+    if dtype == E4M3:
+        cache, tables, rows = filled([x], 32)
+    else:
+        tables, pages = tables_for([n], 32)
+        cache = paged.PagedCache.empty(pages, 32, 2)
+        kv = x.to(BF16).transpose(1, 2).contiguous()
+        paged.paged_write(cache, kv[0], kv[1], paged.build_plan(cache, 8, [n], [n], tables))
+        rows = [x.to(BF16).double()]
+    d = torch.arange(q_len * 8, device="cuda").view(q_len, 8) * 5 % D
+    q = torch.zeros(q_len, 8, D, device="cuda", dtype=BF16).scatter_(2, d[..., None], size)
+    plan = paged.build_plan(cache, 8, [q_len], [n], tables)
+    want = rows[0][1][torch.arange(8, device="cuda") // 4, 300].expand(q_len, 8, D)
+    out = paged.paged_attention(q, cache, plan, SCALE).double()
+    assert ((out - want).abs() <= (2 * 2.0 ** -8 + 2.0 ** -11) * want.abs()).all()
