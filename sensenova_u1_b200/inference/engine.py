@@ -143,7 +143,7 @@ class InferenceEngine:
         self.vc = [torch.zeros(kv_rows, cfg.num_kv_heads, 128, dtype=torch.bfloat16, device=self.dev)
                    for _ in range(cfg.num_layers)]
 
-    def layers(self, x, branch: int, pos3, plan, kv_rows, kv_len: int, publish=None, caches=None):
+    def layers(self, x, branch: int, pos3, plan, kv_rows, kv_len: int, publish=None, caches=None, ws: Optional[Workspace] = None):
         """Runs the decoder stack on rows ``x`` [R,H] with one branch's weights.  The rows'
         K/V are written to cache rows ``kv_rows`` (int64 [R]); attention reads cache rows
         [0, kv_len).  Returns the final hidden state (before the final norm).
@@ -151,9 +151,11 @@ class InferenceEngine:
         With a ``paged.PagedPlan`` the rows' K/V go to their sequences' pages in ``caches`` (one per layer) and attention
         reads those; ``kv_rows`` and ``kv_len`` are not used.
 
+        ``ws``: where the rows' buffers come from (default: the engine's own, which the next call uses again and a larger one replaces).
+
         ``publish`` (sequence-parallel sampling): runs of rows [(first row of x, count, first cache row)]
         whose K/V go to every rank of the sequence-parallel group instead of the local cache only."""
-        cfg, p, ws = self.cfg, self.p, self.ws
+        cfg, p, ws = self.cfg, self.p, self.ws if ws is None else ws
         R, H = x.shape
         qd, kd = cfg.q_dim, cfg.kv_dim
         if self.offload is not None:
@@ -223,7 +225,7 @@ class InferenceEngine:
             else:
                 # the next layer's norm rides on the experts' combination when few rows are routed
                 gain = p[f"layers.{l + 1}.attn_norm"][branch] if static and R <= moe.FEW_ROWS and l + 1 < cfg.num_layers else None
-                x, normed = self._moe_ffn(WE, h2, x1, branch, xo[l & 1], gain, h1), gain is not None
+                x, normed = self._moe_ffn(WE, h2, x1, branch, xo[l & 1], gain, h1, ws), gain is not None
         return x
 
     def _one_launch(self, rows: int, keys: int) -> bool:
@@ -244,12 +246,12 @@ class InferenceEngine:
                                          cfg.num_kv_heads, cfg.ffn_size, plan, kv_rows, pos3, kv_len, self.inv_t, self.inv_hw,
                                          cfg.rms_eps, self.scale)
 
-    def _moe_ffn(self, W, h2, x1, branch, out, gain=None, h=None):
+    def _moe_ffn(self, W, h2, x1, branch, out, gain=None, h=None, ws: Optional[Workspace] = None):
         """Dropless top-k expert FFN of one branch: device-side routing, tokens gathered into expert
         segments, one grouped GEMM per projection, weighted combine + residual (the reference loops
         over experts in Python: src/sensenova_u1/models/neo_unify/modeling_qwen3_moe.py:51-119).  With ``gain`` the norm of
         the result goes to ``h`` as well."""
-        cfg, p, ws = self.cfg, self.p, self.ws
+        cfg, ws = self.cfg, self.ws if ws is None else ws
         br = "und" if branch == UND else "gen"
         K = cfg.num_experts_per_tok if branch == UND else cfg.gen_num_experts_per_tok
         R, H = h2.shape
@@ -341,7 +343,9 @@ class InferenceEngine:
         """Understanding-branch forward of a plan's new tokens: chunks of prompts, decode steps, or both.  ``ids`` [plan.rows] or
         ``embeds`` [plan.rows, H] are those of all sequences one after another, ``pos3`` their (t, h, w) indexes (default: text,
         at the tokens' places in their sequences).  Returns the hidden rows after the last layer, as :meth:`prefill` does for
-        the last ones.  May be captured in a CUDA graph that begins with ``plan.advance()``, with ``ids`` on the device."""
+        the last ones.  May be captured in a CUDA graph that begins with ``plan.advance()``, with ``ids`` on the device: the step's
+        buffers are then the graph's, so larger steps may run between replays, and graphs on several streams at once.  Other steps use the
+        engine's buffers, one after another."""
         if len(caches) != self.cfg.num_layers:
             raise ValueError(f"paged_step needs one cache per layer ({self.cfg.num_layers})")
         if (ids is None) == (embeds is None):
@@ -357,7 +361,9 @@ class InferenceEngine:
         if pos3 is None:
             pos = plan.positions()
             pos3 = torch.stack([pos, torch.zeros_like(pos), torch.zeros_like(pos)])
-        return self.layers(x, UND, pos3.to(self.dev).int().contiguous(), plan, None, 0, caches=caches).clone()
+        # a graph keeps the addresses that it was captured with, and the engine's buffers are replaced when a step needs larger ones
+        ws = Workspace(self.dev) if torch.cuda.is_current_stream_capturing() else None
+        return self.layers(x, UND, pos3.to(self.dev).int().contiguous(), plan, None, 0, caches=caches, ws=ws).clone()
 
     # ------------------------------------------------------------ text decoding
     def decode_greedy(self, layouts: List[DocLayout], last_hidden, max_new_tokens: int,

@@ -168,3 +168,19 @@ def test_rows_of_a_tile():
         assert [rows(n, fp8) for n in (1, 8, 9, 16, 25, 32)] == [8, 8, 16, 16, 32, 32]
     assert [rows(n, True) for n in (17, 24)] == [24, 24]
     assert [rows(n, False) for n in (17, 24)] == [32, 32] and [rows(n, False, 40000) for n in (16, 17, 24, 25)] == [16, 24, 24, 32]
+
+
+def test_a_captured_step_has_buffers_of_its_own(monkeypatch):
+    """The engine's buffers are replaced by larger ones; a graph must not have been captured with them."""
+    from types import SimpleNamespace
+    from sensenova_u1_b200.inference.engine import InferenceEngine
+    eng = InferenceEngine.__new__(InferenceEngine)
+    eng.cfg, eng.dev, eng.ws = SimpleNamespace(num_layers=1, hidden_size=8), torch.device("cpu"), object()
+    eng.p = {"embed_tokens": torch.zeros(4, 8, dtype=torch.bfloat16)}
+    used = []
+    eng.layers = lambda x, *a, ws=None, **k: (used.append(ws), x)[1]
+    plan = SimpleNamespace(rows=2, positions=lambda: torch.zeros(2, dtype=torch.int32))
+    for capturing in (False, True, True):
+        monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing)
+        eng.paged_step(plan, [None], ids=torch.tensor([1, 2]))
+    assert used[0] is None and used[1] is not None and used[2] is not None and len({id(x) for x in [*used, eng.ws]}) == 4

@@ -922,3 +922,54 @@ def test_equal_scores_of_any_size(q_len, size, dtype):
     want = rows[0][1][torch.arange(8, device="cuda") // 4, 300].expand(q_len, 8, D)
     out = paged.paged_attention(q, cache, plan, SCALE).double()
     assert ((out - want).abs() <= (2 * 2.0 ** -8 + 2.0 ** -11) * want.abs()).all()
+
+
+def test_a_captured_engine_step_outlives_larger_ones():
+    """Two captured decode steps; then a chunk larger than anything before, whose buffers replace the engine's, and tensors in whatever
+    memory that left free; then both graphs at once on two streams: they write nothing of that, and give what eager steps give."""
+    from sensenova_u1_b200.config import tiny_mot
+    from sensenova_u1_b200.inference.engine import InferenceEngine
+    from sensenova_u1_b200.models.params import ParamStore
+    from sensenova_u1_b200.ops import paged
+    for moe in ({}, dict(num_experts=8, num_experts_per_tok=2, gen_num_experts=8, gen_num_experts_per_tok=2, moe_intermediate_size=128)):
+        cfg = tiny_mot(head_dim=128, patch_size=16, num_layers=2, **moe)
+        store = ParamStore(cfg, device="cuda", with_grads=False)
+        store.init_weights(3, std=0.05)
+        eng = InferenceEngine(cfg, store)
+        sets = [eng.paged_caches(24, 32) for _ in range(2)]
+        g = torch.Generator().manual_seed(2)
+        jobs = []
+        for caches, n in zip(sets, (2, 5)):
+            tables, kv = [list(range(4 * i, 4 * i + 4)) for i in range(n)], [40 + 7 * i for i in range(n)]
+            prompt = paged.build_plan(caches[0], cfg.num_heads, kv, kv, tables)
+            eng.paged_step(prompt, caches, ids=torch.randint(8, cfg.vocab_size, (sum(kv),), generator=g))
+            plan = paged.build_plan(caches[0], cfg.num_heads, [1] * n, kv, tables, grow=3)
+            tok = torch.randint(8, cfg.vocab_size, (n,), generator=g).cuda()
+            out = torch.zeros(n, cfg.hidden_size, device="cuda", dtype=BF16)
+            plan.advance()
+            want = [eng.paged_step(plan, caches, ids=tok)]
+            plan.advance()
+            want.append(eng.paged_step(plan, caches, ids=tok))
+            plan.advance(-2)
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                plan.advance()
+                out.copy_(eng.paged_step(plan, caches, ids=tok))
+            jobs.append((graph, plan, tok, out, want, torch.cuda.Stream()))
+        large = eng.paged_caches(40, 32)
+        chunk = paged.build_plan(large[0], cfg.num_heads, [1200], [1200], [list(range(38))])
+        before = sum(t.numel() for t in eng.ws.bufs.values())
+        eng.paged_step(chunk, large, ids=torch.randint(8, cfg.vocab_size, (1200,), generator=g))
+        assert sum(t.numel() for t in eng.ws.bufs.values()) > before
+        torch.cuda.synchronize()
+        held = [torch.full((1 << s,), 77, dtype=torch.uint8, device="cuda") for s in range(9, 22) for _ in range(8)]
+        torch.cuda.synchronize()
+        for i in range(2):
+            for graph, _, _, _, _, stream in jobs:
+                with torch.cuda.stream(stream):
+                    graph.replay()
+            torch.cuda.synchronize()
+            for _, _, _, out, want, _ in jobs:
+                assert torch.equal(out, want[i])
+        assert all((x == 77).all() for x in held)
