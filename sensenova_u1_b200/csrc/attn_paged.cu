@@ -278,6 +278,7 @@ __global__ void __launch_bounds__(Few<FP8, NR, WR>::THREADS, Few<FP8, NR, WR>::C
   if (!a.beside) pdl_wait();
   pdl_trigger();
 
+  if (threadIdx.x == 0) report_grown(p, b, a.status);
   const int kv_len = seq_len(p, b);
   const int rows = min(M, q_len * G - row0);
   // the furthest key that a row of this tile may read, and the nearest limit

@@ -304,6 +304,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
       tma_load_3d(sQ + t * CTILE, &tm_q, q_full, 0, kvh * G, q0 + token0 + t * T);
       tma_load_3d(sQ + t * CTILE + CHALF, &tm_q, q_full, 64, kvh * G, q0 + token0 + t * T);
     }
+    report_grown(p, b, args.status);
   }
   const int kv_len = seq_len(p, b);
   int max_a, max_b, min_a, min_b;               // the largest and the smallest limit of row tiles A and B

@@ -64,6 +64,11 @@ __device__ __forceinline__ int tile_exponent(float top) {
 
 __device__ __forceinline__ int seq_len(const Plan& p, int b) { return max(0, min(p.kv_len[b], p.cap[b])); }
 
+// A sequence with new rows that has grown past what the plan has pages for: its rows are not those that the caller means.
+__device__ __forceinline__ void report_grown(const Plan& p, int b, int* status) {
+  if (p.kv_len[b] > p.cap[b]) report_status(status, kBadShape, 10);
+}
+
 // Keys that row ``token`` of a sequence may read.
 __device__ __forceinline__ int row_limit(const Plan& p, int q0, int q_len, int kv_len, int token) {
   const int behind = p.behind != nullptr ? p.behind[q0 + token] : q_len - 1 - token;

@@ -167,8 +167,9 @@ class PagedPlan:
         self._addr = ctypes.addressof(self._args)
 
     def advance(self, tokens: int = 1) -> None:
-        """Every sequence has ``tokens`` more (up to ``grow`` in all; beyond that nothing is written, and ``check_status`` raises):
-        its new rows are the ``q_len`` last ones of the longer sequence.  Runs on the device and may be captured; :func:`paged_read` keeps the lengths that the plan was made with."""
+        """Every sequence has ``tokens`` more (up to ``grow`` in all; beyond that nothing is written, attention reads up to the last
+        token that the plan has room for, and ``check_status`` raises after either): its new rows are the ``q_len`` last ones of the longer
+        sequence.  Runs on the device and may be captured; :func:`paged_read` keeps the lengths that the plan was made with."""
         self.kv_len.add_(tokens)
 
     def positions(self) -> torch.Tensor:

@@ -973,3 +973,18 @@ def test_a_captured_engine_step_outlives_larger_ones():
             for _, _, _, out, want, _ in jobs:
                 assert torch.equal(out, want[i])
         assert all((x == 77).all() for x in held)
+
+
+@pytest.mark.parametrize("q_len,dtype", [(1, BF16), (1, E4M3), (6, E4M3), (40, BF16), (40, E4M3), (300, E4M3)])      # every kernel
+def test_attention_past_the_plan_is_reported(q_len, dtype):
+    from sensenova_u1_b200.ops import _lib, paged
+    cache, tables, _ = make([400, 20], 32, 2, dtype)
+    q = torch.randn(q_len, 8, D, device="cuda", generator=gen(3)).to(BF16)
+    plan = paged.build_plan(cache, 8, [q_len, 0], [398, 20], tables, grow=2)       # a sequence without new rows does not grow
+    for n in range(3):
+        paged.paged_attention(q, cache, plan, SCALE)
+        _lib.check_status()
+        plan.advance()
+    paged.paged_attention(q, cache, plan, SCALE)
+    with pytest.raises(_lib.NativeLibraryError, match="limit"):
+        _lib.check_status()
