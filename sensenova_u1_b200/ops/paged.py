@@ -201,9 +201,17 @@ def _shares(tiles: np.ndarray, heads: int, slots: int, least: int) -> np.ndarray
     return -(-tiles // share)
 
 
+def _whole(what: str, x) -> np.ndarray:
+    """``x`` as int64; numbers that are not whole are refused, not cut."""
+    a = np.asarray(x)
+    if a.size and a.dtype.kind not in "iu":
+        raise ValueError(f"{what} must be whole numbers, not {a.dtype}")
+    return a.astype(np.int64, copy=False)
+
+
 def _lay_out(q_lens, kv_lens, tables, page: int, pages: int, group: int, kv_heads: int, fp8: bool, limits, grow: int):
     """Host side of :func:`build_plan`: checks, and every array of the plan as int32."""
-    q, kv = np.asarray(q_lens, dtype=np.int64).reshape(-1), np.asarray(kv_lens, dtype=np.int64).reshape(-1)
+    q, kv = _whole("lengths", q_lens).reshape(-1), _whole("lengths", kv_lens).reshape(-1)
     n = len(q)
     if len(kv) != n or (q < 0).any() or (kv < q).any() or grow < 0:
         raise ValueError("every sequence has q_len >= 0 new tokens among its kv_len >= q_len tokens, and grow >= 0")
@@ -217,12 +225,13 @@ def _lay_out(q_lens, kv_lens, tables, page: int, pages: int, group: int, kv_head
         if tables.is_cuda or tables.dim() != 2 or tables.is_floating_point():
             raise ValueError("page tables are lists of page numbers, or one host tensor [sequences, pages]")
         tables = tables.numpy()
+    whole = isinstance(tables, np.ndarray) and tables.dtype.kind in "iu"
     if len(tables) != n:
         raise ValueError("one page table per sequence")
     for i in range(n):
         if len(tables[i]) < need[i]:
             raise ValueError(f"sequence {i} needs {need[i]} pages for {cap[i]} tokens, its table has {len(tables[i])}")
-        table[i, :need[i]] = tables[i][:need[i]]
+        table[i, :need[i]] = tables[i][:need[i]] if whole else _whole("pages", tables[i][:need[i]])
     if n and (table.min() < 0 or table.max() >= pages):          # (places that are not needed hold 0)
         i = int(((table < 0) | (table >= pages)).any(1).argmax())
         raise ValueError(f"sequence {i} names a page that the cache does not have")
@@ -231,7 +240,7 @@ def _lay_out(q_lens, kv_lens, tables, page: int, pages: int, group: int, kv_head
     row_seq = np.repeat(np.arange(n, dtype=np.int32), q)
     behind = None
     if limits is not None:
-        lim = np.asarray(limits, dtype=np.int64).reshape(-1)
+        lim = _whole("limits", limits).reshape(-1)
         if grow:
             raise ValueError("limits are fixed: a plan with limits cannot grow")
         if len(lim) != rows or (lim < 0).any() or (lim > kv[row_seq]).any():

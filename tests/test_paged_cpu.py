@@ -184,3 +184,25 @@ def test_a_captured_step_has_buffers_of_its_own(monkeypatch):
         monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing)
         eng.paged_step(plan, [None], ids=torch.tensor([1, 2]))
     assert used[0] is None and used[1] is not None and used[2] is not None and len({id(x) for x in [*used, eng.ws]}) == 4
+
+
+@pytest.mark.parametrize("change", [dict(q=(1.0, 3)), dict(kv=(5, 40.5)), dict(kv=(5, float("nan"))), dict(tables=((0,), (1, 2.9, 3))), dict(limits=[5, 0, 40, 39.5]),
+                                    dict(tables=((0,), (1, 2, float("inf"))))])
+def test_numbers_that_are_not_whole_are_refused(change):
+    """(Not cut to whole ones: page 2.9 is not page 2.)"""
+    with pytest.raises(ValueError, match="whole"):
+        lay(**change)
+
+
+@pytest.mark.parametrize("tables", [np.array([[0, 0, 0], [1, 2.5, 3]]), torch.zeros(2, 3, dtype=torch.bool), [np.array([0.0]), np.array([1, 2, 3])]])
+def test_page_tables_that_are_not_whole_numbers(tables):
+    with pytest.raises(ValueError):
+        paged._lay_out([1, 3], [5, 40], tables, 16, 4, 4, 2, False, None, 0)
+
+
+def test_whole_numbers_of_any_type():
+    want, _ = lay(limits=[5, 0, 40, 39])
+    for kind in (np.int32, np.uint8, np.int64):
+        a, _ = paged._lay_out(np.array([1, 3], kind), torch.tensor([5, 40]), [np.array([0], kind), torch.tensor([1, 2, 3])], 16, 4, 4, 2, False,
+                              np.array([5, 0, 40, 39], kind), 0)
+        assert all(np.array_equal(a[n], want[n]) for n in ("q_start", "kv_len", "table", "behind"))
