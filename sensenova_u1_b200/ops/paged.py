@@ -370,7 +370,9 @@ def build_plan(cache: PagedCache, heads: int, q_lens, kv_lens, tables, limits=No
     sees the whole picture, has the picture's end as its limit.  ``grow``: tokens that :meth:`PagedPlan.advance` may add."""
     if heads < 1 or heads % cache.kv_heads != 0:
         raise ValueError("the number of query heads must be a multiple of the cache's heads")
-    if torch.cuda.is_current_stream_capturing():
+    with torch.cuda.device(cache.device):                     # (the stream that the copy below goes to)
+        capturing = torch.cuda.is_current_stream_capturing()
+    if capturing:
         raise RuntimeError("a plan is made before a CUDA graph is captured: the graph would copy from host memory that is gone")
     arrays, counts = _lay_out(q_lens, kv_lens, tables, cache.page, cache.pages, heads // cache.kv_heads, cache.kv_heads,
                               cache.scales is not None, limits, grow)

@@ -206,3 +206,30 @@ def test_whole_numbers_of_any_type():
         a, _ = paged._lay_out(np.array([1, 3], kind), torch.tensor([5, 40]), [np.array([0], kind), torch.tensor([1, 2, 3])], 16, 4, 4, 2, False,
                               np.array([5, 0, 40, 39], kind), 0)
         assert all(np.array_equal(a[n], want[n]) for n in ("q_start", "kv_len", "table", "behind"))
+
+
+def test_a_capture_on_the_cache_s_device_counts(monkeypatch):
+    """The plan's arrays go up on the current stream of the cache's device, whichever device is current."""
+    from types import SimpleNamespace
+    current = [0]
+
+    class Device:
+        def __init__(self, device):
+            self.index = torch.device(device).index
+
+        def __enter__(self):
+            self.before, current[0] = current[0], self.index
+
+        def __exit__(self, *a):
+            current[0] = self.before
+
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: current[0] == 1)
+    monkeypatch.setattr(paged, "_lay_out", lambda *a: (_ for _ in ()).throw(KeyError("laid out")))
+    cache = SimpleNamespace(kv_heads=1, device=torch.device("cuda:1"), page=16, pages=1, scales=None)
+    with pytest.raises(RuntimeError, match="captured"):
+        paged.build_plan(cache, 1, [1], [1], [[0]])
+    cache.device, current[0] = torch.device("cuda:0"), 1
+    with pytest.raises(KeyError):
+        paged.build_plan(cache, 1, [1], [1], [[0]])
+    assert current == [1]
