@@ -66,7 +66,9 @@ _ENTRY: dict = {}         # the entry points that calls go to
 def _library():
     """The library, its entry points told the types of their arguments (cheaper than an object per argument and call)."""
     lib = _lib.load()
-    if lib.snu1_paged_write.argtypes is None:
+    if not _ENTRY:
+        if lib.snu1_paged_plan_bytes() != ctypes.sizeof(_Args):
+            raise _lib.NativeLibraryError(f"{_lib.lib_path()} has plans of another size: build it again (python -m sensenova_u1_b200.build)")
         P, L, I = c_void_p, c_ll, c_int
         lib.snu1_paged_cache_init.argtypes = (P, P, P, I, I, I, I)
         lib.snu1_paged_read.argtypes = (P, P, P, P, P)

@@ -233,3 +233,16 @@ def test_a_capture_on_the_cache_s_device_counts(monkeypatch):
     with pytest.raises(KeyError):
         paged.build_plan(cache, 1, [1], [1], [[0]])
     assert current == [1]
+
+
+def test_a_library_with_plans_of_another_size_is_refused(monkeypatch):
+    from types import SimpleNamespace
+    from sensenova_u1_b200.ops import _lib
+    if _lib.available():
+        assert _lib.load().snu1_paged_plan_bytes() == paged.ctypes.sizeof(paged._Args)
+    old = SimpleNamespace(snu1_paged_plan_bytes=lambda: paged.ctypes.sizeof(paged._Args) - 8)
+    monkeypatch.setattr(paged, "_ENTRY", {})
+    monkeypatch.setattr(_lib, "load", lambda: old)
+    with pytest.raises(_lib.NativeLibraryError, match="build"):
+        paged._library()
+    assert not paged._ENTRY
