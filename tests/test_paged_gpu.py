@@ -988,3 +988,128 @@ def test_attention_past_the_plan_is_reported(q_len, dtype):
     paged.paged_attention(q, cache, plan, SCALE)
     with pytest.raises(_lib.NativeLibraryError, match="limit"):
         _lib.check_status()
+
+
+SIZES = [0.0, 2.0 ** -40, 1.0, 2.0 ** 8, 2.0 ** -40, 0.0, 1.0, 2.0 ** -20]
+
+
+@pytest.mark.parametrize("q_len,split", [(3, True), (40, True), (40, False), (300, True), (300, False)])
+@pytest.mark.parametrize("order", ["as they are", "backwards"])
+@pytest.mark.parametrize("k_sizes", [[1.0], [2.0 ** -30, 2.0, 0.0, 1.0, 0.25]])
+def test_tiles_of_very_different_sizes(q_len, split, order, k_sizes, monkeypatch):
+    """Tiles of 128 keys with values from 2^-40 to 2^8 or zeros, and keys that differ by tile; rows that read only the first of them."""
+    from sensenova_u1_b200.ops import paged
+    if not split:
+        monkeypatch.setattr(paged, "_waves", lambda tiles, heads, slots: tiles * 0 + 1)
+    kv, sizes = [300 + 128 * 8 - 50, 128 * 7 + 3], SIZES if order == "as they are" else SIZES[::-1]
+    q_lens, xs = [q_len, 2], []
+    for i, n in enumerate(kv):
+        tile = (torch.arange(n) // 128)
+        x = torch.randn(2, 2, n, D, device="cuda", generator=gen(i))
+        x[1] *= torch.tensor(sizes * 2)[tile].cuda()[:, None]
+        x[0] *= torch.tensor(k_sizes * 16)[tile].cuda()[:, None]
+        xs.append(x)
+    cache, tables, rows = filled(xs, 32)
+    lim = [1 + (i * 389) % n for n, k in zip(kv, q_lens) for i in range(k)]
+    lim[0], lim[1] = kv[0], 128
+    q = torch.randn(sum(q_lens), 8, D, device="cuda", generator=gen(7)).to(BF16)
+    for limits in (lim, None):
+        plan = paged.build_plan(cache, 8, q_lens, kv, tables, limits=limits)
+        ref, room = exact(q, q_lens, rows, causal(q_lens, kv) if limits is None else torch.tensor(lim, device="cuda"), E4M3)
+        out = paged.paged_attention(q, cache, plan, SCALE)
+        assert near(out, ref, room)
+
+
+@pytest.mark.parametrize("rows", [4, 8, 12, 16, 20, 24, 28, 32])
+def test_probabilities_of_few_bf16_rows_keep_sixteen_bits(rows):
+    """One-hot queries make scores exact, values of +1 and -1 make the result a difference of probabilities: each is off by 2^-16 of
+    itself (two bf16 numbers) and by 2^-20 (exponential and fp32 sums; scores below 2^3), and the result is rounded once."""
+    from sensenova_u1_b200.ops import paged
+    n = 37
+    g = gen(rows)
+    x = torch.zeros(3, 2, 1, 16, D, device="cuda", dtype=BF16)
+    k = torch.randn(n, D, device="cuda", generator=g).to(BF16)
+    v = torch.ones(n, D, device="cuda", dtype=BF16)
+    v[torch.rand(n, D, device="cuda", generator=g) < 0.5] = -1
+    table = [2, 0, 1]
+    for i in range(n):
+        x[table[i // 16], 0, 0, i % 16], x[table[i // 16], 1, 0, i % 16] = k[i], v[i]
+    cache = paged.PagedCache(x)
+    q = torch.zeros(rows // 4, 4, D, device="cuda", dtype=BF16)
+    q.view(rows, D)[torch.arange(rows), torch.arange(rows) * 3] = 1.0
+    plan = paged.build_plan(cache, 4, [rows // 4], [n], [table], limits=[n] * (rows // 4))
+    out = paged.paged_attention(q, cache, plan, 1.0).view(rows, D).double()
+    p = torch.softmax(k[:, torch.arange(rows) * 3].double().T, -1)
+    ref = p @ v.double()
+    assert ((out - ref).abs() <= 2.0 ** -16 + 2.0 ** -20 + 2.0 ** -8 * ref.abs()).all()
+
+
+def engine_and_oracle(dtype, **kw):
+    """A prompt with a picture through ``InferenceEngine.paged_step`` in three chunks (the picture whole in one) beside a decoding text,
+    and the oracle's layers in fp32 over the whole of both: hidden rows of both, and the routers' logits."""
+    from sensenova_u1_b200.config import tiny_mot
+    from sensenova_u1_b200.inference.engine import InferenceEngine
+    from sensenova_u1_b200.models import oracle
+    from sensenova_u1_b200.models.params import ParamStore
+    from sensenova_u1_b200.ops import paged
+    from sensenova_u1_b200.ops.attention import make_meta
+    cfg = tiny_mot(head_dim=128, patch_size=16, num_layers=2, **kw)
+    store = ParamStore(cfg, device="cuda", with_grads=False)
+    store.init_weights(5, std=0.05)
+    eng = InferenceEngine(cfg, store)
+    total, a, b, wide = [190, 33], 60, 60 + 8 * 9, 9          # the first: 60 tokens of text, a picture of 8 x 9, text again
+    g = gen(3)
+    embeds = [(torch.randn(n, cfg.hidden_size, device="cuda", generator=g) * 0.05).to(BF16) for n in total]
+    t = torch.arange(total[0])
+    t[a:b], t[b:] = a, a + 1 + torch.arange(total[0] - b)
+    h, w, img = torch.zeros_like(t), torch.zeros_like(t), torch.zeros_like(t)
+    h[a:b], w[a:b], img[a:b] = torch.arange(b - a) // wide, torch.arange(b - a) % wide, 1
+    pos3 = [torch.stack([t, h, w]), torch.stack([torch.arange(total[1]), torch.zeros(total[1]), torch.zeros(total[1])]).long()]
+    limits = [[b if a <= i < b else i + 1 for i in range(total[0])], list(range(1, total[1] + 1))]
+    tables, pages = tables_for(total, 32)
+    caches = eng.paged_caches(pages, 32, dtype)
+    got, at = [[], []], [0, 0]
+    for s in ([40, 31], [100, 1], [50, 1]):
+        pick = lambda x, d=0: torch.cat([x[i].narrow(d, at[i], s[i]) for i in range(2)], d)
+        plan = paged.build_plan(caches[0], cfg.num_heads, s, [x + n for x, n in zip(at, s)], tables,
+                                limits=[x for i in range(2) for x in limits[i][at[i]:at[i] + s[i]]])
+        out = eng.paged_step(plan, caches, embeds=pick(embeds), pos3=pick(pos3, 1))
+        for i in range(2):
+            got[i].append(out[sum(s[:i]):sum(s[:i + 1])].clone())
+            at[i] += s[i]
+    assert at == total
+    p32, want, logits = {k: v.float() for k, v in store.p.items()}, [], []
+    for i, n in enumerate(total):
+        x, pos = embeds[i].float(), pos3[i].cuda()
+        meta = make_meta(torch.zeros(n, device="cuda"), pos[0], img.cuda() if i == 0 else None)
+        aux = []
+        for l in range(cfg.num_layers):
+            x = oracle.decoder_layer(p32, l, x, torch.zeros(n, dtype=torch.bool, device="cuda"), pos, oracle.dense_mask(meta, meta), cfg, aux=aux)
+        want.append(x)
+        logits.append([u for u, _ in aux])
+    return [torch.cat(x).float() for x in got], want, logits
+
+
+@pytest.mark.parametrize("dtype", [BF16, E4M3])
+def test_engine_with_a_picture(dtype):
+    got, want, _ = engine_and_oracle(dtype)
+    for h, x in zip(got, want):
+        # the bounds of test_engine_in_chunks_and_captured_tokens
+        assert ((h - x).norm() / x.norm()).item() < 3e-2 + (0 if dtype == BF16 else 2.0 ** -4)
+
+
+@pytest.mark.parametrize("dtype", [BF16, E4M3])
+def test_engine_of_a_mixture_with_a_picture(dtype):
+    got, want, logits = engine_and_oracle(dtype, num_experts=8, num_experts_per_tok=2, gen_num_experts=8, gen_num_experts_per_tok=2,
+                                          moe_intermediate_size=128)
+    room = 5e-2 + (0 if dtype == BF16 else 2.0 ** -4)          # 5e-2: the bound of the engine's other test of a mixture
+    clears = 0
+    for h, x, layers in zip(got, want, logits):
+        # rows whose choice of experts is not near to another one: logits are off by the rows' error, room of their size, random in sign
+        clear = torch.ones(len(h), dtype=torch.bool, device="cuda")
+        for u in layers:
+            top = u.sort(-1, descending=True).values
+            clear &= top[:, 1] - top[:, 2] > 2 * room * u.std()
+        clears += int(clear.sum())
+        assert ((h - x)[clear].norm() / x[clear].norm()).item() < room
+    assert clears > sum(map(len, got)) // 5                     # (of normal logits half are that clear per layer, a quarter in both)
