@@ -33,7 +33,7 @@
 // Measured (32 / 8 heads unless said, of a measured copy bandwidth of 6456 GB/s): e4m3, 48 x 1 token over 32700 keys, 4 heads, 152 us,
 // 5.9 TB/s or 0.91; 24 x 1 over up to 4096 keys 23 us, 0.65, of which 6 are a launch's start and end and the join; one
 // conversation of 840 bf16 keys 6.3 us in a graph, 7.8 called one by one, latency alone.  8 x 5 tokens over up to 12000 bf16 keys 44 us,
-// 0.73.  From 16 rows on instructions count: e4m3 8 x 12000 keys 4 / 16 / 24 / 32 rows 37 / 47 / 61 / 86 us.
+// 0.73.  From 16 rows on instructions count: e4m3 8 x 12000 keys 4 / 16 / 24 / 32 rows 37 / 47 / 63 / 86 us.
 #include <math.h>
 #include <string.h>
 
@@ -51,8 +51,8 @@ constexpr int FEW_LD = 132;                               // a row of 128 values
 // Up to eight rows: their registers let three CTAs run on an SM, with two stages each instead of three.
 // SELF: a fifth warp asks for pages, except with 24 rows per warp.  Five warps of two CTAs are three in a quarter of the SM,
 // 168 registers each; four have 255, which 24 rows need, so there the warp that is the last to be done with a stage asks
-// for what goes there next.  (17 to 24 rows, 8 x 12000 keys: e4m3 61 us, as 2 x 2 groups of eight rows 85, each code then
-// widened by two warps; bf16 67 and 71.  32 rows as four groups per warp: 152 and 89.  Up to 16 rows without the fifth warp: 1 to 4 % slower.)
+// for what goes there next.  (17 to 24 rows, 8 x 12000 keys: e4m3 62 us, as 2 x 2 groups of eight rows 85, each code then
+// widened by two warps; bf16 71 and 75.  32 rows as four groups per warp: 152 and 89.  Up to 16 rows without the fifth warp: 1 to 4 % slower.)
 template <bool FP8, int NR, int WR>
 struct Few {
   static constexpr bool SMALL = NR * WR == 1, SELF = NR == 3;
@@ -760,7 +760,7 @@ __global__ void __launch_bounds__(Few<FP8, NR, WR>::THREADS, Few<FP8, NR, WR>::C
   if (a.beside) pdl_wait();
 }
 
-// Parts of the chunk kernel: a block per four rows of a key/value head, a warp per row.
+// Joins the parts of the chunk kernel, and of more than JOIN_ROWS few rows: a block per four rows of a key/value head, a warp per row.
 constexpr int JOIN_THREADS = 128;
 
 __global__ void __launch_bounds__(JOIN_THREADS) paged_join_kernel(const Plan p, const FewArgs a) {

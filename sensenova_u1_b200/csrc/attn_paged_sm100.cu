@@ -15,19 +15,19 @@
 //   softmax warps.
 // * The mask is one number per row, the keys that it may read; tiles that all rows read whole need no test.
 // * A work item is a part of the key tiles of two row tiles; unnormalised results of parts are joined by
-//   paged_merge_kernel.  ops/paged.py chooses the parts so that the waves of CTAs are full.
+//   paged_join_kernel.  ops/paged.py chooses the parts so that the waves of CTAs are full.
 // * Two warps that have nothing else to do clear values that are not finite (and rows behind the last token) in the bf16 tiles
 //   that some row may not read whole (widening does so for e4m3): a probability of zero does not hide them from the product.
 //   Rows that may read such a value give NaN, the others are as if it were not there.
 //
-// Measured (32 / 8 heads): bf16, 2 x 512 new tokens over 8300 keys 127 us in a graph, 1.06 PFLOP/s, 148 when called for a second on end
-// (the power limit takes the clocks down); a pair of tiles takes 1.78 us, 0.82 of the tensor cores' measured rate if all SMs were at
-// it (128 CTAs on 148 SMs), and a CTA 8 to 10 us to start and end.  e4m3, 4096 tokens at the end of 32001: 1.72 ms, 1.17 PFLOP/s, or 2.03 in
-// a loop.  Chunks of up to 256 rows over e4m3, 8 x 64 rows over 12000 keys: 86 us, 2.4 TB/s, 3100 clocks per tile of 128 rows.  Four warps
-// widen keys, four values, and two turn scales into factors two tiles ahead; with eight warps doing all three one after the
-// other it was 97.  Without the multiplications 80, without the exponentials 76, without both 71: what bounds it is each warp's own
-// chain.  Softmax warps without rows that only keep step made it 87, two places for P (so that its store need not wait for the
-// product before) 95.
+// Measured (32 / 8 heads): bf16, 2 x 512 new tokens over 8300 keys 138 us in a graph of 20 calls, 0.98 PFLOP/s, 146 to 153 when called for a
+// second on end (the power limit takes the clocks down); a pair of tiles takes 1.78 us, 0.82 of the tensor cores' measured rate if all SMs
+// were at it (128 CTAs on 148 SMs), and a CTA 8 to 10 us to start and end.  e4m3, 4096 tokens at the end of 32001: 1.73 ms, 1.16 PFLOP/s, or
+// 2.01 to 2.08 in a loop.  Chunks of up to 256 rows over e4m3, 8 x 64 rows over 12000 keys: 94 us, 2.2 TB/s, 3300 clocks per tile of 128 rows.
+// Four warps widen keys, four values, and two turn scales into factors two tiles ahead; with eight warps doing all three one after
+// the other it took 1.13 times as long.  Without the multiplications 0.93, without the exponentials 0.88, without both 0.83 of the time: what
+// bounds it is each warp's own chain.  Softmax warps without rows that only keep step made it 1.01, two places for P (so that its store need
+// not wait for the product before) 1.10 times as long.
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 #include <float.h>

@@ -3,7 +3,7 @@
 A :class:`PagedCache` holds the keys and values of one layer in pages of 16, 32, 64 or 128 tokens, as bf16 or as e4m3 codes with
 one fp32 scale per token and head (half the memory: 132 bytes of 256).  Codes are finite and scales not negative, as
 :func:`paged_write` leaves them; a row that holds a value that is not finite has NaN as its scale.  A sequence owns pages in any order; several sequences may
-read the same page (a shared prompt), only one may write it.
+read the same page (a shared prompt), only one may write it, and at one place of its table.
 
 One :class:`PagedPlan` describes a step: how many new tokens every sequence brings, how many tokens it has then, and its
 pages.  The plan is made once per step on the host and serves every layer::
@@ -40,20 +40,20 @@ KEY_TILE = 64            # keys of a stage of the kernel for few rows
 FEW_SLOTS = (444, 296)   # its CTAs that run at once: of up to eight rows three on each of 148 SMs, otherwise two
 FEW_LEAST = 4            # a part of a sequence has at least this many key tiles
 # 17 to 24 rows have a kernel of their own (else that for 32): e4m3 always, bf16 from so many key tiles per CTA on.  Us, 20 rows,
-# 32 / 8 heads, the former / the latter: e4m3 1 x 1000 keys 12.0 / 12.6, 8 x 12000 61 / 85; bf16 1 x 1000 12.7 / 11.3, 8 x 1000 16.0 / 15.0,
-# 8 x 12000 67.6 / 71.1, 24 x 4000 80 / 89.
+# 32 / 8 heads, the former / the latter: e4m3 1 x 1000 keys 11.3 / 11.8, 8 x 12000 62 / 85; bf16 1 x 1000 12.2 / 10.4, 8 x 1000 15.5 / 14.4,
+# 8 x 12000 70.7 / 74.6, 24 x 4000 84 / 88.
 FEW_24 = 16
 FEW_JOIN = 8             # up to so many rows the parts of few rows join themselves (JOIN_ROWS in attn_paged.cu)
 FEW_CLUSTER = 8          # up to so many parts are a cluster, if all sequences can have as many
 FEW_TILE = 32            # rows (new tokens x query heads of a group) of one CTA, at most
 # More rows of a sequence are a chunk.  Chunk kernel / few rows, us, 32 / 8 heads, sequences of 12000 keys: bf16 1 x 32 rows
-# 22 / 25, 8 x 32 75 / 72, 1 x 48 22 / 29, 8 x 48 77 / 134; e4m3 1 x 32 22 / 25, 8 x 32 85 / 86, 24 x 32 of 4000 keys 114 / 109, 8 x 32 of
-# 1000 20 / 16, 1 x 48 22 / 33, 8 x 48 86 / 155.
+# 21 / 23, 8 x 32 86 / 79, 1 x 48 24 / 27, 8 x 48 88 / 135; e4m3 1 x 32 22 / 24, 8 x 32 93 / 86, 24 x 32 of 4000 keys 120 / 108, 8 x 32 of
+# 1000 20 / 16, 1 x 48 22 / 32, 8 x 48 93 / 154.
 CHUNK_FROM = FEW_TILE
 CHUNK_TILE = 128         # keys of a tile of the kernel for chunks, and rows of a row tile
 # e4m3 chunks of up to so many rows are widened by the CTAs that read them, one row tile each; longer ones are widened once.
-# Us, the former / the latter: 8 sequences of 12000 keys, 128 rows 89 / 190, 256 154 / 209, 512 314 / 294; of 1000 keys 20 / 29, 22 / 32,
-# 41 / 34.
+# Us, the former / the latter: 8 sequences of 12000 keys, 128 rows 101 / 202, 256 177 / 234, 512 349 / 330; of 1000 keys 21 / 28, 22 / 32,
+# 42 / 34.
 ONE_MOST = 256
 CHUNK_SLOTS = 148        # its CTAs that run at once
 CHUNK_START = 5          # what starting and ending a CTA costs, in key tiles (1.8 us): 8 to 10 us from its start to its end
@@ -369,7 +369,7 @@ def build_plan(cache: PagedCache, heads: int, q_lens, kv_lens, tables, limits=No
     tokens, the new ones (which are its last) among them.  ``tables``: the pages of every sequence in order, as lists or as one
     host tensor [sequences, at least the pages needed].  ``limits``: for every new row, how many of its sequence's first keys it
     may read (0: none, its output is zeros); without it, every row reads up to itself.  A token of a picture, which
-    sees the whole picture, has the picture's end as its limit.  ``grow``: tokens that :meth:`PagedPlan.advance` may add."""
+    sees the whole picture, has the picture's end as its limit: the picture is then among the keys, written in this step or before.  ``grow``: tokens that :meth:`PagedPlan.advance` may add."""
     if heads < 1 or heads % cache.kv_heads != 0:
         raise ValueError("the number of query heads must be a multiple of the cache's heads")
     with torch.cuda.device(cache.device):                     # (the stream that the copy below goes to)
@@ -449,7 +449,7 @@ def paged_write(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, plan: Paged
 
 def paged_read(cache: PagedCache, plan: PagedPlan) -> tuple[torch.Tensor, torch.Tensor]:
     """The cached keys and values of the plan's sequences, one sequence after another: two tensors [plan.keys, kv_heads, 128] bf16
-    (e4m3: code times scale, rounded once)."""
+    (e4m3: code times scale in fp32, rounded to bf16)."""
     _check(cache, plan)
     k, v = torch.empty_like(plan._read), torch.empty_like(plan._read)
     if plan.keys:
@@ -463,11 +463,13 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, plan: PagedPlan, scale: 
     the last sequence are left as they are; ``out`` may be ``q``.  ``scale`` is positive.
 
     A row that may read a key or value that is not finite is NaN, in part or whole; other rows are as if it were not there.
-    What lies behind a sequence's last token or in pages of nobody does not matter.  Over e4m3
-    a key adds nothing to the output where its probability times the size of its value is below 2^-32 of the largest such
-    product.  Chunks (more than 32 rows per key/value head) over e4m3 hold 128 cached tokens' values of a head relative to the largest of them: values 2^27 times smaller than that
-    lose bits.  Where the largest value of another 128 tokens is 2^d times larger (less than 2^-80 counts as that), probabilities below
-    2^(d - 133) of the largest one are lost."""
+    What lies behind a sequence's last token or in pages of nobody does not matter.  Queries and scores may have any size as long as the
+    products of a query and a key and their sum stay within fp32; chunk rows with scores beyond 2^20 (log2 units) take a slow path.
+
+    Over e4m3 a key adds nothing to the output where its probability times the size of its value is below 2^-32 of the largest such
+    product.  Chunks (more than 32 rows per key/value head) over e4m3 hold 128 cached tokens' values of a head relative to the largest of
+    them (less than 2^-80 counts as that): values 2^27 times smaller than that lose bits.  Where the largest value of another 128 tokens is
+    2^d times larger, probabilities below 2^(d - 133) of the largest one are lost."""
     _check(cache, plan)
     ldq = _row_stride("q", q, plan, plan.heads)
     if out is None:
