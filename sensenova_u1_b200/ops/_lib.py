@@ -84,7 +84,8 @@ def error(name: str, rc: int) -> NativeLibraryError:
 
 
 _ROLE = {1: "TMA producer", 2: "MMA issuer (accumulator)", 3: "MMA issuer (operands)",
-         4: "epilogue", 5: "softmax", 6: "correction", 7: "peer flag", 8: "expert-parallel plan", 9: "paged cache", 10: "paged attention"}
+         4: "epilogue", 5: "softmax", 6: "correction", 7: "peer flag", 8: "expert-parallel plan", 9: "paged cache", 10: "paged attention", 11: "beam search",
+         12: "page tables"}
 
 
 def check_status() -> None:
