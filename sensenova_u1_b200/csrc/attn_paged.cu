@@ -232,14 +232,15 @@ __device__ __forceinline__ bool last_part(unsigned long long* flags, int part, i
   return *s_vote != 0;
 }
 
-// NR: groups of eight rows that a warp computes.  WR: sets of warps with other rows; the warps of a set take other keys.
-template <bool FP8, int NR, int WR>
+// NR: groups of eight rows that a warp computes.  WR: sets of warps with other rows; the warps of a set take other keys.  TAIL: keys from the
+// sequence's ``skip`` on, results always to scratch (attn_prefix_sm100.cu reads the keys before).
+template <bool FP8, int NR, int WR, bool TAIL>
 __global__ void __launch_bounds__(Few<FP8, NR, WR>::THREADS, Few<FP8, NR, WR>::CTAS)
     paged_few_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_constant__ CUtensorMap tm_scale, const Plan p,
                      const FewArgs a) {
   using F = Few<FP8, NR, WR>;
   constexpr int KT = F::KT, WK = FEW_WARPS / WR, M = 8 * NR * WR;
-  constexpr bool JOIN = M <= JOIN_ROWS;
+  constexpr bool JOIN = M <= JOIN_ROWS && !TAIL;
   constexpr int BLOCKS = KT / 16 / WK, NB = BLOCKS < 2 ? BLOCKS : 2;     // blocks of 16 keys of a warp, and how many at a time
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -269,9 +270,10 @@ __global__ void __launch_bounds__(Few<FP8, NR, WR>::THREADS, Few<FP8, NR, WR>::C
   }
   __syncthreads();
   // what the plan's host side has set, before the wait: no launch in front writes it
-  const int4 item = p.few[blockIdx.x];
+  const int4 item = (TAIL ? p.tail : p.few)[blockIdx.x];
   const int b = item.x, row0 = item.y, part = item.z & 0xffff, parts = item.z >> 16;
   const int head = blockIdx.y, G = p.group;
+  const int skip = TAIL ? p.skip[b] / KT : 0;                    // tiles
   const int q0 = p.q_start[b], q_len = p.q_start[b + 1] - q0;
   // Chunks in front (attn_paged_sm100.cu) have waited for all work before them when this kernel may start, and nothing that
   // they write is read here: it only has to end after them.
@@ -293,8 +295,8 @@ __global__ void __launch_bounds__(Few<FP8, NR, WR>::THREADS, Few<FP8, NR, WR>::C
     max_lim = __reduce_max_sync(0xffffffffu, max_lim);
     min_lim = __reduce_min_sync(0xffffffffu, min_lim);
   }
-  const int tiles = (max_lim + KT - 1) / KT;
-  const int j0 = (int)((long long)tiles * part / parts), j1 = (int)((long long)tiles * (part + 1) / parts);
+  const int tiles = max(0, (max_lim + KT - 1) / KT - skip);
+  const int j0 = skip + (int)((long long)tiles * part / parts), j1 = skip + (int)((long long)tiles * (part + 1) / parts);
   const int page_log = __ffs(p.page) - 1;
   const int bx_log = min(page_log, KT == 128 ? 7 : 6), bx = 1 << bx_log;      // rows of a box
   const int box_bytes = 2 * 128 << bx_log;
@@ -670,8 +672,8 @@ __global__ void __launch_bounds__(Few<FP8, NR, WR>::THREADS, Few<FP8, NR, WR>::C
         }
       }
     named_bar_sync(1, FEW_WARPS * 32);
-    const bool direct = item.w < 0;
-    const bool near = a.cluster > 1;
+    const bool direct = !TAIL && item.w < 0;
+    const bool near = !TAIL && a.cluster > 1;
     // a warp finishes one row at a time, four values per lane
     for (int row = warp; row < rows; row += FEW_WARPS) {
       const int w0 = row / (8 * NR) * WK, rr = row % (8 * NR);
@@ -725,7 +727,7 @@ __global__ void __launch_bounds__(Few<FP8, NR, WR>::THREADS, Few<FP8, NR, WR>::C
     while (globaltimer_ns() - t0 < 2000000ull) {
     }
   }
-  if (a.cluster > 1) {
+  if (!TAIL && a.cluster > 1) {
     __syncwarp();
     cluster_sync_all();
     if (warp < FEW_WARPS) {
@@ -774,9 +776,52 @@ __global__ void __launch_bounds__(JOIN_THREADS) paged_join_kernel(const Plan p, 
            a.o + (long long)(q0 + row / G) * a.ldo + (long long)(head * G + row % G) * HEAD);
 }
 
-template <bool FP8, int NR, int WR>
+// Joins what rows with shared tokens have of them and of their own: a warp per row and head.
+__global__ void __launch_bounds__(JOIN_THREADS) paged_share_join_kernel(const Plan p, const FewArgs a) {
+  const int i = blockIdx.x * (JOIN_THREADS / 32) + (threadIdx.x >> 5), head = blockIdx.y, lane = threadIdx.x & 31;
+  int4 e[2];
+  if (i < p.join_count) {
+    e[0] = p.joins[2 * i];
+    e[1] = p.joins[2 * i + 1];
+  }
+  pdl_wait();
+  pdl_trigger();
+  if (i >= p.join_count) return;
+  const long long at[2] = {(long long)e[0].z * a.heads + head, (long long)e[1].x * a.heads + head};
+  const long long step[2] = {(long long)PREFIX_ROWS * a.heads, (long long)e[1].z * a.heads};
+  const int parts[2] = {e[0].w, e[1].y};
+  float mt = -INFINITY;
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+    for (int s = lane; s < parts[k]; s += 32) mt = fmaxf(mt, __ldcg(&a.part_ml[at[k] + s * step[k]].x));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, o));
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+  float lt = 0.f;
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+#pragma unroll 4
+    for (int s = 0; s < parts[k]; ++s) {
+      const float2 ml = __ldcg(&a.part_ml[at[k] + s * step[k]]);
+      const float4 y = __ldcg(reinterpret_cast<const float4*>(a.part + (at[k] + s * step[k]) * HEAD) + lane);
+      if (ml.x == -INFINITY) continue;                           // nothing is written then
+      const float f = fast_exp2(ml.x - mt);
+      x.x += f * y.x;
+      x.y += f * y.y;
+      x.z += f * y.z;
+      x.w += f * y.w;
+      lt += f * ml.y;
+    }
+  const float inv = lt == 0.f ? 0.f : 1.f / lt;                  // a row without keys gives zeros
+  uint2 u;
+  u.x = pack_bf16x2(x.x * inv, x.y * inv);
+  u.y = pack_bf16x2(x.z * inv, x.w * inv);
+  *reinterpret_cast<uint2*>(a.o + (long long)e[0].x * a.ldo + (long long)(head * p.group + e[0].y) * HEAD + lane * 4) = u;
+}
+
+template <bool FP8, int NR, int WR, bool TAIL>
 static int launch_few(const Cache& c, const Plan& p, const FewArgs& a, cudaStream_t st) {
-  auto kernel = paged_few_kernel<FP8, NR, WR>;
+  auto kernel = paged_few_kernel<FP8, NR, WR, TAIL>;
   constexpr int SMEM = Few<FP8, NR, WR>::SMEM;
   int dev = 0;
   SNU1_CUDA_CHECK(cudaGetDevice(&dev));
@@ -795,7 +840,7 @@ static int launch_few(const Cache& c, const Plan& p, const FewArgs& a, cudaStrea
   attr[1].val.clusterDim.x = a.cluster;
   attr[1].val.clusterDim.y = 1;
   attr[1].val.clusterDim.z = 1;
-  cfg.gridDim = dim3(p.few_count, c.heads);
+  cfg.gridDim = dim3(TAIL ? p.tail_count : p.few_count, c.heads);
   cfg.blockDim = dim3(Few<FP8, NR, WR>::THREADS);
   cfg.dynamicSmemBytes = SMEM;
   cfg.stream = st;
@@ -808,11 +853,21 @@ static int launch_few(const Cache& c, const Plan& p, const FewArgs& a, cudaStrea
 template <bool FP8>
 static int launch_few(const Cache& c, const Plan& p, const FewArgs& a, cudaStream_t st) {
   switch (p.few_rows) {
-    case 8: return launch_few<FP8, 1, 1>(c, p, a, st);
-    case 16: return launch_few<FP8, 2, 1>(c, p, a, st);
-    case 24: return launch_few<FP8, 3, 1>(c, p, a, st);
-    case 32: return launch_few<FP8, 2, 2>(c, p, a, st);
+    case 8: return launch_few<FP8, 1, 1, false>(c, p, a, st);
+    case 16: return launch_few<FP8, 2, 1, false>(c, p, a, st);
+    case 24: return launch_few<FP8, 3, 1, false>(c, p, a, st);
+    case 32: return launch_few<FP8, 2, 2, false>(c, p, a, st);
     default: set_last_error("paged_attention: no kernel for %d rows", p.few_rows); return kHostBadArg;
+  }
+}
+
+template <bool FP8>
+static int launch_tail(const Cache& c, const Plan& p, const FewArgs& a, cudaStream_t st) {
+  switch (p.tail_rows) {
+    case 8: return launch_few<FP8, 1, 1, true>(c, p, a, st);
+    case 16: return launch_few<FP8, 2, 1, true>(c, p, a, st);
+    case 32: return launch_few<FP8, 2, 2, true>(c, p, a, st);
+    default: set_last_error("paged_attention: no kernel for tails of %d rows", p.tail_rows); return kHostBadArg;
   }
 }
 
@@ -873,6 +928,15 @@ SNU1_API int snu1_paged_attention(const void* cache, const void* plan, const voi
     if (c.fp8) rc = launch_few<true>(c, p, a, st);
     else rc = launch_few<false>(c, p, a, st);
     if (rc != kHostOk) return rc;
+  }
+  if (p.prefix_count > 0) {
+    // these run beside the launch in front, if there is one of this call (see ``beside`` in paged_few_kernel), and beside each other
+    if ((rc = launch_prefix(c, p, q, ldq, a.part, a.part_ml, a.scale_log2, a.beside || p.few_count > 0, st)) != kHostOk) return rc;
+    a.beside = 1;
+    a.cluster = 1;
+    if ((rc = c.fp8 ? launch_tail<true>(c, p, a, st) : launch_tail<false>(c, p, a, st)) != kHostOk) return rc;
+    SNU1_CUDA_CHECK(launch_pdl(paged_share_join_kernel, dim3((p.join_count + JOIN_THREADS / 32 - 1) / (JOIN_THREADS / 32), c.heads),
+                               dim3(JOIN_THREADS), 0, st, p, a));
   }
   if (p.merge_count > 0)
     SNU1_CUDA_CHECK(launch_pdl(paged_join_kernel, dim3(p.merge_count, c.heads), dim3(JOIN_THREADS), 0, st, p, a));

@@ -15,6 +15,7 @@ namespace snu1 {
 namespace paged {
 
 constexpr int HEAD = 128;                  // width of a head
+constexpr int PREFIX_ROWS = 64;            // rows of a work item on shared tokens
 constexpr float E4M3_MAX = 448.f;
 constexpr float TINY = 7.70371977754894342e-34f;   // 2^-110, least row maximum that a scale is made of: 448 / TINY is finite
 
@@ -30,7 +31,7 @@ struct alignas(64) Cache {
   int pages, heads, page, fp8;
 };
 
-constexpr int PLAN_LAYOUT = 0x70670002;
+constexpr int PLAN_LAYOUT = 0x70670003;
 
 // Device arrays and counts of a plan (ops/paged.py builds it).
 struct Plan {
@@ -48,9 +49,15 @@ struct Plan {
   const int4* chunk;       // [chunk_count] the same for chunks
   const int4* one;         // [one_count] the same for e4m3 chunks of one row tile per CTA
   const int4* merge;       // [merge_count] up to four rows to join: sequence, first row, parts | rows << 12 | rows of a part << 16, first partial row
+  const int* skip;         // [seqs] tokens of a sequence that its run shares (a multiple of 128); the tail kernel leaves them out
+  const int4* runs;        // runs of sequences with the same first tokens: first row, rows, sequence whose table is read, shared tokens
+  const int4* prefix;      // [prefix_count] work on shared tokens: run, first of up to PREFIX_ROWS rows (x heads of a group), part | parts << 16, partial row
+  const int4* tail;        // [tail_count] work on the other tokens of such sequences, as ``few``
+  const int4* joins;       // [2 x join_count] row, head of the group, partial row of the shared tokens' part 0, parts | partial row of its tail, parts, rows of a part, -
   int seqs, rows, width, page, group;
   int read_count, few_count, few_rows, few_parts, few_cluster, chunk_count, one_count, merge_count;
   int partial_rows;        // rows of the scratch for partial results (x heads)
+  int prefix_count, tail_count, tail_rows, join_count;
   int unpack_count;        // also the 128-token pages of the scratch for unpacked rows
   int layout;              // PLAN_LAYOUT; changes with the fields
 };
@@ -117,6 +124,9 @@ int launch_widen(const Cache& c, const Plan& p, void* wide, float4* factors, cud
 // attn_paged_sm100.cu: a plan's ``one`` and ``chunk`` items
 int launch_chunks(const Cache& c, const Plan& p, const void* q, long long ldq, void* o, long long ldo, float* part,
                   float2* part_ml, float scale_log2, void* wide, const float4* factors, cudaStream_t st);
+// attn_prefix_sm100.cu: a plan's ``prefix`` items
+int launch_prefix(const Cache& c, const Plan& p, const void* q, long long ldq, float* part, float2* part_ml, float scale_log2, int beside,
+                  cudaStream_t st);
 
 }  // namespace paged
 }  // namespace snu1

@@ -58,6 +58,9 @@ ONE_MOST = 256
 CHUNK_SLOTS = 148        # its CTAs that run at once
 CHUNK_START = 5          # what starting and ending a CTA costs, in key tiles (1.8 us): 8 to 10 us from its start to its end
 CHUNK_JOIN = 3           # what a part costs besides: 128 KB written and read again
+PREFIX_ROWS = 64         # rows of a CTA of the kernel for shared tokens, which are counted in tiles of 128
+PREFIX_SLOTS = 148       # its CTAs that run at once
+PREFIX_LEAST = 2         # a part has at least this many key tiles
 
 
 _ENTRY: dict = {}         # the entry points that calls go to
@@ -127,15 +130,16 @@ class PagedCache:
         return self._data.device
 
 
-PLAN_LAYOUT = 0x70670002     # last word of a plan: the library refuses one whose fields lie elsewhere
+PLAN_LAYOUT = 0x70670003     # last word of a plan: the library refuses one whose fields lie elsewhere
 
 
 class _Args(ctypes.Structure):
     """``Plan`` of csrc/paged.cuh."""
     _fields_ = ([(n, c_void_p) for n in ("q_start", "kv_len", "cap", "table", "behind", "row_seq", "k_start", "read_pages", "unpack",
-                                         "unpack_first", "few", "chunk", "one", "merge")]
+                                         "unpack_first", "few", "chunk", "one", "merge", "skip", "runs", "prefix", "tail", "joins")]
                 + [(n, c_int) for n in ("seqs", "rows", "width", "page", "group", "read_count", "few_count", "few_rows", "few_parts", "few_cluster",
-                                        "chunk_count", "one_count", "merge_count", "partial_rows", "unpack_count", "layout")])
+                                        "chunk_count", "one_count", "merge_count", "partial_rows", "prefix_count", "tail_count", "tail_rows", "join_count",
+                                        "unpack_count", "layout")])
 
 
 @dataclass
@@ -158,6 +162,7 @@ class PagedPlan:
     _args: _Args = field(repr=False)
     _rows: torch.Tensor = field(repr=False)       # sequence of every row
     _ends: torch.Tensor = field(repr=False)       # row behind the last of every sequence
+    tables: object = field(default=None, repr=False)      # the PageTables that it reads
 
     def __post_init__(self):
         self._index = self.device.index
@@ -172,6 +177,8 @@ class PagedPlan:
         """Every sequence has ``tokens`` more (up to ``grow`` in all; beyond that nothing is written, attention reads up to the last
         token that the plan has room for, and ``check_status`` raises after either): its new rows are the ``q_len`` last ones of the longer
         sequence.  Runs on the device and may be captured; :func:`paged_read` keeps the lengths that the plan was made with."""
+        if self.tables is not None:
+            raise RuntimeError("the lengths are those of the plan's tables: their step() moves them on")
         self.kv_len.add_(tokens)
 
     def positions(self) -> torch.Tensor:
@@ -211,8 +218,33 @@ def _whole(what: str, x) -> np.ndarray:
     return a.astype(np.int64, copy=False)
 
 
-def _lay_out(q_lens, kv_lens, tables, page: int, pages: int, group: int, kv_heads: int, fp8: bool, limits, grow: int):
-    """Host side of :func:`build_plan`: checks, and every array of the plan as int32."""
+def _shared_runs(shared, n: int, q, kv, few, table, page: int):
+    """Which sequences read their first tokens together: runs [first sequence, sequences, tokens] of sequences with few rows, tokens in whole
+    tiles of 128, and the tokens that each sequence leaves to its run."""
+    skip, runs, taken = np.zeros(n, dtype=np.int64), [], np.zeros(n, dtype=bool)
+    for entry in shared:
+        first, count, tokens = (int(x) for x in _whole("shared", entry).reshape(3))
+        if first < 0 or count < 1 or first + count > n or tokens < 0 or taken[first:first + count].any():
+            raise ValueError("shared names sequences [first, how many, shared tokens], each at most once")
+        taken[first:first + count] = True
+        if (kv[first:first + count] < tokens).any():
+            raise ValueError("a sequence has fewer tokens than it shares")
+        tokens = tokens // CHUNK_TILE * CHUNK_TILE
+        if table is not None and (table[first:first + count, :tokens // page] != table[first, :tokens // page]).any():
+            raise ValueError("sequences that share tokens must have them in the same pages")
+        start = first
+        for i in range(first, first + count + 1):             # a chunk reads its keys itself
+            if i < first + count and (few[i] or q[i] == 0):
+                continue
+            if tokens and (q[start:i] > 0).sum() > 1:
+                runs.append((start, i - start, tokens))
+                skip[start:i] = np.where(q[start:i] > 0, tokens, 0)
+            start = i + 1
+    return runs, skip
+
+
+def _lay_out(q_lens, kv_lens, tables, page: int, pages: int, group: int, kv_heads: int, fp8: bool, limits, grow: int, shared=()):
+    """Host side of :func:`build_plan`: checks, and every array of the plan as int32.  ``tables`` may be the number of pages of a table on the device."""
     q, kv = _whole("lengths", q_lens).reshape(-1), _whole("lengths", kv_lens).reshape(-1)
     n = len(q)
     if len(kv) != n or (q < 0).any() or (kv < q).any() or grow < 0:
@@ -222,7 +254,12 @@ def _lay_out(q_lens, kv_lens, tables, page: int, pages: int, group: int, kv_head
     cap = np.where(q > 0, kv + grow, kv)
     need = -(-cap // page)
     width = max(1, int(need.max()) if n else 1)
-    table = np.zeros((n, width), dtype=np.int64)
+    on_device = isinstance(tables, int)
+    if on_device:
+        if width > tables:
+            raise ValueError(f"a sequence has up to {cap.max()} tokens, the tables have room for {tables * page}")
+        width, tables = tables, [()] * n
+    table = np.zeros((n, 0 if on_device else width), dtype=np.int64)
     if isinstance(tables, torch.Tensor):
         if tables.is_cuda or tables.dim() != 2 or tables.is_floating_point():
             raise ValueError("page tables are lists of page numbers, or one host tensor [sequences, pages]")
@@ -230,11 +267,11 @@ def _lay_out(q_lens, kv_lens, tables, page: int, pages: int, group: int, kv_head
     whole = isinstance(tables, np.ndarray) and tables.dtype.kind in "iu"
     if len(tables) != n:
         raise ValueError("one page table per sequence")
-    for i in range(n):
+    for i in range(0 if on_device else n):
         if len(tables[i]) < need[i]:
             raise ValueError(f"sequence {i} needs {need[i]} pages for {cap[i]} tokens, its table has {len(tables[i])}")
         table[i, :need[i]] = tables[i][:need[i]] if whole else _whole("pages", tables[i][:need[i]])
-    if n and (table.min() < 0 or table.max() >= pages):          # (places that are not needed hold 0)
+    if table.size and (table.min() < 0 or table.max() >= pages):          # (places that are not needed hold 0)
         i = int(((table < 0) | (table >= pages)).any(1).argmax())
         raise ValueError(f"sequence {i} names a page that the cache does not have")
     table = table.astype(np.int32)
@@ -254,7 +291,8 @@ def _lay_out(q_lens, kv_lens, tables, page: int, pages: int, group: int, kv_head
     # attention: tiles of rows, split over keys
     q_rows = q * group
     chunked = (q_rows > CHUNK_FROM) & (group <= CHUNK_TILE)
-    few_q = np.where(chunked, 0, q_rows)
+    runs, skip = _shared_runs(shared, n, q, kv, (q_rows > 0) & (q_rows <= FEW_TILE) & ~chunked, None if on_device else table, page)
+    few_q = np.where(chunked | (skip > 0), 0, q_rows)
     top = int(few_q.max()) if n else 0
     few_rows = 8 if top <= 8 else 16 if top <= 16 else FEW_TILE
     if 16 < top <= 24 and (fp8 or int((-(-cap[few_q > 0] // KEY_TILE)).sum()) * kv_heads >= FEW_24 * FEW_SLOTS[1]):
@@ -298,17 +336,79 @@ def _lay_out(q_lens, kv_lens, tables, page: int, pages: int, group: int, kv_head
     one, partial = chunks_of(single, tile_rows, partial)
     chunk, partial = chunks_of(chunked & ~single, 2 * tile_rows, partial)
     merge = np.concatenate(merge) if merge else np.zeros((0, 4), np.int32)
+    together = dict(skip=None, runs=None, prefix=None, tail=None, joins=None)
+    tail_rows = 0
+    if runs:
+        together, tail_rows, partial = _together(runs, skip, q_rows, cap, start(q), group, kv_heads, partial)
     unpack = unpack_first = None
     if fp8 and len(chunk):
         wide = np.where(chunked & ~single, -(-cap // CHUNK_TILE), 0)    # 128-token pages
         unpack, unpack_first = pages_of(wide), start(wide)[:n]
     arrays = dict(q_start=start(q), kv_len=kv.astype(np.int32), cap=cap.astype(np.int32), table=table, behind=behind, row_seq=row_seq,
                   k_start=start(kv), read_pages=pages_of(read), unpack=unpack, unpack_first=unpack_first, few=few, chunk=chunk,
-                  one=one, merge=merge)
+                  one=one, merge=merge, **together)
+    if on_device:
+        arrays["table"] = arrays["kv_len"] = None
     counts = dict(seqs=n, rows=rows, width=width, page=page, group=group, read_count=int(read.sum()), few_count=len(few),
                   few_rows=few_rows, few_parts=few_parts, few_cluster=cluster, chunk_count=len(chunk), one_count=len(one), merge_count=len(merge),
-                  partial_rows=partial, unpack_count=0 if unpack is None else len(unpack), layout=PLAN_LAYOUT)
+                  partial_rows=partial, prefix_count=len(together["prefix"]) if runs else 0, tail_count=len(together["tail"]) if runs else 0,
+                  tail_rows=tail_rows, join_count=len(together["joins"]) // 2 if runs else 0, unpack_count=0 if unpack is None else len(unpack), layout=PLAN_LAYOUT)
     return arrays, counts
+
+
+def _together(runs, skip, q_rows, cap, q_start, group: int, heads: int, first: int):
+    """Work on tokens that runs of sequences share (prefix, by runs), on the other tokens of these sequences (tail), and the joins of both,
+    [row, head of the group, partial row, parts | partial row, parts, rows of a part, 0] for every row."""
+    run_rows = np.array([int(q_rows[a:a + n].sum()) for a, n, _ in runs])
+    run_skip = np.array([t for _, _, t in runs])
+    count = -(-run_rows // PREFIX_ROWS)
+    run = np.repeat(np.arange(len(runs)), count)
+    row0 = (np.arange(len(run)) - np.repeat(np.cumsum(count) - count, count)) * PREFIX_ROWS
+    tiles = run_skip[run] // CHUNK_TILE
+    own = np.where(skip > 0, cap - skip, 0)
+    # SMs by what there is to read
+    share = PREFIX_SLOTS * float(tiles.sum()) / float(tiles.sum() + own.sum() / CHUNK_TILE)
+    parts = _shares(tiles, heads, max(heads * len(tiles), int(share)), PREFIX_LEAST)
+    at = first + np.cumsum(parts * PREFIX_ROWS) - parts * PREFIX_ROWS
+    first += int((parts * PREFIX_ROWS).sum())
+    i = np.repeat(np.arange(len(run)), parts)
+    part = np.arange(len(i)) - np.repeat(np.cumsum(parts) - parts, parts)
+    prefix = np.stack([run[i], row0[i], part | parts[i] << 16, at[i] + part * PREFIX_ROWS], 1)
+    # every row of a run: partial rows of its part 0, and parts
+    seqs = np.concatenate([np.arange(a, a + n) for a, n, _ in runs])
+    of_run = np.repeat(np.arange(len(runs)), run_rows)
+    place = np.arange(len(of_run)) - np.repeat(np.cumsum(run_rows) - run_rows, run_rows)
+    item = (np.cumsum(count) - count)[of_run] + place // PREFIX_ROWS
+    joins = np.zeros((len(of_run), 8), dtype=np.int64)
+    joins[:, 0] = np.repeat([q_start[a] for a, _, _ in runs], run_rows) + place // group
+    joins[:, 1] = place % group
+    joins[:, 2] = at[item] + place % PREFIX_ROWS
+    joins[:, 3] = parts[item]
+    # tails
+    rows = q_rows[seqs]
+    top = int(rows.max())
+    m = 8 if top <= 8 else 16 if top <= 16 else FEW_TILE
+    count = -(-rows // m)
+    seq = np.repeat(seqs, count)
+    row0 = (np.arange(len(seq)) - np.repeat(np.cumsum(count) - count, count)) * m
+    tiles = -(-(cap - skip)[seq] // KEY_TILE)
+    slots = FEW_SLOTS[m > 8] * max(8, PREFIX_SLOTS - len(prefix) * heads) // PREFIX_SLOTS
+    parts = _shares(tiles, heads, slots, FEW_LEAST)
+    at = first + np.cumsum(parts * m) - parts * m
+    first += int((parts * m).sum())
+    i = np.repeat(np.arange(len(seq)), parts)
+    part = np.arange(len(i)) - np.repeat(np.cumsum(parts) - parts, parts)
+    tail = np.stack([seq[i], row0[i], part | parts[i] << 16, at[i] + part * m], 1)
+    order = np.argsort(-(tiles[i] / parts[i]), kind="stable")
+    of_seq = np.repeat(np.arange(len(seqs)), rows)
+    place = np.arange(len(of_seq)) - np.repeat(np.cumsum(rows) - rows, rows)
+    item = (np.cumsum(count) - count)[of_seq] + place // m
+    joins[:, 4] = at[item] + place % m
+    joins[:, 5] = parts[item]
+    joins[:, 6] = m
+    of = np.array([[q_start[a], q_start[a + n] - q_start[a], a, t] for a, n, t in runs])
+    return (dict(skip=skip.astype(np.int32), runs=of.astype(np.int32), prefix=prefix.astype(np.int32), tail=tail[order].astype(np.int32),
+                 joins=joins.reshape(-1, 4).astype(np.int32)), m, first)
 
 
 def _waves(tiles: np.ndarray, heads: int, slots: int) -> np.ndarray:
@@ -362,22 +462,36 @@ def _items(seq, row0, tiles, parts, q_rows, m: int, first: int):
     return items[order].astype(np.int32), merge.astype(np.int32), int(first + np.where(split, parts * m, 0).sum())
 
 
-def build_plan(cache: PagedCache, heads: int, q_lens, kv_lens, tables, limits=None, grow: int = 0) -> PagedPlan:
+def build_plan(cache: PagedCache, heads: int, q_lens, kv_lens, tables, limits=None, grow: int = 0, shared=()) -> PagedPlan:
     """Plan of one step, for ``cache`` and every other cache of its geometry on the same device.
 
     ``heads``: query heads, a multiple of the cache's.  ``q_lens`` / ``kv_lens``: new tokens of every sequence, and all its
     tokens, the new ones (which are its last) among them.  ``tables``: the pages of every sequence in order, as lists or as one
     host tensor [sequences, at least the pages needed].  ``limits``: for every new row, how many of its sequence's first keys it
     may read (0: none, its output is zeros); without it, every row reads up to itself.  A token of a picture, which
-    sees the whole picture, has the picture's end as its limit: the picture is then among the keys, written in this step or before.  ``grow``: tokens that :meth:`PagedPlan.advance` may add."""
+    sees the whole picture, has the picture's end as its limit: the picture is then among the keys, written in this step or before.  ``grow``: tokens that :meth:`PagedPlan.advance` may add.
+
+    ``tables`` may be a :class:`~.page_tables.PageTables` of as many sequences: the plan then reads its tables and lengths as they are when a call
+    runs, ``kv_lens`` and ``grow`` say up to how many tokens they go, and its ``step`` stands in for ``advance``.
+
+    ``shared``: [first sequence, how many, tokens] of sequences that begin with the same tokens in the same pages.  Attention
+    reads those once for all of them (in tiles of 128 tokens; the rest, and the keys of chunks, are read by each sequence)."""
     if heads < 1 or heads % cache.kv_heads != 0:
         raise ValueError("the number of query heads must be a multiple of the cache's heads")
     with torch.cuda.device(cache.device):                     # (the stream that the copy below goes to)
         capturing = torch.cuda.is_current_stream_capturing()
     if capturing:
         raise RuntimeError("a plan is made before a CUDA graph is captured: the graph would copy from host memory that is gone")
+    from .page_tables import PageTables
+    live = tables if isinstance(tables, PageTables) else None
+    if live is not None:
+        if live.page != cache.page or live.pages > cache.pages or live.device != cache.device:
+            raise ValueError("the tables are of caches of another page size, size or device")
+        if live.seqs != len(q_lens):
+            raise ValueError(f"the tables have {live.seqs} sequences")
+        tables = live.width
     arrays, counts = _lay_out(q_lens, kv_lens, tables, cache.page, cache.pages, heads // cache.kv_heads, cache.kv_heads,
-                              cache.scales is not None, limits, grow)
+                              cache.scales is not None, limits, grow, shared)
     # all arrays in one copy from pinned memory that nothing waits for
     at, total = {}, 0
     for name, a in arrays.items():
@@ -389,14 +503,20 @@ def build_plan(cache: PagedCache, heads: int, q_lens, kv_lens, tables, limits=No
     for name, o in at.items():
         flat[o:o + arrays[name].size] = arrays[name].reshape(-1)
     store = host.to(cache.device, non_blocking=True)
-    args = _Args(**{name: store.data_ptr() + 4 * o for name, o in at.items()}, **counts)
+    fields = {name: store.data_ptr() + 4 * o for name, o in at.items()}
     n = counts["seqs"]
+    if live is None:
+        kv_len = store[at["kv_len"]:at["kv_len"] + n]
+    else:
+        kv_len = live.lens
+        fields |= dict(table=live.table.data_ptr(), kv_len=live.lens.data_ptr())
+    args = _Args(**fields, **counts)
     joined = counts["partial_rows"] * cache.kv_heads
     scratch = joined * HEAD_DIM * 4 + (joined + counts["few_parts"] * cache.kv_heads + 15) // 16 * 128 + counts["unpack_count"] * cache.kv_heads * (2 * CHUNK_TILE * HEAD_DIM * 2 + 16)
     return PagedPlan(heads, cache.kv_heads, cache.page, cache.pages, cache.data.dtype, cache.device,
                      [int(x) for x in q_lens], [int(x) for x in kv_lens],
-                     counts["rows"], int(arrays["k_start"][-1]), scratch, store[at["kv_len"]:at["kv_len"] + n], grow, store, args,
-                     store[at["row_seq"]:at["row_seq"] + counts["rows"]], store[at["q_start"] + 1:at["q_start"] + 1 + n])
+                     counts["rows"], int(arrays["k_start"][-1]), scratch, kv_len, grow, store, args,
+                     store[at["row_seq"]:at["row_seq"] + counts["rows"]], store[at["q_start"] + 1:at["q_start"] + 1 + n], live)
 
 
 _BF16 = torch.bfloat16
