@@ -788,7 +788,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) paged_share_join_kernel(const Pl
   pdl_trigger();
   if (i >= p.join_count) return;
   const long long at[2] = {(long long)e[0].z * a.heads + head, (long long)e[1].x * a.heads + head};
-  const long long step[2] = {(long long)PREFIX_ROWS * a.heads, (long long)e[1].z * a.heads};
+  const long long step[2] = {(long long)e[1].w * a.heads, (long long)e[1].z * a.heads};
   const int parts[2] = {e[0].w, e[1].y};
   float mt = -INFINITY;
 #pragma unroll
@@ -924,15 +924,32 @@ SNU1_API int snu1_paged_attention(const void* cache, const void* plan, const voi
     if (c.fp8 && p.chunk_count > 0 && (rc = launch_widen(c, p, wide, factors, st)) != kHostOk) return rc;
     if ((rc = launch_chunks(c, p, q, ldq, o, ldo, a.part, a.part_ml, a.scale_log2, wide, factors, st)) != kHostOk) return rc;
   }
+  if (p.many_count > 0) {                  // the products of many rows are long: in front of what runs beside
+    Plan r = p;
+    r.q_start = p.run_start;
+    r.kv_len = r.cap = p.run_len;
+    r.own_q_start = p.q_start;
+    r.own_kv_len = p.kv_len;
+    r.own_cap = p.cap;
+    (c.fp8 ? r.one : r.chunk) = p.many;
+    r.one_count = c.fp8 ? p.many_count : 0;
+    r.chunk_count = c.fp8 ? 0 : p.many_count;
+    if ((rc = launch_chunks(c, r, q, ldq, o, ldo, a.part, a.part_ml, a.scale_log2, nullptr, nullptr, st)) != kHostOk) return rc;
+    a.beside = 1;
+  }
   if (p.few_count > 0) {
     if (c.fp8) rc = launch_few<true>(c, p, a, st);
     else rc = launch_few<false>(c, p, a, st);
     if (rc != kHostOk) return rc;
   }
+  a.beside = a.beside || p.few_count > 0;
+  // Shared tokens first, on the SMs that the plan gives them: a CTA of them fills an SM, tails take what is left.  Both run beside the launch in
+  // front, if that is one of this call (see ``beside`` in paged_few_kernel).
   if (p.prefix_count > 0) {
-    // these run beside the launch in front, if there is one of this call (see ``beside`` in paged_few_kernel), and beside each other
-    if ((rc = launch_prefix(c, p, q, ldq, a.part, a.part_ml, a.scale_log2, a.beside || p.few_count > 0, st)) != kHostOk) return rc;
+    if ((rc = launch_prefix(c, p, q, ldq, a.part, a.part_ml, a.scale_log2, a.beside, st)) != kHostOk) return rc;
     a.beside = 1;
+  }
+  if (p.tail_count > 0) {
     a.cluster = 1;
     if ((rc = c.fp8 ? launch_tail<true>(c, p, a, st) : launch_tail<false>(c, p, a, st)) != kHostOk) return rc;
     SNU1_CUDA_CHECK(launch_pdl(paged_share_join_kernel, dim3((p.join_count + JOIN_THREADS / 32 - 1) / (JOIN_THREADS / 32), c.heads),

@@ -150,7 +150,7 @@ __noinline__ __device__ void far_row(const Plan& p, const ChunkArgs& a, int b, i
     float v[group][4], s[group];
 #pragma unroll
     for (int i = 0; i < group; ++i) {
-      const int key = min(k + i, k1 - 1), pg = p.table[(long long)b * p.width + key / p.page];
+      const int key = min(k + i, k1 - 1), pg = table_of(p, b)[key / p.page];
       float c[2][4];
 #pragma unroll
       for (int kv = 0; kv < 2; ++kv) {
@@ -308,7 +308,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
   }
   const int kv_len = seq_len(p, b);
   int max_a, max_b, min_a, min_b;               // the largest and the smallest limit of row tiles A and B
-  if (p.behind == nullptr) {                    // limits grow from token to token
+  if (p.behind == nullptr && p.own_q_start == nullptr) {      // limits grow from token to token
     const int ends = min(token0 + TILES * T, q_len) - 1;
     min_a = row_limit(p, q0, q_len, kv_len, token0);
     max_a = row_limit(p, q0, q_len, kv_len, min(token0 + T - 1, ends));
@@ -343,7 +343,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         mbar_wait_warp(q_full, 0, abort_flag, args.status, 1);      // nobody else does, and the CTA has to outlive the copy
       } else {
         const int page = args.page, per = BK / page, used = (most + page - 1) / page;   // pages of a tile, of the sequence
-        const int* table = args.first_page == nullptr ? p.table + (long long)b * p.width : nullptr;
+        const int* table = args.first_page == nullptr ? table_of(p, b) : nullptr;
         const int base = args.first_page == nullptr ? 0 : args.first_page[b];
         // a lane's page of tile j, read a tile ahead
         auto page_of = [&](int j) -> int {

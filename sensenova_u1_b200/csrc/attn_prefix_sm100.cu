@@ -34,8 +34,11 @@ template <bool FP8>
 struct Prefix {
   static constexpr int THREADS = FP8 ? 512 : 384;
   static constexpr int K_STAGES = 3, V_STAGES = FP8 ? 3 : 2, W_STAGES = 2, P_STAGES = FP8 ? 2 : 1;
+  // Scales of a tile's keys and values.  Those of tile n are read before S(n + 2) is asked for, and the keys of tile n + K_STAGES + 2 come after that.
+  static constexpr int C_STAGES = 8;
   static constexpr int TILE = PK * HEAD * (FP8 ? 1 : 2), WIDE = PK * HEAD * 2, Q = 16384, P = FP8 ? PK * PR * 2 : 2 * PK * PR * 2;
-  static constexpr int SMEM = Q + (K_STAGES + V_STAGES) * TILE + (FP8 ? W_STAGES * WIDE : 0) + P_STAGES * P + 1024;
+  static constexpr int SCALES = FP8 ? C_STAGES * PK * 8 : 0;
+  static constexpr int SMEM = Q + (K_STAGES + V_STAGES) * TILE + (FP8 ? W_STAGES * WIDE : 0) + P_STAGES * P + SCALES + 1024;
   static constexpr int COLS = FP8 ? 512 : 256;  // of tensor memory: scores twice, output
   static constexpr int S_COLS = FP8 ? 2 * PR : PR, O_AT = 2 * S_COLS;
 };
@@ -45,7 +48,6 @@ struct PrefixArgs {
   long long ldq;
   float* part;
   float2* part_ml;
-  const float* scales;
   int pages, heads;
   float scale_log2;
   int beside;
@@ -99,27 +101,132 @@ __device__ __forceinline__ float log2_of(float x) {
   asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// largest of a warp's; -inf if all are NaN
-__device__ __forceinline__ float warp_max(float x) {
-  const uint32_t b = __float_as_uint(x), k = x != x ? 0u : b & 0x80000000u ? ~b : b | 0x80000000u;
-  const uint32_t m = __reduce_max_sync(0xffffffffu, k);
-  return m == 0 ? -INFINITY : __uint_as_float(m & 0x80000000u ? m & 0x7fffffffu : ~m);
-}
+// A probability may be up to 2^60 before the maximum moves: relative to any key of its row it is an fp32 number, as is its sum.
+constexpr float P_MOST = 60.f;
+// e4m3: exponent of the factor of probabilities times values' scales, whose largest is 2^mv: 2^W_TOP then, as fp16 numbers, and up to 2^15 before it
+// moves.  What is 2^-28 of the largest or less is lost.  (2^7 lets it move in one CTA in five of random scores, 5 us each time.)
+constexpr float W_TOP = 4.f;
+__device__ __forceinline__ int exponent_of(float mv) { return mv == -INFINITY ? 120 : max(-120, min(120, (int)floorf(W_TOP - mv))); }
 
 // What the softmax knows of a row; column n.
 struct RowState {
-  float m;           // running maximum, log2 units; 0 as long as there is none
-  float rs;          // a score's factor
-  float move;        // a score relative to m that is larger moves the maximum: 8, or -inf as long as there is none
-  float move_value;  // e4m3: one that is larger with log2 of its value's scale added does so too
+  float m;           // running maximum, log2 units; -inf as long as there is none
+  float rs;          // e4m3: the power of two that the scores are multiplied by; NaN: a query that is not finite
 };
+
+constexpr int TURN = 32 * 5;
+struct PrefixShared {
+  alignas(16) int lim[PR];                       // limits of the rows, by column
+  // e4m3: the powers of two of RowState::rs and of ec, as bf16: read eight at a time (registers do not suffice for them)
+  alignas(16) uint16_t rs[PR];
+  alignas(16) uint16_t vf[PR];
+  RowState row[PR];
+  float by[PR], f[PR], fo[PR], mv[PR];           // of a move: by how much, factors of the sums and of the output; e4m3: see exponent_of
+  int ec[PR];                                    // e4m3: exponent of a row's factor of p times the value's scale
+  float red[8][32], sum[8][32], turn[8][TURN];
+};
+
+// The largest scores of eight rows over a warp's keys, row i in lane i: log2 units, or relative to the row's maximum plus ``more``.  S: the rows'
+// products; lim: their limits, or null; turn: the warp's own memory, where four rows at a time are turned (a reduction per row by
+// instructions of the warp took 1 us for eight).  A call: it is seldom needed, and its code would crowd the loop's.
+template <bool FP8>
+__device__ __noinline__ float row_tops(uint32_t S, const RowState* row, const int* lim, int key, float ks, bool rel, float more, float* turn) {
+  uint32_t h[8], lo[8];
+  tmem_ld_x8(S, h);
+  if (FP8) tmem_ld_x8(S + PR, lo);
+  tmem_ld_wait();
+  const int lane = threadIdx.x & 31;
+  float mine = -INFINITY;
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int e = 4 * half + k;
+      float y = __uint_as_float(h[e]);
+      if (FP8) y = fmaf(__uint_as_float(lo[e]), 0.0625f, y);
+      y = __fmul_rn(y, FP8 ? __fmul_rn(row[e].rs, ks) : ks);
+      if (rel) y -= row[e].m;
+      if (lim != nullptr && key >= lim[e]) y = -INFINITY;
+      turn[lane * 5 + k] = y == -INFINITY ? y : y + more;
+    }
+    __syncwarp();
+    float top = -INFINITY;                       // (of a NaN and a number fmaxf gives the number)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) top = fmaxf(top, turn[((lane >> 2) * 4 + k) * 5 + (lane & 3)]);
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if ((lane >> 2 & 1) == half) mine = top;
+    __syncwarp();
+  }
+  return mine;
+}
+
+// Moves the maxima of a set of four softmax warps to the largest scores of a tile, and the output with them.  Out of the loop's way.
+template <bool FP8>
+__device__ __noinline__ void move_maxima(PrefixShared& sh, uint32_t S, uint32_t O, int side, int active, int key, float ks, float lv, bool dirty, bool first) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, w = warp - 4, c0 = side * 32, col = c0 + lane;
+  const bool mine = (w & 3) == 0 && lane < 8 * active;
+#pragma unroll 1
+  for (int i = 0; i < active; ++i) {
+    const int c = c0 + 8 * i;
+    const float top = row_tops<FP8>(S + 8 * i, sh.row + c, dirty ? sh.lim + c : nullptr, key, ks, false, 0.f, sh.turn[w]);
+    if (lane < 8) sh.red[w][8 * i + lane] = top;
+  }
+  named_bar_sync(2 + side, 128);
+  if (mine) {
+    const float m = sh.row[col].m;
+    float top = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) top = fmaxf(top, sh.red[side * 4 + k][lane]);
+    const bool fresh = m == -INFINITY;
+    const float now = fmaxf(m, top);
+    sh.by[col] = fresh ? 0.f : now - m;
+    sh.f[col] = fresh ? 0.f : fast_exp2(m - now);
+    sh.row[col].m = now;
+  }
+  named_bar_sync(2 + side, 128);
+  if (FP8) {
+#pragma unroll 1
+    for (int i = 0; i < active; ++i) {
+      const int c = c0 + 8 * i;
+      const float top = row_tops<FP8>(S + 8 * i, sh.row + c, dirty ? sh.lim + c : nullptr, key, ks, true, lv, sh.turn[w]);
+      if (lane < 8) sh.red[w][8 * i + lane] = top;
+    }
+    named_bar_sync(2 + side, 128);
+    if (mine) {
+      float top = sh.mv[col] - sh.by[col];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) top = fmaxf(top, sh.red[side * 4 + k][lane]);
+      const int ec = exponent_of(top);
+      sh.fo[col] = sh.f[col] == 0.f ? 0.f : exp2f((float)(ec - sh.ec[col]) - sh.by[col]);
+      sh.mv[col] = top;
+      sh.ec[col] = ec;
+      sh.vf[col] = (uint16_t)((127 + ec) << 7);
+    }
+    named_bar_sync(2 + side, 128);
+  }
+  if (!first) {
+#pragma unroll 1
+    for (int i = 0; i < active * (FP8 ? 1 : 2); ++i) {
+      const int c = c0 + 8 * (FP8 ? i : i >> 1);
+      const uint32_t at = O + (FP8 ? 0 : (i & 1) * PR) + c;
+      uint32_t o[8];
+      tmem_ld_x8(at, o);
+      tmem_ld_wait();
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * (FP8 ? sh.fo : sh.f)[c + e]);
+      tmem_st_x8(at, o);
+    }
+    tmem_st_wait();
+  }
+}
 
 template <bool FP8>
 __global__ void __launch_bounds__(Prefix<FP8>::THREADS, 1)
-    paged_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ Plan p,
+    paged_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v /* e4m3: of the scales */, const __grid_constant__ Plan p,
                         const __grid_constant__ PrefixArgs args) {
   using F = Prefix<FP8>;
-  constexpr int KS = F::K_STAGES, VS = F::V_STAGES, WS = F::W_STAGES, PS = F::P_STAGES;
+  constexpr int KS = F::K_STAGES, VS = F::V_STAGES, WS = F::W_STAGES, PS = F::P_STAGES, CS = F::C_STAGES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* sQ = smem;                            // e4m3: [hi 64, lo 64][128]; bf16: [half of the values][64][64]
@@ -127,14 +234,12 @@ __global__ void __launch_bounds__(Prefix<FP8>::THREADS, 1)
   uint8_t* sV = sK + KS * F::TILE;
   uint8_t* sP = sV + VS * F::TILE;               // [key][64 rows] fp16; bf16: hi, then lo
   uint8_t* sW = sP + PS * F::P;                  // e4m3: widened values, [half][key][64]
-  __shared__ uint64_t q_ready, k_full[KS], k_empty[KS], v_full[VS], v_empty[VS], w_full[WS], w_empty[WS], s_full[2], s_empty[2], p_full[PS], pv_done[PS];
+  float* sC = reinterpret_cast<float*>(sW + WS * F::WIDE);      // e4m3: [stage][page][keys, values][token]
+  __shared__ uint64_t q_ready, k_full[KS], k_empty[KS], v_full[VS], v_empty[VS], w_full[WS], w_empty[WS], s_full[2], s_empty[2], p_full[PS], pv_done[PS], c_full[CS];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_word, s_poison;
-  __shared__ int s_lim[PR], s_most, s_least;
-  __shared__ RowState s_row[PR];
-  __shared__ float s_by[PR], s_f[PR], s_fo[PR], s_mv[PR];
-  __shared__ int s_ec[PR];                       // e4m3: exponent of a row's factor of p times the value's scale
-  __shared__ float s_red[8][32], s_red2[8][32], s_sum[8][32];
+  __shared__ int s_most, s_least;
+  __shared__ PrefixShared sh;
   volatile int* abort_flag = &abort_word;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
   // what the plan's host side has set, before the wait: no launch in front writes it
@@ -160,6 +265,7 @@ __global__ void __launch_bounds__(Prefix<FP8>::THREADS, 1)
       mbar_init(&s_full[i], 1);
       mbar_init(&s_empty[i], 4 * sides);
     }
+    for (int i = 0; i < CS; ++i) mbar_init(&c_full[i], 1);
     for (int i = 0; i < PS; ++i) {
       mbar_init(&p_full[i], 4 * sides);
       mbar_init(&pv_done[i], 1);
@@ -170,7 +276,7 @@ __global__ void __launch_bounds__(Prefix<FP8>::THREADS, 1)
     s_least = 0x7fffffff;
     mbar_fence_init();
     tma_prefetch_desc(&tm_k);
-    if (!FP8) tma_prefetch_desc(&tm_v);
+    tma_prefetch_desc(&tm_v);
   }
   if (warp == 1) {
     tmem_alloc(&tmem_slot, F::COLS);
@@ -180,34 +286,106 @@ __global__ void __launch_bounds__(Prefix<FP8>::THREADS, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
-  if (!args.beside) pdl_wait();
+  // (also host-set: where this thread's row is)
+  int q_first = 0, q_len = 0, seq = 0;
+  if (tid < rows) {
+    seq = p.row_seq[t0 + (row0 + tid) / G];
+    q_first = p.q_start[seq];
+    q_len = p.q_start[seq + 1] - q_first;
+  }
+  if (!args.beside) pdl_wait();                  // (see paged_few_kernel)
   pdl_trigger();
   // column of row r: 8 (r / 8 / 2) + r % 8 of the half that its set of warps has
+  const int* table = p.table + (long long)run.z * p.width;
+  const int per = PK / p.page;                   // pages of a tile
+  int first_page = 0;                            // warp 0: those of the first tile, if all shared tokens are read
   if (tid < PR) {
+    if (tid < per) first_page = table[(int)((long long)(shared / PK) * part / parts) * per + tid];
     const int col = (tid >> 3 & 1) * 32 + (tid >> 4) * 8 + (tid & 7);
     int lim = 0;
     if (tid < rows) {
-      const int t = t0 + (row0 + tid) / G, b = p.row_seq[t], q0 = p.q_start[b];
-      lim = min(shared, row_limit(p, q0, p.q_start[b + 1] - q0, seq_len(p, b), t - q0));
+      lim = min(shared, row_limit(p, q_first, q_len, seq_len(p, seq), t0 + (row0 + tid) / G - q_first));
       atomicMax(&s_most, lim);
       atomicMin(&s_least, lim);
     }
-    s_lim[col] = lim;
+    sh.lim[col] = lim;
+  } else if (warp >= 4 && warp < 12) {
+    // queries: four threads per row
+    const int s = tid - 128, r = s >> 2, c = s & 3, col = (r >> 3 & 1) * 32 + (r >> 4) * 8 + (r & 7), row = row0 + r;
+    uint4 u[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) u[i] = make_uint4(0, 0, 0, 0);
+    if (r < rows) {
+      const uint4* from = reinterpret_cast<const uint4*>(args.q + (long long)(t0 + row / G) * args.ldq + (long long)(head * G + row % G) * HEAD + c * 32);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) u[i] = from[i];
+    }
+    float rs = 1.f;
+    if (!FP8) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<uint4*>(sQ + (c >> 1) * (PR * 128) + swz128_offset(col, (c & 1) * 4 + i)) = u[i];
+    } else {
+      uint32_t top = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        top = max_u16x2(top, max_u16x2(max_u16x2(u[i].x & 0x7fff7fffu, u[i].y & 0x7fff7fffu), max_u16x2(u[i].z & 0x7fff7fffu, u[i].w & 0x7fff7fffu)));
+      }
+      top = max_u16x2(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max_u16x2(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      top = max(top << 16, top & 0xffff0000u);
+      const int e = (int)(top >> 23) - 127, up = top == 0 || e == 128 ? 0 : min(7 - e, 120);
+      const float f = __int_as_float((127 + up) << 23);
+      rs = e == 128 ? __int_as_float(0x7fffffff) : __int_as_float((127 - up) << 23);      // not finite: NaN
+      uint32_t hi[8], lo[8];                   // four codes each
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const uint32_t x2 = i & 2 ? (i & 1 ? u[i >> 2].w : u[i >> 2].z) : (i & 1 ? u[i >> 2].y : u[i >> 2].x);
+        const float x = __uint_as_float(x2 << 16) * f, y = __uint_as_float(x2 & 0xffff0000u) * f;
+        const uint32_t h = e4m3x2_of(x, y);
+        const float2 back = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)h, __NV_E4M3)));
+        const uint32_t l = e4m3x2_of((x - back.x) * 16.f, (y - back.y) * 16.f);
+        if (i & 1) {
+          hi[i >> 1] |= h << 16;
+          lo[i >> 1] |= l << 16;
+        } else {
+          hi[i >> 1] = h;
+          lo[i >> 1] = l;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        *reinterpret_cast<uint4*>(sQ + swz128_offset(col, 2 * c + i)) = make_uint4(hi[4 * i], hi[4 * i + 1], hi[4 * i + 2], hi[4 * i + 3]);
+        *reinterpret_cast<uint4*>(sQ + swz128_offset(PR + col, 2 * c + i)) = make_uint4(lo[4 * i], lo[4 * i + 1], lo[4 * i + 2], lo[4 * i + 3]);
+      }
+    }
+    if (c == 0) {
+      sh.row[col] = RowState{-INFINITY, rs};
+      sh.rs[col] = (uint16_t)(__float_as_uint(rs) >> 16);
+      sh.ec[col] = 120;
+      sh.vf[col] = (127 + 120) << 7;
+      sh.mv[col] = -INFINITY;
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&q_ready);
   }
   __syncthreads();
   const int most = s_most, least = s_least;
   const int all = (most + PK - 1) / PK;
   const int j0 = (int)((long long)all * part / parts), n_tiles = (int)((long long)all * (part + 1) / parts) - j0;
-  const int* table = p.table + (long long)run.z * p.width;
-
+  // e4m3: 512 threads start with 128 registers, 256 x 72 + 256 x 184 = 512 x 128; bf16: 384 with 168, 128 x 88 + 256 x 208 = 384 x 168
+  if (warp < 4 || warp >= 12) {
+  if (FP8) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+  else asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
   if (warp == 0) {
     // ------------------------------ pages --------------------------------
-    const int page = p.page, per = PK / page, used = (most + page - 1) / page;
+    const int page = p.page, used = (most + page - 1) / page;
     auto page_of = [&](int n) -> int {
       const int i = (j0 + n) * per + lane;
       return n < n_tiles && lane < per && i < used ? table[i] : 0;
     };
-    int pg = page_of(0);
+    int pg = most == shared ? first_page : page_of(0);
     for (int n = 0; n < n_tiles; ++n) {
       const int next = page_of(n + 1), live = min(per, used - (j0 + n) * per);
       if (lane < live && (pg < 0 || pg >= args.pages)) report_status(args.status, kBadPage, 10);     // reads as zeros
@@ -220,10 +398,14 @@ __global__ void __launch_bounds__(Prefix<FP8>::THREADS, 1)
           n = n_tiles;
           break;
         }
-        if (lane == 0) mbar_expect_tx(full, live * page * (FP8 ? 128 : 256));
+        if (lane == 0) {
+          mbar_expect_tx(full, live * page * (FP8 ? 128 : 256));
+          if (FP8 && kv == 0) mbar_expect_tx(&c_full[n % CS], live * page * 8);
+        }
         __syncwarp();
         if (lane < live) {
           if (FP8) {
+            if (kv == 0) tma_load_4d(sC + ((n % CS) * PK + lane * page) * 2, &tm_v, &c_full[n % CS], 0, head, 0, pg);
             tma_load_5d(smem_u32(dst), &tm_k, full, 0, 0, head, kv, pg);
           } else {
             tma_load_4d(dst, kv ? &tm_v : &tm_k, full, 0, 0, head, pg);
@@ -311,258 +493,214 @@ __global__ void __launch_bounds__(Prefix<FP8>::THREADS, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&w_full[n % WS]);
     }
-  } else if (warp >= 4) {
+  }
+  } else {
+    if (FP8) asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+    else asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     // ------------------------------ softmax --------------------------------
     const int w = warp - 4, side = w >> 2, c0 = side * 32, active = (groups + 1 - side) >> 1;      // groups of eight columns from c0 on
     const int in_tile = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;
     bool ok = true;
-    {
-      // queries: four threads per row
-      const int s = tid - 128, r = s >> 2, c = s & 3, col = (r >> 3 & 1) * 32 + (r >> 4) * 8 + (r & 7), row = row0 + r;
-      uint4 u[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) u[i] = make_uint4(0, 0, 0, 0);
-      if (r < rows) {
-        const uint4* from = reinterpret_cast<const uint4*>(args.q + (long long)(t0 + row / G) * args.ldq + (long long)(head * G + row % G) * HEAD + c * 32);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) u[i] = from[i];
-      }
-      float rs = args.scale_log2;
-      if (!FP8) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          *reinterpret_cast<uint4*>(sQ + (c >> 1) * (PR * 128) + swz128_offset(col, (c & 1) * 4 + i)) = u[i];
-      } else {
-        uint32_t top = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          top = max_u16x2(top, max_u16x2(max_u16x2(u[i].x & 0x7fff7fffu, u[i].y & 0x7fff7fffu), max_u16x2(u[i].z & 0x7fff7fffu, u[i].w & 0x7fff7fffu)));
-        }
-        top = max_u16x2(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = max_u16x2(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        top = max(top << 16, top & 0xffff0000u);
-        const int e = (int)(top >> 23) - 127, up = top == 0 || e == 128 ? 0 : min(7 - e, 120);
-        const float f = __int_as_float((127 + up) << 23);
-        rs = e == 128 ? __int_as_float(0x7fffffff) : rs * __int_as_float((127 - up) << 23);      // not finite: NaN
-        uint32_t hi[8], lo[8];                   // four codes each
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const uint32_t x2 = i & 2 ? (i & 1 ? u[i >> 2].w : u[i >> 2].z) : (i & 1 ? u[i >> 2].y : u[i >> 2].x);
-          const float x = __uint_as_float(x2 << 16) * f, y = __uint_as_float(x2 & 0xffff0000u) * f;
-          const uint32_t h = e4m3x2_of(x, y);
-          const float2 back = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)h, __NV_E4M3)));
-          const uint32_t l = e4m3x2_of((x - back.x) * 16.f, (y - back.y) * 16.f);
-          if (i & 1) {
-            hi[i >> 1] |= h << 16;
-            lo[i >> 1] |= l << 16;
-          } else {
-            hi[i >> 1] = h;
-            lo[i >> 1] = l;
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          *reinterpret_cast<uint4*>(sQ + swz128_offset(col, 2 * c + i)) = make_uint4(hi[4 * i], hi[4 * i + 1], hi[4 * i + 2], hi[4 * i + 3]);
-          *reinterpret_cast<uint4*>(sQ + swz128_offset(PR + col, 2 * c + i)) = make_uint4(lo[4 * i], lo[4 * i + 1], lo[4 * i + 2], lo[4 * i + 3]);
-        }
-      }
-      if (c == 0) {
-        s_row[col] = RowState{0.f, rs, -INFINITY, -INFINITY};
-        s_ec[col] = 0;
-        s_mv[col] = -INFINITY;
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&q_ready);
-      named_bar_sync(1, 256);
-    }
     if (active > 0 && n_tiles > 0) {
-      // e4m3: scales of this thread's key and value, read a tile ahead
-      auto scales_of = [&](int n) -> float2 {
-        const int key = (j0 + n) * PK + in_tile;
-        float2 x = make_float2(0.f, 0.f);
-        if (n < n_tiles && key < most) {
-          const int pg = table[key / p.page];
-          if (pg >= 0 && pg < args.pages) {
-            const float* at = args.scales + ((long long)pg * 2 * args.heads + head) * p.page + key % p.page;
-            x = make_float2(at[0], at[(long long)args.heads * p.page]);
-          }
-        }
-        return x;
-      };
-      float x[32], l[32];
+      const int page_log = __ffs(p.page) - 1, c_at = ((in_tile >> page_log) << page_log) * 2 + (in_tile & (p.page - 1));      // of this thread's key
+      // Two rows in every 64-bit register: sums, maxima (negative; + inf as long as there is none, so that the first score moves it), and a
+      // tile's probabilities.
+      uint64_t l2[16], nm[16], p2[16];
 #pragma unroll
-      for (int i = 0; i < 32; ++i) l[i] = 0.f;
-      float2 sc = FP8 ? scales_of(0) : make_float2(1.f, 1.f);
-      for (int n = 0; n < n_tiles; ++n) {        // all tiles also after a time-out
-        const int k0 = (j0 + n) * PK, key = k0 + in_tile;
-        const bool dirty = k0 + PK > least;      // some row may not read all of it
-        const float2 next = FP8 ? scales_of(n + 1) : sc;
-        const float lv = FP8 ? log2_of(sc.y) : 0.f;
-        ok &= mbar_wait(&s_full[n & 1], (n >> 1) & 1, abort_flag, args.status, 5);
+      for (int i = 0; i < 16; ++i) {
+        l2[i] = p2[i] = 0;
+        nm[i] = pack_f32x2(INFINITY, INFINITY);
+      }
+      const uint64_t sixteenth = pack_f32x2(0.0625f, 0.0625f);
+      // e4m3: scales of this thread's key and value.  A value that is not finite makes its key's scores NaN: rows that may read it are NaN, and
+      // elsewhere it is not seen.
+      auto scales_of = [&](int n) -> float2 {
+        const float* c = sC + (n % CS) * PK * 2 + c_at;
+        const float2 x = make_float2(c[0], c[p.page]);
+        return fabsf(x.y) < INFINITY ? x : make_float2(__int_as_float(0x7fffffff), 0.f);
+      };
+              // the registers' copies of what has changed in shared memory
+              auto take = [&](bool sums) {
+      #pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                  if (i >= 4 * active) break;
+                  const int c = c0 + 2 * i;
+                  nm[i] = pack_f32x2(-sh.row[c].m, -sh.row[c + 1].m);
+                  if (sums) l2[i] = mul_f32x2(l2[i], pack_f32x2(sh.f[c], sh.f[c + 1]));
+                      }
+              };
+      {
+        // Where the maxima begin: at those of the first 32 keys (of a tile that the mask cuts: nowhere, see move_maxima).
+        const int key = j0 * PK + in_tile;
+        float2 sc = make_float2(1.f, 1.f);
+        if (FP8) {
+          ok &= mbar_wait(&c_full[0], 0, abort_flag, args.status, 5);
+          sc = scales_of(0);
+        }
+        ok &= mbar_wait(&s_full[0], 0, abort_flag, args.status, 5);
         __syncwarp();
         tc_fence_after();
-        const uint32_t S = tmem + (n & 1) * F::S_COLS + c0 + lanes;
-        bool move = false;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (i >= active) break;
-          uint32_t h[8], lo[8];
-          tmem_ld_x8(S + 8 * i, h);
-          if (FP8) tmem_ld_x8(S + PR + 8 * i, lo);
-          tmem_ld_wait();
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const RowState r = s_row[c0 + 8 * i + e];
-            const float s = FP8 ? fmaf(__uint_as_float(lo[e]), 0.0625f, __uint_as_float(h[e])) : __uint_as_float(h[e]);
-            float y = __fmul_rn(s, FP8 ? r.rs * sc.x : r.rs);      // (never fused with the difference)
-            if (dirty && key >= s_lim[c0 + 8 * i + e]) y = -INFINITY;
-            y -= r.m;
-            move |= y > r.move || (FP8 && y + lv > r.move_value);
-            x[8 * i + e] = y;
-          }
-        }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&s_empty[n & 1]);
-        if (named_bar_any(2 + side, 128, move)) {
-          // the maximum moves (the first tile, and seldom after it)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if (i >= active) break;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const float a = warp_max(x[8 * i + e]), b = FP8 ? warp_max(x[8 * i + e] + lv) : 0.f;
-              if (lane == 0) {
-                s_red[w][8 * i + e] = a;
-                s_red2[w][8 * i + e] = b;
+        if ((w & 3) == 0 && j0 * PK + PK <= least) {
+          const float ks = sc.x * args.scale_log2;
+#pragma unroll 1
+          for (int i = 0; i < active; ++i) {
+            RowState* row = sh.row + c0 + 8 * i;
+            const uint32_t S = tmem + c0 + lanes + 8 * i;
+            const float m = row_tops<FP8>(S, row, nullptr, key, ks, false, 0.f, sh.turn[w]);
+            if (lane < 8) row[lane].m = m;
+            if (FP8) {
+              __syncwarp();
+              const float mv = row_tops<FP8>(S, row, nullptr, key, ks, true, log2_of(sc.y), sh.turn[w]);
+              if (lane < 8) {
+                sh.mv[c0 + 8 * i + lane] = mv;
+                sh.ec[c0 + 8 * i + lane] = exponent_of(mv);
+                sh.vf[c0 + 8 * i + lane] = (uint16_t)((127 + exponent_of(mv)) << 7);
               }
             }
           }
-          named_bar_sync(2 + side, 128);
-          if ((w & 3) == 0 && lane < 8 * active) {
-            const int col = c0 + lane;
-            RowState r = s_row[col];
-            float top = -INFINITY, topv = -INFINITY;
+        }
+        named_bar_sync(2 + side, 128);
+        take(false);
+      }
+      for (int n = 0; n < n_tiles; ++n) {        // all tiles also after a time-out
+        const int k0 = (j0 + n) * PK, key = k0 + in_tile;
+        const bool dirty = k0 + PK > least;      // some row may not read all of it
+        float2 sc = make_float2(1.f, 1.f);
+        if (FP8) {
+          ok &= mbar_wait(&c_full[n % CS], (n / CS) & 1, abort_flag, args.status, 5);
+          sc = scales_of(n);
+        }
+        const float ks = sc.x * args.scale_log2;
+        const uint64_t ks2 = pack_f32x2(ks, ks), vs2 = pack_f32x2(sc.y, sc.y);
+        uint8_t* P = sP + (n % PS) * F::P;
+        ok &= mbar_wait(&s_full[n & 1], (n >> 1) & 1, abort_flag, args.status, 5);
+        if (n >= PS) ok &= mbar_wait(&pv_done[n % PS], ((n - PS) / PS) & 1, abort_flag, args.status, 6);
+        __syncwarp();
+        tc_fence_after();
+        const uint32_t S = tmem + (n & 1) * F::S_COLS + c0 + lanes;
+#pragma unroll 1
+        for (int again = 0; again < 2; ++again) {
+          // Probabilities, and whether one is too large for where the maxima are; their products are written all the same, and once more after the
+          // maxima have moved.
+          float mx = -INFINITY, mw = -INFINITY;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              top = fmaxf(top, s_red[side * 4 + k][lane]);
-              topv = fmaxf(topv, s_red2[side * 4 + k][lane]);
-            }
-            const bool fresh = r.move == -INFINITY, none = fresh && top == -INFINITY;
-            const float by = none ? 0.f : fresh ? top : fmaxf(top, 0.f);
-            r.m += by;
-            if (!none) r.move = 8.f;
-            s_by[col] = by;
-            s_f[col] = fresh ? 0.f : fast_exp2(-by);
+          for (int i = 0; i < 4; ++i) {
+            if (i >= active) break;
+            uint32_t h[8], lo[8];
+            tmem_ld_x8(S + 8 * i, h);
+            if (FP8) tmem_ld_x8(S + PR + 8 * i, lo);
+            uint4 rs4 = make_uint4(0, 0, 0, 0), vf4 = rs4;
             if (FP8) {
-              const float mv = fmaxf(s_mv[col], topv) - by;
-              const int was = s_ec[col], ec = mv == -INFINITY ? was : max(-120, min(120, (int)floorf(P_TOP - mv)));
-              s_mv[col] = mv;
-              s_ec[col] = ec;
-              r.move_value = mv == -INFINITY ? -INFINITY : P_TOP + 8.f - (float)ec;
-              s_fo[col] = fresh ? 0.f : exp2f(-by + (float)(ec - was));
+              rs4 = *reinterpret_cast<const uint4*>(sh.rs + c0 + 8 * i);
+              vf4 = *reinterpret_cast<const uint4*>(sh.vf + c0 + 8 * i);
             }
-            s_row[col] = r;
+            const uint32_t rs2[4] = {rs4.x, rs4.y, rs4.z, rs4.w}, vf2[4] = {vf4.x, vf4.y, vf4.z, vf4.w};
+            tmem_ld_wait();
+            uint64_t y[4];                       // log2 units; product and difference are never fused
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              y[e] = pack_f32x2(__uint_as_float(h[2 * e]), __uint_as_float(h[2 * e + 1]));
+              if (FP8) {
+                y[e] = fma_f32x2(pack_f32x2(__uint_as_float(lo[2 * e]), __uint_as_float(lo[2 * e + 1])), sixteenth, y[e]);
+                y[e] = mul_f32x2(y[e], mul_f32x2(bf16x2_to_f32x2(rs2[e]), ks2));
+              } else {
+                y[e] = mul_f32x2(y[e], ks2);
+              }
+              y[e] = add_f32x2(y[e], nm[4 * i + e]);
+            }
+            if (__builtin_expect(dirty, 0)) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                float a, b;
+                unpack_f32x2(y[e], a, b);
+                const int2 lim = *reinterpret_cast<const int2*>(sh.lim + c0 + 8 * i + 2 * e);
+                y[e] = pack_f32x2(key >= lim.x ? -INFINITY : a, key >= lim.y ? -INFINITY : b);
+              }
+            }
+            uint32_t u[4], v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              float a, b;
+              unpack_f32x2(y[e], a, b);
+              mx = max3(mx, a, b);
+              const float pa = fast_exp2(a), pb = fast_exp2(b);
+              const uint64_t pp = pack_f32x2(pa, pb);
+              p2[4 * i + e] = pp;
+              if (FP8) {
+                float wa, wb;
+                unpack_f32x2(mul_f32x2(mul_f32x2(pp, vs2), bf16x2_to_f32x2(vf2[e])), wa, wb);
+                mw = max3(mw, wa, wb);
+                u[e] = pack_f16x2(wa, wb);
+              } else {
+                const uint32_t hi = pack_bf16x2(pa, pb);
+                float ra, rb;
+                unpack_f32x2(add_f32x2(pp, bf16x2_to_f32x2(hi ^ 0x80008000u)), ra, rb);
+                u[e] = hi;
+                v[e] = pack_bf16x2(ra, rb);
+              }
+            }
+            const uint32_t to = swz128_offset(in_tile, side * 4 + i);
+            *reinterpret_cast<uint4*>(P + to) = make_uint4(u[0], u[1], u[2], u[3]);
+            if (!FP8) *reinterpret_cast<uint4*>(P + PK * 128 + to) = make_uint4(v[0], v[1], v[2], v[3]);
           }
-          named_bar_sync(2 + side, 128);
+          if (__builtin_expect(!named_bar_any(2 + side, 128, again == 0 && (mx > P_MOST || mw > 32768.f)), 1)) break;
           if (n > 0) {
             ok &= mbar_wait(&pv_done[(n - 1) % PS], ((n - 1) / PS) & 1, abort_flag, args.status, 6);
             __syncwarp();
             tc_fence_after();
           }
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if (i >= active) break;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              x[8 * i + e] -= s_by[c0 + 8 * i + e];
-              l[8 * i + e] *= s_f[c0 + 8 * i + e];
-            }
-            if (n > 0) {
-#pragma unroll
-              for (int half = 0; half < (FP8 ? 1 : 2); ++half) {
-                const uint32_t at = tmem + F::O_AT + half * PR + c0 + 8 * i + lanes;
-                uint32_t o[8];
-                tmem_ld_x8(at, o);
-                tmem_ld_wait();
-#pragma unroll
-                for (int e = 0; e < 8; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * (FP8 ? s_fo : s_f)[c0 + 8 * i + e]);
-                tmem_st_x8(at, o);
-              }
-            }
-          }
-          tmem_st_wait();
-          tc_fence_before();
+          move_maxima<FP8>(sh, S, tmem + F::O_AT + lanes, side, active, key, ks, FP8 ? log2_of(sc.y) : 0.f, dirty, n == 0);
+          take(true);
         }
-        if (!FP8 && dirty) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_empty[n & 1]);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) l2[i] = add_f32x2(l2[i], p2[i]);
+        if (!FP8 && __builtin_expect(dirty, 0)) {
           // values that some row may not read: what nobody may and what is not finite is cleared, see attn_paged.cu
           ok &= mbar_wait(&v_full[n % VS], (n / VS) & 1, abort_flag, args.status, 5);
           uint8_t* tile = sV + (n % VS) * F::TILE;
           for (int i = tid - 128; i < PK * 16; i += 128 * sides) {
             const int k = i >> 4;
             uint4* at = reinterpret_cast<uint4*>(tile + ((i & 15) >> 3) * (PK * 128) + swz128_offset(k, i & 7));
-            uint4 v = *at;
-            uint32_t* u = reinterpret_cast<uint32_t*>(&v);
+            uint4 x = *at;
+            uint32_t* z = reinterpret_cast<uint32_t*>(&x);
             bool bad = false;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const bool a = (u[e] & 0x7f80u) == 0x7f80u, b = (u[e] & 0x7f800000u) == 0x7f800000u;
+              const bool a = (z[e] & 0x7f80u) == 0x7f80u, b = (z[e] & 0x7f800000u) == 0x7f800000u;
               bad |= a || b;
-              u[e] &= (a ? 0xffff0000u : 0xffffffffu) & (b ? 0xffffu : 0xffffffffu);
+              z[e] &= (a ? 0xffff0000u : 0xffffffffu) & (b ? 0xffffu : 0xffffffffu);
             }
             if (k0 + k >= most) {
               *at = make_uint4(0, 0, 0, 0);
             } else if (bad) {
-              *at = v;
+              *at = x;
               atomicMin(&s_poison, k0 + k);
             }
           }
         }
-        if (n >= PS) {
-          ok &= mbar_wait(&pv_done[n % PS], ((n - PS) / PS) & 1, abort_flag, args.status, 6);
-          __syncwarp();
-        }
-        uint8_t* P = sP + (n % PS) * F::P;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (i >= active) break;
-          uint32_t u[4], v[4];
-#pragma unroll
-          for (int e = 0; e < 8; e += 2) {
-            float y[2];
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              const int r = 8 * i + e + k;
-              y[k] = fast_exp2(x[r]);
-              l[r] += y[k];
-              // (the scale of a key that is hidden may be anything)
-              if (FP8) y[k] = dirty && x[r] == -INFINITY ? 0.f : y[k] * (sc.y * __int_as_float((127 + s_ec[c0 + r]) << 23));
-            }
-            if (FP8) {
-              u[e >> 1] = pack_f16x2(y[0], y[1]);
-            } else {
-              u[e >> 1] = pack_bf16x2(y[0], y[1]);
-              v[e >> 1] = pack_bf16x2(y[0] - __uint_as_float(u[e >> 1] << 16), y[1] - __uint_as_float(u[e >> 1] & 0xffff0000u));
-            }
-          }
-          const uint32_t at = swz128_offset(in_tile, side * 4 + i);
-          *reinterpret_cast<uint4*>(P + at) = make_uint4(u[0], u[1], u[2], u[3]);
-          if (!FP8) *reinterpret_cast<uint4*>(P + PK * 128 + at) = make_uint4(v[0], v[1], v[2], v[3]);
-        }
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[n % PS]);
-        sc = next;
       }
       // sums over the keys' threads, then the output
 #pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        if (i >= 8 * active) break;
+      for (int i = 0; i < 16; ++i) {
+        if (i >= 4 * active) break;
+        float a, b;
+        unpack_f32x2(l2[i], a, b);
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], o);
-        if (lane == 0) s_sum[w][i] = l[i];
+        for (int o = 16; o > 0; o >>= 1) {
+          a += __shfl_xor_sync(0xffffffffu, a, o);
+          b += __shfl_xor_sync(0xffffffffu, b, o);
+        }
+        if (lane == 0) {
+          sh.sum[w][2 * i] = a;
+          sh.sum[w][2 * i + 1] = b;
+        }
       }
       ok &= mbar_wait(&pv_done[(n_tiles - 1) % PS], ((n_tiles - 1) / PS) & 1, abort_flag, args.status, 6);
       ok = __all_sync(0xffffffffu, ok);
@@ -579,7 +717,7 @@ __global__ void __launch_bounds__(Prefix<FP8>::THREADS, 1)
           const int col = c0 + 8 * i + e, r = (2 * i + side) * 8 + e;
           if (r < rows && ok)
             args.part[((long long)(item.w + r) * args.heads + head) * HEAD + in_tile] =
-                FP8 ? __uint_as_float(h[e]) * __int_as_float((127 - s_ec[col]) << 23) : __uint_as_float(h[e]) + __uint_as_float(lo[e]);
+                FP8 ? __uint_as_float(h[e]) * __int_as_float((127 - sh.ec[col]) << 23) : __uint_as_float(h[e]) + __uint_as_float(lo[e]);
         }
       }
     }
@@ -587,10 +725,10 @@ __global__ void __launch_bounds__(Prefix<FP8>::THREADS, 1)
       const int col = c0 + lane, r = (2 * (lane >> 3) + side) * 8 + (lane & 7);
       float m = -INFINITY, l = 0.f;
       if (n_tiles > 0) {
-        m = s_row[col].move == -INFINITY ? -INFINITY : s_row[col].m;
+        m = sh.row[col].m;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) l += s_sum[side * 4 + k][lane];
-        if (!FP8 && s_lim[col] > *reinterpret_cast<volatile int*>(&s_poison)) l = __int_as_float(0x7fffffff);
+        for (int k = 0; k < 4; ++k) l += sh.sum[side * 4 + k][lane];
+        if (!FP8 && sh.lim[col] > *reinterpret_cast<volatile int*>(&s_poison)) l = __int_as_float(0x7fffffff);
         if (l != l && m == -INFINITY) m = 0.f;   // all NaN: not to be taken for no keys at all
       }
       if (r < rows) args.part_ml[(long long)(item.w + r) * args.heads + head] = make_float2(m, l);
@@ -620,18 +758,16 @@ static int launch(const Cache& c, const Plan& p, const PrefixArgs& a, cudaStream
     err = cudaFuncSetAttribute(paged_prefix_kernel<FP8>, cudaFuncAttributeMaxDynamicSharedMemorySize, Prefix<FP8>::SMEM);
   });
   SNU1_CUDA_CHECK(err);
-  SNU1_CUDA_CHECK(launch_pdl(paged_prefix_kernel<FP8>, dim3(a.heads * p.prefix_count), dim3(Prefix<FP8>::THREADS), Prefix<FP8>::SMEM, st, c.k, c.v, p, a));
+  SNU1_CUDA_CHECK(launch_pdl(paged_prefix_kernel<FP8>, dim3(a.heads * p.prefix_count), dim3(Prefix<FP8>::THREADS), Prefix<FP8>::SMEM, st, c.k, FP8 ? c.scale : c.v, p, a));
   return kHostOk;
 }
 
-int launch_prefix(const Cache& c, const Plan& p, const void* q, long long ldq, float* part, float2* part_ml, float scale_log2, int beside,
-                  cudaStream_t st) {
+int launch_prefix(const Cache& c, const Plan& p, const void* q, long long ldq, float* part, float2* part_ml, float scale_log2, int beside, cudaStream_t st) {
   PrefixArgs a;
   a.q = (const __nv_bfloat16*)q;
   a.ldq = ldq;
   a.part = part;
   a.part_ml = part_ml;
-  a.scales = c.scales;
   a.pages = c.pages;
   a.heads = c.heads;
   a.scale_log2 = scale_log2;

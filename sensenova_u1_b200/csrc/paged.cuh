@@ -31,7 +31,7 @@ struct alignas(64) Cache {
   int pages, heads, page, fp8;
 };
 
-constexpr int PLAN_LAYOUT = 0x70670003;
+constexpr int PLAN_LAYOUT = 0x70670004;
 
 // Device arrays and counts of a plan (ops/paged.py builds it).
 struct Plan {
@@ -53,11 +53,20 @@ struct Plan {
   const int4* runs;        // runs of sequences with the same first tokens: first row, rows, sequence whose table is read, shared tokens
   const int4* prefix;      // [prefix_count] work on shared tokens: run, first of up to PREFIX_ROWS rows (x heads of a group), part | parts << 16, partial row
   const int4* tail;        // [tail_count] work on the other tokens of such sequences, as ``few``
-  const int4* joins;       // [2 x join_count] row, head of the group, partial row of the shared tokens' part 0, parts | partial row of its tail, parts, rows of a part, -
+  const int4* joins;       // [2 x join_count] row, head of the group, partial row of the shared tokens' part 0, parts | partial row of its tail, parts, rows of a part, rows of a part of the shared ones
+  // Runs of many rows go to the kernel for chunks, as sequences 0, 2, ...: a copy of the plan for that launch has q_start, kv_len and cap here, and its
+  // own in ``own_*`` (null otherwise).
+  const int* run_start;    // [2 x runs of many rows] first row, row behind the last
+  const int* run_len;      // [2 x ...] shared tokens
+  const int* run_seq;      // [2 x ...] sequence whose table is read
+  const int4* many;        // [many_count] work on them, as ``chunk``, or for e4m3 as ``one``
+  const int* own_q_start;
+  const int* own_kv_len;
+  const int* own_cap;
   int seqs, rows, width, page, group;
   int read_count, few_count, few_rows, few_parts, few_cluster, chunk_count, one_count, merge_count;
   int partial_rows;        // rows of the scratch for partial results (x heads)
-  int prefix_count, tail_count, tail_rows, join_count;
+  int prefix_count, tail_count, tail_rows, join_count, many_count;
   int unpack_count;        // also the 128-token pages of the scratch for unpacked rows
   int layout;              // PLAN_LAYOUT; changes with the fields
 };
@@ -76,8 +85,18 @@ __device__ __forceinline__ void report_grown(const Plan& p, int b, int* status) 
   if (p.kv_len[b] > p.cap[b]) report_status(status, kBadShape, 10);
 }
 
+// Pages of a sequence.
+__device__ __forceinline__ const int* table_of(const Plan& p, int b) {
+  return p.table + (long long)(p.own_q_start != nullptr ? p.run_seq[b] : b) * p.width;
+}
+
 // Keys that row ``token`` of a sequence may read.
 __device__ __forceinline__ int row_limit(const Plan& p, int q0, int q_len, int kv_len, int token) {
+  if (p.own_q_start != nullptr) {          // of a run's ``kv_len`` shared tokens
+    const int row = q0 + token, b = p.row_seq[row], len = max(0, min(p.own_kv_len[b], p.own_cap[b]));
+    const int behind = p.behind != nullptr ? p.behind[row] : p.own_q_start[b + 1] - 1 - row;
+    return max(0, min(min(kv_len, len), len - behind));
+  }
   const int behind = p.behind != nullptr ? p.behind[q0 + token] : q_len - 1 - token;
   return max(0, min(kv_len, kv_len - behind));
 }
@@ -125,8 +144,7 @@ int launch_widen(const Cache& c, const Plan& p, void* wide, float4* factors, cud
 int launch_chunks(const Cache& c, const Plan& p, const void* q, long long ldq, void* o, long long ldo, float* part,
                   float2* part_ml, float scale_log2, void* wide, const float4* factors, cudaStream_t st);
 // attn_prefix_sm100.cu: a plan's ``prefix`` items
-int launch_prefix(const Cache& c, const Plan& p, const void* q, long long ldq, float* part, float2* part_ml, float scale_log2, int beside,
-                  cudaStream_t st);
+int launch_prefix(const Cache& c, const Plan& p, const void* q, long long ldq, float* part, float2* part_ml, float scale_log2, int beside, cudaStream_t st);
 
 }  // namespace paged
 }  // namespace snu1

@@ -61,6 +61,8 @@ CHUNK_JOIN = 3           # what a part costs besides: 128 KB written and read ag
 PREFIX_ROWS = 64         # rows of a CTA of the kernel for shared tokens, which are counted in tiles of 128
 PREFIX_SLOTS = 148       # its CTAs that run at once
 PREFIX_LEAST = 2         # a part has at least this many key tiles
+# Us on an SM: to start and end a CTA of shared tokens, one of its tiles; the same for tails, of which three share the SM.
+PREFIX_START, PREFIX_TILE, TAIL_START, TAIL_TILE = 8.0, 1.1, 1.5, 0.8
 
 
 _ENTRY: dict = {}         # the entry points that calls go to
@@ -130,15 +132,16 @@ class PagedCache:
         return self._data.device
 
 
-PLAN_LAYOUT = 0x70670003     # last word of a plan: the library refuses one whose fields lie elsewhere
+PLAN_LAYOUT = 0x70670004     # last word of a plan: the library refuses one whose fields lie elsewhere
 
 
 class _Args(ctypes.Structure):
     """``Plan`` of csrc/paged.cuh."""
     _fields_ = ([(n, c_void_p) for n in ("q_start", "kv_len", "cap", "table", "behind", "row_seq", "k_start", "read_pages", "unpack",
-                                         "unpack_first", "few", "chunk", "one", "merge", "skip", "runs", "prefix", "tail", "joins")]
+                                         "unpack_first", "few", "chunk", "one", "merge", "skip", "runs", "prefix", "tail", "joins", "run_start", "run_len", "run_seq",
+                                         "many", "own_q_start", "own_kv_len", "own_cap")]
                 + [(n, c_int) for n in ("seqs", "rows", "width", "page", "group", "read_count", "few_count", "few_rows", "few_parts", "few_cluster",
-                                        "chunk_count", "one_count", "merge_count", "partial_rows", "prefix_count", "tail_count", "tail_rows", "join_count",
+                                        "chunk_count", "one_count", "merge_count", "partial_rows", "prefix_count", "tail_count", "tail_rows", "join_count", "many_count",
                                         "unpack_count", "layout")])
 
 
@@ -336,10 +339,10 @@ def _lay_out(q_lens, kv_lens, tables, page: int, pages: int, group: int, kv_head
     one, partial = chunks_of(single, tile_rows, partial)
     chunk, partial = chunks_of(chunked & ~single, 2 * tile_rows, partial)
     merge = np.concatenate(merge) if merge else np.zeros((0, 4), np.int32)
-    together = dict(skip=None, runs=None, prefix=None, tail=None, joins=None)
+    together = dict(skip=None, runs=None, prefix=None, tail=None, joins=None, run_start=None, run_len=None, run_seq=None, many=None)
     tail_rows = 0
     if runs:
-        together, tail_rows, partial = _together(runs, skip, q_rows, cap, start(q), group, kv_heads, partial)
+        together, tail_rows, partial = _together(runs, skip, q_rows, cap, start(q), group, kv_heads, fp8, partial)
     unpack = unpack_first = None
     if fp8 and len(chunk):
         wide = np.where(chunked & ~single, -(-cap // CHUNK_TILE), 0)    # 128-token pages
@@ -352,48 +355,62 @@ def _lay_out(q_lens, kv_lens, tables, page: int, pages: int, group: int, kv_head
     counts = dict(seqs=n, rows=rows, width=width, page=page, group=group, read_count=int(read.sum()), few_count=len(few),
                   few_rows=few_rows, few_parts=few_parts, few_cluster=cluster, chunk_count=len(chunk), one_count=len(one), merge_count=len(merge),
                   partial_rows=partial, prefix_count=len(together["prefix"]) if runs else 0, tail_count=len(together["tail"]) if runs else 0,
-                  tail_rows=tail_rows, join_count=len(together["joins"]) // 2 if runs else 0, unpack_count=0 if unpack is None else len(unpack), layout=PLAN_LAYOUT)
+                  tail_rows=tail_rows, join_count=len(together["joins"]) // 2 if runs else 0, many_count=len(together["many"]) if runs else 0,
+                  unpack_count=0 if unpack is None else len(unpack), layout=PLAN_LAYOUT)
     return arrays, counts
 
 
-def _together(runs, skip, q_rows, cap, q_start, group: int, heads: int, first: int):
-    """Work on tokens that runs of sequences share (prefix, by runs), on the other tokens of these sequences (tail), and the joins of both,
-    [row, head of the group, partial row, parts | partial row, parts, rows of a part, 0] for every row."""
-    run_rows = np.array([int(q_rows[a:a + n].sum()) for a, n, _ in runs])
-    run_skip = np.array([t for _, _, t in runs])
-    count = -(-run_rows // PREFIX_ROWS)
-    run = np.repeat(np.arange(len(runs)), count)
-    row0 = (np.arange(len(run)) - np.repeat(np.cumsum(count) - count, count)) * PREFIX_ROWS
-    tiles = run_skip[run] // CHUNK_TILE
-    own = np.where(skip > 0, cap - skip, 0)
-    # SMs by what there is to read
-    share = PREFIX_SLOTS * float(tiles.sum()) / float(tiles.sum() + own.sum() / CHUNK_TILE)
-    parts = _shares(tiles, heads, max(heads * len(tiles), int(share)), PREFIX_LEAST)
-    at = first + np.cumsum(parts * PREFIX_ROWS) - parts * PREFIX_ROWS
-    first += int((parts * PREFIX_ROWS).sum())
-    i = np.repeat(np.arange(len(run)), parts)
-    part = np.arange(len(i)) - np.repeat(np.cumsum(parts) - parts, parts)
-    prefix = np.stack([run[i], row0[i], part | parts[i] << 16, at[i] + part * PREFIX_ROWS], 1)
-    # every row of a run: partial rows of its part 0, and parts
-    seqs = np.concatenate([np.arange(a, a + n) for a, n, _ in runs])
-    of_run = np.repeat(np.arange(len(runs)), run_rows)
-    place = np.arange(len(of_run)) - np.repeat(np.cumsum(run_rows) - run_rows, run_rows)
-    item = (np.cumsum(count) - count)[of_run] + place // PREFIX_ROWS
-    joins = np.zeros((len(of_run), 8), dtype=np.int64)
-    joins[:, 0] = np.repeat([q_start[a] for a, _, _ in runs], run_rows) + place // group
-    joins[:, 1] = place % group
-    joins[:, 2] = at[item] + place % PREFIX_ROWS
-    joins[:, 3] = parts[item]
-    # tails
-    rows = q_rows[seqs]
+def _tails(q_rows, skip, cap, heads: int):
+    """Rows of a CTA of the tails, how many CTAs there are for a head, and their tiles of 128 keys."""
+    rows, own = np.where(skip > 0, q_rows, 0), cap - skip
     top = int(rows.max())
     m = 8 if top <= 8 else 16 if top <= 16 else FEW_TILE
+    count = -(-rows // m)
+    return m, int(count.sum()), int((count * -(-own // CHUNK_TILE)).sum())
+
+
+def _together(runs, skip, q_rows, cap, q_start, group: int, heads: int, fp8: bool, first: int):
+    """Work on tokens that runs of sequences share (prefix, and many for runs of more rows than that kernel's CTAs have), on the other tokens of these
+    sequences (tail), and the joins of both, [row, head of the group, partial row, parts | partial row, parts, rows of a part, rows of a part of the
+    shared tokens] for every row."""
+    runs = np.array([[q_start[a], q_start[a + n] - q_start[a], a, t, n] for a, n, t in runs])
+    rows, tokens = runs[:, 1] * group, runs[:, 3]
+    big = (rows > PREFIX_ROWS) & (group <= CHUNK_TILE)
+    m_tail, tail_ctas, tail_tiles = _tails(q_rows, skip, cap, heads)
+    whole = (CHUNK_TILE // group) * group if group <= CHUNK_TILE else 1
+    joins = np.zeros((int(rows.sum()), 8), dtype=np.int64)
+    of_run = np.repeat(np.arange(len(runs)), rows)
+    place = np.arange(len(of_run)) - np.repeat(np.cumsum(rows) - rows, rows)
+    joins[:, 0] = runs[of_run, 0] + place // group
+    joins[:, 1] = place % group
+    work = {}
+    for name, which, m in (("many", big, whole if fp8 else 2 * whole), ("prefix", ~big, PREFIX_ROWS)):
+        count = np.where(which, -(-rows // m), 0)
+        run = np.repeat(np.arange(len(runs)), count)
+        row0 = (np.arange(len(run)) - np.repeat(np.cumsum(count) - count, count)) * m
+        tiles = tokens[run] // CHUNK_TILE
+        parts = _waves(tiles, heads, CHUNK_SLOTS) if name == "many" else _prefix_parts(tiles, heads, tail_ctas, tail_tiles)
+        at = first + np.cumsum(parts * m) - parts * m
+        first += int((parts * m).sum())
+        i = np.repeat(np.arange(len(run)), parts)
+        part = np.arange(len(i)) - np.repeat(np.cumsum(parts) - parts, parts)
+        items = np.stack([run[i], row0[i], part | parts[i] << 16, at[i] + part * m], 1).reshape(-1, 4)
+        if name == "many":
+            items[:, 0] *= 2
+        work[name] = items.astype(np.int32)
+        here = which[of_run]                                      # every row of such a run: partial rows of its part 0, and parts
+        item = ((np.cumsum(count) - count)[of_run] + place // m)[here]
+        joins[here, 2] = at[item] + (place % m)[here]
+        joins[here, 3] = parts[item]
+        joins[here, 7] = m
+    # tails
+    seqs = np.concatenate([np.arange(r[2], r[2] + r[4]) for r in runs])
+    rows, m = q_rows[seqs], m_tail
     count = -(-rows // m)
     seq = np.repeat(seqs, count)
     row0 = (np.arange(len(seq)) - np.repeat(np.cumsum(count) - count, count)) * m
     tiles = -(-(cap - skip)[seq] // KEY_TILE)
-    slots = FEW_SLOTS[m > 8] * max(8, PREFIX_SLOTS - len(prefix) * heads) // PREFIX_SLOTS
-    parts = _shares(tiles, heads, slots, FEW_LEAST)
+    parts = _shares(tiles, heads, FEW_SLOTS[m > 8], FEW_LEAST)
     at = first + np.cumsum(parts * m) - parts * m
     first += int((parts * m).sum())
     i = np.repeat(np.arange(len(seq)), parts)
@@ -406,9 +423,29 @@ def _together(runs, skip, q_rows, cap, q_start, group: int, heads: int, first: i
     joins[:, 4] = at[item] + place % m
     joins[:, 5] = parts[item]
     joins[:, 6] = m
-    of = np.array([[q_start[a], q_start[a + n] - q_start[a], a, t] for a, n, t in runs])
-    return (dict(skip=skip.astype(np.int32), runs=of.astype(np.int32), prefix=prefix.astype(np.int32), tail=tail[order].astype(np.int32),
-                 joins=joins.reshape(-1, 4).astype(np.int32)), m, first)
+    twice = lambda x, y: np.stack([x, y], 1).reshape(-1).astype(np.int32)
+    return (dict(skip=skip.astype(np.int32), runs=runs[:, :4].astype(np.int32), tail=tail[order].astype(np.int32), joins=joins.reshape(-1, 4).astype(np.int32),
+                 run_start=twice(runs[:, 0], runs[:, 0] + runs[:, 1]), run_len=twice(tokens, tokens), run_seq=twice(runs[:, 2], runs[:, 2]), **work),
+            m, first)
+
+
+def _prefix_parts(tiles, heads: int, tail_ctas: int, tail_tiles: int):
+    """Into how many parts the work on shared tokens is split: done soonest, if its CTAs have an SM each, and tails what is left until those are
+    done, then all."""
+    if not len(tiles):
+        return tiles
+    best = None
+    for cut in range(1, 2 * PREFIX_SLOTS):
+        split = -(-tiles // -(-int(tiles.max()) // cut))
+        ctas = int(split.sum()) * heads
+        if best is not None and (ctas > PREFIX_SLOTS or int(tiles.max()) < PREFIX_LEAST * cut):
+            break
+        busy = -(-ctas // PREFIX_SLOTS) * (PREFIX_START + float((-(-tiles // split)).max()) * PREFIX_TILE)
+        left = (tail_ctas * TAIL_START + tail_tiles * TAIL_TILE) * heads - busy * max(0, PREFIX_SLOTS - ctas)
+        done = busy + (left / PREFIX_SLOTS + TAIL_START if left > 0 else 0.0)
+        if best is None or done < best[0]:
+            best = (done, split)
+    return best[1]
 
 
 def _waves(tiles: np.ndarray, heads: int, slots: int) -> np.ndarray:

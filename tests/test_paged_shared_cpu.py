@@ -72,7 +72,8 @@ def test_every_row_and_key_once(seed):
     grow = rng.choice((0, 0, 100))
     if grow:
         tables = [t + list(range(at + 100 * i, at + 100 * i + 100)) for i, t in enumerate(tables)]
-    a, c = lay(q, kv, tables, shared, page, group, heads, rng.random() < 0.5, grow=grow)
+    fp8 = rng.random() < 0.5
+    a, c = lay(q, kv, tables, shared, page, group, heads, fp8, grow=grow)
     rows, n = sum(q), len(q)
     q_start = np.concatenate([[0], np.cumsum(q)])
     direct = np.zeros(rows * group, dtype=int)                       # by few rows and chunks
@@ -82,7 +83,8 @@ def test_every_row_and_key_once(seed):
             if z & 0xffff == 0:
                 r = q_start[b] * group + row0
                 direct[r:min(r + m, q_start[b + 1] * group)] += 1
-    if c["prefix_count"] == 0:
+    if c["tail_count"] == 0:
+        assert c["prefix_count"] == c["many_count"] == 0
         assert (direct == 1).all()
         return
     used = np.zeros(c["partial_rows"], dtype=int)
@@ -95,6 +97,15 @@ def test_every_row_and_key_once(seed):
         used[first:first + 64] += 1
         for k in range(count):
             where.setdefault(t0 * group + row0 + k, []).append(("prefix", part, parts, first + k))
+    wide = (128 // group * group) * (1 if fp8 else 2)
+    for r, row0, z, first in a["many"].tolist():
+        part, parts = z & 0xffff, z >> 16
+        t0, end = a["run_start"][r:r + 2].tolist()
+        assert r % 2 == 0 and a["run_len"][r] % 128 == 0 and 0 <= part < parts <= a["run_len"][r] // 128 and row0 % group == 0
+        used[first:first + wide] += 1
+        assert end > t0 and (end - t0) * group > 64 and q_start[a["run_seq"][r]] == t0
+        for k in range(min(wide, (end - t0) * group - row0)):
+            where.setdefault(t0 * group + row0 + k, []).append(("many", part, parts, first + k))
     for b, row0, z, first in a["tail"].tolist():
         part, parts = z & 0xffff, z >> 16
         m = c["tail_rows"]
@@ -104,9 +115,11 @@ def test_every_row_and_key_once(seed):
             where.setdefault(q_start[b] * group + row0 + k, []).append(("tail", part, parts, first + k))
     assert used.max() <= 1
     joined = a["joins"].reshape(-1, 8)
-    for t, g, pre, parts, tail, tparts, m, _ in joined.tolist():
+    for t, g, pre, parts, tail, tparts, m, mpre in joined.tolist():
         have = sorted(where.pop(t * group + g))
-        assert have == sorted([("prefix", s, parts, pre + 64 * s) for s in range(parts)] + [("tail", s, tparts, tail + m * s) for s in range(tparts)])
+        name = have[0][0]
+        assert mpre == (64 if name == "prefix" else wide)
+        assert have == sorted([(name, s, parts, pre + mpre * s) for s in range(parts)] + [("tail", s, tparts, tail + m * s) for s in range(tparts)])
         direct[t * group + g] += 1
     assert not where and (direct == 1).all()
     for seq, t0 in zip(a["runs"][:, 2], a["runs"][:, 0]):

@@ -45,6 +45,22 @@ def queries(n, hq, seed=1, scale=1.0):
     return (torch.randn(n + 2, hq + 3, D, device="cuda", generator=g) * scale).to(BF16)[:, 1:hq + 1]
 
 
+def wider(room, q, q_lens, rows, limits, plan):
+    """Runs of more than 64 rows over e4m3 go to the kernel for chunks, which rounds code times scale of a key to fp16: 2^-11 of it, so a score
+    moves by 2^-11 of the sum of |q k| at most and a probability by exp of that, before and after the sum is divided by (see ``near``)."""
+    if plan._args.many_count == 0 or rows[0].dtype != torch.float64 or plan.dtype != E4M3:
+        return room
+    room, r = room.clone(), 0
+    for n, kv in zip(q_lens, rows):
+        if n and kv.shape[2]:
+            k = kv[0].repeat_interleave(q.shape[1] // kv.shape[1], 0)
+            hidden = torch.arange(kv.shape[2], device=q.device)[None] >= limits[r:r + n, None]
+            most = (torch.einsum("rhd,hkd->hrk", q[r:r + n].double().abs(), k.abs()) * SCALE).masked_fill(hidden, 0.0).amax(-1)
+            room[r:r + n] *= 1 + 2 * 2.0 ** -11 * most.T[..., None] / (2.0 ** -8 + 2.0 ** -11)
+        r += n
+    return room
+
+
 def check(groups, q_lens, hq, hk, page, dtype, limits=None, seed=0, scale=1.0):
     from sensenova_u1_b200.ops import paged
     cache, tables, kv, rows, shared = setup(groups, page, hk, dtype, seed)
@@ -55,7 +71,7 @@ def check(groups, q_lens, hq, hk, page, dtype, limits=None, seed=0, scale=1.0):
     paged.paged_attention(q, cache, plan, SCALE, out=out)
     lim = causal(q_lens, kv) if limits is None else torch.as_tensor(limits, device="cuda")
     ref, room = exact(q[:n], q_lens, rows, lim, dtype)
-    assert near(out[:n], ref, room)
+    assert near(out[:n], ref, wider(room, q[:n], q_lens, rows, lim, plan))
     assert (out[n:] == 7).all()
     assert (out[:n][lim == 0] == 0).all()
     assert torch.equal(paged.paged_attention(q, cache, plan, SCALE), out[:n])
@@ -70,7 +86,7 @@ BOTH = pytest.mark.parametrize("dtype", [BF16, E4M3])
 @pytest.mark.parametrize("n", [2, 3, 17])
 def test_one_token_each(n, hq, hk, dtype):
     plan = check([(700, [700 + 1 + 13 * i for i in range(n)])], [1] * n, hq, hk, 64, dtype)
-    assert plan._args.prefix_count > 0
+    assert plan._args.tail_count > 0
 
 
 @BOTH
@@ -93,7 +109,7 @@ def test_groups_with_chunks_and_others(dtype):
     groups = [(900, [950, 901, 1300]), (0, [40, 500]), (2000, [2001] * 9), (300, [310]), (640, [700, 900, 641, 800]), (129, [129 + 60, 200])]
     q = [1, 1, 2, 1, 3, *[1] * 9, 1, 1, 150, 2, 1, 60, 1]
     plan = check(groups, q, 8, 2, 16, dtype)
-    assert plan._args.prefix_count > 0 and plan._args.few_count > 0 and plan._args.chunk_count + plan._args.one_count > 0
+    assert plan._args.tail_count > 0 and plan._args.few_count > 0 and plan._args.chunk_count + plan._args.one_count > 0
 
 
 @BOTH
@@ -286,7 +302,7 @@ def test_tables_on_the_device(dtype):
     seen = [[list(x.split(lens)[r]) for r, b in enumerate(beams) for _ in range(b)] for x in kv]
     parents = torch.tensor([0] * 8 + [8] * 3, dtype=torch.int32, device="cuda")
     plan = paged.build_plan(caches[0], hq, [1] * n, [lens[0] + 1] * 8 + [lens[1] + 1] * 3, t, grow=30, shared=[(0, 8, lens[0]), (8, 3, lens[1])])
-    assert plan._args.prefix_count > 0
+    assert plan._args.tail_count > 0
     with pytest.raises(RuntimeError):
         plan.advance()
     new, q = torch.empty(2, n, 2 * hk, D, device="cuda", dtype=BF16), queries(n, hq)
