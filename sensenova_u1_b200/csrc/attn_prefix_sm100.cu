@@ -449,8 +449,7 @@ __global__ void __launch_bounds__(Prefix<FP8>::THREADS, 1)
     if (n_tiles > 0) issue_s(0);
     for (int n = 0; n < n_tiles; ++n) {          // all tiles also after a time-out
       if (n + 1 < n_tiles) issue_s(n + 1);
-      if (FP8) ok &= mbar_wait(&w_full[n % WS], (n / WS) & 1, abort_flag, args.status, 3);
-      else ok &= mbar_wait(&v_full[n % VS], (n / VS) & 1, abort_flag, args.status, 3);
+      ok &= mbar_wait(FP8 ? &w_full[n % WS] : &v_full[n % VS], FP8 ? (n / WS) & 1 : (n / VS) & 1, abort_flag, args.status, 3);
       ok &= mbar_wait(&p_full[n % PS], (n / PS) & 1, abort_flag, args.status, 2);
       tc_fence_after();
       const uint64_t vd = v_desc + (FP8 ? (n % WS) * (F::WIDE >> 4) : (n % VS) * (F::TILE >> 4)), pd = p_desc + (n % PS) * (F::P >> 4);
@@ -520,16 +519,16 @@ __global__ void __launch_bounds__(Prefix<FP8>::THREADS, 1)
         const float2 x = make_float2(c[0], c[p.page]);
         return fabsf(x.y) < INFINITY ? x : make_float2(__int_as_float(0x7fffffff), 0.f);
       };
-              // the registers' copies of what has changed in shared memory
-              auto take = [&](bool sums) {
-      #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                  if (i >= 4 * active) break;
-                  const int c = c0 + 2 * i;
-                  nm[i] = pack_f32x2(-sh.row[c].m, -sh.row[c + 1].m);
-                  if (sums) l2[i] = mul_f32x2(l2[i], pack_f32x2(sh.f[c], sh.f[c + 1]));
-                      }
-              };
+      // the registers' copies of what has changed in shared memory
+      auto take = [&](bool sums) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          if (i >= 4 * active) break;
+          const int c = c0 + 2 * i;
+          nm[i] = pack_f32x2(-sh.row[c].m, -sh.row[c + 1].m);
+          if (sums) l2[i] = mul_f32x2(l2[i], pack_f32x2(sh.f[c], sh.f[c + 1]));
+        }
+      };
       {
         // Where the maxima begin: at those of the first 32 keys (of a tile that the mask cuts: nowhere, see move_maxima).
         const int key = j0 * PK + in_tile;
@@ -575,84 +574,90 @@ __global__ void __launch_bounds__(Prefix<FP8>::THREADS, 1)
         const uint64_t ks2 = pack_f32x2(ks, ks), vs2 = pack_f32x2(sc.y, sc.y);
         uint8_t* P = sP + (n % PS) * F::P;
         ok &= mbar_wait(&s_full[n & 1], (n >> 1) & 1, abort_flag, args.status, 5);
-        if (n >= PS) ok &= mbar_wait(&pv_done[n % PS], ((n - PS) / PS) & 1, abort_flag, args.status, 6);
+        // P's place is free.  (e4m3: PV(n - 2) was asked for before S(n), by the same thread, so s_full says so.)
+        if (!FP8 && n > 0) ok &= mbar_wait(&pv_done[0], (n - 1) & 1, abort_flag, args.status, 6);
         __syncwarp();
         tc_fence_after();
         const uint32_t S = tmem + (n & 1) * F::S_COLS + c0 + lanes;
-#pragma unroll 1
-        for (int again = 0; again < 2; ++again) {
+        bool again = false;                      // the maxima have moved: once more
+        do {
           // Probabilities, and whether one is too large for where the maxima are; their products are written all the same, and once more after the
           // maxima have moved.
           float mx = -INFINITY, mw = -INFINITY;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            if (i >= active) break;
-            uint32_t h[8], lo[8];
-            tmem_ld_x8(S + 8 * i, h);
-            if (FP8) tmem_ld_x8(S + PR + 8 * i, lo);
-            uint4 rs4 = make_uint4(0, 0, 0, 0), vf4 = rs4;
-            if (FP8) {
-              rs4 = *reinterpret_cast<const uint4*>(sh.rs + c0 + 8 * i);
-              vf4 = *reinterpret_cast<const uint4*>(sh.vf + c0 + 8 * i);
-            }
-            const uint32_t rs2[4] = {rs4.x, rs4.y, rs4.z, rs4.w}, vf2[4] = {vf4.x, vf4.y, vf4.z, vf4.w};
-            tmem_ld_wait();
-            uint64_t y[4];                       // log2 units; product and difference are never fused
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              y[e] = pack_f32x2(__uint_as_float(h[2 * e]), __uint_as_float(h[2 * e + 1]));
+            if (i < active) {
+              uint32_t h[8], lo[8];
+              tmem_ld_x8(S + 8 * i, h);
+              if (FP8) tmem_ld_x8(S + PR + 8 * i, lo);
+              uint4 rs4 = make_uint4(0, 0, 0, 0), vf4 = rs4;
               if (FP8) {
-                y[e] = fma_f32x2(pack_f32x2(__uint_as_float(lo[2 * e]), __uint_as_float(lo[2 * e + 1])), sixteenth, y[e]);
-                y[e] = mul_f32x2(y[e], mul_f32x2(bf16x2_to_f32x2(rs2[e]), ks2));
-              } else {
-                y[e] = mul_f32x2(y[e], ks2);
+                rs4 = *reinterpret_cast<const uint4*>(sh.rs + c0 + 8 * i);
+                vf4 = *reinterpret_cast<const uint4*>(sh.vf + c0 + 8 * i);
               }
-              y[e] = add_f32x2(y[e], nm[4 * i + e]);
-            }
-            if (__builtin_expect(dirty, 0)) {
+              const uint32_t rs2[4] = {rs4.x, rs4.y, rs4.z, rs4.w}, vf2[4] = {vf4.x, vf4.y, vf4.z, vf4.w};
+              tmem_ld_wait();
+              uint64_t y[4];                       // log2 units; product and difference are never fused
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                y[e] = pack_f32x2(__uint_as_float(h[2 * e]), __uint_as_float(h[2 * e + 1]));
+                if (FP8) {
+                  y[e] = fma_f32x2(pack_f32x2(__uint_as_float(lo[2 * e]), __uint_as_float(lo[2 * e + 1])), sixteenth, y[e]);
+                  y[e] = mul_f32x2(y[e], mul_f32x2(bf16x2_to_f32x2(rs2[e]), ks2));
+                } else {
+                  y[e] = mul_f32x2(y[e], ks2);
+                }
+                y[e] = add_f32x2(y[e], nm[4 * i + e]);
+              }
+              if (__builtin_expect(dirty, 0)) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  float a, b;
+                  unpack_f32x2(y[e], a, b);
+                  const int2 lim = *reinterpret_cast<const int2*>(sh.lim + c0 + 8 * i + 2 * e);
+                  y[e] = pack_f32x2(key >= lim.x ? -INFINITY : a, key >= lim.y ? -INFINITY : b);
+                }
+              }
+              uint32_t u[4], v[4];
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
                 float a, b;
                 unpack_f32x2(y[e], a, b);
-                const int2 lim = *reinterpret_cast<const int2*>(sh.lim + c0 + 8 * i + 2 * e);
-                y[e] = pack_f32x2(key >= lim.x ? -INFINITY : a, key >= lim.y ? -INFINITY : b);
+                mx = max3(mx, a, b);
+                const float pa = fast_exp2(a), pb = fast_exp2(b);
+                const uint64_t pp = pack_f32x2(pa, pb);
+                p2[4 * i + e] = pp;
+                if (FP8) {
+                  float wa, wb;
+                  unpack_f32x2(mul_f32x2(mul_f32x2(pp, vs2), bf16x2_to_f32x2(vf2[e])), wa, wb);
+                  mw = max3(mw, wa, wb);
+                  u[e] = pack_f16x2(wa, wb);
+                } else {
+                  const uint32_t hi = pack_bf16x2(pa, pb);
+                  float ra, rb;
+                  unpack_f32x2(add_f32x2(pp, bf16x2_to_f32x2(hi ^ 0x80008000u)), ra, rb);
+                  u[e] = hi;
+                  v[e] = pack_bf16x2(ra, rb);
+                }
               }
+              const uint32_t to = swz128_offset(in_tile, side * 4 + i);
+              *reinterpret_cast<uint4*>(P + to) = make_uint4(u[0], u[1], u[2], u[3]);
+              if (!FP8) *reinterpret_cast<uint4*>(P + PK * 128 + to) = make_uint4(v[0], v[1], v[2], v[3]);
             }
-            uint32_t u[4], v[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              float a, b;
-              unpack_f32x2(y[e], a, b);
-              mx = max3(mx, a, b);
-              const float pa = fast_exp2(a), pb = fast_exp2(b);
-              const uint64_t pp = pack_f32x2(pa, pb);
-              p2[4 * i + e] = pp;
-              if (FP8) {
-                float wa, wb;
-                unpack_f32x2(mul_f32x2(mul_f32x2(pp, vs2), bf16x2_to_f32x2(vf2[e])), wa, wb);
-                mw = max3(mw, wa, wb);
-                u[e] = pack_f16x2(wa, wb);
-              } else {
-                const uint32_t hi = pack_bf16x2(pa, pb);
-                float ra, rb;
-                unpack_f32x2(add_f32x2(pp, bf16x2_to_f32x2(hi ^ 0x80008000u)), ra, rb);
-                u[e] = hi;
-                v[e] = pack_bf16x2(ra, rb);
-              }
+          }
+          if (__builtin_expect(named_bar_any(2 + side, 128, !again && (mx > P_MOST || mw > 32768.f)), 0)) {
+            if (n > 0) {
+              ok &= mbar_wait(&pv_done[(n - 1) % PS], ((n - 1) / PS) & 1, abort_flag, args.status, 6);
+              __syncwarp();
+              tc_fence_after();
             }
-            const uint32_t to = swz128_offset(in_tile, side * 4 + i);
-            *reinterpret_cast<uint4*>(P + to) = make_uint4(u[0], u[1], u[2], u[3]);
-            if (!FP8) *reinterpret_cast<uint4*>(P + PK * 128 + to) = make_uint4(v[0], v[1], v[2], v[3]);
+            move_maxima<FP8>(sh, S, tmem + F::O_AT + lanes, side, active, key, ks, FP8 ? log2_of(sc.y) : 0.f, dirty, n == 0);
+            take(true);
+            again = true;
+          } else {
+            again = false;
           }
-          if (__builtin_expect(!named_bar_any(2 + side, 128, again == 0 && (mx > P_MOST || mw > 32768.f)), 1)) break;
-          if (n > 0) {
-            ok &= mbar_wait(&pv_done[(n - 1) % PS], ((n - 1) / PS) & 1, abort_flag, args.status, 6);
-            __syncwarp();
-            tc_fence_after();
-          }
-          move_maxima<FP8>(sh, S, tmem + F::O_AT + lanes, side, active, key, ks, FP8 ? log2_of(sc.y) : 0.f, dirty, n == 0);
-          take(true);
-        }
+        } while (again);
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&s_empty[n & 1]);
@@ -689,7 +694,6 @@ __global__ void __launch_bounds__(Prefix<FP8>::THREADS, 1)
       // sums over the keys' threads, then the output
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        if (i >= 4 * active) break;
         float a, b;
         unpack_f32x2(l2[i], a, b);
 #pragma unroll

@@ -398,15 +398,32 @@ class NEOChatModel:
                 "top_p": gc.get("top_p", 1.0) or 1.0, "top_k": gc.get("top_k", 0) or 0, "repetition_penalty": rp,
                 "seed": gc.get("seed")}
 
+    @staticmethod
+    def _beams(gc: dict) -> Optional[dict]:
+        """Knobs of a beam search (``num_beams / num_return_sequences / length_penalty / early_stopping``); None where there is one beam."""
+        beams, best = int(gc.get("num_beams", 1) or 1), int(gc.get("num_return_sequences", 1) or 1)
+        if beams == 1:
+            if best != 1:
+                raise ValueError("num_return_sequences needs a beam search (num_beams)")
+            return None
+        if gc.get("do_sample", False) or float(gc.get("repetition_penalty", 1.0) or 1.0) != 1.0:
+            raise ValueError("a beam search neither samples nor penalises repetition")
+        penalty = gc.get("length_penalty")
+        return {"beams": beams, "best": best, "length_penalty": 1.0 if penalty is None else float(penalty),
+                "early_stopping": gc.get("early_stopping") or False}
+
     @torch.no_grad()
     def chat(self, tokenizer, pixel_values, question, generation_config=None, history=None, return_history=False,
              system_message=None, **kw):
-        """Answer to ``question`` about ``pixel_values`` (None, one [3,H,W] tensor, or a list): greedy, or sampled
-        when ``generation_config`` has ``do_sample`` (with ``temperature``, ``top_p``, ``top_k``, ``seed``), as the
+        """Answer to ``question`` about ``pixel_values`` (None, one [3,H,W] tensor, or a list): greedy, sampled
+        when ``generation_config`` has ``do_sample`` (with ``temperature``, ``top_p``, ``top_k``, ``seed``), or the best of a beam
+        search (``num_beams``, ``length_penalty``, ``early_stopping``), as the
         reference's ``chat`` forwards them to ``generate`` (modeling_neo_chat.py:1862-1914)."""
         gc = dict(generation_config or {})
         gc.update({k: v for k, v in kw.items() if k in ("do_sample", "temperature", "top_p", "top_k", "repetition_penalty",
-                                                       "seed", "max_new_tokens")})
+                                                       "seed", "max_new_tokens", "num_beams", "length_penalty", "early_stopping")})
+        if gc.get("num_return_sequences") not in (None, 1):
+            raise ValueError("chat gives one answer")
         images = [] if pixel_values is None else (list(pixel_values) if isinstance(pixel_values, (list, tuple)) else [pixel_values])
         n_marked = question.count("<image>") + sum(q.count("<image>") + (a or "").count("<image>") for q, a in (history or []))
         if images and n_marked == 0:
@@ -416,7 +433,7 @@ class NEOChatModel:
             turns += [("user", q), ("assistant", a)]
         ids, x, pos3 = self._embed_prompt(tokenizer, question, images, system=system_message, history=turns)
         eos = int(_encode(tokenizer, prompts.IM_END)[-1])
-        out = self._generate_ids(ids, x, pos3, int(gc.get("max_new_tokens", 256)), (eos,), self._sampling(gc))
+        out = self._generate_ids(ids, x, pos3, int(gc.get("max_new_tokens", 256)), (eos,), self._sampling(gc), self._beams(gc))[0]
         if out and out[-1] == eos:
             out = out[:-1]
         text = tokenizer.decode(out) if hasattr(tokenizer, "decode") else out
@@ -424,9 +441,12 @@ class NEOChatModel:
             return text, (history or []) + [(question, text)]
         return text
 
-    def _generate_ids(self, ids, x, pos3, max_new_tokens, stop_ids, sampling):
+    def _generate_ids(self, ids, x, pos3, max_new_tokens, stop_ids, sampling, beams=None):
+        """New tokens: one list, or the best of a beam search."""
+        if beams is not None:
+            return [t for t, _ in self.engine.beam_search([ids], max_new_tokens=max_new_tokens, stop_ids=stop_ids, docs_embeds=[x], docs_pos3=[pos3], **beams)[0]]
         lay, h = self.engine.prefill([ids], reserve_image_tokens=max_new_tokens, docs_embeds=[x], docs_pos3=[pos3])
-        return self.engine.decode(lay, h, max_new_tokens, stop_ids=stop_ids, sampling=sampling, prompt_ids=[ids])[0]
+        return self.engine.decode(lay, h, max_new_tokens, stop_ids=stop_ids, sampling=sampling, prompt_ids=[ids])
 
     @torch.no_grad()
     def generate(self, pixel_values=None, input_ids=None, grid_hw=None, attention_mask=None, visual_features=None,
@@ -435,7 +455,9 @@ class NEOChatModel:
         [1, N] already holds the ``<IMG_CONTEXT>`` runs; ``pixel_values`` are the flattened 16x16 patches of all
         images in block-major order with ``grid_hw`` [n_images, 2] patch grids (or ``visual_features`` = their
         embeddings).  Returns the new token ids [1, n_new].  Knobs: ``max_new_tokens``, ``eos_token_id``,
-        ``do_sample``, ``temperature``, ``top_p``, ``top_k``, ``seed`` (in ``generation_config`` or as keywords)."""
+        ``do_sample``, ``temperature``, ``top_p``, ``top_k``, ``seed`` (in ``generation_config`` or as keywords); for a beam search ``num_beams``,
+        ``length_penalty``, ``early_stopping`` and ``num_return_sequences`` (rows, best first, filled up with ``pad_token_id``,
+        by default the first ending token)."""
         if input_ids is None or input_ids.shape[0] != 1:
             raise ValueError("generate takes one sequence: input_ids of shape [1, N]")
         if self.img_context_token_id is None:
@@ -461,8 +483,11 @@ class NEOChatModel:
             x.index_copy_(0, dev_rows, visual_features.expand(rows.numel(), -1))       # x is this call's own copy
         eos = gc.get("eos_token_id")
         stops = tuple(eos) if isinstance(eos, (list, tuple)) else ((int(eos),) if eos is not None else ())
-        out = self._generate_ids(ids, x, pos3, int(gc.get("max_new_tokens", 256) or 256), stops, self._sampling(gc))
-        return torch.tensor([out], dtype=torch.long)
+        out = self._generate_ids(ids, x, pos3, int(gc.get("max_new_tokens", 256) or 256), stops, self._sampling(gc), self._beams(gc))
+        pad = gc.get("pad_token_id")
+        pad = int(pad) if pad is not None else stops[0] if stops else 0
+        longest = max(len(o) for o in out)
+        return torch.tensor([list(o) + [pad] * (longest - len(o)) for o in out], dtype=torch.long)
 
 
 class ByteTokenizer:

@@ -23,7 +23,7 @@ from ..data.batch import apply_time_schedule
 from ..models import oracle
 from ..models.engine import Workspace
 from ..models.params import GEN, UND, ParamStore
-from ..ops import _lib, attention as attn_ops, decode_stack, fused, gemm, moe, paged
+from ..ops import _lib, attention as attn_ops, beam, decode_stack, fused, gemm, moe, page_tables, paged
 from ..ops._lib import c_float, c_int, c_void_p
 
 CFG_NORMS = {"none": 0, "global": 1, "channel": 2, "cfg_zero_star": 3}
@@ -364,6 +364,83 @@ class InferenceEngine:
         # a graph keeps the addresses that it was captured with, and the engine's buffers are replaced when a step needs larger ones
         ws = Workspace(self.dev) if torch.cuda.is_current_stream_capturing() else None
         return self.layers(x, UND, pos3.to(self.dev).int().contiguous(), plan, None, 0, caches=caches, ws=ws).clone()
+
+    # ------------------------------------------------------------ beam search
+    @torch.no_grad()
+    def beam_search(self, docs_ids: Sequence[torch.Tensor], beams: int, max_new_tokens: int, stop_ids: Sequence[int] = (),
+                    length_penalty: float = 1.0, early_stopping=False, best: int = 1, docs_embeds: Optional[Sequence[torch.Tensor]] = None,
+                    docs_pos3: Optional[Sequence[torch.Tensor]] = None, page: int = 64, dtype=torch.bfloat16, use_graph: bool = True,
+                    check_every: int = 8):
+        """The ``best`` continuations of every prompt by a search with ``beams`` beams: per prompt a list of (token ids, score), best first, a
+        stop token (up to eight) the last of its continuation.  A finished continuation counts ``sum of log probabilities / tokens ** length_penalty``;
+        ``early_stopping`` as in :class:`ops.beam.BeamSearch`.  ``docs_embeds`` / ``docs_pos3``: as in :meth:`prefill`.
+
+        All beams of a prompt read its keys and values from the same pages (``page`` tokens of ``dtype``), once for all of them; a step (selection,
+        block tables, layers, head) runs without a look by the host and is captured in a CUDA graph, and every ``check_every`` steps the host asks whether
+        all prompts are done."""
+        n, lens = len(docs_ids), [int(d.numel()) for d in docs_ids]
+        if n == 0 or min(lens) < 1 or max_new_tokens < 1 or n * beams > page_tables.MAX_SEQS:
+            raise ValueError(f"beam_search needs prompts, new tokens, and at most {page_tables.MAX_SEQS} beams in all")
+        if page not in paged.PAGE_SIZES:
+            raise ValueError(f"a page holds 16, 32, 64 or 128 tokens, not {page}")
+        if not 1 <= best <= beams:
+            raise ValueError(f"1 to {beams} continuations")
+        cfg, dev, seqs = self.cfg, self.dev, n * beams
+        search = beam.BeamSearch(n, beams, max_new_tokens, stop_ids, length_penalty, early_stopping, dev)
+        pages = sum(m // page + beams * (-(-(m + max_new_tokens) // page) - m // page) for m in lens)
+        caches = self.paged_caches(pages, page, dtype)
+        tables = page_tables.PageTables(caches, seqs, max(lens) + max_new_tokens)
+
+        # the prompts, each in the pages of its first beam
+        q = [m if b == 0 else 0 for m in lens for b in range(beams)]
+        pos3, limits, next_pos = None, None, lens
+        if docs_pos3 is not None:
+            pos3 = torch.cat([p.cpu() for p in docs_pos3], dim=1).int()
+            limits, next_pos = [], []
+            for p in docs_pos3:
+                t = p[0].cpu()
+                # tokens that share a t index see one another (a picture), as in prefill
+                end = torch.searchsorted(t.contiguous(), t.contiguous(), right=True)
+                limits += end.tolist()
+                next_pos.append(int(t[-1]) + 1)
+        q_dev, nobody, pos = upload(dev, torch.tensor(q, dtype=torch.int32), torch.full((seqs,), -1, dtype=torch.int32),
+                                    torch.tensor(next_pos, dtype=torch.int32).repeat_interleave(beams))
+        tables.step(q_dev, parents=nobody)
+        plan = paged.build_plan(caches[0], cfg.num_heads, q, q, tables, limits=limits)
+        ids = None if docs_embeds is not None else upload(dev, torch.cat([d.cpu() for d in docs_ids]).long())[0]
+        h = self.paged_step(plan, caches, ids, None if docs_embeds is None else torch.cat(list(docs_embeds)), pos3)
+        last = upload(dev, (torch.tensor(lens).cumsum(0) - 1).repeat_interleave(beams))[0]
+        logits = torch.empty(seqs, self.p["lm_head"].shape[0], dtype=torch.float32, device=dev)
+
+        def head(hidden):
+            gemm.gemm_nt(self.final_norm(hidden, UND), self.p["lm_head"], out=logits, out_mode=gemm.OUT_F32_STORE)
+
+        head(h.index_select(0, last))
+        if max_new_tokens > 1:
+            plan = paged.build_plan(caches[0], cfg.num_heads, [1] * seqs, [m + 1 for m in lens for _ in range(beams)], tables, grow=max_new_tokens - 2,
+                                    shared=[(i * beams, beams, m) for i, m in enumerate(lens)])
+        zeros = torch.zeros_like(pos)
+
+        def step_fn():
+            search.advance(logits)
+            tables.step(1, parents=search.parents)
+            head(self.paged_step(plan, caches, ids=search.tokens, pos3=torch.stack([pos, zeros, zeros])))
+            pos.add_(1)
+
+        graph = None
+        for done in range(1, max_new_tokens):
+            if graph is not None:
+                graph.replay()
+            else:
+                step_fn()                       # eager: also warms every lazy initialisation
+                if use_graph and self.offload is None and max_new_tokens > 3:
+                    graph = self._capture(step_fn)
+            if done % check_every == 0 and search.finished():
+                break
+        else:
+            search.advance(logits)
+        self.last_decode_graph = graph is not None
+        return search.result(best)
 
     # ------------------------------------------------------------ text decoding
     def decode_greedy(self, layouts: List[DocLayout], last_hidden, max_new_tokens: int,
