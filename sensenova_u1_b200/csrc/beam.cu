@@ -15,6 +15,8 @@
 #include <math.h>
 #include <string.h>
 
+#include <mutex>
+
 #include "host_common.h"
 #include "sm100_common.cuh"
 
@@ -110,8 +112,11 @@ __global__ void __launch_bounds__(THREADS) pick_kernel(const PickArgs a) {
   const auto key = [&](float y, int j) -> unsigned long long {
     return y == -INFINITY ? 0ull : (unsigned long long)order32(y) << 32 | (uint32_t)~token(j);
   };
-  unsigned long long best = key(top, at);
-  s_top[tid] = best;
+  const unsigned long long best = key(top, at);
+  const int G = 1 << a.groups_log, share = THREADS >> a.groups_log;
+  unsigned long long mine = best;                      // of the group: neighbouring threads
+  for (int o = 1; o < share; o <<= 1) mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, o));
+  if ((tid & (share - 1)) == 0) s_top[tid / share] = mine;
   float m = top;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
@@ -125,18 +130,12 @@ __global__ void __launch_bounds__(THREADS) pick_kernel(const PickArgs a) {
     nan |= s_max[w] != s_max[w];
     m = fmaxf(m, s_max[w]);
   }
-  // the bound: of 2^groups_log groups the keep-th largest value, found by counting those above each; 256 >> groups_log threads share a count
-  const int G = 1 << a.groups_log, share = THREADS >> a.groups_log;
+  // the bound: of 2^groups_log groups the keep-th largest value, found by counting those above each; the threads of a group share the count
   {
-    const int g = tid / share, sub = tid % share;
-    unsigned long long mine = 0;
-    for (int i = 0; i < share; ++i) mine = max(mine, s_top[g * share + i]);
+    const int sub = tid & (share - 1);
     int above = 0;
-    for (int i = sub * (G / share); i < (sub + 1) * (G / share); ++i) {
-      unsigned long long other = 0;
-      for (int k = 0; k < share; ++k) other = max(other, s_top[i * share + k]);
-      above += other > mine;
-    }
+#pragma unroll 4
+    for (int i = sub; i < G; i += share) above += s_top[i] > mine;
     for (int o = 1; o < share; o <<= 1) above += __shfl_xor_sync(0xffffffffu, above, o);
     if (sub == 0 && above == a.keep - 1 && mine > 0) s_bound = mine;      // (keys are different unless they are 0)
   }
@@ -184,7 +183,9 @@ __global__ void __launch_bounds__(THREADS) pick_kernel(const PickArgs a) {
 }
 
 constexpr int JOIN_THREADS = 512;
+constexpr int JOIN_LISTS = 1280;     // lists with candidates whose heads are held; of more the bound is that of every thread's best head
 constexpr int JOIN_LIST = 1024;      // candidates that are ranked by counting; more than that are taken one by one
+constexpr int JOIN_GROUPS = 256;     // values that the bound is found among, by counting
 constexpr int MAX_BEAMS = 64;
 
 // A search's state (all on the device); see ops/beam.py.
@@ -313,27 +314,43 @@ __device__ void follow(const JoinArgs& a, int r, Chosen& c) {
   if (tid == 0 && c.done == 2) s.done[r] = 1;
 }
 
+// The heads of the lists while the bound is looked for, then the candidates above it.
+struct JoinShared {
+  double lse[MAX_BEAMS];
+  Best list[JOIN_LISTS > JOIN_LIST ? JOIN_LISTS : JOIN_LIST];
+  Best top[JOIN_THREADS];
+  short id[JOIN_LISTS];
+  Best bound;
+  int heads, count;
+  Chosen out;
+};
+
 __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const JoinArgs a) {
-  __shared__ double s_lse[MAX_BEAMS];
-  __shared__ Best s_list[JOIN_LIST];
-  __shared__ Best s_top[JOIN_THREADS];
-  __shared__ Best s_bound;
-  __shared__ int s_count;
-  __shared__ Chosen s_out;
+  extern __shared__ unsigned long long s_raw[];
+  JoinShared& sh = *reinterpret_cast<JoinShared*>(s_raw);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = blockIdx.x, K = a.beams, keep = a.keep;
   if (tid == 0) {
-    s_count = 0;
-    s_bound = Best{1, 0, 0xffffffffu};                    // everything that is a candidate
+    sh.heads = sh.count = 0;
+    sh.bound = Best{1, 0, 0xffffffffu};                    // everything that is a candidate
   }
   for (int i = tid; i < keep; i += JOIN_THREADS) {
-    s_out.score[i] = -INFINITY;
-    s_out.beam[i] = s_out.token[i] = 0;
+    sh.out.score[i] = -INFINITY;
+    sh.out.beam[i] = sh.out.token[i] = 0;
   }
   pdl_wait();
   pdl_trigger();
+  const int lists = K * a.slices;
+  const unsigned long long* cand = a.cand + (long long)r * lists * keep;
+  // the first list's head of this thread is on its way while the normalisers are made
+  const unsigned long long first = tid < lists ? cand[(long long)tid * keep] : 0ull;
   // normalisers: NaN where the row has no candidates
   for (int b = warp; b < K; b += JOIN_THREADS / 32) {
     const Part* p = a.part + ((long long)r * K + b) * a.slices;
+    const float base = a.scores[(long long)r * K + b];
+    if (!(fabsf(base) < INFINITY)) {                       // (a beam that is not there)
+      if (lane == 0) sh.lse[b] = (double)NAN;
+      continue;
+    }
     float m = -INFINITY;
     bool bad = false;
     for (int i = lane; i < a.slices; i += 32) {
@@ -349,53 +366,107 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const JoinArgs a) {
         if (p[i].max > -INFINITY) sum += p[i].sum * exp((double)p[i].max - (double)m);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) s_lse[b] = bad ? (double)NAN : (double)m + log(sum);
+    if (lane == 0) sh.lse[b] = bad ? (double)NAN : (double)m + log(sum);
   }
   __syncthreads();
-  const int lists = K * a.slices;
-  const unsigned long long* cand = a.cand + (long long)r * lists * keep;
-  // entry ``i`` of a list as a candidate; a place without one has s = 0
-  auto entry = [&](int list, int i) -> Best {
-    const unsigned long long k = i < keep ? cand[(long long)list * keep + i] : 0ull;
-    const int b = list / a.slices;
-    const double score = (double)a.scores[(long long)r * K + b] + ((double)value32((uint32_t)(k >> 32)) - s_lse[b]);
+  // a candidate; s = 0 if it is none
+  auto made = [&](unsigned long long k, int b) -> Best {
+    const double score = (double)a.scores[(long long)r * K + b] + ((double)value32((uint32_t)(k >> 32)) - sh.lse[b]);
     const bool on = k != 0 && score > -INFINITY && score < INFINITY;              // (false for NaN)
     return Best{on ? order64(score) : 0ull, k, (uint32_t)b};
   };
-  // a bound from the heads of every thread's lists
+  auto entry = [&](int list, int i) -> Best { return made(i < keep ? cand[(long long)list * keep + i] : 0ull, list / a.slices); };
+  // the heads of all lists that have any
   Best mine{0, 0, 0};
   for (int l = tid; l < lists; l += JOIN_THREADS) {
-    const Best e = entry(l, 0);
+    const Best e = l == tid ? made(first, l / a.slices) : entry(l, 0);
+    if (e.s == 0) continue;
     if (before(e, mine)) mine = e;
-  }
-  s_top[tid] = mine;
-  __syncthreads();
-  const int groups = min(lists, JOIN_THREADS);            // (the other threads have none)
-  if (tid < groups && mine.s != 0) {
-    int above = 0;
-    for (int i = 0; i < groups; ++i) above += before(s_top[i], mine);
-    if (above == keep - 1) s_bound = mine;
-  }
-  __syncthreads();
-  const Best bound = s_bound;
-  for (int l = tid; l < lists; l += JOIN_THREADS)
-    for (int i = 0; i < keep; ++i) {
-      const Best e = entry(l, i);
-      if (e.s == 0 || before(bound, e)) break;            // sorted: so is the rest
-      const int at = atomicAdd(&s_count, 1);
-      if (at < JOIN_LIST) s_list[at] = e;
+    const int at = atomicAdd(&sh.heads, 1);
+    if (at < JOIN_LISTS) {
+      sh.list[at] = e;
+      sh.id[at] = (short)min(l, 32767);                    // (not read if there are more lists than fit)
     }
+  }
   __syncthreads();
-  const int n = s_count;
+  const int heads = sh.heads;
+  const bool held = heads <= JOIN_LISTS && lists <= 32767;
+  // The bound.  d entries of a list are at least as good as its d-th, so of the lists' d-th entries (or of the best of groups of lists) the
+  // ceil(keep / d)-th largest has ``keep`` candidates that are not behind it.
+  int values = JOIN_THREADS, nth = keep;
+  if (held) {
+    const int d = heads == 0 ? 1 : (keep + heads - 1) / heads, groups = min(heads, JOIN_GROUPS);
+    nth = (keep + d - 1) / d;
+    values = groups;
+    mine = Best{0, 0, 0};
+    if (tid < groups)
+      for (int i = tid; i < heads; i += groups) {
+        const Best e = d == 1 ? sh.list[i] : entry(sh.id[i], d - 1);
+        if (before(e, mine)) mine = e;
+      }
+  }
+  sh.top[tid] = mine;
+  __syncthreads();
+  // a value's place is counted by as many threads as there are for it (a power of two, neighbours)
+  {
+    int share = 1;
+    while (2 * share * values <= JOIN_THREADS && share < 32) share *= 2;
+    const int v = tid / share, sub = tid % share;
+    const Best e = v < values ? sh.top[v] : Best{0, 0, 0};
+    int above = 0;
+    if (e.s != 0)
+      for (int i = sub; i < values; i += share) above += before(sh.top[i], e);
+    for (int o = 1; o < share; o <<= 1) above += __shfl_xor_sync(0xffffffffu, above, o);
+    if (sub == 0 && e.s != 0 && above == nth - 1) sh.bound = e;
+  }
+  __syncthreads();
+  const Best bound = sh.bound;
+  // What is not behind it.  (Heads and candidates share their place, so the heads are looked at again first.)
+  constexpr int OWN = (JOIN_LISTS + JOIN_THREADS - 1) / JOIN_THREADS, DEEP = 4;
+  int go[OWN];
+#pragma unroll
+  for (int k = 0; k < OWN; ++k) {
+    const int i = k * JOIN_THREADS + tid;
+    go[k] = held && i < heads && !before(bound, sh.list[i]) ? sh.id[i] : -1;
+  }
+  __syncthreads();
+  auto walk = [&](int l) {
+    const int b = l / a.slices;
+    for (int i0 = 0; i0 < keep; i0 += DEEP) {
+      unsigned long long k[DEEP];
+#pragma unroll
+      for (int i = 0; i < DEEP; ++i) k[i] = i0 + i < keep ? cand[(long long)l * keep + i0 + i] : 0ull;
+#pragma unroll
+      for (int i = 0; i < DEEP; ++i) {
+        const Best e = made(k[i], b);
+        if (e.s == 0 || before(bound, e)) return;          // sorted: so is the rest
+        const int at = atomicAdd(&sh.count, 1);
+        if (at < JOIN_LIST) sh.list[at] = e;
+      }
+    }
+  };
+  if (held) {
+#pragma unroll
+    for (int k = 0; k < OWN; ++k)
+      if (go[k] >= 0) walk(go[k]);
+  } else {
+    for (int l = tid; l < lists; l += JOIN_THREADS) walk(l);
+  }
+  __syncthreads();
+  const int n = sh.count;
   if (n <= JOIN_LIST) {
-    for (int i = tid; i < n; i += JOIN_THREADS) {
-      const Best e = s_list[i];
+    int share = 1;                                         // threads for one candidate
+    while (2 * share * n <= JOIN_THREADS && share < 32) share *= 2;
+    for (int i0 = 0; i0 < n; i0 += JOIN_THREADS / share) {
+      const int i = i0 + tid / share, sub = tid % share;
+      const Best e = i < n ? sh.list[i] : Best{0, 0, 0};
       int rank = 0;
-      for (int k = 0; k < n; ++k) rank += before(s_list[k], e);
-      if (rank < keep) {
-        s_out.score[rank] = (float)value64(e.s);
-        s_out.beam[rank] = (int)e.beam;
-        s_out.token[rank] = (int)~(uint32_t)e.key;
+      for (int k = sub; k < n; k += share) rank += before(sh.list[k], e);
+      for (int o = 1; o < share; o <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
+      if (sub == 0 && i < n && rank < keep) {
+        sh.out.score[rank] = (float)value64(e.s);
+        sh.out.beam[rank] = (int)e.beam;
+        sh.out.token[rank] = (int)~(uint32_t)e.key;
       }
     }
   } else {
@@ -408,35 +479,35 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const JoinArgs a) {
         for (int i = 0; i < keep; ++i) {
           const Best e = entry(l, i);
           if (e.s == 0) break;
-          if (!before(last, e)) continue;                 // taken
+          if (!before(last, e)) continue;                  // taken
           if (before(e, next)) next = e;
           break;
         }
       __syncthreads();
-      s_top[tid] = next;
+      sh.top[tid] = next;
       __syncthreads();
       for (int o = JOIN_THREADS / 2; o > 0; o >>= 1) {
-        if (tid < o && before(s_top[tid + o], s_top[tid])) s_top[tid] = s_top[tid + o];
+        if (tid < o && before(sh.top[tid + o], sh.top[tid])) sh.top[tid] = sh.top[tid + o];
         __syncthreads();
       }
-      last = s_top[0];
+      last = sh.top[0];
       if (last.s == 0) break;
       if (tid == 0) {
-        s_out.score[c] = (float)value64(last.s);
-        s_out.beam[c] = (int)last.beam;
-        s_out.token[c] = (int)~(uint32_t)last.key;
+        sh.out.score[c] = (float)value64(last.s);
+        sh.out.beam[c] = (int)last.beam;
+        sh.out.token[c] = (int)~(uint32_t)last.key;
       }
     }
   }
   __syncthreads();
   if (a.has_state) {
-    follow(a, r, s_out);
+    follow(a, r, sh.out);
     return;
   }
   for (int i = tid; i < keep; i += JOIN_THREADS) {
-    a.out_scores[(long long)r * keep + i] = s_out.score[i];
-    a.out_beams[(long long)r * keep + i] = s_out.beam[i];
-    a.out_tokens[(long long)r * keep + i] = s_out.token[i];
+    a.out_scores[(long long)r * keep + i] = sh.out.score[i];
+    a.out_beams[(long long)r * keep + i] = sh.out.beam[i];
+    a.out_tokens[(long long)r * keep + i] = sh.out.token[i];
   }
 }
 
@@ -510,6 +581,12 @@ SNU1_API int snu1_beam_step(const void* logits, long long ld, int is_bf16, int V
     j.has_state = 1;
     memcpy(&j.st, state, sizeof(State));
   }
-  SNU1_CUDA_CHECK(launch_pdl(join_kernel, dim3(requests), dim3(JOIN_THREADS), 0, st, j));
+  int dev = 0;
+  SNU1_CUDA_CHECK(cudaGetDevice(&dev));
+  static std::once_flag once[64];
+  cudaError_t err = cudaSuccess;
+  std::call_once(once[dev & 63], [&]() { err = cudaFuncSetAttribute(join_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(JoinShared)); });
+  SNU1_CUDA_CHECK(err);
+  SNU1_CUDA_CHECK(launch_pdl(join_kernel, dim3(requests), dim3(JOIN_THREADS), sizeof(JoinShared), st, j));
   return kHostOk;
 }
