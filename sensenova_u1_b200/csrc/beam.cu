@@ -9,8 +9,9 @@
 // CTA per request: the rows' normalisers, the slices' lists (sorted, so their heads give a bound the same way), the ``keep``
 // best by score, and the beams' bookkeeping, so that a whole step is captured without a look by the host.
 //
-// Candidates of different beams may be closer than fp32 tells apart: a slice's sum is of fp32 terms (the exponent's product with log2 e in
-// two parts), from 32 terms on in 64 bits, and scores are compared in 64 bits.  Equal scores: the lower beam, then the lower token.
+// Candidates of different beams may be closer than fp32 tells apart: a slice's sum is of fp32 terms, from 32 terms on in 64 bits (the largest
+// term of a row is 1 exactly, the errors of the others, 2^-22 of each at most, are of either sign: 1e-8 of the normaliser where they were measured),
+// and scores are compared in 64 bits.  Equal scores: the lower beam, then the lower token.
 // A row with NaN, + inf or nothing but - inf has no candidates.
 #include <math.h>
 #include <string.h>
@@ -96,18 +97,16 @@ __global__ void __launch_bounds__(THREADS) pick_kernel(const PickArgs a) {
       for (int e = 0; e < VEC; ++e) v[j * VEC + e] = i + e < a.V ? (float)x[i + e] : -INFINITY;
     }
   }
-  // the thread's largest value and its first token; NaN in the maximum is kept
-  float top = -INFINITY;
-  int at = 0;
-  bool nan = false;
+  // The thread's largest value and its first token (NaN is passed over).
+  float top = v[0];
 #pragma unroll
-  for (int j = 0; j < E; ++j) {
-    nan |= v[j] != v[j];
-    if (v[j] > top) {
-      top = v[j];
-      at = j;
-    }
-  }
+  for (int j = 1; j + 1 < E; j += 2) top = fmaxf(top, fmaxf(v[j], v[j + 1]));
+  top = fmaxf(top, v[E - 1]);
+  int at = 0;
+#pragma unroll
+  for (int j = E - 1; j >= 0; --j)
+    if (v[j] == top) at = j;
+  if (!(top > -INFINITY)) top = -INFINITY;               // nothing but NaN
   const auto token = [&](int j) { return ((slice * LOADS + j / VEC) * THREADS + tid) * VEC + j % VEC; };
   const auto key = [&](float y, int j) -> unsigned long long {
     return y == -INFINITY ? 0ull : (unsigned long long)order32(y) << 32 | (uint32_t)~token(j);
@@ -120,16 +119,11 @@ __global__ void __launch_bounds__(THREADS) pick_kernel(const PickArgs a) {
   float m = top;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  if (__any_sync(0xffffffffu, nan)) m = __int_as_float(0x7fffffff);
   if (lane == 0) s_max[warp] = m;
   __syncthreads();
   m = -INFINITY;
-  nan = false;
 #pragma unroll
-  for (int w = 0; w < THREADS / 32; ++w) {
-    nan |= s_max[w] != s_max[w];
-    m = fmaxf(m, s_max[w]);
-  }
+  for (int w = 0; w < THREADS / 32; ++w) m = fmaxf(m, s_max[w]);
   // the bound: of 2^groups_log groups the keep-th largest value, found by counting those above each; the threads of a group share the count
   {
     const int sub = tid & (share - 1);
@@ -139,16 +133,11 @@ __global__ void __launch_bounds__(THREADS) pick_kernel(const PickArgs a) {
     for (int o = 1; o < share; o <<= 1) above += __shfl_xor_sync(0xffffffffu, above, o);
     if (sub == 0 && above == a.keep - 1 && mine > 0) s_bound = mine;      // (keys are different unless they are 0)
   }
-  // the sum
+  // The sum; NaN if there is one.
   float sum = 0.f;
-  if (m > -INFINITY && m < INFINITY) {
-    constexpr float L = 1.44269502162933349609375f, L_LOW = 1.92596299112661746887e-8f, LN2 = 0.693147182464599609375f;
+  constexpr float LOG2E = 1.44269502162933349609375f;
 #pragma unroll
-    for (int j = 0; j < E; ++j) {
-      const float d = v[j] - m, hi = d * L, lo = fmaf(d, L_LOW, fmaf(d, L, -hi)), e = ex2(hi);
-      sum += hi > -126.f ? fmaf(e, lo * LN2, e) : 0.f;
-    }
-  }
+  for (int j = 0; j < E; ++j) sum += ex2((v[j] - (m > -INFINITY ? m : 0.f)) * LOG2E);
   double total = sum;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
@@ -158,17 +147,19 @@ __global__ void __launch_bounds__(THREADS) pick_kernel(const PickArgs a) {
     Part p;
     p.sum = 0.0;
     for (int w = 0; w < THREADS / 32; ++w) p.sum += s_sum[w];
-    p.max = nan ? __int_as_float(0x7fffffff) : m;
+    p.max = p.sum == p.sum ? m : __int_as_float(0x7fffffff);
     p.pad = 0;
     a.part[(long long)row * a.slices + slice] = p;
   }
   const unsigned long long bound = s_bound;
   if (best >= bound) {
+    const float least = value32((uint32_t)(bound >> 32));         // (of a bound of 1: NaN, which nothing is below)
 #pragma unroll
-    for (int j = 0; j < E; ++j) {
-      const unsigned long long k = key(v[j], j);
-      if (k >= bound && v[j] == v[j]) s_list[atomicAdd(&s_count, 1)] = k;
-    }
+    for (int j = 0; j < E; ++j)
+      if (!(v[j] < least) && v[j] == v[j]) {
+        const unsigned long long k = key(v[j], j);
+        if (k >= bound) s_list[atomicAdd(&s_count, 1)] = k;
+      }
   }
   __syncthreads();
   const int n = s_count;
@@ -317,6 +308,8 @@ __device__ void follow(const JoinArgs& a, int r, Chosen& c) {
 // The heads of the lists while the bound is looked for, then the candidates above it.
 struct JoinShared {
   double lse[MAX_BEAMS];
+  float base[MAX_BEAMS];
+  unsigned long long top_s[JOIN_THREADS], list_s[JOIN_LIST];      // the first words once more, to be counted
   Best list[JOIN_LISTS > JOIN_LIST ? JOIN_LISTS : JOIN_LIST];
   Best top[JOIN_THREADS];
   short id[JOIN_LISTS];
@@ -346,14 +339,23 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const JoinArgs a) {
   // normalisers: NaN where the row has no candidates
   for (int b = warp; b < K; b += JOIN_THREADS / 32) {
     const Part* p = a.part + ((long long)r * K + b) * a.slices;
+    constexpr int HELD = 3;                                // of a lane; more slices are looked up again
     const float base = a.scores[(long long)r * K + b];
-    if (!(fabsf(base) < INFINITY)) {                       // (a beam that is not there)
-      if (lane == 0) sh.lse[b] = (double)NAN;
-      continue;
-    }
+    Part x[HELD];
     float m = -INFINITY;
-    bool bad = false;
-    for (int i = lane; i < a.slices; i += 32) {
+    bool bad = !(fabsf(base) < INFINITY);                  // (a beam that is not there)
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) {
+      x[i].max = -INFINITY;
+      x[i].sum = 0.0;
+      if (lane + 32 * i < a.slices) x[i] = p[lane + 32 * i];
+    }
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) {
+      bad |= !(x[i].max < INFINITY);
+      m = fmaxf(m, x[i].max);
+    }
+    for (int i = lane + 32 * HELD; i < a.slices; i += 32) {
       bad |= !(p[i].max < INFINITY);
       m = fmaxf(m, p[i].max);
     }
@@ -361,17 +363,24 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const JoinArgs a) {
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     bad = __any_sync(0xffffffffu, bad) || m == -INFINITY;
     double sum = 0.0;
-    if (!bad)
-      for (int i = lane; i < a.slices; i += 32)
+    if (!bad) {
+#pragma unroll
+      for (int i = 0; i < HELD; ++i)
+        if (x[i].max > -INFINITY) sum += x[i].sum * exp((double)x[i].max - (double)m);
+      for (int i = lane + 32 * HELD; i < a.slices; i += 32)
         if (p[i].max > -INFINITY) sum += p[i].sum * exp((double)p[i].max - (double)m);
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) sh.lse[b] = bad ? (double)NAN : (double)m + log(sum);
+    if (lane == 0) {
+      sh.lse[b] = bad ? (double)NAN : (double)m + log(sum);
+      sh.base[b] = base;
+    }
   }
   __syncthreads();
   // a candidate; s = 0 if it is none
   auto made = [&](unsigned long long k, int b) -> Best {
-    const double score = (double)a.scores[(long long)r * K + b] + ((double)value32((uint32_t)(k >> 32)) - sh.lse[b]);
+    const double score = (double)sh.base[b] + ((double)value32((uint32_t)(k >> 32)) - sh.lse[b]);
     const bool on = k != 0 && score > -INFINITY && score < INFINITY;              // (false for NaN)
     return Best{on ? order64(score) : 0ull, k, (uint32_t)b};
   };
@@ -395,8 +404,9 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const JoinArgs a) {
   // ceil(keep / d)-th largest has ``keep`` candidates that are not behind it.
   int values = JOIN_THREADS, nth = keep;
   if (held) {
-    const int d = heads == 0 ? 1 : (keep + heads - 1) / heads, groups = min(heads, JOIN_GROUPS);
+    const int d = heads == 0 ? 1 : (keep + heads - 1) / heads;
     nth = (keep + d - 1) / d;
+    const int groups = min(heads, max(64, min(2 * nth, JOIN_GROUPS)));
     values = groups;
     mine = Best{0, 0, 0};
     if (tid < groups)
@@ -406,8 +416,9 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const JoinArgs a) {
       }
   }
   sh.top[tid] = mine;
+  sh.top_s[tid] = mine.s;
   __syncthreads();
-  // a value's place is counted by as many threads as there are for it (a power of two, neighbours)
+  // A value's place is counted by as many threads as there are for it (a power of two, neighbours).
   {
     int share = 1;
     while (2 * share * values <= JOIN_THREADS && share < 32) share *= 2;
@@ -415,7 +426,12 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const JoinArgs a) {
     const Best e = v < values ? sh.top[v] : Best{0, 0, 0};
     int above = 0;
     if (e.s != 0)
-      for (int i = sub; i < values; i += share) above += before(sh.top[i], e);
+#pragma unroll 4
+      for (int i = sub; i < values; i += share) {
+        const unsigned long long s = sh.top_s[i];
+        above += s > e.s;
+        if (s == e.s) above += before(sh.top[i], e);       // (itself, seldom another)
+      }
     for (int o = 1; o < share; o <<= 1) above += __shfl_xor_sync(0xffffffffu, above, o);
     if (sub == 0 && e.s != 0 && above == nth - 1) sh.bound = e;
   }
@@ -441,7 +457,10 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const JoinArgs a) {
         const Best e = made(k[i], b);
         if (e.s == 0 || before(bound, e)) return;          // sorted: so is the rest
         const int at = atomicAdd(&sh.count, 1);
-        if (at < JOIN_LIST) sh.list[at] = e;
+        if (at < JOIN_LIST) {
+          sh.list[at] = e;
+          sh.list_s[at] = e.s;
+        }
       }
     }
   };
@@ -461,7 +480,12 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const JoinArgs a) {
       const int i = i0 + tid / share, sub = tid % share;
       const Best e = i < n ? sh.list[i] : Best{0, 0, 0};
       int rank = 0;
-      for (int k = sub; k < n; k += share) rank += before(sh.list[k], e);
+#pragma unroll 4
+      for (int k = sub; k < n; k += share) {
+        const unsigned long long s = sh.list_s[k];
+        rank += s > e.s;
+        if (s == e.s) rank += before(sh.list[k], e);
+      }
       for (int o = 1; o < share; o <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
       if (sub == 0 && i < n && rank < keep) {
         sh.out.score[rank] = (float)value64(e.s);
