@@ -13,6 +13,7 @@
 // term of a row is 1 exactly, the errors of the others, 2^-22 of each at most, are of either sign: 1e-8 of the normaliser where they were measured),
 // and scores are compared in 64 bits.  Equal scores: the lower beam, then the lower token.
 // A row with NaN, + inf or nothing but - inf has no candidates.
+#include <float.h>
 #include <math.h>
 #include <string.h>
 
@@ -55,7 +56,8 @@ struct Part {          // of a slice
 struct PickArgs {
   const void* logits;
   long long ld;                      // elements from row to row
-  int V, keep, slices, groups_log;   // groups of threads whose largest values give the bound: 2^groups_log
+  int V, keep, slices;
+  int share, second, room;           // threads of a group and which of its values gives the bound, see launch_pick; candidates that fit
   Part* part;                        // [rows][slices]
   unsigned long long* cand;          // [rows][slices][keep] (logit, complement of the token), largest first, 0: none
 };
@@ -63,12 +65,13 @@ struct PickArgs {
 // E values per thread, by token and not by address: the sum of a row does not depend on where it lies, so that beams with the same logits have the
 // same scores.  16 bytes are loaded at once if rows are aligned to them.
 template <typename T, int E>
-__global__ void __launch_bounds__(THREADS) pick_kernel(const PickArgs a) {
+__global__ void __launch_bounds__(THREADS, 4) pick_kernel(const PickArgs a) {
   constexpr int VEC = 16 / sizeof(T), LOADS = E / VEC;
   extern __shared__ unsigned long long s_list[];       // [keep * most values of a group]
-  __shared__ unsigned long long s_top[THREADS];
+  __shared__ float s_top[THREADS];
+  __shared__ unsigned long long s_key[THREADS];
   __shared__ double s_sum[THREADS / 32];
-  __shared__ float s_max[THREADS / 32];
+  __shared__ float s_max[THREADS / 32], s_least;
   __shared__ unsigned long long s_bound;
   __shared__ int s_count;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, row = blockIdx.y, slice = blockIdx.x;
@@ -77,6 +80,7 @@ __global__ void __launch_bounds__(THREADS) pick_kernel(const PickArgs a) {
   if (tid == 0) {
     s_count = 0;
     s_bound = 1;
+    s_least = -FLT_MAX;                                  // everything but - inf and NaN
   }
   pdl_wait();
   pdl_trigger();
@@ -97,24 +101,22 @@ __global__ void __launch_bounds__(THREADS) pick_kernel(const PickArgs a) {
       for (int e = 0; e < VEC; ++e) v[j * VEC + e] = i + e < a.V ? (float)x[i + e] : -INFINITY;
     }
   }
-  // The thread's largest value and its first token (NaN is passed over).
-  float top = v[0];
+  const auto token = [&](int j) { return ((slice * LOADS + j / VEC) * THREADS + tid) * VEC + j % VEC; };
+  const auto key = [&](float y, int j) -> unsigned long long { return (unsigned long long)order32(y) << 32 | (uint32_t)~token(j); };
+  float top = v[0];                                      // (NaN is passed over)
 #pragma unroll
   for (int j = 1; j + 1 < E; j += 2) top = fmaxf(top, fmaxf(v[j], v[j + 1]));
   top = fmaxf(top, v[E - 1]);
-  int at = 0;
-#pragma unroll
-  for (int j = E - 1; j >= 0; --j)
-    if (v[j] == top) at = j;
-  if (!(top > -INFINITY)) top = -INFINITY;               // nothing but NaN
-  const auto token = [&](int j) { return ((slice * LOADS + j / VEC) * THREADS + tid) * VEC + j % VEC; };
-  const auto key = [&](float y, int j) -> unsigned long long {
-    return y == -INFINITY ? 0ull : (unsigned long long)order32(y) << 32 | (uint32_t)~token(j);
-  };
-  const unsigned long long best = key(top, at);
-  const int G = 1 << a.groups_log, share = THREADS >> a.groups_log;
-  unsigned long long mine = best;                      // of the group: neighbouring threads
-  for (int o = 1; o < share; o <<= 1) mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, o));
+  if (!(top > -INFINITY)) top = -INFINITY;
+  // The group's value: its threads' largest, or with ``second`` their second largest, which has two values that are not below it.
+  const int share = a.share;
+  float mine = top, other = -INFINITY;
+  for (int o = 1; o < share; o <<= 1) {
+    const float x = __shfl_xor_sync(0xffffffffu, mine, o), y = __shfl_xor_sync(0xffffffffu, other, o);
+    other = fmaxf(fminf(mine, x), fmaxf(other, y));
+    mine = fmaxf(mine, x);
+  }
+  if (a.second) mine = other;
   if ((tid & (share - 1)) == 0) s_top[tid / share] = mine;
   float m = top;
 #pragma unroll
@@ -124,14 +126,22 @@ __global__ void __launch_bounds__(THREADS) pick_kernel(const PickArgs a) {
   m = -INFINITY;
 #pragma unroll
   for (int w = 0; w < THREADS / 32; ++w) m = fmaxf(m, s_max[w]);
-  // the bound: of 2^groups_log groups the keep-th largest value, found by counting those above each; the threads of a group share the count
+  // The bound: of the groups' values the keep-th largest (with ``second`` half as many suffice), found by counting those above each; the
+  // threads of a group share the count.
   {
-    const int sub = tid & (share - 1);
-    int above = 0;
+    const int sub = tid & (share - 1), groups = THREADS / share, nth = a.second ? (a.keep + 1) / 2 : a.keep;
+    int above = 0, equal = 0;
 #pragma unroll 4
-    for (int i = sub; i < G; i += share) above += s_top[i] > mine;
-    for (int o = 1; o < share; o <<= 1) above += __shfl_xor_sync(0xffffffffu, above, o);
-    if (sub == 0 && above == a.keep - 1 && mine > 0) s_bound = mine;      // (keys are different unless they are 0)
+    for (int i = sub; i < groups; i += share) {
+      const float x = s_top[i];
+      above += x > mine;
+      equal += x == mine;
+    }
+    for (int o = 1; o < share; o <<= 1) {
+      above += __shfl_xor_sync(0xffffffffu, above, o);
+      equal += __shfl_xor_sync(0xffffffffu, equal, o);
+    }
+    if (sub == 0 && above < nth && above + equal >= nth && mine > -INFINITY) s_least = mine;      // (whoever writes, writes the same)
   }
   // The sum; NaN if there is one.
   float sum = 0.f;
@@ -151,17 +161,41 @@ __global__ void __launch_bounds__(THREADS) pick_kernel(const PickArgs a) {
     p.pad = 0;
     a.part[(long long)row * a.slices + slice] = p;
   }
-  const unsigned long long bound = s_bound;
-  if (best >= bound) {
-    const float least = value32((uint32_t)(bound >> 32));         // (of a bound of 1: NaN, which nothing is below)
+  {
+    const float least = s_least;
+    if (top >= least) {
 #pragma unroll
-    for (int j = 0; j < E; ++j)
-      if (!(v[j] < least) && v[j] == v[j]) {
-        const unsigned long long k = key(v[j], j);
-        if (k >= bound) s_list[atomicAdd(&s_count, 1)] = k;
-      }
+      for (int j = 0; j < E; ++j)
+        if (v[j] >= least) {
+          const int at = atomicAdd(&s_count, 1);
+          if (at < a.room) s_list[at] = key(v[j], j);
+        }
+    }
   }
   __syncthreads();
+  if (s_count > a.room) {
+    // Too many pass: equal values, or all that are large in a few threads.  Once more by value and token, which are never equal, and with the threads' own
+    // best, of which ``keep`` have any that passes.
+    unsigned long long best = 0;
+#pragma unroll
+    for (int j = 0; j < E; ++j)
+      if (v[j] > -INFINITY) best = max(best, key(v[j], j));
+    __syncthreads();
+    s_key[tid] = best;
+    if (tid == 0) s_count = 0;
+    __syncthreads();
+    int above = 0;
+    for (int i = 0; i < THREADS; ++i) above += s_key[i] > best;
+    if (above == a.keep - 1 && best > 0) s_bound = best;
+    __syncthreads();
+    const unsigned long long bound = s_bound;
+    if (best >= bound) {
+#pragma unroll
+      for (int j = 0; j < E; ++j)
+        if (v[j] > -INFINITY && key(v[j], j) >= bound) s_list[atomicAdd(&s_count, 1)] = key(v[j], j);
+    }
+    __syncthreads();
+  }
   const int n = s_count;
   unsigned long long* out = a.cand + ((long long)row * a.slices + slice) * a.keep;
   for (int i = tid; i < n; i += THREADS) {
@@ -543,10 +577,13 @@ static int slice_of(long long rows, int V) {
 static int slices_of(int E, int V) { return (V + THREADS * E - 1) / (THREADS * E); }
 
 template <typename T, int E>
-static int launch_pick(const PickArgs& a, int rows, cudaStream_t st) {
-  // a group's values: all that can pass the bound are ``keep`` groups'
-  const int smem = a.keep * ((THREADS >> a.groups_log) * E) * 8;
-  SNU1_CUDA_CHECK(launch_pdl(pick_kernel<T, E>, dim3(a.slices, rows), dim3(THREADS), smem, st, a));
+static int launch_pick(PickArgs a, int rows, cudaStream_t st) {
+  // Groups by how many values have to pass: fewer groups are sooner counted, as long as there are several times as many.  The room is for
+  // what the exact bound lets pass, and four times as many where that is little.
+  a.share = a.keep <= 32 ? 4 : a.keep <= 64 ? 2 : 1;
+  a.second = a.keep > 16 && a.keep <= 64;
+  a.room = a.keep * E * (a.keep <= 16 ? 4 : 1);
+  SNU1_CUDA_CHECK(launch_pdl(pick_kernel<T, E>, dim3(a.slices, rows), dim3(THREADS), a.room * 8, st, a));
   return kHostOk;
 }
 
@@ -583,7 +620,6 @@ SNU1_API int snu1_beam_step(const void* logits, long long ld, int is_bf16, int V
   a.V = V;
   a.keep = keep;
   a.slices = slices_of(E, V);
-  a.groups_log = keep <= 16 ? 6 : keep <= 32 ? 7 : 8;
   a.part = (Part*)scratch;
   a.cand = (unsigned long long*)(a.part + rows * a.slices);
   int rc = is_bf16 ? (E == 32 ? launch_pick<__nv_bfloat16, 32>(a, (int)rows, st) : launch_pick<__nv_bfloat16, 8>(a, (int)rows, st))
