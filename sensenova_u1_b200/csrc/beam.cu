@@ -2,14 +2,13 @@
 //
 //   c(b, v) = s_b + (x_bv - lse_b),   lse_b = log sum_v exp(x_bv)          of all beams b and tokens v the ``keep`` largest
 //
-// What bounds it is one pass over the logits (beams x vocabulary, 0.6 MB a row of the released models).  First kernel: a CTA
-// holds a slice of a row in registers, leaves its maximum and sum of exponentials, and its ``keep`` largest logits: within a row the
-// order of the candidates is that of the logits, so no normaliser is needed to choose them.  A bound from below comes from
-// the largest values of small groups of threads (the keep-th of them), few values pass it, and those are ranked by counting.  Second kernel, a
-// CTA per request: the rows' normalisers, the slices' lists (sorted, so their heads give a bound the same way), the ``keep``
-// best by score, and the beams' bookkeeping, so that a whole step is captured without a look by the host.
+// What bounds it is one pass over the logits (beams x vocabulary, 0.6 MB a row of the released models).  First kernel: every warp takes a group of a row's
+// logits, 256 or 1024 of them, and leaves their maximum and sum of exponentials: no barriers, so the pass is as fast as memory.  Second
+// kernel, a CTA per request: the rows' normalisers; a bound from below, the keep-th largest of the groups' maxima as scores, so only about as many
+// groups as continuations are kept can hold one, and those are read again; what is not below the bound is ranked by counting.  Then the beams'
+// bookkeeping, so that a whole step is captured without a look by the host.
 //
-// Candidates of different beams may be closer than fp32 tells apart: a slice's sum is of fp32 terms, from 32 terms on in 64 bits (the largest
+// Candidates of different beams may be closer than fp32 tells apart: a group's sum is of fp32 terms, from 32 terms on in 64 bits (the largest
 // term of a row is 1 exactly, the errors of the others, 2^-22 of each at most, are of either sign: 1e-8 of the normaliser where they were measured),
 // and scores are compared in 64 bits.  Equal scores: the lower beam, then the lower token.
 // A row with NaN, + inf or nothing but - inf has no candidates.
@@ -33,7 +32,6 @@ __device__ __forceinline__ uint32_t order32(float x) {          // keeps the ord
   const uint32_t b = __float_as_uint(x + 0.f);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
-__device__ __forceinline__ float value32(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 __device__ __forceinline__ unsigned long long order64(double x) {
   const unsigned long long b = (unsigned long long)__double_as_longlong(x + 0.0);
   return b >> 63 ? ~b : b | 1ull << 63;
@@ -47,170 +45,77 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-struct Part {          // of a slice
+struct Group {         // of a row's logits
   double sum;          // of exp(x - max)
-  float max;           // NaN if the slice holds one
+  float max;           // NaN if there is one
   int pad;
 };
 
-struct PickArgs {
+struct PassArgs {
   const void* logits;
-  long long ld;                      // elements from row to row
-  int V, keep, slices;
-  int share, second, room;           // threads of a group and which of its values gives the bound, see launch_pick; candidates that fit
-  Part* part;                        // [rows][slices]
-  unsigned long long* cand;          // [rows][slices][keep] (logit, complement of the token), largest first, 0: none
+  long long ld;        // elements from row to row
+  int V, rows, groups; // groups of a row
+  Group* out;          // [rows][groups]
 };
 
-// E values per thread, by token and not by address: the sum of a row does not depend on where it lies, so that beams with the same logits have the
-// same scores.  16 bytes are loaded at once if rows are aligned to them.
+// Token of value j of a group of 32 E; a lane has 16 bytes of every 512.
 template <typename T, int E>
-__global__ void __launch_bounds__(THREADS, 4) pick_kernel(const PickArgs a) {
-  constexpr int VEC = 16 / sizeof(T), LOADS = E / VEC;
-  extern __shared__ unsigned long long s_list[];       // [keep * most values of a group]
-  __shared__ float s_top[THREADS];
-  __shared__ unsigned long long s_key[THREADS];
-  __shared__ double s_sum[THREADS / 32];
-  __shared__ float s_max[THREADS / 32], s_least;
-  __shared__ unsigned long long s_bound;
-  __shared__ int s_count;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, row = blockIdx.y, slice = blockIdx.x;
-  const T* x = reinterpret_cast<const T*>(a.logits) + row * a.ld;
+__device__ __forceinline__ int token_of(int group, int j) {
+  constexpr int VEC = 16 / sizeof(T);
+  return group * 32 * E + ((j / VEC) * 32 + (threadIdx.x & 31)) * VEC + j % VEC;
+}
+// A group's values, by token and not by address: the sum of a row does not depend on where it lies, so that beams with the same logits have
+// the same scores.  - inf behind the last.
+template <typename T, int E>
+__device__ __forceinline__ void load_group(const T* x, int V, int group, float (&v)[E]) {
+  constexpr int VEC = 16 / sizeof(T);
   const bool aligned = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
-  if (tid == 0) {
-    s_count = 0;
-    s_bound = 1;
-    s_least = -FLT_MAX;                                  // everything but - inf and NaN
-  }
-  pdl_wait();
-  pdl_trigger();
-  float v[E];
 #pragma unroll
-  for (int j = 0; j < LOADS; ++j) {
-    const int i = ((slice * LOADS + j) * THREADS + tid) * VEC;                    // token of the first of VEC
-    if (aligned && i + VEC <= a.V) {
-      const uint4 u = __ldcs(reinterpret_cast<const uint4*>(x + i));
+  for (int j = 0; j < E; j += VEC) {
+    const int i = token_of<T, E>(group, j);
+    if (aligned && i + VEC <= V) {
+      const uint4 u = *reinterpret_cast<const uint4*>(x + i);
       const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        if (sizeof(T) == 4) v[j * VEC + e] = __uint_as_float(w[e & 3]);
-        else v[j * VEC + e] = __uint_as_float(e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
+        if (sizeof(T) == 4) v[j + e] = __uint_as_float(w[e & 3]);
+        else v[j + e] = __uint_as_float(e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
       }
     } else {
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) v[j * VEC + e] = i + e < a.V ? (float)x[i + e] : -INFINITY;
+      for (int e = 0; e < VEC; ++e) v[j + e] = i + e < V ? (float)x[i + e] : -INFINITY;
     }
   }
-  const auto token = [&](int j) { return ((slice * LOADS + j / VEC) * THREADS + tid) * VEC + j % VEC; };
-  const auto key = [&](float y, int j) -> unsigned long long { return (unsigned long long)order32(y) << 32 | (uint32_t)~token(j); };
-  float top = v[0];                                      // (NaN is passed over)
+}
+
+template <typename T, int E>
+__global__ void __launch_bounds__(THREADS) pass_kernel(const PassArgs a) {
+  const int lane = threadIdx.x & 31, row = blockIdx.y, group = blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5);
+  pdl_wait();
+  pdl_trigger();
+  if (group >= a.groups) return;
+  float v[E];
+  load_group<T, E>(reinterpret_cast<const T*>(a.logits) + row * a.ld, a.V, group, v);
+  float m = v[0];                                        // (NaN is passed over)
 #pragma unroll
-  for (int j = 1; j + 1 < E; j += 2) top = fmaxf(top, fmaxf(v[j], v[j + 1]));
-  top = fmaxf(top, v[E - 1]);
-  if (!(top > -INFINITY)) top = -INFINITY;
-  // The group's value: its threads' largest, or with ``second`` their second largest, which has two values that are not below it.
-  const int share = a.share;
-  float mine = top, other = -INFINITY;
-  for (int o = 1; o < share; o <<= 1) {
-    const float x = __shfl_xor_sync(0xffffffffu, mine, o), y = __shfl_xor_sync(0xffffffffu, other, o);
-    other = fmaxf(fminf(mine, x), fmaxf(other, y));
-    mine = fmaxf(mine, x);
-  }
-  if (a.second) mine = other;
-  if ((tid & (share - 1)) == 0) s_top[tid / share] = mine;
-  float m = top;
+  for (int j = 1; j + 1 < E; j += 2) m = fmaxf(m, fmaxf(v[j], v[j + 1]));
+  m = fmaxf(m, v[E - 1]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  if (lane == 0) s_max[warp] = m;
-  __syncthreads();
-  m = -INFINITY;
-#pragma unroll
-  for (int w = 0; w < THREADS / 32; ++w) m = fmaxf(m, s_max[w]);
-  // The bound: of the groups' values the keep-th largest (with ``second`` half as many suffice), found by counting those above each; the
-  // threads of a group share the count.
-  {
-    const int sub = tid & (share - 1), groups = THREADS / share, nth = a.second ? (a.keep + 1) / 2 : a.keep;
-    int above = 0, equal = 0;
-#pragma unroll 4
-    for (int i = sub; i < groups; i += share) {
-      const float x = s_top[i];
-      above += x > mine;
-      equal += x == mine;
-    }
-    for (int o = 1; o < share; o <<= 1) {
-      above += __shfl_xor_sync(0xffffffffu, above, o);
-      equal += __shfl_xor_sync(0xffffffffu, equal, o);
-    }
-    if (sub == 0 && above < nth && above + equal >= nth && mine > -INFINITY) s_least = mine;      // (whoever writes, writes the same)
-  }
-  // The sum; NaN if there is one.
-  float sum = 0.f;
   constexpr float LOG2E = 1.44269502162933349609375f;
+  const float from = m > -INFINITY ? m : 0.f;
+  float sum = 0.f;                                       // NaN if there is one
 #pragma unroll
-  for (int j = 0; j < E; ++j) sum += ex2((v[j] - (m > -INFINITY ? m : 0.f)) * LOG2E);
+  for (int j = 0; j < E; ++j) sum += ex2((v[j] - from) * LOG2E);
   double total = sum;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-  if (lane == 0) s_sum[warp] = total;
-  __syncthreads();
-  if (tid == 0) {
-    Part p;
-    p.sum = 0.0;
-    for (int w = 0; w < THREADS / 32; ++w) p.sum += s_sum[w];
-    p.max = p.sum == p.sum ? m : __int_as_float(0x7fffffff);
-    p.pad = 0;
-    a.part[(long long)row * a.slices + slice] = p;
-  }
-  {
-    const float least = s_least;
-    if (top >= least) {
-#pragma unroll
-      for (int j = 0; j < E; ++j)
-        if (v[j] >= least) {
-          const int at = atomicAdd(&s_count, 1);
-          if (at < a.room) s_list[at] = key(v[j], j);
-        }
-    }
-  }
-  __syncthreads();
-  if (s_count > a.room) {
-    // Too many pass: equal values, or all that are large in a few threads.  Once more by value and token, which are never equal, and with the threads' own
-    // best, of which ``keep`` have any that passes.
-    unsigned long long best = 0;
-#pragma unroll
-    for (int j = 0; j < E; ++j)
-      if (v[j] > -INFINITY) best = max(best, key(v[j], j));
-    __syncthreads();
-    s_key[tid] = best;
-    if (tid == 0) s_count = 0;
-    __syncthreads();
-    int above = 0;
-    for (int i = 0; i < THREADS; ++i) above += s_key[i] > best;
-    if (above == a.keep - 1 && best > 0) s_bound = best;
-    __syncthreads();
-    const unsigned long long bound = s_bound;
-    if (best >= bound) {
-#pragma unroll
-      for (int j = 0; j < E; ++j)
-        if (v[j] > -INFINITY && key(v[j], j) >= bound) s_list[atomicAdd(&s_count, 1)] = key(v[j], j);
-    }
-    __syncthreads();
-  }
-  const int n = s_count;
-  unsigned long long* out = a.cand + ((long long)row * a.slices + slice) * a.keep;
-  for (int i = tid; i < n; i += THREADS) {
-    const unsigned long long mine = s_list[i];
-    int rank = 0;
-    for (int k = 0; k < n; ++k) rank += s_list[k] > mine;
-    if (rank < a.keep) out[rank] = mine;
-  }
-  for (int i = n + tid; i < a.keep; i += THREADS) out[i] = 0;
+  if (lane == 0) a.out[(long long)row * a.groups + group] = Group{total, total == total ? m : __int_as_float(0x7fffffff), 0};
 }
 
-constexpr int JOIN_THREADS = 512;
-constexpr int JOIN_LISTS = 1280;     // lists with candidates whose heads are held; of more the bound is that of every thread's best head
-constexpr int JOIN_LIST = 1024;      // candidates that are ranked by counting; more than that are taken one by one
-constexpr int JOIN_GROUPS = 256;     // values that the bound is found among, by counting
+constexpr int JOIN_THREADS = 1024;
+constexpr int JOIN_LIST = 2048;      // candidates that fit; where more are not below the bound, it is raised to the keep-th best of these
+constexpr int JOIN_GROUPS = 1024;    // groups that fit a list; more are looked for by every warp in its own share
 constexpr int MAX_BEAMS = 64;
 
 // A search's state (all on the device); see ops/beam.py.
@@ -234,13 +139,15 @@ struct State {
 };
 
 struct JoinArgs {
-  const Part* part;
-  const unsigned long long* cand;
+  const void* logits;
+  long long ld;
+  int V, groups;
+  const Group* group;      // [requests * beams][groups]
   const float* scores;     // [requests][beams]
   float* out_scores;       // [requests][keep]
   int* out_beams;
   int* out_tokens;
-  int beams, keep, slices, has_state;
+  int beams, keep, has_state;
   int* status;
   State st;
 };
@@ -339,59 +246,56 @@ __device__ void follow(const JoinArgs& a, int r, Chosen& c) {
   if (tid == 0 && c.done == 2) s.done[r] = 1;
 }
 
-// The heads of the lists while the bound is looked for, then the candidates above it.
 struct JoinShared {
   double lse[MAX_BEAMS];
-  float base[MAX_BEAMS];
-  unsigned long long top_s[JOIN_THREADS], list_s[JOIN_LIST];      // the first words once more, to be counted
-  Best list[JOIN_LISTS > JOIN_LIST ? JOIN_LISTS : JOIN_LIST];
-  Best top[JOIN_THREADS];
-  short id[JOIN_LISTS];
+  float base[MAX_BEAMS], least[MAX_BEAMS];
+  unsigned long long top[JOIN_THREADS / 4], list_s[JOIN_LIST];      // (list_s: the candidates' scores once more, to be counted)
+  Best list[JOIN_LIST];
+  int pass[JOIN_GROUPS];
   Best bound;
-  int heads, count;
+  int passing, count;
   Chosen out;
 };
 
+template <typename T, int E>
 __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const JoinArgs a) {
   extern __shared__ unsigned long long s_raw[];
   JoinShared& sh = *reinterpret_cast<JoinShared*>(s_raw);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = blockIdx.x, K = a.beams, keep = a.keep;
-  if (tid == 0) {
-    sh.heads = sh.count = 0;
-    sh.bound = Best{1, 0, 0xffffffffu};                    // everything that is a candidate
-  }
+  if (tid == 0) sh.bound = Best{1, 0, 0xffffffffu};        // everything that is a candidate
   for (int i = tid; i < keep; i += JOIN_THREADS) {
     sh.out.score[i] = -INFINITY;
     sh.out.beam[i] = sh.out.token[i] = 0;
   }
   pdl_wait();
   pdl_trigger();
-  const int lists = K * a.slices;
-  const unsigned long long* cand = a.cand + (long long)r * lists * keep;
-  // the first list's head of this thread is on its way while the normalisers are made
-  const unsigned long long first = tid < lists ? cand[(long long)tid * keep] : 0ull;
+  const int all = K * a.groups;
+  const Group* group = a.group + (long long)r * all;
+  const T* logits = reinterpret_cast<const T*>(a.logits) + (long long)r * K * a.ld;
   // normalisers: NaN where the row has no candidates
   for (int b = warp; b < K; b += JOIN_THREADS / 32) {
-    const Part* p = a.part + ((long long)r * K + b) * a.slices;
-    constexpr int HELD = 3;                                // of a lane; more slices are looked up again
+    const Group* p = group + (long long)b * a.groups;
+    constexpr int HELD = 5;                                // of a lane; more are looked up again
     const float base = a.scores[(long long)r * K + b];
-    Part x[HELD];
+    Group x[HELD];
     float m = -INFINITY;
     bool bad = !(fabsf(base) < INFINITY);                  // (a beam that is not there)
 #pragma unroll
     for (int i = 0; i < HELD; ++i) {
       x[i].max = -INFINITY;
       x[i].sum = 0.0;
-      if (lane + 32 * i < a.slices) x[i] = p[lane + 32 * i];
+      if (lane + 32 * i < a.groups) x[i] = p[lane + 32 * i];
     }
 #pragma unroll
     for (int i = 0; i < HELD; ++i) {
       bad |= !(x[i].max < INFINITY);
       m = fmaxf(m, x[i].max);
     }
-    for (int i = lane + 32 * HELD; i < a.slices; i += 32) {
-      bad |= !(p[i].max < INFINITY);
-      m = fmaxf(m, p[i].max);
+#pragma unroll 4
+    for (int i = lane + 32 * HELD; i < a.groups; i += 32) {
+      const float y = p[i].max;
+      bad |= !(y < INFINITY);
+      m = fmaxf(m, y);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
@@ -401,8 +305,11 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const JoinArgs a) {
 #pragma unroll
       for (int i = 0; i < HELD; ++i)
         if (x[i].max > -INFINITY) sum += x[i].sum * exp((double)x[i].max - (double)m);
-      for (int i = lane + 32 * HELD; i < a.slices; i += 32)
-        if (p[i].max > -INFINITY) sum += p[i].sum * exp((double)p[i].max - (double)m);
+#pragma unroll 4
+      for (int i = lane + 32 * HELD; i < a.groups; i += 32) {
+        const Group y = p[i];
+        if (y.max > -INFINITY) sum += y.sum * exp((double)y.max - (double)m);
+      }
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -412,152 +319,117 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const JoinArgs a) {
     }
   }
   __syncthreads();
-  // a candidate; s = 0 if it is none
-  auto made = [&](unsigned long long k, int b) -> Best {
-    const double score = (double)sh.base[b] + ((double)value32((uint32_t)(k >> 32)) - sh.lse[b]);
-    const bool on = k != 0 && score > -INFINITY && score < INFINITY;              // (false for NaN)
-    return Best{on ? order64(score) : 0ull, k, (uint32_t)b};
+  // a logit's score as a number that can be compared; 0: it is no candidate
+  auto score_of = [&](float x, int b) -> unsigned long long {
+    const double score = (double)sh.base[b] + ((double)x - sh.lse[b]);
+    return x > -INFINITY && score > -INFINITY && score < INFINITY ? order64(score) : 0ull;       // (false for NaN)
   };
-  auto entry = [&](int list, int i) -> Best { return made(i < keep ? cand[(long long)list * keep + i] : 0ull, list / a.slices); };
-  // the heads of all lists that have any
-  Best mine{0, 0, 0};
-  for (int l = tid; l < lists; l += JOIN_THREADS) {
-    const Best e = l == tid ? made(first, l / a.slices) : entry(l, 0);
-    if (e.s == 0) continue;
-    if (before(e, mine)) mine = e;
-    const int at = atomicAdd(&sh.heads, 1);
-    if (at < JOIN_LISTS) {
-      sh.list[at] = e;
-      sh.id[at] = (short)min(l, 32767);                    // (not read if there are more lists than fit)
-    }
-  }
-  __syncthreads();
-  const int heads = sh.heads;
-  const bool held = heads <= JOIN_LISTS && lists <= 32767;
-  // The bound.  d entries of a list are at least as good as its d-th, so of the lists' d-th entries (or of the best of groups of lists) the
-  // ceil(keep / d)-th largest has ``keep`` candidates that are not behind it.
-  int values = JOIN_THREADS, nth = keep;
-  if (held) {
-    const int d = heads == 0 ? 1 : (keep + heads - 1) / heads;
-    nth = (keep + d - 1) / d;
-    const int groups = min(heads, max(64, min(2 * nth, JOIN_GROUPS)));
-    values = groups;
-    mine = Best{0, 0, 0};
-    if (tid < groups)
-      for (int i = tid; i < heads; i += groups) {
-        const Best e = d == 1 ? sh.list[i] : entry(sh.id[i], d - 1);
-        if (before(e, mine)) mine = e;
-      }
-  }
-  sh.top[tid] = mine;
-  sh.top_s[tid] = mine.s;
-  __syncthreads();
-  // A value's place is counted by as many threads as there are for it (a power of two, neighbours).
-  {
-    int share = 1;
-    while (2 * share * values <= JOIN_THREADS && share < 32) share *= 2;
-    const int v = tid / share, sub = tid % share;
-    const Best e = v < values ? sh.top[v] : Best{0, 0, 0};
-    int above = 0;
-    if (e.s != 0)
-#pragma unroll 4
-      for (int i = sub; i < values; i += share) {
-        const unsigned long long s = sh.top_s[i];
-        above += s > e.s;
-        if (s == e.s) above += before(sh.top[i], e);       // (itself, seldom another)
-      }
-    for (int o = 1; o < share; o <<= 1) above += __shfl_xor_sync(0xffffffffu, above, o);
-    if (sub == 0 && e.s != 0 && above == nth - 1) sh.bound = e;
-  }
-  __syncthreads();
-  const Best bound = sh.bound;
-  // What is not behind it.  (Heads and candidates share their place, so the heads are looked at again first.)
-  constexpr int OWN = (JOIN_LISTS + JOIN_THREADS - 1) / JOIN_THREADS, DEEP = 4;
-  int go[OWN];
+  constexpr int OWN = 2;                                   // the first groups of a thread: their maxima as scores, looked up once
+  unsigned long long own[OWN];
 #pragma unroll
   for (int k = 0; k < OWN; ++k) {
-    const int i = k * JOIN_THREADS + tid;
-    go[k] = held && i < heads && !before(bound, sh.list[i]) ? sh.id[i] : -1;
+    const int i = tid + k * JOIN_THREADS;
+    own[k] = i < all ? score_of(group[i].max, i / a.groups) : 0ull;
   }
-  __syncthreads();
-  auto walk = [&](int l) {
-    const int b = l / a.slices;
-    for (int i0 = 0; i0 < keep; i0 += DEEP) {
-      unsigned long long k[DEEP];
+  // The bound: the keep-th largest of ``values`` sets of groups' maxima, every values-th group a set, so that few groups are a set each.
+  // A value's place is counted by ``share`` threads.
+  {
+    unsigned long long mine = 0;
 #pragma unroll
-      for (int i = 0; i < DEEP; ++i) k[i] = i0 + i < keep ? cand[(long long)l * keep + i0 + i] : 0ull;
-#pragma unroll
-      for (int i = 0; i < DEEP; ++i) {
-        const Best e = made(k[i], b);
-        if (e.s == 0 || before(bound, e)) return;          // sorted: so is the rest
-        const int at = atomicAdd(&sh.count, 1);
-        if (at < JOIN_LIST) {
-          sh.list[at] = e;
-          sh.list_s[at] = e.s;
-        }
-      }
+    for (int k = 0; k < OWN; ++k) mine = max(mine, own[k]);
+#pragma unroll 4
+    for (int i = tid + OWN * JOIN_THREADS; i < all; i += JOIN_THREADS) mine = max(mine, score_of(group[i].max, i / a.groups));
+    const int share = keep <= 32 ? 16 : keep <= 64 ? 8 : 4, values = JOIN_THREADS / share, sub = tid & (share - 1);
+    sh.list_s[tid] = mine;
+    __syncthreads();
+    mine = sh.list_s[tid / share + sub * values];          // (groups side by side are in different sets)
+    for (int o = 1; o < share; o <<= 1) mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, o));
+    if (sub == 0) sh.top[tid / share] = mine;
+    __syncthreads();
+    int above = 0, equal = 0;
+#pragma unroll 4
+    for (int i = sub; i < values; i += share) {
+      const unsigned long long x = sh.top[i];
+      above += x > mine;
+      equal += x == mine;
     }
-  };
-  if (held) {
-#pragma unroll
-    for (int k = 0; k < OWN; ++k)
-      if (go[k] >= 0) walk(go[k]);
-  } else {
-    for (int l = tid; l < lists; l += JOIN_THREADS) walk(l);
+    for (int o = 1; o < share; o <<= 1) {
+      above += __shfl_xor_sync(0xffffffffu, above, o);
+      equal += __shfl_xor_sync(0xffffffffu, equal, o);
+    }
+    if (sub == 0 && mine != 0 && above < keep && above + equal >= keep) sh.bound.s = mine;         // (whoever writes, writes the same)
   }
+  if (tid == 0) sh.count = sh.passing = 0;
   __syncthreads();
-  const int n = sh.count;
-  if (n <= JOIN_LIST) {
-    int share = 1;                                         // threads for one candidate
-    while (2 * share * n <= JOIN_THREADS && share < 32) share *= 2;
-    for (int i0 = 0; i0 < n; i0 += JOIN_THREADS / share) {
-      const int i = i0 + tid / share, sub = tid % share;
-      const Best e = i < n ? sh.list[i] : Best{0, 0, 0};
+  int n;
+  for (bool exactly = false;; exactly = true) {
+    const Best bound = sh.bound;
+    // The groups that can hold a candidate, and for every beam a logit that is a little below what the bound's score asks for.
+    auto see = [&](unsigned long long s, int i) {
+      if (s >= bound.s) {
+        const int at = atomicAdd(&sh.passing, 1);
+        if (at < JOIN_GROUPS) sh.pass[at] = i;
+      }
+    };
+#pragma unroll
+    for (int k = 0; k < OWN; ++k) see(own[k], tid + k * JOIN_THREADS);
+#pragma unroll 4
+    for (int i = tid + OWN * JOIN_THREADS; i < all; i += JOIN_THREADS) see(score_of(group[i].max, i / a.groups), i);
+    if (tid < K) {
+      const double to = value64(bound.s), from = sh.base[tid], x = to - from + sh.lse[tid];
+      sh.least[tid] = bound.s == 1 ? -FLT_MAX
+                                   : fmaxf((float)(x - 1e-6 * fabs(x) - 1e-15 * (fabs(to) + fabs(from) + fabs(sh.lse[tid]))) - FLT_MIN, -FLT_MAX);
+    }
+    __syncthreads();
+    const int passing = sh.passing;
+    const bool listed = passing <= JOIN_GROUPS;
+    for (int i = warp; i < (listed ? passing : all); i += JOIN_THREADS / 32) {
+      const int g = listed ? sh.pass[i] : i, b = g / a.groups;
+      if (!listed && score_of(group[g].max, b) < bound.s) continue;
+      float v[E];
+      load_group<T, E>(logits + b * a.ld, a.V, g - b * a.groups, v);
+      const float least = sh.least[b];
+#pragma unroll
+      for (int j = 0; j < E; ++j)
+        if (v[j] >= least) {
+          const unsigned long long key = (unsigned long long)order32(v[j]) << 32 | (uint32_t)~token_of<T, E>(g - b * a.groups, j);
+          if (!exactly || !before(bound, Best{score_of(v[j], b), key, (uint32_t)b})) {
+            const int at = atomicAdd(&sh.count, 1);
+            if (at < JOIN_LIST) sh.list[at] = Best{(unsigned long long)__float_as_uint(v[j]), key, (uint32_t)b};
+          }
+        }
+    }
+    __syncthreads();
+    n = sh.count;
+    const int here = min(n, JOIN_LIST);
+    for (int i = tid; i < here; i += JOIN_THREADS) sh.list_s[i] = sh.list[i].s = score_of(__uint_as_float((uint32_t)sh.list[i].s), (int)sh.list[i].beam);
+    if (tid == 0) sh.count = sh.passing = 0;
+    __syncthreads();
+    int share = 1;                                         // threads for one candidate (a power of two, neighbours)
+    while (2 * share * here <= JOIN_THREADS && share < 32) share *= 2;
+    for (int i0 = 0; i0 < here; i0 += JOIN_THREADS / share) {
+      const int i = i0 + tid / share, sub = tid & (share - 1);
+      const Best e = i < here ? sh.list[i] : Best{0, 0, 0};
       int rank = 0;
 #pragma unroll 4
-      for (int k = sub; k < n; k += share) {
+      for (int k = sub; k < here; k += share) {
         const unsigned long long s = sh.list_s[k];
         rank += s > e.s;
-        if (s == e.s) rank += before(sh.list[k], e);
+        if (s == e.s) rank += before(sh.list[k], e);       // (itself, seldom another)
       }
       for (int o = 1; o < share; o <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
-      if (sub == 0 && i < n && rank < keep) {
+      if (sub == 0 && e.s != 0 && rank < keep) {
         sh.out.score[rank] = (float)value64(e.s);
         sh.out.beam[rank] = (int)e.beam;
         sh.out.token[rank] = (int)~(uint32_t)e.key;
+        if (rank == keep - 1) sh.bound = e;
       }
     }
-  } else {
-    // Many lists share their best (rows that are alike, say): the best of all threads' next entries, ``keep`` times.  Behind the last one
-    // taken a list goes on with its first entry that is not before it.
-    Best last{~0ull, 0, 0};
-    for (int c = 0; c < keep; ++c) {
-      Best next{0, 0, 0};
-      for (int l = tid; l < lists; l += JOIN_THREADS)
-        for (int i = 0; i < keep; ++i) {
-          const Best e = entry(l, i);
-          if (e.s == 0) break;
-          if (!before(last, e)) continue;                  // taken
-          if (before(e, next)) next = e;
-          break;
-        }
-      __syncthreads();
-      sh.top[tid] = next;
-      __syncthreads();
-      for (int o = JOIN_THREADS / 2; o > 0; o >>= 1) {
-        if (tid < o && before(sh.top[tid + o], sh.top[tid])) sh.top[tid] = sh.top[tid + o];
-        __syncthreads();
-      }
-      last = sh.top[0];
-      if (last.s == 0) break;
-      if (tid == 0) {
-        sh.out.score[c] = (float)value64(last.s);
-        sh.out.beam[c] = (int)last.beam;
-        sh.out.token[c] = (int)~(uint32_t)last.key;
-      }
-    }
+    __syncthreads();
+    // Where more pass than fit (equal logits, say), the keep-th best of these is a better bound, and is kept to exactly: every time at
+    // least those of them that are behind it pass no more.
+    if (n <= JOIN_LIST) break;
   }
-  __syncthreads();
   if (a.has_state) {
     follow(a, r, sh.out);
     return;
@@ -569,21 +441,21 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const JoinArgs a) {
   }
 }
 
-// Values per thread of the first kernel: 8 where slices of 32 values would leave SMs without one (1 x 4 beams of 151936 tokens).
-static int slice_of(long long rows, int V) {
-  const long long slices = ((long long)V + THREADS * 32 - 1) / (THREADS * 32);
-  return rows * slices >= num_sms() ? 32 : 8;
-}
-static int slices_of(int E, int V) { return (V + THREADS * E - 1) / (THREADS * E); }
+// Values per lane of a group: of short rows 8, so that there are several times as many groups as continuations are kept.
+static int group_of(int V) { return V >= 32768 ? 32 : 8; }
+static int groups_of(int E, int V) { return (V + 32 * E - 1) / (32 * E); }
 
 template <typename T, int E>
-static int launch_pick(PickArgs a, int rows, cudaStream_t st) {
-  // Groups by how many values have to pass: fewer groups are sooner counted, as long as there are several times as many.  The room is for
-  // what the exact bound lets pass, and four times as many where that is little.
-  a.share = a.keep <= 32 ? 4 : a.keep <= 64 ? 2 : 1;
-  a.second = a.keep > 16 && a.keep <= 64;
-  a.room = a.keep * E * (a.keep <= 16 ? 4 : 1);
-  SNU1_CUDA_CHECK(launch_pdl(pick_kernel<T, E>, dim3(a.slices, rows), dim3(THREADS), a.room * 8, st, a));
+static int launch(const PassArgs& a, const JoinArgs& j, int requests, cudaStream_t st) {
+  int dev = 0;
+  SNU1_CUDA_CHECK(cudaGetDevice(&dev));
+  static std::once_flag once[64];
+  cudaError_t err = cudaSuccess;
+  std::call_once(once[dev & 63], [&]() { err = cudaFuncSetAttribute(join_kernel<T, E>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(JoinShared)); });
+  SNU1_CUDA_CHECK(err);
+  constexpr int WARPS = THREADS / 32;
+  SNU1_CUDA_CHECK(launch_pdl(pass_kernel<T, E>, dim3((a.groups + WARPS - 1) / WARPS, a.rows), dim3(THREADS), 0, st, a));
+  SNU1_CUDA_CHECK(launch_pdl(join_kernel<T, E>, dim3(requests), dim3(JOIN_THREADS), sizeof(JoinShared), st, j));
   return kHostOk;
 }
 
@@ -594,10 +466,9 @@ using namespace snu1;
 
 SNU1_API int snu1_beam_state_bytes() { return (int)sizeof(beam::State); }
 
-// Bytes of scratch for ``rows`` rows of ``V`` logits of which ``keep`` are kept.
-SNU1_API long long snu1_beam_scratch_bytes(int rows, int V, int keep) {
-  const long long slices = beam::slices_of(beam::slice_of(rows, V), V);
-  return rows * slices * ((long long)sizeof(beam::Part) + 8ll * keep);
+// Bytes of scratch for ``rows`` rows of ``V`` logits.
+SNU1_API long long snu1_beam_scratch_bytes(int rows, int V) {
+  return (long long)rows * beam::groups_of(beam::group_of(V), V) * (long long)sizeof(beam::Group);
 }
 
 // logits [requests * beams][V] (fp32, or bf16 with is_bf16), rows ld elements apart; scores [requests][beams] fp32.  Without ``state`` the best
@@ -606,47 +477,39 @@ SNU1_API int snu1_beam_step(const void* logits, long long ld, int is_bf16, int V
                             void* scratch, void* out_scores, void* out_beams, void* out_tokens, const void* state, void* stream) {
   using namespace beam;
   const long long rows = (long long)requests * beams;
-  if (requests <= 0 || beams <= 0 || beams > MAX_BEAMS || rows > 65535 || V <= 0 || V > (1 << 30) || keep <= 0 || keep > MAX_KEEP ||
+  if (requests <= 0 || beams <= 0 || beams > MAX_BEAMS || rows > 65535 || V <= 0 || V > (1 << 24) || keep <= 0 || keep > MAX_KEEP ||
       keep > (long long)beams * V || ld < V || ((reinterpret_cast<uintptr_t>(scratch) & 15) != 0)) {
     set_last_error("beam_step: %d requests of %d beams (at most %d), %d tokens, %d kept (at most %d)", requests, beams, MAX_BEAMS, V, keep,
                    MAX_KEEP);
     return kHostBadArg;
   }
-  cudaStream_t st = (cudaStream_t)stream;
-  const int E = slice_of(rows, V);
-  PickArgs a;
+  const int E = group_of(V);
+  PassArgs a;
   a.logits = logits;
   a.ld = ld;
   a.V = V;
-  a.keep = keep;
-  a.slices = slices_of(E, V);
-  a.part = (Part*)scratch;
-  a.cand = (unsigned long long*)(a.part + rows * a.slices);
-  int rc = is_bf16 ? (E == 32 ? launch_pick<__nv_bfloat16, 32>(a, (int)rows, st) : launch_pick<__nv_bfloat16, 8>(a, (int)rows, st))
-                   : (E == 32 ? launch_pick<float, 32>(a, (int)rows, st) : launch_pick<float, 8>(a, (int)rows, st));
-  if (rc != kHostOk) return rc;
+  a.rows = (int)rows;
+  a.groups = groups_of(E, V);
+  a.out = (Group*)scratch;
   JoinArgs j;
   memset(&j, 0, sizeof(j));
-  j.part = a.part;
-  j.cand = a.cand;
+  j.logits = logits;
+  j.ld = ld;
+  j.V = V;
+  j.groups = a.groups;
+  j.group = a.out;
   j.scores = (const float*)scores;
   j.out_scores = (float*)out_scores;
   j.out_beams = (int*)out_beams;
   j.out_tokens = (int*)out_tokens;
   j.beams = beams;
   j.keep = keep;
-  j.slices = a.slices;
   j.status = device_status_word();
   if (state != nullptr) {
     j.has_state = 1;
     memcpy(&j.st, state, sizeof(State));
   }
-  int dev = 0;
-  SNU1_CUDA_CHECK(cudaGetDevice(&dev));
-  static std::once_flag once[64];
-  cudaError_t err = cudaSuccess;
-  std::call_once(once[dev & 63], [&]() { err = cudaFuncSetAttribute(join_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(JoinShared)); });
-  SNU1_CUDA_CHECK(err);
-  SNU1_CUDA_CHECK(launch_pdl(join_kernel, dim3(requests), dim3(JOIN_THREADS), sizeof(JoinShared), st, j));
-  return kHostOk;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (is_bf16) return E == 32 ? launch<__nv_bfloat16, 32>(a, j, requests, st) : launch<__nv_bfloat16, 8>(a, j, requests, st);
+  return E == 32 ? launch<float, 32>(a, j, requests, st) : launch<float, 8>(a, j, requests, st);
 }

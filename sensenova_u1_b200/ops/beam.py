@@ -21,7 +21,7 @@ from . import _lib
 from ._lib import c_float, c_int, c_ll, c_void_p
 
 MAX_BEAMS, MAX_KEEP, MAX_EOS = 64, 128, 8
-MAX_VOCAB = 1 << 30
+MAX_VOCAB = 1 << 24
 _ENTRY: dict = {}
 
 
@@ -38,7 +38,7 @@ def _entry():
         if lib.snu1_beam_state_bytes() != ctypes.sizeof(_State):
             raise _lib.NativeLibraryError(f"{_lib.lib_path()} has searches of another layout: build it again (python -m sensenova_u1_b200.build)")
         P, L, I = c_void_p, c_ll, c_int
-        lib.snu1_beam_scratch_bytes.argtypes, lib.snu1_beam_scratch_bytes.restype = (I, I, I), L
+        lib.snu1_beam_scratch_bytes.argtypes, lib.snu1_beam_scratch_bytes.restype = (I, I), L
         lib.snu1_beam_step.argtypes = (P, L, I, I, P, I, I, I, P, P, P, P, P, P)
         _ENTRY.update(scratch=lib.snu1_beam_scratch_bytes, step=lib.snu1_beam_step)
     return _ENTRY
@@ -73,7 +73,7 @@ def _launch(logits, scores, requests, beams, vocab, keep, out, state) -> None:
         with torch.cuda.device(index):
             return _launch(logits, scores, requests, beams, vocab, keep, out, state)
     entry = _entry()
-    scratch = torch.empty(entry["scratch"](requests * beams, vocab, keep), dtype=torch.uint8, device=logits.device)
+    scratch = torch.empty(entry["scratch"](requests * beams, vocab), dtype=torch.uint8, device=logits.device)
     _lib.LAUNCHES += 2
     rc = entry["step"](logits.data_ptr(), max(logits.stride(0), vocab), logits.dtype == torch.bfloat16, vocab, scores.data_ptr(), requests, beams,
                        keep, scratch.data_ptr(), *out, state, torch._C._cuda_getCurrentRawStream(index))
