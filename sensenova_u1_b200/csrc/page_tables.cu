@@ -204,39 +204,43 @@ __global__ void __launch_bounds__(THREADS) step_kernel(const StepArgs a) {
 struct CopyArgs {
   const long long* layers;   // [2][layers] data and scales
   const int4* copies;
-  int heads, page, pages, row_bytes;       // row_bytes: of a token's values of one head
+  int heads, page, pages, row_bytes, sides;       // row_bytes: of a token's values of one head; sides: of a block
 };
 
 constexpr int COPY_THREADS = 256;
 
-// A block copies the rows of one sequence, layer, and side (keys or values) of one head; the rows of a head are contiguous in a page.
+// A block copies the rows of one sequence and layer, of ``sides`` sides (a side: keys or values of one head, whose rows are contiguous in a
+// page): as many as a full page of them is 32 KB.  (A block per side: 16 x 8 sequences, 12 layers, pages of 16 tokens 24 us, so 10.)
 __global__ void __launch_bounds__(COPY_THREADS) copy_kernel(const CopyArgs a) {
   pdl_wait();
   pdl_trigger();
   const int4 c = a.copies[blockIdx.x];
   if (c.z <= 0 || c.x < 0 || c.x >= a.pages || c.y < 0 || c.y >= a.pages) return;
-  const int layer = blockIdx.z;
+  const int layer = blockIdx.z, first = blockIdx.y * a.sides, sides = min(a.sides, 2 * a.heads - first);
   uint8_t* data = reinterpret_cast<uint8_t*>(a.layers[layer]);
   float* scales = reinterpret_cast<float*>(a.layers[gridDim.z + layer]);
-  const int side = blockIdx.y;                               // 2 x heads
-  const long long from = (long long)c.x * 2 * a.heads + side, to = (long long)c.y * 2 * a.heads + side;
-  const uint4* x = reinterpret_cast<const uint4*>(data + from * a.page * a.row_bytes);
-  uint4* y = reinterpret_cast<uint4*>(data + to * a.page * a.row_bytes);
-  const int n = c.z * (a.row_bytes / 16);
-  for (int i0 = 0; i0 < n; i0 += COPY_THREADS * 4) {
+  const long long from = (long long)c.x * 2 * a.heads + first, to = (long long)c.y * 2 * a.heads + first;
+  const int n = c.z * (a.row_bytes / 16), step = a.page * (a.row_bytes / 16);        // 16 bytes at a time: of a side, and from side to side
+  const uint4* x = reinterpret_cast<const uint4*>(data) + from * step;
+  uint4* y = reinterpret_cast<uint4*>(data) + to * step;
+  for (int i0 = 0; i0 < n * sides; i0 += COPY_THREADS * 4) {
     uint4 v[4];
+    int at[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const int i = i0 + k * COPY_THREADS + threadIdx.x;
-      if (i < n) v[k] = x[i];
+      at[k] = i < n * sides ? i / n * step + i % n : -1;
+      if (at[k] >= 0) v[k] = x[at[k]];
     }
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int i = i0 + k * COPY_THREADS + threadIdx.x;
-      if (i < n) y[i] = v[k];
-    }
+    for (int k = 0; k < 4; ++k)
+      if (at[k] >= 0) y[at[k]] = v[k];
   }
-  if (scales != nullptr && threadIdx.x < c.z) scales[to * a.page + threadIdx.x] = scales[from * a.page + threadIdx.x];
+  if (scales != nullptr)
+    for (int i = threadIdx.x; i < c.z * sides; i += COPY_THREADS) {
+      const int at = i / c.z * a.page + i % c.z;
+      scales[to * a.page + at] = scales[from * a.page + at];
+    }
 }
 
 }  // namespace pages
@@ -289,6 +293,7 @@ SNU1_API int snu1_page_tables_copy(const void* tables, const void* layers, int c
   a.page = t.page;
   a.pages = t.pages;
   a.row_bytes = fp8 ? paged::HEAD : 2 * paged::HEAD;
-  SNU1_CUDA_CHECK(launch_pdl(copy_kernel, dim3(t.seqs, 2 * heads, count), dim3(COPY_THREADS), 0, (cudaStream_t)stream, a));
+  a.sides = max(1, min(2 * heads, 32768 / (t.page * a.row_bytes)));
+  SNU1_CUDA_CHECK(launch_pdl(copy_kernel, dim3(t.seqs, (2 * heads + a.sides - 1) / a.sides, count), dim3(COPY_THREADS), 0, (cudaStream_t)stream, a));
   return kHostOk;
 }
