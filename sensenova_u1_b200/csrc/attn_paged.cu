@@ -787,31 +787,48 @@ __global__ void __launch_bounds__(JOIN_THREADS) paged_share_join_kernel(const Pl
   pdl_wait();
   pdl_trigger();
   if (i >= p.join_count) return;
-  const long long at[2] = {(long long)e[0].z * a.heads + head, (long long)e[1].x * a.heads + head};
-  const long long step[2] = {(long long)e[1].w * a.heads, (long long)e[1].z * a.heads};
-  const int parts[2] = {e[0].w, e[1].y};
-  float mt = -INFINITY;
-#pragma unroll
-  for (int k = 0; k < 2; ++k)
-    for (int s = lane; s < parts[k]; s += 32) mt = fmaxf(mt, __ldcg(&a.part_ml[at[k] + s * step[k]].x));
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, o));
+  // a lane has the maximum and the sum of one part, 32 parts at a time; eight parts' values are on their way
+  const int shared = e[0].w, all = shared + e[1].y;
+  float mt = -INFINITY, lt = 0.f;
   float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-  float lt = 0.f;
+  for (int s0 = 0; s0 < all; s0 += 32) {
+    const int s = s0 + lane;
+    const int row = s < shared ? e[0].z + s * e[1].w : e[1].x + (s - shared) * e[1].z;
+    float2 ml = make_float2(-INFINITY, 0.f);
+    if (s < all) ml = __ldcg(&a.part_ml[(long long)row * a.heads + head]);
+    float top = fmaxf(ml.x, mt);
 #pragma unroll
-  for (int k = 0; k < 2; ++k)
-#pragma unroll 4
-    for (int s = 0; s < parts[k]; ++s) {
-      const float2 ml = __ldcg(&a.part_ml[at[k] + s * step[k]]);
-      const float4 y = __ldcg(reinterpret_cast<const float4*>(a.part + (at[k] + s * step[k]) * HEAD) + lane);
-      if (ml.x == -INFINITY) continue;                           // nothing is written then
-      const float f = fast_exp2(ml.x - mt);
-      x.x += f * y.x;
-      x.y += f * y.y;
-      x.z += f * y.z;
-      x.w += f * y.w;
-      lt += f * ml.y;
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float old = mt == -INFINITY ? 0.f : fast_exp2(mt - top), f = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - top);
+    mt = top;
+    float l = f == 0.f ? 0.f : f * ml.y;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    lt = lt * old + l;
+    x.x *= old;
+    x.y *= old;
+    x.z *= old;
+    x.w *= old;
+    const int here = min(32, all - s0);
+    for (int k = 0; k < here; k += 8) {
+      float4 y[8];
+      float g[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int from = __shfl_sync(0xffffffffu, row, min(k + i, here - 1));
+        g[i] = __shfl_sync(0xffffffffu, f, k + i & 31);
+        y[i] = __ldcg(reinterpret_cast<const float4*>(a.part + ((long long)from * a.heads + head) * HEAD) + lane);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (k + i >= here || g[i] == 0.f) continue;              // (nothing is written where there is nothing)
+        x.x += g[i] * y[i].x;
+        x.y += g[i] * y[i].y;
+        x.z += g[i] * y[i].z;
+        x.w += g[i] * y[i].w;
+      }
     }
+  }
   const float inv = lt == 0.f ? 0.f : 1.f / lt;                  // a row without keys gives zeros
   uint2 u;
   u.x = pack_bf16x2(x.x * inv, x.y * inv);
