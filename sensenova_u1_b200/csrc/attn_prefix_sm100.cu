@@ -114,7 +114,6 @@ struct RowState {
   float rs;          // e4m3: the power of two that the scores are multiplied by; NaN: a query that is not finite
 };
 
-constexpr int TURN = 32 * 5;
 struct PrefixShared {
   alignas(16) int lim[PR];                       // limits of the rows, by column
   // e4m3: the powers of two of RowState::rs and of ec, as bf16: read eight at a time (registers do not suffice for them)
@@ -123,42 +122,38 @@ struct PrefixShared {
   RowState row[PR];
   float by[PR], f[PR], fo[PR], mv[PR];           // of a move: by how much, factors of the sums and of the output; e4m3: see exponent_of
   int ec[PR];                                    // e4m3: exponent of a row's factor of p times the value's scale
-  float red[8][32], sum[8][32], turn[8][TURN];
+  float red[8][32], sum[8][32];
 };
 
 // The largest scores of eight rows over a warp's keys, row i in lane i: log2 units, or relative to the row's maximum plus ``more``.  S: the rows'
-// products; lim: their limits, or null; turn: the warp's own memory, where four rows at a time are turned (a reduction per row by
-// instructions of the warp took 1 us for eight).  A call: it is seldom needed, and its code would crowd the loop's.
+// products; lim: their limits, or null.  Every step takes half of the rows across half of the lanes.
 template <bool FP8>
-__device__ __noinline__ float row_tops(uint32_t S, const RowState* row, const int* lim, int key, float ks, bool rel, float more, float* turn) {
+__device__ __forceinline__ float row_tops(uint32_t S, const RowState* row, const int* lim, int key, float ks, bool rel, float more) {
   uint32_t h[8], lo[8];
   tmem_ld_x8(S, h);
   if (FP8) tmem_ld_x8(S + PR, lo);
   tmem_ld_wait();
   const int lane = threadIdx.x & 31;
-  float mine = -INFINITY;
+  float y[8];
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int e = 4 * half + k;
-      float y = __uint_as_float(h[e]);
-      if (FP8) y = fmaf(__uint_as_float(lo[e]), 0.0625f, y);
-      y = __fmul_rn(y, FP8 ? __fmul_rn(row[e].rs, ks) : ks);
-      if (rel) y -= row[e].m;
-      if (lim != nullptr && key >= lim[e]) y = -INFINITY;
-      turn[lane * 5 + k] = y == -INFINITY ? y : y + more;
-    }
-    __syncwarp();
-    float top = -INFINITY;                       // (of a NaN and a number fmaxf gives the number)
-#pragma unroll
-    for (int k = 0; k < 4; ++k) top = fmaxf(top, turn[((lane >> 2) * 4 + k) * 5 + (lane & 3)]);
-#pragma unroll
-    for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if ((lane >> 2 & 1) == half) mine = top;
-    __syncwarp();
+  for (int e = 0; e < 8; ++e) {
+    y[e] = __uint_as_float(h[e]);
+    if (FP8) y[e] = fmaf(__uint_as_float(lo[e]), 0.0625f, y[e]);
+    y[e] = __fmul_rn(y[e], FP8 ? __fmul_rn(row[e].rs, ks) : ks);
+    if (rel) y[e] -= row[e].m;
+    if (lim != nullptr && key >= lim[e]) y[e] = -INFINITY;
+    y[e] = y[e] > -INFINITY ? y[e] + more : -INFINITY;           // (NaN counts for nothing)
   }
-  return mine;
+#pragma unroll
+  for (int n = 4; n > 0; n >>= 1)
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+      const float send = lane & 4 * n ? y[i] : y[i + n], keep = lane & 4 * n ? y[i + n] : y[i];
+      y[i] = fmaxf(keep, __shfl_xor_sync(0xffffffffu, send, 4 * n));
+    }
+  y[0] = fmaxf(y[0], __shfl_xor_sync(0xffffffffu, y[0], 2));
+  y[0] = fmaxf(y[0], __shfl_xor_sync(0xffffffffu, y[0], 1));
+  return __shfl_sync(0xffffffffu, y[0], lane << 2 & 31);         // (lane / 4 was the row)
 }
 
 // Moves the maxima of a set of four softmax warps to the largest scores of a tile, and the output with them.  Out of the loop's way.
@@ -169,7 +164,7 @@ __device__ __noinline__ void move_maxima(PrefixShared& sh, uint32_t S, uint32_t 
 #pragma unroll 1
   for (int i = 0; i < active; ++i) {
     const int c = c0 + 8 * i;
-    const float top = row_tops<FP8>(S + 8 * i, sh.row + c, dirty ? sh.lim + c : nullptr, key, ks, false, 0.f, sh.turn[w]);
+    const float top = row_tops<FP8>(S + 8 * i, sh.row + c, dirty ? sh.lim + c : nullptr, key, ks, false, 0.f);
     if (lane < 8) sh.red[w][8 * i + lane] = top;
   }
   named_bar_sync(2 + side, 128);
@@ -189,7 +184,7 @@ __device__ __noinline__ void move_maxima(PrefixShared& sh, uint32_t S, uint32_t 
 #pragma unroll 1
     for (int i = 0; i < active; ++i) {
       const int c = c0 + 8 * i;
-      const float top = row_tops<FP8>(S + 8 * i, sh.row + c, dirty ? sh.lim + c : nullptr, key, ks, true, lv, sh.turn[w]);
+      const float top = row_tops<FP8>(S + 8 * i, sh.row + c, dirty ? sh.lim + c : nullptr, key, ks, true, lv);
       if (lane < 8) sh.red[w][8 * i + lane] = top;
     }
     named_bar_sync(2 + side, 128);
@@ -272,8 +267,6 @@ __global__ void __launch_bounds__(Prefix<FP8>::THREADS, 1)
     }
     abort_word = 0;
     s_poison = 0x7fffffff;
-    s_most = 0;
-    s_least = 0x7fffffff;
     mbar_fence_init();
     tma_prefetch_desc(&tm_k);
     tma_prefetch_desc(&tm_v);
@@ -286,29 +279,72 @@ __global__ void __launch_bounds__(Prefix<FP8>::THREADS, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
-  // (also host-set: where this thread's row is)
-  int q_first = 0, q_len = 0, seq = 0;
-  if (tid < rows) {
-    seq = p.row_seq[t0 + (row0 + tid) / G];
-    q_first = p.q_start[seq];
-    q_len = p.q_start[seq + 1] - q_first;
+  // (also host-set: where the rows of warp 0's threads are)
+  int q_first[2], q_len[2], seq[2];
+  if (warp == 0) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int r = min(lane + 32 * k, rows - 1);
+      seq[k] = p.row_seq[t0 + (row0 + r) / G];
+      q_first[k] = p.q_start[seq[k]];
+      q_len[k] = p.q_start[seq[k] + 1] - q_first[k];
+    }
   }
   if (!args.beside) pdl_wait();                  // (see paged_few_kernel)
   pdl_trigger();
-  // column of row r: 8 (r / 8 / 2) + r % 8 of the half that its set of warps has
   const int* table = p.table + (long long)run.z * p.width;
-  const int per = PK / p.page;                   // pages of a tile
-  int first_page = 0;                            // warp 0: those of the first tile, if all shared tokens are read
-  if (tid < PR) {
-    if (tid < per) first_page = table[(int)((long long)(shared / PK) * part / parts) * per + tid];
-    const int col = (tid >> 3 & 1) * 32 + (tid >> 4) * 8 + (tid & 7);
-    int lim = 0;
-    if (tid < rows) {
-      lim = min(shared, row_limit(p, q_first, q_len, seq_len(p, seq), t0 + (row0 + tid) / G - q_first));
-      atomicMax(&s_most, lim);
-      atomicMin(&s_least, lim);
+  const int page = p.page, per = PK / page;      // pages of a tile
+  // a tile's keys, values and scales; the whole of warp 0, a lane per page
+  auto ask = [&](int n, int pg, int live, int kv) {
+    const int s = n % (kv ? VS : KS);
+    uint64_t* full = kv ? &v_full[s] : &k_full[s];
+    uint8_t* dst = (kv ? sV : sK) + s * F::TILE + lane * page * 128;
+    if (lane == 0) {
+      mbar_expect_tx(full, live * page * (FP8 ? 128 : 256));
+      if (FP8 && kv == 0) mbar_expect_tx(&c_full[n % CS], live * page * 8);
     }
-    sh.lim[col] = lim;
+    __syncwarp();
+    if (lane < live) {
+      if (pg < 0 || pg >= args.pages) report_status(args.status, kBadPage, 10);     // reads as zeros
+      if (FP8) {
+        if (kv == 0) tma_load_4d(sC + ((n % CS) * PK + lane * page) * 2, &tm_v, &c_full[n % CS], 0, head, 0, pg);
+        tma_load_5d(smem_u32(dst), &tm_k, full, 0, 0, head, kv, pg);
+      } else {
+        tma_load_4d(dst, kv ? &tm_v : &tm_k, full, 0, 0, head, pg);
+        tma_load_4d(dst + PK * 128, kv ? &tm_v : &tm_k, full, 64, 0, head, pg);
+      }
+    }
+    __syncwarp();
+  };
+  if (warp == 0) {
+    // column of row r: 8 (r / 8 / 2) + r % 8 of the half that its set of warps has
+    const int guess = lane < per ? table[(int)((long long)(shared / PK) * part / parts) * per + lane] : 0;      // if all shared tokens are read
+    int most = 0, least = 0x7fffffff;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int r = lane + 32 * k, col = (r >> 3 & 1) * 32 + (r >> 4) * 8 + (r & 7);
+      int lim = 0;
+      if (r < rows) {
+        lim = min(shared, row_limit(p, q_first[k], q_len[k], seq_len(p, seq[k]), t0 + (row0 + r) / G - q_first[k]));
+        least = min(least, lim);
+      }
+      most = max(most, lim);
+      sh.lim[col] = lim;
+    }
+    most = __reduce_max_sync(0xffffffffu, most);
+    least = __reduce_min_sync(0xffffffffu, least);
+    if (lane == 0) {
+      s_most = most;
+      s_least = least;
+    }
+    // the first tile is on its way before anybody else is ready
+    const int all = (most + PK - 1) / PK, first = (int)((long long)all * part / parts);
+    if (first < (int)((long long)all * (part + 1) / parts)) {
+      const int live = min(per, (most + page - 1) / page - first * per);
+      const int pg = most == shared ? guess : lane < live ? table[first * per + lane] : 0;
+      ask(0, pg, live, 0);
+      ask(0, pg, live, 1);
+    }
   } else if (warp >= 4 && warp < 12) {
     // queries: four threads per row
     const int s = tid - 128, r = s >> 2, c = s & 3, col = (r >> 3 & 1) * 32 + (r >> 4) * 8 + (r & 7), row = row0 + r;
@@ -380,39 +416,20 @@ __global__ void __launch_bounds__(Prefix<FP8>::THREADS, 1)
   else asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
   if (warp == 0) {
     // ------------------------------ pages --------------------------------
-    const int page = p.page, used = (most + page - 1) / page;
+    const int used = (most + page - 1) / page;
     auto page_of = [&](int n) -> int {
       const int i = (j0 + n) * per + lane;
       return n < n_tiles && lane < per && i < used ? table[i] : 0;
     };
-    int pg = most == shared ? first_page : page_of(0);
-    for (int n = 0; n < n_tiles; ++n) {
+    int pg = page_of(1);
+    bool ok = true;
+    for (int n = 1; n < n_tiles && ok; ++n) {
       const int next = page_of(n + 1), live = min(per, used - (j0 + n) * per);
-      if (lane < live && (pg < 0 || pg >= args.pages)) report_status(args.status, kBadPage, 10);     // reads as zeros
 #pragma unroll
       for (int kv = 0; kv < 2; ++kv) {
-        const int stages = kv ? VS : KS, s = n % stages;
-        uint64_t *const full = kv ? &v_full[s] : &k_full[s], *const empty = kv ? &v_empty[s] : &k_empty[s];
-        uint8_t* dst = (kv ? sV : sK) + s * F::TILE + lane * page * 128;
-        if (!mbar_wait_warp(empty, ((n / stages) & 1) ^ 1, abort_flag, args.status, 1)) {
-          n = n_tiles;
-          break;
-        }
-        if (lane == 0) {
-          mbar_expect_tx(full, live * page * (FP8 ? 128 : 256));
-          if (FP8 && kv == 0) mbar_expect_tx(&c_full[n % CS], live * page * 8);
-        }
-        __syncwarp();
-        if (lane < live) {
-          if (FP8) {
-            if (kv == 0) tma_load_4d(sC + ((n % CS) * PK + lane * page) * 2, &tm_v, &c_full[n % CS], 0, head, 0, pg);
-            tma_load_5d(smem_u32(dst), &tm_k, full, 0, 0, head, kv, pg);
-          } else {
-            tma_load_4d(dst, kv ? &tm_v : &tm_k, full, 0, 0, head, pg);
-            tma_load_4d(dst + PK * 128, kv ? &tm_v : &tm_k, full, 64, 0, head, pg);
-          }
-        }
-        __syncwarp();
+        const int stages = kv ? VS : KS;
+        ok = ok && mbar_wait_warp(kv ? &v_empty[n % stages] : &k_empty[n % stages], ((n / stages) & 1) ^ 1, abort_flag, args.status, 1);
+        if (ok) ask(n, pg, live, kv);
       }
       pg = next;
     }
@@ -530,8 +547,7 @@ __global__ void __launch_bounds__(Prefix<FP8>::THREADS, 1)
         }
       };
       {
-        // Where the maxima begin: at those of the first 32 keys (of a tile that the mask cuts: nowhere, see move_maxima).
-        const int key = j0 * PK + in_tile;
+        // Where the maxima begin: at those of 32 keys (of a tile that the mask cuts: nowhere, see move_maxima).  Every warp sets one group of rows.
         float2 sc = make_float2(1.f, 1.f);
         if (FP8) {
           ok &= mbar_wait(&c_full[0], 0, abort_flag, args.status, 5);
@@ -540,22 +556,19 @@ __global__ void __launch_bounds__(Prefix<FP8>::THREADS, 1)
         ok &= mbar_wait(&s_full[0], 0, abort_flag, args.status, 5);
         __syncwarp();
         tc_fence_after();
-        if ((w & 3) == 0 && j0 * PK + PK <= least) {
+        const int i = w & 3, col = c0 + 8 * i;
+        if (i < active && j0 * PK + PK <= least) {
           const float ks = sc.x * args.scale_log2;
-#pragma unroll 1
-          for (int i = 0; i < active; ++i) {
-            RowState* row = sh.row + c0 + 8 * i;
-            const uint32_t S = tmem + c0 + lanes + 8 * i;
-            const float m = row_tops<FP8>(S, row, nullptr, key, ks, false, 0.f, sh.turn[w]);
-            if (lane < 8) row[lane].m = m;
-            if (FP8) {
-              __syncwarp();
-              const float mv = row_tops<FP8>(S, row, nullptr, key, ks, true, log2_of(sc.y), sh.turn[w]);
-              if (lane < 8) {
-                sh.mv[c0 + 8 * i + lane] = mv;
-                sh.ec[c0 + 8 * i + lane] = exponent_of(mv);
-                sh.vf[c0 + 8 * i + lane] = (uint16_t)((127 + exponent_of(mv)) << 7);
-              }
+          const uint32_t S = tmem + col + lanes;
+          const float m = row_tops<FP8>(S, sh.row + col, nullptr, 0, ks, false, 0.f);
+          if (lane < 8) sh.row[col + lane].m = m;
+          if (FP8) {
+            __syncwarp();
+            const float mv = row_tops<FP8>(S, sh.row + col, nullptr, 0, ks, true, log2_of(sc.y));
+            if (lane < 8) {
+              sh.mv[col + lane] = mv;
+              sh.ec[col + lane] = exponent_of(mv);
+              sh.vf[col + lane] = (uint16_t)((127 + exponent_of(mv)) << 7);
             }
           }
         }
@@ -691,21 +704,18 @@ __global__ void __launch_bounds__(Prefix<FP8>::THREADS, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[n % PS]);
       }
-      // sums over the keys' threads, then the output
+      // Sums over the keys' threads, row i in lane i: every step adds half of the rows across half of the lanes.  Then the output.
+      float l[32];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        float a, b;
-        unpack_f32x2(l2[i], a, b);
+      for (int i = 0; i < 16; ++i) unpack_f32x2(l2[i], l[2 * i], l[2 * i + 1]);
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-          a += __shfl_xor_sync(0xffffffffu, a, o);
-          b += __shfl_xor_sync(0xffffffffu, b, o);
+      for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+        for (int i = 0; i < o; ++i) {
+          const float send = lane & o ? l[i] : l[i + o], keep = lane & o ? l[i + o] : l[i];
+          l[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
         }
-        if (lane == 0) {
-          sh.sum[w][2 * i] = a;
-          sh.sum[w][2 * i + 1] = b;
-        }
-      }
+      sh.sum[w][lane] = l[0];
       ok &= mbar_wait(&pv_done[(n_tiles - 1) % PS], ((n_tiles - 1) / PS) & 1, abort_flag, args.status, 6);
       ok = __all_sync(0xffffffffu, ok);
       tc_fence_after();

@@ -59,10 +59,12 @@ CHUNK_SLOTS = 148        # its CTAs that run at once
 CHUNK_START = 5          # what starting and ending a CTA costs, in key tiles (1.8 us): 8 to 10 us from its start to its end
 CHUNK_JOIN = 3           # what a part costs besides: 128 KB written and read again
 PREFIX_ROWS = 64         # rows of a CTA of the kernel for shared tokens, which are counted in tiles of 128
-PREFIX_SLOTS = 148       # its CTAs that run at once
 PREFIX_LEAST = 2         # a part has at least this many key tiles
-# Us on an SM: to start and end a CTA of shared tokens, one of its tiles; the same for tails, of which three share the SM.
-PREFIX_START, PREFIX_TILE, TAIL_START, TAIL_TILE = 8.0, 1.1, 1.5, 0.8
+# Us on an SM, by type (bf16, e4m3): to start and end a CTA, and one of its tiles.  Of shared tokens: 64 rows, and as chunks 256 (128) rows.  Of
+# tails, three of which share the SM, both for one third of it.
+PREFIX_COST = ((6.0, 1.5), (6.0, 1.55))
+MANY_COST = ((9.0, 1.8), (9.0, 1.75))
+TAIL_COST = ((1.7, 1.5), (1.7, 0.75))
 
 
 _ENTRY: dict = {}         # the entry points that calls go to
@@ -383,13 +385,20 @@ def _together(runs, skip, q_rows, cap, q_start, group: int, heads: int, fp8: boo
     place = np.arange(len(of_run)) - np.repeat(np.cumsum(rows) - rows, rows)
     joins[:, 0] = runs[of_run, 0] + place // group
     joins[:, 1] = place % group
+    # Long runs as chunks or as many items of 64 rows, whichever is done sooner.
+    best = None
+    for by_chunks in (big, np.zeros_like(big)):
+        kinds = []
+        for name, which, m, cost in (("many", by_chunks, whole if fp8 else 2 * whole, MANY_COST[fp8]), ("prefix", ~by_chunks, PREFIX_ROWS, PREFIX_COST[fp8])):
+            count = np.where(which, -(-rows // m), 0)
+            run = np.repeat(np.arange(len(runs)), count)
+            kinds.append((name, which, m, count, run, tokens[run] // CHUNK_TILE, cost))
+        done, parts = _shared_parts([(k[5], *k[6]) for k in kinds], heads, (tail_ctas * TAIL_COST[fp8][0] + tail_tiles * TAIL_COST[fp8][1]) * heads)
+        if best is None or done < best[0]:
+            best = (done, kinds, parts)
     work = {}
-    for name, which, m in (("many", big, whole if fp8 else 2 * whole), ("prefix", ~big, PREFIX_ROWS)):
-        count = np.where(which, -(-rows // m), 0)
-        run = np.repeat(np.arange(len(runs)), count)
+    for (name, which, m, count, run, tiles, _), parts in zip(best[1], best[2]):
         row0 = (np.arange(len(run)) - np.repeat(np.cumsum(count) - count, count)) * m
-        tiles = tokens[run] // CHUNK_TILE
-        parts = _waves(tiles, heads, CHUNK_SLOTS) if name == "many" else _prefix_parts(tiles, heads, tail_ctas, tail_tiles)
         at = first + np.cumsum(parts * m) - parts * m
         first += int((parts * m).sum())
         i = np.repeat(np.arange(len(run)), parts)
@@ -429,23 +438,26 @@ def _together(runs, skip, q_rows, cap, q_start, group: int, heads: int, fp8: boo
             m, first)
 
 
-def _prefix_parts(tiles, heads: int, tail_ctas: int, tail_tiles: int):
-    """Into how many parts the work on shared tokens is split: done soonest, if its CTAs have an SM each, and tails what is left until those are
-    done, then all."""
-    if not len(tiles):
-        return tiles
+def _shared_parts(kinds, heads: int, tails: float):
+    """Into how many parts the work on shared tokens is split, for every kind [tiles of its items, us to start a CTA, us of a tile], and when all is
+    done: its CTAs have an SM each, tails (``tails`` us of an SM) what is left until those are done, then all SMs."""
+    longest = max((int(t.max()) for t, _, _ in kinds if len(t)), default=1)
     best = None
-    for cut in range(1, 2 * PREFIX_SLOTS):
-        split = -(-tiles // -(-int(tiles.max()) // cut))
-        ctas = int(split.sum()) * heads
-        if best is not None and (ctas > PREFIX_SLOTS or int(tiles.max()) < PREFIX_LEAST * cut):
+    for cut in range(1, 2 * CHUNK_SLOTS):
+        share = -(-longest // cut)
+        parts = [-(-t // share) for t, _, _ in kinds]
+        ctas = heads * sum(int(p.sum()) for p in parts)
+        if best is not None and (ctas > CHUNK_SLOTS or share < PREFIX_LEAST):
             break
-        busy = -(-ctas // PREFIX_SLOTS) * (PREFIX_START + float((-(-tiles // split)).max()) * PREFIX_TILE)
-        left = (tail_ctas * TAIL_START + tail_tiles * TAIL_TILE) * heads - busy * max(0, PREFIX_SLOTS - ctas)
-        done = busy + (left / PREFIX_SLOTS + TAIL_START if left > 0 else 0.0)
+        ends = [start + -(-t // p) * tile for (t, start, tile), p in zip(kinds, parts) if len(t)]
+        busy = max(float(e.max()) for e in ends)
+        if ctas > CHUNK_SLOTS:
+            busy = max(busy, heads / CHUNK_SLOTS * sum(float((e * p).sum()) for e, p in zip(ends, (p for p in parts if len(p)))) + busy / 2)
+        left = tails - busy * max(0, CHUNK_SLOTS - ctas)
+        done = busy + max(0.0, left) / CHUNK_SLOTS + (2.0 if left > 0 else 0.0)
         if best is None or done < best[0]:
-            best = (done, split)
-    return best[1]
+            best = (done, parts)
+    return best
 
 
 def _waves(tiles: np.ndarray, heads: int, slots: int) -> np.ndarray:
