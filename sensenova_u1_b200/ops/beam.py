@@ -23,6 +23,7 @@ from ._lib import c_float, c_int, c_ll, c_void_p
 MAX_BEAMS, MAX_KEEP, MAX_EOS = 64, 128, 8
 MAX_VOCAB = 1 << 24
 _ENTRY: dict = {}
+_SCRATCH: dict = {}         # bytes of scratch by rows and tokens
 
 
 class _State(ctypes.Structure):
@@ -53,14 +54,14 @@ def _check(logits, scores, keep: int):
     requests, beams = scores.shape
     if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16) or logits.shape[0] != requests * beams:
         raise ValueError(f"logits must be fp32 or bf16 [{requests} x {beams}, vocab], not {tuple(logits.shape)} {logits.dtype}")
-    vocab = logits.shape[1]
+    vocab, (row, one) = logits.shape[1], logits.stride()
     if not 1 <= beams <= MAX_BEAMS or not 1 <= keep <= MAX_KEEP:
         raise ValueError(f"1 to {MAX_BEAMS} beams, of which 1 to {MAX_KEEP} continuations are kept")
     if requests * beams > 65535 or vocab > MAX_VOCAB:
         raise ValueError("too many rows or tokens")
     if keep > beams * vocab:
         raise ValueError(f"{beams} beams of {vocab} tokens have no {keep} continuations")
-    if logits.stride(1) != 1 and vocab > 1 or (logits.shape[0] > 1 and logits.stride(0) < vocab):
+    if one != 1 and vocab > 1 or (row < vocab and requests * beams > 1):
         raise ValueError("the logits of a row must be contiguous, and rows may not overlap")
     if not logits.is_cuda or scores.device != logits.device:
         raise ValueError("logits and scores must be on one GPU")
@@ -72,8 +73,12 @@ def _launch(logits, scores, requests, beams, vocab, keep, out, state) -> None:
     if index != torch._C._cuda_getDevice():
         with torch.cuda.device(index):
             return _launch(logits, scores, requests, beams, vocab, keep, out, state)
-    entry = _entry()
-    scratch = torch.empty(entry["scratch"](requests * beams, vocab), dtype=torch.uint8, device=logits.device)
+    entry, size = _entry(), (requests * beams, vocab)
+    if size not in _SCRATCH:
+        if len(_SCRATCH) > 64:
+            _SCRATCH.clear()
+        _SCRATCH[size] = entry["scratch"](*size)
+    scratch = torch.empty(_SCRATCH[size], dtype=torch.uint8, device=logits.device)
     _lib.LAUNCHES += 2
     rc = entry["step"](logits.data_ptr(), max(logits.stride(0), vocab), logits.dtype == torch.bfloat16, vocab, scores.data_ptr(), requests, beams,
                        keep, scratch.data_ptr(), *out, state, torch._C._cuda_getCurrentRawStream(index))
@@ -89,13 +94,15 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, keep: int | None = N
     64 bits; of equal ones the lower beam comes first, then the lower token (of one beam, the larger logit).  A beam whose score is -inf or not finite, or whose
     logits hold NaN or +inf, has no continuations, and no token of logit -inf is one; places for which none is left hold score -inf, beam
     0, token 0."""
-    requests, beams, vocab = _check(logits, scores, 2 * scores.shape[-1] if keep is None else keep)
-    keep = 2 * beams if keep is None else keep
-    best = torch.empty(requests, keep, dtype=torch.float32, device=logits.device)
-    at = torch.empty(2, requests, keep, dtype=torch.int32, device=logits.device)
+    if keep is None:
+        keep = 2 * scores.shape[-1]
+    requests, beams, vocab = _check(logits, scores, keep)
+    out = torch.empty((3, requests, keep), dtype=torch.int32, device=logits.device)
     if requests:
-        _launch(logits, scores, requests, beams, vocab, keep, (best.data_ptr(), at.data_ptr(), at.data_ptr() + 4 * requests * keep), None)
-    return best, at[0], at[1]
+        at, row = out.data_ptr(), 4 * requests * keep
+        _launch(logits, scores, requests, beams, vocab, keep, (at, at + row, at + 2 * row), None)
+    best, at, tokens = out.unbind()
+    return best.view(torch.float32), at, tokens
 
 
 class BeamSearch:

@@ -60,11 +60,15 @@ CHUNK_START = 5          # what starting and ending a CTA costs, in key tiles (1
 CHUNK_JOIN = 3           # what a part costs besides: 128 KB written and read again
 PREFIX_ROWS = 64         # rows of a CTA of the kernel for shared tokens, which are counted in tiles of 128
 PREFIX_LEAST = 2         # a part has at least this many key tiles
+# Sharing costs two launches more, so a run has at least so many tokens (bf16, e4m3), or all runs save at least so many tiles of 128 keys of a head.  Us in
+# a graph, with / without, 32 / 8 heads: 2 sequences of 2048 bf16 tokens 10.1 / 9.7, of 4096 11.3 / 13.0; e4m3 11.0 / 9.1, 12.2 / 12.7; 32
+# sequences of 512 12.6 / 10.9, of 1024 14.0 / 15.8, of 8192 22 / 83; 32 / 4 heads, 8 of 2048 12.1 / 12.1, of 4096 12.9 / 14.2.
+SHARE_TOKENS, SHARE_TILES = (2048, 2560), 1900
 # Us on an SM, by type (bf16, e4m3): to start and end a CTA, and one of its tiles.  Of shared tokens: 64 rows, and as chunks 256 (128) rows.  Of
 # tails, three of which share the SM, both for one third of it.
 PREFIX_COST = ((6.0, 1.5), (6.0, 1.55))
 MANY_COST = ((9.0, 1.8), (9.0, 1.75))
-TAIL_COST = ((1.7, 1.5), (1.7, 0.75))
+TAIL_COST = ((1.7, 1.5), (1.7, 1.05))
 
 
 _ENTRY: dict = {}         # the entry points that calls go to
@@ -297,6 +301,9 @@ def _lay_out(q_lens, kv_lens, tables, page: int, pages: int, group: int, kv_head
     q_rows = q * group
     chunked = (q_rows > CHUNK_FROM) & (group <= CHUNK_TILE)
     runs, skip = _shared_runs(shared, n, q, kv, (q_rows > 0) & (q_rows <= FEW_TILE) & ~chunked, None if on_device else table, page)
+    if runs and max(t for _, _, t in runs) < SHARE_TOKENS[fp8] and (
+            kv_heads * sum((int((q[a:a + c] > 0).sum()) - 1) * t for a, c, t in runs) < SHARE_TILES * CHUNK_TILE):
+        runs, skip = [], np.zeros(n, dtype=np.int64)
     few_q = np.where(chunked | (skip > 0), 0, q_rows)
     top = int(few_q.max()) if n else 0
     few_rows = 8 if top <= 8 else 16 if top <= 16 else FEW_TILE
@@ -393,7 +400,7 @@ def _together(runs, skip, q_rows, cap, q_start, group: int, heads: int, fp8: boo
             count = np.where(which, -(-rows // m), 0)
             run = np.repeat(np.arange(len(runs)), count)
             kinds.append((name, which, m, count, run, tokens[run] // CHUNK_TILE, cost))
-        done, parts = _shared_parts([(k[5], *k[6]) for k in kinds], heads, (tail_ctas * TAIL_COST[fp8][0] + tail_tiles * TAIL_COST[fp8][1]) * heads)
+        done, parts = _shared_parts([(k[5], *k[6]) for k in kinds], heads, tail_ctas * TAIL_COST[fp8][0] + tail_tiles * TAIL_COST[fp8][1], tail_ctas)
         if best is None or done < best[0]:
             best = (done, kinds, parts)
     work = {}
@@ -438,9 +445,11 @@ def _together(runs, skip, q_rows, cap, q_start, group: int, heads: int, fp8: boo
             m, first)
 
 
-def _shared_parts(kinds, heads: int, tails: float):
+def _shared_parts(kinds, heads: int, tails: float, tail_ctas: int):
     """Into how many parts the work on shared tokens is split, for every kind [tiles of its items, us to start a CTA, us of a tile], and when all is
-    done: its CTAs have an SM each, tails (``tails`` us of an SM) what is left until those are done, then all SMs."""
+    done.  Its CTAs have an SM each.  Tails (``tails`` us of an SM in ``tail_ctas`` CTAs) take no time of their own if all of them fit the
+    SMs that are left; otherwise most of them run afterwards (fewer parts, to leave them more SMs, were slower: 48 conversations with 6000 common
+    tokens 43 us with 144 CTAs, 52 with 64)."""
     longest = max((int(t.max()) for t, _, _ in kinds if len(t)), default=1)
     best = None
     for cut in range(1, 2 * CHUNK_SLOTS):
@@ -453,8 +462,8 @@ def _shared_parts(kinds, heads: int, tails: float):
         busy = max(float(e.max()) for e in ends)
         if ctas > CHUNK_SLOTS:
             busy = max(busy, heads / CHUNK_SLOTS * sum(float((e * p).sum()) for e, p in zip(ends, (p for p in parts if len(p)))) + busy / 2)
-        left = tails - busy * max(0, CHUNK_SLOTS - ctas)
-        done = busy + max(0.0, left) / CHUNK_SLOTS + (2.0 if left > 0 else 0.0)
+        beside = tail_ctas * heads <= 3 * (CHUNK_SLOTS - ctas)
+        done = busy + (0.0 if beside else heads * tails / CHUNK_SLOTS + 3.0)
         if best is None or done < best[0]:
             best = (done, parts)
     return best
@@ -524,7 +533,7 @@ def build_plan(cache: PagedCache, heads: int, q_lens, kv_lens, tables, limits=No
     runs, ``kv_lens`` and ``grow`` say up to how many tokens they go, and its ``step`` stands in for ``advance``.
 
     ``shared``: [first sequence, how many, tokens] of sequences that begin with the same tokens in the same pages.  Attention
-    reads those once for all of them (in tiles of 128 tokens; the rest, and the keys of chunks, are read by each sequence)."""
+    reads those once for all of them, where that is faster (in tiles of 128 tokens; the rest, and the keys of chunks, are read by each sequence)."""
     if heads < 1 or heads % cache.kv_heads != 0:
         raise ValueError("the number of query heads must be a multiple of the cache's heads")
     with torch.cuda.device(cache.device):                     # (the stream that the copy below goes to)
@@ -540,7 +549,7 @@ def build_plan(cache: PagedCache, heads: int, q_lens, kv_lens, tables, limits=No
             raise ValueError(f"the tables have {live.seqs} sequences")
         tables = live.width
     arrays, counts = _lay_out(q_lens, kv_lens, tables, cache.page, cache.pages, heads // cache.kv_heads, cache.kv_heads,
-                              cache.scales is not None, limits, grow, shared)
+                              cache.scales is not None, limits, grow, shared or ())
     # all arrays in one copy from pinned memory that nothing waits for
     at, total = {}, 0
     for name, a in arrays.items():

@@ -53,9 +53,11 @@ ROOM = {BF16: 0.15, E4M3: 0.45}
 
 
 @pytest.mark.parametrize("dtype", [BF16, E4M3])
-@pytest.mark.parametrize("beams,penalty", [(2, 1.0), (4, 0.0), (8, 1.0)])
-def test_scores_are_those_of_the_sequences(beams, penalty, dtype):
-    from sensenova_u1_b200.ops import _lib
+@pytest.mark.parametrize("beams,penalty,always", [(2, 1.0, True), (4, 0.0, False), (8, 1.0, True)])
+def test_scores_are_those_of_the_sequences(beams, penalty, always, dtype, monkeypatch):
+    from sensenova_u1_b200.ops import _lib, paged
+    if always:                                  # prompts are read together however short they are
+        monkeypatch.setattr(paged, "SHARE_TOKENS", (0, 0))
     cfg, store, eng = model()
     docs = prompts(cfg, [290, 37, 131])
     out = eng.beam_search(docs, beams, 12, stop_ids=(5,), length_penalty=penalty, best=beams, page=16, dtype=dtype)

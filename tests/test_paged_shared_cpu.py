@@ -7,6 +7,12 @@ import pytest
 from sensenova_u1_b200.ops import paged
 
 
+@pytest.fixture(autouse=True)
+def always(monkeypatch):
+    """Shared however short it is."""
+    monkeypatch.setattr(paged, "SHARE_TOKENS", (0, 0))
+
+
 def lay(q, kv, tables, shared, page=16, group=4, heads=2, fp8=False, limits=None, grow=0, pages=1 << 20):
     return paged._lay_out(list(q), list(kv), tables, page, pages, group, heads, fp8, limits, grow, shared)
 
@@ -131,3 +137,17 @@ def test_tables_on_the_device_are_not_looked_at():
     assert a["table"] is None and a["kv_len"] is None and c["width"] == 20 and c["prefix_count"] > 0
     with pytest.raises(ValueError):
         lay([1, 1], [300, 330], 20, [])
+
+
+def test_shared_where_it_is_faster(monkeypatch):
+    monkeypatch.undo()
+    for fp8, n, tokens, heads, want in [(False, 2, 1920, 8, False), (False, 2, 2048, 8, True), (True, 2, 2048, 8, False), (True, 2, 2560, 4, True),
+                                        (False, 16, 1024, 8, False), (False, 33, 1024, 8, True), (True, 64, 256, 8, False)]:
+        kv = [tokens + 5 + i for i in range(n)]
+        a, c = lay([1] * n, kv, alike(kv, tokens, 64), [(0, n, tokens)], page=64, heads=heads, fp8=fp8)
+        assert (c["tail_count"] > 0) == want and (c["few_count"] == 0) == want
+    kv = [1030] * 20                                                 # several runs together
+    t = alike(kv[:10], 1024, 64)
+    t += [[p + 10000 for p in x] for x in t]
+    assert lay([1] * 20, kv, t, [(0, 10, 1024), (10, 10, 1024)], page=64, heads=16)[1]["tail_count"] > 0
+    assert lay([1] * 20, kv, t, [(0, 10, 1024), (10, 10, 1024)], page=64, heads=8)[1]["tail_count"] == 0

@@ -7,6 +7,13 @@ from test_paged_gpu import BF16, D, E4M3, SCALE, causal, exact, near, quantised
 pytestmark = pytest.mark.gpu
 
 
+@pytest.fixture(autouse=True)
+def always(monkeypatch):
+    """Shared however short it is."""
+    from sensenova_u1_b200.ops import paged
+    monkeypatch.setattr(paged, "SHARE_TOKENS", (0, 0))
+
+
 def setup(groups, page, hk, dtype, seed=0, room=0, stretch=True):
     """``groups``: (shared tokens, lengths of the sequences).  The cache, tables, what every sequence holds in 64 bits, and the argument ``shared``."""
     from sensenova_u1_b200.ops import paged
