@@ -47,9 +47,9 @@ __device__ __forceinline__ float ex2(float x) {
 
 struct Group {         // of a row's logits
   double sum;          // of exp(x - max)
-  float max;           // NaN if there is one
-  int pad;
+  float quarter[4];    // maxima of its quarters; NaN if the group holds one
 };
+__device__ __forceinline__ float top_of(const Group& g) { return fmaxf(fmaxf(g.quarter[0], g.quarter[1]), fmaxf(g.quarter[2], g.quarter[3])); }
 
 struct PassArgs {
   const void* logits;
@@ -101,7 +101,10 @@ __global__ void __launch_bounds__(THREADS) pass_kernel(const PassArgs a) {
   for (int j = 1; j + 1 < E; j += 2) m = fmaxf(m, fmaxf(v[j], v[j + 1]));
   m = fmaxf(m, v[E - 1]);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  for (int o = 1; o < 8; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  const float quarter = m;                               // eight lanes'
+#pragma unroll
+  for (int o = 8; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   constexpr float LOG2E = 1.44269502162933349609375f;
   const float from = m > -INFINITY ? m : 0.f;
   float sum = 0.f;                                       // NaN if there is one
@@ -110,11 +113,14 @@ __global__ void __launch_bounds__(THREADS) pass_kernel(const PassArgs a) {
   double total = sum;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-  if (lane == 0) a.out[(long long)row * a.groups + group] = Group{total, total == total ? m : __int_as_float(0x7fffffff), 0};
+  Group* out = a.out + (long long)row * a.groups + group;
+  if ((lane & 7) == 0) out->quarter[lane >> 3] = total == total ? quarter : __int_as_float(0x7fffffff);
+  if (lane == 0) out->sum = total;
 }
 
 constexpr int JOIN_THREADS = 1024;
 constexpr int JOIN_LIST = 2048;      // candidates that fit; where more are not below the bound, it is raised to the keep-th best of these
+constexpr int RANKED = 384;          // as many are ranked at once
 constexpr int JOIN_GROUPS = 1024;    // groups that fit a list; more are looked for by every warp in its own share
 constexpr int MAX_BEAMS = 64;
 
@@ -249,9 +255,10 @@ __device__ void follow(const JoinArgs& a, int r, Chosen& c) {
 struct JoinShared {
   double lse[MAX_BEAMS];
   float base[MAX_BEAMS], least[MAX_BEAMS];
-  unsigned long long top[JOIN_THREADS / 4], list_s[JOIN_LIST];      // (list_s: the candidates' scores once more, to be counted)
+  unsigned long long set[JOIN_THREADS], top[JOIN_THREADS / 4], nth, list_s[JOIN_LIST];      // (list_s: the candidates' scores once more, to be counted)
   Best list[JOIN_LIST];
   int pass[JOIN_GROUPS];
+  short pick[JOIN_LIST];
   Best bound;
   int passing, count;
   Chosen out;
@@ -277,23 +284,27 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const JoinArgs a) {
     const Group* p = group + (long long)b * a.groups;
     constexpr int HELD = 5;                                // of a lane; more are looked up again
     const float base = a.scores[(long long)r * K + b];
-    Group x[HELD];
+    double sums[HELD];
+    float tops[HELD];
     float m = -INFINITY;
     bool bad = !(fabsf(base) < INFINITY);                  // (a beam that is not there)
 #pragma unroll
     for (int i = 0; i < HELD; ++i) {
-      x[i].max = -INFINITY;
-      x[i].sum = 0.0;
-      if (lane + 32 * i < a.groups) x[i] = p[lane + 32 * i];
+      tops[i] = -INFINITY;
+      sums[i] = 0.0;
+      if (lane + 32 * i < a.groups) {
+        tops[i] = top_of(p[lane + 32 * i]);
+        sums[i] = p[lane + 32 * i].sum;
+      }
     }
 #pragma unroll
     for (int i = 0; i < HELD; ++i) {
-      bad |= !(x[i].max < INFINITY);
-      m = fmaxf(m, x[i].max);
+      bad |= !(tops[i] < INFINITY);
+      m = fmaxf(m, tops[i]);
     }
 #pragma unroll 4
     for (int i = lane + 32 * HELD; i < a.groups; i += 32) {
-      const float y = p[i].max;
+      const float y = top_of(p[i]);
       bad |= !(y < INFINITY);
       m = fmaxf(m, y);
     }
@@ -304,11 +315,11 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const JoinArgs a) {
     if (!bad) {
 #pragma unroll
       for (int i = 0; i < HELD; ++i)
-        if (x[i].max > -INFINITY) sum += x[i].sum * exp((double)x[i].max - (double)m);
+        if (tops[i] > -INFINITY) sum += sums[i] * exp((double)tops[i] - (double)m);
 #pragma unroll 4
       for (int i = lane + 32 * HELD; i < a.groups; i += 32) {
-        const Group y = p[i];
-        if (y.max > -INFINITY) sum += y.sum * exp((double)y.max - (double)m);
+        const float y = top_of(p[i]);
+        if (y > -INFINITY) sum += p[i].sum * exp((double)y - (double)m);
       }
     }
 #pragma unroll
@@ -329,20 +340,16 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const JoinArgs a) {
 #pragma unroll
   for (int k = 0; k < OWN; ++k) {
     const int i = tid + k * JOIN_THREADS;
-    own[k] = i < all ? score_of(group[i].max, i / a.groups) : 0ull;
+    own[k] = i < all ? score_of(top_of(group[i]), i / a.groups) : 0ull;
   }
-  // The bound: the keep-th largest of ``values`` sets of groups' maxima, every values-th group a set, so that few groups are a set each.
-  // A value's place is counted by ``share`` threads.
-  {
-    unsigned long long mine = 0;
-#pragma unroll
-    for (int k = 0; k < OWN; ++k) mine = max(mine, own[k]);
-#pragma unroll 4
-    for (int i = tid + OWN * JOIN_THREADS; i < all; i += JOIN_THREADS) mine = max(mine, score_of(group[i].max, i / a.groups));
+  // The keep-th largest of the largest of 64 to 256 sets of the threads' values, every 64th to 256th thread a set (threads side by side are in
+  // different ones, so that few values are a set each); 0 if fewer sets have any.  Its place is counted by ``share`` threads.
+  auto nth_of = [&](unsigned long long mine) -> unsigned long long {
     const int share = keep <= 32 ? 16 : keep <= 64 ? 8 : 4, values = JOIN_THREADS / share, sub = tid & (share - 1);
-    sh.list_s[tid] = mine;
+    sh.set[tid] = mine;
+    if (tid == 0) sh.nth = 0;
     __syncthreads();
-    mine = sh.list_s[tid / share + sub * values];          // (groups side by side are in different sets)
+    mine = sh.set[tid / share + sub * values];
     for (int o = 1; o < share; o <<= 1) mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, o));
     if (sub == 0) sh.top[tid / share] = mine;
     __syncthreads();
@@ -357,7 +364,25 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const JoinArgs a) {
       above += __shfl_xor_sync(0xffffffffu, above, o);
       equal += __shfl_xor_sync(0xffffffffu, equal, o);
     }
-    if (sub == 0 && mine != 0 && above < keep && above + equal >= keep) sh.bound.s = mine;         // (whoever writes, writes the same)
+    if (sub == 0 && mine != 0 && above < keep && above + equal >= keep) sh.nth = mine;            // (whoever writes, writes the same)
+    __syncthreads();
+    return sh.nth;
+  };
+  {
+    // the bound, from the groups' maxima
+    unsigned long long mine = 0;
+#pragma unroll
+    for (int k = 0; k < OWN; ++k) mine = max(mine, own[k]);
+#pragma unroll 4
+    for (int i = tid + OWN * JOIN_THREADS; i < all; i += JOIN_THREADS) mine = max(mine, score_of(top_of(group[i]), i / a.groups));
+    // (of few groups, the first step's one beam, say, from their quarters)
+    if (all <= JOIN_THREADS / 4 || __syncthreads_count(mine != 0) < 2 * keep) {
+      mine = 0;
+#pragma unroll 4
+      for (int i = tid; i < 4 * all; i += JOIN_THREADS) mine = max(mine, score_of(group[i >> 2].quarter[i & 3], (i >> 2) / a.groups));
+    }
+    const unsigned long long nth = nth_of(mine);
+    if (tid == 0 && nth != 0) sh.bound.s = nth;
   }
   if (tid == 0) sh.count = sh.passing = 0;
   __syncthreads();
@@ -374,7 +399,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const JoinArgs a) {
 #pragma unroll
     for (int k = 0; k < OWN; ++k) see(own[k], tid + k * JOIN_THREADS);
 #pragma unroll 4
-    for (int i = tid + OWN * JOIN_THREADS; i < all; i += JOIN_THREADS) see(score_of(group[i].max, i / a.groups), i);
+    for (int i = tid + OWN * JOIN_THREADS; i < all; i += JOIN_THREADS) see(score_of(top_of(group[i]), i / a.groups), i);
     if (tid < K) {
       const double to = value64(bound.s), from = sh.base[tid], x = to - from + sh.lse[tid];
       sh.least[tid] = bound.s == 1 ? -FLT_MAX
@@ -385,7 +410,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const JoinArgs a) {
     const bool listed = passing <= JOIN_GROUPS;
     for (int i = warp; i < (listed ? passing : all); i += JOIN_THREADS / 32) {
       const int g = listed ? sh.pass[i] : i, b = g / a.groups;
-      if (!listed && score_of(group[g].max, b) < bound.s) continue;
+      if (!listed && score_of(top_of(group[g]), b) < bound.s) continue;
       float v[E];
       load_group<T, E>(logits + b * a.ld, a.V, g - b * a.groups, v);
       const float least = sh.least[b];
@@ -405,17 +430,32 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const JoinArgs a) {
     for (int i = tid; i < here; i += JOIN_THREADS) sh.list_s[i] = sh.list[i].s = score_of(__uint_as_float((uint32_t)sh.list[i].s), (int)sh.list[i].beam);
     if (tid == 0) sh.count = sh.passing = 0;
     __syncthreads();
+    // of many only those are ranked that can be among the best
+    int few = here;
+    const bool picked = here > RANKED;
+    if (picked) {
+      unsigned long long mine = 0;
+      for (int i = tid; i < here; i += JOIN_THREADS) mine = max(mine, sh.list_s[i]);
+      const unsigned long long nth = max(nth_of(mine), 1ull);
+      for (int i = tid; i < here; i += JOIN_THREADS)
+        if (sh.list_s[i] >= nth) sh.pick[atomicAdd(&sh.count, 1)] = (short)i;
+      __syncthreads();
+      few = sh.count;
+      __syncthreads();
+      if (tid == 0) sh.count = 0;
+    }
     int share = 1;                                         // threads for one candidate (a power of two, neighbours)
-    while (2 * share * here <= JOIN_THREADS && share < 32) share *= 2;
-    for (int i0 = 0; i0 < here; i0 += JOIN_THREADS / share) {
-      const int i = i0 + tid / share, sub = tid & (share - 1);
-      const Best e = i < here ? sh.list[i] : Best{0, 0, 0};
+    while (2 * share * few <= JOIN_THREADS && share < 32) share *= 2;
+    for (int i0 = 0; i0 < few; i0 += JOIN_THREADS / share) {
+      const int i = i0 + tid / share, sub = tid & (share - 1), at = i < few && picked ? sh.pick[i] : i;
+      const Best e = i < few ? sh.list[at] : Best{0, 0, 0};
       int rank = 0;
 #pragma unroll 4
-      for (int k = sub; k < here; k += share) {
-        const unsigned long long s = sh.list_s[k];
+      for (int k = sub; k < few; k += share) {
+        const int other = picked ? sh.pick[k] : k;
+        const unsigned long long s = sh.list_s[other];
         rank += s > e.s;
-        if (s == e.s) rank += before(sh.list[k], e);       // (itself, seldom another)
+        if (s == e.s) rank += before(sh.list[other], e);   // (itself, seldom another)
       }
       for (int o = 1; o < share; o <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
       if (sub == 0 && e.s != 0 && rank < keep) {
