@@ -95,7 +95,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, keep: int | None = N
     logits hold NaN or +inf, has no continuations, and no token of logit -inf is one; places for which none is left hold score -inf, beam
     0, token 0."""
     if keep is None:
-        keep = 2 * scores.shape[-1]
+        keep = 2 * scores.shape[-1] if scores.dim() == 2 else 0
     requests, beams, vocab = _check(logits, scores, keep)
     out = torch.empty((3, requests, keep), dtype=torch.int32, device=logits.device)
     if requests:

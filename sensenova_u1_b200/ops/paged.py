@@ -450,23 +450,25 @@ def _shared_parts(kinds, heads: int, tails: float, tail_ctas: int):
     done.  Its CTAs have an SM each.  Tails (``tails`` us of an SM in ``tail_ctas`` CTAs) take no time of their own if all of them fit the
     SMs that are left; otherwise most of them run afterwards (fewer parts, to leave them more SMs, were slower: 48 conversations with 6000 common
     tokens 43 us with 144 CTAs, 52 with 64)."""
-    longest = max((int(t.max()) for t, _, _ in kinds if len(t)), default=1)
-    best = None
+    sizes = [(int(t), int(c), start, tile) for tiles, start, tile in kinds for t, c in zip(*np.unique(tiles, return_counts=True))]
+    longest = max((t for t, *_ in sizes), default=1)
+    best, share = None, 0
     for cut in range(1, 2 * CHUNK_SLOTS):
+        if -(-longest // cut) == share:
+            continue
         share = -(-longest // cut)
-        parts = [-(-t // share) for t, _, _ in kinds]
-        ctas = heads * sum(int(p.sum()) for p in parts)
+        split = [(c, -(-t // share), start + -(-t // -(-t // share)) * tile) for t, c, start, tile in sizes]       # items, parts, us of one
+        ctas = heads * sum(c * n for c, n, _ in split)
         if best is not None and (ctas > CHUNK_SLOTS or share < PREFIX_LEAST):
             break
-        ends = [start + -(-t // p) * tile for (t, start, tile), p in zip(kinds, parts) if len(t)]
-        busy = max(float(e.max()) for e in ends)
+        busy = max(us for *_, us in split)
         if ctas > CHUNK_SLOTS:
-            busy = max(busy, heads / CHUNK_SLOTS * sum(float((e * p).sum()) for e, p in zip(ends, (p for p in parts if len(p)))) + busy / 2)
+            busy = max(busy, heads / CHUNK_SLOTS * sum(c * n * us for c, n, us in split) + busy / 2)
         beside = tail_ctas * heads <= 3 * (CHUNK_SLOTS - ctas)
         done = busy + (0.0 if beside else heads * tails / CHUNK_SLOTS + 3.0)
         if best is None or done < best[0]:
-            best = (done, parts)
-    return best
+            best = (done, share)
+    return best[0], [-(-tiles // best[1]) for tiles, _, _ in kinds]
 
 
 def _waves(tiles: np.ndarray, heads: int, slots: int) -> np.ndarray:

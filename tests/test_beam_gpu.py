@@ -63,7 +63,7 @@ def some(r, k, v, dtype=torch.float32, seed=0):
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("r,k,v,keep", [(1, 1, 1, 1), (3, 2, 5, 10), (2, 4, 1000, None), (1, 4, 151936, 8), (5, 3, 4099, 6), (2, 64, 700, 128),
-                                        (4, 8, 32001, 16), (1, 1, 2048, 17), (7, 5, 8193, 33), (40, 4, 8191, 1), (3, 32, 20000, 64), (1, 2, 300000, 128)])
+                                        (4, 8, 32001, 16), (1, 1, 2048, 17), (7, 5, 8193, 33), (40, 4, 8191, 1), (3, 32, 20000, 64), (1, 2, 300000, 128), (2, 3, 1 << 21, 12)])
 def test_best_of_all(r, k, v, keep, dtype):
     check(*some(r, k, v, dtype, seed=v), keep)
 
@@ -141,7 +141,7 @@ def test_first_step_and_large_values():
 def test_refusals():
     from sensenova_u1_b200.ops import beam
     x, s = some(2, 3, 50)
-    for logits, scores, keep in [(x[:5], s, 6), (x.double(), s, 6), (x, s.double(), 6), (x, s, 0), (x, s, 129), (x, s, 151), (x, s, 2.0), (x.cpu(), s.cpu(), 6),
+    for logits, scores, keep in [(x[:5], s, 6), (x.double(), s, 6), (x, s.double(), 6), (x, s, 0), (x, s, 129), (x, s, 151), (x, s, 2.0), (x.cpu(), s.cpu(), 6), (x, s[0], None), (x, s.view(-1), None),
                                  (x, s.t(), 6), (x.t().contiguous().t(), s, 6), (x[:, None], s, 6), (x[:1].expand(6, 50), s, 6),
                                  (torch.zeros(65, 50, device="cuda"), torch.zeros(1, 65, device="cuda"), 6)]:
         with pytest.raises(ValueError):

@@ -76,7 +76,7 @@ def raw(x):
 
 
 @pytest.mark.parametrize("page,hk,dtype,layers", [(16, 3, BF16, 2), (64, 1, E4M3, 3), (128, 2, BF16, 1), (32, 4, E4M3, 1)])
-@pytest.mark.parametrize("seqs,most", [(1, 300), (5, 700), (33, 260), (600, 90)])
+@pytest.mark.parametrize("seqs,most", [(1, 300), (5, 700), (33, 260), (600, 90), (1024, 40)])
 def test_random_walks(page, hk, dtype, layers, seqs, most):
     from sensenova_u1_b200.ops import _lib, page_tables
     rng = random.Random(seqs * page)
@@ -204,3 +204,19 @@ def test_refusals():
         with pytest.raises(ValueError):
             t.step(**kw)
     assert t.lens.tolist() == [0, 0, 0]
+
+
+def test_a_large_pool_and_long_tables():
+    """Free pages far apart in a pool of 70000, tables of 2048 pages."""
+    from sensenova_u1_b200.ops import _lib, page_tables, paged
+    pages, page, seqs = 70000, 16, 33
+    cache = paged.PagedCache.empty(pages, page, 1)
+    t, plain = page_tables.PageTables(cache, seqs, 2048 * page), Plain(pages, page, seqs)
+    parents = [-1] * seqs
+    lens = [2048 * page - 20 - 16 * i for i in range(seqs)]
+    for args in [(lens, parents, None), ([0] * seqs, [i if i % 3 else -1 for i in range(seqs)], None), ([5] * seqs, [1, 1] + [2] * 20 + list(range(22, 33)), None),
+                 ([17] * seqs, list(range(seqs)), [1000 * i for i in range(seqs)])]:
+        plain.step(*args)
+        t.step(on(args[0]), parents=on(args[1]), keep=None if args[2] is None else on(args[2]))
+        _lib.check_status()
+        same(t, plain)

@@ -136,6 +136,67 @@ def test_limits(dtype):
 
 
 @BOTH
+def test_limits_of_many_rows(dtype):
+    """The same where a run has more rows than a CTA of 64: some read part of the shared tokens, some nothing."""
+    g = torch.Generator().manual_seed(4)
+    kv = [900 + 17 * i for i in range(24)]
+    q = [1 + i % 3 for i in range(24)]
+    limits = [int(torch.randint(0, k + 1, (), generator=g)) if i % 3 else k for k, n in zip(kv, q) for i in range(n)]
+    plan = check([(896, kv)], q, 8, 2, 64, dtype, limits=limits)
+    assert plan._args.tail_count > 0
+    check([(896, kv)], q, 8, 2, 64, dtype, limits=[0] * sum(q))
+    check([(896, kv)], [1] * 24, 32, 4, 16, dtype, limits=[min(k, 128 * i) for i, k in enumerate(kv)])
+
+
+@BOTH
+@pytest.mark.parametrize("n", [5, 40])
+def test_in_place_and_two_streams(n, dtype):
+    """The output over the queries, and calls of one plan side by side."""
+    from sensenova_u1_b200.ops import paged
+    cache, tables, kv, _, shared = setup([(1500, [1501 + 9 * i for i in range(n)]), (0, [300, 90])], 64, 2, dtype)
+    q = queries(n + 3, 8)
+    plan = paged.build_plan(cache, 8, [1] * n + [2, 1], kv, tables, shared=shared)
+    want = paged.paged_attention(q, cache, plan, SCALE)
+    streams, outs = [torch.cuda.Stream() for _ in range(3)], []
+    for i in range(9):
+        s = streams[i % 3]
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            outs.append(paged.paged_attention(q, cache, plan, SCALE))
+    torch.cuda.synchronize()
+    for o in outs:
+        assert torch.equal(o, want)
+    x = q[:n + 3].clone()
+    paged.paged_attention(x, cache, plan, SCALE, out=x)
+    assert torch.equal(x, want)
+
+
+@BOTH
+def test_tables_that_have_been_cut(dtype):
+    """Sequences of a device's tables that are shorter than the plan says: they read what they have, one that is empty reads nothing."""
+    from sensenova_u1_b200.ops import _lib, page_tables, paged
+    for n in (4, 30):
+        cache, tables, kv, _, shared = setup([(640, [700 + i for i in range(n)])], 64, 2, dtype)
+        t = page_tables.PageTables(cache, n, 800)
+        t.load(kv, tables)
+        plan = paged.build_plan(cache, 8, [1] * n, kv, t, shared=shared)
+        keep = [k if i % 3 == 0 else 0 if i % 3 == 1 else 333 for i, k in enumerate(kv)]
+        t.step(0, keep=torch.tensor(keep, dtype=torch.int32, device="cuda"))
+        _lib.check_status()
+        q = queries(n, 8)
+        out = paged.paged_attention(q, cache, plan, SCALE)
+        _lib.check_status()
+        held = cache.data.double() if dtype == BF16 else cache.data.double() * cache.scales.double()[..., None]      # (rows have been copied)
+        rows = rows_of(held, t.table.tolist(), keep)
+        ref, room = exact(q[:n], [1] * n, rows, torch.tensor(keep, device="cuda"), dtype)
+        some = [i for i in range(n) if i % 3 != 1]
+        full = [r if r.shape[2] else rows[0][:, :, :1] for r in rows]
+        room = wider(room, q[:n], [1] * n, full, torch.tensor([max(k, 1) for k in keep], device="cuda"), plan)
+        assert near(out[some], ref[some], room[some])
+        assert not out[[i for i in range(n) if i % 3 == 1]].any()
+
+
+@BOTH
 def test_no_tokens_beyond_the_shared(dtype):
     check([(512, [512, 512, 513])], [1, 3, 1], 8, 2, 64, dtype)
 
