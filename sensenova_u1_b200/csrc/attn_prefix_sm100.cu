@@ -7,13 +7,18 @@
 // The rows of a run are its new tokens times the query heads of the group, up to 64 per CTA.  They are the N of both products
 // (tcgen05.mma, accumulators in tensor memory), the 128 keys of a tile (the 128 values of a head) the M: eight rows cost an eighth of 64,
 // where rows as the M would fill 128 lanes whatever their number.  A thread of the softmax has one key and a column per row, so the
-// maximum over keys lies across lanes; it moves only when it is outgrown (by 2^8), and a vote per tile is all that costs.  Sums stay
-// with the threads until the end.
+// maximum over keys lies across lanes.  It begins at that of 32 keys and moves only when a probability would pass 2^60 (P_MOST), and a vote per
+// tile is all that costs.  Sums stay with the threads until the end.
 //
 // e4m3 codes go to the first product as they are; a query is two e4m3 numbers, each row times a power of two: hi has 4 of the 8 bits
-// of bf16, lo the others, 16 times as large, as 64 more columns.  A value of less than 2^-14 of its row's largest loses bits below 2^-22 of it.  A key's scale
-// is a number of the thread's.  For the second product four warps widen codes to fp16, which is exact; a value's scale goes into its probability, times a
-// power of two per row that keeps the largest product at 2^7 to 2^15.  bf16: probabilities are two bf16 numbers, hi and lo as 64 columns each.
+// of bf16, lo the others, 16 times as large, as 64 more columns.  A value of less than 2^-14 of its row's largest loses bits below 2^-22 of it.  A key's
+// scale is a number of the thread's.  For the second product four warps widen codes to fp16, which is exact; a value's scale goes into its probability,
+// times a power of two per row that keeps the largest product between 2^4 and 2^15 (W_TOP), and what that leaves of fp16's range is 28 bits below
+// the largest.  bf16: probabilities are two bf16 numbers, hi and lo as 64 columns each.
+//
+// What bounds it: with bf16 memory (8 heads, 80000 shared tokens: 8 rows 57 us, 64 rows 62, their bytes alone 50).  With e4m3 the softmax warps' issue,
+// 1.45 us a tile at 64 rows, and the widening at 8 (43 and 66 us, the bytes alone 26).  Short prefixes: the start and the end of a CTA, 8 us together, of
+// which the first page look-up, its copy, the first product and the last one follow each other (8 heads, 16000 tokens: 17 us and 25 to 27).
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 #include <math.h>
@@ -412,104 +417,104 @@ __global__ void __launch_bounds__(Prefix<FP8>::THREADS, 1)
   const int j0 = (int)((long long)all * part / parts), n_tiles = (int)((long long)all * (part + 1) / parts) - j0;
   // e4m3: 512 threads start with 128 registers, 256 x 72 + 256 x 184 = 512 x 128; bf16: 384 with 168, 128 x 88 + 256 x 208 = 384 x 168
   if (warp < 4 || warp >= 12) {
-  if (FP8) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-  else asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-  if (warp == 0) {
-    // ------------------------------ pages --------------------------------
-    const int used = (most + page - 1) / page;
-    auto page_of = [&](int n) -> int {
-      const int i = (j0 + n) * per + lane;
-      return n < n_tiles && lane < per && i < used ? table[i] : 0;
-    };
-    int pg = page_of(1);
-    bool ok = true;
-    for (int n = 1; n < n_tiles && ok; ++n) {
-      const int next = page_of(n + 1), live = min(per, used - (j0 + n) * per);
-#pragma unroll
-      for (int kv = 0; kv < 2; ++kv) {
-        const int stages = kv ? VS : KS;
-        ok = ok && mbar_wait_warp(kv ? &v_empty[n % stages] : &k_empty[n % stages], ((n / stages) & 1) ^ 1, abort_flag, args.status, 1);
-        if (ok) ask(n, pg, live, kv);
-      }
-      pg = next;
-    }
-  } else if (warp == 1) {
-    // ------------------------------ products --------------------------------
-    bool ok = mbar_wait(&q_ready, 0, abort_flag, args.status, 3);
-    const uint64_t q_desc = make_smem_desc(smem_u32(sQ), 0, 1024), k_desc = make_smem_desc(smem_u32(sK), 0, 1024);
-    const uint64_t v_desc = make_smem_desc(smem_u32(FP8 ? sW : sV), PK * 128, 1024), p_desc = make_smem_desc(smem_u32(sP), PK * 128, 1024);
-    // (e4m3: bits [7,13) of the descriptor are 0 for e4m3 operands, and for fp16 ones)
-    constexpr uint32_t types = 1u << 7 | 1u << 10;
-    constexpr uint32_t idesc_s = FP8 ? make_idesc_bf16(128, 2 * PR, false, false) & ~types : make_idesc_bf16(128, PR, false, false);
-    constexpr uint32_t idesc_o = FP8 ? make_idesc_bf16(128, PR, true, true) & ~types : make_idesc_bf16(128, 2 * PR, true, true);
-    auto issue_s = [&](int n) {
-      ok &= mbar_wait(&k_full[n % KS], (n / KS) & 1, abort_flag, args.status, 3);
-      ok &= mbar_wait(&s_empty[n & 1], ((n >> 1) & 1) ^ 1, abort_flag, args.status, 2);
-      tc_fence_after();
-      const uint64_t kd = k_desc + (n % KS) * (F::TILE >> 4);
-      const uint32_t d = tmem + (n & 1) * F::S_COLS;
-      __syncwarp();
-      if (elect_one()) {
-        if (FP8) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k) umma_f8_ss(d, kd + 2 * k, q_desc + 2 * k, idesc_s, k > 0);
-        } else {
-#pragma unroll
-          for (int k = 0; k < 8; ++k)
-            umma_bf16_ss(d, kd + (k >> 2) * (PK * 128 >> 4) + (k & 3) * 2, q_desc + (k >> 2) * (PR * 128 >> 4) + (k & 3) * 2, idesc_s, k > 0);
+    if (FP8) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if (warp == 0) {
+      // ------------------------------ pages --------------------------------
+      const int used = (most + page - 1) / page;
+      auto page_of = [&](int n) -> int {
+        const int i = (j0 + n) * per + lane;
+        return n < n_tiles && lane < per && i < used ? table[i] : 0;
+      };
+      int pg = page_of(1);
+      bool ok = true;
+      for (int n = 1; n < n_tiles && ok; ++n) {
+        const int next = page_of(n + 1), live = min(per, used - (j0 + n) * per);
+  #pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+          const int stages = kv ? VS : KS;
+          ok = ok && mbar_wait_warp(kv ? &v_empty[n % stages] : &k_empty[n % stages], ((n / stages) & 1) ^ 1, abort_flag, args.status, 1);
+          if (ok) ask(n, pg, live, kv);
         }
-        umma_commit(&s_full[n & 1]);
-        umma_commit(&k_empty[n % KS]);
+        pg = next;
       }
-      __syncwarp();
-    };
-    if (n_tiles > 0) issue_s(0);
-    for (int n = 0; n < n_tiles; ++n) {          // all tiles also after a time-out
-      if (n + 1 < n_tiles) issue_s(n + 1);
-      ok &= mbar_wait(FP8 ? &w_full[n % WS] : &v_full[n % VS], FP8 ? (n / WS) & 1 : (n / VS) & 1, abort_flag, args.status, 3);
-      ok &= mbar_wait(&p_full[n % PS], (n / PS) & 1, abort_flag, args.status, 2);
-      tc_fence_after();
-      const uint64_t vd = v_desc + (FP8 ? (n % WS) * (F::WIDE >> 4) : (n % VS) * (F::TILE >> 4)), pd = p_desc + (n % PS) * (F::P >> 4);
-      __syncwarp();
-      if (elect_one()) {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) umma_bf16_ss(tmem + F::O_AT, vd + k * (2048 >> 4), pd + k * (2048 >> 4), idesc_o, n > 0 || k > 0);
-        umma_commit(&pv_done[n % PS]);
-        umma_commit(FP8 ? &w_empty[n % WS] : &v_empty[n % VS]);
+    } else if (warp == 1) {
+      // ------------------------------ products --------------------------------
+      bool ok = mbar_wait(&q_ready, 0, abort_flag, args.status, 3);
+      const uint64_t q_desc = make_smem_desc(smem_u32(sQ), 0, 1024), k_desc = make_smem_desc(smem_u32(sK), 0, 1024);
+      const uint64_t v_desc = make_smem_desc(smem_u32(FP8 ? sW : sV), PK * 128, 1024), p_desc = make_smem_desc(smem_u32(sP), PK * 128, 1024);
+      // (e4m3: bits [7,13) of the descriptor are 0 for e4m3 operands, and for fp16 ones)
+      constexpr uint32_t types = 1u << 7 | 1u << 10;
+      constexpr uint32_t idesc_s = FP8 ? make_idesc_bf16(128, 2 * PR, false, false) & ~types : make_idesc_bf16(128, PR, false, false);
+      constexpr uint32_t idesc_o = FP8 ? make_idesc_bf16(128, PR, true, true) & ~types : make_idesc_bf16(128, 2 * PR, true, true);
+      auto issue_s = [&](int n) {
+        ok &= mbar_wait(&k_full[n % KS], (n / KS) & 1, abort_flag, args.status, 3);
+        ok &= mbar_wait(&s_empty[n & 1], ((n >> 1) & 1) ^ 1, abort_flag, args.status, 2);
+        tc_fence_after();
+        const uint64_t kd = k_desc + (n % KS) * (F::TILE >> 4);
+        const uint32_t d = tmem + (n & 1) * F::S_COLS;
+        __syncwarp();
+        if (elect_one()) {
+          if (FP8) {
+  #pragma unroll
+            for (int k = 0; k < 4; ++k) umma_f8_ss(d, kd + 2 * k, q_desc + 2 * k, idesc_s, k > 0);
+          } else {
+  #pragma unroll
+            for (int k = 0; k < 8; ++k)
+              umma_bf16_ss(d, kd + (k >> 2) * (PK * 128 >> 4) + (k & 3) * 2, q_desc + (k >> 2) * (PR * 128 >> 4) + (k & 3) * 2, idesc_s, k > 0);
+          }
+          umma_commit(&s_full[n & 1]);
+          umma_commit(&k_empty[n % KS]);
+        }
+        __syncwarp();
+      };
+      if (n_tiles > 0) issue_s(0);
+      for (int n = 0; n < n_tiles; ++n) {          // all tiles also after a time-out
+        if (n + 1 < n_tiles) issue_s(n + 1);
+        ok &= mbar_wait(FP8 ? &w_full[n % WS] : &v_full[n % VS], FP8 ? (n / WS) & 1 : (n / VS) & 1, abort_flag, args.status, 3);
+        ok &= mbar_wait(&p_full[n % PS], (n / PS) & 1, abort_flag, args.status, 2);
+        tc_fence_after();
+        const uint64_t vd = v_desc + (FP8 ? (n % WS) * (F::WIDE >> 4) : (n % VS) * (F::TILE >> 4)), pd = p_desc + (n % PS) * (F::P >> 4);
+        __syncwarp();
+        if (elect_one()) {
+  #pragma unroll
+          for (int k = 0; k < 8; ++k) umma_bf16_ss(tmem + F::O_AT, vd + k * (2048 >> 4), pd + k * (2048 >> 4), idesc_o, n > 0 || k > 0);
+          umma_commit(&pv_done[n % PS]);
+          umma_commit(FP8 ? &w_empty[n % WS] : &v_empty[n % VS]);
+        }
+        __syncwarp();
       }
-      __syncwarp();
+      ok = __all_sync(0xffffffffu, ok);            // (the warp goes on as one)
+    } else if (FP8 && warp >= 12) {
+      // ------------------------------ widening of values --------------------------------
+      const int row = tid & 127, sw = (row & 7) << 4;
+      bool ok = true;
+      for (int n = 0; n < n_tiles && ok; ++n) {
+        ok = mbar_wait_warp(&v_full[n % VS], (n / VS) & 1, abort_flag, args.status, 3);
+        if (!ok) break;
+        const uint8_t* from = sV + (n % VS) * F::TILE + row * 128;
+        uint4 x[8];
+  #pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = *reinterpret_cast<const uint4*>(from + ((i << 4) ^ sw));
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&v_empty[n % VS]);
+        if ((j0 + n) * PK + row >= most) {         // nobody reads it, and its codes may be NaN
+  #pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] = make_uint4(0, 0, 0, 0);
+        }
+        ok = mbar_wait_warp(&w_empty[n % WS], ((n / WS) & 1) ^ 1, abort_flag, args.status, 3);
+        if (!ok) break;
+        uint8_t* to = sW + (n % WS) * F::WIDE + row * 128;
+  #pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const uint2 y0 = widen4(i & 1 ? x[i >> 1].z : x[i >> 1].x), y1 = widen4(i & 1 ? x[i >> 1].w : x[i >> 1].y);
+          *reinterpret_cast<uint4*>(to + (i >> 3) * (PK * 128) + (((i & 7) << 4) ^ sw)) = make_uint4(y0.x, y0.y, y1.x, y1.y);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&w_full[n % WS]);
+      }
     }
-    ok = __all_sync(0xffffffffu, ok);            // (the warp goes on as one)
-  } else if (FP8 && warp >= 12) {
-    // ------------------------------ widening of values --------------------------------
-    const int row = tid & 127, sw = (row & 7) << 4;
-    bool ok = true;
-    for (int n = 0; n < n_tiles && ok; ++n) {
-      ok = mbar_wait_warp(&v_full[n % VS], (n / VS) & 1, abort_flag, args.status, 3);
-      if (!ok) break;
-      const uint8_t* from = sV + (n % VS) * F::TILE + row * 128;
-      uint4 x[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = *reinterpret_cast<const uint4*>(from + ((i << 4) ^ sw));
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&v_empty[n % VS]);
-      if ((j0 + n) * PK + row >= most) {         // nobody reads it, and its codes may be NaN
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = make_uint4(0, 0, 0, 0);
-      }
-      ok = mbar_wait_warp(&w_empty[n % WS], ((n / WS) & 1) ^ 1, abort_flag, args.status, 3);
-      if (!ok) break;
-      uint8_t* to = sW + (n % WS) * F::WIDE + row * 128;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const uint2 y0 = widen4(i & 1 ? x[i >> 1].z : x[i >> 1].x), y1 = widen4(i & 1 ? x[i >> 1].w : x[i >> 1].y);
-        *reinterpret_cast<uint4*>(to + (i >> 3) * (PK * 128) + (((i & 7) << 4) ^ sw)) = make_uint4(y0.x, y0.y, y1.x, y1.y);
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&w_full[n % WS]);
-    }
-  }
   } else {
     if (FP8) asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
     else asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");

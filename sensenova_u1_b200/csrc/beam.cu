@@ -8,6 +8,10 @@
 // groups as continuations are kept can hold one, and those are read again; what is not below the bound is ranked by counting.  Then the beams'
 // bookkeeping, so that a whole step is captured without a look by the host.
 //
+// 151936 fp32 logits a row, in a graph: 16 requests of 8 beams 17.5 us, where their bytes alone take 11.9 and the second kernel 5; 4 beams 9.9, of which
+// the second kernel's seven dependent phases are 7.  A first kernel that also chose the best
+// of its slice of a row had barriers in its pass: 30 us for the 16 requests.
+//
 // Candidates of different beams may be closer than fp32 tells apart: a group's sum is of fp32 terms, from 32 terms on in 64 bits (the largest
 // term of a row is 1 exactly, the errors of the others, 2^-22 of each at most, are of either sign: 1e-8 of the normaliser where they were measured),
 // and scores are compared in 64 bits.  Equal scores: the lower beam, then the lower token.

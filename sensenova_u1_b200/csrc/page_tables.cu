@@ -10,7 +10,8 @@
 // First kernel: a block has a few columns of all tables, which are independent of one another, so rows are moved in place; where an
 // entry changes, the use counts of the old and the new page do.  The block that is last does what needs all of them: which partial pages
 // stay, a scan over the use counts for free pages, lengths, and the list of copies.  Second kernel: the copies, in all layers at once.
-// What bounds it: latency (launch, three dependent look-ups, the scan), and for the copies memory.
+// What bounds it: latency (launch, three dependent look-ups, the scan), and for the copies memory.  In a graph, both kernels: 4 beams over 864 tokens,
+// 12 layers 8.5 us; 16 x 8 beams over 1570 e4m3 tokens in pages of 16 17 us, 4.5 of them the bytes; 32 beams over 32301 tokens 11.2.
 #include <string.h>
 
 #include <mutex>
@@ -210,7 +211,8 @@ struct CopyArgs {
 constexpr int COPY_THREADS = 256;
 
 // A block copies the rows of one sequence and layer, of ``sides`` sides (a side: keys or values of one head, whose rows are contiguous in a
-// page): as many as a full page of them is 32 KB.  (A block per side: 16 x 8 sequences, 12 layers, pages of 16 tokens 24 us, so 10.)
+// page): as many as a full page of them is 32 KB.  (16 x 8 sequences, 12 layers, pages of 16 tokens: the whole step 37 us with a
+// block per side, so 17.)
 __global__ void __launch_bounds__(COPY_THREADS) copy_kernel(const CopyArgs a) {
   pdl_wait();
   pdl_trigger();
