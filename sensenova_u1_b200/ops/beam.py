@@ -97,7 +97,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, keep: int | None = N
     if keep is None:
         keep = 2 * scores.shape[-1] if scores.dim() == 2 else 0
     requests, beams, vocab = _check(logits, scores, keep)
-    out = torch.empty((3, requests, keep), dtype=torch.int32, device=logits.device)
+    out = scores.new_empty((3, requests, keep), dtype=torch.int32)
     if requests:
         at, row = out.data_ptr(), 4 * requests * keep
         _launch(logits, scores, requests, beams, vocab, keep, (at, at + row, at + 2 * row), None)

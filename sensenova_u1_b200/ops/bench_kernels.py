@@ -8,7 +8,8 @@ Kernels: gemm_w13 / gemm_w2 / gemm_qkv (8B-MoT projection shapes at 16384 rows, 
 branch), gemm_wgrad (dy^T x), attn_fwd / attn_bwd (causal packed documents, 32 query / 8 kv heads,
 head 128), rmsnorm, qknorm_rope, swiglu, adamw, paged_write / paged_read (32 K tokens into and out of an e4m3 cache, 8 heads),
 paged_step (24 sequences of up to 4 K keys, one new token each, 32 / 8 heads), paged_drafts (8 new tokens each), paged_chunk
-(2 x 512 new tokens over 8 K keys), each over bf16 and e4m3 pages.  Prints one JSON line per kernel with the time,
+(2 x 512 new tokens over 8 K keys), paged_shared (16 sequences of one new token after 32 K common ones), each over bf16 and e4m3 pages; beam_select
+(16 requests of 8 beams, 151936 fp32 logits each) and page_tables (their step: forks, copies in 12 layers).  Prints one JSON line per kernel with the time,
 achieved TFLOP/s or GB/s and the fraction of the measured peaks when MEASURED_PEAKS.json is present.
 """
 from __future__ import annotations
@@ -244,6 +245,36 @@ def main():
             ms = _time(lambda: paged.paged_attention(q, cache, plan, D ** -0.5, out=o), args.iters, flush)
             pairs = sum(n * (k - n) + n * (n + 1) / 2 for n, k in zip(q_lens, kv_lens))
             report(f"{name}_{tag}", ms, flops=4.0 * D * Hq * pairs, nbytes=float(sum(kv_lens) * row + 4 * sum(q_lens) * Hq * D))
+        if want("paged_shared"):
+            P, n = 32000, 16
+            cache = paged.PagedCache.empty(P // page + n, page, Hk, fmt)
+            tables = [list(range(P // page)) + [P // page + i] for i in range(n)]
+            for first, count in ((0, P // page), (P // page, n)):
+                fill = paged.build_plan(cache, Hq, [count * page], [count * page], [range(first, first + count)])
+                kv = rnd(2, count * page, Hk, D) * 20
+                paged.paged_write(cache, kv[0], kv[1], fill)
+            q = rnd(n, Hq, D) * 20
+            o = torch.empty_like(q)
+            plan = paged.build_plan(cache, Hq, [1] * n, [P + page] * n, tables, shared=[(0, n, P)])
+            ms = _time(lambda: paged.paged_attention(q, cache, plan, D ** -0.5, out=o), args.iters, flush)
+            report("paged_shared_" + tag, ms, flops=4.0 * D * Hq * n * (P + page), nbytes=float((P + n * page) * row + 4 * n * Hq * D))
+    if want("beam_select"):
+        from .beam import beam_select
+        logits, scores = torch.randn(128, 151936, device=dev), torch.randn(16, 8, device=dev)
+        ms = _time(lambda: beam_select(logits, scores), args.iters, flush)
+        report("beam_select_16x8", ms, nbytes=4.0 * logits.numel())
+    if want("page_tables"):
+        from . import paged
+        from .page_tables import PageTables
+        n, page, layers, prompt = 128, 16, 12, 1500
+        caches = [paged.PagedCache.empty(16 * 94 + 2 * n * 8, page, 8, torch.float8_e4m3fn) for _ in range(layers)]
+        tables = PageTables(caches, n, prompt + 100)
+        order = torch.arange(n, dtype=torch.int32, device=dev)
+        tables.step(torch.where(order % 8 == 0, prompt, 0).int(), parents=torch.full_like(order, -1))
+        tables.step(13, parents=order // 8 * 8)
+        parents = order // 8 * 8 + torch.tensor([0, 0, 1, 3, 3, 3, 6, 7], dtype=torch.int32, device=dev).repeat(16)
+        ms = _time(lambda: tables.step(0, parents=parents), args.iters, flush)
+        report("page_tables_16x8", ms)
     check_status()
 
 
