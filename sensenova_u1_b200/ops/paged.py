@@ -65,7 +65,7 @@ PREFIX_LEAST = 2         # a part has at least this many key tiles
 # sequences of 512 12.6 / 10.9, of 1024 14.0 / 15.8, of 8192 22 / 83; 32 / 4 heads, 8 of 2048 12.1 / 12.1, of 4096 12.9 / 14.2.
 SHARE_TOKENS, SHARE_TILES = (2048, 2560), 1900
 # Us on an SM, by type (bf16, e4m3): to start and end a CTA, and one of its tiles.  Of shared tokens: 64 rows, and as chunks 256 (128) rows.  Of
-# tails, three of which share the SM, both for one third of it.
+# tails, two or three of which share the SM, both for the CTA's share of it.
 PREFIX_COST = ((6.0, 1.5), (6.0, 1.55))
 MANY_COST = ((9.0, 1.8), (9.0, 1.75))
 TAIL_COST = ((1.7, 1.5), (1.7, 1.05))
@@ -369,15 +369,6 @@ def _lay_out(q_lens, kv_lens, tables, page: int, pages: int, group: int, kv_head
     return arrays, counts
 
 
-def _tails(q_rows, skip, cap, heads: int):
-    """Rows of a CTA of the tails, how many CTAs there are for a head, and their tiles of 128 keys."""
-    rows, own = np.where(skip > 0, q_rows, 0), cap - skip
-    top = int(rows.max())
-    m = 8 if top <= 8 else 16 if top <= 16 else FEW_TILE
-    count = -(-rows // m)
-    return m, int(count.sum()), int((count * -(-own // CHUNK_TILE)).sum())
-
-
 def _together(runs, skip, q_rows, cap, q_start, group: int, heads: int, fp8: bool, first: int):
     """Work on tokens that runs of sequences share (prefix, and many for runs of more rows than that kernel's CTAs have), on the other tokens of these
     sequences (tail), and the joins of both, [row, head of the group, partial row, parts | partial row, parts, rows of a part, rows of a part of the
@@ -385,7 +376,16 @@ def _together(runs, skip, q_rows, cap, q_start, group: int, heads: int, fp8: boo
     runs = np.array([[q_start[a], q_start[a + n] - q_start[a], a, t, n] for a, n, t in runs])
     rows, tokens = runs[:, 1] * group, runs[:, 3]
     big = (rows > PREFIX_ROWS) & (group <= CHUNK_TILE)
-    m_tail, tail_ctas, tail_tiles = _tails(q_rows, skip, cap, heads)
+    # tails: sequences, rows of a CTA, items, their tiles and parts
+    seqs = np.concatenate([np.arange(a, a + n) for a, n in runs[:, [2, 4]]])
+    top = int(q_rows[seqs].max())
+    m_tail = 8 if top <= 8 else 16 if top <= 16 else FEW_TILE
+    slots = FEW_SLOTS[m_tail > 8]
+    tail_count = -(-q_rows[seqs] // m_tail)
+    tail_seq = np.repeat(seqs, tail_count)
+    tail_tiles = -(-(cap - skip)[tail_seq] // KEY_TILE)
+    tail_parts = _shares(tail_tiles, heads, slots, FEW_LEAST)
+    tail_us = heads / CHUNK_SLOTS * (tail_parts.sum() * TAIL_COST[fp8][0] + tail_tiles.sum() * KEY_TILE / CHUNK_TILE * TAIL_COST[fp8][1])
     whole = (CHUNK_TILE // group) * group if group <= CHUNK_TILE else 1
     joins = np.zeros((int(rows.sum()), 8), dtype=np.int64)
     of_run = np.repeat(np.arange(len(runs)), rows)
@@ -400,7 +400,7 @@ def _together(runs, skip, q_rows, cap, q_start, group: int, heads: int, fp8: boo
             count = np.where(which, -(-rows // m), 0)
             run = np.repeat(np.arange(len(runs)), count)
             kinds.append((name, which, m, count, run, tokens[run] // CHUNK_TILE, cost))
-        done, parts = _shared_parts([(k[5], *k[6]) for k in kinds], heads, tail_ctas * TAIL_COST[fp8][0] + tail_tiles * TAIL_COST[fp8][1], tail_ctas)
+        done, parts = _shared_parts([(k[5], *k[6]) for k in kinds], heads, heads * int(tail_parts.sum()), slots, tail_us)
         if best is None or done < best[0]:
             best = (done, kinds, parts)
     work = {}
@@ -419,37 +419,32 @@ def _together(runs, skip, q_rows, cap, q_start, group: int, heads: int, fp8: boo
         joins[here, 2] = at[item] + (place % m)[here]
         joins[here, 3] = parts[item]
         joins[here, 7] = m
-    # tails
-    seqs = np.concatenate([np.arange(r[2], r[2] + r[4]) for r in runs])
-    rows, m = q_rows[seqs], m_tail
-    count = -(-rows // m)
-    seq = np.repeat(seqs, count)
-    row0 = (np.arange(len(seq)) - np.repeat(np.cumsum(count) - count, count)) * m
-    tiles = -(-(cap - skip)[seq] // KEY_TILE)
-    parts = _shares(tiles, heads, FEW_SLOTS[m > 8], FEW_LEAST)
-    at = first + np.cumsum(parts * m) - parts * m
-    first += int((parts * m).sum())
-    i = np.repeat(np.arange(len(seq)), parts)
-    part = np.arange(len(i)) - np.repeat(np.cumsum(parts) - parts, parts)
-    tail = np.stack([seq[i], row0[i], part | parts[i] << 16, at[i] + part * m], 1)
-    order = np.argsort(-(tiles[i] / parts[i]), kind="stable")
+    row0 = (np.arange(len(tail_seq)) - np.repeat(np.cumsum(tail_count) - tail_count, tail_count)) * m_tail
+    at = first + np.cumsum(tail_parts * m_tail) - tail_parts * m_tail
+    first += int((tail_parts * m_tail).sum())
+    i = np.repeat(np.arange(len(tail_seq)), tail_parts)
+    part = np.arange(len(i)) - np.repeat(np.cumsum(tail_parts) - tail_parts, tail_parts)
+    tail = np.stack([tail_seq[i], row0[i], part | tail_parts[i] << 16, at[i] + part * m_tail], 1)
+    order = np.argsort(-(tail_tiles[i] / tail_parts[i]), kind="stable")
+    rows = q_rows[seqs]
     of_seq = np.repeat(np.arange(len(seqs)), rows)
     place = np.arange(len(of_seq)) - np.repeat(np.cumsum(rows) - rows, rows)
-    item = (np.cumsum(count) - count)[of_seq] + place // m
-    joins[:, 4] = at[item] + place % m
-    joins[:, 5] = parts[item]
-    joins[:, 6] = m
+    item = (np.cumsum(tail_count) - tail_count)[of_seq] + place // m_tail
+    joins[:, 4] = at[item] + place % m_tail
+    joins[:, 5] = tail_parts[item]
+    joins[:, 6] = m_tail
     twice = lambda x, y: np.stack([x, y], 1).reshape(-1).astype(np.int32)
     return (dict(skip=skip.astype(np.int32), runs=runs[:, :4].astype(np.int32), tail=tail[order].astype(np.int32), joins=joins.reshape(-1, 4).astype(np.int32),
                  run_start=twice(runs[:, 0], runs[:, 0] + runs[:, 1]), run_len=twice(tokens, tokens), run_seq=twice(runs[:, 2], runs[:, 2]), **work),
-            m, first)
+            m_tail, first)
 
 
-def _shared_parts(kinds, heads: int, tails: float, tail_ctas: int):
+def _shared_parts(kinds, heads: int, tails: int, slots: int, us: float):
     """Into how many parts the work on shared tokens is split, for every kind [tiles of its items, us to start a CTA, us of a tile], and when all is
-    done.  Its CTAs have an SM each.  Tails (``tails`` us of an SM in ``tail_ctas`` CTAs) take no time of their own if all of them fit the
-    SMs that are left; otherwise most of them run afterwards (fewer parts, to leave them more SMs, were slower: 48 conversations with 6000 common
-    tokens 43 us with 144 CTAs, 52 with 64)."""
+    done.  Its CTAs have an SM each.  ``tails`` CTAs, of which ``slots`` fill all SMs, take no time of their own if all of them fit the SMs that are left;
+    otherwise most of them run afterwards, ``us`` in all.  (bf16, 32 / 8 heads, by CTAs for shared tokens: 8 sequences of 4200 + 60 tokens 128: 15.8 us, 88: 11.9;
+    16 of 32000 + 1000, whose tails need all SMs, 104: 48.9, 144: 44.6.  Over 25 such calls, cut into 3 to 20 parts each, the choice took 1.2 % more than
+    the best.  Most of that is calls whose last few tails are alone: 64 of 8000 + 400 50.8, with 88 CTAs 45.5; models of their turns chose worse elsewhere.)"""
     sizes = [(int(t), int(c), start, tile) for tiles, start, tile in kinds for t, c in zip(*np.unique(tiles, return_counts=True))]
     longest = max((t for t, *_ in sizes), default=1)
     best, share = None, 0
@@ -461,11 +456,10 @@ def _shared_parts(kinds, heads: int, tails: float, tail_ctas: int):
         ctas = heads * sum(c * n for c, n, _ in split)
         if best is not None and (ctas > CHUNK_SLOTS or share < PREFIX_LEAST):
             break
-        busy = max(us for *_, us in split)
+        busy = max(t for *_, t in split)
         if ctas > CHUNK_SLOTS:
-            busy = max(busy, heads / CHUNK_SLOTS * sum(c * n * us for c, n, us in split) + busy / 2)
-        beside = tail_ctas * heads <= 3 * (CHUNK_SLOTS - ctas)
-        done = busy + (0.0 if beside else heads * tails / CHUNK_SLOTS + 3.0)
+            busy = max(busy, heads / CHUNK_SLOTS * sum(c * n * t for c, n, t in split) + busy / 2)
+        done = busy + (0.0 if tails <= slots // CHUNK_SLOTS * (CHUNK_SLOTS - ctas) else us + 4.0)
         if best is None or done < best[0]:
             best = (done, share)
     return best[0], [-(-tiles // best[1]) for tiles, _, _ in kinds]
