@@ -430,7 +430,7 @@ __global__ void __launch_bounds__(Prefix<FP8>::THREADS, 1)
       bool ok = true;
       for (int n = 1; n < n_tiles && ok; ++n) {
         const int next = page_of(n + 1), live = min(per, used - (j0 + n) * per);
-  #pragma unroll
+#pragma unroll
         for (int kv = 0; kv < 2; ++kv) {
           const int stages = kv ? VS : KS;
           ok = ok && mbar_wait_warp(kv ? &v_empty[n % stages] : &k_empty[n % stages], ((n / stages) & 1) ^ 1, abort_flag, args.status, 1);
@@ -456,10 +456,10 @@ __global__ void __launch_bounds__(Prefix<FP8>::THREADS, 1)
         __syncwarp();
         if (elect_one()) {
           if (FP8) {
-  #pragma unroll
+#pragma unroll
             for (int k = 0; k < 4; ++k) umma_f8_ss(d, kd + 2 * k, q_desc + 2 * k, idesc_s, k > 0);
           } else {
-  #pragma unroll
+#pragma unroll
             for (int k = 0; k < 8; ++k)
               umma_bf16_ss(d, kd + (k >> 2) * (PK * 128 >> 4) + (k & 3) * 2, q_desc + (k >> 2) * (PR * 128 >> 4) + (k & 3) * 2, idesc_s, k > 0);
           }
@@ -477,7 +477,7 @@ __global__ void __launch_bounds__(Prefix<FP8>::THREADS, 1)
         const uint64_t vd = v_desc + (FP8 ? (n % WS) * (F::WIDE >> 4) : (n % VS) * (F::TILE >> 4)), pd = p_desc + (n % PS) * (F::P >> 4);
         __syncwarp();
         if (elect_one()) {
-  #pragma unroll
+#pragma unroll
           for (int k = 0; k < 8; ++k) umma_bf16_ss(tmem + F::O_AT, vd + k * (2048 >> 4), pd + k * (2048 >> 4), idesc_o, n > 0 || k > 0);
           umma_commit(&pv_done[n % PS]);
           umma_commit(FP8 ? &w_empty[n % WS] : &v_empty[n % VS]);
@@ -494,18 +494,18 @@ __global__ void __launch_bounds__(Prefix<FP8>::THREADS, 1)
         if (!ok) break;
         const uint8_t* from = sV + (n % VS) * F::TILE + row * 128;
         uint4 x[8];
-  #pragma unroll
+#pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = *reinterpret_cast<const uint4*>(from + ((i << 4) ^ sw));
         __syncwarp();
         if (lane == 0) mbar_arrive(&v_empty[n % VS]);
         if ((j0 + n) * PK + row >= most) {         // nobody reads it, and its codes may be NaN
-  #pragma unroll
+#pragma unroll
           for (int i = 0; i < 8; ++i) x[i] = make_uint4(0, 0, 0, 0);
         }
         ok = mbar_wait_warp(&w_empty[n % WS], ((n / WS) & 1) ^ 1, abort_flag, args.status, 3);
         if (!ok) break;
         uint8_t* to = sW + (n % WS) * F::WIDE + row * 128;
-  #pragma unroll
+#pragma unroll
         for (int i = 0; i < 16; ++i) {
           const uint2 y0 = widen4(i & 1 ? x[i >> 1].z : x[i >> 1].x), y1 = widen4(i & 1 ? x[i >> 1].w : x[i >> 1].y);
           *reinterpret_cast<uint4*>(to + (i >> 3) * (PK * 128) + (((i & 7) << 4) ^ sw)) = make_uint4(y0.x, y0.y, y1.x, y1.y);
