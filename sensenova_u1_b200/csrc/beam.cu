@@ -8,9 +8,9 @@
 // groups as continuations are kept can hold one, and those are read again; what is not below the bound is ranked by counting.  Then the beams'
 // bookkeeping, so that a whole step is captured without a look by the host.
 //
-// 151936 fp32 logits a row, in a graph: 16 requests of 8 beams 17.5 us, where their bytes alone take 11.9 and the second kernel 5; 4 beams 9.9, of which
-// the second kernel's seven dependent phases are 7.  A first kernel that also chose the best
-// of its slice of a row had barriers in its pass: 30 us for the 16 requests.
+// 151936 fp32 logits a row, in a graph: 16 requests of 8 beams 17.9 us, where their bytes alone take 11.9 and the second kernel 5; 4 beams 10.1, of which
+// the second kernel's seven dependent phases are 7; a first step of 2 x 32 beams, 64 kept, 18.5.  A first kernel that also chose the best of its
+// slice of a row had barriers in its pass: 30 us for the 16 requests.
 //
 // Candidates of different beams may be closer than fp32 tells apart: a group's sum is of fp32 terms, from 32 terms on in 64 bits (the largest
 // term of a row is 1 exactly, the errors of the others, 2^-22 of each at most, are of either sign: 1e-8 of the normaliser where they were measured),
@@ -62,21 +62,21 @@ struct PassArgs {
   Group* out;          // [rows][groups]
 };
 
-// Token of value j of a group of 32 E; a lane has 16 bytes of every 512.
+// Token of a lane's value j of a group of 32 E; a lane has 16 bytes of every 512, eight lanes a quarter.
 template <typename T, int E>
-__device__ __forceinline__ int token_of(int group, int j) {
+__device__ __forceinline__ int token_of(int group, int lane, int j) {
   constexpr int VEC = 16 / sizeof(T);
-  return group * 32 * E + ((j / VEC) * 32 + (threadIdx.x & 31)) * VEC + j % VEC;
+  return group * 32 * E + ((j / VEC) * 32 + lane) * VEC + j % VEC;
 }
-// A group's values, by token and not by address: the sum of a row does not depend on where it lies, so that beams with the same logits have
+// A lane's values of a group, by token and not by address: the sum of a row does not depend on where it lies, so that beams with the same logits have
 // the same scores.  - inf behind the last.
 template <typename T, int E>
-__device__ __forceinline__ void load_group(const T* x, int V, int group, float (&v)[E]) {
+__device__ __forceinline__ void load_group(const T* x, int V, int group, int lane, float (&v)[E]) {
   constexpr int VEC = 16 / sizeof(T);
   const bool aligned = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
 #pragma unroll
   for (int j = 0; j < E; j += VEC) {
-    const int i = token_of<T, E>(group, j);
+    const int i = token_of<T, E>(group, lane, j);
     if (aligned && i + VEC <= V) {
       const uint4 u = *reinterpret_cast<const uint4*>(x + i);
       const uint32_t w[4] = {u.x, u.y, u.z, u.w};
@@ -92,14 +92,12 @@ __device__ __forceinline__ void load_group(const T* x, int V, int group, float (
   }
 }
 
+// A warp: a group's maxima and sum.
 template <typename T, int E>
-__global__ void __launch_bounds__(THREADS) pass_kernel(const PassArgs a) {
-  const int lane = threadIdx.x & 31, row = blockIdx.y, group = blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5);
-  pdl_wait();
-  pdl_trigger();
-  if (group >= a.groups) return;
+__device__ __forceinline__ void sum_group(const T* x, int V, int group, Group* out) {
+  const int lane = threadIdx.x & 31;
   float v[E];
-  load_group<T, E>(reinterpret_cast<const T*>(a.logits) + row * a.ld, a.V, group, v);
+  load_group<T, E>(x, V, group, lane, v);
   float m = v[0];                                        // (NaN is passed over)
 #pragma unroll
   for (int j = 1; j + 1 < E; j += 2) m = fmaxf(m, fmaxf(v[j], v[j + 1]));
@@ -117,9 +115,17 @@ __global__ void __launch_bounds__(THREADS) pass_kernel(const PassArgs a) {
   double total = sum;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-  Group* out = a.out + (long long)row * a.groups + group;
   if ((lane & 7) == 0) out->quarter[lane >> 3] = total == total ? quarter : __int_as_float(0x7fffffff);
   if (lane == 0) out->sum = total;
+}
+
+template <typename T, int E>
+__global__ void __launch_bounds__(THREADS) pass_kernel(const PassArgs a) {
+  const int row = blockIdx.y, group = blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5);
+  pdl_wait();
+  pdl_trigger();
+  if (group >= a.groups) return;
+  sum_group<T, E>(reinterpret_cast<const T*>(a.logits) + row * a.ld, a.V, group, a.out + (long long)row * a.groups + group);
 }
 
 constexpr int JOIN_THREADS = 1024;
@@ -152,7 +158,7 @@ struct JoinArgs {
   const void* logits;
   long long ld;
   int V, groups;
-  const Group* group;      // [requests * beams][groups]
+  Group* group;            // [requests * beams][groups]
   const float* scores;     // [requests][beams]
   float* out_scores;       // [requests][keep]
   int* out_beams;
@@ -261,14 +267,15 @@ struct JoinShared {
   float base[MAX_BEAMS], least[MAX_BEAMS];
   unsigned long long set[JOIN_THREADS], top[JOIN_THREADS / 4], nth, list_s[JOIN_LIST];      // (list_s: the candidates' scores once more, to be counted)
   Best list[JOIN_LIST];
-  int pass[JOIN_GROUPS];
+  int pass[JOIN_GROUPS], quarter[JOIN_GROUPS];
   short pick[JOIN_LIST];
   Best bound;
   int passing, count;
   Chosen out;
 };
 
-template <typename T, int E>
+// ALONE: the groups' maxima and sums too.
+template <typename T, int E, bool ALONE>
 __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const JoinArgs a) {
   extern __shared__ unsigned long long s_raw[];
   JoinShared& sh = *reinterpret_cast<JoinShared*>(s_raw);
@@ -281,8 +288,12 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const JoinArgs a) {
   pdl_wait();
   pdl_trigger();
   const int all = K * a.groups;
-  const Group* group = a.group + (long long)r * all;
+  Group* group = a.group + (long long)r * all;
   const T* logits = reinterpret_cast<const T*>(a.logits) + (long long)r * K * a.ld;
+  if (ALONE) {
+    for (int i = warp; i < all; i += JOIN_THREADS / 32) sum_group<T, E>(logits + i / a.groups * a.ld, a.V, i % a.groups, group + i);
+    __syncthreads();
+  }
   // normalisers: NaN where the row has no candidates
   for (int b = warp; b < K; b += JOIN_THREADS / 32) {
     const Group* p = group + (long long)b * a.groups;
@@ -412,16 +423,37 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const JoinArgs a) {
     __syncthreads();
     const int passing = sh.passing;
     const bool listed = passing <= JOIN_GROUPS;
-    for (int i = warp; i < (listed ? passing : all); i += JOIN_THREADS / 32) {
-      const int g = listed ? sh.pass[i] : i, b = g / a.groups;
-      if (!listed && score_of(top_of(group[g]), b) < bound.s) continue;
+    // More of them than warps: only their quarters that can, four to a warp (2 x 32 beams of 151936, first step 21.3 -> 18.7 us; for 8 groups 0.7 more).
+    int quarters = -1;
+    if (listed && passing > JOIN_THREADS / 32) {
+      if (tid == 0) sh.count = 0;
+      __syncthreads();
+      for (int i = tid; i < 4 * passing; i += JOIN_THREADS) {
+        const int g = sh.pass[i >> 2];
+        if (score_of(group[g].quarter[i & 3], g / a.groups) >= bound.s) {
+          const int at = atomicAdd(&sh.count, 1);
+          if (at < JOIN_GROUPS) sh.quarter[at] = 4 * g + (i & 3);
+        }
+      }
+      __syncthreads();
+      if (sh.count <= JOIN_GROUPS) quarters = sh.count;
+      __syncthreads();
+      if (tid == 0) sh.count = 0;
+      __syncthreads();
+    }
+    for (int i = warp; i < (quarters >= 0 ? (quarters + 3) / 4 : listed ? passing : all); i += JOIN_THREADS / 32) {     // eight lanes have a quarter
+      const int sub = lane >> 3;
+      const int at = quarters < 0 ? 4 * (listed ? sh.pass[i] : i) + sub : 4 * i + sub < quarters ? sh.quarter[4 * i + sub] : 0;
+      const int g = at >> 2, b = g / a.groups, from = (at & 3) * 8 + (lane & 7);
+      const bool on = quarters < 0 ? listed || score_of(group[g].quarter[at & 3], b) >= bound.s : 4 * i + sub < quarters;
+      if (!__any_sync(0xffffffffu, on)) continue;
       float v[E];
-      load_group<T, E>(logits + b * a.ld, a.V, g - b * a.groups, v);
-      const float least = sh.least[b];
+      load_group<T, E>(logits + b * a.ld, a.V, g - b * a.groups, from, v);
+      const float least = on ? sh.least[b] : INFINITY;
 #pragma unroll
       for (int j = 0; j < E; ++j)
         if (v[j] >= least) {
-          const unsigned long long key = (unsigned long long)order32(v[j]) << 32 | (uint32_t)~token_of<T, E>(g - b * a.groups, j);
+          const unsigned long long key = (unsigned long long)order32(v[j]) << 32 | (uint32_t)~token_of<T, E>(g - b * a.groups, from, j);
           if (!exactly || !before(bound, Best{score_of(v[j], b), key, (uint32_t)b})) {
             const int at = atomicAdd(&sh.count, 1);
             if (at < JOIN_LIST) sh.list[at] = Best{(unsigned long long)__float_as_uint(v[j]), key, (uint32_t)b};
@@ -489,18 +521,28 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const JoinArgs a) {
 static int group_of(int V) { return V >= 32768 ? 32 : 8; }
 static int groups_of(int E, int V) { return (V + 32 * E - 1) / (32 * E); }
 
-template <typename T, int E>
-static int launch(const PassArgs& a, const JoinArgs& j, int requests, cudaStream_t st) {
+// Groups of a request up to which its one CTA takes them all: one launch less.  Us in a graph (called from Python), with / without: 12 groups 7.6 / 8.2 (14.9 /
+// 17.1), 32 7.9 / 8.3 (14.9 / 16.8), 64 9.0 / 8.4 (14.9 / 16.8), 256 13.9 / 8.5.
+constexpr int ALONE_GROUPS = 32;
+static bool alone(int beams, int V) { return group_of(V) == 8 && (long long)beams * groups_of(8, V) <= ALONE_GROUPS; }
+
+template <typename T, int E, bool ALONE>
+static int launch_join(const JoinArgs& j, int requests, cudaStream_t st) {
   int dev = 0;
   SNU1_CUDA_CHECK(cudaGetDevice(&dev));
   static std::once_flag once[64];
   cudaError_t err = cudaSuccess;
-  std::call_once(once[dev & 63], [&]() { err = cudaFuncSetAttribute(join_kernel<T, E>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(JoinShared)); });
+  std::call_once(once[dev & 63], [&]() { err = cudaFuncSetAttribute(join_kernel<T, E, ALONE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(JoinShared)); });
   SNU1_CUDA_CHECK(err);
+  SNU1_CUDA_CHECK(launch_pdl(join_kernel<T, E, ALONE>, dim3(requests), dim3(JOIN_THREADS), sizeof(JoinShared), st, j));
+  return kHostOk;
+}
+
+template <typename T, int E>
+static int launch(const PassArgs& a, const JoinArgs& j, int requests, cudaStream_t st) {
   constexpr int WARPS = THREADS / 32;
   SNU1_CUDA_CHECK(launch_pdl(pass_kernel<T, E>, dim3((a.groups + WARPS - 1) / WARPS, a.rows), dim3(THREADS), 0, st, a));
-  SNU1_CUDA_CHECK(launch_pdl(join_kernel<T, E>, dim3(requests), dim3(JOIN_THREADS), sizeof(JoinShared), st, j));
-  return kHostOk;
+  return launch_join<T, E, false>(j, requests, st);
 }
 
 }  // namespace beam
@@ -509,6 +551,9 @@ static int launch(const PassArgs& a, const JoinArgs& j, int requests, cudaStream
 using namespace snu1;
 
 SNU1_API int snu1_beam_state_bytes() { return (int)sizeof(beam::State); }
+
+// Launches of a step.
+SNU1_API int snu1_beam_launches(int beams, int V) { return beam::alone(beams, V) ? 1 : 2; }
 
 // Bytes of scratch for ``rows`` rows of ``V`` logits.
 SNU1_API long long snu1_beam_scratch_bytes(int rows, int V) {
@@ -554,6 +599,8 @@ SNU1_API int snu1_beam_step(const void* logits, long long ld, int is_bf16, int V
     memcpy(&j.st, state, sizeof(State));
   }
   cudaStream_t st = (cudaStream_t)stream;
+  if (alone(beams, V))
+    return is_bf16 ? launch_join<__nv_bfloat16, 8, true>(j, requests, st) : launch_join<float, 8, true>(j, requests, st);
   if (is_bf16) return E == 32 ? launch<__nv_bfloat16, 32>(a, j, requests, st) : launch<__nv_bfloat16, 8>(a, j, requests, st);
   return E == 32 ? launch<float, 32>(a, j, requests, st) : launch<float, 8>(a, j, requests, st);
 }

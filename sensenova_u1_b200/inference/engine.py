@@ -440,7 +440,9 @@ class InferenceEngine:
         else:
             search.advance(logits)
         self.last_decode_graph = graph is not None
-        return search.result(best)
+        found = search.result(best)
+        _lib.check_status()
+        return found
 
     # ------------------------------------------------------------ text decoding
     def decode_greedy(self, layouts: List[DocLayout], last_hidden, max_new_tokens: int,

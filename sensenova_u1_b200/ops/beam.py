@@ -23,7 +23,7 @@ from ._lib import c_float, c_int, c_ll, c_void_p
 MAX_BEAMS, MAX_KEEP, MAX_EOS = 64, 128, 8
 MAX_VOCAB = 1 << 24
 _ENTRY: dict = {}
-_SCRATCH: dict = {}         # bytes of scratch by rows and tokens
+_SCRATCH: dict = {}         # bytes of scratch and launches by requests, beams and tokens
 
 
 class _State(ctypes.Structure):
@@ -40,8 +40,9 @@ def _entry():
             raise _lib.NativeLibraryError(f"{_lib.lib_path()} has searches of another layout: build it again (python -m sensenova_u1_b200.build)")
         P, L, I = c_void_p, c_ll, c_int
         lib.snu1_beam_scratch_bytes.argtypes, lib.snu1_beam_scratch_bytes.restype = (I, I), L
+        lib.snu1_beam_launches.argtypes = (I, I)
         lib.snu1_beam_step.argtypes = (P, L, I, I, P, I, I, I, P, P, P, P, P, P)
-        _ENTRY.update(scratch=lib.snu1_beam_scratch_bytes, step=lib.snu1_beam_step)
+        _ENTRY.update(scratch=lib.snu1_beam_scratch_bytes, launches=lib.snu1_beam_launches, step=lib.snu1_beam_step)
     return _ENTRY
 
 
@@ -73,13 +74,14 @@ def _launch(logits, scores, requests, beams, vocab, keep, out, state) -> None:
     if index != torch._C._cuda_getDevice():
         with torch.cuda.device(index):
             return _launch(logits, scores, requests, beams, vocab, keep, out, state)
-    entry, size = _entry(), (requests * beams, vocab)
+    entry, size = _entry(), (requests, beams, vocab)
     if size not in _SCRATCH:
         if len(_SCRATCH) > 64:
             _SCRATCH.clear()
-        _SCRATCH[size] = entry["scratch"](*size)
-    scratch = torch.empty(_SCRATCH[size], dtype=torch.uint8, device=logits.device)
-    _lib.LAUNCHES += 2
+        _SCRATCH[size] = entry["scratch"](requests * beams, vocab), entry["launches"](beams, vocab)
+    count, launches = _SCRATCH[size]
+    scratch = torch.empty(count, dtype=torch.uint8, device=logits.device)
+    _lib.LAUNCHES += launches
     rc = entry["step"](logits.data_ptr(), max(logits.stride(0), vocab), logits.dtype == torch.bfloat16, vocab, scores.data_ptr(), requests, beams,
                        keep, scratch.data_ptr(), *out, state, torch._C._cuda_getCurrentRawStream(index))
     if rc != 0:
