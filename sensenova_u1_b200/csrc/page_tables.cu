@@ -10,8 +10,9 @@
 // First kernel: a block has a few columns of all tables, which are independent of one another, so rows are moved in place; where an
 // entry changes, the use counts of the old and the new page do.  The block that is last does what needs all of them: which partial pages
 // stay, a scan over the use counts for free pages, lengths, and the list of copies.  Second kernel: the copies, in all layers at once.
-// What bounds it: latency (launch, three dependent look-ups, the scan), and for the copies memory.  In a graph, both kernels: 4 beams over 864 tokens,
-// 12 layers 8.5 us; 16 x 8 beams over 1570 e4m3 tokens in pages of 16 17 us, 4.5 of them the bytes; 32 beams over 32301 tokens 11.2.
+// What bounds it: latency (launch, dependent look-ups, the scan), and for the copies memory.  So table entries are on their way before lengths and parents are
+// known, and use counts before it is known which pages stay.  In a graph, both kernels: 4 beams over 864 tokens, 12 layers 7.6 us; 16 x 8
+// beams over 1570 e4m3 tokens in pages of 16 15.1 (17.0 with all look-ups one after another), 4.5 of them the bytes; 32 beams over 32301 tokens 10.8.
 #include <string.h>
 
 #include <mutex>
@@ -26,6 +27,8 @@ constexpr int THREADS = 512;
 constexpr int MAX_SEQS = 1024;
 constexpr int COLUMNS = 16;          // of a block
 constexpr int MAX_LAYERS = 256;
+constexpr int AHEAD = 4;             // table entries of a thread that are on their way before anything else is known
+constexpr int FREE_CHUNKS = 4;       // the use counts of as many times 2048 pages are looked at early
 
 // Device arrays of ops/page_tables.py's PageTables.
 struct Tables {
@@ -85,22 +88,35 @@ __global__ void __launch_bounds__(THREADS) step_kernel(const StepArgs a) {
   extern __shared__ int s_col[];                 // [seqs][COLUMNS] the columns before the step
   __shared__ int s_warp[THREADS / 32];
   __shared__ int s_vote;
-  __shared__ int s_parent[MAX_SEQS], s_kept[MAX_SEQS], s_from[MAX_SEQS], s_need[MAX_SEQS], s_src[MAX_SEQS];
+  __shared__ int s_parent[MAX_SEQS], s_kept[MAX_SEQS], s_from[MAX_SEQS], s_need[MAX_SEQS], s_src[MAX_SEQS], s_used[MAX_SEQS];
+  __shared__ uint32_t s_stays[FREE_CHUNKS * THREADS * 4 / 32];       // pages that stay with one sequence, by bit
   const Tables& t = a.t;
-  const int tid = threadIdx.x, S = t.seqs, W = t.width, page = t.page;
+  const int tid = threadIdx.x, S = t.seqs, W = t.width, page = t.page, page_log = __ffs(page) - 1;
+  const int c0 = blockIdx.x * COLUMNS, cn = min(COLUMNS, W - c0);
+  for (int i = tid; i < FREE_CHUNKS * THREADS * 4 / 32; i += THREADS) s_stays[i] = 0;
   pdl_wait();
   pdl_trigger();
+  int ahead[AHEAD];
+#pragma unroll
+  for (int k = 0; k < AHEAD; ++k) {
+    const int i = tid + k * THREADS, s = i / COLUMNS, c = i % COLUMNS;
+    ahead[k] = s < S && c < cn ? t.table[(long long)s * W + c0 + c] : -1;
+  }
   for (int s = tid; s < S; s += THREADS) {
+    const int len = max(0, t.lens[s]);
     int p;
     s_kept[s] = kept_of(a, s, &p);
     s_parent[s] = p;
-    const int len = max(0, t.lens[s]);
-    s_from[s] = min(W, (len + page - 1) / page);          // pages before
-    s_src[s] = -1;
+    s_from[s] = min(W, (len + page - 1) >> page_log);     // pages before
+    s_src[s] = s_used[s] = -1;
   }
   __syncthreads();
-  const int c0 = blockIdx.x * COLUMNS, cn = min(COLUMNS, W - c0);
-  for (int i = tid; i < S * COLUMNS; i += THREADS) {
+#pragma unroll
+  for (int k = 0; k < AHEAD; ++k) {
+    const int i = tid + k * THREADS;
+    if (i < S * COLUMNS) s_col[i] = c0 + i % COLUMNS < s_from[i / COLUMNS] ? ahead[k] : -1;
+  }
+  for (int i = tid + AHEAD * THREADS; i < S * COLUMNS; i += THREADS) {
     const int s = i / COLUMNS, c = i % COLUMNS;
     s_col[i] = c < cn && c0 + c < s_from[s] ? t.table[(long long)s * W + c0 + c] : -1;
   }
@@ -108,30 +124,44 @@ __global__ void __launch_bounds__(THREADS) step_kernel(const StepArgs a) {
   for (int i = tid; i < S * COLUMNS; i += THREADS) {
     const int s = i / COLUMNS, c = i % COLUMNS, j = c0 + c;
     if (c >= cn) continue;
-    const int kept = s_kept[s], full = kept / page, old = s_col[i];
-    const int src = j < (kept + page - 1) / page ? s_col[s_parent[s] * COLUMNS + c] : -1;       // (kept > 0: there is a parent)
+    const int kept = s_kept[s], full = kept >> page_log, part = kept & (page - 1), old = s_col[i];
+    const int src = j < full + (part != 0) ? s_col[s_parent[s] * COLUMNS + c] : -1;             // (kept > 0: there is a parent)
     const int now = j < full ? src : -1;
     if (j >= full || now != old) t.table[(long long)s * W + j] = now;
     if (now != old) {
       if (old >= 0 && old < t.pages) atomicSub(&t.refs[old], 1);
       if (now >= 0 && now < t.pages) atomicAdd(&t.refs[now], 1);
     }
-    if (j == full && kept % page != 0) {                                                          // the page that is not full
-      t.copies[s] = make_int4(src, -1, kept % page, 0);
+    if (j == full && part != 0) {                                                                // the page that is not full
+      t.copies[s] = make_int4(src, -1, part, 0);
       if (src >= 0 && src < t.pages) atomicMin(&t.claim[src], s);
     }
   }
   // the last block goes on
-  __threadfence();
-  __syncthreads();
-  if (tid == 0) {
-    const int before = atomicAdd(t.count, 1);
-    s_vote = before == (int)gridDim.x - 1;
+  if (gridDim.x > 1) {
+    __threadfence();
+    __syncthreads();
+    if (tid == 0) s_vote = atomicAdd(t.count, 1) == (int)gridDim.x - 1;
+    __syncthreads();
+    if (!s_vote) return;
+    __threadfence();
+    if (tid == 0) *t.count = 0;
+  } else {
+    __syncthreads();
   }
-  __syncthreads();
-  if (!s_vote) return;
-  __threadfence();
-  if (tid == 0) *t.count = 0;
+  int4 uses[FREE_CHUNKS];                        // as they are now: a page that stays is told by its bit
+#pragma unroll
+  for (int k = 0; k < FREE_CHUNKS; ++k) {
+    const int p = (k * THREADS + tid) * 4;
+    uses[k] = make_int4(1, 1, 1, 1);
+    if (p + 3 < t.pages) {
+      uses[k] = __ldcg(reinterpret_cast<const int4*>(t.refs + p));
+    } else if (p < t.pages) {
+      uses[k].x = __ldcg(t.refs + p);
+      if (p + 1 < t.pages) uses[k].y = __ldcg(t.refs + p + 1);
+      if (p + 2 < t.pages) uses[k].z = __ldcg(t.refs + p + 2);
+    }
+  }
   // partial pages: stay or are copied; how many pages every sequence needs
   int total = 0;
   for (int s0 = 0; s0 < S; s0 += THREADS) {
@@ -139,18 +169,20 @@ __global__ void __launch_bounds__(THREADS) step_kernel(const StepArgs a) {
     int need = 0, begin = 0, src = -1, part = 0;
     bool stays = false;
     if (s < S) {
-      const int kept = s_kept[s], full = kept / page;
+      const int kept = s_kept[s], full = kept >> page_log;
       const long long more = a.more != nullptr ? max(0, a.more[s]) : a.each;
       const long long want = min((long long)kept + more, (long long)W * page);
       if (want < kept + more) report_status(a.status, kBadShape, 12);
-      part = kept % page;
+      part = kept & (page - 1);
       if (part != 0) {
         src = __ldcg(&t.copies[s].x);
         stays = src >= 0 && src < t.pages && __ldcg(&t.refs[src]) == 0 && __ldcg(&t.claim[src]) == s;
       }
       begin = full + (stays ? 1 : 0);
-      need = max(0, (int)((want + page - 1) / page) - begin);
+      need = max(0, (int)((want + page - 1) >> page_log) - begin);
       s_src[s] = stays ? src : -1;
+      s_used[s] = src;
+      if (stays && src < FREE_CHUNKS * THREADS * 4) atomicOr(&s_stays[src >> 5], 1u << (src & 31));
       t.copies[s] = part != 0 && !stays ? make_int4(src, -1, part, 0) : make_int4(-1, -1, 0, 0);
       if (stays) t.table[(long long)s * W + full] = src;
       t.lens[s] = (int)want;
@@ -164,19 +196,13 @@ __global__ void __launch_bounds__(THREADS) step_kernel(const StepArgs a) {
   }
   __syncthreads();
   for (int s = tid; s < S; s += THREADS) {       // after everybody has looked at the counts
-    const int4 c = t.copies[s];
     if (s_src[s] >= 0) t.refs[s_src[s]] = 1;
-    const int used = s_src[s] >= 0 ? s_src[s] : c.x;
-    if (used >= 0 && used < t.pages) t.claim[used] = MAX_SEQS;
+    if (s_used[s] >= 0 && s_used[s] < t.pages) t.claim[s_used[s]] = MAX_SEQS;
   }
   __syncthreads();
   // the first ``total`` free pages, in order
   int found = 0;
-  for (int p0 = 0; p0 < t.pages && found < total; p0 += THREADS * 4) {
-    const int p = p0 + tid * 4;
-    int free[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) free[i] = p + i < t.pages && __ldcg(&t.refs[p + i]) == 0;
+  auto deal = [&](int p, const bool (&free)[4]) {
     const int2 sc = scan_block(free[0] + free[1] + free[2] + free[3], s_warp);
     int n = found + sc.x;
 #pragma unroll
@@ -190,14 +216,29 @@ __global__ void __launch_bounds__(THREADS) step_kernel(const StepArgs a) {
           if (s_need[mid] <= n) lo = mid;
           else hi = mid - 1;
         }
-        const int j = s_from[lo] + n - s_need[lo];
+        const int j = s_from[lo] + n - s_need[lo], kept = s_kept[lo];
         t.table[(long long)lo * W + j] = p + i;
         t.refs[p + i] = 1;
-        if (j == s_kept[lo] / page && s_kept[lo] % page != 0) t.copies[lo].y = p + i;
+        if (j == kept >> page_log && (kept & (page - 1)) != 0) t.copies[lo].y = p + i;
       }
       ++n;
     }
     found += sc.y;
+  };
+#pragma unroll
+  for (int k = 0; k < FREE_CHUNKS; ++k) {
+    const int p = (k * THREADS + tid) * 4;
+    if (k * THREADS * 4 >= t.pages || found >= total) break;
+    const uint32_t stays = s_stays[p >> 5] >> (p & 31);
+    const bool free[4] = {uses[k].x == 0 && !(stays & 1), uses[k].y == 0 && !(stays & 2), uses[k].z == 0 && !(stays & 4), uses[k].w == 0 && !(stays & 8)};
+    deal(p, free);
+  }
+  for (int p0 = FREE_CHUNKS * THREADS * 4; p0 < t.pages && found < total; p0 += THREADS * 4) {
+    const int p = p0 + tid * 4;
+    bool free[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) free[i] = p + i < t.pages && __ldcg(&t.refs[p + i]) == 0;
+    deal(p, free);
   }
   if (found < total && tid == 0) report_status(a.status, kBadPage, 12);       // fewer free pages than are needed: -1 stays in their places
 }
