@@ -16,8 +16,9 @@
 // times a power of two per row that keeps the largest product between 2^4 and 2^15 (W_TOP), and what that leaves of fp16's range is 28 bits below
 // the largest.  bf16: probabilities are two bf16 numbers, hi and lo as 64 columns each.
 //
-// What bounds it: with bf16 memory (8 heads, 80000 shared tokens: 8 rows 57 us, 64 rows 62, their bytes alone 50).  With e4m3 the softmax warps' issue,
-// 1.45 us a tile at 64 rows, and the widening at 8 (43 and 66 us, the bytes alone 26).  Short prefixes: the start and the end of a CTA, 8 us together, of
+// What bounds it: with bf16 memory (8 heads, 80000 shared tokens: 8 rows 57 us, 64 rows 62, their bytes alone 50).  With e4m3 8 rows
+// read 5 TB/s, and every eight rows more that a warp has take 0.15 us a tile, 1.45 at 64 rows (43 and 62 us, the bytes alone 26): their arithmetic, of which no part
+// (exponentials, conversions, products) is the bound by itself.  Short prefixes: the start and the end of a CTA, 8 us together, of
 // which the first page look-up, its copy, the first product and the last one follow each other (8 heads, 16000 tokens: 17 us and 25 to 27).
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
