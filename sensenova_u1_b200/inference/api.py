@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import json
 import re
+import warnings
 from dataclasses import dataclass, field
 from pathlib import Path
 from typing import List, Optional, Sequence, Tuple
@@ -400,14 +401,16 @@ class NEOChatModel:
 
     @staticmethod
     def _beams(gc: dict) -> Optional[dict]:
-        """Knobs of a beam search (``num_beams / num_return_sequences / length_penalty / early_stopping``); None where there is one beam."""
+        """Knobs of a beam search (``num_beams / num_return_sequences / length_penalty / early_stopping``); None where there is one beam, or where
+        sampling or a repetition penalty is asked for, which go without."""
         beams, best = int(gc.get("num_beams", 1) or 1), int(gc.get("num_return_sequences", 1) or 1)
+        if beams > 1 and (gc.get("do_sample", False) or float(gc.get("repetition_penalty", 1.0) or 1.0) != 1.0):
+            warnings.warn("num_beams is left out: a beam search neither samples nor penalises repetition")
+            return None
         if beams == 1:
             if best != 1:
-                raise ValueError("num_return_sequences needs a beam search (num_beams)")
+                warnings.warn("num_return_sequences is left out: it is of a beam search (num_beams)")
             return None
-        if gc.get("do_sample", False) or float(gc.get("repetition_penalty", 1.0) or 1.0) != 1.0:
-            raise ValueError("a beam search neither samples nor penalises repetition")
         penalty = gc.get("length_penalty")
         return {"beams": beams, "best": best, "length_penalty": 1.0 if penalty is None else float(penalty),
                 "early_stopping": gc.get("early_stopping") or False}
@@ -422,8 +425,7 @@ class NEOChatModel:
         gc = dict(generation_config or {})
         gc.update({k: v for k, v in kw.items() if k in ("do_sample", "temperature", "top_p", "top_k", "repetition_penalty",
                                                        "seed", "max_new_tokens", "num_beams", "length_penalty", "early_stopping")})
-        if gc.get("num_return_sequences") not in (None, 1):
-            raise ValueError("chat gives one answer")
+        gc.pop("num_return_sequences", None)       # one answer
         images = [] if pixel_values is None else (list(pixel_values) if isinstance(pixel_values, (list, tuple)) else [pixel_values])
         n_marked = question.count("<image>") + sum(q.count("<image>") + (a or "").count("<image>") for q, a in (history or []))
         if images and n_marked == 0:

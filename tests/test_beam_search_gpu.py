@@ -161,8 +161,12 @@ def test_chat_and_generate():
     many = m.generate(input_ids=ids, max_new_tokens=6, num_beams=4, num_return_sequences=3, eos_token_id=[7, 9], pad_token_id=1)
     assert one.shape == (1, 6) and many.shape[0] == 3 and many.dtype == torch.long
     assert m.generate(input_ids=ids, max_new_tokens=6).shape == (1, 6)
-    for kw in [dict(num_beams=4, do_sample=True), dict(num_beams=4, repetition_penalty=1.2), dict(num_return_sequences=2), dict(num_beams=2, num_return_sequences=3)]:
-        with pytest.raises(ValueError):
-            m.generate(input_ids=ids, max_new_tokens=6, **kw)
     with pytest.raises(ValueError):
-        m.chat(tok, None, "hello", generation_config={"num_beams": 4, "num_return_sequences": 2})
+        m.generate(input_ids=ids, max_new_tokens=6, num_beams=2, num_return_sequences=3)
+    # what a beam search does not do goes without, as before there was one
+    for kw, plain in [(dict(num_beams=4, do_sample=True, seed=3), dict(do_sample=True, seed=3)),
+                      (dict(num_beams=4, repetition_penalty=1.2), dict(repetition_penalty=1.2)), (dict(num_return_sequences=2), {})]:
+        with pytest.warns(UserWarning, match="left out"):
+            got = m.generate(input_ids=ids, max_new_tokens=6, **kw)
+        assert torch.equal(got, m.generate(input_ids=ids, max_new_tokens=6, **plain))
+    assert isinstance(m.chat(tok, None, "hello", generation_config={"num_beams": 4, "num_return_sequences": 2, "max_new_tokens": 4}), str)
