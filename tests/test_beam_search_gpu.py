@@ -170,3 +170,15 @@ def test_chat_and_generate():
             got = m.generate(input_ids=ids, max_new_tokens=6, **kw)
         assert torch.equal(got, m.generate(input_ids=ids, max_new_tokens=6, **plain))
     assert isinstance(m.chat(tok, None, "hello", generation_config={"num_beams": 4, "num_return_sequences": 2, "max_new_tokens": 4}), str)
+
+
+def test_layers_that_are_not_on_the_device():
+    from sensenova_u1_b200.inference.api import NEOChatModel
+    from sensenova_u1_b200.models.params import ParamStore
+    cfg, store, eng = model(5)
+    host = ParamStore(cfg, device="cpu", with_grads=False)
+    for name in host.p:
+        host.p[name].copy_(store.p[name])
+    docs = prompts(cfg, [70, 33])
+    kw = dict(beams=3, max_new_tokens=7, stop_ids=(5,), best=2)
+    assert NEOChatModel(cfg, host, vram_mode="low", device="cuda").engine.beam_search(docs, **kw) == eng.beam_search(docs, **kw)
