@@ -262,6 +262,10 @@ __device__ void follow(const JoinArgs& a, int r, Chosen& c) {
   if (tid == 0 && c.done == 2) s.done[r] = 1;
 }
 
+// Groups of a request up to which its one CTA takes them all: one launch less.  Us in a graph (called from Python), with / without: 12 groups 7.6 / 8.2 (14.9 /
+// 17.1), 32 7.9 / 8.3 (14.9 / 16.8), 64 9.0 / 8.4 (14.9 / 16.8), 256 13.9 / 8.5.
+constexpr int ALONE_GROUPS = 32;
+
 struct JoinShared {
   double lse[MAX_BEAMS];
   float base[MAX_BEAMS], least[MAX_BEAMS];
@@ -272,9 +276,10 @@ struct JoinShared {
   Best bound;
   int passing, count;
   Chosen out;
+  Group alone[ALONE_GROUPS];
 };
 
-// ALONE: the groups' maxima and sums too.
+// ALONE: the groups' maxima and sums too, in shared memory.
 template <typename T, int E, bool ALONE>
 __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const JoinArgs a) {
   extern __shared__ unsigned long long s_raw[];
@@ -288,7 +293,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const JoinArgs a) {
   pdl_wait();
   pdl_trigger();
   const int all = K * a.groups;
-  Group* group = a.group + (long long)r * all;
+  Group* group = ALONE ? sh.alone : a.group + (long long)r * all;
   const T* logits = reinterpret_cast<const T*>(a.logits) + (long long)r * K * a.ld;
   if (ALONE) {
     for (int i = warp; i < all; i += JOIN_THREADS / 32) sum_group<T, E>(logits + i / a.groups * a.ld, a.V, i % a.groups, group + i);
@@ -521,9 +526,6 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const JoinArgs a) {
 static int group_of(int V) { return V >= 32768 ? 32 : 8; }
 static int groups_of(int E, int V) { return (V + 32 * E - 1) / (32 * E); }
 
-// Groups of a request up to which its one CTA takes them all: one launch less.  Us in a graph (called from Python), with / without: 12 groups 7.6 / 8.2 (14.9 /
-// 17.1), 32 7.9 / 8.3 (14.9 / 16.8), 64 9.0 / 8.4 (14.9 / 16.8), 256 13.9 / 8.5.
-constexpr int ALONE_GROUPS = 32;
 static bool alone(int beams, int V) { return group_of(V) == 8 && (long long)beams * groups_of(8, V) <= ALONE_GROUPS; }
 
 template <typename T, int E, bool ALONE>
@@ -555,9 +557,9 @@ SNU1_API int snu1_beam_state_bytes() { return (int)sizeof(beam::State); }
 // Launches of a step.
 SNU1_API int snu1_beam_launches(int beams, int V) { return beam::alone(beams, V) ? 1 : 2; }
 
-// Bytes of scratch for ``rows`` rows of ``V`` logits.
-SNU1_API long long snu1_beam_scratch_bytes(int rows, int V) {
-  return (long long)rows * beam::groups_of(beam::group_of(V), V) * (long long)sizeof(beam::Group);
+// Bytes of scratch for ``rows`` rows of ``V`` logits, ``beams`` of each request; may be 0.
+SNU1_API long long snu1_beam_scratch_bytes(int rows, int beams, int V) {
+  return beam::alone(beams, V) ? 0 : (long long)rows * beam::groups_of(beam::group_of(V), V) * (long long)sizeof(beam::Group);
 }
 
 // logits [requests * beams][V] (fp32, or bf16 with is_bf16), rows ld elements apart; scores [requests][beams] fp32.  Without ``state`` the best

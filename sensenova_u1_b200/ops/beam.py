@@ -39,7 +39,7 @@ def _entry():
         if lib.snu1_beam_state_bytes() != ctypes.sizeof(_State):
             raise _lib.NativeLibraryError(f"{_lib.lib_path()} has searches of another layout: build it again (python -m sensenova_u1_b200.build)")
         P, L, I = c_void_p, c_ll, c_int
-        lib.snu1_beam_scratch_bytes.argtypes, lib.snu1_beam_scratch_bytes.restype = (I, I), L
+        lib.snu1_beam_scratch_bytes.argtypes, lib.snu1_beam_scratch_bytes.restype = (I, I, I), L
         lib.snu1_beam_launches.argtypes = (I, I)
         lib.snu1_beam_step.argtypes = (P, L, I, I, P, I, I, I, P, P, P, P, P, P)
         _ENTRY.update(scratch=lib.snu1_beam_scratch_bytes, launches=lib.snu1_beam_launches, step=lib.snu1_beam_step)
@@ -78,12 +78,12 @@ def _launch(logits, scores, requests, beams, vocab, keep, out, state) -> None:
     if size not in _SCRATCH:
         if len(_SCRATCH) > 64:
             _SCRATCH.clear()
-        _SCRATCH[size] = entry["scratch"](requests * beams, vocab), entry["launches"](beams, vocab)
+        _SCRATCH[size] = entry["scratch"](requests * beams, beams, vocab), entry["launches"](beams, vocab)
     count, launches = _SCRATCH[size]
-    scratch = torch.empty(count, dtype=torch.uint8, device=logits.device)
+    scratch = torch.empty(count, dtype=torch.uint8, device=logits.device) if count else None
     _lib.LAUNCHES += launches
     rc = entry["step"](logits.data_ptr(), max(logits.stride(0), vocab), logits.dtype == torch.bfloat16, vocab, scores.data_ptr(), requests, beams,
-                       keep, scratch.data_ptr(), *out, state, torch._C._cuda_getCurrentRawStream(index))
+                       keep, None if scratch is None else scratch.data_ptr(), *out, state, torch._C._cuda_getCurrentRawStream(index))
     if rc != 0:
         raise _lib.error("beam_step", rc)
 
