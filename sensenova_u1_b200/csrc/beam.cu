@@ -262,9 +262,9 @@ __device__ void follow(const JoinArgs& a, int r, Chosen& c) {
   if (tid == 0 && c.done == 2) s.done[r] = 1;
 }
 
-// Groups of a request up to which its one CTA takes them all: one launch less.  Us in a graph (called from Python), with / without: 12 groups 7.6 / 8.2 (14.9 /
-// 17.1), 32 7.9 / 8.3 (14.9 / 16.8), 64 9.0 / 8.4 (14.9 / 16.8), 256 13.9 / 8.5.
-constexpr int ALONE_GROUPS = 32;
+// Groups of a request up to which its one CTA takes them all: one launch less, no scratch.  Us in a graph (called from Python), with / without: 12 groups
+// 7.6 / 8.2 (12.9 / 17.1), 32 7.9 / 8.3 (12.9 / 16.8), 64 8.9 / 8.3 (12.8 / 17.2), 128 10.5 / 8.5 (12.9 / 17.5).
+constexpr int ALONE_GROUPS = 64;
 
 struct JoinShared {
   double lse[MAX_BEAMS];

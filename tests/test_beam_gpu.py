@@ -69,9 +69,9 @@ def test_best_of_all(r, k, v, keep, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("beams,v", [(4, 2048), (4, 2049), (33, 256), (16, 4096), (16, 4097), (64, 4096), (64, 4097), (3, 33000), (26, 40000)])
+@pytest.mark.parametrize("beams,v", [(4, 2048), (8, 2048), (8, 2049), (64, 256), (33, 257), (33, 256), (16, 4096), (16, 4097), (64, 4096), (64, 4097), (3, 33000), (26, 40000)])
 def test_lists_that_are_just_full(beams, v, dtype):
-    """One launch or two (32 groups of 256); groups and quarters of them that can hold one of the best: few, as many as a list holds, more."""
+    """One launch or two (64 groups of 256); groups and quarters of them that can hold one of the best: few, as many as a list holds, more."""
     zeros = torch.zeros(2, beams, device="cuda")
     for keep in (1, 40, 128):
         check(torch.ones(2 * beams, v, device="cuda", dtype=dtype), zeros, keep, ties=True)
