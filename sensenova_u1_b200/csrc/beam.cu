@@ -469,8 +469,8 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const JoinArgs a) {
     n = sh.count;
     const int here = min(n, JOIN_LIST);
     for (int i = tid; i < here; i += JOIN_THREADS) sh.list_s[i] = sh.list[i].s = score_of(__uint_as_float((uint32_t)sh.list[i].s), (int)sh.list[i].beam);
+    __syncthreads();                                       // (everybody has read the count)
     if (tid == 0) sh.count = sh.passing = 0;
-    __syncthreads();
     // of many only those are ranked that can be among the best
     int few = here;
     const bool picked = here > RANKED;
