@@ -243,7 +243,7 @@ __device__ void follow(const JoinArgs& a, int r, Chosen& c) {
   }
   __syncthreads();
   if (tid >= K) return;
-  const int n = c.done ? 0 : c.beams, pad = s.eos_count > 0 ? s.eos[0] : 0;
+  const int n = c.done ? 0 : c.beams, pad = s.eos_count > 0 && s.eos[0] < a.V ? s.eos[0] : 0;        // (its embedding is looked up)
   const bool on = tid < n;                                // (a row that does not go on stays where it is)
   const int pick = on ? c.pick[tid] : 0, token = on ? c.token[pick] : pad, from = on ? c.beam[pick] : tid;
   const long long h = ((long long)t * gridDim.x + r) * K + tid;

@@ -2,9 +2,9 @@
 import pytest
 import torch
 
-pytestmark = pytest.mark.gpu
+from test_beam_gpu import INF, LSE, Plain
 
-INF = float("inf")
+pytestmark = pytest.mark.gpu
 
 
 @pytest.mark.parametrize("r,k,v,keep", [(3, 4, 1000, 8), (2, 1, 5, 5), (150, 4, 5000, 8), (2, 8, 40000, 16), (1, 64, 700, 128)])
@@ -20,3 +20,16 @@ def test_over_and_over(r, k, v, keep):
     for _ in range(40):
         graph.replay()
         assert all(torch.equal(a, b) for o in out for a, b in zip(o, want))
+
+
+@pytest.mark.parametrize("eos", [(50,), (1 << 20, 3), (49,), ()])
+def test_next_tokens_are_of_the_vocabulary(eos):
+    """Rows that nobody goes on with, also where the ending token is none of the vocabulary (they look up an embedding all the same)."""
+    from sensenova_u1_b200.ops import beam
+    x = torch.randn(12, 50, device="cuda")
+    x[6:] = float("nan")                                    # a request that ends at once
+    x[:6, 3:] = -INF                                        # and one with fewer continuations than beams
+    search = beam.BeamSearch(2, 6, 3, eos)
+    for _ in range(3):
+        search.advance(x)
+        assert 0 <= int(search.tokens.min()) and int(search.tokens.max()) < 50
