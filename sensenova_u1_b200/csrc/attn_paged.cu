@@ -799,9 +799,10 @@ __global__ void __launch_bounds__(JOIN_THREADS) paged_share_join_kernel(const Pl
     float top = fmaxf(ml.x, mt);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const float old = mt == -INFINITY ? 0.f : fast_exp2(mt - top), f = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - top);
+    // (-1: the part has nothing.  One that is far below still counts: its NaN is the row's.)
+    const float old = mt == -INFINITY ? 0.f : fast_exp2(mt - top), f = ml.x == -INFINITY ? -1.f : fast_exp2(ml.x - top);
     mt = top;
-    float l = f == 0.f ? 0.f : f * ml.y;
+    float l = f < 0.f ? 0.f : f * ml.y;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
     lt = lt * old + l;
@@ -821,7 +822,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) paged_share_join_kernel(const Pl
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        if (k + i >= here || g[i] == 0.f) continue;              // (nothing is written where there is nothing)
+        if (k + i >= here || g[i] < 0.f) continue;               // (nothing is written where there is nothing)
         x.x += g[i] * y[i].x;
         x.y += g[i] * y[i].y;
         x.z += g[i] * y[i].z;

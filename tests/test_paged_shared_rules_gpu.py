@@ -1,0 +1,68 @@
+"""Attention of sequences that share their first tokens: values of any size, what is not finite far below, tables that change behind a plan."""
+import pytest
+import torch
+
+from test_paged_gpu import BF16, D, E4M3, quantised
+
+pytestmark = pytest.mark.gpu
+BOTH = pytest.mark.parametrize("dtype", [BF16, E4M3])
+
+
+@pytest.fixture(autouse=True)
+def always(monkeypatch):
+    """Shared however short it is."""
+    from sensenova_u1_b200.ops import paged
+    monkeypatch.setattr(paged, "SHARE_TOKENS", (0, 0))
+
+
+def as_chunks(monkeypatch, wanted):
+    """Runs of more than 64 rows go to the kernel for chunks, whatever is faster."""
+    from sensenova_u1_b200.ops import paged
+    if wanted:
+        monkeypatch.setattr(paged, "MANY_COST", ((0.0, 0.01), (0.0, 0.01)))
+
+
+def caches(x, dtype):
+    """A cache of pages ``x``, and what it holds in 64 bits."""
+    from sensenova_u1_b200.ops import paged
+    if dtype == BF16:
+        return paged.PagedCache(x.to(BF16)), x.to(BF16).double()
+    codes, scales = quantised(x.to(BF16))
+    return paged.PagedCache(codes, scales), codes.double() * scales.double()[..., None]
+
+
+def ramp(n, shared, page, score, g):
+    """Pages of ``n`` sequences: random values, and keys whose first number is ``score`` (nats) of their place; tables and lengths."""
+    whole = shared // page
+    x = torch.zeros(whole + n, 2, 1, page, D, device="cuda")
+    x[:, 1] = torch.randn(whole + n, 1, page, D, device="cuda", generator=g)
+    for p in range(whole):
+        for i in range(page):
+            x[p, 0, :, i, 0] = score(p * page + i)
+    x[whole:, 0, :, :, 0] = score(shared)
+    return x, [list(range(whole)) + [whole + i] for i in range(n)], [shared + 1 + i % page for i in range(n)]
+
+
+@BOTH
+@pytest.mark.parametrize("n", [4, 24])
+@pytest.mark.parametrize("side", ["shared", "own", "part"])
+def test_not_finite_far_below(side, n, dtype, monkeypatch):
+    """A value that is not finite makes the row NaN however small its probability is, with and without shared reads."""
+    from sensenova_u1_b200.ops import paged
+    as_chunks(monkeypatch, n > 16)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    shared = 4096
+    score = {"shared": lambda t: 0.0 if t < shared else 200.0, "own": lambda t: 200.0 if t < shared else 0.0, "part": lambda t: 200.0 if 3000 <= t < 3010 else 0.0}[side]
+    x, tables, kv = ramp(n, shared, 64, score, g)
+    at = (0, 5) if side != "own" else (tables[1][-1], 0)                     # a page and a place
+    cache, _ = caches(x, dtype)
+    if dtype == BF16:
+        cache.data[at[0], 1, 0, at[1], 3] = float("nan")
+    else:
+        cache.scales[at[0], 1, 0, at[1]] = float("nan")
+    q = torch.zeros(n, 4, D, device="cuda", dtype=BF16)
+    q[..., 0] = 1
+    for plan in (paged.build_plan(cache, 4, [1] * n, kv, tables, shared=[(0, n, shared)]), paged.build_plan(cache, 4, [1] * n, kv, tables)):
+        assert (plan._args.many_count > 0) == (plan._args.tail_count > 0 and n > 16)
+        bad = torch.isnan(paged.paged_attention(q, cache, plan, 1.0)).flatten(1).any(1)
+        assert bad.tolist() == [side != "own" or i == 1 for i in range(n)]
