@@ -7,7 +7,7 @@
 // The rows of a run are its new tokens times the query heads of the group, up to 64 per CTA.  They are the N of both products
 // (tcgen05.mma, accumulators in tensor memory), the 128 keys of a tile (the 128 values of a head) the M: eight rows cost an eighth of 64,
 // where rows as the M would fill 128 lanes whatever their number.  A thread of the softmax has one key and a column per row, so the
-// maximum over keys lies across lanes.  It begins at that of 32 keys and moves only when a probability would pass 2^60 (P_MOST), and a vote per
+// maximum over keys lies across lanes.  It begins at that of 32 keys and moves only when a probability would be too large (Range), and a vote per
 // tile is all that costs.  Sums stay with the threads until the end.
 //
 // e4m3 codes go to the first product as they are; a query is two e4m3 numbers, each row times a power of two: hi has 4 of the 8 bits
@@ -107,8 +107,13 @@ __device__ __forceinline__ float log2_of(float x) {
   asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// A probability may be up to 2^60 before the maximum moves: relative to any key of its row it is an fp32 number, as is its sum.
-constexpr float P_MOST = 60.f;
+// The maximum that probabilities are relative to moves when one would pass 2^MOST.  bf16: it begins, and is moved, LEAD above the largest score that has
+// been seen, so scores may rise by LEAD + MOST before it moves, and products with values of up to 2^100 still fit fp32 sums (p is at most 2^8, as in
+// the kernel for chunks).  What is 2^-100 of the largest probability or less is lost.  e4m3: values' scales have a power of two of their
+// own (W_TOP), which bounds the products.
+template <bool FP8> struct Range {
+  static constexpr float MOST = FP8 ? 60.f : 8.f, LEAD = FP8 ? 0.f : 24.f;
+};
 // e4m3: exponent of the factor of probabilities times values' scales, whose largest is 2^mv: 2^W_TOP then, as fp16 numbers, and up to 2^15 before it
 // moves.  What is 2^-28 of the largest or less is lost.  (2^7 lets it move in one CTA in five of random scores, 5 us each time.)
 constexpr float W_TOP = 4.f;
@@ -180,7 +185,7 @@ __device__ __noinline__ void move_maxima(PrefixShared& sh, uint32_t S, uint32_t 
 #pragma unroll
     for (int k = 0; k < 4; ++k) top = fmaxf(top, sh.red[side * 4 + k][lane]);
     const bool fresh = m == -INFINITY;
-    const float now = fmaxf(m, top);
+    const float now = fmaxf(m, top + Range<FP8>::LEAD);
     sh.by[col] = fresh ? 0.f : now - m;
     sh.f[col] = fresh ? 0.f : fast_exp2(m - now);
     sh.row[col].m = now;
@@ -567,7 +572,7 @@ __global__ void __launch_bounds__(Prefix<FP8>::THREADS, 1)
           const float ks = sc.x * args.scale_log2;
           const uint32_t S = tmem + col + lanes;
           const float m = row_tops<FP8>(S, sh.row + col, nullptr, 0, ks, false, 0.f);
-          if (lane < 8) sh.row[col + lane].m = m;
+          if (lane < 8) sh.row[col + lane].m = m + Range<FP8>::LEAD;
           if (FP8) {
             __syncwarp();
             const float mv = row_tops<FP8>(S, sh.row + col, nullptr, 0, ks, true, log2_of(sc.y));
@@ -664,7 +669,7 @@ __global__ void __launch_bounds__(Prefix<FP8>::THREADS, 1)
               if (!FP8) *reinterpret_cast<uint4*>(P + PK * 128 + to) = make_uint4(v[0], v[1], v[2], v[3]);
             }
           }
-          if (__builtin_expect(named_bar_any(2 + side, 128, !again && (mx > P_MOST || mw > 32768.f)), 0)) {
+          if (__builtin_expect(named_bar_any(2 + side, 128, !again && (mx > Range<FP8>::MOST || mw > 32768.f)), 0)) {
             if (n > 0) {
               ok &= mbar_wait(&pv_done[(n - 1) % PS], ((n - 1) / PS) & 1, abort_flag, args.status, 6);
               __syncwarp();
@@ -726,6 +731,23 @@ __global__ void __launch_bounds__(Prefix<FP8>::THREADS, 1)
       ok = __all_sync(0xffffffffu, ok);
       tc_fence_after();
       named_bar_sync(2 + side, 128);
+      if ((w & 3) == 0 && lane < 8 * active) {
+        // The maximum that is left goes up by the whole part of the sum's logarithm: the part is then the mean of values, times less than two, and as
+        // large as they are at most.
+        const int col = c0 + lane;
+        const float m = sh.row[col].m;
+        float sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sum += sh.sum[side * 4 + k][lane];
+        const float up = sum >= 2.f && sum < INFINITY ? m + (float)((int)(__float_as_uint(sum) >> 23) - 127) : m;
+        const float f = up == m ? 1.f : exp2f(m - up);
+        sum *= f;
+        if (!FP8 && sh.lim[col] > *reinterpret_cast<volatile int*>(&s_poison)) sum = __int_as_float(0x7fffffff);
+        sh.f[col] = f;
+        sh.row[col].m = sum != sum && m == -INFINITY ? 0.f : up;       // all NaN: not to be taken for no keys at all
+        sh.sum[side * 4][lane] = sum;
+      }
+      named_bar_sync(2 + side, 128);
 #pragma unroll 1
       for (int i = 0; i < active; ++i) {
         uint32_t h[8], lo[8];
@@ -735,23 +757,17 @@ __global__ void __launch_bounds__(Prefix<FP8>::THREADS, 1)
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const int col = c0 + 8 * i + e, r = (2 * i + side) * 8 + e;
+          const float o = FP8 ? __uint_as_float(h[e]) : __uint_as_float(h[e]) + __uint_as_float(lo[e]);
           if (r < rows && ok)
-            args.part[((long long)(item.w + r) * args.heads + head) * HEAD + in_tile] =
-                FP8 ? __uint_as_float(h[e]) * __int_as_float((127 - sh.ec[col]) << 23) : __uint_as_float(h[e]) + __uint_as_float(lo[e]);
+            args.part[((long long)(item.w + r) * args.heads + head) * HEAD + in_tile] = FP8 ? o * sh.f[col] * __int_as_float((127 - sh.ec[col]) << 23) : o * sh.f[col];
         }
       }
     }
     if ((w & 3) == 0 && lane < 8 * active) {
       const int col = c0 + lane, r = (2 * (lane >> 3) + side) * 8 + (lane & 7);
-      float m = -INFINITY, l = 0.f;
-      if (n_tiles > 0) {
-        m = sh.row[col].m;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) l += sh.sum[side * 4 + k][lane];
-        if (!FP8 && sh.lim[col] > *reinterpret_cast<volatile int*>(&s_poison)) l = __int_as_float(0x7fffffff);
-        if (l != l && m == -INFINITY) m = 0.f;   // all NaN: not to be taken for no keys at all
-      }
-      if (r < rows) args.part_ml[(long long)(item.w + r) * args.heads + head] = make_float2(m, l);
+      if (r < rows)
+        args.part_ml[(long long)(item.w + r) * args.heads + head] =
+            n_tiles > 0 ? make_float2(sh.row[col].m, sh.sum[side * 4][lane]) : make_float2(-INFINITY, 0.f);
     }
   }
   tc_fence_before();

@@ -2,7 +2,8 @@
 import pytest
 import torch
 
-from test_paged_gpu import BF16, D, E4M3, quantised
+from test_paged_gpu import BF16, D, E4M3, causal, exact, near, quantised
+from test_paged_shared_gpu import queries, rows_of, setup, wider
 
 pytestmark = pytest.mark.gpu
 BOTH = pytest.mark.parametrize("dtype", [BF16, E4M3])
@@ -66,3 +67,32 @@ def test_not_finite_far_below(side, n, dtype, monkeypatch):
         assert (plan._args.many_count > 0) == (plan._args.tail_count > 0 and n > 16)
         bad = torch.isnan(paged.paged_attention(q, cache, plan, 1.0)).flatten(1).any(1)
         assert bad.tolist() == [side != "own" or i == 1 for i in range(n)]
+
+
+@BOTH
+@pytest.mark.parametrize("n", [4, 24, 25])
+@pytest.mark.parametrize("rise", [5, 10, 20, 31, 33, 50, 100])
+def test_large_values(rise, n, dtype, monkeypatch):
+    """Values of up to 2^100 (e4m3: 2^110 of scale), where the largest score is ``rise`` log2 units above those that the maxima begin at."""
+    from sensenova_u1_b200.ops import _lib, paged
+    as_chunks(monkeypatch, n > 24)
+    g = torch.Generator(device="cuda").manual_seed(rise)
+    x, tables, kv = ramp(n, 2048, 64, lambda t: 0.0 if t != 700 and t < 2048 else rise * 0.6931, g)
+    x[:, 1] *= 2.0 ** 100
+    cache, held = caches(x, dtype)
+    if dtype == E4M3:                                       # the largest code is 448
+        up = 2.0 ** 110 / cache.scales[:, 1].amax()
+        cache.scales[:, 1] *= up
+        held[:, 1] *= up.double()
+    q = torch.zeros(n, 4, D, device="cuda", dtype=BF16)
+    q[..., 0] = 1
+    plan = paged.build_plan(cache, 4, [1] * n, kv, tables, shared=[(0, n, 2048)])
+    assert plan._args.tail_count > 0 and (plan._args.many_count > 0) == (n > 24)
+    out = paged.paged_attention(q, cache, plan, 1.0)
+    _lib.check_status()
+    assert torch.isfinite(out).all()
+    q = q / D ** -0.5                                       # (exact has a scale of its own)
+    rows = rows_of(held, tables, kv)
+    ref, room = exact(q, [1] * n, rows, causal([1] * n, kv), dtype)
+    room = wider(room, q, [1] * n, rows, causal([1] * n, kv), plan)
+    assert near(out * 2.0 ** -60, ref * 2.0 ** -60, room * 2.0 ** -60)
