@@ -273,7 +273,7 @@ __global__ void __launch_bounds__(Few<FP8, NR, WR>::THREADS, Few<FP8, NR, WR>::C
   const int4 item = (TAIL ? p.tail : p.few)[blockIdx.x];
   const int b = item.x, row0 = item.y, part = item.z & 0xffff, parts = item.z >> 16;
   const int head = blockIdx.y, G = p.group;
-  const int skip = TAIL ? p.skip[b] / KT : 0;                    // tiles
+  const int shared = TAIL ? p.skip[b] : 0;
   const int q0 = p.q_start[b], q_len = p.q_start[b + 1] - q0;
   // Chunks in front (attn_paged_sm100.cu) have waited for all work before them when this kernel may start, and nothing that
   // they write is read here: it only has to end after them.
@@ -282,6 +282,7 @@ __global__ void __launch_bounds__(Few<FP8, NR, WR>::THREADS, Few<FP8, NR, WR>::C
 
   if (threadIdx.x == 0) report_grown(p, b, a.status);
   const int kv_len = seq_len(p, b);
+  const int skip = TAIL ? still_shared(p, b, kv_len, shared) / KT : 0;         // tiles
   const int rows = min(M, q_len * G - row0);
   // the furthest key that a row of this tile may read, and the nearest limit
   int max_lim = 0, min_lim = kv_len;

@@ -243,6 +243,8 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
   int* lim_min = lim_max + 2;
   int* poison = lim_min + 2;                               // first key of a tile not read whole whose value was not finite
 
+  __shared__ int s_lim[TILES * 128];                        // limits of tokens, where they do not grow from one to the next
+
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
@@ -318,7 +320,8 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     if (threadIdx.x < TILES * T) {
       const int t = threadIdx.x / T, token = token0 + threadIdx.x;
       if (token < q_len) {
-        const int l = row_limit(p, q0, q_len, kv_len, token);
+        const int l = p.own_q_start != nullptr ? run_limit(p, q0 + token, kv_len) : row_limit(p, q0, q_len, kv_len, token);
+        s_lim[threadIdx.x] = l;
         atomicMax(&lim_max[t], l);
         atomicMin(&lim_min[t], l);
       }
@@ -638,7 +641,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       const int row = base + (lane >> 2) + 8 * r, token = token0 + t * T + row / G;
-      lim[r] = row < T * G && token < q_len ? row_limit(p, q0, q_len, kv_len, token) : -1;
+      lim[r] = row >= T * G || token >= q_len ? -1 : p.behind == nullptr && p.own_q_start == nullptr ? row_limit(p, q0, q_len, kv_len, token) : s_lim[token - token0];
     }
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};      // running maximum, log2 units
     float sc[2] = {args.scale_log2, args.scale_log2};

@@ -336,7 +336,8 @@ __global__ void __launch_bounds__(Prefix<FP8>::THREADS, 1)
       const int r = lane + 32 * k, col = (r >> 3 & 1) * 32 + (r >> 4) * 8 + (r & 7);
       int lim = 0;
       if (r < rows) {
-        lim = min(shared, row_limit(p, q_first[k], q_len[k], seq_len(p, seq[k]), t0 + (row0 + r) / G - q_first[k]));
+        const int len = seq_len(p, seq[k]);
+        lim = min(still_shared(p, seq[k], len, shared), row_limit(p, q_first[k], q_len[k], len, t0 + (row0 + r) / G - q_first[k]));
         least = min(least, lim);
       }
       most = max(most, lim);

@@ -31,7 +31,7 @@ struct alignas(64) Cache {
   int pages, heads, page, fp8;
 };
 
-constexpr int PLAN_LAYOUT = 0x70670004;
+constexpr int PLAN_LAYOUT = 0x70670005;
 
 // Device arrays and counts of a plan (ops/paged.py builds it).
 struct Plan {
@@ -50,6 +50,7 @@ struct Plan {
   const int4* one;         // [one_count] the same for e4m3 chunks of one row tile per CTA
   const int4* merge;       // [merge_count] up to four rows to join: sequence, first row, parts | rows << 12 | rows of a part << 16, first partial row
   const int* skip;         // [seqs] tokens of a sequence that its run shares (a multiple of 128); the tail kernel leaves them out
+  const int* lead;         // [seqs] sequence whose table its run is read through, where the tables may change; null: they may not, and begin alike
   const int4* runs;        // runs of sequences with the same first tokens: first row, rows, sequence whose table is read, shared tokens
   const int4* prefix;      // [prefix_count] work on shared tokens: run, first of up to PREFIX_ROWS rows (x heads of a group), part | parts << 16, partial row
   const int4* tail;        // [tail_count] work on the other tokens of such sequences, as ``few``
@@ -85,6 +86,28 @@ __device__ __forceinline__ void report_grown(const Plan& p, int b, int* status) 
   if (p.kv_len[b] > p.cap[b]) report_status(status, kBadShape, 10);
 }
 
+// How many of a run's ``tokens`` shared ones (a multiple of 128) sequence b still has in the run's pages.  Tables that change behind a plan: the run's
+// first sequence may have gone, others may have been cut and have grown again.  Whoever holds a page holds all pages before it as they were, so
+// tables are alike up to one place; nearly always that is the last one, which two look-ups tell.
+static __noinline__ __device__ int still_shared_cut(const int* x, const int* y, int page, int len, int tokens) {
+  if (len <= 0) return 0;
+  int n = (min(tokens, len) - 1) / page, from = 0;
+  if (x[n] == y[n]) return tokens;               // all that it has
+  while (from < n) {                             // the first place where they differ
+    const int mid = (from + n) / 2;
+    if (x[mid] == y[mid]) from = mid + 1;
+    else n = mid;
+  }
+  return from * page / 128 * 128;
+}
+__device__ __forceinline__ int still_shared(const Plan& p, int b, int len, int tokens) {
+  if (p.lead == nullptr || tokens == 0) return tokens;
+  const int *x = p.table + (long long)b * p.width, *y = p.table + (long long)p.lead[b] * p.width;
+  const int last = tokens / p.page - 1;
+  const bool same = x[last] == y[last];          // (on their way before the length is known)
+  return same && len >= tokens ? tokens : still_shared_cut(x, y, p.page, len, tokens);
+}
+
 // Pages of a sequence.
 __device__ __forceinline__ const int* table_of(const Plan& p, int b) {
   return p.table + (long long)(p.own_q_start != nullptr ? p.run_seq[b] : b) * p.width;
@@ -92,13 +115,15 @@ __device__ __forceinline__ const int* table_of(const Plan& p, int b) {
 
 // Keys that row ``token`` of a sequence may read.
 __device__ __forceinline__ int row_limit(const Plan& p, int q0, int q_len, int kv_len, int token) {
-  if (p.own_q_start != nullptr) {          // of a run's ``kv_len`` shared tokens
-    const int row = q0 + token, b = p.row_seq[row], len = max(0, min(p.own_kv_len[b], p.own_cap[b]));
-    const int behind = p.behind != nullptr ? p.behind[row] : p.own_q_start[b + 1] - 1 - row;
-    return max(0, min(min(kv_len, len), len - behind));
-  }
   const int behind = p.behind != nullptr ? p.behind[q0 + token] : q_len - 1 - token;
   return max(0, min(kv_len, kv_len - behind));
+}
+
+// Of a run's ``tokens`` shared ones, those that row ``row`` may read (a plan with ``own_*``).
+__device__ __forceinline__ int run_limit(const Plan& p, int row, int tokens) {
+  const int b = p.row_seq[row], len = max(0, min(p.own_kv_len[b], p.own_cap[b]));
+  const int behind = p.behind != nullptr ? p.behind[row] : p.own_q_start[b + 1] - 1 - row;
+  return max(0, min(min(still_shared(p, b, len, tokens), len), len - behind));
 }
 
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {

@@ -138,13 +138,13 @@ class PagedCache:
         return self._data.device
 
 
-PLAN_LAYOUT = 0x70670004     # last word of a plan: the library refuses one whose fields lie elsewhere
+PLAN_LAYOUT = 0x70670005     # last word of a plan: the library refuses one whose fields lie elsewhere
 
 
 class _Args(ctypes.Structure):
     """``Plan`` of csrc/paged.cuh."""
     _fields_ = ([(n, c_void_p) for n in ("q_start", "kv_len", "cap", "table", "behind", "row_seq", "k_start", "read_pages", "unpack",
-                                         "unpack_first", "few", "chunk", "one", "merge", "skip", "runs", "prefix", "tail", "joins", "run_start", "run_len", "run_seq",
+                                         "unpack_first", "few", "chunk", "one", "merge", "skip", "lead", "runs", "prefix", "tail", "joins", "run_start", "run_len", "run_seq",
                                          "many", "own_q_start", "own_kv_len", "own_cap")]
                 + [(n, c_int) for n in ("seqs", "rows", "width", "page", "group", "read_count", "few_count", "few_rows", "few_parts", "few_cluster",
                                         "chunk_count", "one_count", "merge_count", "partial_rows", "prefix_count", "tail_count", "tail_rows", "join_count", "many_count",
@@ -348,10 +348,14 @@ def _lay_out(q_lens, kv_lens, tables, page: int, pages: int, group: int, kv_head
     one, partial = chunks_of(single, tile_rows, partial)
     chunk, partial = chunks_of(chunked & ~single, 2 * tile_rows, partial)
     merge = np.concatenate(merge) if merge else np.zeros((0, 4), np.int32)
-    together = dict(skip=None, runs=None, prefix=None, tail=None, joins=None, run_start=None, run_len=None, run_seq=None, many=None)
+    together = dict(skip=None, lead=None, runs=None, prefix=None, tail=None, joins=None, run_start=None, run_len=None, run_seq=None, many=None)
     tail_rows = 0
     if runs:
         together, tail_rows, partial = _together(runs, skip, q_rows, cap, start(q), group, kv_heads, fp8, partial)
+        if on_device:
+            together["lead"] = np.arange(n, dtype=np.int32)
+            for first, count, _ in runs:
+                together["lead"][first:first + count] = first
     unpack = unpack_first = None
     if fp8 and len(chunk):
         wide = np.where(chunked & ~single, -(-cap // CHUNK_TILE), 0)    # 128-token pages

@@ -96,3 +96,61 @@ def test_large_values(rise, n, dtype, monkeypatch):
     ref, room = exact(q, [1] * n, rows, causal([1] * n, kv), dtype)
     room = wider(room, q, [1] * n, rows, causal([1] * n, kv), plan)
     assert near(out * 2.0 ** -60, ref * 2.0 ** -60, room * 2.0 ** -60)
+
+
+@BOTH
+@pytest.mark.parametrize("n", [5, 30, 31])
+def test_requests_that_come_and_go_behind_a_plan(n, dtype, monkeypatch):
+    """The first sequence of a run ends and another request takes its place; others are cut inside the shared tokens and grow again.  Every one reads
+    its own tokens, as the tables are."""
+    from sensenova_u1_b200.ops import _lib, page_tables, paged
+    as_chunks(monkeypatch, n > 30)
+    cache, tables, kv, _, shared = setup([(640, [700 + i for i in range(n)])], 64, 2, dtype, room=400, stretch=False)
+    t = page_tables.PageTables(cache, n, 1000)
+    t.load(kv, tables)
+    plan = paged.build_plan(cache, 8, [1] * n, [1000] * n, t, shared=shared)
+    assert plan._args.tail_count > 0 and (plan._args.many_count > 0) == (n > 30)
+    q = queries(n, 8)
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+
+    def look():
+        _lib.check_status()
+        out = paged.paged_attention(q, cache, plan, 128 ** -0.5)
+        _lib.check_status()
+        held = cache.data.double() if dtype == BF16 else cache.data.double() * cache.scales.double()[..., None]
+        lens = t.lens.tolist()
+        some = [i for i in range(n) if lens[i]]
+        rows = rows_of(held, t.table.tolist(), lens)
+        ref, room = exact(q[:n], [1] * n, rows, ints(lens), dtype)
+        full = [r if r.shape[2] else rows[some[0]][:, :, :1] for r in rows]
+        room = wider(room, q[:n], [1] * n, full, ints([max(k, 1) for k in lens]), plan)
+        assert near(out[some], ref[some], room[some])
+        assert not out[[i for i in range(n) if not lens[i]]].any()
+
+    look()
+    own = list(range(n))
+    t.step(0, parents=ints([-1] + own[1:]))                                  # the first one ends
+    look()
+    t.step(ints([300] + [1] * (n - 1)), parents=ints([-1] + own[1:]), keep=ints([0, 1000, 333, 128, 0] + [1000] * (n - 5)))
+    look()                                                                   # 333 and 128 are 334 and 129 now, with a token of their own
+    for more in (1, 60, 200):
+        t.step(more if more < 200 else ints([200] * 4 + [1] * (n - 4)))
+        look()
+
+
+@BOTH
+def test_cut_and_grown_all_together(dtype):
+    """All sequences are cut to the same place and go on differently."""
+    from sensenova_u1_b200.ops import _lib, page_tables, paged
+    n = 4
+    cache, tables, kv, _, shared = setup([(640, [700 + i for i in range(n)])], 32, 2, dtype, room=400, stretch=False)
+    t = page_tables.PageTables(cache, n, 1000)
+    t.load(kv, tables)
+    plan = paged.build_plan(cache, 8, [1] * n, [1000] * n, t, shared=shared)
+    t.step(100, keep=torch.full((n,), 270, dtype=torch.int32, device="cuda"))
+    q = queries(n, 8)
+    out = paged.paged_attention(q, cache, plan, 128 ** -0.5)
+    _lib.check_status()
+    held = cache.data.double() if dtype == BF16 else cache.data.double() * cache.scales.double()[..., None]
+    rows = rows_of(held, t.table.tolist(), [370] * n)
+    assert near(out, *exact(q[:n], [1] * n, rows, torch.full((n,), 370, device="cuda"), dtype))
