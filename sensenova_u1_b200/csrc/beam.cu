@@ -29,8 +29,10 @@ namespace snu1 {
 namespace beam {
 
 constexpr int THREADS = 256;
-constexpr int MAX_KEEP = 128;
+constexpr int MAX_BEAMS = 64;
 constexpr int MAX_EOS = 8;
+// A search's step: every beam may end in each of the ending tokens, so that the beams' number of others is only certain among as many.
+constexpr int MAX_KEEP = MAX_BEAMS * (1 + MAX_EOS);
 
 __device__ __forceinline__ uint32_t order32(float x) {          // keeps the order, - 0 equal to 0
   const uint32_t b = __float_as_uint(x + 0.f);
@@ -132,7 +134,6 @@ constexpr int JOIN_THREADS = 1024;
 constexpr int JOIN_LIST = 2048;      // candidates that fit; where more are not below the bound, it is raised to the keep-th best of these
 constexpr int RANKED = 384;          // as many are ranked at once
 constexpr int JOIN_GROUPS = 1024;    // groups that fit a list; more are looked for by every warp in its own share
-constexpr int MAX_BEAMS = 64;
 
 // A search's state (all on the device); see ops/beam.py.
 struct State {
@@ -269,7 +270,7 @@ constexpr int ALONE_GROUPS = 64;
 struct JoinShared {
   double lse[MAX_BEAMS];
   float base[MAX_BEAMS], least[MAX_BEAMS];
-  unsigned long long set[JOIN_THREADS], top[JOIN_THREADS / 4], nth, list_s[JOIN_LIST];      // (list_s: the candidates' scores once more, to be counted)
+  unsigned long long set[JOIN_THREADS], top[JOIN_THREADS], nth, list_s[JOIN_LIST];      // (list_s: the candidates' scores once more, to be counted)
   Best list[JOIN_LIST];
   int pass[JOIN_GROUPS], quarter[JOIN_GROUPS];
   short pick[JOIN_LIST];
@@ -362,10 +363,10 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const JoinArgs a) {
     const int i = tid + k * JOIN_THREADS;
     own[k] = i < all ? score_of(top_of(group[i]), i / a.groups) : 0ull;
   }
-  // The keep-th largest of the largest of 64 to 256 sets of the threads' values, every 64th to 256th thread a set (threads side by side are in
+  // The keep-th largest of the largest of 64 to 1024 sets of the threads' values, every 64th to 1024th thread a set (threads side by side are in
   // different ones, so that few values are a set each); 0 if fewer sets have any.  Its place is counted by ``share`` threads.
   auto nth_of = [&](unsigned long long mine) -> unsigned long long {
-    const int share = keep <= 32 ? 16 : keep <= 64 ? 8 : 4, values = JOIN_THREADS / share, sub = tid & (share - 1);
+    const int share = keep <= 32 ? 16 : keep <= 64 ? 8 : keep <= 128 ? 4 : keep <= 256 ? 2 : 1, values = JOIN_THREADS / share, sub = tid & (share - 1);
     sh.set[tid] = mine;
     if (tid == 0) sh.nth = 0;
     __syncthreads();

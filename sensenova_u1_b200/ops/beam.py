@@ -46,7 +46,7 @@ def _entry():
     return _ENTRY
 
 
-def _check(logits, scores, keep: int):
+def _check(logits, scores, keep: int, most: int = MAX_KEEP):
     """Requests, beams and tokens of a selection; refuses what the kernels are not made for."""
     if not isinstance(keep, int) or isinstance(keep, bool):
         raise ValueError("keep is a whole number")
@@ -56,8 +56,8 @@ def _check(logits, scores, keep: int):
     if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16) or logits.shape[0] != requests * beams:
         raise ValueError(f"logits must be fp32 or bf16 [{requests} x {beams}, vocab], not {tuple(logits.shape)} {logits.dtype}")
     vocab, (row, one) = logits.shape[1], logits.stride()
-    if not 1 <= beams <= MAX_BEAMS or not 1 <= keep <= MAX_KEEP:
-        raise ValueError(f"1 to {MAX_BEAMS} beams, of which 1 to {MAX_KEEP} continuations are kept")
+    if not 1 <= beams <= MAX_BEAMS or not 1 <= keep <= most:
+        raise ValueError(f"1 to {MAX_BEAMS} beams, of which 1 to {most} continuations are kept")
     if requests * beams > 65535 or vocab > MAX_VOCAB:
         raise ValueError("too many rows or tokens")
     if keep > beams * vocab:
@@ -121,7 +121,7 @@ class BeamSearch:
     def __init__(self, requests: int, beams: int, steps: int, eos=(), length_penalty: float = 1.0, early_stopping=False, device="cuda"):
         if requests < 1 or not 1 <= beams <= MAX_BEAMS or requests * beams > 65535 or steps < 1:
             raise ValueError(f"a search has requests, 1 to {MAX_BEAMS} beams and steps")
-        eos = [int(t) for t in eos]
+        eos = list(dict.fromkeys(int(t) for t in eos))
         if len(eos) > MAX_EOS or any(not 0 <= t < MAX_VOCAB for t in eos):
             raise ValueError(f"up to {MAX_EOS} ending tokens, none negative")
         if early_stopping not in (False, True, "never"):
@@ -149,8 +149,9 @@ class BeamSearch:
     def advance(self, logits: torch.Tensor) -> None:
         """One step, from the logits of the present rows (fp32 or bf16 [requests * beams, vocab]); the first one looks only at every request's first
         row.  A step beyond ``steps`` changes nothing, and ``check_status`` raises after it.  May be captured."""
-        keep = min(2 * self.beams, self.beams * logits.shape[-1])
-        requests, beams, vocab = _check(logits, self.scores, keep)
+        # (every beam may end in each of the ending tokens: only among so many are as many that go on as there are beams)
+        keep = min(self.beams * max(2, 1 + self._state.eos_count), self.beams * logits.shape[-1])
+        requests, beams, vocab = _check(logits, self.scores, keep, MAX_BEAMS * (1 + MAX_EOS))
         _launch(logits, self.scores, requests, beams, vocab, keep, (None, None, None), ctypes.addressof(self._state))
 
     def finished(self) -> bool:

@@ -33,3 +33,118 @@ def test_next_tokens_are_of_the_vocabulary(eos):
     for _ in range(3):
         search.advance(x)
         assert 0 <= int(search.tokens.min()) and int(search.tokens.max()) < 50
+
+
+class All(Plain):
+    """The search with all candidates of a step looked at; one without any is over, and its beams count as they are.
+
+    ``sure``: no decision of a request was between scores that are as good as equal.  Logits by the last token give equal sums in another order
+    (a, b, b after a, a, b: the same steps), which the device's fp32 scores need not see as equal: after t steps a score is off by up to
+    t (LSE + 2^-24 |s|), the difference of two by twice that.  Either order is right then, and what follows is another search."""
+
+    def __init__(self, requests, *args):
+        super().__init__(requests, *args)
+        self.sure = [True] * requests
+
+    def compare(self, r, x, y, by=1.0):
+        """Two scores divided by ``by`` are about to be compared."""
+        if abs(x - y) * by <= 2 * (self.t + 1) * (LSE + max(abs(x), abs(y)) * by * 2.0 ** -24):
+            self.sure[r] = False
+
+    def advance(self, logp):
+        for r, live in enumerate(self.live):
+            if self.done[r]:
+                continue
+            table = logp[r].tolist()
+            cand = sorted(((s + x, -b, -v) for b, (s, _, _) in enumerate(live) for v, x in enumerate(table[b]) if s + x > -INF), reverse=True)
+            new, length = [], (self.t + 1) ** self.penalty
+            for i, (s, b, v) in enumerate(cand):
+                if len(new) == self.k:
+                    break
+                if i + 1 < len(cand):
+                    self.compare(r, s, cand[i + 1][0])
+                if -v not in self.eos:
+                    new.append((s, live[-b][1] + [-v], -b))
+                elif i < self.k:
+                    self.put(r, (s / length, live[-b][1] + [-v]))
+            if not cand and self.t:
+                for s, tokens, _ in live:
+                    self.put(r, (s / self.t ** self.penalty, tokens))
+            self.live[r] = new
+            if not new:
+                self.done[r] = True
+            elif len(self.pool[r]) == self.k:
+                at = self.steps ** self.penalty if self.early == "never" and self.penalty > 0 else length
+                worst = min(p[0] for p in self.pool[r])
+                self.compare(r, worst, new[0][0] / at, min(at, length))
+                self.done[r] = self.early is True or worst >= new[0][0] / at
+        self.t += 1
+
+    def put(self, r, x):
+        pool = self.pool[r]
+        if len(pool) < self.k:
+            pool.append(x)
+            return
+        w = min(range(self.k), key=lambda j: pool[j][0])
+        self.compare(r, x[0], pool[w][0], min(1.0, (self.t + 1) ** self.penalty))
+        if x[0] > pool[w][0]:
+            pool[w] = x
+
+
+def run(table, beams, steps, eos, penalty, early, logits=None):
+    """A search over logits by the last token [requests, vocab, vocab], step by step beside the plain one."""
+    from sensenova_u1_b200.ops import _lib, beam
+    requests, vocab = table.shape[:2]
+    search, plain = beam.BeamSearch(requests, beams, steps, eos, penalty, early), All(requests, beams, steps, eos, penalty, early)
+    rows = torch.arange(requests, device="cuda").repeat_interleave(beams)
+    exact = torch.log_softmax(table.double(), -1).cpu()
+    exact[(torch.isnan(table) | (table == INF)).any(-1).cpu() | (table == -INF).all(-1).cpu()] = -INF
+    short = compared = 0
+    for t in range(steps):
+        x = table[rows, search.tokens]
+        logp = torch.full((requests, beams, vocab), -INF, dtype=torch.float64)
+        for r in range(requests):
+            for b, (_, tokens, _) in enumerate(plain.live[r]):
+                logp[r, b] = exact[r, tokens[-1] if tokens else 0]
+        if logits is not None:
+            logits(t, x, logp)
+        search.advance(x)
+        plain.advance(logp)
+        tokens, parents = search.tokens.view(requests, beams).tolist(), search.parents.view(requests, beams).tolist()
+        for r in range(requests):
+            here = int((search.scores[r] > -INF).sum())
+            short += not search.done[r] and here < beams
+            if plain.sure[r]:
+                assert search.done[r] == int(plain.done[r])
+                compared += 1
+            if not plain.sure[r] or plain.done[r]:
+                continue
+            assert here == len(plain.live[r])
+            for b, (s, path, parent) in enumerate(plain.live[r]):
+                assert (tokens[r][b], parents[r][b]) == (path[-1], r * beams + parent)
+                assert abs(float(search.scores[r, b]) - s) <= (t + 1) * (LSE + abs(s) * 2.0 ** -24) + 1e-9
+    for a, b, sure in zip(search.result(beams), plain.result(beams), plain.sure):
+        if not sure:
+            continue
+        assert [x[0] for x in a] == [x[1] for x in b]
+        for (_, x), (y, _) in zip(a, b):
+            assert abs(x - y) <= 1e-4 * max(1, abs(y))
+    _lib.check_status()
+    return short, compared
+
+
+@pytest.mark.parametrize("early", [False, True, "never"])
+@pytest.mark.parametrize("beams,vocab,eos,penalty", [(4, 20, (3, 7), 2.0), (4, 20, (3, 7, 11), 2.0), (4, 20, tuple(range(8)), 1.0), (2, 30, (1, 2, 3, 4, 5), 0.0), (3, 400, (0, 399, 9, 9, 0), 1.0),
+                                                     (1, 12, tuple(range(8)), 1.0), (40, 300, (3, 5), 1.0), (64, 500, (1, 2, 3, 4), 1.0), (64, 700, tuple(range(8)), 1.0)])
+def test_several_ending_tokens(beams, vocab, eos, penalty, early):
+    """Each of the beams may end in each of them: as many as there are beams go on all the same."""
+    compared = 0
+    for seed in range(8 if beams < 16 else 1):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        table = torch.randn(3, vocab, vocab, generator=g, device="cuda")
+        table[:2, :, list(eos)] += 3                            # often all of the best
+        short, n = run(table, beams, 7, eos, penalty, early)
+        compared += n
+        if vocab - len(set(eos)) >= beams:
+            assert short == 0
+    assert compared >= 3
