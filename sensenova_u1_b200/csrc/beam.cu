@@ -183,7 +183,7 @@ struct Chosen {
   int beam[MAX_KEEP], token[MAX_KEEP];
   int pick[MAX_BEAMS];                                    // the candidate that a beam goes on with
   float pool_score[MAX_BEAMS];
-  int pool_step[MAX_BEAMS], pool_pick[MAX_BEAMS];         // pool_pick: the candidate that has just come in, -1: none
+  int pool_step[MAX_BEAMS], pool_pick[MAX_BEAMS];         // pool_pick: the candidate that has just come in, -1: none, -2 - beam: a beam as it is
   int beams, done;
 };
 
@@ -215,6 +215,14 @@ __device__ void follow(const JoinArgs& a, int r, Chosen& c) {
         }
         return w;
       };
+      auto finish = [&](float x, int step, int pick) {
+        const int w = worst();
+        if (c.pool_step[w] < 0 || x > c.pool_score[w]) {
+          c.pool_score[w] = x;
+          c.pool_step[w] = step;
+          c.pool_pick[w] = pick;
+        }
+      };
       for (int i = 0; i < a.keep && n < K; ++i) {
         if (c.score[i] == -INFINITY) break;
         bool eos = false;
@@ -222,14 +230,13 @@ __device__ void follow(const JoinArgs& a, int r, Chosen& c) {
         if (!eos) {
           c.pick[n++] = i;
         } else if (i < K) {
-          const float x = c.score[i] / len;
-          const int w = worst();
-          if (c.pool_step[w] < 0 || x > c.pool_score[w]) {
-            c.pool_score[w] = x;
-            c.pool_step[w] = t;
-            c.pool_pick[w] = i;
-          }
+          finish(c.score[i] / len, t, i);
         }
+      }
+      if (c.score[0] == -INFINITY && t > 0) {        // no beam has a continuation: they count as they are
+        const float now = powf((float)t, s.penalty);
+        for (int b = 0; b < K; ++b)
+          if (s.scores[at + b] > -INFINITY) finish(s.scores[at + b] / now, t - 1, -2 - b);
       }
       const int w = worst();
       bool done = n == 0;
@@ -254,11 +261,12 @@ __device__ void follow(const JoinArgs& a, int r, Chosen& c) {
   s.history_token[h] = token;
   s.history_parent[h] = from;
   const int in = c.pool_pick[tid];
-  if (in >= 0) {
+  if (in != -1) {
+    const long long was = ((long long)(t - 1) * gridDim.x + r) * K - 2 - in;          // (of a beam as it is: its last token)
     s.pool_score[at + tid] = c.pool_score[tid];
-    s.pool_step[at + tid] = t;
-    s.pool_parent[at + tid] = c.beam[in];
-    s.pool_token[at + tid] = c.token[in];
+    s.pool_step[at + tid] = c.pool_step[tid];
+    s.pool_parent[at + tid] = in >= 0 ? c.beam[in] : s.history_parent[was];
+    s.pool_token[at + tid] = in >= 0 ? c.token[in] : s.history_token[was];
   }
   if (tid == 0 && c.done == 2) s.done[r] = 1;
 }

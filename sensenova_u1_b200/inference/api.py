@@ -446,7 +446,10 @@ class NEOChatModel:
     def _generate_ids(self, ids, x, pos3, max_new_tokens, stop_ids, sampling, beams=None):
         """New tokens: one list, or the best of a beam search."""
         if beams is not None:
-            return [t for t, _ in self.engine.beam_search([ids], max_new_tokens=max_new_tokens, stop_ids=stop_ids, docs_embeds=[x], docs_pos3=[pos3], **beams)[0]]
+            found = self.engine.beam_search([ids], max_new_tokens=max_new_tokens, stop_ids=stop_ids, docs_embeds=[x], docs_pos3=[pos3], **beams)[0]
+            if not found:
+                raise RuntimeError("the beam search has no continuation: the logits behind the prompt are not finite")
+            return [t for t, _ in found]
         lay, h = self.engine.prefill([ids], reserve_image_tokens=max_new_tokens, docs_embeds=[x], docs_pos3=[pos3])
         return self.engine.decode(lay, h, max_new_tokens, stop_ids=stop_ids, sampling=sampling, prompt_ids=[ids])
 

@@ -373,7 +373,8 @@ class InferenceEngine:
                     check_every: int = 8):
         """The ``best`` continuations of every prompt by a search with ``beams`` beams: per prompt a list of (token ids, score), best first, a
         stop token (up to eight) the last of its continuation.  A finished continuation counts ``sum of log probabilities / tokens ** length_penalty``;
-        ``early_stopping`` as in :class:`ops.beam.BeamSearch`.  ``docs_embeds`` / ``docs_pos3``: as in :meth:`prefill`.
+        ``early_stopping`` as in :class:`ops.beam.BeamSearch`.  ``docs_embeds`` / ``docs_pos3``: as in :meth:`prefill`.  There are fewer than ``best`` where
+        a search finds no more; none at all where the logits behind the prompt hold NaN or infinity.
 
         All beams of a prompt read its keys and values from the same pages (``page`` tokens of ``dtype``), once for all of them; a step (selection,
         block tables, layers, head) runs without a look by the host and is captured in a CUDA graph, and every ``check_every`` steps the host asks whether

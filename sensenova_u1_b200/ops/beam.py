@@ -112,7 +112,8 @@ class BeamSearch:
 
     ``eos``: up to eight tokens that end a hypothesis.  A finished one counts ``score / tokens ** length_penalty``, the ending token among its
     tokens.  ``early_stopping``: False, a request is done when it has ``beams`` finished hypotheses and none of its beams would be better at its
-    present length; True, as soon as it has that many; "never", when no beam could be better at any length.
+    present length; True, as soon as it has that many; "never", when no beam could be better at any length.  One whose beams have no
+    continuation left (logits of NaN, or all -inf) is done too, and they count as they are.
 
     On the device: ``scores`` fp32 [requests, beams] (-inf: no such beam), ``tokens`` int64 [requests * beams], what the next step reads, and
     ``parents`` int32 [requests * beams], the row of the step before that each row goes on from.  Rows that nobody goes on with keep

@@ -148,3 +148,32 @@ def test_several_ending_tokens(beams, vocab, eos, penalty, early):
         if vocab - len(set(eos)) >= beams:
             assert short == 0
     assert compared >= 3
+
+
+@pytest.mark.parametrize("when", [0, 1, 3])
+@pytest.mark.parametrize("beams,eos", [(1, ()), (4, (2, 5)), (64, (3,))])
+def test_no_continuation_is_left(when, beams, eos):
+    """From some step on a request's logits are NaN: its beams count as they are, beside what had ended."""
+    g = torch.Generator(device="cuda").manual_seed(beams)
+    table = torch.randn(3, 200, 200, generator=g, device="cuda") * 2
+
+    def broken(t, x, logp):
+        if t >= when:
+            x[beams:2 * beams] = float("nan")
+            logp[1] = -INF
+
+    run(table, beams, 6, eos, 1.0, "never", broken)
+
+
+def test_generate_without_a_continuation():
+    from sensenova_u1_b200.inference.api import ByteTokenizer, NEOChatModel
+    from test_beam_search_gpu import model, prompts
+    cfg, store, eng = model()
+    store.p["lm_head"].fill_(float("nan"))
+    docs = prompts(cfg, [40, 150])
+    assert eng.beam_search(docs, 4, 6, stop_ids=(5,)) == [[], []]
+    m, tok = NEOChatModel(cfg, store), ByteTokenizer(cfg.vocab_size)
+    with pytest.raises(RuntimeError, match="no continuation"):
+        m.chat(tok, None, "hello", generation_config={"num_beams": 4, "max_new_tokens": 6})
+    with pytest.raises(RuntimeError, match="no continuation"):
+        m.generate(input_ids=torch.tensor([tok.encode("what is shown?")]), max_new_tokens=6, num_beams=4, num_return_sequences=2)
