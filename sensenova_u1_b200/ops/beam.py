@@ -75,11 +75,12 @@ def _launch(logits, scores, requests, beams, vocab, keep, out, state) -> None:
         with torch.cuda.device(index):
             return _launch(logits, scores, requests, beams, vocab, keep, out, state)
     entry, size = _entry(), (requests, beams, vocab)
-    if size not in _SCRATCH:
+    found = _SCRATCH.get(size)                      # (another thread may empty it at any time)
+    if found is None:
         if len(_SCRATCH) > 64:
             _SCRATCH.clear()
-        _SCRATCH[size] = entry["scratch"](requests * beams, beams, vocab), entry["launches"](beams, vocab)
-    count, launches = _SCRATCH[size]
+        found = _SCRATCH[size] = entry["scratch"](requests * beams, beams, vocab), entry["launches"](beams, vocab)
+    count, launches = found
     scratch = torch.empty(count, dtype=torch.uint8, device=logits.device) if count else None
     _lib.LAUNCHES += launches
     rc = entry["step"](logits.data_ptr(), max(logits.stride(0), vocab), logits.dtype == torch.bfloat16, vocab, scores.data_ptr(), requests, beams,

@@ -177,3 +177,23 @@ def test_generate_without_a_continuation():
         m.chat(tok, None, "hello", generation_config={"num_beams": 4, "max_new_tokens": 6})
     with pytest.raises(RuntimeError, match="no continuation"):
         m.generate(input_ids=torch.tensor([tok.encode("what is shown?")]), max_new_tokens=6, num_beams=4, num_return_sequences=2)
+
+
+def test_sizes_that_another_thread_forgets(monkeypatch):
+    """The table of sizes is emptied between a look and the next one."""
+    from sensenova_u1_b200.ops import beam
+
+    class Emptied(dict):
+        def __contains__(self, key):
+            here = super().__contains__(key)
+            self.clear()
+            return here
+
+        def __setitem__(self, key, value):
+            pass
+
+    x, s = torch.randn(8, 40000, device="cuda"), torch.zeros(2, 4, device="cuda")
+    want = beam.beam_select(x, s)
+    monkeypatch.setattr(beam, "_SCRATCH", Emptied(beam._SCRATCH))
+    for _ in range(2):
+        assert all(torch.equal(a, b) for a, b in zip(beam.beam_select(x, s), want))
