@@ -14,6 +14,7 @@ A call runs on the current stream of its tensors' device.
 from __future__ import annotations
 
 import ctypes
+import math
 
 import torch
 
@@ -130,6 +131,8 @@ class BeamSearch:
             raise ValueError('early_stopping is False, True or "never"')
         if not abs(length_penalty) < float("inf"):
             raise ValueError("length_penalty is a number")
+        if abs(length_penalty) * math.log2(steps) > 100:
+            raise ValueError(f"{steps} tokens ** {length_penalty} leaves fp32: hypotheses could not be compared")
         _entry()
         self.requests, self.beams, self.steps, self.length_penalty = requests, beams, steps, float(length_penalty)
         self.device = torch.device(device)

@@ -197,3 +197,15 @@ def test_sizes_that_another_thread_forgets(monkeypatch):
     monkeypatch.setattr(beam, "_SCRATCH", Emptied(beam._SCRATCH))
     for _ in range(2):
         assert all(torch.equal(a, b) for a, b in zip(beam.beam_select(x, s), want))
+
+
+def test_penalties_that_leave_fp32_are_refused():
+    """(tokens ** penalty was infinite on the device, so hypotheses counted alike, and an OverflowError in the result)"""
+    from sensenova_u1_b200.ops import beam
+    for penalty in (101.0, -101.0, 1e30):
+        with pytest.raises(ValueError, match="fp32"):
+            beam.BeamSearch(1, 2, 2, (), penalty)
+    for steps, penalty in ((1, 1e30), (2, 100.0), (1024, -10.0)):
+        search = beam.BeamSearch(1, 2, steps, (3,), penalty)
+        search.advance(torch.randn(2, 9, device="cuda"))
+        assert all(abs(s) < INF for _, s in search.result(2)[0])
