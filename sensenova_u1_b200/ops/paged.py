@@ -448,7 +448,10 @@ def _shared_parts(kinds, heads: int, tails: int, slots: int, us: float):
     done.  Its CTAs have an SM each.  ``tails`` CTAs, of which ``slots`` fill all SMs, take no time of their own if all of them fit the SMs that are left;
     otherwise most of them run afterwards, ``us`` in all.  (bf16, 32 / 8 heads, by CTAs for shared tokens: 8 sequences of 4200 + 60 tokens 128: 15.8 us, 88: 11.9;
     16 of 32000 + 1000, whose tails need all SMs, 104: 48.9, 144: 44.6.  Over 25 such calls, cut into 3 to 20 parts each, the choice took 1.2 % more than
-    the best.  Most of that is calls whose last few tails are alone: 64 of 8000 + 400 50.8, with 88 CTAs 45.5; models of their turns chose worse elsewhere.)"""
+    the best.  Most of that is calls whose last few tails are alone: 64 of 8000 + 400 50.8, with 88 CTAs 45.5; models of their turns chose worse elsewhere.)
+
+    More CTAs than SMs are taken up where that is clearly sooner: a long run beside many short ones is not left whole (8 sequences of 40000 tokens and 18 runs of
+    4 x 2560 363 -> 85 us, 4 x (8 of 3000, 6000, 9000, 12000 and 30000) 323 -> 199).  By less than a tenth the model does not know (30 runs of 8 x 8000, cut in two 202 -> 218)."""
     sizes = [(int(t), int(c), start, tile) for tiles, start, tile in kinds for t, c in zip(*np.unique(tiles, return_counts=True))]
     longest = max((t for t, *_ in sizes), default=1)
     best, share = None, 0
@@ -458,13 +461,13 @@ def _shared_parts(kinds, heads: int, tails: int, slots: int, us: float):
         share = -(-longest // cut)
         split = [(c, -(-t // share), start + -(-t // -(-t // share)) * tile) for t, c, start, tile in sizes]       # items, parts, us of one
         ctas = heads * sum(c * n for c, n, _ in split)
-        if best is not None and (ctas > CHUNK_SLOTS or share < PREFIX_LEAST):
+        if best is not None and share < PREFIX_LEAST:
             break
         busy = max(t for *_, t in split)
         if ctas > CHUNK_SLOTS:
             busy = max(busy, heads / CHUNK_SLOTS * sum(c * n * t for c, n, t in split) + busy / 2)
         done = busy + (0.0 if tails <= slots // CHUNK_SLOTS * (CHUNK_SLOTS - ctas) else us + 4.0)
-        if best is None or done < best[0]:
+        if best is None or done < (0.9 if ctas > CHUNK_SLOTS else 1.0) * best[0]:
             best = (done, share)
     return best[0], [-(-tiles // best[1]) for tiles, _, _ in kinds]
 
