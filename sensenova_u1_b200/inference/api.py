@@ -18,6 +18,7 @@ import torch
 
 from ..config import ModelConfig
 from ..models.params import ParamStore
+from ..ops.beam import MAX_BEAMS, MAX_EOS
 from . import prompts
 from .engine import upload
 from .images import load_image_native, smart_resize  # noqa: F401  (re-exported: the reference's utils expose them next to the model)
@@ -399,20 +400,27 @@ class NEOChatModel:
                 "top_p": gc.get("top_p", 1.0) or 1.0, "top_k": gc.get("top_k", 0) or 0, "repetition_penalty": rp,
                 "seed": gc.get("seed")}
 
-    @staticmethod
-    def _beams(gc: dict) -> Optional[dict]:
-        """Knobs of a beam search (``num_beams / num_return_sequences / length_penalty / early_stopping``); None where there is one beam, or where
-        sampling or a repetition penalty is asked for, which go without."""
+    def _beams(self, gc: dict, stops: Sequence[int], max_new_tokens: int) -> Optional[dict]:
+        """Knobs of a beam search (``num_beams / num_return_sequences / length_penalty / early_stopping``); None where there is one beam, or what a
+        search does not do is asked for: sampling, a repetition penalty, more beams or ending tokens than it has places for.  Those calls go without."""
         beams, best = int(gc.get("num_beams", 1) or 1), int(gc.get("num_return_sequences", 1) or 1)
+        stops = list(dict.fromkeys(int(t) for t in stops if 0 <= int(t) < self.cfg.vocab_size))          # (others are never met)
+        why = None
         if beams > 1 and (gc.get("do_sample", False) or float(gc.get("repetition_penalty", 1.0) or 1.0) != 1.0):
-            warnings.warn("num_beams is left out: a beam search neither samples nor penalises repetition")
+            why = "a beam search neither samples nor penalises repetition"
+        elif beams > MAX_BEAMS or (beams > 1 and len(stops) > MAX_EOS):
+            why = f"a beam search has up to {MAX_BEAMS} beams and {MAX_EOS} ending tokens"
+        if why is not None:
+            warnings.warn("num_beams is left out: " + why)
             return None
         if beams == 1:
             if best != 1:
                 warnings.warn("num_return_sequences is left out: it is of a beam search (num_beams)")
             return None
+        if max_new_tokens < 1:
+            return None
         penalty = gc.get("length_penalty")
-        return {"beams": beams, "best": best, "length_penalty": 1.0 if penalty is None else float(penalty),
+        return {"beams": beams, "best": best, "stop_ids": stops, "length_penalty": 1.0 if penalty is None else float(penalty),
                 "early_stopping": gc.get("early_stopping") or False}
 
     @torch.no_grad()
@@ -435,7 +443,8 @@ class NEOChatModel:
             turns += [("user", q), ("assistant", a)]
         ids, x, pos3 = self._embed_prompt(tokenizer, question, images, system=system_message, history=turns)
         eos = int(_encode(tokenizer, prompts.IM_END)[-1])
-        out = self._generate_ids(ids, x, pos3, int(gc.get("max_new_tokens", 256)), (eos,), self._sampling(gc), self._beams(gc))[0]
+        new = int(gc.get("max_new_tokens", 256))
+        out = self._generate_ids(ids, x, pos3, new, (eos,), self._sampling(gc), self._beams(gc, (eos,), new))[0]
         if out and out[-1] == eos:
             out = out[:-1]
         text = tokenizer.decode(out) if hasattr(tokenizer, "decode") else out
@@ -446,7 +455,7 @@ class NEOChatModel:
     def _generate_ids(self, ids, x, pos3, max_new_tokens, stop_ids, sampling, beams=None):
         """New tokens: one list, or the best of a beam search."""
         if beams is not None:
-            found = self.engine.beam_search([ids], max_new_tokens=max_new_tokens, stop_ids=stop_ids, docs_embeds=[x], docs_pos3=[pos3], **beams)[0]
+            found = self.engine.beam_search([ids], max_new_tokens=max_new_tokens, docs_embeds=[x], docs_pos3=[pos3], **beams)[0]
             if not found:
                 raise RuntimeError("the beam search has no continuation: the logits behind the prompt are not finite")
             return [t for t, _ in found]
@@ -488,7 +497,8 @@ class NEOChatModel:
             x.index_copy_(0, dev_rows, visual_features.expand(rows.numel(), -1))       # x is this call's own copy
         eos = gc.get("eos_token_id")
         stops = tuple(eos) if isinstance(eos, (list, tuple)) else ((int(eos),) if eos is not None else ())
-        out = self._generate_ids(ids, x, pos3, int(gc.get("max_new_tokens", 256) or 256), stops, self._sampling(gc), self._beams(gc))
+        new = int(gc.get("max_new_tokens", 256) or 256)
+        out = self._generate_ids(ids, x, pos3, new, stops, self._sampling(gc), self._beams(gc, stops, new))
         pad = gc.get("pad_token_id")
         pad = int(pad) if pad is not None else stops[0] if stops else 0
         longest = max(len(o) for o in out)

@@ -209,3 +209,22 @@ def test_penalties_that_leave_fp32_are_refused():
         search = beam.BeamSearch(1, 2, steps, (3,), penalty)
         search.advance(torch.randn(2, 9, device="cuda"))
         assert all(abs(s) < INF for _, s in search.result(2)[0])
+
+
+def test_calls_that_a_search_has_no_place_for():
+    """More beams or ending tokens than a search takes, ending tokens that are none: chat and generate answer as they did before there were beams."""
+    from sensenova_u1_b200.inference.api import ByteTokenizer, NEOChatModel
+    from test_beam_search_gpu import model
+    cfg, store, _ = model(8)
+    m, tok = NEOChatModel(cfg, store), ByteTokenizer(cfg.vocab_size)
+    assert m.chat(tok, None, "hello", generation_config={"num_beams": 4, "max_new_tokens": 0}) == m.chat(tok, None, "hello", generation_config={"max_new_tokens": 0})
+    ids = torch.tensor([tok.encode("what is shown in this picture?")])
+    for kw, plain in [(dict(num_beams=65), {}), (dict(num_beams=4, eos_token_id=list(range(20, 29))), dict(eos_token_id=list(range(20, 29))))]:
+        with pytest.warns(UserWarning, match="left out"):
+            got = m.generate(input_ids=ids, max_new_tokens=6, **kw)
+        assert torch.equal(got, m.generate(input_ids=ids, max_new_tokens=6, **plain))
+    want = m.generate(input_ids=ids, max_new_tokens=6, num_beams=4)
+    for eos in (-1, [-1, cfg.vocab_size, cfg.vocab_size + 5]):
+        assert torch.equal(m.generate(input_ids=ids, max_new_tokens=6, num_beams=4, eos_token_id=eos), want)
+    eos = [int(want[0, 2]), -1, int(want[0, 2]), cfg.vocab_size]
+    assert m.generate(input_ids=ids, max_new_tokens=6, num_beams=4, eos_token_id=eos).shape[1] <= 6
