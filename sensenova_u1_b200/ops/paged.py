@@ -552,7 +552,7 @@ def build_plan(cache: PagedCache, heads: int, q_lens, kv_lens, tables, limits=No
             raise ValueError(f"the tables have {live.seqs} sequences")
         tables = live.width
     arrays, counts = _lay_out(q_lens, kv_lens, tables, cache.page, cache.pages, heads // cache.kv_heads, cache.kv_heads,
-                              cache.scales is not None, limits, grow, shared or ())
+                              cache.scales is not None, limits, grow, () if shared is None else shared)
     # all arrays in one copy from pinned memory that nothing waits for
     at, total = {}, 0
     for name, a in arrays.items():

@@ -24,3 +24,23 @@ def test_a_long_run_beside_many_short_ones_is_split(short, count, fp8):
     # no item much longer than all the work over all SMs
     tiles = max(runs[r, 3] // 128 / n for r, n in parts.items())
     assert tiles <= max(2 * 8 * sum(runs[r, 3] // 128 for r in parts) / 148, 25)
+
+
+@pytest.mark.parametrize("kind", ["array", "tensor", "list", "none"])
+def test_shared_as_an_array(monkeypatch, kind):
+    """``shared`` as lengths and tables may be given: several entries in one array had no truth value."""
+    import torch
+    seen = []
+    monkeypatch.setattr(paged, "_lay_out", lambda *a: seen.append(a[-1]) or 1 / 0)
+
+    class Cache:
+        kv_heads, page, pages, scales, device = 2, 64, 8, None, torch.device("cpu")
+
+    entries = [[0, 2, 128], [2, 2, 256]]
+    shared = {"array": np.array(entries), "tensor": torch.tensor(entries), "list": entries, "none": None}[kind]
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(torch.cuda, "device", lambda d: __import__("contextlib").nullcontext())
+    with pytest.raises(ZeroDivisionError):
+        paged.build_plan(Cache, 8, [1] * 4, [300] * 4, [[0]] * 4, shared=shared)
+    runs, _ = paged._shared_runs(seen[0], 4, np.ones(4, int), np.full(4, 300), np.ones(4, bool), None, 64)
+    assert runs == ([] if kind == "none" else [(0, 2, 128), (2, 2, 256)])
