@@ -8,13 +8,17 @@
 // groups as continuations are kept can hold one, and those are read again; what is not below the bound is ranked by counting.  Then the beams'
 // bookkeeping, so that a whole step is captured without a look by the host.
 //
-// 151936 fp32 logits a row, in a graph: 16 requests of 8 beams 17.9 us, where their bytes alone take 11.9 and the second kernel 5; 4 beams 10.1, of which
-// the second kernel's seven dependent phases are 7; a first step of 2 x 32 beams, 64 kept, 18.5.  A first kernel that also chose the best of its
+// 151936 fp32 logits a row, in a graph: 16 requests of 8 beams 18.0 us, where their bytes alone take 11.9 and the second kernel 5; 4 beams 10.4, of which
+// the second kernel's seven dependent phases are 7; a first step of 2 x 32 beams, 64 kept, 18.8.  A search's step (follow) takes 2 to 6 more: 20.9 for the 16
+// requests, 12.8 for the 4 beams.  What is kept is ranked by one CTA, so that many beams with many ending tokens take longer: 2 x 64 beams
+// with one 51, with two 64, with eight (576 kept) 211.  A first kernel that also chose the best of its
 // slice of a row had barriers in its pass: 30 us for the 16 requests.
 //
-// Candidates of different beams may be closer than fp32 tells apart: a group's sum is of fp32 terms, from 32 terms on in 64 bits (the largest
-// term of a row is 1 exactly, the errors of the others, 2^-22 of each at most, are of either sign: 1e-8 of the normaliser where they were measured),
-// and scores are compared in 64 bits.  Equal scores: the lower beam, then the lower token.
+// Candidates of different beams may be closer than fp32 tells apart: a group's sum is of fp32 terms, from 32 terms on in 64 bits, and scores are compared in 64
+// bits.  The largest term of a row is 1 exactly.  Another one, exp(-d), has an error of 2^-22 of itself from ex2, up to d 2^-24 from its rounded argument and
+// d 2^-26 from the constant, the last always of one sign, and where many terms are alike so are the others.  So normalisers are good to some 1e-8 for random
+// logits, to 3e-7 where one logit is far above 151935 others that are alike, and candidates of different beams are told apart to that; those of one beam always
+// are.  Equal scores: the lower beam, then the lower token.
 // A row with NaN, + inf or nothing but - inf has no candidates.
 #include <float.h>
 #include <math.h>

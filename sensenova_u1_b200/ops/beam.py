@@ -9,7 +9,7 @@ parents, finished hypotheses), so that a step needs no look by the host and may 
         logits = model(search.tokens, search.parents)
     best = search.result()
 
-A call runs on the current stream of its tensors' device.
+A call runs on the current stream of its tensors' device.  A graph reads and writes a search's arrays whenever it is replayed: keep the search as long as the graph.
 """
 from __future__ import annotations
 
@@ -95,7 +95,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, keep: int | None = N
     best first: their scores fp32 [requests, keep], beams and tokens int32 [requests, keep].
 
     ``logits``: fp32 or bf16 [requests * beams, vocab], rows may be slices of wider ones; ``scores``: fp32 [requests, beams].  Scores are compared in
-    64 bits; of equal ones the lower beam comes first, then the lower token (of one beam, the larger logit).  A beam whose score is -inf or not finite, or whose
+    64 bits, with normalisers that are good to about 1e-7; of equal ones the lower beam comes first, then the lower token (of one beam, the larger logit).  A beam whose score is -inf or not finite, or whose
     logits hold NaN or +inf, has no continuations, and no token of logit -inf is one; places for which none is left hold score -inf, beam
     0, token 0."""
     if keep is None:

@@ -11,7 +11,8 @@ ones.  So a step of beam search is ``step(1, parents=search.parents)``, a decode
 
 Whole pages are shared by all sequences that go on from them; the rows of a page that is not full are copied (in all caches), so no sequence
 writes where another one reads.  Pages are taken lowest number first, sequence after sequence.  A call runs on the current stream of the
-caches' device; the copies are done before the next call on that stream.
+caches' device; the copies are done before the next call on that stream.  A graph with a step reads and writes the tables whenever it is replayed: keep them,
+and the caches, as long as the graph.
 """
 from __future__ import annotations
 

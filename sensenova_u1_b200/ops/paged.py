@@ -61,8 +61,9 @@ CHUNK_JOIN = 3           # what a part costs besides: 128 KB written and read ag
 PREFIX_ROWS = 64         # rows of a CTA of the kernel for shared tokens, which are counted in tiles of 128
 PREFIX_LEAST = 2         # a part has at least this many key tiles
 # Sharing costs two launches more, so a run has at least so many tokens (bf16, e4m3), or all runs save at least so many tiles of 128 keys of a head.  Us in
-# a graph, with / without, 32 / 8 heads: 2 sequences of 2048 bf16 tokens 10.1 / 9.7, of 4096 11.3 / 13.0; e4m3 11.0 / 9.1, 12.2 / 12.7; 32
-# sequences of 512 12.6 / 10.9, of 1024 14.0 / 15.8, of 8192 22 / 83; 32 / 4 heads, 8 of 2048 12.1 / 12.1, of 4096 12.9 / 14.2.
+# a graph, with / without, 32 / 8 heads: 32 sequences of 512 bf16 tokens 12.6 / 10.9, of 1024 14.0 / 15.8, of 8192 22 / 83; 4 of 2048 10.6 / 11.3, e4m3 11.3 /
+# 11.5; 8 of 3200 11.6 / 12.3, e4m3 12.3 / 13.2.  Two sequences alone are even at 3000 (e4m3 3300) tokens, and with 4 heads beyond 4096: from the limit up to there
+# sharing takes 0.5 to 2 us more (2 of 2048 10.2 / 8.2; e4m3, 4 heads, 2 of 2560 10.6 / 8.4).
 SHARE_TOKENS, SHARE_TILES = (2048, 2560), 1900
 # Us on an SM, by type (bf16, e4m3): to start and end a CTA, and one of its tiles.  Of shared tokens: 64 rows, and as chunks 256 (128) rows.  Of
 # tails, two or three of which share the SM, both for the CTA's share of it.
@@ -379,6 +380,8 @@ def _together(runs, skip, q_rows, cap, q_start, group: int, heads: int, fp8: boo
     shared tokens] for every row."""
     runs = np.array([[q_start[a], q_start[a + n] - q_start[a], a, t, n] for a, n, t in runs])
     rows, tokens = runs[:, 1] * group, runs[:, 3]
+    # (The kernel for chunks holds probabilities over bf16 in one bf16 number, 2^-8 of each, and keys over e4m3 as fp16, where the one for 64 rows has two numbers
+    # and the codes: 2.2e-3 of the output's norm instead of 1.7e-3, of which 1.6e-3 are its own rounding.  64 sequences of 32000 tokens 71 us instead of 115.)
     big = (rows > PREFIX_ROWS) & (group <= CHUNK_TILE)
     # tails: sequences, rows of a CTA, items, their tiles and parts
     seqs = np.concatenate([np.arange(a, a + n) for a, n in runs[:, [2, 4]]])
@@ -535,8 +538,11 @@ def build_plan(cache: PagedCache, heads: int, q_lens, kv_lens, tables, limits=No
     ``tables`` may be a :class:`~.page_tables.PageTables` of as many sequences: the plan then reads its tables and lengths as they are when a call
     runs, ``kv_lens`` and ``grow`` say up to how many tokens they go, and its ``step`` stands in for ``advance``.
 
-    ``shared``: [first sequence, how many, tokens] of sequences that begin with the same tokens in the same pages.  Attention
-    reads those once for all of them, where that is faster (in tiles of 128 tokens; the rest, and the keys of chunks, are read by each sequence)."""
+    ``shared``: one [first sequence, how many, tokens] or more, of sequences that begin with the same tokens in the same pages.  Attention
+    reads those once for all of them, where that is faster (in tiles of 128 tokens; the rest, and the keys of chunks, are read by each sequence).  Where more
+    than 64 rows (sequences x new tokens x heads of a group) share, it may round as it does for chunks.  Over a ``PageTables`` the sequences need not stay
+    alike: one that has been cut, has ended or is another request by now reads from its own pages what it does not hold in common with the
+    first of them any more, as long as the tables come from ``step``."""
     if heads < 1 or heads % cache.kv_heads != 0:
         raise ValueError("the number of query heads must be a multiple of the cache's heads")
     with torch.cuda.device(cache.device):                     # (the stream that the copy below goes to)
@@ -648,7 +654,8 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, plan: PagedPlan, scale: 
     products of a query and a key and their sum stay within fp32; chunk rows with scores beyond 2^20 (log2 units) take a slow path.
 
     Over e4m3 a key adds nothing to the output where its probability times the size of its value is below 2^-32 of the largest such
-    product.  Chunks (more than 32 rows per key/value head) over e4m3 hold 128 cached tokens' values of a head relative to the largest of
+    product, for shared tokens 2^-28 (and has less than 11 bits below 2^-18); there a query's value below 2^-14 of its row's largest has no bits below
+    2^-22 of that.  Over shared bf16 tokens a key adds nothing where its probability is below 2^-100 of the largest.  Chunks (more than 32 rows per key/value head) over e4m3 hold 128 cached tokens' values of a head relative to the largest of
     them (less than 2^-80 counts as that): values 2^27 times smaller than that lose bits.  Where the largest value of another 128 tokens is
     2^d times larger, probabilities below 2^(d - 133) of the largest one are lost."""
     _check(cache, plan)
