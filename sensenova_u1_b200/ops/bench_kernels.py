@@ -9,7 +9,7 @@ branch), gemm_wgrad (dy^T x), attn_fwd / attn_bwd (causal packed documents, 32 q
 head 128), rmsnorm, qknorm_rope, swiglu, adamw, paged_write / paged_read (32 K tokens into and out of an e4m3 cache, 8 heads),
 paged_step (24 sequences of up to 4 K keys, one new token each, 32 / 8 heads), paged_drafts (8 new tokens each), paged_chunk
 (2 x 512 new tokens over 8 K keys), paged_shared (16 sequences of one new token after 32 K common ones), each over bf16 and e4m3 pages; beam_select
-(16 requests of 8 beams, 151936 fp32 logits each) and page_tables (their step: forks, copies in 12 layers).  Prints one JSON line per kernel with the time,
+(16 requests of 8 beams, 151936 fp32 logits each; beam_advance: a search's whole step) and page_tables (their step: forks, copies in 12 layers).  Prints one JSON line per kernel with the time,
 achieved TFLOP/s or GB/s and the fraction of the measured peaks when MEASURED_PEAKS.json is present.
 """
 from __future__ import annotations
@@ -259,10 +259,14 @@ def main():
             ms = _time(lambda: paged.paged_attention(q, cache, plan, D ** -0.5, out=o), args.iters, flush)
             report("paged_shared_" + tag, ms, flops=4.0 * D * Hq * n * (P + page), nbytes=float((P + n * page) * row + 4 * n * Hq * D))
     if want("beam_select"):
-        from .beam import beam_select
+        from .beam import BeamSearch, beam_select
         logits, scores = torch.randn(128, 151936, device=dev), torch.randn(16, 8, device=dev)
         ms = _time(lambda: beam_select(logits, scores), args.iters, flush)
         report("beam_select_16x8", ms, nbytes=4.0 * logits.numel())
+        for tag, eos in (("", (5,)), ("_8_eos", range(8))):
+            search = BeamSearch(16, 8, 4096, eos, early_stopping="never", device=dev)
+            ms = _time(lambda: search.advance(logits), args.iters, flush)
+            report("beam_advance_16x8" + tag, ms, nbytes=4.0 * logits.numel())
     if want("page_tables"):
         from . import paged
         from .page_tables import PageTables
